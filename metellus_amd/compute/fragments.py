@@ -157,11 +157,21 @@ def device_header() -> str:
         return "".join(f"{line}\n" for line in lines if line and not line.lstrip().startswith("//"))
 
 
-_PARAM_RE = re.compile(r"^\s*(const\s+)?float\s*\*\s*__restrict__\s+(\w+)\s*$")
+@functools.lru_cache(maxsize=1)
+def serving_header() -> str:
+    """The device code of the serving operators, for the helpers of their
+    kernels (the others do not carry it)."""
+    path = os.path.join(os.path.dirname(os.path.dirname(__file__)), "csrc", "mt_serving.h")
+    with open(path, encoding="utf-8") as f:
+        lines = (line.rstrip() for line in f)
+        return "".join(f"{line}\n" for line in lines if line and not line.lstrip().startswith("//"))
+
+
+_PARAM_RE = re.compile(r"^\s*(const\s+)?(\w[\w ]*?)\s*\*\s*__restrict__\s+(\w+)\s*$")
 
 
 def batched_params(buffers: tuple[str, ...]) -> tuple[list[str], list[str]]:
-    """Batched variant of a kernel signature: every ``[const] float*
+    """Batched variant of a kernel signature: every ``[const] T*
     __restrict__ g_X`` parameter becomes a device table of per-program
     pointers ``g_X_tab`` and the body starts by picking entry ``blockIdx.z``.
 
@@ -175,9 +185,9 @@ def batched_params(buffers: tuple[str, ...]) -> tuple[list[str], list[str]]:
         m = _PARAM_RE.match(decl)
         if m is None:
             raise ValueError(f"cannot batch kernel parameter {decl!r}")
-        const, name = m.group(1) or "", m.group(2)
-        params.append(f"{const}MT_GLOBAL float* const* __restrict__ {name}_tab")
-        picks.append(f"{const}float* __restrict__ {name} = ({const}float*){name}_tab[blockIdx.z];")
+        const, kind, name = m.group(1) or "", m.group(2), m.group(3)
+        params.append(f"{const}MT_GLOBAL {kind}* const* __restrict__ {name}_tab")
+        picks.append(f"{const}{kind}* __restrict__ {name} = ({const}{kind}*){name}_tab[blockIdx.z];")
     return params, picks
 
 

@@ -18,19 +18,35 @@ from metellus_amd.orchestrator.ir import (
     ShapeOp,
     Tensor,
 )
+from metellus_amd.orchestrator.serving import (
+    CacheReadOp,
+    CacheWriteOp,
+    DequantizeOp,
+    Int4MatmulOp,
+    KVCache,
+    PagedAttentionOp,
+    RmsNormOp,
+)
 
 __all__ = [
     "BroadcastSpec",
+    "CacheReadOp",
+    "CacheWriteOp",
     "DAG",
+    "DequantizeOp",
     "ElementwiseOp",
     "Graph",
+    "Int4MatmulOp",
+    "KVCache",
     "Layout",
     "MatmulOp",
     "Op",
     "OperandValue",
     "Operations",
+    "PagedAttentionOp",
     "Program",
     "ReductionOp",
+    "RmsNormOp",
     "Scalar",
     "ShapeOp",
     "Tensor",

@@ -9,6 +9,7 @@ from metellus_amd.orchestrator.assembly.elementwise import assemble_elementwise
 from metellus_amd.orchestrator.assembly.matmul import assemble_matmul
 from metellus_amd.orchestrator.assembly.multi_anchor import assemble_multi_anchor
 from metellus_amd.orchestrator.assembly.reduction import assemble_reduction
+from metellus_amd.orchestrator.assembly.serving import SERVING, assemble_serving
 from metellus_amd.orchestrator.assembly.shape import assemble_shape
 from metellus_amd.orchestrator.graph import Vertex
 from metellus_amd.orchestrator.kernel_group import FusionStrategy, KernelGroup
@@ -45,6 +46,8 @@ def assemble(vertex: Vertex, *, function_name: str | None = None, batch: int = 1
         return assemble_shape(decision, function_name)
     if s in _MULTI:
         return assemble_multi_anchor(decision, function_name, batch=batch)
+    if s in SERVING:
+        return assemble_serving(decision, function_name, batch=batch)
     raise ValueError(f"unknown strategy {s!r}")
 
 

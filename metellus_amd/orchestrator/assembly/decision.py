@@ -11,6 +11,24 @@ from metellus_amd.compute.elementwise.elementwise import TERNARY_EXPRESSIONS
 from metellus_amd.orchestrator.graph import Vertex
 from metellus_amd.orchestrator.ir import ElementwiseOp, MatmulOp, Op, ReductionOp, Scalar, ShapeOp, Tensor
 from metellus_amd.orchestrator.kernel_group import FusionStrategy
+from metellus_amd.orchestrator.serving import (
+    CacheReadOp,
+    CacheWriteOp,
+    DequantizeOp,
+    Int4MatmulOp,
+    PagedAttentionOp,
+    RmsNormOp,
+    ServingOp,
+)
+
+_SERVING = {
+    RmsNormOp: FusionStrategy.RMS_NORM,
+    DequantizeOp: FusionStrategy.DEQUANTIZE,
+    Int4MatmulOp: FusionStrategy.INT4_MATMUL,
+    CacheWriteOp: FusionStrategy.CACHE_WRITE,
+    CacheReadOp: FusionStrategy.CACHE_READ,
+    PagedAttentionOp: FusionStrategy.PAGED_ATTENTION,
+}
 
 
 @dataclass
@@ -22,6 +40,7 @@ class DecisionView:
     epilogue: tuple[ElementwiseOp, ...] = ()
     chain_only: tuple[ElementwiseOp, ...] = ()
     shape_op: ShapeOp | None = None
+    serving_op: ServingOp | None = None
     ops: tuple[Op, ...] = ()
     anchors: tuple[MatmulOp, ...] = ()
     merge_elem: ElementwiseOp | None = None
@@ -104,6 +123,9 @@ def _classify_multi_anchor(ops: tuple[Op, ...], anchors: tuple[MatmulOp, ...]) -
 
 def classify(vertex: Vertex) -> DecisionView:
     ops = vertex.ops
+    if isinstance(ops[0], ServingOp):
+        assert len(ops) == 1, "a serving op is a kernel of its own"
+        return DecisionView(strategy=_SERVING[type(ops[0])], serving_op=ops[0], ops=ops)
     shape_op = next((op for op in ops if isinstance(op, ShapeOp)), None)
     if shape_op is not None:
         assert len(ops) == 1, "ShapeOp must be standalone (no fusion in v0)"

@@ -1,0 +1,289 @@
+"""Serving strategies: one kernel per op, a call of a device function of
+``csrc/mt_serving.h`` specialised for the op's sizes and strides.
+
+Bindings are the op's tensors in the order of the device function's
+parameters; the rows (or tokens) are a runtime dim.  How a kernel splits its
+work is chosen here, by sizes and types alone.
+"""
+
+from __future__ import annotations
+
+from metellus_amd.compute.fragments import CodegenContext, serving_header
+from metellus_amd.compute.serving import ServingFragment
+from metellus_amd.orchestrator.assembly.decision import DecisionView
+from metellus_amd.orchestrator.ir import Tensor
+from metellus_amd.orchestrator.kernel_group import FusionStrategy, KernelGroup
+from metellus_amd.orchestrator.serving import (
+    CacheReadOp,
+    CacheWriteOp,
+    DequantizeOp,
+    Int4MatmulOp,
+    KVCache,
+    PagedAttentionOp,
+    RmsNormOp,
+)
+from metellus_amd.runtime.program import Kernel
+
+SERVING = frozenset(
+    {
+        FusionStrategy.RMS_NORM,
+        FusionStrategy.DEQUANTIZE,
+        FusionStrategy.INT4_MATMUL,
+        FusionStrategy.CACHE_WRITE,
+        FusionStrategy.CACHE_READ,
+        FusionStrategy.PAGED_ATTENTION,
+    }
+)
+
+_KIND = {"float32": 0, "int8": 1, "float8_e4m3": 2}
+_CTYPE = {"float32": "float", "int32": "int", "int8": "signed char", "uint8": "unsigned char"}
+WS_HEAD_BYTES = 4096  # the workspace's flag words
+
+
+def _ceil(a: int, b: int) -> int:
+    return -(-a // b)
+
+
+class _Signature:
+    """Kernel parameters in order; a parameter is named by its role, since two may
+    be bound to the same buffer."""
+
+    def __init__(self) -> None:
+        self.buffers: list[str] = []
+        self.bindings: list[str] = []
+
+    def add(self, role: str, t: Tensor | None, *, out: bool = False) -> str:
+        """The argument for ``t`` (``nullptr`` for a tensor that is not there)."""
+        if t is None:
+            return "nullptr"
+        self.buffers.append(f"{'' if out else 'const '}{_CTYPE[t.dtype]}* __restrict__ p_{role}")
+        self.bindings.append(t.buffer_key)
+        return f"p_{role}"
+
+
+def _group(decision: DecisionView, sig: _Signature, fragment: ServingFragment, function_name: str, dims: dict[str, int],
+           grid: tuple[int, int, int], lanes: int, **context) -> KernelGroup:
+    ctx = CodegenContext(
+        function_name=function_name,
+        buffers=tuple(sig.buffers),
+        dims=tuple(dims),
+        tg_x=lanes,
+        tg_y=1,
+        helpers=(serving_header(),),
+        **context,
+    )
+    return KernelGroup(
+        kernel=Kernel(fragments=(fragment,), ctx=ctx),
+        bindings=tuple(sig.bindings),
+        dims=tuple(dims.values()),
+        grid=grid,
+        threads=(lanes, 1, 1),
+        ops=decision.ops,
+        strategy=decision.strategy,
+    )
+
+
+# ---------------------------------------------------------------------------
+# norm
+# ---------------------------------------------------------------------------
+
+NORM_KEEP = 8  # float4s a lane keeps of a row at most; longer rows are read again for each pass
+
+
+def norm_lanes(rows: int, cols: int) -> int:
+    """Lanes that share a row: a wave where it keeps the row in 4 float4s a lane, 256
+    or 1024 for longer ones; more lanes of fewer elements while the rows alone leave
+    most of the GPU's 256 compute units idle."""
+    lanes = 64
+    while lanes < 1024 and (cols > 16 * lanes or (rows * lanes < 64 * 1024 and cols >= 8 * lanes)):
+        lanes *= 4
+    return lanes
+
+
+def _assemble_norm(decision: DecisionView, op: RmsNormOp, function_name: str | None) -> KernelGroup:
+    rows, cols = op.x.shape
+    T = norm_lanes(rows, cols)
+    per = _ceil(cols, 4 * T)
+    eight = op.scales is not None
+    res = op.residual
+    sig = _Signature()
+    args = (
+        sig.add("x", op.x),
+        sig.add("residual", res),
+        sig.add("weight", op.weight),
+        repr(op.eps),
+        sig.add("sum", op.sum_out, out=True),
+        "nullptr" if eight else sig.add("y", op.y, out=True),
+        sig.add("y", op.y, out=True) if eight else "nullptr",
+        sig.add("scales", op.scales, out=True),
+        "M",
+        "(double*)mt_lds" if T > 64 else "nullptr",
+    )
+    frag = ServingFragment(
+        "mt_rms_norm",
+        (cols, T, per if per <= NORM_KEEP else 0, op.x.row_stride, op.x.col_stride,
+         res.row_stride if res else 0, res.col_stride if res else 0, res is not None, op.sum_out is not None,
+         op.weight is not None, eight),
+        args,
+        lds_bytes=8 * T // 64 if T > 64 else 0,
+        name="rms_norm",
+    )
+    grid = (_ceil(rows, 4) if T == 64 else rows, 1, 1)
+    return _group(decision, sig, frag, function_name or f"rms_norm_{op.y.name}", {"M": rows}, grid, max(T, 256))
+
+
+def _assemble_dequantize(decision: DecisionView, op: DequantizeOp, function_name: str | None) -> KernelGroup:
+    rows, cols = op.x.shape
+    sig = _Signature()
+    args = (sig.add("x", op.x), sig.add("scales", op.scales), sig.add("y", op.y, out=True), f"(size_t)M * {cols}u")
+    frag = ServingFragment("mt_dequantize", (cols,), args, name="dequantize")
+    grid = (_ceil(rows * cols, 16 * 256), 1, 1)
+    return _group(decision, sig, frag, function_name or f"dequantize_{op.y.name}", {"M": rows}, grid, 256)
+
+
+# ---------------------------------------------------------------------------
+# cache
+# ---------------------------------------------------------------------------
+
+
+def _cache_template(spec: KVCache) -> tuple[int, ...]:
+    return (_KIND[spec.dtype], spec.kv_heads, spec.page_size, spec.dim)
+
+
+def cache_write_tokens(tokens: int, kv_heads: int) -> int:
+    """Tokens of a workgroup: its 16 row slots full, and up to 16 while more than
+    1024 workgroups remain, for each of them looks through the slots behind its own."""
+    few = max(1, 8 // kv_heads)
+    return max(few, min(16, tokens // 1024))
+
+
+def _assemble_cache_write(decision: DecisionView, op: CacheWriteOp, function_name: str | None) -> KernelGroup:
+    spec, tokens = op.spec, op.k.shape[0]
+    tb = cache_write_tokens(tokens, spec.kv_heads)
+    sig = _Signature()
+    args = (sig.add("k", op.k), sig.add("v", op.v), sig.add("slots", op.slots),
+            sig.add("cache", op.cache, out=True), "M", "(unsigned*)mt_lds")
+    frag = ServingFragment(
+        "mt_cache_write",
+        (*_cache_template(spec), spec.pages, tb, op.k.row_stride, op.k.col_stride, op.v.row_stride, op.v.col_stride),
+        args,
+        lds_bytes=16,
+        name="cache_write",
+    )
+    return _group(decision, sig, frag, function_name or f"cache_write_{op.written.name}", {"M": tokens},
+                  (_ceil(tokens, tb), 1, 1), 256)
+
+
+def _assemble_cache_read(decision: DecisionView, op: CacheReadOp, function_name: str | None) -> KernelGroup:
+    spec, rows = op.spec, op.slots.shape[0]
+    sig = _Signature()
+    args = (sig.add("cache", op.cache), sig.add("slots", op.slots), sig.add("k", op.k, out=True),
+            sig.add("v", op.v, out=True), "M")
+    frag = ServingFragment("mt_cache_read", (*_cache_template(spec), spec.pages), args, name="cache_read")
+    grid = (_ceil(rows * 2 * spec.kv_heads, 16), 1, 1)
+    return _group(decision, sig, frag, function_name or f"cache_read_{op.k.name}", {"M": rows}, grid, 256)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+ATTENTION_WAVES = 4
+ATTENTION_SPLITS = 64  # at most, for the workgroup that joins them
+ATTENTION_GROUPS = 1024  # workgroups aimed at
+ATTENTION_MIN_BYTES = 65536  # of keys and values for a workgroup at least
+
+
+def attention_splits(pairs: int, capacity: int, position_bytes: int) -> tuple[int, int]:
+    """(splits, positions of each) of a sequence's length, for ``pairs`` sequences
+    times key heads."""
+    least = max(16 * ATTENTION_WAVES, _ceil(ATTENTION_MIN_BYTES, position_bytes))
+    splits = max(1, min(ATTENTION_SPLITS, _ceil(ATTENTION_GROUPS, pairs), capacity // least))
+    if pairs >= 1023:  # a counter each is all the workspace's head has room for
+        splits = 1
+    each = _ceil(_ceil(capacity, splits), 16 * ATTENTION_WAVES) * 16 * ATTENTION_WAVES
+    return _ceil(capacity, each), each
+
+
+def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_name: str | None, batch: int) -> KernelGroup:
+    spec, rows = op.spec, op.q.shape[0]
+    share = op.heads // spec.kv_heads  # query heads of a key head
+    parts = _ceil(share, 16)  # of at most 16 query heads, one matrix instruction's columns
+    held = min(share, 16)
+    pairs = rows * spec.kv_heads * parts
+    splits, each = attention_splits(pairs * batch, op.capacity, 2 * spec.dim * spec.item_bytes)
+    floats = held * (spec.dim + 2)
+    ws = WS_HEAD_BYTES + 4 * batch * pairs * splits * floats if splits > 1 else 0
+    sig = _Signature()
+    args = (sig.add("q", op.q), sig.add("cache", op.cache), sig.add("pages", op.pages), sig.add("lengths", op.lengths),
+            sig.add("o", op.o, out=True), f"{op.scale!r}", "mt_ws" if ws else "nullptr", "M", "mt_lds")
+    frag = ServingFragment(
+        "mt_paged_attention",
+        (*_cache_template(spec), spec.pages, op.pages.shape[1], share, ATTENTION_WAVES, splits, each, batch,
+         op.q.row_stride, op.q.col_stride),
+        args,
+        lds_bytes=4 * ATTENTION_WAVES * floats + 4 * held * splits + 16,
+        name="paged_attention",
+    )
+    return _group(decision, sig, frag, function_name or f"paged_attention_{op.o.name}", {"M": rows},
+                  (pairs * splits, 1, 1), 64 * ATTENTION_WAVES, workspace_bytes=ws, workspace_batched=True,
+                  workspace_waits=False)
+
+
+# ---------------------------------------------------------------------------
+# 4-bit products
+# ---------------------------------------------------------------------------
+
+
+def int4_shape(rows: int, k: int, n: int) -> tuple[int, int]:
+    """(waves of a workgroup, which split k; tiles of 16 weight rows of each)."""
+    blocks = _ceil(k, 128)
+    tiles = 1
+    while tiles < 4 and _ceil(n, 32 * tiles) >= 512 and (rows > 1 or tiles < 2):
+        tiles *= 2
+    return min(8, blocks), tiles
+
+
+def _assemble_int4(decision: DecisionView, op: Int4MatmulOp, function_name: str | None) -> KernelGroup:
+    (rows, k), n = op.x.shape, op.weights.shape[0]
+    eight = op.x_scales is not None
+    waves, tiles = int4_shape(rows, k, n)
+    held = min(rows, 16)
+    sets = 1 if eight else _ceil(held, 4)  # matrix instructions' rows: 16 of x, or 4 of x in four digits each
+    sig = _Signature()
+    args = (
+        "nullptr" if eight else sig.add("x", op.x),
+        sig.add("x", op.x) if eight else "nullptr",
+        sig.add("x_scales", op.x_scales),
+        sig.add("weights", op.weights),
+        sig.add("scales", op.scales),
+        sig.add("zeros", op.zeros),
+        sig.add("y", op.y, out=True),
+        "M",
+        "mt_lds",
+    )
+    frag = ServingFragment(
+        "mt_matmul_int4",
+        (eight, sets, k, n, op.group, op.zeros is not None, tiles, waves, op.x.row_stride, op.x.col_stride),
+        args,
+        lds_bytes=max(0 if eight else 2048 * sets * waves, waves * tiles * 16 * 4 * 4 * (4 if eight else sets)),
+        name="int4_matmul",
+    )
+    grid = (_ceil(n, 16 * tiles), _ceil(rows, 16), 1)
+    return _group(decision, sig, frag, function_name or f"int4_matmul_{op.y.name}", {"M": rows}, grid, 64 * waves)
+
+
+_ASSEMBLE = {
+    RmsNormOp: _assemble_norm,
+    DequantizeOp: _assemble_dequantize,
+    CacheWriteOp: _assemble_cache_write,
+    CacheReadOp: _assemble_cache_read,
+    Int4MatmulOp: _assemble_int4,
+}
+
+
+def assemble_serving(decision: DecisionView, function_name: str | None, *, batch: int = 1) -> KernelGroup:
+    op = decision.serving_op
+    if isinstance(op, PagedAttentionOp):
+        return _assemble_attention(decision, op, function_name, batch)
+    return _ASSEMBLE[type(op)](decision, op, function_name)

@@ -3,7 +3,9 @@
 Same surface as the reference builder (reference:
 src/orchestrator/builder.py:50-342): ``input``, ``from_numpy``, ``matmul``,
 ``elementwise``, ``transpose``, ``reshape``, ``reduction``, ``build``,
-``tensors``, ``uploads``.  Validation is delegated to the op dataclasses;
+``tensors``, ``uploads``; beyond it the serving ops (``rms_norm``,
+``dequantize``, ``matmul_int4``, ``kv_cache``, ``cache_write``, ``cache_read``,
+``paged_attention``) and inputs of their types.  Validation is delegated to the op dataclasses;
 the builder resolves names, keeps SSA freshness and records host payloads.
 
     ops = Operations()
@@ -19,6 +21,7 @@ import numpy as np
 
 from metellus_amd.compute.elementwise.elementwise import BroadcastSpec
 from metellus_amd.orchestrator.ir import (
+    ITEM_BYTES,
     ElementwiseOp,
     Layout,
     MatmulOp,
@@ -28,6 +31,15 @@ from metellus_amd.orchestrator.ir import (
     Scalar,
     ShapeOp,
     Tensor,
+)
+from metellus_amd.orchestrator.serving import (
+    CacheReadOp,
+    CacheWriteOp,
+    DequantizeOp,
+    Int4MatmulOp,
+    KVCache,
+    PagedAttentionOp,
+    RmsNormOp,
 )
 
 
@@ -51,6 +63,9 @@ class Operations:
         self._tensors: dict[str, Tensor] = {}
         self._ops: Program = []
         self._uploads: dict[str, np.ndarray] = {}
+        self._caches: dict[str, KVCache] = {}
+        self._written: dict[str, str] = {}  # a cache's older state -> the state after the write
+        self._cache_readers: dict[str, list[Tensor]] = {}
 
     # -- registry ------------------------------------------------------------
 
@@ -61,17 +76,25 @@ class Operations:
         layout: Layout = Layout.ROW_MAJOR,
         row_stride: int | None = None,
         col_stride: int | None = None,
+        dtype: str | None = None,
     ) -> Tensor:
         """Declare a caller-supplied tensor.  Redeclaring with the same shape
-        returns the existing tensor."""
-        return self._declare(name, shape, layout=layout, row_stride=row_stride, col_stride=col_stride)
+        returns the existing tensor.  ``dtype`` (default: the program's) is one of
+        ``float32``, ``int32``, ``int8``, ``uint8``; the serving ops say which of
+        their operands take the others."""
+        if dtype is not None and dtype not in ITEM_BYTES:
+            raise ValueError(f"input: dtype must be one of {tuple(ITEM_BYTES)}; got {dtype!r}")
+        return self._declare(name, shape, layout=layout, row_stride=row_stride, col_stride=col_stride, dtype=dtype)
 
     def from_numpy(self, arr: np.ndarray, name: str) -> Tensor:
         """Declare ``name`` as an input and record ``arr`` for upload.  Only
-        float32 arrays and storage owners (not views) are accepted
+        float32 arrays -- arrays of its type for a name declared as an input of
+        another type -- and storage owners (not views) are accepted
         (reference: builder.py:80-118)."""
-        if arr.dtype != np.float32:
-            raise ValueError(f"from_numpy: array dtype must be float32; got {arr.dtype}")
+        known = self._tensors.get(name)
+        want = known.dtype if known is not None and known.dtype in ITEM_BYTES else "float32"
+        if arr.dtype != np.dtype(want):
+            raise ValueError(f"from_numpy: array dtype must be {want}; got {arr.dtype}")
         t = self._declare(name, tuple(arr.shape))
         if t.buffer_key != name:
             raise ValueError(
@@ -99,6 +122,7 @@ class Operations:
         layout: Layout = Layout.ROW_MAJOR,
         row_stride: int | None = None,
         col_stride: int | None = None,
+        dtype: str | None = None,
     ) -> Tensor:
         shape = tuple(shape)
         known = self._tensors.get(name)
@@ -108,11 +132,13 @@ class Operations:
                     f"tensor {name!r} already declared with shape {known.shape}, "
                     f"cannot redeclare as {shape}"
                 )
+            if dtype is not None and known.dtype != dtype:
+                raise ValueError(f"tensor {name!r} already declared as {known.dtype}, cannot redeclare as {dtype}")
             return known
         t = Tensor(
             name=name,
             shape=shape,
-            dtype=self._dtype,
+            dtype=self._dtype if dtype is None else dtype,
             layout=layout,
             row_stride=-1 if row_stride is None else row_stride,
             col_stride=-1 if col_stride is None else col_stride,
@@ -128,12 +154,19 @@ class Operations:
             )
         return t
 
-    def _fresh(self, name: str, shape: tuple[int, ...]) -> Tensor:
+    def _lookup_float(self, name: str) -> Tensor:
+        """An operand of the primitive ops, whose kernels read fp32."""
+        t = self._lookup(name)
+        if t.dtype != "float32" and t.dtype in ITEM_BYTES:
+            raise ValueError(f"tensor {name!r} is {t.dtype}; this op takes fp32 tensors")
+        return t
+
+    def _fresh(self, name: str, shape: tuple[int, ...], dtype: str | None = None) -> Tensor:
         """Output tensor for a new op; registered only after the op
         validates, so a rejected op leaves no stray name."""
         if name in self._tensors:
             raise ValueError(f"output tensor {name!r} already defined; IR is SSA — pick a fresh name")
-        return Tensor(name=name, shape=tuple(shape), dtype=self._dtype)
+        return Tensor(name=name, shape=tuple(shape), dtype=self._dtype if dtype is None else dtype)
 
     def _emit(self, out: Tensor, op) -> Tensor:
         self._tensors[out.name] = out
@@ -143,7 +176,7 @@ class Operations:
     # -- ops -----------------------------------------------------------------
 
     def matmul(self, a: str, b: str, out: str) -> Tensor:
-        ta, tb = self._lookup(a), self._lookup(b)
+        ta, tb = self._lookup_float(a), self._lookup_float(b)
         t_out = self._fresh(out, (ta.shape[0], tb.shape[-1]))
         return self._emit(t_out, MatmulOp(out=t_out, a=ta, b=tb))
 
@@ -162,7 +195,7 @@ class Operations:
         resolved: list[OperandValue] = []
         for o in operands:
             if isinstance(o, str):
-                resolved.append(self._lookup(o))
+                resolved.append(self._lookup_float(o))
             elif isinstance(o, (int, float)) and not isinstance(o, bool):
                 resolved.append(Scalar(value=float(o)))
             else:
@@ -182,6 +215,7 @@ class Operations:
     def transpose(self, name: str, out: str) -> Tensor:
         """Metadata-only transpose: a view sharing ``name``'s buffer."""
         src = self._lookup(name)
+        self._no_cache("transpose", name)
         if out in self._tensors:
             raise ValueError(f"view tensor {out!r} already declared; pick a fresh name")
         view = src.transpose(out)
@@ -193,6 +227,7 @@ class Operations:
         unchanged); otherwise a ``ShapeOp`` copy into a fresh buffer
         (reference: builder.py:259-305)."""
         src = self._lookup(name)
+        self._no_cache("reshape", name)
         if out in self._tensors:
             raise ValueError(f"reshape output {out!r} already declared; pick a fresh name")
         target = tuple(new_shape)
@@ -210,14 +245,14 @@ class Operations:
                 f"reshape element-count mismatch: {src.shape} ({src.element_count}) → {target} ({count})"
             )
         t_out = self._fresh(out, target)
-        return self._emit(t_out, ShapeOp(out=t_out, input=src))
+        return self._emit(t_out, ShapeOp(out=t_out, input=self._lookup_float(name)))
 
     def reduction(self, op: str, out: str, x: str, axis: int = -1) -> Tensor:
         from metellus_amd.compute.reduction.reduction import REDUCTION_OPS
 
         if op not in REDUCTION_OPS:
             raise ValueError(f"reduction op {op!r} not in {REDUCTION_OPS}")
-        tx = self._lookup(x)
+        tx = self._lookup_float(x)
         ax = axis if axis >= 0 else len(tx.shape) + axis
         if 0 <= ax < len(tx.shape):
             shape = tx.shape[:ax] + tx.shape[ax + 1 :]
@@ -225,6 +260,181 @@ class Operations:
             shape = tx.shape[:-1] or (1,)
         t_out = self._fresh(out, shape)
         return self._emit(t_out, ReductionOp(out=t_out, op=op, input=tx, axis=axis))
+
+    # -- serving ops (no counterpart in the reference) -------------------------
+
+    def _owners(self, *tensors: Tensor | None) -> tuple[Tensor, ...]:
+        """The owners of the views among ``tensors``, whose writers an op that
+        reads the views comes after."""
+        found = {t.buffer_key: self._tensors[t.buffer_key] for t in tensors if t is not None and t.buffer_key != t.name}
+        return tuple(found.values())
+
+    def _emit_all(self, op) -> None:
+        names = [t.name for t in op.outs]
+        if len(set(names)) < len(names):
+            raise ValueError(f"output names must differ; got {names}")
+        for t in op.outs:
+            self._tensors[t.name] = t
+        self._ops.append(op)
+
+    def _no_cache(self, what: str, name: str) -> None:
+        if name in self._caches:
+            raise ValueError(f"{what}: {name!r} is a kv cache; only cache_write, cache_read and paged_attention take one")
+
+    def _cache(self, name: str) -> tuple[Tensor, KVCache]:
+        t = self._lookup(name)
+        if name not in self._caches:
+            raise ValueError(f"tensor {name!r} is not a kv cache — declare it with ops.kv_cache(...)")
+        if name in self._written:
+            raise ValueError(
+                f"kv cache {name!r} has been written since; its buffer now holds {self._written[name]!r} — read that"
+            )
+        return t, self._caches[name]
+
+    def _optional(self, name: str | None) -> Tensor | None:
+        return None if name is None else self._lookup(name)
+
+    def rms_norm(
+        self,
+        x: str,
+        out: str,
+        weight: str | None = None,
+        residual: str | None = None,
+        sum_out: str | None = None,
+        scales: str | None = None,
+        eps: float = 1e-5,
+    ) -> Tensor:
+        """``out`` = h / sqrt(mean(h^2) + eps) * weight by rows, h = x + residual
+        (``sum_out`` keeps it).  ``scales`` names a further output: ``out`` is then
+        int8, rounded to the nearest multiple of its row's scale, max / 127."""
+        tx, tw, tr = self._lookup(x), self._optional(weight), self._optional(residual)
+        op = RmsNormOp(
+            y=self._fresh(out, tx.shape, "float32" if scales is None else "int8"),
+            x=tx,
+            weight=tw,
+            residual=tr,
+            sum_out=None if sum_out is None else self._fresh(sum_out, tx.shape, "float32"),
+            scales=None if scales is None else self._fresh(scales, tx.shape[:1], "float32"),
+            eps=float(eps),
+            after=self._owners(tx, tw, tr),
+        )
+        self._emit_all(op)
+        return op.y
+
+    def dequantize(self, x: str, scales: str, out: str) -> Tensor:
+        """``out`` = ``x`` (int8) times its row's scale, fp32."""
+        tx, ts = self._lookup(x), self._lookup(scales)
+        op = DequantizeOp(y=self._fresh(out, tx.shape, "float32"), x=tx, scales=ts, after=self._owners(tx, ts))
+        self._emit_all(op)
+        return op.y
+
+    def matmul_int4(
+        self,
+        x: str,
+        weights: str,
+        scales: str,
+        out: str,
+        zeros: str | None = None,
+        x_scales: str | None = None,
+    ) -> Tensor:
+        """``out`` = x @ W^T for a W held in 4 bits: W[n, k] = scales[n, k / group] *
+        (q[n, k] - zeros[n, k / group]), zeros 8 where not given.  ``weights``
+        (uint8, N x K/2): two of a row's q to a byte, the even one in the low bits.
+        Groups of 32, 64 or 128, by the width of ``scales``.  ``x_scales``: x is
+        int8 with a scale per row.  Made for few rows; any number is right, 16 at a
+        time."""
+        tx, tw, ts = self._lookup(x), self._lookup(weights), self._lookup(scales)
+        self._no_cache("matmul_int4", weights)
+        tz, txs = self._optional(zeros), self._optional(x_scales)
+        op = Int4MatmulOp(
+            y=self._fresh(out, (tx.shape[0], tw.shape[0]), "float32"),
+            x=tx,
+            weights=tw,
+            scales=ts,
+            zeros=tz,
+            x_scales=txs,
+            after=self._owners(tx, tw, ts, tz, txs),
+        )
+        self._emit_all(op)
+        return op.y
+
+    def kv_cache(
+        self, name: str, pages: int, page_size: int, kv_heads: int, dim: int, dtype: str = "float32"
+    ) -> KVCache:
+        """Declare a paged key-value cache as an input (uint8, one row per page;
+        see ``KVCache`` for its layout and for packing on the host)."""
+        spec = KVCache(pages=pages, page_size=page_size, kv_heads=kv_heads, dim=dim, dtype=dtype)
+        if name in self._tensors and self._caches.get(name) != spec:
+            raise ValueError(f"tensor {name!r} already declared, cannot redeclare as {spec}")
+        self._declare(name, spec.shape, dtype="uint8")
+        self._caches[name] = spec
+        return spec
+
+    def cache_write(self, cache: str, k: str, v: str, slots: str, out: str) -> Tensor:
+        """Store row t of ``k`` and ``v`` (fp32, kv_heads * dim) in slot
+        ``slots[t]`` (int32), quantised to the cache's type.  In place: ``out`` is
+        the cache's state after it, on the same buffer, and ``cache`` may not be
+        read any more.  A slot outside the cache is passed over (-1 for a padded
+        row); of rows that name one slot the last is stored."""
+        tc, spec = self._cache(cache)
+        tk, tv, ts = self._lookup(k), self._lookup(v), self._lookup(slots)
+        fresh = self._fresh(out, tc.shape, "uint8")
+        op = CacheWriteOp(
+            written=Tensor(name=fresh.name, shape=tc.shape, dtype="uint8", buffer_key=tc.buffer_key),
+            cache=tc,
+            spec=spec,
+            k=tk,
+            v=tv,
+            slots=ts,
+            after=(*self._owners(tk, tv, ts), *self._cache_readers.get(cache, ())),
+        )
+        self._emit_all(op)
+        self._caches[out] = spec
+        self._written[cache] = out
+        return op.written
+
+    def cache_read(self, cache: str, slots: str, k_out: str, v_out: str) -> tuple[Tensor, Tensor]:
+        """Keys and values of the slots ``slots`` (int32) as fp32 rows of
+        kv_heads * dim; zeros for a slot outside the cache."""
+        tc, spec = self._cache(cache)
+        ts = self._lookup(slots)
+        shape = (ts.shape[0], spec.row) if len(ts.shape) == 1 else (1, spec.row)
+        op = CacheReadOp(
+            k=self._fresh(k_out, shape, "float32"),
+            v=self._fresh(v_out, shape, "float32"),
+            cache=tc,
+            spec=spec,
+            slots=ts,
+            after=self._owners(ts),
+        )
+        self._emit_all(op)
+        self._cache_readers.setdefault(cache, []).append(op.out)
+        return op.k, op.v
+
+    def paged_attention(
+        self, q: str, cache: str, pages: str, lengths: str, out: str, heads: int, scale: float | None = None
+    ) -> Tensor:
+        """Attention of one new token per sequence: row b of ``q`` (heads * dim)
+        against the first ``lengths[b]`` positions of its pages ``pages[b]`` (both
+        int32), ``scale`` 1 / sqrt(dim) unless given.  Heads may share key heads.
+        Positions in pages outside the cache (-1) hold no keys; a sequence without
+        keys gives zeros."""
+        tc, spec = self._cache(cache)
+        tq, tp, tl = self._lookup(q), self._lookup(pages), self._lookup(lengths)
+        op = PagedAttentionOp(
+            o=self._fresh(out, tq.shape, "float32"),
+            q=tq,
+            cache=tc,
+            spec=spec,
+            pages=tp,
+            lengths=tl,
+            heads=heads,
+            scale=float(spec.dim**-0.5 if scale is None else scale),
+            after=self._owners(tq, tp, tl),
+        )
+        self._emit_all(op)
+        self._cache_readers.setdefault(cache, []).append(op.out)
+        return op.o
 
     # -- results -------------------------------------------------------------
 

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
-from metellus_amd.orchestrator.ir import Op, Program
+from metellus_amd.orchestrator.ir import Op, Program, outs_of
 
 
 @dataclass(frozen=True)
@@ -31,15 +31,15 @@ def build_dag(program: Program) -> DAG:
     for op in program:
         for t in op.inputs:
             readers.setdefault(t.name, []).append(op)
-        name = op.out.name
-        if name in producer_of:
-            raise ValueError(f"SSA violation: tensor {name!r} produced by two ops")
-        if name in readers:
-            raise ValueError(
-                f"def-after-use: tensor {name!r} consumed before it is defined "
-                "(program must be in topological order)"
-            )
-        producer_of[name] = op
+        for name in (t.name for t in outs_of(op)):
+            if name in producer_of:
+                raise ValueError(f"SSA violation: tensor {name!r} produced by two ops")
+            if name in readers:
+                raise ValueError(
+                    f"def-after-use: tensor {name!r} consumed before it is defined "
+                    "(program must be in topological order)"
+                )
+            producer_of[name] = op
     used = set(readers)
     produced = set(producer_of)
     return DAG(

@@ -25,7 +25,7 @@ import heapq
 from dataclasses import dataclass
 from functools import cached_property
 
-from metellus_amd.orchestrator.ir import Op, Program
+from metellus_amd.orchestrator.ir import Op, Program, outs_of
 
 
 @dataclass(frozen=True)
@@ -60,12 +60,11 @@ class Graph:
         (produced, never read).  A vertex exports its tensor iff something
         reads it or it is a program output."""
         read: set[str] = {t.name for op in program for t in op.inputs}
-        made: set[str] = {op.out.name for op in program}
+        made: set[str] = {t.name for op in program for t in outs_of(op)}
         outs = frozenset(made - read) if program_outputs is None else frozenset(program_outputs)
         verts = []
         for op in program:
-            name = op.out.name
-            exported = (name,) if (name in read or name in outs) else ()
+            exported = tuple(t.name for t in outs_of(op) if t.name in read or t.name in outs)
             verts.append(Vertex(ops=(op,), inputs=tuple(t.name for t in op.inputs), outputs=exported))
         return cls(
             vertices=tuple(verts),
@@ -155,7 +154,7 @@ class Graph:
                 "graph contains ops not in original IR — replace() received "
                 "ops that don't belong to this Program"
             )
-        made_by = {op.out.name: op for op in original}
+        made_by = {t.name: op for op in original for t in outs_of(op)}
         for op in original:
             for t in op.inputs:
                 prod = made_by.get(t.name)
@@ -202,7 +201,7 @@ class Graph:
         if positions != sorted(positions):
             raise ValueError("replace: ops must be in original-IR program order")
 
-        made = {op.out.name for op in ops}
+        made = {t.name for op in ops for t in outs_of(op)}
         read_outside: set[str] = set()
         for v in self.vertices:
             if id(v) not in taken:

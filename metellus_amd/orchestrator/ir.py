@@ -1,4 +1,5 @@
-"""Primitive IR: fp32 tensors of rank <= 2 and four op kinds.
+"""Primitive IR: fp32 tensors of rank <= 2 and four op kinds (the serving ops
+of ``orchestrator.serving`` add tensors of other types; these four take fp32).
 
 Restates the reference IR (reference: src/orchestrator/ir.py:1-491) with the
 same classes, fields, defaults and validation messages, so programs built
@@ -43,6 +44,11 @@ def _default_strides(shape: tuple[int, ...], layout: Layout) -> tuple[int, int]:
     raise ValueError(f"v0 supports 0D/1D/2D tensors only; got shape {shape}")
 
 
+# Bytes of an element.  Types that are not listed count as fp32, which is what
+# the four op kinds here compute in whatever the tensor's label.
+ITEM_BYTES = {"float32": 4, "int32": 4, "int8": 1, "uint8": 1}
+
+
 def _count(shape: tuple[int, ...]) -> int:
     n = 1
     for d in shape:
@@ -78,7 +84,7 @@ class Tensor:
 
     @property
     def nbytes(self) -> int:
-        return 4 * _count(self.shape)  # fp32 only
+        return ITEM_BYTES.get(self.dtype, 4) * _count(self.shape)
 
     @property
     def element_count(self) -> int:
@@ -337,3 +343,9 @@ class ShapeOp:
 
 Op = MatmulOp | ElementwiseOp | ReductionOp | ShapeOp
 Program = list[Op]
+
+
+def outs_of(op: Op) -> tuple[Tensor, ...]:
+    """Every tensor ``op`` writes: ``op.out`` alone for the ops here, ``op.outs``
+    for the serving ops."""
+    return getattr(op, "outs", None) or (op.out,)

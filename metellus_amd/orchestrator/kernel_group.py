@@ -8,7 +8,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 from enum import Enum
 
-from metellus_amd.orchestrator.ir import Op
+from metellus_amd.orchestrator.ir import Op, outs_of
 from metellus_amd.runtime.program import Kernel
 
 
@@ -28,6 +28,13 @@ class FusionStrategy(str, Enum):
     # extension (fusion.MATMUL_REDUCTION_EPILOGUES): a matmul whose output
     # also feeds a last-axis reduction computed in the same kernel
     MATMUL_REDUCTION_EPILOGUE = "matmul_reduction_epilogue"
+    # the serving ops (orchestrator.serving): one kernel each
+    RMS_NORM = "rms_norm"
+    DEQUANTIZE = "dequantize"
+    INT4_MATMUL = "int4_matmul"
+    CACHE_WRITE = "cache_write"
+    CACHE_READ = "cache_read"
+    PAGED_ATTENTION = "paged_attention"
 
     def __str__(self) -> str:
         return self.value
@@ -49,4 +56,4 @@ class KernelGroup:
 
     @property
     def outputs(self) -> tuple[str, ...]:
-        return tuple(op.out.name for op in self.ops if op.out.name in self.bindings)
+        return tuple(t.name for op in self.ops for t in outs_of(op) if t.buffer_key in self.bindings)

@@ -14,7 +14,8 @@ Plan, in order:
    strides), then the owner itself if it is a named tensor (which ends the
    buffer's life) -- or freed.
 
-Fused intermediates never get a buffer, so they are never downloaded.
+Fused intermediates never get a buffer, so they are never downloaded.  A
+state of a kv cache that a later write overwrote is gone too.
 Frees are stream-ordered in the native shim, so they need no host sync.
 """
 
@@ -26,8 +27,14 @@ import numpy as np
 
 from metellus_amd.orchestrator.builder import Operations
 from metellus_amd.orchestrator.dag import build_dag
+from metellus_amd.orchestrator.ir import ITEM_BYTES, outs_of
 from metellus_amd.orchestrator.kernel_group import KernelGroup
+from metellus_amd.orchestrator.serving import CacheWriteOp
 from metellus_amd.runtime.program import Allocate, Dispatch, Download, Free, FromNumpy, Runtime
+
+
+def _host_dtype(t) -> np.dtype:
+    return np.dtype(t.dtype if t.dtype in ITEM_BYTES else np.float32)
 
 
 def schedule(
@@ -46,7 +53,10 @@ def schedule(
     tensors = ops.tensors
     uploads = ops.uploads
 
-    produced = {op.out.buffer_key for op in program}
+    # (a cache is written in place: its buffer is the input's)
+    made = [t for op in program for t in outs_of(op) if not isinstance(op, CacheWriteOp)]
+    overwritten = {op.cache.name for op in program if isinstance(op, CacheWriteOp)}
+    produced = {t.buffer_key for t in made}
     required = {tensors[n].buffer_key for n in dag.inputs} - produced
     provided = set(uploads)
     if required - provided:
@@ -54,7 +64,7 @@ def schedule(
     if provided - required:
         raise ValueError(f"schedule: uploads {sorted(provided - required)} do not correspond to any program input")
 
-    nbytes = {op.out.buffer_key: op.out.nbytes for op in program}
+    nbytes = {t.buffer_key: t.nbytes for t in made}
     for name in uploads:
         nbytes[tensors[name].buffer_key] = tensors[name].nbytes
     input_keys = {tensors[n].buffer_key for n in uploads}
@@ -68,11 +78,16 @@ def schedule(
         unknown = sorted(n for n in wanted if n not in tensors)
         if unknown:
             raise ValueError(f"schedule: unknown output names {unknown}")
+        gone = sorted(n for n in wanted if n in overwritten and n not in uploads)
+        if gone:
+            raise ValueError(f"schedule: outputs {gone} are states of a kv cache that a later write overwrites")
         absent = sorted(n for n in wanted if n in uploads or tensors[n].buffer_key not in live_keys)
         if absent:
             raise ValueError(f"schedule: outputs {absent} are program inputs or not materialised by any kernel")
     names_by_key: dict[str, list[str]] = {}
     for name, t in tensors.items():
+        if name in overwritten:
+            continue
         if name not in uploads and t.buffer_key in live_keys and (wanted is None or name in wanted):
             names_by_key.setdefault(t.buffer_key, []).append(name)
 
@@ -112,7 +127,7 @@ def schedule(
                     Download(
                         name=t.buffer_key,
                         shape=t.shape,
-                        dtype=np.float32,
+                        dtype=_host_dtype(t),
                         into=t.name,
                         row_stride=t.row_stride,
                         col_stride=t.col_stride,
@@ -120,7 +135,7 @@ def schedule(
                 )
             if k in names:
                 t = tensors[k]
-                steps.append(Download(name=k, shape=t.shape, dtype=np.float32, into=t.name))
+                steps.append(Download(name=k, shape=t.shape, dtype=_host_dtype(t), into=t.name))
             else:
                 steps.append(Free(name=k))
             retired.add(k)

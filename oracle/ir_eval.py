@@ -23,7 +23,8 @@ the program is fused:
 * last-axis reductions with identities sum 0, product 1, max -inf, min +inf
   (reference: src/compute/reduction/reduction.py:172-193);
 * matmul accumulated in float64 (the reference for a tolerance check);
-* ``ShapeOp`` -- a strided gather (reference: src/compute/copy/copy.py:25-54).
+* ``ShapeOp`` -- a strided gather (reference: src/compute/copy/copy.py:25-54);
+* the serving ops -- ``oracle/serving_eval.py``, in float64.
 
 ``ordered_row_reduce`` additionally replays the exact combine order of the
 gfx950 reduction kernel (lane chunks, four vector accumulators, wave64
@@ -210,16 +211,27 @@ def evaluate(ops, inputs: dict | None = None) -> dict:
 
     ``inputs`` maps storage-owner names to arrays (default: ``ops.uploads``).
     Returns ``{tensor name: ndarray}`` for every produced tensor and every
-    view of a produced tensor.  Matmul results are float64; everything else
-    float32."""
+    view of a produced tensor.  Matmul results and fp32 results of the serving
+    ops are float64; everything else float32 (or the serving tensor's type)."""
     from metellus_amd.orchestrator.ir import ElementwiseOp, MatmulOp, ReductionOp, ShapeOp
+    from metellus_amd.orchestrator.serving import ServingOp
+
+    from oracle.serving_eval import evaluate_serving
 
     storage: dict[str, np.ndarray] = {}
     src = ops.uploads if inputs is None else inputs
     for name, arr in src.items():
-        storage[name] = np.ascontiguousarray(arr, dtype=F32)
+        own = ops.tensors[name].dtype if name in ops.tensors else "float32"
+        storage[name] = np.ascontiguousarray(arr, dtype=own if own in ("int32", "int8", "uint8") else F32)
     out: dict[str, np.ndarray] = {}
     for op in ops.build():
+        if isinstance(op, ServingOp):
+            found = evaluate_serving(op, lambda t: _view(storage[t.buffer_key], t))
+            for t in op.outs:
+                v = found[t.name]
+                storage[t.buffer_key] = np.ascontiguousarray(v, dtype=F32 if v.dtype == np.float64 else v.dtype)
+                out[t.name] = v
+            continue
         if isinstance(op, MatmulOp):
             a = _view(storage[op.a.buffer_key], op.a).astype(np.float64)
             b = _view(storage[op.b.buffer_key], op.b).astype(np.float64)

@@ -1,0 +1,700 @@
+"""The serving ops on the GPU against the oracle in float64 (``oracle.serving_eval``).
+
+Tolerances follow from the kernels' roundings (u = 2^-24, half a step of fp32):
+
+* rms_norm: h is one fp32 addition (exact match), y one rounding of a float64 value
+  (1.01 u of itself); 8-bit values and scales match the oracle's exactly (both sides
+  round a float64 quotient; the inputs are no ties).
+* cache: exact, bytes and scales.
+* matmul_int4: see ``_int4_bound``.
+* paged_attention: see ``_attention_bound``.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from metellus_amd.api import compile_program, run, run_batch
+from metellus_amd.orchestrator import KVCache, Operations
+from metellus_amd.runtime import Buffer, Dispatch, Runtime, hip_backend
+from oracle import serving_eval
+from oracle.ir_eval import evaluate
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+TYPES = ["float32", "int8", "float8_e4m3"]
+
+
+def _put(ops: Operations, name: str, a: np.ndarray) -> None:
+    ops.input(name, a.shape, dtype=str(a.dtype))
+    ops.from_numpy(a, name)
+
+
+def _close(got, want, bound):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    flat = np.isfinite(want)
+    np.testing.assert_array_equal(got[~flat & ~np.isnan(want)], want[~flat & ~np.isnan(want)])
+    bound = np.broadcast_to(bound, want.shape)
+    off = np.abs(got - want)[flat]
+    assert np.all(off <= bound[flat]), f"off by {np.max(off / np.maximum(bound[flat], 1e-300)):.3g} times the bound"
+
+
+# ---------------------------------------------------------------------------
+# norm
+# ---------------------------------------------------------------------------
+
+
+def _norm_check(ops, eight: bool, summed: bool):
+    env, ref = run(ops).env, evaluate(ops)
+    if summed:
+        np.testing.assert_array_equal(env["h"], ref["h"])
+    if eight:
+        np.testing.assert_array_equal(env["s"], ref["s"])
+        np.testing.assert_array_equal(env["y"], ref["y"])
+        with np.errstate(invalid="ignore"):
+            want = env["y"].astype(np.float32) * env["s"][:, None]
+        np.testing.assert_array_equal(env["z"], want)
+    else:
+        _close(env["y"], ref["y"], 1.01 * U * np.abs(ref["y"]) + 1e-45)
+
+
+@pytest.mark.parametrize("rows, cols", [
+    (1, 1), (1, 3), (5, 64), (3, 255), (300, 256), (1, 4096), (70, 4096), (37, 1023), (2, 8191), (9, 16384), (2, 40001),
+    (1100, 130),
+])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("eight", [False, True])
+def test_rms_norm(rows, cols, residual, eight):
+    rng = np.random.default_rng(rows * 100003 + cols)
+    ops = Operations()
+    _put(ops, "x", rng.standard_normal((rows, cols)).astype(np.float32))
+    _put(ops, "w", (1 + 0.1 * rng.standard_normal(cols)).astype(np.float32))
+    kwargs = {}
+    if residual:
+        _put(ops, "r", (3 * rng.standard_normal((rows, cols))).astype(np.float32))
+        kwargs = {"residual": "r", "sum_out": "h"}
+    ops.rms_norm("x", out="y", weight="w", scales="s" if eight else None, **kwargs)
+    if eight:
+        ops.dequantize("y", scales="s", out="z")
+    _norm_check(ops, eight, residual)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_rms_norm_of_strided_rows(eight):
+    """x a transposed view, the residual rows with gaps, no weight."""
+    rng = np.random.default_rng(5)
+    ops = Operations()
+    _put(ops, "x_", rng.standard_normal((130, 33)).astype(np.float32))
+    ops.transpose("x_", out="x")
+    ops.input("r", (33, 130), row_stride=130, col_stride=1)
+    ops.from_numpy(rng.standard_normal((33, 130)).astype(np.float32), "r")
+    ops.rms_norm("x", out="y", residual="r", sum_out="h", scales="s" if eight else None)
+    if eight:
+        ops.dequantize("y", scales="s", out="z")
+    _norm_check(ops, eight, True)
+
+
+def test_rms_norm_special_rows():
+    """Zeros (eps keeps them), the largest and the smallest values, infinities and NaN."""
+    x = np.random.default_rng(6).standard_normal((7, 300)).astype(np.float32)
+    x[0] = 0
+    x[1] *= np.float32(1e38)
+    x[2] *= np.float32(1e-38)
+    x[3, 17] = np.inf
+    x[4, 200] = np.nan
+    x[5, :] = 0
+    x[5, 7] = 1e-45
+    for eight in (False, True):
+        ops = Operations()
+        _put(ops, "x", x)
+        ops.rms_norm("x", out="y", scales="s" if eight else None)
+        if eight:
+            ops.dequantize("y", scales="s", out="z")
+        env = run(ops).env
+        if eight:
+            ref = evaluate(ops)
+            np.testing.assert_array_equal(env["s"], ref["s"])
+            np.testing.assert_array_equal(env["y"], ref["y"])
+            assert np.all(np.isnan(env["z"][3:5])) and np.all(env["z"][0] == 0)
+        else:
+            ref = evaluate(ops)["y"]
+            # a row with an infinity: inf / inf at it, 0 elsewhere
+            _close(env["y"], ref, 1.01 * U * np.abs(ref) + 1e-45)
+
+
+@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 5), (4, 16), (7, 1023), (1, 4097)])
+def test_dequantize(rows, cols):
+    rng = np.random.default_rng(rows + cols)
+    ops = Operations()
+    _put(ops, "q", rng.integers(-128, 128, (rows, cols)).astype(np.int8))
+    s = rng.standard_normal(rows).astype(np.float32)
+    s[-1] = np.nan
+    _put(ops, "s", s)
+    ops.dequantize("q", scales="s", out="y")
+    np.testing.assert_array_equal(run(ops).env["y"], ops.uploads["q"].astype(np.float32) * s[:, None])
+
+
+# ---------------------------------------------------------------------------
+# 4-bit products
+# ---------------------------------------------------------------------------
+
+
+def _int4_bound(ops: Operations) -> np.ndarray:
+    """Per block of 128 k and row n, with s the group's scale:
+
+    * x in fp32 becomes multiples of 2^-30 of a power of two P, max < P <= 2 max:
+      128 * (8 + |8 - z|) * 2 max * 2^-30 * |s| (truncation, so a whole step);
+    * the product's digits are exact integers; hi and lo each round once (lo < 2^30
+      steps, 2^6 steps of 2^-30 P / 16), their fma once, with zeros another fma of
+      that on both terms, times s, the addition: under 8 u of sum |x| (8 + |8 - z|) |s|,
+      and 2^6 * 2 max * 2^-30 |s|;
+    * adding up: a running sum of at most blocks * groups terms and 8 waves, u each of
+      the magnitude so far.
+    """
+    (op,) = ops.build()
+    x = np.abs(ops.uploads["x"].astype(np.float64))
+    s = np.abs(ops.uploads["s"].astype(np.float64))
+    z = ops.uploads["z"].astype(np.float64) if op.zeros is not None else np.full(s.shape, 8.0)
+    weight = (8 + np.abs(8 - z)) * s
+    k, group = x.shape[1], op.group
+    total, steps = 0.0, 0.0
+    for g in range(k // group):
+        xs = x[:, g * group : (g + 1) * group]
+        total = total + xs.sum(axis=1)[:, None] * weight[None, :, g]
+        blk = g * group // 128
+        top = x[:, blk * 128 : blk * 128 + 128].max(axis=1)
+        steps = steps + top[:, None] * 2.0**-29 * (group * weight[:, g] + 64 * s[:, g])[None]
+    bound = (8 + k // group + 8) * U * total
+    if op.x_scales is None:
+        return bound + steps
+    return (bound + 2 * U * total) * np.abs(ops.uploads["xs"].astype(np.float64))[:, None]
+
+
+def _int4(rows, k, n, group, eight, zeros, seed, strides=False):
+    rng = np.random.default_rng(seed)
+    ops = Operations()
+    if eight:
+        _put(ops, "x", rng.integers(-127, 128, (rows, k)).astype(np.int8))
+        _put(ops, "xs", rng.uniform(0.01, 0.02, rows).astype(np.float32))
+    elif strides:
+        ops.input("x_", (k, rows))
+        ops.from_numpy(rng.standard_normal((k, rows)).astype(np.float32), "x_")
+        ops.transpose("x_", out="x")
+    else:
+        _put(ops, "x", rng.standard_normal((rows, k)).astype(np.float32))
+    _put(ops, "w", rng.integers(0, 256, (n, k // 2)).astype(np.uint8))
+    _put(ops, "s", rng.uniform(-0.02, 0.02, (n, k // group)).astype(np.float32))
+    if zeros:
+        _put(ops, "z", rng.uniform(0, 15, (n, k // group)).astype(np.float32))
+    ops.matmul_int4("x", weights="w", scales="s", out="y", zeros="z" if zeros else None, x_scales="xs" if eight else None)
+    return ops
+
+
+@pytest.mark.parametrize("rows, k, n", [
+    (1, 32, 1), (1, 128, 16), (2, 160, 17), (1, 4096, 100), (3, 1024, 64), (4, 416, 33), (5, 5024, 99), (8, 768, 1000),
+    (13, 256, 31), (16, 2048, 48), (17, 128, 16), (50, 320, 70), (1, 128, 16500), (6, 128, 33000),
+])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_matmul_int4(rows, k, n, group, eight, zeros):
+    group = group if k % group == 0 else 32
+    ops = _int4(rows, k, n, group, eight, zeros, rows * 1000 + k + n)
+    got, want = run(ops).env["y"], evaluate(ops)["y"]
+    assert got.shape == (rows, n) and got.dtype == np.float32
+    _close(got, want, _int4_bound(ops))
+
+
+def test_matmul_int4_of_a_transposed_x():
+    ops = _int4(7, 288, 40, 32, False, True, 3, strides=True)
+    want = evaluate(ops)["y"]
+    x = ops.uploads["x_"].T
+    ops._uploads["x"] = np.ascontiguousarray(x)  # (for the bound alone)
+    bound = _int4_bound(ops)
+    del ops._uploads["x"]
+    _close(run(ops).env["y"], want, bound)
+
+
+def test_matmul_int4_ranges_and_special_values():
+    """Blocks of very different size in a row, subnormal and huge x, zero rows, and rows
+    with infinities and NaN, whose other blocks and neighbours are as ever."""
+    ops = _int4(9, 512, 37, 64, False, True, 4)
+    x = ops.uploads["x"]
+    x[0, :128] *= np.float32(1e30)
+    x[1, 128:256] *= np.float32(1e-30)
+    x[2] = (x[2].astype(np.float64) * 1e-40).astype(np.float32)
+    x[3] = 0
+    x[4, 5] = 3e38
+    x[5, 130] = np.inf
+    x[6, 300] = np.nan
+    x[7, 10], x[7, 400] = np.inf, -np.inf
+    x[8, 64:70] = -np.inf
+    got, want = run(ops).env["y"], evaluate(ops)["y"]
+    with np.errstate(invalid="ignore", over="ignore"):
+        bound = np.nan_to_num(_int4_bound(ops), nan=0.0, posinf=0.0) + 2e-45
+        want = np.where(np.abs(want) > np.finfo(np.float32).max, np.copysign(np.inf, want), want)
+    _close(got, want, bound)
+
+
+def test_matmul_int4_nibble_order_and_zero():
+    """q = 8 with no zeros is nothing; one q of 9 takes one x out, exactly."""
+    k = 256
+    x = np.arange(1, k + 1, dtype=np.float32)[None]
+    for at in (0, 1, 31, 32, 127, 128, 255):
+        w = np.full((3, k // 2), 0x88, np.uint8)
+        w[1, at // 2] += 16 if at % 2 else 1
+        ops = Operations()
+        _put(ops, "x", x)
+        _put(ops, "w", w)
+        _put(ops, "s", np.ones((3, k // 128), np.float32))
+        ops.matmul_int4("x", weights="w", scales="s", out="y")
+        np.testing.assert_array_equal(run(ops).env["y"], [[0, at + 1, 0]])
+
+
+# ---------------------------------------------------------------------------
+# cache
+# ---------------------------------------------------------------------------
+
+
+def _state(spec: KVCache, data: np.ndarray):
+    """Values as bytes and scales of all pages (the padding apart)."""
+    parts = [serving_eval._page_parts(spec, np.ascontiguousarray(data), p) for p in range(spec.pages)]
+    return np.stack([p[0] for p in parts]), None if parts[0][1] is None else np.stack([p[1] for p in parts])
+
+
+def _same_state(spec, got, want):
+    for a, b in zip(_state(spec, got), _state(spec, want)):
+        if a is not None:
+            np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pages, page_size, kv_heads, dim, tokens", [
+    (1, 1, 1, 16, 1), (5, 4, 2, 48, 7), (9, 16, 8, 128, 40), (3, 20, 3, 80, 33), (40, 64, 1, 256, 2100), (7, 3, 33, 16, 5),
+])
+def test_cache_write_and_read(dtype, pages, page_size, kv_heads, dim, tokens):
+    spec = KVCache(pages=pages, page_size=page_size, kv_heads=kv_heads, dim=dim, dtype=dtype)
+    rng = np.random.default_rng(pages * 7 + dim)
+    ops = Operations()
+    ops.kv_cache("cache", pages=pages, page_size=page_size, kv_heads=kv_heads, dim=dim, dtype=dtype)
+    old = rng.standard_normal((2, spec.slots, kv_heads, dim)).astype(np.float32)
+    ops.from_numpy(spec.pack(old[0], old[1]), "cache")
+    for name in ("k", "v"):
+        _put(ops, name, (10 ** rng.uniform(-3, 3, (tokens, 1)) * rng.standard_normal((tokens, spec.row))).astype(np.float32))
+    slots = rng.permutation(max(tokens, spec.slots))[:tokens].astype(np.int32)  # those past the cache are passed over
+    if tokens > 4:
+        slots[1], slots[2], slots[4] = -1, np.int32(2**31 - 1), slots[0]  # padding, and the same slot twice
+    _put(ops, "slots", slots)
+    back = np.concatenate([rng.permutation(spec.slots), [-5, spec.slots]]).astype(np.int32)
+    _put(ops, "back", back)
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="written")
+    ops.cache_read("written", slots="back", k_out="kb", v_out="vb")
+    env, ref = run(ops).env, evaluate(ops)
+    _same_state(spec, env["written"], ref["written"])
+    for name in ("kb", "vb"):
+        np.testing.assert_array_equal(env[name], ref[name].astype(np.float32))
+        assert np.all(env[name][-2:] == 0)
+
+
+@pytest.mark.parametrize("dtype", ["int8", "float8_e4m3"])
+def test_cache_write_rounds_to_the_nearest_step(dtype):
+    """Values on and next to every border between two steps, at scales from the
+    smallest to the largest: the exact quotient decides."""
+    rng = np.random.default_rng(8)
+    steps = np.arange(-127, 127) + 0.5 if dtype == "int8" else np.concatenate(
+        [(serving_eval.E4M3[:126] + serving_eval.E4M3[1:127]) / 2, -serving_eval.E4M3[:127]])
+    peak = 127.0 if dtype == "int8" else 448.0
+    spec = KVCache(pages=64, page_size=1, kv_heads=1, dim=256, dtype=dtype)
+    rows = []
+    for i in range(spec.slots):
+        scale = np.float32(2.0 ** rng.uniform(-149 + 9, 118) if i % 4 else 2.0 ** rng.integers(-130, 118))
+        row = (np.resize(steps, 256) * np.float64(scale)).astype(np.float32)
+        row[1::3] = np.nextafter(row[1::3], np.float32(np.inf))
+        row[2::3] = np.nextafter(row[2::3], np.float32(-np.inf))
+        row[0] = np.float32(np.float64(scale) * peak)
+        rows.append(row)
+    k = np.stack(rows)
+    k[-1], k[-2], k[-3, 5], k[-4, 6] = 0, 1e-45, np.nan, -np.inf
+    ops = Operations()
+    ops.kv_cache("cache", pages=64, page_size=1, kv_heads=1, dim=256, dtype=dtype)
+    ops.from_numpy(spec.empty(), "cache")
+    _put(ops, "k", k)
+    _put(ops, "v", -k)
+    _put(ops, "slots", rng.permutation(64).astype(np.int32))
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="written")
+    _same_state(spec, run(ops).env["written"], evaluate(ops)["written"])
+
+
+@pytest.mark.parametrize("tokens, kv_heads", [(100, 1), (300, 8), (3000, 2)])
+def test_of_rows_that_name_one_slot_the_last_is_stored(tokens, kv_heads):
+    spec = KVCache(pages=4, page_size=4, kv_heads=kv_heads, dim=16, dtype="int8")
+    rng = np.random.default_rng(tokens)
+    ops = Operations()
+    ops.kv_cache("cache", pages=4, page_size=4, kv_heads=kv_heads, dim=16, dtype="int8")
+    ops.from_numpy(spec.empty(), "cache")
+    for name in ("k", "v"):
+        _put(ops, name, rng.standard_normal((tokens, spec.row)).astype(np.float32))
+    _put(ops, "slots", rng.integers(-2, 18, tokens).astype(np.int32))
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="written")
+    want = evaluate(ops)["written"]
+    for _ in range(3):
+        _same_state(spec, run(ops).env["written"], want)
+
+
+def test_cache_write_of_strided_rows():
+    spec = KVCache(pages=3, page_size=8, kv_heads=2, dim=32, dtype="float8_e4m3")
+    rng = np.random.default_rng(11)
+    ops = Operations()
+    ops.kv_cache("cache", pages=3, page_size=8, kv_heads=2, dim=32, dtype="float8_e4m3")
+    ops.from_numpy(spec.empty(), "cache")
+    _put(ops, "k_", rng.standard_normal((64, 9)).astype(np.float32))
+    ops.transpose("k_", out="k")
+    _put(ops, "v_", rng.standard_normal((18, 32)).astype(np.float32))
+    ops.reshape("v_", (9, 64), out="v")
+    _put(ops, "slots", rng.permutation(24)[:9].astype(np.int32))
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="written")
+    _same_state(spec, run(ops).env["written"], evaluate(ops)["written"])
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+
+def _attention(dtype, heads, kv_heads, dim, page_size, width, lengths, seed=0, holes=(), scale=None):
+    """A program over pages in no order; rows that no position reaches hold NaN."""
+    rng = np.random.default_rng(seed)
+    b = len(lengths)
+    used = [min(width, max(0, -(-n // page_size))) for n in lengths]
+    pages = sum(used) + 2
+    spec = KVCache(pages=pages, page_size=page_size, kv_heads=kv_heads, dim=dim, dtype=dtype)
+    k, v = rng.standard_normal((2, spec.slots, kv_heads, dim)).astype(np.float32)
+    order, at = rng.permutation(pages), 0
+    table = np.full((b, width), -1, np.int32)
+    live = np.zeros(spec.slots, bool)
+    for i, u in enumerate(used):
+        table[i, :u] = order[at : at + u]
+        at += u
+        for p in range(min(lengths[i], width * page_size)):
+            live[table[i, p // page_size] * page_size + p % page_size] = True
+    for i, page, bad in holes:
+        table[i, page] = bad
+    k[~live], v[~live] = np.nan, np.nan
+    ops = Operations()
+    ops.kv_cache("cache", pages=pages, page_size=page_size, kv_heads=kv_heads, dim=dim, dtype=dtype)
+    ops.from_numpy(spec.pack(k, v), "cache")
+    _put(ops, "q", rng.standard_normal((b, heads * dim)).astype(np.float32))
+    _put(ops, "pages", table)
+    _put(ops, "lengths", np.array(lengths, np.int32))
+    ops.paged_attention("q", cache="cache", pages="pages", lengths="lengths", out="o", heads=heads, scale=scale)
+    return ops
+
+
+def _attention_bound(ops: Operations) -> np.ndarray:
+    """A score q . k * scale * log2(e): the factor rounds once, q times it once, the
+    products' fma chain dim times, the two halves' sum and a key's scale once more, so
+    (dim + 5) u of sum |q||k| scale, in both numerator and denominator: twice that in
+    the exponent.  2^x of the device and the difference x - m add 2^-22 and u of the
+    largest |score| log2(e).  Weights and sums are added in chains no longer than the
+    positions, with at most 3 more roundings for each joining step and a value's scale."""
+    (op,) = ops.build()
+    found = []
+    get = lambda t: ops.uploads[t.buffer_key]  # noqa: E731
+    share = op.heads // op.spec.kv_heads
+    for q, k, v in serving_eval.attention_rows(op, get):
+        o = np.zeros(q.shape)
+        for h in range(op.heads if k.shape[1] else 0):
+            kk, vv = np.nan_to_num(np.abs(k[h // share])), np.nan_to_num(np.abs(v[h // share]))
+            mag = (kk @ np.abs(q[h])) * abs(op.scale)
+            s = k[h // share] @ q[h] * op.scale
+            e = np.exp(s - s.max())
+            p = e / e.sum()
+            chain = kk.shape[0]
+            rel = 2 * (op.spec.dim + 5) * U * mag.max() + 4 * U * mag.max() + 2 * 2.0**-22 + 2 * (chain + 16) * U
+            o[h] = 1.1 * rel * (p @ vv)
+        found.append(o.reshape(-1))
+    return np.stack(found) + 1e-30
+
+
+CASES = [
+    # heads, kv_heads, dim, page_size, width, lengths
+    (1, 1, 16, 1, 3, [1, 2, 3]),
+    (4, 4, 64, 16, 4, [0, 1, 15, 16, 17, 64]),
+    (8, 2, 128, 16, 40, [640, 5, 0, 333]),
+    (6, 2, 96, 20, 9, [180, 41, 1]),
+    (16, 1, 128, 64, 5, [320, 257]),
+    (40, 2, 80, 48, 7, [336, 47, 49]),
+    (17, 1, 32, 7, 30, [210, 100]),
+    (8, 8, 256, 32, 12, [384, 31]),
+    (3, 3, 48, 5, 13, [65, 64, 1]),
+    (12, 4, 112, 16, 20, [77, 320]),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv_heads, dim, page_size, width, lengths", CASES)
+def test_paged_attention(dtype, heads, kv_heads, dim, page_size, width, lengths):
+    ops = _attention(dtype, heads, kv_heads, dim, page_size, width, lengths, seed=dim + heads)
+    _close(run(ops).env["o"], evaluate(ops)["o"], _attention_bound(ops))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_paged_attention_of_long_split_sequences(dtype):
+    """Lengths that end inside a part, at its border and in the first of many, joined
+    by the last workgroup; the same bits every time."""
+    ops = _attention(dtype, 8, 2, 64, 16, 256, [4096, 4095, 1, 1023, 0, 2049], seed=3)
+    (g,) = compile_program(ops)
+    assert g.kernel.workspace_bytes > 0
+    first = run(ops).env["o"]
+    _close(first, evaluate(ops)["o"], _attention_bound(ops))
+    for _ in range(4):
+        np.testing.assert_array_equal(run(ops).env["o"], first)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page_size", [16, 12])
+def test_paged_attention_bad_pages_and_lengths(dtype, page_size):
+    """Holes in the table (negative numbers, numbers past the cache), lengths below
+    zero and beyond the table."""
+    holes = [(0, 1, -1), (0, 2, 10**6), (1, 0, -(2**31)), (1, 1, 2**31 - 1), (1, 2, -7), (3, 0, -1)]
+    ops = _attention(dtype, 4, 2, 64, page_size, 6, [6 * page_size, 3 * page_size, 5, 2 * page_size + 1], seed=9, holes=holes)
+    lengths = ops.uploads["lengths"]
+    lengths[0] = 2**31 - 1
+    lengths[2] = -3
+    env = run(ops).env["o"]
+    _close(env, evaluate(ops)["o"], _attention_bound(ops))
+    assert np.all(env[1] == 0) and np.all(env[2] == 0)
+
+
+def test_paged_attention_values_that_are_not_finite():
+    """Scores of -inf weigh nothing beside others and give NaN alone, as softmax does;
+    an infinite value reaches its own dim."""
+    spec = KVCache(pages=3, page_size=16, kv_heads=1, dim=16)
+    rng = np.random.default_rng(12)
+    k, v = rng.standard_normal((2, spec.slots, 1, 16)).astype(np.float32)
+    k[:, 0, 0] = np.abs(k[:, 0, 0]) + 1
+    k[3, 0, 0] = k[20, 0, 0] = -np.inf  # one among others
+    k[32:, 0, 0] = -np.inf  # a sequence of nothing else
+    v[5, 0, 2], v[7, 0, 3] = np.inf, np.nan
+    ops = Operations()
+    ops.kv_cache("cache", pages=3, page_size=16, kv_heads=1, dim=16)
+    ops.from_numpy(spec.pack(k, v), "cache")
+    _put(ops, "q", np.abs(rng.standard_normal((2, 32))).astype(np.float32))
+    _put(ops, "pages", np.array([[0, 1], [2, -1]], np.int32))
+    _put(ops, "lengths", np.array([32, 16], np.int32))
+    ops.paged_attention("q", cache="cache", pages="pages", lengths="lengths", out="o", heads=2)
+    got, want = run(ops).env["o"], evaluate(ops)["o"]
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    np.testing.assert_array_equal(np.isinf(got), np.isinf(want))
+    assert np.all(np.isnan(got[1])) and np.isinf(got[0, 2]) and np.isnan(got[0, 3])
+    fine = np.isfinite(want)
+    np.testing.assert_allclose(got[fine], want[fine], rtol=1e-5, atol=1e-6)
+
+
+def test_paged_attention_large_and_small_scores():
+    """Scores of hundreds (one position takes all), and a scale of 0 (the mean)."""
+    ops = _attention("float32", 4, 2, 64, 16, 8, [100, 128], seed=4, scale=20.0)
+    got, want = run(ops).env["o"], evaluate(ops)["o"]
+    _close(got, want, _attention_bound(ops))
+    ops = _attention("int8", 4, 2, 64, 16, 8, [100, 128], seed=4, scale=0.0)
+    _close(run(ops).env["o"], evaluate(ops)["o"], _attention_bound(ops))
+
+
+# ---------------------------------------------------------------------------
+# together, and the ways a program runs
+# ---------------------------------------------------------------------------
+
+B, DIM, HEADS, KV, WIDTH_FF = 3, 64, 4, 2, 384
+
+
+def _step_program(dtype: str, seed: int, weights_seed: int = 1) -> Operations:
+    """One decode step: norm in 8 bits -> q, k, v -> cache -> attention -> output
+    projection -> residual norm -> gated block, in the framework's other ops too."""
+    hidden = HEADS * DIM
+    rng, wrng = np.random.default_rng(seed), np.random.default_rng(weights_seed)
+    ops = Operations()
+    _put(ops, "h0", rng.standard_normal((B, hidden)).astype(np.float32))
+    _put(ops, "norm1", (1 + 0.1 * wrng.standard_normal(hidden)).astype(np.float32))
+    _put(ops, "norm2", (1 + 0.1 * wrng.standard_normal(hidden)).astype(np.float32))
+
+    def weight(name, n, k, group=64):
+        _put(ops, name, wrng.integers(0, 256, (n, k // 2)).astype(np.uint8))
+        _put(ops, name + "_s", (wrng.uniform(0.5, 1.5, (n, k // group)) / (4.6 * np.sqrt(k))).astype(np.float32))
+
+    weight("wq", hidden, hidden)
+    weight("wk", KV * DIM, hidden)
+    weight("wv", KV * DIM, hidden)
+    weight("wo", hidden, hidden)
+    weight("w1", WIDTH_FF, hidden)
+    weight("w2", WIDTH_FF, hidden)
+    weight("w3", hidden, WIDTH_FF, 128)
+    spec = ops.kv_cache("cache", pages=8, page_size=4, kv_heads=KV, dim=DIM, dtype=dtype)
+    old = rng.standard_normal((2, spec.slots, KV, DIM)).astype(np.float32)
+    ops.from_numpy(spec.pack(old[0], old[1]), "cache")
+    table = rng.permutation(8)[: 2 * B].reshape(B, 2).astype(np.int32)
+    lengths = np.array([1, 4, 7], np.int32)  # with the new token
+    _put(ops, "pages", table)
+    _put(ops, "lengths", lengths)
+    _put(ops, "slots", np.array([table[i, (n - 1) // 4] * 4 + (n - 1) % 4 for i, n in enumerate(lengths)], np.int32))
+
+    ops.rms_norm("h0", weight="norm1", out="x8", scales="xs")
+    for p in "qkv":
+        ops.matmul_int4("x8", weights=f"w{p}", scales=f"w{p}_s", x_scales="xs", out=p)
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="cache1")
+    ops.paged_attention("q", cache="cache1", pages="pages", lengths="lengths", heads=HEADS, out="a")
+    ops.matmul_int4("a", weights="wo", scales="wo_s", out="attn")
+    ops.rms_norm("attn", residual="h0", sum_out="h1", weight="norm2", out="x2")
+    ops.matmul_int4("x2", weights="w1", scales="w1_s", out="g1")
+    ops.matmul_int4("x2", weights="w2", scales="w2_s", out="g2")
+    ops.elementwise("negate", out="n", operands=("g1",))
+    ops.elementwise("exp", out="e", operands=("n",))
+    ops.elementwise("add", out="p", operands=("e", 1.0))
+    ops.elementwise("recip", out="sig", operands=("p",))
+    ops.elementwise("mul", out="g", operands=("g1", "sig"))
+    ops.elementwise("mul", out="z", operands=("g", "g2"))
+    ops.matmul_int4("z", weights="w3", scales="w3_s", out="mlp")
+    ops.elementwise("add", out="h2", operands=("mlp", "h1"))
+    return ops
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_decode_step(dtype):
+    """Stages round to 8 bits between exact ones, so a last bit before a border moves a
+    value by a step (1/127 of its row's largest, 2^-4 of itself in e4m3); a step moves a
+    few values in hundreds, each weighed by about 1/sqrt(256)."""
+    ops = _step_program(dtype, 2)
+    env, ref = run(ops).env, evaluate(ops)
+    np.testing.assert_array_equal(env["x8"], ref["x8"])
+    for name in ("q", "k", "v"):
+        np.testing.assert_allclose(env[name], ref[name], rtol=0, atol=256 * 40 * U)
+    step = 2.0**-4 if dtype == "float8_e4m3" else 2.0**-7
+    assert np.all(np.isfinite(env["h2"]))
+    rms = np.sqrt(np.mean(ref["h2"] ** 2))
+    assert np.sqrt(np.mean((env["h2"] - ref["h2"]) ** 2)) <= (step if dtype != "float32" else 1e-5) * rms
+
+
+def _resident(ops: Operations, groups):
+    env = {name: Buffer.from_numpy(a) for name, a in ops.uploads.items()}
+    for t in ops.tensors.values():
+        if t.buffer_key not in env:
+            env[t.buffer_key] = Buffer(t.nbytes)
+            env[t.buffer_key].fill(0xFF)
+    return env
+
+
+def test_a_resident_program_runs_again_and_again():
+    """Device buffers, one launch sequence: the same results each time, and two programs
+    in turn (they share the workspace) do not disturb each other."""
+    programs = [_attention("int8", 8, 2, 64, 16, 256, [4096, 700], seed=s) for s in (1, 2)]
+    want = [run(ops).env["o"] for ops in programs]
+    made = []
+    for ops in programs:
+        groups = compile_program(ops)
+        made.append((Runtime(tuple(Dispatch(g.kernel, g.bindings, g.dims, g.grid, g.threads) for g in groups)), _resident(ops, groups)))
+    for _ in range(3):
+        for (runtime, env), o in zip(made, want):
+            runtime.run(env)
+        for (runtime, env), o in zip(made, want):
+            np.testing.assert_array_equal(env["o"].numpy(o.shape, np.float32), o)
+
+
+def test_decoding_token_after_token():
+    """The cache lives in a device buffer over several steps, each writing a slot and
+    attending over what is there: as a whole recomputation gives it."""
+    spec = KVCache(pages=4, page_size=4, kv_heads=2, dim=32, dtype="int8")
+    rng = np.random.default_rng(21)
+    ops = Operations()
+    ops.kv_cache("cache", pages=4, page_size=4, kv_heads=2, dim=32, dtype="int8")
+    ops.from_numpy(spec.empty(), "cache")
+    for name in ("k", "v"):
+        _put(ops, name, np.zeros((1, 64), np.float32))
+    _put(ops, "q", np.zeros((1, 128), np.float32))
+    _put(ops, "slots", np.zeros(1, np.int32))
+    _put(ops, "pages", np.array([[2, 0, 3, 1]], np.int32))
+    _put(ops, "lengths", np.zeros(1, np.int32))
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="c1")
+    ops.paged_attention("q", cache="c1", pages="pages", lengths="lengths", heads=4, out="o")
+    groups = compile_program(ops)
+    env = _resident(ops, groups)
+    runtime = Runtime(tuple(Dispatch(g.kernel, g.bindings, g.dims, g.grid, g.threads) for g in groups))
+    state = spec.empty()
+    for t in range(16):
+        step = {n: rng.standard_normal(ops.tensors[n].shape).astype(np.float32) for n in ("k", "v", "q")}
+        step["slots"] = np.array([[2, 0, 3, 1][t // 4] * 4 + t % 4], np.int32)
+        step["lengths"] = np.array([t + 1], np.int32)
+        for name, a in step.items():
+            env[name].write(a)
+        runtime.run(env)
+        inputs = {**ops.uploads, **step, "cache": state}
+        ref = evaluate(ops, inputs)
+        state = ref["c1"]
+        np.testing.assert_allclose(env["o"].numpy((1, 128), np.float32), ref["o"], rtol=0, atol=2e-5)
+    _same_state(spec, env["cache"].numpy(spec.shape, np.uint8), state)
+
+
+def test_batched_programs_give_the_same_as_each_alone():
+    programs = [_step_program("int8", s) for s in (1, 2, 3)]
+    alone = [run(ops).env for ops in programs]
+    together = run_batch(programs)
+    for a, b in zip(alone, together):
+        for name in ("x8", "k", "cache1", "a", "h2"):
+            np.testing.assert_array_equal(a[name], b.env[name])
+
+
+def test_a_batch_of_split_attentions():
+    programs = [_attention("float32", 4, 2, 64, 16, 128, [2048, 1000 + s], seed=s) for s in range(3)]
+    for ops, got in zip(programs, run_batch(programs)):
+        _close(got.env["o"], evaluate(ops)["o"], _attention_bound(ops))
+
+
+def test_launches_that_allocate_nothing():
+    """``launch_noalloc`` with its static scratch: the join's counters are left zero."""
+    ops = _attention("float8_e4m3", 8, 2, 64, 16, 256, [4096, 513], seed=6)
+    want = run(ops).env["o"]
+    (g,) = compile_program(ops)
+    env = _resident(ops, (g,))
+    for _ in range(3):
+        env["o"].fill(0xFF)
+        err = hip_backend.launch_noalloc(g.kernel.handle, [env[k] for k in g.bindings], g.dims, g.kernel.dims_slot_index, g.grid,
+                                         g.threads, scratch=g.kernel.workspace_bytes)
+        assert err == 0
+        np.testing.assert_array_equal(env["o"].numpy(want.shape, np.float32), want)
+
+
+def test_a_cache_beyond_4_gib():
+    """Pages whose bytes lie past 32 bits."""
+    pages, page_size = 5000, 16
+    spec = KVCache(pages=pages, page_size=page_size, kv_heads=32, dim=256)
+    assert spec.pages * spec.page_bytes > 2**32 + 2**28
+    ops = Operations()
+    ops.kv_cache("cache", pages=pages, page_size=page_size, kv_heads=32, dim=256)
+    rng = np.random.default_rng(30)
+    t = 20
+    slots = np.concatenate([[(pages - 1) * page_size + i for i in range(10)], 4 * page_size + np.arange(10)]).astype(np.int32)
+    for name in ("k", "v"):
+        _put(ops, name, rng.standard_normal((t, spec.row)).astype(np.float32))
+    _put(ops, "slots", slots)
+    _put(ops, "q", rng.standard_normal((1, 32 * 256)).astype(np.float32))
+    _put(ops, "pages", np.array([[pages - 1, 4]], np.int32))
+    _put(ops, "lengths", np.array([10], np.int32))
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="c1")
+    ops.cache_read("c1", slots="slots", k_out="kb", v_out="vb")
+    ops.paged_attention("q", cache="c1", pages="pages", lengths="lengths", heads=32, out="o")
+    groups = compile_program(ops)
+    env = _resident(ops, groups)  # 0xFF everywhere: NaN
+    env["cache"] = env["cache"] if "cache" in env else Buffer(spec.pages * spec.page_bytes)
+    Runtime(tuple(Dispatch(g.kernel, g.bindings, g.dims, g.grid, g.threads) for g in groups)).run(env)
+    for name, src in (("kb", "k"), ("vb", "v")):
+        np.testing.assert_array_equal(env[name].numpy((t, spec.row), np.float32), ops.uploads[src])
+    k, v = (ops.uploads[n][:10].reshape(10, 32, 256).astype(np.float64) for n in "kv")
+    q = ops.uploads["q"].reshape(32, 256).astype(np.float64)
+    s = np.einsum("hd,phd->hp", q, k) / 16
+    p = np.exp(s - s.max(1, keepdims=True))
+    want = np.einsum("hp,phd->hd", p / p.sum(1, keepdims=True), v)
+    np.testing.assert_allclose(env["o"].numpy((32, 256), np.float32), want, rtol=0, atol=1e-4)
+    for b in env.values():
+        b.release()
+    hip_backend.trim()
