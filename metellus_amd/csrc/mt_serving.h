@@ -276,7 +276,9 @@ MT_INLINE void mt_cache_put(unsigned char* cache, const mt_f32x4 (&v)[(D + 63u) 
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) top = __builtin_fmaxf(top, mt_shfl_xor(top, off));
         const bool fine = top < INFINITY;
-        const float s = fine ? top / (KIND == 2 ? 448.0f : 127.0f) : NAN;
+        // (the reciprocal's rounding moves a scale by an ulp at most; values are
+        // rounded against the scale that is stored)
+        const float s = fine ? top * (1.0f / (KIND == 2 ? 448.0f : 127.0f)) : NAN;
         // Near the smallest scales the reciprocal overflows and steps times the
         // scale lose bits: there both sides of the quotient are taken 2^64 larger.
         const float up = s < 0x1.0p-100f ? 0x1.0p+64f : 1.0f;
@@ -384,33 +386,46 @@ MT_INLINE void mt_cache_read(const unsigned char* cache, const int* slots, float
 // ---------------------------------------------------------------------------
 // Attention of one new token per sequence over the paged cache.
 //
-// A workgroup takes one sequence, one key head with the (at most 16) query
-// heads that share it, and one part of the sequence's length; each of its waves
-// takes every WAVES-th tile of 16 positions on its own, and they meet at the end.
+// The work is a row of units, STEP positions each of one sequence and one key head
+// with HELD (at most 16) of the query heads that share it, sequence after sequence.
+// The lengths are known on the device alone, so the P workgroups of the launch cut
+// that row into equal ranges there: a workgroup has the same share of a ragged batch
+// as the others, and a table with room for far more positions costs nothing.  Where
+// a range begins or ends inside a sequence's head, the parts go to the workspace and
+// the last workgroup to arrive joins them, in their order.
 //
-//   scores  S[position, head] = K . q: fp32 MFMAs 16x16x4, K the rows.  Lane
-//     (n, g) = (lane % 16, lane / 16) loads row n's dims VK (4 jj + g) .. + VK - 1
-//     whole, and element e of load jj is its operand of MFMA (jj, e): the four
-//     dims of that product are the ones at e in each g's piece, for K and q alike.
-//   softmax S comes back with lane (n, g) holding head n at positions 4 g + i,
-//     i < 4; the running maximum m (in units of log 2: the scale carries
+// Within a range each of the workgroup's waves takes every WAVES-th tile of positions
+// on its own, and they meet at the end.  With (n, g) = (lane % 16, lane / 16):
+//
+//   scores  S[position, column] = K . q by MFMAs whose rows are 16 positions:
+//     lane (n, g) loads row n's dims VK (4 jj + g) .. + VK - 1 whole, and they are
+//     its operands as they stand: which dims one MFMA takes together is the same
+//     for K and q, so nothing is rearranged.
+//   softmax S comes back with lane (n, g) holding column n at positions 4 g + i,
+//     i < 4.  The running maximum m (in units of log 2: the scale carries
 //     log2(e)) is shared by the four g of a head, the sum l is each lane's own
-//     until the end.  The sums so far are rescaled only when some head's
-//     maximum grows.
-//   output  O[head, dim] += P . V: MFMA i takes positions {4 g + i}, so p[i] is
-//     its P operand where it stands, and lane (n, g) loads row 4 g + i's dims
-//     VV (16 c + n) .. + VV - 1 of V, element e being the operand for the dims
-//     that stand at e.  No value changes lanes and nothing is transposed.
+//     until the end.  The sums so far are rescaled only when some head's maximum
+//     grows.
+//   output  O[row, dim] += P . V: p[i] of positions 4 g + i is the P operand where
+//     it stands, and lane (n, g) loads rows 4 g + i's dims VV (16 c + n) .. + VV - 1
+//     of V.  No value changes lanes.
 //
-// 8-bit values are widened in registers; a position's scales multiply its score
-// and its weight.  A position that is masked (behind the length, or in a page
-// outside the cache) scores -inf and its values are replaced by zeros, whatever
-// its bytes hold.
+// KIND 0 (fp32): MFMAs 16x16x4 in fp32, tiles of 16 positions, a column a head, and
+// each value of V an operand by itself.
+// 8 bits: the values are exact in bf16, and q and p are three bf16 parts each (hi,
+// mid, lo: their 24 bits), in columns and rows 4 h + part of sets of 4 heads: MFMAs
+// 16x16x32, tiles of 32 positions.  The fp32 MFMAs take 64 values of the cache in 32
+// cycles, 4.9e12 a second on the GPU -- no more than HBM brings at one byte each;
+// these take 512 in 16.  Four rows of V are exchanged byte by byte in registers, so
+// that a dim's positions stand together.  (Weights below 2^-110 lose low parts.)
 //
-// Bound: HBM, K and V once.  The fp32 MFMAs take 64 elements in 32 cycles
-// whatever the number of heads that share them, 4.9e12 elements a second, which
-// exceeds HBM for fp32 and about matches it for 8 bits.
+// A position's scales multiply its score and its weight.  A position that is
+// masked (behind the length, or in a page outside the cache) scores -inf and its
+// values are replaced by zeros, whatever its bytes hold.  Bound: HBM, K and V once.
 // ---------------------------------------------------------------------------
+
+typedef short mt_i16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned mt_u32x2 __attribute__((ext_vector_type(2)));
 
 template <unsigned W>
 MT_INLINE void mt_ld_words(unsigned (&to)[W], const unsigned char* p) {
@@ -418,226 +433,466 @@ MT_INLINE void mt_ld_words(unsigned (&to)[W], const unsigned char* p) {
         const mt_u32x4 v = *reinterpret_cast<const mt_u32x4*>(p);
         to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
     } else if constexpr (W == 2u) {
-        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-        const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+        const mt_u32x2 v = *reinterpret_cast<const mt_u32x2*>(p);
         to[0] = v.x, to[1] = v.y;
     } else {
         to[0] = *reinterpret_cast<const unsigned*>(p);
     }
 }
-// Four values of a held type from the words at 4 e of a row.
-template <int KIND, unsigned W>
-MT_INLINE mt_f32x4 mt_four(const unsigned (&w)[W], unsigned e) {
-    if constexpr (KIND == 0)
-        return mt_f32x4{__uint_as_float(w[4u * e]), __uint_as_float(w[4u * e + 1u]), __uint_as_float(w[4u * e + 2u]),
-                        __uint_as_float(w[4u * e + 3u])};
-    else
-        return mt_held4<KIND>(w[e]);
+
+// Byte i of a, b, c, d together in to[i].
+MT_INLINE void mt_bytes4(unsigned a, unsigned b, unsigned c, unsigned d, unsigned (&to)[4]) {
+    const unsigned ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+    const unsigned cd0 = __builtin_amdgcn_perm(d, c, 0x05010400u), cd1 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+    to[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u);
+    to[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
+    to[2] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u);
+    to[3] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
 }
 
-template <int KIND, unsigned HK, unsigned PS, unsigned D, unsigned PAGES, unsigned WIDTH, unsigned SHARE, unsigned WAVES,
-          unsigned SPLITS, unsigned EACH, unsigned BATCH, unsigned QRS, unsigned QCS>
-MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, const int* pages, const int* lengths,
-                                  float* o, double scale, float* ws, unsigned rows, unsigned char* lds) {
-    using C = mt_cache<KIND, HK, PS, D>;
-    constexpr unsigned ITEM = C::ITEM, PARTS = (SHARE + 15u) / 16u, HELD = SHARE < 16u ? SHARE : 16u;
-    constexpr unsigned VK = KIND == 0 ? 4u : D % 64u == 0u ? 16u : D % 32u == 0u ? 8u : 4u, NJ = D / (4u * VK);
-    constexpr unsigned VV = KIND == 0 || D <= 64u ? 4u : 8u, NV = (D + 16u * VV - 1u) / (16u * VV);
-    constexpr unsigned KW = VK * ITEM / 4u, VW = VV * ITEM / 4u, FLOATS = HELD * (D + 2u);
-    constexpr bool ONE_PAGE = PS % 16u == 0u;  // a tile lies in one page
-    const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
-    const unsigned split = blockIdx.x % SPLITS, pair = blockIdx.x / SPLITS;
-    const unsigned part = pair % PARTS, head = pair / PARTS % HK, b = pair / (PARTS * HK);
-    // (a batch larger than the workspace was laid out for is not split)
-    const bool joined = SPLITS > 1u && gridDim.z <= BATCH;
-    const int asked = lengths[b];
-    const unsigned len = asked < 0 ? 0u : (unsigned)asked < WIDTH * PS ? (unsigned)asked : WIDTH * PS;
-    const unsigned active = joined && len > EACH ? (len + EACH - 1u) / EACH : 1u;
-    if (split >= active) return;
-    const unsigned first = active > 1u ? split * EACH : 0u;
-    const unsigned last = active > 1u && len - first > EACH ? first + EACH : len;
-    const unsigned tiles = (last - first + 15u) / 16u;
-
-    mt_f32x4 qf[NJ][VK / 4u];
-    {
-        const unsigned h = part * 16u + n;
-        const float by = (float)(scale * 1.4426950408889634);
-#pragma unroll
-        for (unsigned jj = 0; jj < NJ; ++jj)
-#pragma unroll
-            for (unsigned e = 0; e < VK / 4u; ++e) {
-                qf[jj][e] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-                if (n < HELD && h < SHARE)
-                    qf[jj][e] = mt_row4<HK * SHARE * D, QCS>(q + (size_t)b * QRS,
-                                                             (head * SHARE + h) * D + VK * (4u * jj + g) + 4u * e) * by;
-            }
+// Four 8-bit values as four bf16 in two words (exact).
+template <int KIND>
+MT_INLINE mt_u32x2 mt_held4_bf16(unsigned w) {
+    if constexpr (KIND == 1) {
+        const mt_f32x4 f = mt_held4<1>(w);
+        return mt_u32x2{__builtin_amdgcn_perm(__float_as_uint(f.y), __float_as_uint(f.x), 0x07060302u),
+                        __builtin_amdgcn_perm(__float_as_uint(f.w), __float_as_uint(f.z), 0x07060302u)};
+    } else {
+        return mt_u32x2{__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+                        __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
     }
+}
+
+// Part `j` of x's three bf16 parts (8 bits each, together all 24), as a float whose
+// low half is 0; nothing for j = 3.
+MT_INLINE float mt_bf16_part(float x, unsigned j) {
+    const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), r = x - hi;
+    const float mid = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
+    return j == 0u ? hi : j == 1u ? mid : j == 2u ? r - mid : 0.f;
+}
+// Two such parts in one word.
+MT_INLINE unsigned mt_bf16_pair(float lo, float hi) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+MT_INLINE mt_f32x4 mt_mfma16_bf16(mt_u32x4 a, mt_u32x4 b, mt_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mt_bf16x8, a), __builtin_bit_cast(mt_bf16x8, b),
+                                                   c, 0, 0, 0);
+}
+
+// v (op) over the four lanes of the same n.
+template <typename OP>
+MT_INLINE float mt_fold_g(float v, OP op) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <bool SMALL>
+struct mt_count {
+    using type = unsigned;
+};
+template <>
+struct mt_count<false> {
+    using type = unsigned long long;
+};
+
+// The units of a launch: which sequence and head they belong to, and which
+// workgroup has them.  Whole waves call its functions; their results are uniform.
+template <unsigned ROWS, unsigned STEP, unsigned MOST, unsigned HEADS, unsigned GROUPS>
+struct mt_units {
+    // Every product of units and workgroups fits in N.
+    static constexpr unsigned long long ROOM = (unsigned long long)ROWS * HEADS * ((MOST + STEP - 1ull) / STEP);
+    using N = typename mt_count<(ROOM * (GROUPS + 1ull) < (1ull << 32))>::type;
+    static constexpr int LAST = ROWS < 64u ? (int)ROWS - 1 : 63;  // the lane whose sum is a scan's whole
+    const int* lengths;
+    unsigned steps_, sum_;  // of this lane's sequence, and those up to it (64 sequences at most)
+    unsigned workgroups;
+    N all;
+
+    MT_INLINE static unsigned length(int asked) { return asked < 0 ? 0u : (unsigned)asked < MOST ? (unsigned)asked : MOST; }
+    // The steps of this lane's sequence of the 64 from b0, and the sum of those up to
+    // it.  A sequence without keys has a step too: its zeros are somebody's.
+    MT_INLINE void scan(unsigned b0, unsigned& steps, unsigned& sum) const {
+        const unsigned b = b0 + mt_lane();
+        const unsigned n = b < ROWS ? (length(lengths[b]) + STEP - 1u) / STEP : 0u;
+        steps = b < ROWS && n == 0u ? 1u : n;
+        sum = steps;
+#pragma unroll
+        for (unsigned off = 1u; off < (ROWS < 64u ? ROWS : 64u); off <<= 1) {
+            const unsigned v = (unsigned)__shfl_up((int)sum, off, 64);
+            if (mt_lane() >= off) sum += v;
+        }
+    }
+    MT_INLINE void init(const int* lengths_, unsigned most) {
+        lengths = lengths_;
+        all = 0u;
+        for (unsigned b0 = 0; b0 < ROWS; b0 += 64u) {
+            scan(b0, steps_, sum_);
+            all += (N)(unsigned)__builtin_amdgcn_readlane((int)sum_, LAST) * HEADS;
+        }
+        workgroups = all < most ? (unsigned)all : most;
+    }
+    // The sequence that unit u < all belongs to, the units before it and its steps.
+    MT_INLINE unsigned find(N u, N& at, unsigned& steps) const {
+        at = 0u;
+        for (unsigned b0 = 0;; b0 += 64u) {
+            unsigned mine = steps_, sum = sum_;
+            if (ROWS > 64u) scan(b0, mine, sum);
+            const unsigned long long past = __ballot(at + (N)sum * HEADS > u);
+            if (past || b0 + 64u >= ROWS) {
+                const int who = __builtin_ctzll(past);
+                steps = (unsigned)__builtin_amdgcn_readlane((int)mine, who);
+                at += (N)((unsigned)__builtin_amdgcn_readlane((int)sum, who) - steps) * HEADS;
+                return b0 + (unsigned)who;
+            }
+            at += (N)(unsigned)__builtin_amdgcn_readlane((int)sum, LAST) * HEADS;
+        }
+    }
+    MT_INLINE N first(unsigned w) const { return all * w / workgroups; }
+    MT_INLINE unsigned owner(N u) const { return (unsigned)(((u + 1u) * workgroups - 1u) / all); }
+};
+
+template <int KIND, unsigned HK, unsigned PS, unsigned D, unsigned PAGES, unsigned WIDTH, unsigned SHARE, unsigned HELD,
+          unsigned WAVES, unsigned GROUPS, unsigned BATCH, unsigned ROWS, unsigned QRS, unsigned QCS>
+MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, const int* pages, const int* lengths,
+                                  float* o, double scale, float* ws, unsigned char* lds) {
+    using C = mt_cache<KIND, HK, PS, D>;
+    constexpr unsigned ITEM = C::ITEM, PARTS = (SHARE + HELD - 1u) / HELD;
+    constexpr bool WIDE = KIND == 0;
+    constexpr unsigned BLOCKS = WIDE ? 1u : 2u, TILE = 16u * BLOCKS;       // positions of a tile
+    constexpr unsigned SETS = WIDE ? 1u : (HELD + 3u) / 4u;                // MFMA column sets
+    constexpr unsigned VK = WIDE ? 4u : D % 64u == 0u ? 16u : D % 32u == 0u ? 8u : 4u, NJ = D / (4u * VK);
+    constexpr unsigned VV = WIDE || D <= 64u ? 4u : 8u, NV = (D + 16u * VV - 1u) / (16u * VV);
+    constexpr unsigned KW = VK * ITEM / 4u, VW = VV * ITEM / 4u, FLOATS = HELD * (D + 2u);
+    constexpr unsigned STEP = TILE * WAVES;
+    constexpr bool ONE_PAGE = PS % 16u == 0u;  // 16 positions lie in one page
+    const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
+
+    // LDS: the operands of q, 16 bytes a lane each; then the waves' parts, [WAVES][HELD][D]
+    // sums and [WAVES][HELD] of m and of l.
+    constexpr unsigned KO = WIDE ? 4u : VK < 8u ? VK : 8u, NO = VK / KO, OPS = NJ * NO;
+    mt_u32x4* qs = reinterpret_cast<mt_u32x4*>(lds);  // [SETS][OPS][64]
+    float* sums = reinterpret_cast<float*>(lds + SETS * OPS * 1024u);
+    float* ms = sums + WAVES * HELD * D;
+    float* ls = ms + WAVES * HELD;
+    unsigned* flag = reinterpret_cast<unsigned*>(ls + WAVES * HELD);
+
+    using U = mt_units<ROWS, STEP, WIDTH * PS, HK * PARTS, GROUPS>;
+    U units;
+    // (a batch larger than the workspace was laid out for is not split)
+    units.init(lengths, gridDim.z <= BATCH ? GROUPS : 1u);
+    if (blockIdx.x >= units.workgroups) return;
+    const typename U::N end = units.first(blockIdx.x + 1u);
+    for (typename U::N unit = units.first(blockIdx.x); unit < end;) {
+    typename U::N before;
+    unsigned steps;
+    const unsigned b = units.find(unit, before, steps);
+    const unsigned in = (unsigned)(unit - before);  // from the sequence's first unit
+    const unsigned pair = in / steps, step = in % steps, part = pair % PARTS, head = pair / PARTS;
+    const typename U::N begins = unit - step;  // the head's first unit
+    const unsigned taken = end - unit < steps - step ? (unsigned)(end - unit) : steps - step;
+    const bool entire = taken == steps;
+    unit += taken;
+    const unsigned len = units.length(lengths[b]);
+    const unsigned first = step * STEP;
+    const unsigned last = len < (step + taken) * STEP ? len : (step + taken) * STEP;
+    const unsigned tiles = (last - first + TILE - 1u) / TILE;
 
     const int* table = pages + (size_t)b * WIDTH;
-    // The page of this lane's row n of a tile (of the tile, where it lies in one).
-    const auto page_of = [&](unsigned ti) -> int {
+    // The page of row n of block `bi` of a tile (of the block, where it lies in one).
+    const auto page_of = [&](unsigned ti, unsigned bi) -> int {
+        const unsigned t0 = first + TILE * ti + 16u * bi;
         if constexpr (ONE_PAGE) {
-            return ti < tiles ? __builtin_amdgcn_readfirstlane(table[(first + 16u * ti) / PS]) : -1;
+            return t0 < last ? __builtin_amdgcn_readfirstlane(table[t0 / PS]) : -1;
         } else {
-            const unsigned at = first + 16u * ti + n;
-            return ti < tiles && at < last ? table[at / PS] : -1;
+            return t0 + n < last ? table[(t0 + n) / PS] : -1;
         }
     };
     const auto row_page = [&](int page, unsigned i) -> int { return ONE_PAGE ? page : __shfl(page, (int)(4u * g + i), 64); };
     const auto safe = [&](int page) -> unsigned { return (unsigned)page < PAGES ? (unsigned)page : 0u; };
 
-    unsigned kw[NJ][KW], vw[4][NV][VW];
-    float ks[4], vs[4];
-    const auto load_k = [&](unsigned ti, int page) {
-        const unsigned t0 = first + 16u * ti;
-        const unsigned char* p = cache + C::row(safe(page), 0u, head, (t0 + n) % PS) + g * (VK * ITEM);
+    unsigned kw[BLOCKS][NJ][KW], vw[BLOCKS][4][NV][VW];
+    float ks[BLOCKS][4], vs[BLOCKS][4];
+    const auto load_k = [&](unsigned ti, const int (&page)[BLOCKS]) {
 #pragma unroll
-        for (unsigned jj = 0; jj < NJ; ++jj) mt_ld_words<KW>(kw[jj], p + jj * (4u * VK * ITEM));
-        if constexpr (KIND != 0) {
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) {
+            const unsigned t0 = first + TILE * ti + 16u * bi;
+            const unsigned char* p = cache + C::row(safe(page[bi]), 0u, head, (t0 + n) % PS) + g * (VK * ITEM);
 #pragma unroll
-            for (unsigned i = 0; i < 4u; ++i)
-                ks[i] = *reinterpret_cast<const float*>(
-                    cache + C::scale(safe(row_page(page, i)), 0u, head, (t0 + 4u * g + i) % PS));
+            for (unsigned jj = 0; jj < NJ; ++jj) mt_ld_words<KW>(kw[bi][jj], p + jj * (4u * VK * ITEM));
+            if constexpr (!WIDE) {
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i)
+                    ks[bi][i] = *reinterpret_cast<const float*>(
+                        cache + C::scale(safe(row_page(page[bi], i)), 0u, head, (t0 + 4u * g + i) % PS));
+            }
         }
     };
-    const auto load_v = [&](unsigned ti, int page) {
-        const unsigned t0 = first + 16u * ti;
+    const auto load_v = [&](unsigned ti, const int (&page)[BLOCKS]) {
 #pragma unroll
-        for (unsigned i = 0; i < 4u; ++i) {
-            const unsigned pg = safe(row_page(page, i)), r = (t0 + 4u * g + i) % PS;
-            const unsigned char* p = cache + C::row(pg, 1u, head, r);
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) {
+            const unsigned t0 = first + TILE * ti + 16u * bi;
 #pragma unroll
-            for (unsigned c = 0; c < NV; ++c) {
-                unsigned d = VV * (16u * c + n);
-                if (D % (16u * VV) != 0u && d >= D) d = 0u;  // (columns that no output takes)
-                mt_ld_words<VW>(vw[i][c], p + d * ITEM);
+            for (unsigned i = 0; i < 4u; ++i) {
+                const unsigned pg = safe(row_page(page[bi], i)), r = (t0 + 4u * g + i) % PS;
+                const unsigned char* p = cache + C::row(pg, 1u, head, r);
+#pragma unroll
+                for (unsigned c = 0; c < NV; ++c) {
+                    unsigned d = VV * (16u * c + n);
+                    if (D % (16u * VV) != 0u && d >= D) d = 0u;  // (columns that no output takes)
+                    mt_ld_words<VW>(vw[bi][i][c], p + d * ITEM);
+                }
+                if constexpr (!WIDE) vs[bi][i] = *reinterpret_cast<const float*>(cache + C::scale(pg, 1u, head, r));
             }
-            if constexpr (KIND != 0) vs[i] = *reinterpret_cast<const float*>(cache + C::scale(pg, 1u, head, r));
         }
     };
 
-    mt_f32x4 acc[NV * VV];
+    int page[BLOCKS], page_next[BLOCKS];
 #pragma unroll
-    for (unsigned i = 0; i < NV * VV; ++i) acc[i] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    bool seen = false;
-    int page = -1, page_next = -1;
+    for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = wave < tiles ? page_of(wave, bi) : -1, page_next[bi] = -1;
     if (wave < tiles) {
-        page = page_of(wave);
         load_k(wave, page);
         load_v(wave, page);
-        page_next = page_of(wave + WAVES);
+#pragma unroll
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) page_next[bi] = page_of(wave + WAVES, bi);
     }
-    for (unsigned ti = wave; ti < tiles; ti += WAVES) {
-        const int page_after = page_of(ti + 2u * WAVES);
-        const bool more = ti + WAVES < tiles;
-        mt_f32x4 s = {0.f, 0.f, 0.f, 0.f}, s2 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (unsigned jj = 0; jj < NJ; ++jj)
-#pragma unroll
-            for (unsigned e = 0; e < VK / 4u; ++e) {
-                const mt_f32x4 k4 = mt_four<KIND, KW>(kw[jj], e);
-                s = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.x, qf[jj][e].x, s, 0, 0, 0);
-                s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.y, qf[jj][e].y, s2, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.z, qf[jj][e].z, s, 0, 0, 0);
-                s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(k4.w, qf[jj][e].w, s2, 0, 0, 0);
-            }
-        s = s + s2;
-        if constexpr (KIND != 0) {
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) s[i] *= ks[i];
-        }
-        if (more) load_k(ti + WAVES, page_next);
-        bool ok[4], any = false, all = true;
-#pragma unroll
-        for (unsigned i = 0; i < 4u; ++i) {
-            ok[i] = (unsigned)row_page(page, i) < PAGES && first + 16u * ti + 4u * g + i < last;
-            if (!ok[i]) s[i] = -INFINITY;
-            any = any || ok[i];
-            all = all && ok[i];
-        }
-        seen = seen || __any(any);
-        float top = __builtin_fmaxf(__builtin_fmaxf(s[0], s[1]), __builtin_fmaxf(s[2], s[3]));
-        top = __builtin_fmaxf(top, mt_shfl_xor(top, 16));
-        top = __builtin_fmaxf(top, mt_shfl_xor(top, 32));
-        if (__any(top > m)) {
-            const float grown = __builtin_fmaxf(m, top);
-            const float by = grown > m ? __builtin_amdgcn_exp2f(m - grown) : 1.f;
-            m = grown;
-            l *= by;
-            mt_f32x4 rows_by;
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) rows_by[i] = __shfl(by, (int)(4u * g + i), 64);
-#pragma unroll
-            for (unsigned i = 0; i < NV * VV; ++i) acc[i] = acc[i] * rows_by;
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-        float p[4];
-#pragma unroll
-        for (unsigned i = 0; i < 4u; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(s[i] - base);
-            l += p[i];
-            if constexpr (KIND != 0) p[i] *= vs[i];
-        }
-        if (!__all(all)) {
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) {
-                if (ok[i]) continue;
-                p[i] = 0.f;
-#pragma unroll
-                for (unsigned c = 0; c < NV; ++c)
-#pragma unroll
-                    for (unsigned w = 0; w < VW; ++w) vw[i][c][w] = 0u;
-            }
-        }
-#pragma unroll
-        for (unsigned i = 0; i < 4u; ++i)
-#pragma unroll
-            for (unsigned c = 0; c < NV; ++c)
-#pragma unroll
-                for (unsigned e = 0; e < VV / 4u; ++e) {
-                    const mt_f32x4 v4 = mt_four<KIND, VW>(vw[i][c], e);
-#pragma unroll
-                    for (unsigned u = 0; u < 4u; ++u)
-                        acc[VV * c + 4u * e + u] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                            p[i], v4[u], acc[VV * c + 4u * e + u], 0, 0, 0);
-                }
-        if (more) load_v(ti + WAVES, page_next);
-        page = page_next;
-        page_next = page_after;
-    }
-    l += mt_shfl_xor(l, 16);
-    l += mt_shfl_xor(l, 32);
-    if (m == -INFINITY) l = seen ? 1.f : 0.f;
 
-    // The waves' parts: [WAVES][HELD][D] sums, then [WAVES][HELD] of m and of l.  A
-    // part weighs 2^(m - the largest m); one whose scores are all -inf weighs nothing
-    // and says in l whether it has positions: a softmax over such scores alone is
-    // 0 / 0, one over no positions gives zeros.
-    float* sums = reinterpret_cast<float*>(lds);
-    float* ms = sums + WAVES * HELD * D;
-    float* ls = ms + WAVES * HELD;
-    float* by = ls + WAVES * HELD;  // [SPLITS][HELD] weights
-    unsigned* flag = reinterpret_cast<unsigned*>(by + SPLITS * HELD);
+    // q, times the scale, as the MFMAs take it: dim d is element d % VK % KO of operand
+    // (d / (4 VK), d % VK / KO) in the lanes of g = d / VK % 4; fp32 in column h, or the
+    // parts of 8 (or 4) bf16 in columns 4 h + part of the set.
+    {
+        const float by = (float)(scale * 1.4426950408889634);
+        const float* qr = q + (size_t)b * QRS;
+        for (unsigned at = threadIdx.x; at < (WIDE ? 16u : 4u * SETS) * D; at += 64u * WAVES) {
+            const unsigned h = at / D, d = at % D, op = d / (4u * VK) * NO + d % VK / KO, e = d % KO, gd = d / VK % 4u;
+            float v = 0.f;
+            if (h < HELD && part * HELD + h < SHARE) v = qr[(size_t)((head * SHARE + part * HELD + h) * D + d) * QCS] * by;
+            if constexpr (WIDE) {
+                reinterpret_cast<float*>(qs + op * 64u + gd * 16u + h)[e] = v;
+            } else {
+                unsigned short* to = reinterpret_cast<unsigned short*>(qs + (h / 4u * OPS + op) * 64u + gd * 16u + h % 4u * 4u);
 #pragma unroll
-    for (unsigned c = 0; c < NV; ++c)
-#pragma unroll
-        for (unsigned e = 0; e < VV; ++e) {
-            const unsigned d = VV * (16u * c + n) + e;
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) {
-                const unsigned h = 4u * g + i;
-                if (h < HELD && (D % (16u * VV) == 0u || d < D)) sums[(wave * HELD + h) * D + d] = acc[VV * c + e][i];
+                for (unsigned j = 0; j < 4u; ++j) to[8u * j + e] = (unsigned short)(__float_as_uint(mt_bf16_part(v, j)) >> 16);
             }
         }
-    if (g == 0u && n < HELD) {
-        ms[wave * HELD + n] = m;
-        ls[wave * HELD + n] = l;
     }
     __syncthreads();
 
-    float* mine = nullptr;
-    if (active > 1u) mine = ws + MT_WS_HEAD + (((size_t)blockIdx.z * (rows * HK * PARTS) + pair) * SPLITS + split) * FLOATS;
+    mt_f32x4 acc[SETS][NV * VV];
+    float m[SETS], l[SETS];
+#pragma unroll
+    for (unsigned t = 0; t < SETS; ++t) {
+        m[t] = -INFINITY, l[t] = 0.f;
+#pragma unroll
+        for (unsigned i = 0; i < NV * VV; ++i) acc[t][i] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    bool seen = false;
+    for (unsigned ti = wave; ti < tiles; ti += WAVES) {
+        int page_after[BLOCKS];
+#pragma unroll
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) page_after[bi] = page_of(ti + 2u * WAVES, bi);
+        const bool more = ti + WAVES < tiles;
+        mt_f32x4 s[SETS][BLOCKS];
+#pragma unroll
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) {
+            if constexpr (WIDE) {
+                mt_f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (unsigned jj = 0; jj < NJ; ++jj) {
+                    const mt_f32x4 qv = __builtin_bit_cast(mt_f32x4, qs[jj * 64u + lane]);
+#pragma unroll
+                    for (unsigned e = 0; e < 4u; e += 2u) {
+                        s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[bi][jj][e]), qv[e], s0, 0, 0, 0);
+                        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[bi][jj][e + 1u]), qv[e + 1u], s1, 0, 0, 0);
+                    }
+                }
+                s[0][bi] = s0 + s1;
+            } else {
+#pragma unroll
+                for (unsigned t = 0; t < SETS; ++t) s[t][bi] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (unsigned jj = 0; jj < NJ; ++jj)
+#pragma unroll
+                    for (unsigned e = 0; e < NO; ++e) {
+                        if constexpr (KO == 8u) {
+                            const mt_u32x2 lo = mt_held4_bf16<KIND>(kw[bi][jj][2u * e]);
+                            const mt_u32x2 hi = mt_held4_bf16<KIND>(kw[bi][jj][2u * e + 1u]);
+                            const mt_u32x4 k8 = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                            for (unsigned t = 0; t < SETS; ++t)
+                                s[t][bi] = mt_mfma16_bf16(k8, qs[(t * OPS + jj * NO + e) * 64u + lane], s[t][bi]);
+                        } else {
+                            const mt_u32x2 k4 = mt_held4_bf16<KIND>(kw[bi][jj][e]);
+#pragma unroll
+                            for (unsigned t = 0; t < SETS; ++t) {
+                                const mt_u32x2 o4 = qs[(t * OPS + jj * NO + e) * 64u + lane].xy;
+                                s[t][bi] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+                                    __builtin_bit_cast(mt_i16x4, k4), __builtin_bit_cast(mt_i16x4, o4), s[t][bi], 0, 0, 0);
+                            }
+                        }
+                    }
+#pragma unroll
+                for (unsigned t = 0; t < SETS; ++t)
+#pragma unroll
+                    for (unsigned i = 0; i < 4u; ++i) {  // the parts of q together
+                        float v = s[t][bi][i];
+                        v += mt_xor_lanes<1u>(v);
+                        v += mt_xor_lanes<2u>(v);
+                        s[t][bi][i] = v * ks[bi][i];
+                    }
+            }
+        }
+        if (more) load_k(ti + WAVES, page_next);
+        bool ok[BLOCKS][4], any = false, all = true;
+#pragma unroll
+        for (unsigned bi = 0; bi < BLOCKS; ++bi)
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i) {
+                ok[bi][i] = (unsigned)row_page(page[bi], i) < PAGES && first + TILE * ti + 16u * bi + 4u * g + i < last;
+                any = any || ok[bi][i];
+                all = all && ok[bi][i];
+            }
+        seen = seen || __any(any);
+        const bool whole = __all(all);
+        if (!whole) {
+#pragma unroll
+            for (unsigned bi = 0; bi < BLOCKS; ++bi)
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i)
+#pragma unroll
+                    for (unsigned t = 0; t < SETS; ++t)
+                        if (!ok[bi][i]) s[t][bi][i] = -INFINITY;
+        }
+        float p[SETS][BLOCKS][4];
+#pragma unroll
+        for (unsigned t = 0; t < SETS; ++t) {
+            float top = -INFINITY;
+#pragma unroll
+            for (unsigned bi = 0; bi < BLOCKS; ++bi)
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i) top = __builtin_fmaxf(top, s[t][bi][i]);
+            top = mt_fold_g(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+            if (__any(top > m[t])) {
+                const float grown = __builtin_fmaxf(m[t], top);
+                const float by = grown > m[t] ? __builtin_amdgcn_exp2f(m[t] - grown) : 1.f;
+                m[t] = grown;
+                l[t] *= by;
+                if constexpr (WIDE) {
+                    mt_f32x4 rows_by;
+#pragma unroll
+                    for (unsigned i = 0; i < 4u; ++i) rows_by[i] = __shfl(by, (int)(4u * g + i), 64);
+#pragma unroll
+                    for (unsigned i = 0; i < NV * VV; ++i) acc[t][i] = acc[t][i] * rows_by;
+                } else {
+                    const float row_by = __shfl(by, (int)(4u * g), 64);
+#pragma unroll
+                    for (unsigned i = 0; i < NV * VV; ++i) acc[t][i] = acc[t][i] * row_by;
+                }
+            }
+            const float base = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+            for (unsigned bi = 0; bi < BLOCKS; ++bi)
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(s[t][bi][i] - base);
+                    l[t] += e;
+                    p[t][bi][i] = WIDE ? e : e * vs[bi][i];
+                }
+        }
+        if (!whole) {
+#pragma unroll
+            for (unsigned bi = 0; bi < BLOCKS; ++bi)
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i) {
+                    if (ok[bi][i]) continue;
+#pragma unroll
+                    for (unsigned t = 0; t < SETS; ++t) p[t][bi][i] = 0.f;
+#pragma unroll
+                    for (unsigned c = 0; c < NV; ++c)
+#pragma unroll
+                        for (unsigned w = 0; w < VW; ++w) vw[bi][i][c][w] = 0u;
+                }
+        }
+        if constexpr (WIDE) {
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i)
+#pragma unroll
+                for (unsigned c = 0; c < NV; ++c)
+#pragma unroll
+                    for (unsigned e = 0; e < VV; ++e)
+                        acc[0][VV * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][0][i], __uint_as_float(vw[0][i][c][e]),
+                                                                                  acc[0][VV * c + e], 0, 0, 0);
+        } else {
+            mt_u32x4 pb[SETS];
+#pragma unroll
+            for (unsigned t = 0; t < SETS; ++t)
+#pragma unroll
+                for (unsigned bi = 0; bi < 2u; ++bi) {
+                    float f[4];
+#pragma unroll
+                    for (unsigned i = 0; i < 4u; ++i) f[i] = mt_bf16_part(p[t][bi % BLOCKS][i], n & 3u);
+                    pb[t][2u * bi] = mt_bf16_pair(f[0], f[1]);
+                    pb[t][2u * bi + 1u] = mt_bf16_pair(f[2], f[3]);
+                }
+#pragma unroll
+            for (unsigned c = 0; c < NV; ++c)
+#pragma unroll
+                for (unsigned w = 0; w < VW; ++w) {
+                    unsigned lo[4], hi[4];
+                    mt_bytes4(vw[0][0][c][w], vw[0][1][c][w], vw[0][2][c][w], vw[0][3][c][w], lo);
+                    mt_bytes4(vw[BLOCKS - 1u][0][c][w], vw[BLOCKS - 1u][1][c][w], vw[BLOCKS - 1u][2][c][w],
+                              vw[BLOCKS - 1u][3][c][w], hi);
+#pragma unroll
+                    for (unsigned u = 0; u < 4u; ++u) {
+                        const mt_u32x2 v0 = mt_held4_bf16<KIND>(lo[u]), v1 = mt_held4_bf16<KIND>(hi[u]);
+                        const mt_u32x4 v8 = {v0.x, v0.y, v1.x, v1.y};
+#pragma unroll
+                        for (unsigned t = 0; t < SETS; ++t)
+                            acc[t][VV * c + 4u * w + u] = mt_mfma16_bf16(pb[t], v8, acc[t][VV * c + 4u * w + u]);
+                    }
+                }
+        }
+        if (more) load_v(ti + WAVES, page_next);
+#pragma unroll
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = page_next[bi], page_next[bi] = page_after[bi];
+    }
+
+    // A part weighs 2^(m - the largest m); one whose scores are all -inf weighs nothing
+    // and says in l whether it has positions: a softmax over such scores alone is 0 / 0,
+    // one over no positions gives zeros.
+#pragma unroll
+    for (unsigned t = 0; t < SETS; ++t) {
+        l[t] = mt_fold_g(l[t], [](float x, float y) { return x + y; });
+        if (m[t] == -INFINITY) l[t] = seen ? 1.f : 0.f;
+        const unsigned h = WIDE ? n : 4u * t + (n >> 2);
+        if (g == 0u && h < HELD && (WIDE || (n & 3u) == 0u)) {
+            ms[wave * HELD + h] = m[t];
+            ls[wave * HELD + h] = l[t];
+        }
+#pragma unroll
+        for (unsigned c = 0; c < NV; ++c)
+#pragma unroll
+            for (unsigned e = 0; e < VV; ++e) {
+                const unsigned d = VV * (16u * c + n) + e;
+                if (D % (16u * VV) != 0u && d >= D) continue;
+                const mt_f32x4 a = acc[t][VV * c + e];
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (unsigned i = 0; i < 4u; ++i)
+                        if (4u * g + i < HELD) sums[(wave * HELD + 4u * g + i) * D + d] = a[i];
+                } else {
+                    if (4u * t + g < HELD) sums[(wave * HELD + 4u * t + g) * D + d] = a[0] + a[1] + a[2];
+                }
+            }
+    }
+    __syncthreads();
+
+    // Slot 2 w of the workspace is the part of workgroup w that began before it, 2 w + 1
+    // the part that begins in it.
+    float* slots = ws + MT_WS_HEAD + (size_t)blockIdx.z * gridDim.x * 2u * FLOATS;
+    float* mine = slots + (size_t)(2u * blockIdx.x + (step == 0u ? 1u : 0u)) * FLOATS;
     for (unsigned at = threadIdx.x; at < HELD * D; at += 64u * WAVES) {
         const unsigned h = at / D, d = at % D;
         float top = -INFINITY, empty = 0.f, total = 0.f, value = 0.f;
@@ -645,58 +900,71 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         for (unsigned w = 0; w < WAVES; ++w) top = __builtin_fmaxf(top, ms[w * HELD + h]);
 #pragma unroll
         for (unsigned w = 0; w < WAVES; ++w) {
-            const float mw = ms[w * HELD + h], lw = ls[w * HELD + h];
-            if (mw == -INFINITY) {
-                empty += lw;
-                continue;
-            }
+            const float mw = ms[w * HELD + h], lw = ls[w * HELD + h], v = sums[(w * HELD + h) * D + d];
+            const bool none = mw == -INFINITY;
             const float u = __builtin_amdgcn_exp2f(mw - top);
-            total += u * lw;
-            value += u * sums[(w * HELD + h) * D + d];
+            empty += none ? lw : 0.f;
+            total += none ? 0.f : u * lw;
+            value += none ? 0.f : u * v;
         }
         if (top == -INFINITY) total = empty;
-        if (active > 1u) {
+        if (!entire) {
             mt_sn_put(mine + at, value);
             if (d == 0u) {
                 mt_sn_put(mine + HELD * D + h, top);
                 mt_sn_put(mine + HELD * D + HELD + h, total);
             }
-        } else if (part * 16u + h < SHARE) {
+        } else if (part * HELD + h < SHARE) {
             const float r = top == -INFINITY ? (total > 0.f ? NAN : 0.f) : value / total;
-            o[((size_t)b * HK * SHARE + head * SHARE + part * 16u + h) * D + d] = r;
+            o[((size_t)b * HK * SHARE + head * SHARE + part * HELD + h) * D + d] = r;
         }
     }
-    if (active <= 1u) return;
+    if (entire) {
+        __syncthreads();  // (the next unit's waves write where this one's are read)
+        continue;
+    }
 
-    // The last workgroup of the sequence's head joins the parts: maxima into `by`,
-    // sums of weights into `sums` (at most 64 parts, which is no more than WAVES * D).
-    unsigned* counter = reinterpret_cast<unsigned*>(ws) + blockIdx.z * (rows * HK * PARTS) + pair;
-    if (!mt_sn_arrive(counter, active, flag)) return;
-    const float* all = mine - (size_t)split * FLOATS;
-    for (unsigned at = threadIdx.x; at < HELD * active; at += 64u * WAVES) {
-        const unsigned s = at / HELD, h = at % HELD;
-        by[at] = mt_sn_get(all + (size_t)s * FLOATS + HELD * D + h);
-        sums[at] = mt_sn_get(all + (size_t)s * FLOATS + HELD * D + HELD + h);
+    // The last workgroup of the sequence's head to arrive joins the parts.
+    const unsigned from = units.owner(begins), active = units.owner(begins + steps - 1u) - from + 1u;
+    unsigned* counter = reinterpret_cast<unsigned*>(ws) + blockIdx.z * gridDim.x + from;
+    if (mt_sn_arrive(counter, active, flag)) {
+        const auto slot = [&](unsigned i) { return slots + (size_t)(2u * (from + i) + (i == 0u ? 1u : 0u)) * FLOATS; };
+        for (unsigned at = threadIdx.x; at < HELD * D; at += 64u * WAVES) {
+            const unsigned h = at / D, d = at % D;
+            float top = -INFINITY, empty = 0.f, total = 0.f, value = 0.f;
+            for (unsigned i0 = 0; i0 < active; i0 += 16u) {  // 16 parts' loads at a time, one latency
+                float pm[16], pl[16], pv[16], most = top;
+#pragma unroll
+                for (unsigned k = 0; k < 16u; ++k) {
+                    const float* p = slot(i0 + k < active ? i0 + k : i0);
+                    pm[k] = mt_sn_get(p + HELD * D + h);
+                    pl[k] = mt_sn_get(p + HELD * D + HELD + h);
+                    pv[k] = mt_sn_get(p + at);
+                }
+#pragma unroll
+                for (unsigned k = 0; k < 16u; ++k) most = __builtin_fmaxf(most, pm[k]);
+                if (most > top) {
+                    const float by = __builtin_amdgcn_exp2f(top - most);
+                    total *= by, value *= by;
+                    top = most;
+                }
+#pragma unroll
+                for (unsigned k = 0; k < 16u; ++k) {
+                    if (i0 + k >= active) continue;
+                    const bool none = pm[k] == -INFINITY;
+                    const float u = none ? 0.f : __builtin_amdgcn_exp2f(pm[k] - top);
+                    empty += none ? pl[k] : 0.f;
+                    total += none ? 0.f : u * pl[k];
+                    value += none ? 0.f : u * pv[k];
+                }
+            }
+            if (part * HELD + h < SHARE) {
+                const float r = top == -INFINITY ? (empty > 0.f ? NAN : 0.f) : value / total;
+                o[((size_t)b * HK * SHARE + head * SHARE + part * HELD + h) * D + d] = r;
+            }
+        }
     }
     __syncthreads();
-    for (unsigned at = threadIdx.x; at < HELD * D; at += 64u * WAVES) {
-        const unsigned h = at / D, d = at % D;
-        float top = -INFINITY, empty = 0.f, total = 0.f, value = 0.f;
-        for (unsigned s = 0; s < active; ++s) top = __builtin_fmaxf(top, by[s * HELD + h]);
-#pragma unroll 8
-        for (unsigned s = 0; s < active; ++s) {
-            const float v = mt_sn_get(all + (size_t)s * FLOATS + at);
-            const float mw = by[s * HELD + h], lw = sums[s * HELD + h];
-            const bool none = mw == -INFINITY;
-            const float u = none ? 0.f : __builtin_amdgcn_exp2f(mw - top);
-            empty += none ? lw : 0.f;
-            total += none ? 0.f : u * lw;
-            value += none ? 0.f : u * v;
-        }
-        if (part * 16u + h < SHARE) {
-            const float r = top == -INFINITY ? (empty > 0.f ? NAN : 0.f) : value / total;
-            o[((size_t)b * HK * SHARE + head * SHARE + part * 16u + h) * D + d] = r;
-        }
     }
 }
 
@@ -723,16 +991,6 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 // and split k, so that few rows of weights still keep many loads in flight; each
 // makes the digits of its own part of k (LDS of its own, no barrier).
 // ---------------------------------------------------------------------------
-
-// Byte i of a, b, c, d together in to[i].
-MT_INLINE void mt_bytes4(unsigned a, unsigned b, unsigned c, unsigned d, unsigned (&to)[4]) {
-    const unsigned ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
-    const unsigned cd0 = __builtin_amdgcn_perm(d, c, 0x05010400u), cd1 = __builtin_amdgcn_perm(d, c, 0x07030602u);
-    to[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u);
-    to[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
-    to[2] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u);
-    to[3] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
-}
 
 // The whole number that an MFMA's four digit rows stand for.
 MT_INLINE float mt_digits(mt_i32x4 c) {

@@ -188,45 +188,48 @@ def _assemble_cache_read(decision: DecisionView, op: CacheReadOp, function_name:
 # attention
 # ---------------------------------------------------------------------------
 
-ATTENTION_WAVES = 4
-ATTENTION_SPLITS = 64  # at most, for the workgroup that joins them
-ATTENTION_GROUPS = 1024  # workgroups aimed at
-ATTENTION_MIN_BYTES = 65536  # of keys and values for a workgroup at least
+ATTENTION_WAVES = 8
+ATTENTION_WORKGROUPS = 256  # at most; the device cuts the work into as many equal ranges
 
 
-def attention_splits(pairs: int, capacity: int, position_bytes: int) -> tuple[int, int]:
-    """(splits, positions of each) of a sequence's length, for ``pairs`` sequences
-    times key heads."""
-    least = max(16 * ATTENTION_WAVES, _ceil(ATTENTION_MIN_BYTES, position_bytes))
-    splits = max(1, min(ATTENTION_SPLITS, _ceil(ATTENTION_GROUPS, pairs), capacity // least))
-    if pairs >= 1023:  # a counter each is all the workspace's head has room for
-        splits = 1
-    each = _ceil(_ceil(capacity, splits), 16 * ATTENTION_WAVES) * 16 * ATTENTION_WAVES
-    return _ceil(capacity, each), each
+def attention_workgroups(pairs: int, capacity: int, step: int, batch: int) -> int:
+    """Workgroups of a launch: one for each unit of ``step`` positions of a sequence
+    (``pairs`` of them, times key heads) that there is room for, as many as fit on the
+    GPU at once, and a counter each in the workspace's head for all of a batch."""
+    return max(1, min(ATTENTION_WORKGROUPS, pairs * _ceil(capacity, step), (WS_HEAD_BYTES // 4 - 1) // batch))
 
 
 def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_name: str | None, batch: int) -> KernelGroup:
     spec, rows = op.spec, op.q.shape[0]
     share = op.heads // spec.kv_heads  # query heads of a key head
-    parts = _ceil(share, 16)  # of at most 16 query heads, one matrix instruction's columns
-    held = min(share, 16)
+    # At most 16 query heads at once, one fp32 MFMA's columns; 8 where 16 long rows would
+    # not fit in a wave's registers (four sets of bf16 columns) or in LDS.
+    held = min(share, 16 if spec.dim <= 128 else 8)
+    parts = _ceil(share, held)
     pairs = rows * spec.kv_heads * parts
-    splits, each = attention_splits(pairs * batch, op.capacity, 2 * spec.dim * spec.item_bytes)
+    waves = ATTENTION_WAVES
+    step = (16 if spec.dtype == "float32" else 32) * waves
+    groups = attention_workgroups(pairs, op.capacity, step, batch)
     floats = held * (spec.dim + 2)
-    ws = WS_HEAD_BYTES + 4 * batch * pairs * splits * floats if splits > 1 else 0
+    # q's operands in LDS: 16 bytes a lane for 16 dims of fp32 columns, or for 32 (16) of bf16 sets
+    if spec.dtype == "float32":
+        q_bytes = 1024 * (spec.dim // 16)
+    else:
+        q_bytes = 1024 * _ceil(held, 4) * (spec.dim // (32 if spec.dim % 32 == 0 else 16))
+    ws = WS_HEAD_BYTES + 4 * batch * groups * 2 * floats if groups > 1 else 0
     sig = _Signature()
     args = (sig.add("q", op.q), sig.add("cache", op.cache), sig.add("pages", op.pages), sig.add("lengths", op.lengths),
-            sig.add("o", op.o, out=True), f"{op.scale!r}", "mt_ws" if ws else "nullptr", "M", "mt_lds")
+            sig.add("o", op.o, out=True), f"{op.scale!r}", "mt_ws" if ws else "nullptr", "mt_lds")
     frag = ServingFragment(
         "mt_paged_attention",
-        (*_cache_template(spec), spec.pages, op.pages.shape[1], share, ATTENTION_WAVES, splits, each, batch,
+        (*_cache_template(spec), spec.pages, op.pages.shape[1], share, held, waves, groups, batch, rows,
          op.q.row_stride, op.q.col_stride),
         args,
-        lds_bytes=4 * ATTENTION_WAVES * floats + 4 * held * splits + 16,
+        lds_bytes=q_bytes + 4 * waves * floats + 16,
         name="paged_attention",
     )
     return _group(decision, sig, frag, function_name or f"paged_attention_{op.o.name}", {"M": rows},
-                  (pairs * splits, 1, 1), 64 * ATTENTION_WAVES, workspace_bytes=ws, workspace_batched=True,
+                  (groups, 1, 1), 64 * waves, workspace_bytes=ws, workspace_batched=True,
                   workspace_waits=False)
 
 

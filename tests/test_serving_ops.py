@@ -11,7 +11,7 @@ from metellus_amd.api import compile_program
 from metellus_amd.compute.fragments import CodegenEngine
 from metellus_amd.orchestrator import KVCache, Operations
 from metellus_amd.orchestrator.assembly.serving import (
-    attention_splits,
+    attention_workgroups,
     cache_write_tokens,
     int4_shape,
     norm_lanes,
@@ -366,10 +366,9 @@ def test_launch_rules_stay_within_what_the_kernels_take():
             assert norm_lanes(rows, cols) in (64, 256, 1024)
     for pairs in (1, 8, 256, 1022, 1023, 5000):
         for capacity in (1, 16, 100, 2048, 131072, 2**31 - 2048):
-            for nbytes in (32, 256, 2048):
-                splits, each = attention_splits(pairs, capacity, nbytes)
-                assert each % 64 == 0 and splits * each >= capacity > (splits - 1) * each and 1 <= splits <= 64
-                assert splits == 1 or pairs < 1023
+            for batch in (1, 3, 32, 1023, 5000):
+                groups = attention_workgroups(pairs, capacity, 128, batch)
+                assert 1 <= groups <= pairs * -(-capacity // 128) and (groups == 1 or groups * batch <= 1023)
     for tokens in (1, 5, 1024, 100000):
         for heads in (1, 8, 64):
             assert 1 <= cache_write_tokens(tokens, heads) <= 32
