@@ -977,19 +977,23 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 // X = 2^24 d3 + 2^16 d2 + 2^8 d1 + d0 with digits of 8 bits.  The digits of 4
 // rows of x are the 16 rows of an MFMA 16x16x64; 16 weight rows are its columns.
 // What is lost is 2^-30 of the block's largest value per element; a block that
-// holds an infinity or a NaN is summed in fp32 as the formula says.  x in 8 bits
-// is 16 rows as it stands.
+// holds an infinity or a NaN counts as zeros there and is added in fp32, as the
+// formula says, at the end.  One or two rows of x (XR) make the digits of four or two
+// blocks at once instead.  x in 8 bits is 16 rows as it stands.
 //
-// A lane's 16 bytes of weights are q of 32 consecutive k, even ones in the low
-// nibbles: xor 0x88 turns q into q - 8 in two's complement, and in the high
-// nibble of a byte that is 16 (q - 8) as int8, so w & 0xF0.. are the odd k and
-// (w << 4) & 0xF0.. the even k: two MFMAs, with x's digits in the same order.  A
-// block of 128 k is four lanes' pieces of a row; with groups of 32 or 64 the
-// pieces of the other groups are zeroed in x.
+// With (n, g) = (lane % 16, lane / 16): lane (n, g) loads 16 bytes of weight row n, q of
+// k = 32 g .. + 31 of a block of 128, even ones in the low nibbles.  xor 0x88 turns q
+// into q - 8 in two's complement, and in the high nibble of a byte that is 16 (q - 8)
+// as int8: (v << 4) & 0xF0.. are a word's four even k, v & 0xF0.. its odd ones, and
+// those two words in turn are the operand, in weights and digits alike.  Groups of 64
+// or 32: the words of a group are spread over all g first, by exchanges of halves and
+// rows of the wave (permlane swaps: 2 or 4 for 32 k a lane), so that an MFMA takes
+// one group whole.
 //
-// Bound: HBM, the weights once.  The waves of a workgroup share its weight rows
-// and split k, so that few rows of weights still keep many loads in flight; each
-// makes the digits of its own part of k (LDS of its own, no barrier).
+// Bound: HBM, the weights once.  SHARED: the digits of all of x stay in LDS and every
+// wave takes weight tiles of its own, row after row; otherwise the waves of a
+// workgroup share its weight rows and split k, each making the digits of its part as
+// it goes, so that few weight rows still keep many loads in flight.
 // ---------------------------------------------------------------------------
 
 // The whole number that an MFMA's four digit rows stand for.
@@ -998,226 +1002,384 @@ MT_INLINE float mt_digits(mt_i32x4 c) {
     return __builtin_fmaf((float)hi, 65536.0f, (float)lo);
 }
 
-template <bool EIGHT, unsigned SETS, unsigned K, unsigned N, unsigned GROUP, bool ZEROS, unsigned R, unsigned WAVES,
-          unsigned XRS, unsigned XCS>
+// The largest of a value's bits over 16 lanes (DPP: quads, halves, rows mirrored).
+MT_INLINE unsigned mt_max16(unsigned v) {
+    const auto step = [&](unsigned other) { v = v > other ? v : other; };
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+    step((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+    return v;
+}
+
+// a's upper half of the wave for b's lower half; a's odd rows of 16 for b's even ones.
+MT_INLINE void mt_swap32(unsigned& a, unsigned& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0], b = r[1];
+}
+MT_INLINE void mt_swap16(unsigned& a, unsigned& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0], b = r[1];
+}
+
+// What one MFMA of a block takes: 16 bytes a lane of 64 k, or 8 of 32.  A block is two
+// of the first kind (both of one group of 128, or one of each group of 64), or four.
+template <unsigned GB>
+struct mt_operand {
+    static constexpr unsigned COUNT = GB == 4u ? 4u : 2u, WORDS = GB == 4u ? 2u : 4u;
+    // Where in a row's 128 bytes of a block, in digits (the even and the odd k of 8 in turn).
+    MT_INLINE static unsigned at(unsigned i, unsigned g) {
+        return GB == 1u ? 32u * g + 16u * i : GB == 2u ? 64u * i + 32u * (g % 2u) + 16u * (g / 2u) : 32u * i + 8u * g;
+    }
+    // This lane's words of weights, k 32 g .. + 31, so that words WORDS / 2 * i .. make operand i.
+    MT_INLINE static void spread(unsigned (&w)[4]) {
+        if constexpr (GB > 1u) {
+            mt_swap32(w[0], w[2]);
+            mt_swap32(w[1], w[3]);
+        }
+        if constexpr (GB == 4u) {
+            mt_swap16(w[0], w[1]);
+            mt_swap16(w[2], w[3]);
+        }
+    }
+    MT_INLINE static mt_i32x4 product(const unsigned (&a)[WORDS], const unsigned (&b)[WORDS], mt_i32x4 c) {
+        if constexpr (GB == 4u) {
+            return __builtin_amdgcn_mfma_i32_16x16x32_i8((long)(((unsigned long long)a[1] << 32) | a[0]),
+                                                         (long)(((unsigned long long)b[1] << 32) | b[0]), c, 0, 0, 0);
+        } else {
+            return __builtin_amdgcn_mfma_i32_16x16x64_i8(mt_i32x4{(int)a[0], (int)a[1], (int)a[2], (int)a[3]},
+                                                         mt_i32x4{(int)b[0], (int)b[1], (int)b[2], (int)b[3]}, c, 0, 0, 0);
+        }
+    }
+};
+
+template <bool EIGHT, bool SHARED, unsigned XR, unsigned SETS, unsigned K, unsigned N, unsigned GROUP, bool ZEROS, unsigned R,
+          unsigned U, unsigned WAVES, unsigned XRS, unsigned XCS>
 MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float* xs, const unsigned char* w,
                               const float* scales, const float* zeros, float* y, unsigned rows, unsigned char* lds) {
-    constexpr unsigned NB = (K + 127u) / 128u, NG = K / GROUP, GB = 128u / GROUP, ACC = EIGHT ? 4u : SETS;
-    constexpr bool RAGGED = K % 128u != 0u;
+    constexpr unsigned NB = (K + 127u) / 128u, NG = K / GROUP, GB = 128u / GROUP, GU = GB * U, ACC = EIGHT ? 4u : SETS;
+    constexpr unsigned NC = (NB + U - 1u) / U;        // chunks of U blocks, whose loads are in flight together
+    constexpr unsigned BL = EIGHT ? 1u : 4u / XR;     // blocks of x made into digits at once
+    constexpr unsigned DIGITS = 512u * XR * SETS;     // bytes of a block's digits: [SETS][4 XR rows][128]
+    constexpr bool RAGGED = K % (128u * U) != 0u;
+    using OP = mt_operand<GB>;
     const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
-    const unsigned n0 = blockIdx.x * (16u * R), m0 = blockIdx.y * 16u;
-    const unsigned b0 = NB * wave / WAVES, b1 = NB * (wave + 1u) / WAVES;
+    const unsigned m0 = blockIdx.y * 16u;
+    const unsigned c0 = SHARED ? 0u : NC * wave / WAVES, c1 = SHARED ? NC : NC * (wave + 1u) / WAVES;
 
-    const unsigned char* wr[R];
-    size_t sr[R];
+    // x for one making of digits: rows 4 t + g % XR of block blk + g / XR, k 8 n .. + 7; x
+    // in 8 bits: row n's share of the operands of block blk.
+    constexpr unsigned XV = EIGHT ? 2u : 2u * SETS;
+    const auto load_x = [&](unsigned blk, mt_u32x4 (&to)[XV]) {
+        if constexpr (EIGHT) {
+            const signed char* row = x8 + (size_t)(m0 + n < rows ? m0 + n : m0) * K;
 #pragma unroll
-    for (unsigned r = 0; r < R; ++r) {
-        const unsigned row = n0 + 16u * r + n < N ? n0 + 16u * r + n : N - 1u;
-        wr[r] = w + (size_t)row * (K / 2u) + 16u * g;
-        sr[r] = (size_t)row * NG;
-    }
-    struct block {
-        mt_u32x4 q[R];
-        float s[R][GB], z[R][ZEROS ? GB : 1u];
-        mt_f32x4 f[EIGHT ? 1u : SETS][2];  // x: rows 4 t + g, k 8 n .. + 7
-        mt_u32x4 e[EIGHT ? 2u : 1u];       // x in 8 bits: row n, k 32 g .. + 31
+            for (unsigned i = 0; i < OP::COUNT; ++i) {
+                const unsigned k = blk * 128u + OP::at(i, g);
+                const bool in = m0 + n < rows && (!RAGGED || k < K);
+                if constexpr (GB == 4u) {
+                    mt_u32x2 v = {0u, 0u};
+                    if (in) v = *reinterpret_cast<const mt_u32x2*>(row + k);
+                    to[i / 2u][2u * (i % 2u)] = v.x, to[i / 2u][2u * (i % 2u) + 1u] = v.y;
+                } else {
+                    to[i] = mt_u32x4{0u, 0u, 0u, 0u};
+                    if (in) to[i] = *reinterpret_cast<const mt_u32x4*>(row + k);
+                }
+            }
+        } else {
+#pragma unroll
+            for (unsigned t = 0; t < SETS; ++t) {
+                to[2u * t] = to[2u * t + 1u] = mt_u32x4{0u, 0u, 0u, 0u};
+                const unsigned row = m0 + 4u * t + g % XR, k = (blk + g / XR) * 128u + 8u * n;
+                if (row < rows && k < K) {
+                    to[2u * t] = __builtin_bit_cast(mt_u32x4, mt_row4<K, XCS>(x + (size_t)row * XRS, k));
+                    to[2u * t + 1u] = __builtin_bit_cast(mt_u32x4, mt_row4<K, XCS>(x + (size_t)row * XRS, k + 4u));
+                }
+            }
+        }
     };
-    const auto load = [&](unsigned blk, block& to) {
-        const bool in = !RAGGED || blk * 128u + 32u * g < K;
+    // Row r's 16 bytes c of a block's digits stand at c ^ (r / 2 % 8): the 16 rows that a
+    // quarter of a wave reads lie in different banks.
+    const auto place = [](unsigned r, unsigned byte) { return 128u * r + (byte ^ (16u * (r / 2u % 8u))); };
+    // The digits of BL blocks to `to`, and E of this lane group's row and block (255: not finite).
+    const auto make_digits = [&](const mt_u32x4 (&xv)[XV], unsigned char* to, int (&made)[SETS]) {
+#pragma unroll
+        for (unsigned t = 0; t < SETS; ++t) {
+            unsigned top = 0u;  // the bits of |x| order as the values do, infinities and NaN last
+            unsigned d[8];
+#pragma unroll
+            for (unsigned j = 0; j < 8u; ++j) {
+                d[j] = xv[EIGHT ? 0u : 2u * t + j / 4u][j % 4u];
+                const unsigned a = d[j] & 0x7FFFFFFFu;
+                top = top > a ? top : a;
+            }
+            const int e = (int)(mt_max16(top) >> 23);
+            made[t] = e < 1 ? 1 : e;
+#pragma unroll
+            for (unsigned j = 0; j < 8u; ++j) {
+                const int whole = e == 255 ? 0 : (int)__builtin_ldexpf(__uint_as_float(d[j]), 156 - made[t]);
+                d[j] = ((unsigned)whole + 0x00808080u) ^ 0x00808080u;
+            }
+            unsigned ev[4], od[4];
+            mt_bytes4(d[0], d[2], d[4], d[6], ev);
+            mt_bytes4(d[1], d[3], d[5], d[7], od);
+            unsigned char* block = to + (g / XR) * DIGITS + t * (512u * XR);
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i)
+                *reinterpret_cast<mt_u32x2*>(block + place(4u * (g % XR) + i, 8u * n)) = mt_u32x2{ev[3u - i], od[3u - i]};
+        }
+    };
+
+    bool special = false;
+    int* es = reinterpret_cast<int*>(lds + (SHARED ? (NB + BL - 1u) / BL * BL * DIGITS : 0u));  // SHARED: E, [blocks][SETS][4]
+    if constexpr (SHARED) {
+        for (unsigned blk = wave * BL; blk < NB; blk += WAVES * BL) {
+            mt_u32x4 xv[XV];
+            int made[SETS];
+            load_x(blk, xv);
+            make_digits(xv, lds + blk * DIGITS, made);
+#pragma unroll
+            for (unsigned t = 0; t < SETS; ++t) {
+                special = special || made[t] == 255;
+                if (n == 0u) es[((blk + g / XR) * SETS + t) * 4u + g % XR] = made[t];
+            }
+        }
+        special = __syncthreads_or(special);
+    }
+
+    constexpr unsigned TILES = (N + 16u * R - 1u) / (16u * R);
+    for (unsigned tile = SHARED ? blockIdx.x * WAVES + wave : blockIdx.x; tile < TILES;
+         tile += SHARED ? gridDim.x * WAVES : gridDim.x) {
+        const unsigned n0 = tile * (16u * R);
+        const unsigned char* wr[R];
+        size_t sr[R];
 #pragma unroll
         for (unsigned r = 0; r < R; ++r) {
-            to.q[r] = mt_u32x4{0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};
-            if (in) to.q[r] = __builtin_nontemporal_load(reinterpret_cast<const mt_u32x4*>(wr[r] + (size_t)blk * 64u));
-#pragma unroll
-            for (unsigned j = 0; j < GB; ++j) {
-                const unsigned gr = blk * GB + j;
-                to.s[r][j] = !RAGGED || gr < NG ? scales[sr[r] + gr] : 0.f;
-                if constexpr (ZEROS) to.z[r][j] = !RAGGED || gr < NG ? zeros[sr[r] + gr] : 0.f;
-            }
+            const unsigned row = n0 + 16u * r + n < N ? n0 + 16u * r + n : N - 1u;
+            wr[r] = w + (size_t)row * (K / 2u) + 16u * g;
+            sr[r] = (size_t)row * NG;
         }
-        if constexpr (EIGHT) {
-            to.e[0] = to.e[1] = mt_u32x4{0u, 0u, 0u, 0u};
-            if (in && m0 + n < rows) {
-                const mt_u32x4* p = reinterpret_cast<const mt_u32x4*>(x8 + (size_t)(m0 + n) * K + blk * 128u + 32u * g);
-                to.e[0] = p[0];
-                to.e[1] = p[1];
-            }
-        } else {
+        const auto load_w = [&](unsigned c, mt_u32x4 (&q)[U][R], float (&s)[R][GU], float (&z)[R][ZEROS ? GU : 1u]) {
 #pragma unroll
-            for (unsigned t = 0; t < SETS; ++t) {
-                to.f[t][0] = to.f[t][1] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-                const unsigned row = m0 + 4u * t + g, k = blk * 128u + 8u * n;
-                if (row < rows && (!RAGGED || k < K)) {
-                    to.f[t][0] = mt_row4<K, XCS>(x + (size_t)row * XRS, k);
-                    to.f[t][1] = mt_row4<K, XCS>(x + (size_t)row * XRS, k + 4u);
+            for (unsigned u = 0; u < U; ++u)
+#pragma unroll
+                for (unsigned r = 0; r < R; ++r) {
+                    q[u][r] = mt_u32x4{0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u};
+                    if (!RAGGED || (c * U + u) * 128u + 32u * g < K)
+                        q[u][r] = *reinterpret_cast<const mt_u32x4*>(wr[r] + (size_t)(c * U + u) * 64u);
                 }
+#pragma unroll
+            for (unsigned r = 0; r < R; ++r) {
+                const auto some = [&](const float* from, float* to) {
+                    if (GU % 4u == 0u && (!RAGGED || (c + 1u) * GU <= NG)) {
+#pragma unroll
+                        for (unsigned i = 0; i + 3u < GU; i += 4u) {
+                            const mt_f32x4 v = mt_ld4u(from + i);
+                            to[i] = v.x, to[i + 1u] = v.y, to[i + 2u] = v.z, to[i + 3u] = v.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (unsigned i = 0; i < GU; ++i) to[i] = !RAGGED || c * GU + i < NG ? from[i] : 0.f;
+                    }
+                };
+                some(scales + sr[r] + c * GU, s[r]);
+                if constexpr (ZEROS) some(zeros + sr[r] + c * GU, z[r]);
             }
-        }
-    };
+        };
 
-    float acc[R][ACC];
-#pragma unroll
-    for (unsigned r = 0; r < R; ++r)
-#pragma unroll
-        for (unsigned a = 0; a < ACC; ++a) acc[r][a] = 0.f;
-    unsigned char* own = lds + wave * (2048u * SETS);
-    const mt_i32x4 zero4 = {0, 0, 0, 0}, ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-
-    block now;
-    if (b0 < b1) load(b0, now);
-    for (unsigned blk = b0; blk < b1; ++blk) {
-        block next = now;
-        if (blk + 1u < b1) load(blk + 1u, next);
-        mt_i32x4 ae[SETS], ao[SETS];  // x of the even and the odd k, as the MFMA's rows
-        int ex[SETS];                 // E of this lane group's row of each set
-        bool odd = false;             // a block with values that are not finite
-        if constexpr (EIGHT) {
-            unsigned ev[4], od[4];
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) {
-                const unsigned lo = now.e[i / 2u][2u * (i % 2u)], hi = now.e[i / 2u][2u * (i % 2u) + 1u];
-                ev[i] = __builtin_amdgcn_perm(hi, lo, 0x06040200u);
-                od[i] = __builtin_amdgcn_perm(hi, lo, 0x07050301u);
-            }
-            ae[0] = mt_i32x4{(int)ev[0], (int)ev[1], (int)ev[2], (int)ev[3]};
-            ao[0] = mt_i32x4{(int)od[0], (int)od[1], (int)od[2], (int)od[3]};
-            ex[0] = 0;
-        } else {
-#pragma unroll
-            for (unsigned t = 0; t < SETS; ++t) {
-                unsigned top = 0u;  // the bits of |x| order as the values do, infinities and NaN last
-                float v[8];
-#pragma unroll
-                for (unsigned j = 0; j < 8u; ++j) {
-                    v[j] = now.f[t][j / 4u][j % 4u];
-                    const unsigned a = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-                    top = top > a ? top : a;
-                }
-#pragma unroll
-                for (int off = 8; off > 0; off >>= 1) {
-                    const unsigned a = (unsigned)__shfl_xor((int)top, off, 64);
-                    top = top > a ? top : a;
-                }
-                const int e = (int)(top >> 23);
-                ex[t] = e < 1 ? 1 : e;
-                odd = odd || e == 255;
-                unsigned d[8];
-#pragma unroll
-                for (unsigned j = 0; j < 8u; ++j) {
-                    const int whole = e == 255 ? 0 : (int)__builtin_ldexpf(v[j], 156 - ex[t]);
-                    d[j] = ((unsigned)whole + 0x00808080u) ^ 0x00808080u;
-                }
-                unsigned ev[4], od[4];
-                mt_bytes4(d[0], d[2], d[4], d[6], ev);
-                mt_bytes4(d[1], d[3], d[5], d[7], od);
-                unsigned char* to = own + 2048u * t + 4u * n + 256u * g;
-#pragma unroll
-                for (unsigned i = 0; i < 4u; ++i) {
-                    *reinterpret_cast<unsigned*>(to + 64u * i) = ev[3u - i];
-                    *reinterpret_cast<unsigned*>(to + 1024u + 64u * i) = od[3u - i];
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (unsigned t = 0; t < SETS; ++t) {
-                ae[t] = *reinterpret_cast<const mt_i32x4*>(own + 2048u * t + 64u * n + 16u * g);
-                ao[t] = *reinterpret_cast<const mt_i32x4*>(own + 2048u * t + 1024u + 64u * n + 16u * g);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
-        mt_i32x4 we[R], wo[R];
+        float acc[R][ACC];
 #pragma unroll
         for (unsigned r = 0; r < R; ++r)
 #pragma unroll
-            for (unsigned i = 0; i < 4u; ++i) {
-                const unsigned v = now.q[r][i] ^ 0x88888888u;
-                we[r][i] = (int)((v << 4) & 0xF0F0F0F0u);
-                wo[r][i] = (int)(v & 0xF0F0F0F0u);
-            }
+            for (unsigned a = 0; a < ACC; ++a) acc[r][a] = 0.f;
+        const mt_i32x4 zero4 = {0, 0, 0, 0};
+        mt_u32x4 q[U][R], xv[XV];
+        float s[R][GU], z[R][ZEROS ? GU : 1u];
+        if (c0 < c1) {
+            load_w(c0, q, s, z);
+            if constexpr (!SHARED) load_x(c0 * U, xv);
+        }
+        for (unsigned c = c0; c < c1; ++c) {
+            mt_u32x4 qn[U][R];
+            float sn[R][GU], zn[R][ZEROS ? GU : 1u];
+            if (c + 1u < c1) load_w(c + 1u, qn, sn, zn);
 #pragma unroll
-        for (unsigned j = 0; j < GB; ++j) {
-            const bool mine = GB == 1u || 32u * g / GROUP == j;
+            for (unsigned pu = 0; pu < U; pu += BL) {
+                mt_u32x4 xn[XV];
+                unsigned char* digits = SHARED ? lds + (c * U + pu) * DIGITS : lds + wave * (2048u * SETS);
+                int made[SETS];
+                if constexpr (!SHARED) {
+                    const unsigned after = c * U + pu + BL;
+                    if (after < c1 * U) load_x(after, xn);
+                    if constexpr (!EIGHT) {
+                        make_digits(xv, digits, made);
 #pragma unroll
-            for (unsigned t = 0; t < SETS; ++t) {
-                const mt_i32x4 je = mine ? ae[t] : zero4, jo = mine ? ao[t] : zero4;
-                mt_i32x4 cz = zero4;
-                if constexpr (ZEROS) {
-                    cz = __builtin_amdgcn_mfma_i32_16x16x64_i8(je, ones, cz, 0, 0, 0);
-                    cz = __builtin_amdgcn_mfma_i32_16x16x64_i8(jo, ones, cz, 0, 0, 0);
+                        for (unsigned t = 0; t < SETS; ++t) special = special || made[t] == 255;
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+                    }
                 }
 #pragma unroll
-                for (unsigned r = 0; r < R; ++r) {
-                    mt_i32x4 c = __builtin_amdgcn_mfma_i32_16x16x64_i8(je, we[r], zero4, 0, 0, 0);
-                    c = __builtin_amdgcn_mfma_i32_16x16x64_i8(jo, wo[r], c, 0, 0, 0);
-                    const float s = now.s[r][j];
-                    if constexpr (EIGHT) {
+                for (unsigned bl = 0; bl < BL; ++bl) {
+                    const unsigned u = pu + bl;
+                    if (RAGGED && (c * U + u) >= NB) continue;
+                    unsigned a[SETS][OP::COUNT][OP::WORDS];
+                    int ex[SETS];  // E of this lane group's row of the products
+#pragma unroll
+                    for (unsigned t = 0; t < SETS; ++t) {
+                        if constexpr (EIGHT) {
+#pragma unroll
+                            for (unsigned i = 0; i < 4u; ++i) {  // 8 k at a time, the even and the odd ones
+                                const unsigned lo = xv[i / 2u][2u * (i % 2u)], hi = xv[i / 2u][2u * (i % 2u) + 1u];
+                                constexpr unsigned PER = OP::WORDS / 2u;
+                                a[0][i / PER][2u * (i % PER)] = __builtin_amdgcn_perm(hi, lo, 0x06040200u);
+                                a[0][i / PER][2u * (i % PER) + 1u] = __builtin_amdgcn_perm(hi, lo, 0x07050301u);
+                            }
+                        } else {
+                            const unsigned char* from = digits + bl * DIGITS + t * (512u * XR);
+#pragma unroll
+                            for (unsigned i = 0; i < OP::COUNT; ++i)
+                                mt_ld_words<OP::WORDS>(a[t][i], from + place(n % (4u * XR), OP::at(i, g)));
+                            if constexpr (SHARED) ex[t] = es[((c * U + u) * SETS + t) * 4u + g % XR];
+                            else
+                                ex[t] = XR == 4u ? made[t]
+                                        : XR == 1u ? __builtin_amdgcn_readlane(made[t], (int)(16u * bl))
+                                                   : __shfl(made[t], (int)(16u * (bl * XR + g % XR)), 64);
+                        }
+                    }
+                    mt_i32x4 cz[SETS][OP::COUNT];
+                    if constexpr (ZEROS) {
+                        unsigned one[OP::WORDS];
+#pragma unroll
+                        for (unsigned i = 0; i < OP::WORDS; ++i) one[i] = 0x01010101u;
+#pragma unroll
+                        for (unsigned t = 0; t < SETS; ++t)
+#pragma unroll
+                            for (unsigned i = 0; i < OP::COUNT; ++i) cz[t][i] = OP::product(a[t][i], one, zero4);
+                    }
+#pragma unroll
+                    for (unsigned r = 0; r < R; ++r) {
+                        unsigned v[4], b[OP::COUNT][OP::WORDS];
+#pragma unroll
+                        for (unsigned i = 0; i < 4u; ++i) v[i] = q[u][r][i] ^ 0x88888888u;
+                        OP::spread(v);
 #pragma unroll
                         for (unsigned i = 0; i < 4u; ++i) {
-                            float f = (float)c[i];
-                            if constexpr (ZEROS) f = __builtin_fmaf((float)cz[i], 128.f - 16.f * now.z[r][j], f);
-                            acc[r][i] = __builtin_fmaf(f, s, acc[r][i]);
+                            constexpr unsigned PER = OP::WORDS / 2u;
+                            b[i / PER][2u * (i % PER)] = (v[i] << 4) & 0xF0F0F0F0u;
+                            b[i / PER][2u * (i % PER) + 1u] = v[i] & 0xF0F0F0F0u;
                         }
-                    } else {
-                        float f = mt_digits(c);
-                        if constexpr (ZEROS) f = __builtin_fmaf(mt_digits(cz), 128.f - 16.f * now.z[r][j], f);
-                        acc[r][t] += __builtin_ldexpf(f * s, ex[t] - 160);
+#pragma unroll
+                        for (unsigned t = 0; t < SETS; ++t) {
+                            float sum = 0.f;
+#pragma unroll
+                            for (unsigned j = 0; j < GB; ++j) {
+                                mt_i32x4 p = OP::product(a[t][j], b[j], zero4), o = zero4;
+                                if constexpr (ZEROS) o = cz[t][j];
+                                if constexpr (GB == 1u) {
+                                    p = OP::product(a[t][1], b[1], p);
+                                    if constexpr (ZEROS) o = o + cz[t][1];
+                                }
+                                const float by = s[r][u * GB + j];
+                                if constexpr (EIGHT) {
+#pragma unroll
+                                    for (unsigned i = 0; i < 4u; ++i) {
+                                        float f = (float)p[i];
+                                        if constexpr (ZEROS) f = __builtin_fmaf((float)o[i], 128.f - 16.f * z[r][u * GB + j], f);
+                                        acc[r][i] = __builtin_fmaf(f, by, acc[r][i]);
+                                    }
+                                } else {
+                                    float f = mt_digits(p);
+                                    if constexpr (ZEROS) f = __builtin_fmaf(mt_digits(o), 128.f - 16.f * z[r][u * GB + j], f);
+                                    sum = GB == 1u ? f * by : __builtin_fmaf(f, by, sum);
+                                }
+                            }
+                            if constexpr (!EIGHT) acc[r][t] += __builtin_ldexpf(sum, ex[t] - 160);
+                        }
                     }
+                }
+                if constexpr (!SHARED) {
+                    if constexpr (!EIGHT) {
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+                    }
+#pragma unroll
+                    for (unsigned i = 0; i < XV; ++i) xv[i] = xn[i];
+                }
+            }
+#pragma unroll
+            for (unsigned r = 0; r < R; ++r) {
+#pragma unroll
+                for (unsigned u = 0; u < U; ++u) q[u][r] = qn[u][r];
+#pragma unroll
+                for (unsigned i = 0; i < GU; ++i) {
+                    s[r][i] = sn[r][i];
+                    if constexpr (ZEROS) z[r][i] = zn[r][i];
                 }
             }
         }
         if constexpr (!EIGHT) {
-            if (__any(odd)) {
-                // Rare: the rows of this block that hold infinities or NaN, in fp32.  Every
-                // lane sums its 32 k of its weight rows, the four pieces meet.
-#pragma unroll
-                for (unsigned t = 0; t < SETS; ++t)
-                    for (unsigned mm = 0; mm < 4u; ++mm) {
-                        if (__shfl(ex[t], (int)(16u * mm), 64) != 255) continue;
-                        const float* xr = x + (size_t)(m0 + 4u * t + mm) * XRS;
+            if (SHARED ? special : __any(special)) {
+                // Rare: rows of x with infinities or NaN in a block.  Every lane sums its 32 k of
+                // its weight rows, the four pieces meet.
+#pragma unroll 1
+                for (unsigned blk = c0 * U; blk < c1 * U && blk < NB; ++blk)
+#pragma unroll 1
+                    for (unsigned m = 0; m < 4u * SETS && m0 + m < rows; ++m) {
+                        const float* xr = x + (size_t)(m0 + m) * XRS;
+                        bool bad = false;
+                        for (unsigned k = blk * 128u + lane; k < blk * 128u + 128u && k < K; k += 64u)
+                            bad = bad || !(__builtin_fabsf(xr[(size_t)k * XCS]) < INFINITY);
+                        if (!__any(bad)) continue;
+                        const unsigned k0 = blk * 128u + 32u * g;
 #pragma unroll
                         for (unsigned r = 0; r < R; ++r) {
                             float part = 0.f;
-                            float z = 8.f, s = now.s[r][0];
-#pragma unroll
-                            for (unsigned j = 0; j < GB; ++j)
-                                if (32u * g / GROUP == j) {
-                                    s = now.s[r][j];
-                                    if constexpr (ZEROS) z = now.z[r][j];
+                            if (k0 < K) {
+                                float zero = 8.f;
+                                if constexpr (ZEROS) zero = zeros[sr[r] + k0 / GROUP];
+#pragma unroll 1
+                                for (unsigned i = 0; i < 32u; ++i) {
+                                    const unsigned v = (wr[r][(size_t)blk * 64u + i / 2u] >> (4u * (i % 2u))) & 15u;
+                                    part += xr[(size_t)(k0 + i) * XCS] * ((float)v - zero);
                                 }
-                            for (unsigned i = 0; i < 32u; ++i) {
-                                const unsigned k = blk * 128u + 32u * g + i;
-                                const unsigned word = i < 8u ? now.q[r].x : i < 16u ? now.q[r].y
-                                                      : i < 24u ? now.q[r].z : now.q[r].w;
-                                const float q = (float)((word >> (4u * (i % 8u))) & 15u);
-                                if (!RAGGED || k < K) part += xr[(size_t)k * XCS] * (q - z);
+                                part *= scales[sr[r] + k0 / GROUP];
                             }
-                            if (!RAGGED || blk * 128u + 32u * g < K) part *= s;
                             part += mt_shfl_xor(part, 16);
                             part += mt_shfl_xor(part, 32);
-                            if (g == mm) acc[r][t] += part;
+#pragma unroll
+                            for (unsigned t = 0; t < SETS; ++t)
+                                if (m / 4u == t && m % 4u == g) acc[r][t] += part;
                         }
                     }
             }
         }
-        now = next;
-    }
-
-    // The waves' sums, [WAVES][R][ACC][64 lanes].
-    float* sums = reinterpret_cast<float*>(lds);
-    __syncthreads();
+        const auto put = [&](unsigned r, unsigned a, unsigned ln, float v) {
+            const unsigned col = n0 + 16u * r + (ln & 15u), row = m0 + (EIGHT ? 4u * (ln >> 4) + a : 4u * a + (ln >> 4));
+            if (col < N && row < rows && (EIGHT || ln / 16u < XR))
+                y[(size_t)row * N + col] = EIGHT ? v * (xs[row] * 0.0625f) : v;
+        };
+        if constexpr (SHARED) {
 #pragma unroll
-    for (unsigned r = 0; r < R; ++r)
+            for (unsigned r = 0; r < R; ++r)
 #pragma unroll
-        for (unsigned a = 0; a < ACC; ++a) sums[((wave * R + r) * ACC + a) * 64u + lane] = acc[r][a];
-    __syncthreads();
-    for (unsigned at = threadIdx.x; at < R * ACC * 64u; at += 64u * WAVES) {
-        float v = 0.f;
+                for (unsigned a = 0; a < ACC; ++a) put(r, a, lane, acc[r][a]);
+        } else {
+            // The waves' sums, [WAVES][R][ACC][64 lanes].
+            float* sums = reinterpret_cast<float*>(lds);
+            __syncthreads();
 #pragma unroll
-        for (unsigned i = 0; i < WAVES; ++i) v += sums[i * (R * ACC * 64u) + at];
-        const unsigned r = at / (ACC * 64u), a = at / 64u % ACC, ln = at % 64u;
-        const unsigned col = n0 + 16u * r + (ln & 15u), row = m0 + (EIGHT ? 4u * (ln >> 4) + a : 4u * a + (ln >> 4));
-        if (col < N && row < rows) y[(size_t)row * N + col] = EIGHT ? v * (xs[row] * 0.0625f) : v;
+            for (unsigned r = 0; r < R; ++r)
+#pragma unroll
+                for (unsigned a = 0; a < ACC; ++a) sums[((wave * R + r) * ACC + a) * 64u + lane] = acc[r][a];
+            __syncthreads();
+            for (unsigned at = threadIdx.x; at < R * ACC * 64u; at += 64u * WAVES) {
+                float v = 0.f;
+#pragma unroll
+                for (unsigned i = 0; i < WAVES; ++i) v += sums[i * (R * ACC * 64u) + at];
+                put(at / (ACC * 64u), at / 64u % ACC, at % 64u, v);
+            }
+            __syncthreads();
+        }
     }
 }

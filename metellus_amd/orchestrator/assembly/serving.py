@@ -238,21 +238,34 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
 # ---------------------------------------------------------------------------
 
 
-def int4_shape(rows: int, k: int, n: int) -> tuple[int, int]:
-    """(waves of a workgroup, which split k; tiles of 16 weight rows of each)."""
-    blocks = _ceil(k, 128)
+INT4_TUNE: dict = {}  # tuning overrides of ``int4_shape``
+
+
+def int4_shape(rows: int, k: int, n: int, eight: bool) -> dict:
+    """How a product is cut: ``shared`` (digits of all of x in LDS, waves on tiles of
+    their own) or waves that split k; ``waves`` of a workgroup, ``tiles`` of 16 weight
+    rows that a wave takes together, blocks of 128 k that it loads ``together``."""
+    sets = 1 if eight else _ceil(min(rows, 16), 4)
+    shared = not eight and n >= 32768 and 4 * min(rows, 4) * sets * k <= 65536
     tiles = 1
-    while tiles < 4 and _ceil(n, 32 * tiles) >= 512 and (rows > 1 or tiles < 2):
+    while tiles < 4 and _ceil(n, 32 * tiles) >= 512 and (rows > 4 or tiles < 2):
         tiles *= 2
-    return min(8, blocks), tiles
+    shape = {"shared": shared, "waves": 8, "tiles": tiles, "together": 2 if tiles == 4 else 4, **INT4_TUNE}
+    if not shape["shared"]:
+        shape["waves"] = min(shape["waves"], _ceil(k, 128 * shape["together"]))
+    return shape
 
 
 def _assemble_int4(decision: DecisionView, op: Int4MatmulOp, function_name: str | None) -> KernelGroup:
     (rows, k), n = op.x.shape, op.weights.shape[0]
     eight = op.x_scales is not None
-    waves, tiles = int4_shape(rows, k, n)
+    shape = int4_shape(rows, k, n, eight)
+    waves, tiles, shared = shape["waves"], shape["tiles"], shape["shared"]
     held = min(rows, 16)
     sets = 1 if eight else _ceil(held, 4)  # matrix instructions' rows: 16 of x, or 4 of x in four digits each
+    each = 4 if eight or held > 2 else held
+    made = 1 if eight else 4 // each  # blocks of x made into digits at once
+    together = max(shape["together"], made)
     sig = _Signature()
     args = (
         "nullptr" if eight else sig.add("x", op.x),
@@ -265,15 +278,23 @@ def _assemble_int4(decision: DecisionView, op: Int4MatmulOp, function_name: str 
         "M",
         "mt_lds",
     )
+    if shared:
+        lds = _ceil(k, 128 * made) * made * (512 * each + 16) * sets
+    else:
+        lds = max(0 if eight else 2048 * sets * waves, waves * tiles * 256 * (4 if eight else sets))
     frag = ServingFragment(
         "mt_matmul_int4",
-        (eight, sets, k, n, op.group, op.zeros is not None, tiles, waves, op.x.row_stride, op.x.col_stride),
+        (eight, shared, each, sets, k, n, op.group, op.zeros is not None, tiles, together, waves, op.x.row_stride,
+         op.x.col_stride),
         args,
-        lds_bytes=max(0 if eight else 2048 * sets * waves, waves * tiles * 16 * 4 * 4 * (4 if eight else sets)),
+        lds_bytes=lds,
         name="int4_matmul",
     )
-    grid = (_ceil(n, 16 * tiles), _ceil(rows, 16), 1)
-    return _group(decision, sig, frag, function_name or f"int4_matmul_{op.y.name}", {"M": rows}, grid, 64 * waves)
+    groups = _ceil(n, 16 * tiles)
+    if shared:
+        groups = min(_ceil(groups, waves), shape.get("groups", 512))
+    return _group(decision, sig, frag, function_name or f"int4_matmul_{op.y.name}", {"M": rows}, (groups, _ceil(rows, 16), 1),
+                  64 * waves)
 
 
 _ASSEMBLE = {

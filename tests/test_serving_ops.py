@@ -375,5 +375,6 @@ def test_launch_rules_stay_within_what_the_kernels_take():
     for rows in (1, 4, 16, 100):
         for k in (32, 128, 4096, 16384):
             for n in (1, 100, 4096, 131072):
-                waves, tiles = int4_shape(rows, k, n)
-                assert 1 <= waves <= 8 and tiles in (1, 2, 4)
+                for eight in (False, True):
+                    shape = int4_shape(rows, k, n, eight)
+                    assert 1 <= shape["waves"] <= 16 and shape["tiles"] in (1, 2, 4) and shape["together"] in (1, 2, 4)
