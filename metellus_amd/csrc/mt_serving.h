@@ -13,6 +13,16 @@
 
 typedef int mt_i32x4 __attribute__((ext_vector_type(4)));
 
+// 32 bits where they hold every value, 64 otherwise.
+template <bool SMALL>
+struct mt_count {
+    using type = unsigned;
+};
+template <>
+struct mt_count<false> {
+    using type = unsigned long long;
+};
+
 // Elements c .. c + 3 of a row of COLS elements CS apart, 0 behind its end.
 template <unsigned COLS, unsigned CS>
 MT_INLINE mt_f32x4 mt_row4(const float* row, unsigned c) {
@@ -198,17 +208,19 @@ MT_INLINE void mt_dequantize(const signed char* q, const float* s, float* y, siz
 // rows, keys first.  KIND 0: fp32, 1: int8, 2: e4m3 (OCP).
 // ---------------------------------------------------------------------------
 
-template <int KIND, unsigned HK, unsigned PS, unsigned D>
+template <int KIND, unsigned HK, unsigned PS, unsigned D, unsigned PAGES>
 struct mt_cache {
     static constexpr unsigned ITEM = KIND == 0 ? 4u : 1u;
     static constexpr unsigned HALF = HK * PS * D * ITEM;  // bytes of a page's keys (or values)
     static constexpr unsigned SCALES = 2u * HALF;
     static constexpr unsigned PAGE = (2u * HALF + (KIND == 0 ? 0u : 8u * HK * PS) + 15u) / 16u * 16u;
-    MT_INLINE static size_t row(unsigned page, unsigned part, unsigned head, unsigned r) {
-        return (size_t)page * PAGE + (size_t)part * HALF + (size_t)((head * PS + r) * D) * ITEM;
+    // Offsets in the cache: 32 bits (a register less, one base) up to 4 GiB of it.
+    using offset = typename mt_count<((unsigned long long)PAGES * PAGE < (1ull << 32))>::type;
+    MT_INLINE static offset row(unsigned page, unsigned part, unsigned head, unsigned r) {
+        return (offset)page * PAGE + part * HALF + ((head * PS + r) * D) * ITEM;
     }
-    MT_INLINE static size_t scale(unsigned page, unsigned part, unsigned head, unsigned r) {
-        return (size_t)page * PAGE + SCALES + (size_t)((part * HK + head) * PS + r) * 4u;
+    MT_INLINE static offset scale(unsigned page, unsigned part, unsigned head, unsigned r) {
+        return (offset)page * PAGE + SCALES + ((part * HK + head) * PS + r) * 4u;
     }
 };
 
@@ -253,10 +265,10 @@ MT_INLINE float mt_step_round(float x, float s, float inv) {
 // One row of D values held by 16 lanes (lane j has dims 64 c + 4 j .. + 3) into
 // the cache.  `live`: whether the row is stored at all; every lane takes part
 // in the exchange of the maximum.
-template <int KIND, unsigned HK, unsigned PS, unsigned D>
+template <int KIND, unsigned HK, unsigned PS, unsigned D, unsigned PAGES>
 MT_INLINE void mt_cache_put(unsigned char* cache, const mt_f32x4 (&v)[(D + 63u) / 64u], unsigned j, bool live,
                             unsigned page, unsigned part, unsigned head, unsigned r) {
-    using C = mt_cache<KIND, HK, PS, D>;
+    using C = mt_cache<KIND, HK, PS, D, PAGES>;
     constexpr unsigned NC = (D + 63u) / 64u;
     if constexpr (KIND == 0) {
         if (!live) return;
@@ -347,7 +359,7 @@ MT_INLINE void mt_cache_write(const float* k, const float* v, const int* slots, 
                 x[c] = part ? mt_row4<HK * D, VCS>(v + (size_t)t * VRS, head * D + d)
                             : mt_row4<HK * D, KCS>(k + (size_t)t * KRS, head * D + d);
         }
-        mt_cache_put<KIND, HK, PS, D>(cache, x, j, live, slot / PS, part, head, slot % PS);
+        mt_cache_put<KIND, HK, PS, D, PAGES>(cache, x, j, live, slot / PS, part, head, slot % PS);
     }
 }
 
@@ -355,7 +367,7 @@ MT_INLINE void mt_cache_write(const float* k, const float* v, const int* slots, 
 // outside it.  16 lanes take a row of one head.
 template <int KIND, unsigned HK, unsigned PS, unsigned D, unsigned PAGES>
 MT_INLINE void mt_cache_read(const unsigned char* cache, const int* slots, float* k, float* v, unsigned rows) {
-    using C = mt_cache<KIND, HK, PS, D>;
+    using C = mt_cache<KIND, HK, PS, D, PAGES>;
     constexpr unsigned long long ALL = (unsigned long long)PAGES * PS;
     constexpr unsigned SLOTS = ALL > 0x80000000ull ? 0x80000000u : (unsigned)ALL;
     constexpr unsigned NC = (D + 63u) / 64u;
@@ -489,15 +501,6 @@ MT_INLINE float mt_fold_g(float v, OP op) {
     return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <bool SMALL>
-struct mt_count {
-    using type = unsigned;
-};
-template <>
-struct mt_count<false> {
-    using type = unsigned long long;
-};
-
 // The units of a launch: which sequence and head they belong to, and which
 // workgroup has them.  Whole waves call its functions; their results are uniform.
 template <unsigned ROWS, unsigned STEP, unsigned MOST, unsigned HEADS, unsigned GROUPS>
@@ -558,7 +561,7 @@ template <int KIND, unsigned HK, unsigned PS, unsigned D, unsigned PAGES, unsign
           unsigned WAVES, unsigned GROUPS, unsigned BATCH, unsigned ROWS, unsigned QRS, unsigned QCS>
 MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, const int* pages, const int* lengths,
                                   float* o, double scale, float* ws, unsigned char* lds) {
-    using C = mt_cache<KIND, HK, PS, D>;
+    using C = mt_cache<KIND, HK, PS, D, PAGES>;
     constexpr unsigned ITEM = C::ITEM, PARTS = (SHARE + HELD - 1u) / HELD;
     constexpr bool WIDE = KIND == 0;
     constexpr unsigned BLOCKS = WIDE ? 1u : 2u, TILE = 16u * BLOCKS;       // positions of a tile
@@ -619,9 +622,9 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 #pragma unroll
         for (unsigned bi = 0; bi < BLOCKS; ++bi) {
             const unsigned t0 = first + TILE * ti + 16u * bi;
-            const unsigned char* p = cache + C::row(safe(page[bi]), 0u, head, (t0 + n) % PS) + g * (VK * ITEM);
+            const typename C::offset p = C::row(safe(page[bi]), 0u, head, (t0 + n) % PS) + g * (VK * ITEM);
 #pragma unroll
-            for (unsigned jj = 0; jj < NJ; ++jj) mt_ld_words<KW>(kw[bi][jj], p + jj * (4u * VK * ITEM));
+            for (unsigned jj = 0; jj < NJ; ++jj) mt_ld_words<KW>(kw[bi][jj], cache + p + jj * (4u * VK * ITEM));
             if constexpr (!WIDE) {
 #pragma unroll
                 for (unsigned i = 0; i < 4u; ++i)
@@ -637,12 +640,12 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 #pragma unroll
             for (unsigned i = 0; i < 4u; ++i) {
                 const unsigned pg = safe(row_page(page[bi], i)), r = (t0 + 4u * g + i) % PS;
-                const unsigned char* p = cache + C::row(pg, 1u, head, r);
+                const typename C::offset p = C::row(pg, 1u, head, r);
 #pragma unroll
                 for (unsigned c = 0; c < NV; ++c) {
                     unsigned d = VV * (16u * c + n);
                     if (D % (16u * VV) != 0u && d >= D) d = 0u;  // (columns that no output takes)
-                    mt_ld_words<VW>(vw[bi][i][c], p + d * ITEM);
+                    mt_ld_words<VW>(vw[bi][i][c], cache + (p + d * ITEM));
                 }
                 if constexpr (!WIDE) vs[bi][i] = *reinterpret_cast<const float*>(cache + C::scale(pg, 1u, head, r));
             }
@@ -689,6 +692,7 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         for (unsigned i = 0; i < NV * VV; ++i) acc[t][i] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
     }
     bool seen = false;
+#pragma unroll 1
     for (unsigned ti = wave; ti < tiles; ti += WAVES) {
         int page_after[BLOCKS];
 #pragma unroll
@@ -990,10 +994,10 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 // rows of the wave (permlane swaps: 2 or 4 for 32 k a lane), so that an MFMA takes
 // one group whole.
 //
-// Bound: HBM, the weights once.  SHARED: the digits of all of x stay in LDS and every
-// wave takes weight tiles of its own, row after row; otherwise the waves of a
-// workgroup share its weight rows and split k, each making the digits of its part as
-// it goes, so that few weight rows still keep many loads in flight.
+// Bound: HBM, the weights once.  SHARED: the digits of x stay in LDS, PB blocks of k at a
+// time, and every wave takes weight tiles of its own, row after row; otherwise the
+// waves of a workgroup share its weight rows and split k, each making the digits of its
+// part as it goes, so that few weight rows still keep many loads in flight.
 // ---------------------------------------------------------------------------
 
 // The whole number that an MFMA's four digit rows stand for.
@@ -1053,7 +1057,7 @@ struct mt_operand {
     }
 };
 
-template <bool EIGHT, bool SHARED, unsigned XR, unsigned SETS, unsigned K, unsigned N, unsigned GROUP, bool ZEROS, unsigned R,
+template <bool EIGHT, bool SHARED, unsigned PB, unsigned XR, unsigned SETS, unsigned K, unsigned N, unsigned GROUP, bool ZEROS, unsigned R,
           unsigned U, unsigned WAVES, unsigned XRS, unsigned XCS>
 MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float* xs, const unsigned char* w,
                               const float* scales, const float* zeros, float* y, unsigned rows, unsigned char* lds) {
@@ -1066,12 +1070,21 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
     const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
     const unsigned m0 = blockIdx.y * 16u;
     const unsigned c0 = SHARED ? 0u : NC * wave / WAVES, c1 = SHARED ? NC : NC * (wave + 1u) / WAVES;
+    constexpr unsigned PHASES = SHARED ? (NB + PB - 1u) / PB : 1u;
 
     // x for one making of digits: rows 4 t + g % XR of block blk + g / XR, k 8 n .. + 7; x
     // in 8 bits: row n's share of the operands of block blk.
     constexpr unsigned XV = EIGHT ? 2u : 2u * SETS;
     const auto load_x = [&](unsigned blk, mt_u32x4 (&to)[XV]) {
-        if constexpr (EIGHT) {
+        if constexpr (EIGHT && SHARED) {
+            const unsigned k = blk * 128u + 32u * g;
+            const bool in = m0 + n < rows && k < K;
+#pragma unroll
+            for (unsigned i = 0; i < 2u; ++i) {
+                to[i] = mt_u32x4{0u, 0u, 0u, 0u};
+                if (in) to[i] = *reinterpret_cast<const mt_u32x4*>(x8 + (size_t)(m0 + n) * K + k + 16u * i);
+            }
+        } else if constexpr (EIGHT) {
             const signed char* row = x8 + (size_t)(m0 + n < rows ? m0 + n : m0) * K;
 #pragma unroll
             for (unsigned i = 0; i < OP::COUNT; ++i) {
@@ -1131,25 +1144,37 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
     };
 
     bool special = false;
-    int* es = reinterpret_cast<int*>(lds + (SHARED ? (NB + BL - 1u) / BL * BL * DIGITS : 0u));  // SHARED: E, [blocks][SETS][4]
-    if constexpr (SHARED) {
-        for (unsigned blk = wave * BL; blk < NB; blk += WAVES * BL) {
+    int* es = reinterpret_cast<int*>(lds + (SHARED ? PB * DIGITS : 0u));  // SHARED: E, [PB][SETS][4]
+    // SHARED: the digits of blocks p0 .. p0 + PB - 1.
+    const auto make_phase = [&](unsigned p0) {
+        for (unsigned at = wave * BL; at < PB && p0 + at < NB; at += WAVES * BL) {
             mt_u32x4 xv[XV];
-            int made[SETS];
-            load_x(blk, xv);
-            make_digits(xv, lds + blk * DIGITS, made);
+            load_x(p0 + at, xv);
+            if constexpr (EIGHT) {
 #pragma unroll
-            for (unsigned t = 0; t < SETS; ++t) {
-                special = special || made[t] == 255;
-                if (n == 0u) es[((blk + g / XR) * SETS + t) * 4u + g % XR] = made[t];
+                for (unsigned i = 0; i < 4u; ++i) {  // 8 k at a time, the even and the odd ones
+                    const unsigned lo = xv[i / 2u][2u * (i % 2u)], hi = xv[i / 2u][2u * (i % 2u) + 1u];
+                    *reinterpret_cast<mt_u32x2*>(lds + at * DIGITS + place(n, 32u * g + 8u * i)) =
+                        mt_u32x2{__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u)};
+                }
+            } else {
+                int made[SETS];
+                make_digits(xv, lds + at * DIGITS, made);
+#pragma unroll
+                for (unsigned t = 0; t < SETS; ++t) {
+                    special = special || made[t] == 255;
+                    if (n == 0u) es[((at + g / XR) * SETS + t) * 4u + g % XR] = made[t];
+                }
             }
         }
-        special = __syncthreads_or(special);
-    }
+        if constexpr (EIGHT) __syncthreads();
+        else special = __syncthreads_or(special);
+    };
 
     constexpr unsigned TILES = (N + 16u * R - 1u) / (16u * R);
-    for (unsigned tile = SHARED ? blockIdx.x * WAVES + wave : blockIdx.x; tile < TILES;
-         tile += SHARED ? gridDim.x * WAVES : gridDim.x) {
+    // (all waves of a workgroup go round together where they share digits)
+    for (unsigned at = blockIdx.x; at * (SHARED ? WAVES : 1u) < TILES; at += gridDim.x) {
+        const unsigned tile = SHARED ? at * WAVES + wave : at;
         const unsigned n0 = tile * (16u * R);
         const unsigned char* wr[R];
         size_t sr[R];
@@ -1199,14 +1224,25 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
             load_w(c0, q, s, z);
             if constexpr (!SHARED) load_x(c0 * U, xv);
         }
-        for (unsigned c = c0; c < c1; ++c) {
+#pragma unroll 1
+        for (unsigned phase = 0; phase < PHASES; ++phase) {
+        if constexpr (SHARED) {
+            if (PHASES > 1u || at == blockIdx.x) {
+                if (phase > 0u || at != blockIdx.x) __syncthreads();
+                make_phase(phase * PB);
+            }
+        }
+        const unsigned cp = SHARED ? phase * (PB / U) : c0;
+        const unsigned cq = SHARED ? (cp + PB / U < c1 ? cp + PB / U : c1) : c1;
+#pragma unroll 1
+        for (unsigned c = cp; c < cq; ++c) {
             mt_u32x4 qn[U][R];
             float sn[R][GU], zn[R][ZEROS ? GU : 1u];
             if (c + 1u < c1) load_w(c + 1u, qn, sn, zn);
 #pragma unroll
             for (unsigned pu = 0; pu < U; pu += BL) {
                 mt_u32x4 xn[XV];
-                unsigned char* digits = SHARED ? lds + (c * U + pu) * DIGITS : lds + wave * (2048u * SETS);
+                unsigned char* digits = SHARED ? lds + (c * U + pu - phase * PB) * DIGITS : lds + wave * (2048u * SETS);
                 int made[SETS];
                 if constexpr (!SHARED) {
                     const unsigned after = c * U + pu + BL;
@@ -1227,7 +1263,7 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
                     int ex[SETS];  // E of this lane group's row of the products
 #pragma unroll
                     for (unsigned t = 0; t < SETS; ++t) {
-                        if constexpr (EIGHT) {
+                        if constexpr (EIGHT && !SHARED) {
 #pragma unroll
                             for (unsigned i = 0; i < 4u; ++i) {  // 8 k at a time, the even and the odd ones
                                 const unsigned lo = xv[i / 2u][2u * (i % 2u)], hi = xv[i / 2u][2u * (i % 2u) + 1u];
@@ -1240,14 +1276,15 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
 #pragma unroll
                             for (unsigned i = 0; i < OP::COUNT; ++i)
                                 mt_ld_words<OP::WORDS>(a[t][i], from + place(n % (4u * XR), OP::at(i, g)));
-                            if constexpr (SHARED) ex[t] = es[((c * U + u) * SETS + t) * 4u + g % XR];
+                            if constexpr (EIGHT) ex[t] = 0;
+                            else if constexpr (SHARED) ex[t] = es[((c * U + u - phase * PB) * SETS + t) * 4u + g % XR];
                             else
                                 ex[t] = XR == 4u ? made[t]
                                         : XR == 1u ? __builtin_amdgcn_readlane(made[t], (int)(16u * bl))
                                                    : __shfl(made[t], (int)(16u * (bl * XR + g % XR)), 64);
                         }
                     }
-                    mt_i32x4 cz[SETS][OP::COUNT];
+                    float cz[SETS][GB][EIGHT ? 4u : 1u];  // the sums of x by group, for the zeros
                     if constexpr (ZEROS) {
                         unsigned one[OP::WORDS];
 #pragma unroll
@@ -1255,7 +1292,16 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
 #pragma unroll
                         for (unsigned t = 0; t < SETS; ++t)
 #pragma unroll
-                            for (unsigned i = 0; i < OP::COUNT; ++i) cz[t][i] = OP::product(a[t][i], one, zero4);
+                            for (unsigned j = 0; j < GB; ++j) {
+                                mt_i32x4 o = OP::product(a[t][j], one, zero4);
+                                if constexpr (GB == 1u) o = OP::product(a[t][1], one, o);
+                                if constexpr (EIGHT) {
+#pragma unroll
+                                    for (unsigned i = 0; i < 4u; ++i) cz[t][j][i] = (float)o[i];
+                                } else {
+                                    cz[t][j][0] = mt_digits(o);
+                                }
+                            }
                     }
 #pragma unroll
                     for (unsigned r = 0; r < R; ++r) {
@@ -1274,23 +1320,19 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
                             float sum = 0.f;
 #pragma unroll
                             for (unsigned j = 0; j < GB; ++j) {
-                                mt_i32x4 p = OP::product(a[t][j], b[j], zero4), o = zero4;
-                                if constexpr (ZEROS) o = cz[t][j];
-                                if constexpr (GB == 1u) {
-                                    p = OP::product(a[t][1], b[1], p);
-                                    if constexpr (ZEROS) o = o + cz[t][1];
-                                }
+                                mt_i32x4 p = OP::product(a[t][j], b[j], zero4);
+                                if constexpr (GB == 1u) p = OP::product(a[t][1], b[1], p);
                                 const float by = s[r][u * GB + j];
                                 if constexpr (EIGHT) {
 #pragma unroll
                                     for (unsigned i = 0; i < 4u; ++i) {
                                         float f = (float)p[i];
-                                        if constexpr (ZEROS) f = __builtin_fmaf((float)o[i], 128.f - 16.f * z[r][u * GB + j], f);
+                                        if constexpr (ZEROS) f = __builtin_fmaf(cz[t][j][i], 128.f - 16.f * z[r][u * GB + j], f);
                                         acc[r][i] = __builtin_fmaf(f, by, acc[r][i]);
                                     }
                                 } else {
                                     float f = mt_digits(p);
-                                    if constexpr (ZEROS) f = __builtin_fmaf(mt_digits(o), 128.f - 16.f * z[r][u * GB + j], f);
+                                    if constexpr (ZEROS) f = __builtin_fmaf(cz[t][j][0], 128.f - 16.f * z[r][u * GB + j], f);
                                     sum = GB == 1u ? f * by : __builtin_fmaf(f, by, sum);
                                 }
                             }
@@ -1317,6 +1359,7 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
                     if constexpr (ZEROS) z[r][i] = zn[r][i];
                 }
             }
+        }
         }
         if constexpr (!EIGHT) {
             if (SHARED ? special : __any(special)) {

@@ -207,7 +207,11 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
     held = min(share, 16 if spec.dim <= 128 else 8)
     parts = _ceil(share, held)
     pairs = rows * spec.kv_heads * parts
-    waves = ATTENTION_WAVES
+    # Eight waves to a compute unit; four, with twice the registers each, where the sums
+    # of a wave's heads (or its tile of long fp32 rows) would not fit otherwise.
+    sets = 1 if spec.dtype == "float32" else _ceil(held, 4)
+    heavy = spec.dim > 128 or sets * spec.dim > (256 if spec.page_size % 16 == 0 else 128)
+    waves = 4 if heavy else ATTENTION_WAVES
     step = (16 if spec.dtype == "float32" else 32) * waves
     groups = attention_workgroups(pairs, op.capacity, step, batch)
     floats = held * (spec.dim + 2)
@@ -239,33 +243,52 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
 
 
 INT4_TUNE: dict = {}  # tuning overrides of ``int4_shape``
+INT4_LDS = 131072  # bytes of digits at a time, where the waves share them
 
 
-def int4_shape(rows: int, k: int, n: int, eight: bool) -> dict:
-    """How a product is cut: ``shared`` (digits of all of x in LDS, waves on tiles of
-    their own) or waves that split k; ``waves`` of a workgroup, ``tiles`` of 16 weight
-    rows that a wave takes together, blocks of 128 k that it loads ``together``."""
-    sets = 1 if eight else _ceil(min(rows, 16), 4)
-    shared = not eight and n >= 32768 and 4 * min(rows, 4) * sets * k <= 65536
-    tiles = 1
-    while tiles < 4 and _ceil(n, 32 * tiles) >= 512 and (rows > 4 or tiles < 2):
-        tiles *= 2
-    shape = {"shared": shared, "waves": 8, "tiles": tiles, "together": 2 if tiles == 4 else 4, **INT4_TUNE}
+def int4_shape(rows: int, k: int, n: int, group: int, eight: bool, zeros: bool) -> dict:
+    """How a product is cut: ``shared`` (digits of x in LDS, waves on tiles of their
+    own) or waves that split k; ``waves`` of a workgroup, ``tiles`` of 16 weight rows
+    that a wave takes together, blocks of 128 k that it loads ``together``; ``each`` row
+    of x in a set of MFMA rows, ``sets`` of them; ``phase``, blocks of k whose digits
+    are in LDS at once."""
+    held = min(rows, 16)
+    sets = 1 if eight else _ceil(held, 4)
+    each = 4 if eight or held > 2 else held
+    # Enough weight rows for a tile to most waves of the GPU: the waves share x's digits
+    # (4 rows, 4096 x 131072: 54 us, splitting k 80; 16 rows, 8192 x 28672: 57 and 74; one
+    # row 30 and 29).  Fewer rows: splitting k (16 rows, 4096 x 11008: 24 us).
+    shared = _ceil(n, 16) >= 1536
+    blocks = _ceil(k, 128)
+    made = 1 if eight else 4 // each  # blocks of x made into digits at once
+    if shared:
+        tiles, waves, together = 1, 8, 4
+    else:
+        # Two tiles a wave halve the work on x, where two still leave a workgroup to each
+        # compute unit (7 rows, 8192 x 8192: 21 us, one tile 27); 16 waves where one does
+        # not (3 rows, 9600 x 1000: 9 us, 8 waves 10.6).
+        tiles = 2 if rows > 4 and _ceil(n, 16) >= 512 else 1
+        waves = 16 if _ceil(n, 16) <= 128 and sets <= 2 else 8
+        # As many blocks loaded together as leave the waves' shares even (5 rows,
+        # 5024 x 4099, 40 blocks: one 17 us, four 28), and whose scales fit in registers.
+        share = {u: _ceil(_ceil(blocks, u), waves) * u for u in (1, 2, 4)
+                 if u == 1 or u * tiles * max(1, sets // 2) * (1 + zeros) <= group // 16}
+        together = max(u for u in share if share[u] <= 1.1 * min(share.values()))
+    shape = {"shared": shared, "waves": waves, "tiles": tiles, "together": max(together, made), "groups": 256, "each": each,
+             **INT4_TUNE}
+    shape["together"] = max(shape["together"], 1 if eight else 4 // shape["each"])
+    block = (512 * shape["each"] + 16) * sets
+    shape.update(sets=sets, phase=min(_ceil(blocks, 4) * 4, INT4_LDS // block // 4 * 4), block=block)
     if not shape["shared"]:
-        shape["waves"] = min(shape["waves"], _ceil(k, 128 * shape["together"]))
+        shape["waves"] = min(shape["waves"], _ceil(blocks, shape["together"]))
     return shape
 
 
 def _assemble_int4(decision: DecisionView, op: Int4MatmulOp, function_name: str | None) -> KernelGroup:
     (rows, k), n = op.x.shape, op.weights.shape[0]
     eight = op.x_scales is not None
-    shape = int4_shape(rows, k, n, eight)
-    waves, tiles, shared = shape["waves"], shape["tiles"], shape["shared"]
-    held = min(rows, 16)
-    sets = 1 if eight else _ceil(held, 4)  # matrix instructions' rows: 16 of x, or 4 of x in four digits each
-    each = 4 if eight or held > 2 else held
-    made = 1 if eight else 4 // each  # blocks of x made into digits at once
-    together = max(shape["together"], made)
+    shape = int4_shape(rows, k, n, op.group, eight, op.zeros is not None)
+    waves, tiles, shared, sets = shape["waves"], shape["tiles"], shape["shared"], shape["sets"]
     sig = _Signature()
     args = (
         "nullptr" if eight else sig.add("x", op.x),
@@ -279,20 +302,20 @@ def _assemble_int4(decision: DecisionView, op: Int4MatmulOp, function_name: str 
         "mt_lds",
     )
     if shared:
-        lds = _ceil(k, 128 * made) * made * (512 * each + 16) * sets
+        lds = shape["phase"] * shape["block"]
     else:
         lds = max(0 if eight else 2048 * sets * waves, waves * tiles * 256 * (4 if eight else sets))
     frag = ServingFragment(
         "mt_matmul_int4",
-        (eight, shared, each, sets, k, n, op.group, op.zeros is not None, tiles, together, waves, op.x.row_stride,
-         op.x.col_stride),
+        (eight, shared, shape["phase"], shape["each"], sets, k, n, op.group, op.zeros is not None, tiles, shape["together"],
+         waves, op.x.row_stride, op.x.col_stride),
         args,
         lds_bytes=lds,
         name="int4_matmul",
     )
     groups = _ceil(n, 16 * tiles)
     if shared:
-        groups = min(_ceil(groups, waves), shape.get("groups", 512))
+        groups = min(_ceil(groups, waves), shape["groups"])
     return _group(decision, sig, frag, function_name or f"int4_matmul_{op.y.name}", {"M": rows}, (groups, _ceil(rows, 16), 1),
                   64 * waves)
 

@@ -376,5 +376,5 @@ def test_launch_rules_stay_within_what_the_kernels_take():
         for k in (32, 128, 4096, 16384):
             for n in (1, 100, 4096, 131072):
                 for eight in (False, True):
-                    shape = int4_shape(rows, k, n, eight)
+                    shape = int4_shape(rows, k, n, 32, eight, True)
                     assert 1 <= shape["waves"] <= 16 and shape["tiles"] in (1, 2, 4) and shape["together"] in (1, 2, 4)
