@@ -38,7 +38,7 @@ MT_INLINE mt_f32x4 mt_row4(const float* row, unsigned c) {
 template <unsigned COLS>
 MT_INLINE void mt_put_row4(float* row, unsigned c, mt_f32x4 v) {
     if (COLS % 4u == 0u || c + 4u <= COLS) {
-        *reinterpret_cast<mt_f32x4u*>(row + c) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<mt_f32x4u*>(row + c));
         return;
     }
 #pragma unroll
@@ -52,7 +52,8 @@ MT_INLINE void mt_put_row4(float* row, unsigned c, mt_f32x4 v) {
 //
 // T lanes (a power of two of at least 64) share a row, which they keep in PER
 // float4s each, so x and the residual are read once; rows longer than that
-// (PER 0) are read again for each pass.  Squares, the mean and y are in 64
+// (PER 0) are read again for each pass.  Outputs go past the caches (4096 rows of 4096
+// with a residual and 8 bits: 47 -> 44 us).  Squares, the mean and y are in 64
 // bits: HBM bounds the kernel many times over, no square overflows, y is
 // rounded once, and q falls on the side of its border that the formula says.
 // A row with a value that is not finite has no scale: it is stored as zeros
@@ -173,32 +174,40 @@ MT_INLINE void mt_rms_norm(const float* x, const float* res, const float* w, dou
 }
 
 // ---------------------------------------------------------------------------
-// y[r, c] = q[r, c] * s[r].  The matrix is dense, so lanes take 16 elements of
-// the flat array each, aligned whatever the row length.
+// y[r, c] = q[r, c] * s[r].  The matrix is dense, so lanes take four elements of the
+// flat array at a time, aligned whatever the row length; a wave's stores are
+// contiguous, and its four loads are on the way together.
 // ---------------------------------------------------------------------------
 
 template <unsigned COLS>
 MT_INLINE void mt_dequantize(const signed char* q, const float* s, float* y, size_t n) {
-    const size_t at = ((size_t)blockIdx.x * 256u + threadIdx.x) * 16u;
-    if (at >= n) return;
-    size_t row = at / COLS;
-    unsigned c = (unsigned)(at - row * COLS);
-    if (at + 16u <= n) {
-        const mt_u32x4 v = *reinterpret_cast<const mt_u32x4*>(q + at);
-        float scale = s[row];
+    const size_t base = (size_t)blockIdx.x * 4096u + 4u * threadIdx.x;
+    unsigned v[4];
+    float scale[4];
 #pragma unroll
-        for (unsigned i = 0; i < 4u; ++i) {
+    for (unsigned i = 0; i < 4u; ++i) {
+        const size_t at = base + 1024u * i;
+        v[i] = 0u, scale[i] = 0.f;
+        if (at + 4u <= n) {
+            v[i] = *reinterpret_cast<const unsigned*>(q + at);
+            scale[i] = s[at / COLS];
+        }
+    }
+#pragma unroll
+    for (unsigned i = 0; i < 4u; ++i) {
+        const size_t at = base + 1024u * i;
+        if (at + 4u <= n) {
             mt_f32x4 o;
 #pragma unroll
             for (unsigned j = 0; j < 4u; ++j) {
-                if (c == COLS) c = 0u, scale = s[++row];
-                o[j] = (float)(int)(signed char)(v[i] >> (8u * j)) * scale;
-                ++c;
+                float by = scale[i];
+                if (COLS % 4u != 0u && (at + j) / COLS != at / COLS) by = s[(at + j) / COLS];
+                o[j] = (float)(int)(signed char)(v[i] >> (8u * j)) * by;
             }
-            mt_st4(y + at + 4u * i, o);
+            mt_st4_nt(y + at, o);
+        } else {
+            for (size_t e = at; e < n; ++e) y[e] = (float)(int)q[e] * s[e / COLS];
         }
-    } else {
-        for (size_t i = at; i < n; ++i) y[i] = (float)(int)q[i] * s[i / COLS];
     }
 }
 
@@ -330,36 +339,70 @@ MT_INLINE void mt_cache_write(const float* k, const float* v, const int* slots, 
     constexpr unsigned long long ALL = (unsigned long long)PAGES * PS;
     constexpr unsigned SLOTS = ALL > 0x80000000ull ? 0x80000000u : (unsigned)ALL;
     constexpr unsigned NC = (D + 63u) / 64u;
-    const unsigned t0 = blockIdx.x * TB;
-    unsigned mine[TB], hit = 0u;
-#pragma unroll
-    for (unsigned i = 0; i < TB; ++i) mine[i] = t0 + i < tokens ? (unsigned)slots[t0 + i] : 0xFFFFFFFFu;
+    constexpr unsigned ROWS = TB * 2u * HK, MANY = ROWS >= 64u ? 4u : 1u;  // rows whose loads are on the way together
+    const unsigned t0 = blockIdx.x * TB, j = threadIdx.x & 15u;
+    unsigned lost = 0u;
     if (threadIdx.x == 0u) *dead = 0u;
-    for (unsigned j = t0 + 1u + threadIdx.x; j < tokens; j += 256u) {
-        const unsigned other = (unsigned)slots[j];
+    for (unsigned first = 0; first < ROWS; first += 16u * MANY) {
+        mt_f32x4 x[MANY][NC];
+        unsigned slot[MANY];
 #pragma unroll
-        for (unsigned i = 0; i < TB; ++i)
-            if (other == mine[i] && j > t0 + i) hit |= 1u << i;
-    }
-    __syncthreads();
-    if (hit) atomicOr(dead, hit);
-    __syncthreads();
-    const unsigned lost = *dead, j = threadIdx.x & 15u;
-    for (unsigned at = threadIdx.x >> 4; at < TB * 2u * HK; at += 16u) {
-        const unsigned i = at / (2u * HK), part = (at / HK) % 2u, head = at % HK, t = t0 + i;
-        // (no mine[i]: an index that is not constant would put the array into memory)
-        const unsigned slot = t < tokens ? (unsigned)slots[t] : 0xFFFFFFFFu;
-        const bool live = slot < SLOTS && !((lost >> i) & 1u);
-        mt_f32x4 x[NC];
+        for (unsigned u = 0; u < MANY; ++u) {
+            const unsigned at = first + 16u * u + (threadIdx.x >> 4), part = at / HK % 2u, head = at % HK;
+            const unsigned t = t0 + at / (2u * HK);
+            const bool in = at < ROWS && t < tokens;
+            slot[u] = in ? (unsigned)slots[t] : 0xFFFFFFFFu;
 #pragma unroll
-        for (unsigned c = 0; c < NC; ++c) {
-            x[c] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-            const unsigned d = 64u * c + 4u * j;
-            if (live && (D % 64u == 0u || d < D))
-                x[c] = part ? mt_row4<HK * D, VCS>(v + (size_t)t * VRS, head * D + d)
-                            : mt_row4<HK * D, KCS>(k + (size_t)t * KRS, head * D + d);
+            for (unsigned c = 0; c < NC; ++c) {
+                x[u][c] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                const unsigned d = 64u * c + 4u * j;
+                if (in && (D % 64u == 0u || d < D))
+                    x[u][c] = part ? mt_row4<HK * D, VCS>(v + (size_t)t * VRS, head * D + d)
+                                   : mt_row4<HK * D, KCS>(k + (size_t)t * KRS, head * D + d);
+            }
         }
-        mt_cache_put<KIND, HK, PS, D, PAGES>(cache, x, j, live, slot / PS, part, head, slot % PS);
+        if (first == 0u) {  // while the first rows are on the way
+            unsigned mine[TB], hit = 0u;
+            bool same[TB];
+#pragma unroll
+            for (unsigned i = 0; i < TB; ++i) mine[i] = t0 + i < tokens ? (unsigned)slots[t0 + i] : 0xFFFFFFFFu, same[i] = false;
+            // Slots behind this workgroup's, four at a time (eight loads on the way): one
+            // comparison for each of its tokens.  Then the ones around its own and the last.
+            const unsigned from = (t0 + TB + 3u) / 4u, whole = tokens / 4u;
+            for (unsigned q0 = from + threadIdx.x; q0 < whole; q0 += 8u * 256u) {
+                mt_u32x4 s4[8];
+#pragma unroll
+                for (unsigned u = 0; u < 8u; ++u) {
+                    s4[u] = mt_u32x4{0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+                    if (q0 + 256u * u < whole) s4[u] = reinterpret_cast<const mt_u32x4*>(slots)[q0 + 256u * u];
+                }
+#pragma unroll
+                for (unsigned u = 0; u < 8u; ++u)
+#pragma unroll
+                    for (unsigned e = 0; e < 4u; ++e)
+#pragma unroll
+                        for (unsigned i = 0; i < TB; ++i) same[i] = same[i] | (s4[u][e] == mine[i]);
+            }
+            const auto look = [&](unsigned at) {
+                const unsigned other = at < tokens ? (unsigned)slots[at] : 0xFFFFFFFFu;
+#pragma unroll
+                for (unsigned i = 0; i < TB; ++i) same[i] = same[i] | (other == mine[i] && at > t0 + i);
+            };
+            if (threadIdx.x < TB + 3u) look(t0 + 1u + threadIdx.x);
+            if (threadIdx.x < 4u && 4u * whole + threadIdx.x > t0) look(4u * whole + threadIdx.x);
+#pragma unroll
+            for (unsigned i = 0; i < TB; ++i) hit |= same[i] ? 1u << i : 0u;
+            __syncthreads();
+            if (hit) atomicOr(dead, hit);
+            __syncthreads();
+            lost = *dead;
+        }
+#pragma unroll
+        for (unsigned u = 0; u < MANY; ++u) {
+            const unsigned at = first + 16u * u + (threadIdx.x >> 4);
+            const bool live = slot[u] < SLOTS && !((lost >> (at / (2u * HK) % 32u)) & 1u);
+            mt_cache_put<KIND, HK, PS, D, PAGES>(cache, x[u], j, live, slot[u] / PS, at / HK % 2u, at % HK, slot[u] % PS);
+        }
     }
 }
 
@@ -371,27 +414,49 @@ MT_INLINE void mt_cache_read(const unsigned char* cache, const int* slots, float
     constexpr unsigned long long ALL = (unsigned long long)PAGES * PS;
     constexpr unsigned SLOTS = ALL > 0x80000000ull ? 0x80000000u : (unsigned)ALL;
     constexpr unsigned NC = (D + 63u) / 64u;
-    const size_t at = (size_t)blockIdx.x * 16u + (threadIdx.x >> 4);
+    constexpr unsigned MANY = 4u;  // rows whose loads are on the way together
     const unsigned j = threadIdx.x & 15u;
-    const size_t r = at / (2u * HK);
-    if (r >= rows) return;
-    const unsigned part = (unsigned)(at / HK) % 2u, head = (unsigned)(at % HK);
-    const unsigned slot = (unsigned)slots[r];
-    const bool live = slot < SLOTS;
-    const unsigned page = live ? slot / PS : 0u, in = live ? slot % PS : 0u;
-    const unsigned char* from = cache + C::row(page, part, head, in);
-    float s = 1.f;
-    if constexpr (KIND != 0) s = *reinterpret_cast<const float*>(cache + C::scale(page, part, head, in));
-    float* to = (part ? v : k) + r * (HK * D) + head * D;
+    unsigned slot[MANY], w[MANY][NC];
+    mt_f32x4 x[MANY][NC];
+    float s[MANY];
+    bool live[MANY];
 #pragma unroll
-    for (unsigned c = 0; c < NC; ++c) {
-        const unsigned d = 64u * c + 4u * j;
-        if (D % 64u != 0u && d >= D) continue;
-        mt_f32x4 x;
-        if constexpr (KIND == 0) x = mt_ld4(reinterpret_cast<const float*>(from) + d);
-        else x = mt_held4<KIND>(*reinterpret_cast<const unsigned*>(from + d)) * s;
-        if (!live) x = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-        mt_st4(to + d, x);
+    for (unsigned u = 0; u < MANY; ++u) {
+        const size_t at = ((size_t)blockIdx.x * MANY + u) * 16u + (threadIdx.x >> 4), r = at / (2u * HK);
+        slot[u] = r < rows ? (unsigned)slots[r] : 0xFFFFFFFFu;
+    }
+#pragma unroll
+    for (unsigned u = 0; u < MANY; ++u) {
+        const size_t at = ((size_t)blockIdx.x * MANY + u) * 16u + (threadIdx.x >> 4);
+        const unsigned part = (unsigned)(at / HK) % 2u, head = (unsigned)(at % HK);
+        live[u] = slot[u] < SLOTS;
+        const unsigned page = live[u] ? slot[u] / PS : 0u, in = live[u] ? slot[u] % PS : 0u;
+        const unsigned char* from = cache + C::row(page, part, head, in);
+        s[u] = 1.f;
+        if constexpr (KIND != 0) s[u] = *reinterpret_cast<const float*>(cache + C::scale(page, part, head, in));
+#pragma unroll
+        for (unsigned c = 0; c < NC; ++c) {
+            const unsigned d = 64u * c + 4u * j;
+            if (D % 64u != 0u && d >= D) continue;
+            if constexpr (KIND == 0) x[u][c] = mt_ld4(reinterpret_cast<const float*>(from) + d);
+            else w[u][c] = *reinterpret_cast<const unsigned*>(from + d);
+        }
+    }
+#pragma unroll
+    for (unsigned u = 0; u < MANY; ++u) {
+        const size_t at = ((size_t)blockIdx.x * MANY + u) * 16u + (threadIdx.x >> 4), r = at / (2u * HK);
+        if (r >= rows) return;
+        float* to = ((unsigned)(at / HK) % 2u ? v : k) + r * (HK * D) + (unsigned)(at % HK) * D;
+#pragma unroll
+        for (unsigned c = 0; c < NC; ++c) {
+            const unsigned d = 64u * c + 4u * j;
+            if (D % 64u != 0u && d >= D) continue;
+            mt_f32x4 o;
+            if constexpr (KIND == 0) o = x[u][c];
+            else o = mt_held4<KIND>(w[u][c]) * s[u];
+            if (!live[u]) o = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+            mt_st4_nt(to + d, o);
+        }
     }
 }
 
@@ -501,6 +566,25 @@ MT_INLINE float mt_fold_g(float v, OP op) {
     return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// The parts of a launch in the workspace, at device scope.
+struct mt_parts : mt_sn_part {
+    using mt_sn_part::mt_sn_part;
+    MT_INLINE void put1(unsigned at, float v) const {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, at, 0, 16);
+    }
+    MT_INLINE float get1(unsigned at) const { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 16)); }
+};
+
+// A part (its maximum, sum of weights and sums) added to the joined ones, whose maximum is `top`.
+MT_INLINE void mt_join(mt_f32x4& value, float& total, float& empty, float top, float m, float l, mt_f32x4 v) {
+    const bool none = m == -INFINITY;
+    const float u = none ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    empty += none ? l : 0.f;
+    total += none ? 0.f : u * l;
+#pragma unroll
+    for (unsigned e = 0; e < 4u; ++e) value[e] += none ? 0.f : u * v[e];
+}
+
 // The units of a launch: which sequence and head they belong to, and which
 // workgroup has them.  Whole waves call its functions; their results are uniform.
 template <unsigned ROWS, unsigned STEP, unsigned MOST, unsigned HEADS, unsigned GROUPS>
@@ -568,7 +652,7 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     constexpr unsigned SETS = WIDE ? 1u : (HELD + 3u) / 4u;                // MFMA column sets
     constexpr unsigned VK = WIDE ? 4u : D % 64u == 0u ? 16u : D % 32u == 0u ? 8u : 4u, NJ = D / (4u * VK);
     constexpr unsigned VV = WIDE || D <= 64u ? 4u : 8u, NV = (D + 16u * VV - 1u) / (16u * VV);
-    constexpr unsigned KW = VK * ITEM / 4u, VW = VV * ITEM / 4u, FLOATS = HELD * (D + 2u);
+    constexpr unsigned KW = VK * ITEM / 4u, VW = VV * ITEM / 4u, FLOATS = (HELD * (D + 2u) + 3u) / 4u * 4u;
     constexpr unsigned STEP = TILE * WAVES;
     constexpr bool ONE_PAGE = PS % 16u == 0u;  // 16 positions lie in one page
     const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
@@ -588,22 +672,12 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     units.init(lengths, gridDim.z <= BATCH ? GROUPS : 1u);
     if (blockIdx.x >= units.workgroups) return;
     const typename U::N end = units.first(blockIdx.x + 1u);
-    for (typename U::N unit = units.first(blockIdx.x); unit < end;) {
-    typename U::N before;
-    unsigned steps;
-    const unsigned b = units.find(unit, before, steps);
-    const unsigned in = (unsigned)(unit - before);  // from the sequence's first unit
-    const unsigned pair = in / steps, step = in % steps, part = pair % PARTS, head = pair / PARTS;
-    const typename U::N begins = unit - step;  // the head's first unit
-    const unsigned taken = end - unit < steps - step ? (unsigned)(end - unit) : steps - step;
-    const bool entire = taken == steps;
-    unit += taken;
-    const unsigned len = units.length(lengths[b]);
-    const unsigned first = step * STEP;
-    const unsigned last = len < (step + taken) * STEP ? len : (step + taken) * STEP;
-    const unsigned tiles = (last - first + TILE - 1u) / TILE;
 
-    const int* table = pages + (size_t)b * WIDTH;
+    // The range's current piece: `taken` of the `steps` of a sequence's head, from `step` on
+    // (positions first .. last - 1), the head's first unit being `begins`.
+    typename U::N unit = units.first(blockIdx.x), begins;
+    unsigned b, head, part, step, steps, taken, first, last, tiles;
+    const int* table;
     // The page of row n of block `bi` of a tile (of the block, where it lies in one).
     const auto page_of = [&](unsigned ti, unsigned bi) -> int {
         const unsigned t0 = first + TILE * ti + 16u * bi;
@@ -653,14 +727,50 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     };
 
     int page[BLOCKS], page_next[BLOCKS];
+    // Opens the piece at `unit`, its first tile on the way.
+    const auto open = [&]() {
+        typename U::N before;
+        b = units.find(unit, before, steps);
+        const unsigned in = (unsigned)(unit - before), pair = in / steps;
+        step = in % steps, part = pair % PARTS, head = pair / PARTS;
+        begins = unit - step;
+        taken = end - unit < steps - step ? (unsigned)(end - unit) : steps - step;
+        unit += taken;
+        const unsigned len = units.length(lengths[b]);
+        first = step * STEP;
+        last = len < (step + taken) * STEP ? len : (step + taken) * STEP;
+        tiles = (last - first + TILE - 1u) / TILE;
+        table = pages + (size_t)b * WIDTH;
 #pragma unroll
-    for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = wave < tiles ? page_of(wave, bi) : -1, page_next[bi] = -1;
-    if (wave < tiles) {
-        load_k(wave, page);
-        load_v(wave, page);
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = wave < tiles ? page_of(wave, bi) : -1, page_next[bi] = -1;
+        if (wave < tiles) {
+            load_k(wave, page);
+            load_v(wave, page);
 #pragma unroll
-        for (unsigned bi = 0; bi < BLOCKS; ++bi) page_next[bi] = page_of(wave + WAVES, bi);
-    }
+            for (unsigned bi = 0; bi < BLOCKS; ++bi) page_next[bi] = page_of(wave + WAVES, bi);
+        }
+    };
+
+    // Slot 2 w of the workspace is the part of workgroup w that began before it, 2 w + 1
+    // the part that begins in it: [HELD][D] sums, [HELD] of m, [HELD] of l.  Four dims a
+    // lane, written and read at device scope.
+    float* slots = ws + MT_WS_HEAD + (size_t)blockIdx.z * gridDim.x * 2u * FLOATS;
+    constexpr unsigned QUADS = HELD * D / 4u, LANES = 64u * WAVES;
+    // Lanes that share four dims of a head when the parts of other workgroups are joined,
+    // and parts of each whose loads are on the way together.
+    constexpr unsigned SHARED = QUADS * WAVES <= LANES ? WAVES : LANES / QUADS > 0u ? LANES / QUADS : 1u;
+    constexpr unsigned DEEP = SHARED > 2u ? 4u : 16u;
+    const auto put = [&](unsigned b_, unsigned head_, unsigned part_, unsigned at, mt_f32x4 value, float top, float total) {
+        const unsigned h = at / (D / 4u);
+        if (part_ * HELD + h >= SHARE) return;
+        const float by = 1.0f / total, none = total > 0.f ? NAN : 0.f;
+        mt_f32x4 r = value * by;
+        if (top == -INFINITY) r = mt_f32x4{none, none, none, none};
+        mt_st4(o + ((size_t)b_ * HK * SHARE + head_ * SHARE + part_ * HELD + h) * D + 4u * (at % (D / 4u)), r);
+    };
+
+    open();
+    for (;;) {
 
     // q, times the scale, as the MFMAs take it: dim d is element d % VK % KO of operand
     // (d / (4 VK), d % VK / KO) in the lanes of g = d / VK % 4; fp32 in column h, or the
@@ -863,6 +973,12 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = page_next[bi], page_next[bi] = page_after[bi];
     }
 
+    // The next piece's first tile is on the way while this one's waves meet.
+    const unsigned b_ = b, head_ = head, part_ = part, steps_ = steps;
+    const typename U::N begins_ = begins;
+    const bool opening = step == 0u, entire = taken == steps, again = unit < end;
+    if (again) open();
+
     // A part weighs 2^(m - the largest m); one whose scores are all -inf weighs nothing
     // and says in l whether it has positions: a softmax over such scores alone is 0 / 0,
     // one over no positions gives zeros.
@@ -893,82 +1009,78 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     }
     __syncthreads();
 
-    // Slot 2 w of the workspace is the part of workgroup w that began before it, 2 w + 1
-    // the part that begins in it.
-    float* slots = ws + MT_WS_HEAD + (size_t)blockIdx.z * gridDim.x * 2u * FLOATS;
-    float* mine = slots + (size_t)(2u * blockIdx.x + (step == 0u ? 1u : 0u)) * FLOATS;
-    for (unsigned at = threadIdx.x; at < HELD * D; at += 64u * WAVES) {
-        const unsigned h = at / D, d = at % D;
-        float top = -INFINITY, empty = 0.f, total = 0.f, value = 0.f;
+#pragma unroll 1
+    for (bool others = false;; others = true) {
+        // The waves' parts, or those of the workgroups as SHARED lanes joined them.
+        const mt_parts mine(slots + (size_t)(2u * blockIdx.x + (opening ? 1u : 0u)) * FLOATS, FLOATS * 4u);
+#pragma unroll 1
+        for (unsigned at = threadIdx.x; at < QUADS; at += LANES) {
+            const unsigned h = at / (D / 4u);
+            float top = -INFINITY, empty = 0.f, total = 0.f;
+            mt_f32x4 value = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (unsigned w = 0; w < WAVES; ++w) top = __builtin_fmaxf(top, ms[w * HELD + h]);
+            for (unsigned w = 0; w < WAVES; ++w) top = __builtin_fmaxf(top, ms[w * HELD + h]);
 #pragma unroll
-        for (unsigned w = 0; w < WAVES; ++w) {
-            const float mw = ms[w * HELD + h], lw = ls[w * HELD + h], v = sums[(w * HELD + h) * D + d];
-            const bool none = mw == -INFINITY;
-            const float u = __builtin_amdgcn_exp2f(mw - top);
-            empty += none ? lw : 0.f;
-            total += none ? 0.f : u * lw;
-            value += none ? 0.f : u * v;
-        }
-        if (top == -INFINITY) total = empty;
-        if (!entire) {
-            mt_sn_put(mine + at, value);
-            if (d == 0u) {
-                mt_sn_put(mine + HELD * D + h, top);
-                mt_sn_put(mine + HELD * D + HELD + h, total);
+            for (unsigned w = 0; w < WAVES; ++w)
+                mt_join(value, total, empty, top, ms[w * HELD + h], ls[w * HELD + h],
+                        *reinterpret_cast<const mt_f32x4*>(sums + w * HELD * D + 4u * at));
+            if (top == -INFINITY) total = empty;
+            if (entire || others) {
+                put(b_, head_, part_, at, value, top, total);
+            } else {
+                mine.put(16u * at, value);
+                if (at % (D / 4u) == 0u) {
+                    mine.put1(4u * (HELD * D + h), top);
+                    mine.put1(4u * (HELD * D + HELD + h), total);
+                }
             }
-        } else if (part * HELD + h < SHARE) {
-            const float r = top == -INFINITY ? (total > 0.f ? NAN : 0.f) : value / total;
-            o[((size_t)b * HK * SHARE + head * SHARE + part * HELD + h) * D + d] = r;
         }
-    }
-    if (entire) {
-        __syncthreads();  // (the next unit's waves write where this one's are read)
-        continue;
-    }
+        if (entire || others) break;
 
-    // The last workgroup of the sequence's head to arrive joins the parts.
-    const unsigned from = units.owner(begins), active = units.owner(begins + steps - 1u) - from + 1u;
-    unsigned* counter = reinterpret_cast<unsigned*>(ws) + blockIdx.z * gridDim.x + from;
-    if (mt_sn_arrive(counter, active, flag)) {
-        const auto slot = [&](unsigned i) { return slots + (size_t)(2u * (from + i) + (i == 0u ? 1u : 0u)) * FLOATS; };
-        for (unsigned at = threadIdx.x; at < HELD * D; at += 64u * WAVES) {
-            const unsigned h = at / D, d = at % D;
-            float top = -INFINITY, empty = 0.f, total = 0.f, value = 0.f;
-            for (unsigned i0 = 0; i0 < active; i0 += 16u) {  // 16 parts' loads at a time, one latency
-                float pm[16], pl[16], pv[16], most = top;
+        // The last workgroup of the sequence's head to arrive joins the parts.
+        const unsigned from = units.owner(begins_), parts = units.owner(begins_ + steps_ - 1u) - from + 1u;
+        unsigned* counter = reinterpret_cast<unsigned*>(ws) + blockIdx.z * gridDim.x + from;
+        if (!mt_sn_arrive(counter, parts, flag)) break;
+        const mt_parts all_parts(slots, gridDim.x * 2u * FLOATS * 4u);
+        const unsigned who = SHARED > 1u ? threadIdx.x / QUADS : 0u;
+        for (unsigned at = SHARED > 1u ? threadIdx.x % QUADS : threadIdx.x; at < QUADS && who < SHARED; at += LANES) {
+            const unsigned h = at / (D / 4u);
+            float top = -INFINITY, empty = 0.f, total = 0.f;
+            mt_f32x4 value = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (unsigned i0 = who; i0 < parts; i0 += DEEP * SHARED) {
+                float pm[DEEP], pl[DEEP], most = top;
+                mt_f32x4 pv[DEEP];
 #pragma unroll
-                for (unsigned k = 0; k < 16u; ++k) {
-                    const float* p = slot(i0 + k < active ? i0 + k : i0);
-                    pm[k] = mt_sn_get(p + HELD * D + h);
-                    pl[k] = mt_sn_get(p + HELD * D + HELD + h);
-                    pv[k] = mt_sn_get(p + at);
+                for (unsigned k = 0; k < DEEP; ++k) {
+                    const unsigned i = i0 + k * SHARED < parts ? i0 + k * SHARED : i0;
+                    const unsigned p = (2u * (from + i) + (i == 0u ? 1u : 0u)) * FLOATS * 4u;
+                    pm[k] = all_parts.get1(p + 4u * (HELD * D + h));
+                    pl[k] = all_parts.get1(p + 4u * (HELD * D + HELD + h));
+                    pv[k] = all_parts.get(p + 16u * at);
                 }
 #pragma unroll
-                for (unsigned k = 0; k < 16u; ++k) most = __builtin_fmaxf(most, pm[k]);
+                for (unsigned k = 0; k < DEEP; ++k) most = __builtin_fmaxf(most, pm[k]);
                 if (most > top) {
                     const float by = __builtin_amdgcn_exp2f(top - most);
-                    total *= by, value *= by;
+                    total *= by, value = value * by;
                     top = most;
                 }
 #pragma unroll
-                for (unsigned k = 0; k < 16u; ++k) {
-                    if (i0 + k >= active) continue;
-                    const bool none = pm[k] == -INFINITY;
-                    const float u = none ? 0.f : __builtin_amdgcn_exp2f(pm[k] - top);
-                    empty += none ? pl[k] : 0.f;
-                    total += none ? 0.f : u * pl[k];
-                    value += none ? 0.f : u * pv[k];
-                }
+                for (unsigned k = 0; k < DEEP; ++k)
+                    if (k == 0u || i0 + k * SHARED < parts) mt_join(value, total, empty, top, pm[k], pl[k], pv[k]);
             }
-            if (part * HELD + h < SHARE) {
-                const float r = top == -INFINITY ? (empty > 0.f ? NAN : 0.f) : value / total;
-                o[((size_t)b * HK * SHARE + head * SHARE + part * HELD + h) * D + d] = r;
+            *reinterpret_cast<mt_f32x4*>(sums + who * HELD * D + 4u * at) = value;
+            if (at % (D / 4u) == 0u) {
+                ms[who * HELD + h] = top;
+                ls[who * HELD + h] = top == -INFINITY ? empty : total;
             }
         }
+        for (unsigned at = threadIdx.x; at < (WAVES - SHARED) * HELD; at += LANES)
+            ms[SHARED * HELD + at] = -INFINITY, ls[SHARED * HELD + at] = 0.f;
+        __syncthreads();
     }
-    __syncthreads();
+    if (!again) return;
     }
 }
 

@@ -361,9 +361,8 @@ def test_int4_kernels_compile(rows, k, n, group, eight):
 
 
 def test_launch_rules_stay_within_what_the_kernels_take():
-    for rows in (1, 7, 300, 100000):
-        for cols in (1, 63, 64, 255, 1024, 4096, 16384, 100000):
-            assert norm_lanes(rows, cols) in (64, 256, 1024)
+    for cols in (1, 63, 64, 255, 1024, 4096, 16384, 100000):
+        assert norm_lanes(cols) in (64, 256, 1024)
     for pairs in (1, 8, 256, 1022, 1023, 5000):
         for capacity in (1, 16, 100, 2048, 131072, 2**31 - 2048):
             for batch in (1, 3, 32, 1023, 5000):
