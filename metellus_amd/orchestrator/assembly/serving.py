@@ -238,7 +238,7 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
 # ---------------------------------------------------------------------------
 
 
-INT4_TUNE: dict = {}  # tuning overrides of ``int4_shape``
+INT4_WORKGROUPS = 256  # one for each compute unit
 INT4_LDS = 131072  # bytes of digits at a time, where the waves share them
 
 
@@ -257,27 +257,29 @@ def int4_shape(rows: int, k: int, n: int, group: int, eight: bool, zeros: bool) 
     shared = _ceil(n, 16) >= 1536
     blocks = _ceil(k, 128)
     made = 1 if eight else 4 // each  # blocks of x made into digits at once
-    if shared:
-        tiles, waves, together = 1, 8, 4
-    else:
-        # Two tiles a wave halve the work on x, where two still leave a workgroup to each
-        # compute unit (7 rows, 8192 x 8192: 21 us, one tile 27); 16 waves where one does
-        # not (3 rows, 9600 x 1000: 9 us, 8 waves 10.6).
-        tiles = 2 if rows > 4 and _ceil(n, 16) >= 512 else 1
-        waves = 16 if _ceil(n, 16) <= 128 and sets <= 2 else 8
-        # As many blocks loaded together as leave the waves' shares even (5 rows,
-        # 5024 x 4099, 40 blocks: one 17 us, four 28), and whose scales fit in registers.
-        share = {u: _ceil(_ceil(blocks, u), waves) * u for u in (1, 2, 4)
-                 if u == 1 or u * tiles * max(1, sets // 2) * (1 + zeros) <= group // 16}
-        together = max(u for u in share if share[u] <= 1.1 * min(share.values()))
-    shape = {"shared": shared, "waves": waves, "tiles": tiles, "together": max(together, made), "groups": 256, "each": each,
-             **INT4_TUNE}
-    shape["together"] = max(shape["together"], 1 if eight else 4 // shape["each"])
-    block = (512 * shape["each"] + 16) * sets
-    shape.update(sets=sets, phase=min(_ceil(blocks, 4) * 4, INT4_LDS // block // 4 * 4), block=block)
-    if not shape["shared"]:
-        shape["waves"] = min(shape["waves"], _ceil(blocks, shape["together"]))
-    return shape
+    tiles, waves, together = 1, 8, 4
+    if not shared:
+        # Two tiles a wave halve the work on x, once one is more than a workgroup to each
+        # compute unit (5 rows, 5024 x 4099: 15 us, one tile 17; 16 rows 24 and 35; 8 bits,
+        # 16 rows, 11008 x 8192: 15 and 19; up to 4 rows one tile is as fast or faster).
+        # Sixteen waves where it is not (1 row, 11008 x 4096: 9.5 us, 8 waves 11.2).
+        many = _ceil(n, 16) > INT4_WORKGROUPS
+        tiles = 2 if rows > 4 and many else 1
+        waves = 16 if not many and sets <= 2 else 8
+        if eight:  # (1 row, 8192 x 11008: groups of 128 one block 17.3 us, two 15.3; of 32, 20.6 and 24.2)
+            together = 1 if group == 32 else 2
+        elif rows <= 2:  # (2 rows, 8192 x 11008: two blocks 16.8 us, four 18.2)
+            together = made
+        else:
+            # As many as leave the waves' shares even (5 rows, 5024 x 4099, 40 blocks: one
+            # 17 us, four 29), and whose scales fit in registers.
+            share = {u: _ceil(_ceil(blocks, u), waves) * u for u in (1, 2, 4)
+                     if u == 1 or u * tiles * max(1, sets // 2) * (1 + zeros) <= group // 16}
+            together = max(u for u in share if share[u] <= 1.1 * min(share.values()))
+        waves = min(waves, _ceil(blocks, together))
+    block = (512 * each + 16) * sets
+    return {"shared": shared, "waves": waves, "tiles": tiles, "together": together, "each": each, "sets": sets,
+            "phase": min(_ceil(blocks, 4) * 4, INT4_LDS // block // 4 * 4), "block": block}
 
 
 def _assemble_int4(decision: DecisionView, op: Int4MatmulOp, function_name: str | None) -> KernelGroup:
@@ -311,7 +313,7 @@ def _assemble_int4(decision: DecisionView, op: Int4MatmulOp, function_name: str 
     )
     groups = _ceil(n, 16 * tiles)
     if shared:
-        groups = min(_ceil(groups, waves), shape["groups"])
+        groups = min(_ceil(groups, waves), INT4_WORKGROUPS)
     return _group(decision, sig, frag, function_name or f"int4_matmul_{op.y.name}", {"M": rows}, (groups, _ceil(rows, 16), 1),
                   64 * waves)
 
