@@ -107,7 +107,7 @@ def _assemble_norm(decision: DecisionView, op: RmsNormOp, function_name: str | N
         sig.add("x", op.x),
         sig.add("residual", res),
         sig.add("weight", op.weight),
-        repr(op.eps),
+        repr(float(op.eps)),
         sig.add("sum", op.sum_out, out=True),
         "nullptr" if eight else sig.add("y", op.y, out=True),
         sig.add("y", op.y, out=True) if eight else "nullptr",
@@ -219,7 +219,7 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
     ws = WS_HEAD_BYTES + 4 * batch * groups * 2 * floats if groups > 1 else 0
     sig = _Signature()
     args = (sig.add("q", op.q), sig.add("cache", op.cache), sig.add("pages", op.pages), sig.add("lengths", op.lengths),
-            sig.add("o", op.o, out=True), f"{op.scale!r}", "mt_ws" if ws else "nullptr", "mt_lds")
+            sig.add("o", op.o, out=True), repr(float(op.scale)), "mt_ws" if ws else "nullptr", "mt_lds")
     frag = ServingFragment(
         "mt_paged_attention",
         (*_cache_template(spec), spec.pages, op.pages.shape[1], share, held, waves, groups, batch, rows,

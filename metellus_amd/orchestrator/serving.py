@@ -414,8 +414,8 @@ class PagedAttentionOp(ServingOp):
         _dense("paged_attention lengths", self.lengths)
         if self.capacity > _INT32_MAX - 1024:
             raise ValueError(f"paged_attention: a table of {self.capacity} positions; lengths are int32")
-        if not abs(self.scale) < float("inf"):
-            raise ValueError(f"paged_attention scale must be finite; got {self.scale}")
+        if not abs(self.scale) <= 2e38:  # (times log2(e) it is fp32 on the device)
+            raise ValueError(f"paged_attention scale must be finite and within 2e38; got {self.scale}")
 
     @property
     def capacity(self) -> int:

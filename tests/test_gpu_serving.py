@@ -151,8 +151,8 @@ def _int4_bound(ops: Operations) -> np.ndarray:
       steps, 2^6 steps of 2^-30 P / 16), their fma once, with zeros another fma of
       that on both terms, times s, the addition: under 8 u of sum |x| (8 + |8 - z|) |s|,
       and 2^6 * 2 max * 2^-30 |s|;
-    * adding up: a running sum of at most blocks * groups terms and 8 waves, u each of
-      the magnitude so far.
+    * adding up: a running sum of a wave's groups, then of at most 16 waves that have a
+      block each at the least: under groups + 8 terms, u each of the magnitude so far.
     """
     (op,) = ops.build()
     x = np.abs(ops.uploads["x"].astype(np.float64))
@@ -206,6 +206,40 @@ def test_matmul_int4(rows, k, n, group, eight, zeros):
     got, want = run(ops).env["y"], evaluate(ops)["y"]
     assert got.shape == (rows, n) and got.dtype == np.float32
     _close(got, want, _int4_bound(ops))
+
+
+@pytest.mark.parametrize("rows, k, n, group, eight, zeros", [
+    # enough weight rows that the waves share x: one, two and more rows, k in phases,
+    # ragged, weight rows that end inside a tile, more rows than one pass takes
+    (1, 1056, 24590, 32, False, True), (2, 1152, 24577, 64, False, False), (3, 640, 33000, 128, False, True),
+    (16, 1632, 24600, 32, False, False), (16, 1664, 24576, 128, False, True), (7, 1024, 24579, 64, False, True),
+    (20, 416, 24601, 32, False, True), (16, 1632, 24600, 32, True, True), (5, 7744, 24577, 64, True, False),
+    # two tiles of weight rows a wave, with an odd number of tiles and without
+    (5, 416, 4099, 32, False, True), (16, 1056, 4128, 32, False, True), (9, 512, 8200, 128, False, False),
+    (16, 704, 4100, 64, True, True), (6, 384, 5000, 128, True, False), (33, 288, 4097, 32, True, True),
+    # sixteen waves, shares of k that differ by one, k shorter than the waves
+    (1, 5024, 2000, 32, False, True), (2, 4416, 300, 64, False, False), (4, 2592, 4096, 32, False, True),
+    (8, 3200, 500, 128, False, True), (16, 11008, 40, 64, True, False), (1, 2080, 33, 32, True, True),
+])
+def test_matmul_int4_however_it_is_cut(rows, k, n, group, eight, zeros):
+    ops = _int4(rows, k, n, group, eight, zeros, rows + k + n)
+    _close(run(ops).env["y"], evaluate(ops)["y"], _int4_bound(ops))
+
+
+@pytest.mark.parametrize("rows, n", [(1, 24577), (6, 24577), (6, 4100), (1, 100)])
+def test_matmul_int4_values_that_are_not_finite_however_it_is_cut(rows, n):
+    """Blocks at the ends and inside a wave's share of k; the row's other blocks hold
+    finite values, the row after it stays finite."""
+    ops = _int4(rows, 1696, n, 32, False, False, n)
+    x = ops.uploads["x"]
+    x[0, 3] = np.inf
+    if rows > 5:
+        x[2, 1695], x[4, 800], x[4, 1000] = np.nan, np.inf, -np.inf
+    got, want = run(ops).env["y"], evaluate(ops)["y"]
+    with np.errstate(invalid="ignore"):
+        _close(got, want, np.nan_to_num(_int4_bound(ops), nan=0.0, posinf=0.0))
+    if rows > 5:
+        assert np.all(np.isfinite(got[[1, 3, 5]])) and np.all(np.isnan(got[2]))
 
 
 def test_matmul_int4_of_a_transposed_x():
@@ -274,6 +308,7 @@ def _same_state(spec, got, want):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("pages, page_size, kv_heads, dim, tokens", [
     (1, 1, 1, 16, 1), (5, 4, 2, 48, 7), (9, 16, 8, 128, 40), (3, 20, 3, 80, 33), (40, 64, 1, 256, 2100), (7, 3, 33, 16, 5),
+    (90, 64, 4, 32, 5001), (150, 128, 2, 16, 18005),
 ])
 def test_cache_write_and_read(dtype, pages, page_size, kv_heads, dim, tokens):
     spec = KVCache(pages=pages, page_size=page_size, kv_heads=kv_heads, dim=dim, dtype=dtype)
@@ -437,6 +472,25 @@ CASES = [
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads, kv_heads, dim, page_size, width, lengths", CASES)
 def test_paged_attention(dtype, heads, kv_heads, dim, page_size, width, lengths):
+    ops = _attention(dtype, heads, kv_heads, dim, page_size, width, lengths, seed=dim + heads)
+    _close(run(ops).env["o"], evaluate(ops)["o"], _attention_bound(ops))
+
+
+MANY = [
+    # more sequences than a wave has lanes; a key head's query heads taken in parts;
+    # 16 of them with long rows; pages that end anywhere
+    (4, 2, 32, 16, 6, [(37 * i) % 97 for i in range(130)]),
+    (2, 1, 64, 8, 70, [0] * 63 + [500, 0, 3] + [1] * 62 + [560, 0]),
+    (32, 2, 256, 16, 40, [640, 100]),
+    (36, 1, 256, 9, 30, [270]),
+    (16, 1, 128, 5, 60, [300, 298, 7]),
+    (33, 1, 128, 16, 20, [320, 1]),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads, kv_heads, dim, page_size, width, lengths", MANY)
+def test_paged_attention_of_many_sequences_and_heads(dtype, heads, kv_heads, dim, page_size, width, lengths):
     ops = _attention(dtype, heads, kv_heads, dim, page_size, width, lengths, seed=dim + heads)
     _close(run(ops).env["o"], evaluate(ops)["o"], _attention_bound(ops))
 
@@ -648,6 +702,21 @@ def test_a_batch_of_split_attentions():
     programs = [_attention("float32", 4, 2, 64, 16, 128, [2048, 1000 + s], seed=s) for s in range(3)]
     for ops, got in zip(programs, run_batch(programs)):
         _close(got.env["o"], evaluate(ops)["o"], _attention_bound(ops))
+
+
+def test_a_batch_that_the_kernel_was_not_made_for():
+    """The kernel of one program launched for four: its workspace has room for one, so
+    each runs in one workgroup."""
+    programs = [_attention("int8", 4, 2, 64, 16, 128, [2048, 1000 + s], seed=s) for s in range(4)]
+    (g,) = compile_program(programs[0])
+    assert g.grid[0] > 1 and g.kernel.workspace_bytes > 0
+    envs = [_resident(ops, (g,)) for ops in programs]
+    kernel = g.kernel.batched()
+    tables = [Buffer.from_numpy(np.array([env[key].device_address for env in envs], np.uint64)) for key in g.bindings]
+    hip_backend.launch(kernel.handle, tables, g.dims, kernel.dims_slot_index, (*g.grid[:2], 4), g.threads,
+                       workspace=kernel.workspace_bytes)
+    for ops, env in zip(programs, envs):
+        _close(env["o"].numpy(ops.tensors["o"].shape, np.float32), evaluate(ops)["o"], _attention_bound(ops))
 
 
 def test_launches_that_allocate_nothing():

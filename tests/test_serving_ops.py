@@ -184,6 +184,8 @@ def test_cache_ops_refuse():
     (dict(pages="pf"), "pages must be int32"),
     (dict(lengths="slots"), "lengths must have shape"),
     (dict(scale=float("inf")), "scale must be finite"),
+    (dict(scale=float("nan")), "scale must be finite"),
+    (dict(scale=-3e38), "within 2e38"),
     (dict(pages="pt"), "must be dense"),
     (dict(cache="q"), "is not a kv cache"),
 ])
@@ -351,8 +353,7 @@ def test_cache_kernels_compile(dtype, heads, kv_heads, dim, page_size, width):
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("eight", [False, True])
 def test_int4_kernels_compile(rows, k, n, group, eight):
-    if k % group:
-        pytest.skip("groups divide the columns")
+    group = group if k % group == 0 else 32
     ops = _ops(x=((rows, k), "int8" if eight else "float32"), w=((n, k // 2), "uint8"), s=(n, k // group), z=(n, k // group),
                xs=(rows,))
     ops.matmul_int4("x", weights="w", scales="s", zeros="z", x_scales="xs" if eight else None, out="y")
