@@ -23,11 +23,12 @@ struct mt_count<false> {
     using type = unsigned long long;
 };
 
-// Elements c .. c + 3 of a row of COLS elements CS apart, 0 behind its end.
-template <unsigned COLS, unsigned CS>
+// Elements c .. c + 3 of a row of COLS elements CS apart, 0 behind its end.  NT: loads
+// that keep nothing in the caches, for rows that are read once.
+template <unsigned COLS, unsigned CS, bool NT = false>
 MT_INLINE mt_f32x4 mt_row4(const float* row, unsigned c) {
     if constexpr (CS == 1u) {
-        if (COLS % 4u == 0u || c + 4u <= COLS) return mt_ld4u(row + c);
+        if (COLS % 4u == 0u || c + 4u <= COLS) return NT ? mt_ld4u_nt(row + c) : mt_ld4u(row + c);
     }
     mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -52,8 +53,9 @@ MT_INLINE void mt_put_row4(float* row, unsigned c, mt_f32x4 v) {
 //
 // T lanes (a power of two of at least 64) share a row, which they keep in PER
 // float4s each, so x and the residual are read once; rows longer than that
-// (PER 0) are read again for each pass.  Outputs go past the caches (4096 rows of 4096
-// with a residual and 8 bits: 47 -> 44 us).  Squares, the mean and y are in 64
+// (PER 0) are read again for each pass.  What is read and written once goes past the
+// caches (4096 rows of 4096 with a residual and 8 bits: outputs 47 -> 44 us, inputs too,
+// with the pass that reads y back, 58 -> 55).  Squares, the mean and y are in 64
 // bits: HBM bounds the kernel many times over, no square overflows, y is
 // rounded once, and q falls on the side of its border that the formula says.
 // A row with a value that is not finite has no scale: it is stored as zeros
@@ -86,8 +88,8 @@ MT_INLINE void mt_rms_norm(const float* x, const float* res, const float* w, dou
     const float* xr = x + (size_t)row * XRS;
     const float* rr = RES ? res + (size_t)row * RRS : nullptr;
     const auto load = [&](unsigned c) {
-        mt_f32x4 v = mt_row4<COLS, XCS>(xr, c);
-        if constexpr (RES) v = v + mt_row4<COLS, RCS>(rr, c);
+        mt_f32x4 v = mt_row4<COLS, XCS, PER != 0u>(xr, c);
+        if constexpr (RES) v = v + mt_row4<COLS, RCS, PER != 0u>(rr, c);
         return v;
     };
     mt_f32x4 h[KEEP];
@@ -271,6 +273,42 @@ MT_INLINE float mt_step_round(float x, float s, float inv) {
     return __builtin_fminf(__builtin_fmaxf(n * st, -most), most);
 }
 
+// Four of them in the held type's bytes.
+template <int KIND>
+MT_INLINE unsigned mt_step_word_slow(mt_f32x4 v, float s, float inv) {
+    unsigned word = 0u;
+#pragma unroll 1
+    for (unsigned i = 0; i < 4u; ++i) {
+        const float q = mt_step_round<KIND>(i < 2u ? (i == 0u ? v[0] : v[1]) : (i == 2u ? v[2] : v[3]), s, inv);
+        const unsigned byte = KIND == 1 ? (unsigned)(int)q : (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
+        word |= (byte & 255u) << (8u * i);
+    }
+    return word;
+}
+
+// Four of a row's values in a held type's bytes, for a scale s of at least 2^-100 and
+// its reciprocal.  Both are off by 2^-22 of the quotient at most, so it lies between the
+// quotients by scales 2^-20 smaller and larger: where those round to the same four
+// bytes (all but one in thousands), these are it; where not, the remainders decide
+// (8192 tokens of 8 heads of 128 in e4m3: 28 us -> 22).
+template <int KIND>
+MT_INLINE unsigned mt_step_word(mt_f32x4 v, float s, float inv) {
+    const auto word = [&](float by) {
+        if constexpr (KIND == 1) {
+            unsigned b[4];  // a whole number in a float's last byte, rounded there by the addition
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i) b[i] = __float_as_uint(__builtin_fmaf(v[i], by, 12582912.0f));
+            return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u),
+                                         __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), 0x05040100u);
+        } else {
+            const unsigned lo = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[0] * by, v[1] * by, 0, false);
+            return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * by, v[3] * by, (int)lo, true);
+        }
+    };
+    const unsigned low = word(inv * (1.0f - 0x1.0p-20f));
+    return low == word(inv * (1.0f + 0x1.0p-20f)) ? low : mt_step_word_slow<KIND>(v, s, inv);
+}
+
 // One row of D values held by 16 lanes (lane j has dims 64 c + 4 j .. + 3) into
 // the cache.  `live`: whether the row is stored at all; every lane takes part
 // in the exchange of the maximum.
@@ -309,18 +347,8 @@ MT_INLINE void mt_cache_put(unsigned char* cache, const mt_f32x4 (&v)[(D + 63u) 
 #pragma unroll
         for (unsigned c = 0; c < NC; ++c) {
             if (D % 64u != 0u && 64u * c + 4u * j >= D) continue;
-            float q[4];
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i)
-                q[i] = fine && s > 0.f ? mt_step_round<KIND>(v[c][i] * up, big, inv) : 0.f;
             unsigned word = 0u;
-            if constexpr (KIND == 1) {
-#pragma unroll
-                for (unsigned i = 0; i < 4u; ++i) word |= ((unsigned)(int)q[i] & 255u) << (8u * i);
-            } else {
-                word = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-                word = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)word, true);
-            }
+            if (fine && s > 0.f) word = up == 1.0f ? mt_step_word<KIND>(v[c], s, inv) : mt_step_word_slow<KIND>(v[c] * up, big, inv);
             *reinterpret_cast<unsigned*>(to + 64u * c + 4u * j) = word;
         }
         if (j == 0u) *reinterpret_cast<float*>(cache + C::scale(page, part, head, r)) = s;
@@ -357,8 +385,8 @@ MT_INLINE void mt_cache_write(const float* k, const float* v, const int* slots, 
                 x[u][c] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
                 const unsigned d = 64u * c + 4u * j;
                 if (in && (D % 64u == 0u || d < D))
-                    x[u][c] = part ? mt_row4<HK * D, VCS>(v + (size_t)t * VRS, head * D + d)
-                                   : mt_row4<HK * D, KCS>(k + (size_t)t * KRS, head * D + d);
+                    x[u][c] = part ? mt_row4<HK * D, VCS, true>(v + (size_t)t * VRS, head * D + d)
+                                   : mt_row4<HK * D, KCS, true>(k + (size_t)t * KRS, head * D + d);
             }
         }
         if (first == 0u) {  // while the first rows are on the way
