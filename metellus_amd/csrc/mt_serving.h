@@ -493,13 +493,23 @@ MT_INLINE void mt_cache_read(const unsigned char* cache, const int* slots, float
 //
 // The work is a row of units, STEP positions each of one sequence and one key head
 // with HELD (at most 16) of the query heads that share it, sequence after sequence.
-// The lengths are known on the device alone, so the P workgroups of the launch cut
+// The lengths are known on the device alone, so the workgroups of the launch cut
 // that row into equal ranges there: a workgroup has the same share of a ragged batch
 // as the others, and a table with room for far more positions costs nothing.  Where
 // a range begins or ends inside a sequence's head, the parts go to the workspace and
-// the last workgroup to arrive joins them, in their order.
+// the last workgroup to arrive joins them, in their order.  Where the heads divide the
+// workgroups well each has a row of units of its own (SIDES of them), cut alike: the
+// heads of a page are then read at about one time (key heads of 128 in int8, 32 ragged
+// sequences: 8 heads, up to 8192 keys 64 -> 63 us; 32 heads, up to 2048 69 -> 65).
 //
-// Within a range each of the workgroup's waves takes every WAVES-th tile of positions
+// A piece is what a range has of one sequence's head.  Each costs as long as about
+// 64 KB of the cache (its q, the waves' meeting), so it counts for as many units more
+// where ranges are long (these two 65 -> 63 and 69 -> 65 us).  Its place, q and pages
+// are there before the piece ahead of it ends, whose waves load its first tiles as they
+// finish.  All of a piece's places are in scalar registers: loads of pages by lanes
+// would wait for the tiles on the way before them (78 -> 63 us).
+//
+// Within a piece each of the workgroup's waves takes every WAVES-th tile of positions
 // on its own, and they meet at the end.  With (n, g) = (lane % 16, lane / 16):
 //
 //   scores  S[position, column] = K . q by MFMAs whose rows are 16 positions:
@@ -613,17 +623,25 @@ MT_INLINE void mt_join(mt_f32x4& value, float& total, float& empty, float top, f
     for (unsigned e = 0; e < 4u; ++e) value[e] += none ? 0.f : u * v[e];
 }
 
+// A value that is the same in all lanes, in scalar registers.
+MT_INLINE unsigned mt_uniform(unsigned v) { return (unsigned)__builtin_amdgcn_readfirstlane((int)v); }
+MT_INLINE unsigned long long mt_uniform(unsigned long long v) {
+    return ((unsigned long long)mt_uniform((unsigned)(v >> 32)) << 32) | mt_uniform((unsigned)v);
+}
+
 // The units of a launch: which sequence and head they belong to, and which
-// workgroup has them.  Whole waves call its functions; their results are uniform.
-template <unsigned ROWS, unsigned STEP, unsigned MOST, unsigned HEADS, unsigned GROUPS>
+// workgroup has them.  The first `extra` ones of a sequence's head hold nothing: where
+// a workgroup has four or more (with fewer, equal numbers of real ones count).  Whole
+// waves call its functions; their results are uniform.
+template <unsigned ROWS, unsigned STEP, unsigned MOST, unsigned HEADS, unsigned GROUPS, unsigned EXTRA>
 struct mt_units {
     // Every product of units and workgroups fits in N.
-    static constexpr unsigned long long ROOM = (unsigned long long)ROWS * HEADS * ((MOST + STEP - 1ull) / STEP);
+    static constexpr unsigned long long ROOM = (unsigned long long)ROWS * HEADS * ((MOST + STEP - 1ull) / STEP + EXTRA);
     using N = typename mt_count<(ROOM * (GROUPS + 1ull) < (1ull << 32))>::type;
     static constexpr int LAST = ROWS < 64u ? (int)ROWS - 1 : 63;  // the lane whose sum is a scan's whole
     const int* lengths;
     unsigned steps_, sum_;  // of this lane's sequence, and those up to it (64 sequences at most)
-    unsigned workgroups;
+    unsigned workgroups, extra;
     N all;
 
     MT_INLINE static unsigned length(int asked) { return asked < 0 ? 0u : (unsigned)asked < MOST ? (unsigned)asked : MOST; }
@@ -642,10 +660,14 @@ struct mt_units {
     }
     MT_INLINE void init(const int* lengths_, unsigned most) {
         lengths = lengths_;
-        all = 0u;
+        all = 0u, extra = 0u;
         for (unsigned b0 = 0; b0 < ROWS; b0 += 64u) {
             scan(b0, steps_, sum_);
             all += (N)(unsigned)__builtin_amdgcn_readlane((int)sum_, LAST) * HEADS;
+        }
+        if (all >= (N)4u * most) {
+            extra = EXTRA;
+            all += (N)ROWS * EXTRA * HEADS;
         }
         workgroups = all < most ? (unsigned)all : most;
     }
@@ -655,17 +677,18 @@ struct mt_units {
         for (unsigned b0 = 0;; b0 += 64u) {
             unsigned mine = steps_, sum = sum_;
             if (ROWS > 64u) scan(b0, mine, sum);
+            sum += extra * (mt_lane() + 1u);
             const unsigned long long past = __ballot(at + (N)sum * HEADS > u);
             if (past || b0 + 64u >= ROWS) {
                 const int who = __builtin_ctzll(past);
                 steps = (unsigned)__builtin_amdgcn_readlane((int)mine, who);
-                at += (N)((unsigned)__builtin_amdgcn_readlane((int)sum, who) - steps) * HEADS;
+                at += (N)((unsigned)__builtin_amdgcn_readlane((int)sum, who) - steps - extra) * HEADS;
                 return b0 + (unsigned)who;
             }
             at += (N)(unsigned)__builtin_amdgcn_readlane((int)sum, LAST) * HEADS;
         }
     }
-    MT_INLINE N first(unsigned w) const { return all * w / workgroups; }
+    MT_INLINE N first(unsigned w) const { return mt_uniform(all * w / workgroups); }
     MT_INLINE unsigned owner(N u) const { return (unsigned)(((u + 1u) * workgroups - 1u) / all); }
 };
 
@@ -685,34 +708,62 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     constexpr bool ONE_PAGE = PS % 16u == 0u;  // 16 positions lie in one page
     const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
 
-    // LDS: the operands of q, 16 bytes a lane each; then the waves' parts, [WAVES][HELD][D]
-    // sums and [WAVES][HELD] of m and of l.
+    // LDS: the operands of q, 16 bytes a lane each, of two pieces in turn; then the waves'
+    // parts, [WAVES][HELD][D] sums and [WAVES][HELD] of m and of l.
     constexpr unsigned KO = WIDE ? 4u : VK < 8u ? VK : 8u, NO = VK / KO, OPS = NJ * NO;
-    mt_u32x4* qs = reinterpret_cast<mt_u32x4*>(lds);  // [SETS][OPS][64]
-    float* sums = reinterpret_cast<float*>(lds + SETS * OPS * 1024u);
+    mt_u32x4* q2 = reinterpret_cast<mt_u32x4*>(lds);  // [2][SETS][OPS][64]
+    float* sums = reinterpret_cast<float*>(lds + 2u * SETS * OPS * 1024u);
     float* ms = sums + WAVES * HELD * D;
     float* ls = ms + WAVES * HELD;
     unsigned* flag = reinterpret_cast<unsigned*>(ls + WAVES * HELD);
 
-    using U = mt_units<ROWS, STEP, WIDTH * PS, HK * PARTS, GROUPS>;
+    constexpr unsigned UNIT = STEP * 2u * D * ITEM, EXTRA = (65536u + UNIT / 2u) / UNIT;
+    constexpr unsigned HEADS = HK * PARTS, SIDES = GROUPS / HEADS * HEADS * 16u >= GROUPS * 15u ? HEADS : 1u;
+    constexpr unsigned RANGES = GROUPS / SIDES;
+    using U = mt_units<ROWS, STEP, WIDTH * PS, HEADS / SIDES, RANGES, EXTRA>;
+    const unsigned range = blockIdx.x / SIDES, side = blockIdx.x % SIDES;
     U units;
     // (a batch larger than the workspace was laid out for is not split)
-    units.init(lengths, gridDim.z <= BATCH ? GROUPS : 1u);
-    if (blockIdx.x >= units.workgroups) return;
-    const typename U::N end = units.first(blockIdx.x + 1u);
+    units.init(lengths, gridDim.z <= BATCH ? RANGES : 1u);
+    if (range >= units.workgroups) return;
+    const typename U::N end = units.first(range + 1u);
 
-    // The range's current piece: `taken` of the `steps` of a sequence's head, from `step` on
+    // A piece of the range: `taken` of the `steps` of a sequence's head, from `step` on
     // (positions first .. last - 1), the head's first unit being `begins`.
-    typename U::N unit = units.first(blockIdx.x), begins;
-    unsigned b, head, part, step, steps, taken, first, last, tiles;
-    const int* table;
+    struct piece {
+        typename U::N begins;
+        unsigned b, head, part, step, steps, taken, first, last, tiles;
+        const int* table;
+    };
+    typename U::N unit = units.first(range);
+    const auto piece_at = [&]() {
+        piece p;
+        typename U::N before;
+        p.b = units.find(unit, before, p.steps);
+        const unsigned in = (unsigned)(unit - before), wide = p.steps + units.extra;
+        const unsigned pair = HEADS == SIDES ? side : mt_uniform(in / wide), at = HEADS == SIDES ? in : mt_uniform(in % wide);
+        p.part = pair % PARTS, p.head = pair / PARTS;
+        p.begins = unit - at + units.extra;
+        p.step = at > units.extra ? at - units.extra : 0u;
+        unit = p.begins + p.step;
+        const typename U::N left = unit < end ? end - unit : 0u;
+        p.taken = left < p.steps - p.step ? (unsigned)left : p.steps - p.step;
+        unit += p.taken;
+        const unsigned len = units.length(lengths[p.b]);
+        p.first = p.step * STEP;
+        p.last = len < (p.step + p.taken) * STEP ? len : (p.step + p.taken) * STEP;
+        p.last = p.last < p.first ? p.first : p.last;
+        p.tiles = (p.last - p.first + TILE - 1u) / TILE;
+        p.table = pages + (size_t)p.b * WIDTH;
+        return p;
+    };
     // The page of row n of block `bi` of a tile (of the block, where it lies in one).
-    const auto page_of = [&](unsigned ti, unsigned bi) -> int {
-        const unsigned t0 = first + TILE * ti + 16u * bi;
+    const auto page_of = [&](const piece& p, unsigned ti, unsigned bi) -> int {
+        const unsigned t0 = p.first + TILE * ti + 16u * bi;
         if constexpr (ONE_PAGE) {
-            return t0 < last ? __builtin_amdgcn_readfirstlane(table[t0 / PS]) : -1;
+            return t0 < p.last ? __builtin_amdgcn_readfirstlane(p.table[t0 / PS]) : -1;
         } else {
-            return t0 + n < last ? table[(t0 + n) / PS] : -1;
+            return t0 + n < p.last ? p.table[(t0 + n) / PS] : -1;
         }
     };
     const auto row_page = [&](int page, unsigned i) -> int { return ONE_PAGE ? page : __shfl(page, (int)(4u * g + i), 64); };
@@ -720,10 +771,10 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 
     unsigned kw[BLOCKS][NJ][KW], vw[BLOCKS][4][NV][VW];
     float ks[BLOCKS][4], vs[BLOCKS][4];
-    const auto load_k = [&](unsigned ti, const int (&page)[BLOCKS]) {
+    const auto load_k = [&](unsigned start, unsigned head, unsigned ti, const int (&page)[BLOCKS]) {
 #pragma unroll
         for (unsigned bi = 0; bi < BLOCKS; ++bi) {
-            const unsigned t0 = first + TILE * ti + 16u * bi;
+            const unsigned t0 = start + TILE * ti + 16u * bi;
             const typename C::offset p = C::row(safe(page[bi]), 0u, head, (t0 + n) % PS) + g * (VK * ITEM);
 #pragma unroll
             for (unsigned jj = 0; jj < NJ; ++jj) mt_ld_words<KW>(kw[bi][jj], cache + p + jj * (4u * VK * ITEM));
@@ -735,10 +786,10 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
             }
         }
     };
-    const auto load_v = [&](unsigned ti, const int (&page)[BLOCKS]) {
+    const auto load_v = [&](unsigned start, unsigned head, unsigned ti, const int (&page)[BLOCKS]) {
 #pragma unroll
         for (unsigned bi = 0; bi < BLOCKS; ++bi) {
-            const unsigned t0 = first + TILE * ti + 16u * bi;
+            const unsigned t0 = start + TILE * ti + 16u * bi;
 #pragma unroll
             for (unsigned i = 0; i < 4u; ++i) {
                 const unsigned pg = safe(row_page(page[bi], i)), r = (t0 + 4u * g + i) % PS;
@@ -754,35 +805,11 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         }
     };
 
-    int page[BLOCKS], page_next[BLOCKS];
-    // Opens the piece at `unit`, its first tile on the way.
-    const auto open = [&]() {
-        typename U::N before;
-        b = units.find(unit, before, steps);
-        const unsigned in = (unsigned)(unit - before), pair = in / steps;
-        step = in % steps, part = pair % PARTS, head = pair / PARTS;
-        begins = unit - step;
-        taken = end - unit < steps - step ? (unsigned)(end - unit) : steps - step;
-        unit += taken;
-        const unsigned len = units.length(lengths[b]);
-        first = step * STEP;
-        last = len < (step + taken) * STEP ? len : (step + taken) * STEP;
-        tiles = (last - first + TILE - 1u) / TILE;
-        table = pages + (size_t)b * WIDTH;
-#pragma unroll
-        for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = wave < tiles ? page_of(wave, bi) : -1, page_next[bi] = -1;
-        if (wave < tiles) {
-            load_k(wave, page);
-            load_v(wave, page);
-#pragma unroll
-            for (unsigned bi = 0; bi < BLOCKS; ++bi) page_next[bi] = page_of(wave + WAVES, bi);
-        }
-    };
-
     // Slot 2 w of the workspace is the part of workgroup w that began before it, 2 w + 1
     // the part that begins in it: [HELD][D] sums, [HELD] of m, [HELD] of l.  Four dims a
     // lane, written and read at device scope.
-    float* slots = ws + MT_WS_HEAD + (size_t)blockIdx.z * gridDim.x * 2u * FLOATS;
+    const unsigned own = blockIdx.z * gridDim.x + side * RANGES;  // this side's counters and slots
+    float* slots = ws + MT_WS_HEAD + (size_t)own * 2u * FLOATS;
     constexpr unsigned QUADS = HELD * D / 4u, LANES = 64u * WAVES;
     // Lanes that share four dims of a head when the parts of other workgroups are joined,
     // and parts of each whose loads are on the way together.
@@ -797,19 +824,16 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         mt_st4(o + ((size_t)b_ * HK * SHARE + head_ * SHARE + part_ * HELD + h) * D + 4u * (at % (D / 4u)), r);
     };
 
-    open();
-    for (;;) {
-
     // q, times the scale, as the MFMAs take it: dim d is element d % VK % KO of operand
     // (d / (4 VK), d % VK / KO) in the lanes of g = d / VK % 4; fp32 in column h, or the
     // parts of 8 (or 4) bf16 in columns 4 h + part of the set.
-    {
+    const auto put_q = [&](const piece& p, mt_u32x4* qs) {
         const float by = (float)(scale * 1.4426950408889634);
-        const float* qr = q + (size_t)b * QRS;
+        const float* qr = q + (size_t)p.b * QRS;
         for (unsigned at = threadIdx.x; at < (WIDE ? 16u : 4u * SETS) * D; at += 64u * WAVES) {
             const unsigned h = at / D, d = at % D, op = d / (4u * VK) * NO + d % VK / KO, e = d % KO, gd = d / VK % 4u;
             float v = 0.f;
-            if (h < HELD && part * HELD + h < SHARE) v = qr[(size_t)((head * SHARE + part * HELD + h) * D + d) * QCS] * by;
+            if (h < HELD && p.part * HELD + h < SHARE) v = qr[(size_t)((p.head * SHARE + p.part * HELD + h) * D + d) * QCS] * by;
             if constexpr (WIDE) {
                 reinterpret_cast<float*>(qs + op * 64u + gd * 16u + h)[e] = v;
             } else {
@@ -818,7 +842,31 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
                 for (unsigned j = 0; j < 4u; ++j) to[8u * j + e] = (unsigned short)(__float_as_uint(mt_bf16_part(v, j)) >> 16);
             }
         }
-    }
+    };
+
+    piece now = piece_at();
+    if (now.taken == 0u) return;
+    int page[BLOCKS], page_next[BLOCKS];
+#pragma unroll
+    for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = page_of(now, wave, bi), page_next[bi] = page_of(now, wave + WAVES, bi);
+    load_k(now.first, now.head, wave, page);
+    load_v(now.first, now.head, wave, page);
+    put_q(now, q2);
+    for (unsigned turn = 0;; turn ^= 1u) {
+    // The piece after this one: known, its pages and q there, from this one's start, and
+    // its first tile on the way from each wave's last one.  (Pages that are not there are
+    // -1, whose loads are page 0's and whose rows are masked: a wave without a tile of a
+    // piece passes through one of those.)
+    piece next = now;
+    next.taken = next.tiles = next.first = next.last = 0u;
+    if (unit < end) next = piece_at();
+    const bool again = next.taken > 0u;
+    int page_then[BLOCKS], page_then_next[BLOCKS];
+#pragma unroll
+    for (unsigned bi = 0; bi < BLOCKS; ++bi)
+        page_then[bi] = page_of(next, wave, bi), page_then_next[bi] = page_of(next, wave + WAVES, bi);
+    if (again) put_q(next, q2 + (turn ^ 1u) * (SETS * OPS * 64u));
+    const mt_u32x4* qs = q2 + turn * (SETS * OPS * 64u);
     __syncthreads();
 
     mt_f32x4 acc[SETS][NV * VV];
@@ -831,11 +879,12 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     }
     bool seen = false;
 #pragma unroll 1
-    for (unsigned ti = wave; ti < tiles; ti += WAVES) {
+    for (unsigned ti = wave;; ti += WAVES) {
         int page_after[BLOCKS];
 #pragma unroll
-        for (unsigned bi = 0; bi < BLOCKS; ++bi) page_after[bi] = page_of(ti + 2u * WAVES, bi);
-        const bool more = ti + WAVES < tiles;
+        for (unsigned bi = 0; bi < BLOCKS; ++bi) page_after[bi] = page_of(now, ti + 2u * WAVES, bi);
+        const bool more = ti + WAVES < now.tiles;
+        const unsigned start = more ? now.first : next.first, head = more ? now.head : next.head, tn = more ? ti + WAVES : wave;
         mt_f32x4 s[SETS][BLOCKS];
 #pragma unroll
         for (unsigned bi = 0; bi < BLOCKS; ++bi) {
@@ -886,13 +935,17 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
                     }
             }
         }
-        if (more) load_k(ti + WAVES, page_next);
+        if (!more) {
+#pragma unroll
+            for (unsigned bi = 0; bi < BLOCKS; ++bi) page_next[bi] = page_then[bi], page_after[bi] = page_then_next[bi];
+        }
+        if (more || again) load_k(start, head, tn, page_next);
         bool ok[BLOCKS][4], any = false, all = true;
 #pragma unroll
         for (unsigned bi = 0; bi < BLOCKS; ++bi)
 #pragma unroll
             for (unsigned i = 0; i < 4u; ++i) {
-                ok[bi][i] = (unsigned)row_page(page[bi], i) < PAGES && first + TILE * ti + 16u * bi + 4u * g + i < last;
+                ok[bi][i] = (unsigned)row_page(page[bi], i) < PAGES && now.first + TILE * ti + 16u * bi + 4u * g + i < now.last;
                 any = any || ok[bi][i];
                 all = all && ok[bi][i];
             }
@@ -996,16 +1049,13 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
                     }
                 }
         }
-        if (more) load_v(ti + WAVES, page_next);
+        if (more || again) load_v(start, head, tn, page_next);
 #pragma unroll
         for (unsigned bi = 0; bi < BLOCKS; ++bi) page[bi] = page_next[bi], page_next[bi] = page_after[bi];
+        if (!more) break;
     }
 
-    // The next piece's first tile is on the way while this one's waves meet.
-    const unsigned b_ = b, head_ = head, part_ = part, steps_ = steps;
-    const typename U::N begins_ = begins;
-    const bool opening = step == 0u, entire = taken == steps, again = unit < end;
-    if (again) open();
+    const bool opening = now.step == 0u, entire = now.taken == now.steps;
 
     // A part weighs 2^(m - the largest m); one whose scores are all -inf weighs nothing
     // and says in l whether it has positions: a softmax over such scores alone is 0 / 0,
@@ -1040,7 +1090,7 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 #pragma unroll 1
     for (bool others = false;; others = true) {
         // The waves' parts, or those of the workgroups as SHARED lanes joined them.
-        const mt_parts mine(slots + (size_t)(2u * blockIdx.x + (opening ? 1u : 0u)) * FLOATS, FLOATS * 4u);
+        const mt_parts mine(slots + (size_t)(2u * range + (opening ? 1u : 0u)) * FLOATS, FLOATS * 4u);
 #pragma unroll 1
         for (unsigned at = threadIdx.x; at < QUADS; at += LANES) {
             const unsigned h = at / (D / 4u);
@@ -1054,7 +1104,7 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
                         *reinterpret_cast<const mt_f32x4*>(sums + w * HELD * D + 4u * at));
             if (top == -INFINITY) total = empty;
             if (entire || others) {
-                put(b_, head_, part_, at, value, top, total);
+                put(now.b, now.head, now.part, at, value, top, total);
             } else {
                 mine.put(16u * at, value);
                 if (at % (D / 4u) == 0u) {
@@ -1066,10 +1116,10 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         if (entire || others) break;
 
         // The last workgroup of the sequence's head to arrive joins the parts.
-        const unsigned from = units.owner(begins_), parts = units.owner(begins_ + steps_ - 1u) - from + 1u;
-        unsigned* counter = reinterpret_cast<unsigned*>(ws) + blockIdx.z * gridDim.x + from;
+        const unsigned from = units.owner(now.begins), parts = units.owner(now.begins + now.steps - 1u) - from + 1u;
+        unsigned* counter = reinterpret_cast<unsigned*>(ws) + own + from;
         if (!mt_sn_arrive(counter, parts, flag)) break;
-        const mt_parts all_parts(slots, gridDim.x * 2u * FLOATS * 4u);
+        const mt_parts all_parts(slots, RANGES * 2u * FLOATS * 4u);
         const unsigned who = SHARED > 1u ? threadIdx.x / QUADS : 0u;
         for (unsigned at = SHARED > 1u ? threadIdx.x % QUADS : threadIdx.x; at < QUADS && who < SHARED; at += LANES) {
             const unsigned h = at / (D / 4u);
@@ -1109,6 +1159,7 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         __syncthreads();
     }
     if (!again) return;
+    now = next;
     }
 }
 

@@ -225,7 +225,7 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
         (*_cache_template(spec), spec.pages, op.pages.shape[1], share, held, waves, groups, batch, rows,
          op.q.row_stride, op.q.col_stride),
         args,
-        lds_bytes=q_bytes + 4 * waves * floats + 16,
+        lds_bytes=2 * q_bytes + 4 * waves * floats + 16,
         name="paged_attention",
     )
     return _group(decision, sig, frag, function_name or f"paged_attention_{op.o.name}", {"M": rows},
