@@ -198,15 +198,20 @@ def attention_workgroups(pairs: int, capacity: int, step: int, batch: int) -> in
 def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_name: str | None, batch: int) -> KernelGroup:
     spec, rows = op.spec, op.q.shape[0]
     share = op.heads // spec.kv_heads  # query heads of a key head
-    # At most 16 query heads at once, one fp32 MFMA's columns; 8 where 16 long rows would
-    # not fit in a wave's registers (four sets of bf16 columns) or in LDS.
-    held = min(share, 16 if spec.dim <= 128 else 8)
-    parts = _ceil(share, held)
-    pairs = rows * spec.kv_heads * parts
     # Eight waves to a compute unit; four, with twice the registers each, where the sums
     # of a wave's heads (or its tile of long fp32 rows) would not fit otherwise.
-    sets = 1 if spec.dtype == "float32" else _ceil(held, 4)
-    heavy = spec.dim > 128 or sets * spec.dim > (256 if spec.page_size % 16 == 0 else 128)
+    def heavy_with(held: int) -> bool:
+        sets = 1 if spec.dtype == "float32" else _ceil(held, 4)
+        return spec.dim > 128 or sets * spec.dim > (256 if spec.page_size % 16 == 0 else 128)
+
+    # At most 16 query heads at once, one fp32 MFMA's columns (four sets of bf16 ones); 8,
+    # and the keys read again for the others at the same time, where 16 long rows would not
+    # fit in registers or LDS, or where 8 leave eight waves (16 heads of 128 in int8: 130 us
+    # for 157, of 64 in pages of 20: 126 for 149; of 64 in pages of 16 16 do: 82 for 94).
+    held = min(share, 8 if spec.dim > 128 or (heavy_with(min(share, 16)) and not heavy_with(8)) else 16)
+    heavy = heavy_with(held)
+    parts = _ceil(share, held)
+    pairs = rows * spec.kv_heads * parts
     waves = 4 if heavy else ATTENTION_WAVES
     step = (16 if spec.dtype == "float32" else 32) * waves
     groups = attention_workgroups(pairs, op.capacity, step, batch)
