@@ -60,6 +60,9 @@ MT_INLINE void mt_put_row4(float* row, unsigned c, mt_f32x4 v) {
 // rounded once, and q falls on the side of its border that the formula says.
 // A row with a value that is not finite has no scale: it is stored as zeros
 // with the scale NaN, and reads back as NaN.
+//
+// Measured: 4096 rows of 4096, residual, 8 bits: 41 us, 5.3 TB/s of a copy's 5.5; 777
+// rows of 5003: 7.4 us (4.2 TB/s; 777 workgroups on 256 compute units); one row 3 us.
 // ---------------------------------------------------------------------------
 
 template <unsigned T, typename OP>
@@ -178,7 +181,8 @@ MT_INLINE void mt_rms_norm(const float* x, const float* res, const float* w, dou
 // ---------------------------------------------------------------------------
 // y[r, c] = q[r, c] * s[r].  The matrix is dense, so lanes take four elements of the
 // flat array at a time, aligned whatever the row length; a wave's stores are
-// contiguous, and its four loads are on the way together.
+// contiguous, and its four loads are on the way together.  4096 x 4096: 13 us, 6.3 TB/s
+// (what was just written is in the last-level cache).
 // ---------------------------------------------------------------------------
 
 template <unsigned COLS>
@@ -355,6 +359,9 @@ MT_INLINE void mt_cache_put(unsigned char* cache, const mt_f32x4 (&v)[(D + 63u) 
     }
 }
 
+// Bound: HBM, or the launch for few tokens.  8192 tokens of 8 heads of 128 in e4m3: 22.6
+// us, 3.7 TB/s, of which the look through the slots is about 4 us.
+//
 // Token t's keys and values go to slot slots[t] (page slot / PS, row slot % PS);
 // a slot outside the cache is passed over, and of tokens that name the same
 // slot the last is stored, whole: a token looks through the slots behind it
@@ -435,7 +442,8 @@ MT_INLINE void mt_cache_write(const float* k, const float* v, const int* slots, 
 }
 
 // Row r of k and v is slot slots[r] of the cache in 32 bits, zeros for a slot
-// outside it.  16 lanes take a row of one head.
+// outside it.  16 lanes take a row of one head.  16384 slots of 8 heads of 128 in e4m3:
+// 27 us, 6.2 TB/s (what was just written is in the last-level cache).
 template <int KIND, unsigned HK, unsigned PS, unsigned D, unsigned PAGES>
 MT_INLINE void mt_cache_read(const unsigned char* cache, const int* slots, float* k, float* v, unsigned rows) {
     using C = mt_cache<KIND, HK, PS, D, PAGES>;
@@ -536,7 +544,14 @@ MT_INLINE void mt_cache_read(const unsigned char* cache, const int* slots, float
 //
 // A position's scales multiply its score and its weight.  A position that is
 // masked (behind the length, or in a page outside the cache) scores -inf and its
-// values are replaced by zeros, whatever its bytes hold.  Bound: HBM, K and V once.
+// values are replaced by zeros, whatever its bytes hold.
+//
+// Bound: HBM, K and V once, up to 4 query heads of a key head in 8 bits and any number in
+// fp32 (32 sequences of 4096 keys, 8 key heads of 128: int8 with 1 to 4 query heads each
+// 55 us, e4m3 53 to 55, a copy's rate 50); with 8 the softmax and the splits of p, two
+// sets of columns in turn, take as long (74 and 66 us), with 16 130 and 118.  One
+// sequence of 131071 keys in e4m3 59 us, 4.7 TB/s; 2048 keys of 32 heads in fp32 15 us.
+// Beyond the stream a launch takes 5 us and a join over workgroups 4.
 // ---------------------------------------------------------------------------
 
 typedef short mt_i16x4 __attribute__((ext_vector_type(4)));
@@ -1185,10 +1200,16 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 // rows of the wave (permlane swaps: 2 or 4 for 32 k a lane), so that an MFMA takes
 // one group whole.
 //
-// Bound: HBM, the weights once.  SHARED: the digits of x stay in LDS, PB blocks of k at a
-// time, and every wave takes weight tiles of its own, row after row; otherwise the
-// waves of a workgroup share its weight rows and split k, each making the digits of its
-// part as it goes, so that few weight rows still keep many loads in flight.
+// SHARED: the digits of x stay in LDS, PB blocks of k at a time, and every wave takes
+// weight tiles of its own, row after row; otherwise the waves of a workgroup share its
+// weight rows and split k, each making the digits of its part as it goes, so that few
+// weight rows still keep many loads in flight.
+//
+// Bound: HBM, the weights once, for many weight rows (4 rows of x, 131072 x 4096: 54 us,
+// 5.3 TB/s).  For few a wave's share of k is a handful of blocks, and the waits for them
+// and the making of digits (about 12 vector instructions a value, in every workgroup)
+// count: 1 row, 11008 x 4096 7.5 us; 16 rows in 8 bits, 4096 x 11008 10.5; 5 rows, 4099 x
+// 5024 in groups of 32 15, of which vector instructions are 8.
 // ---------------------------------------------------------------------------
 
 // The whole number that an MFMA's four digit rows stand for.
