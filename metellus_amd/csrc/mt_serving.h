@@ -1278,6 +1278,7 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
     constexpr unsigned BL = EIGHT ? 1u : 4u / XR;     // blocks of x made into digits at once
     constexpr unsigned DIGITS = 512u * XR * SETS;     // bytes of a block's digits: [SETS][4 XR rows][128]
     constexpr bool RAGGED = K % (128u * U) != 0u;
+    static_assert(U % BL == 0u && (!SHARED || PB % U == 0u), "makings of digits are whole in a chunk, chunks in a phase");
     using OP = mt_operand<GB>;
     const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
     const unsigned m0 = blockIdx.y * 16u;

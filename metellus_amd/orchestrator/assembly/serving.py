@@ -263,7 +263,13 @@ def int4_shape(rows: int, k: int, n: int, group: int, eight: bool, zeros: bool) 
     blocks = _ceil(k, 128)
     made = 1 if eight else 4 // each  # blocks of x made into digits at once
     tiles, waves, together = 1, 8, 4
-    if not shared:
+    if shared:
+        # Sixteen waves to a making of digits, each making some, where they still leave a
+        # workgroup to each compute unit (fp32, 131072 x 4096: 8 rows 71 us, eight waves 78;
+        # 16 rows 90 and 118; 4 rows 59 and 55; groups of 32 with zeros 65536 x 2048: 44, 41).
+        if sets > 1 and group > 32 and _ceil(n, 16) >= 16 * INT4_WORKGROUPS:
+            waves, together = 16, 2
+    else:
         # Two tiles a wave halve the work on x, once one is more than a workgroup to each
         # compute unit (5 rows, 5024 x 4099: 15 us, one tile 17; 16 rows 24 and 35; 8 bits,
         # 16 rows, 11008 x 8192: 15 and 19; up to 4 rows one tile is as fast or faster).
