@@ -9,9 +9,11 @@ contained op's program position, and ``check_dependencies`` verifies a
 rewritten graph against the original program.
 
 Views (transpose / reshape) are not graph nodes; a consumer of a view sees
-the view's name as an external input.  Ordering between a view's owner and
-its consumers therefore comes only from the position tie-break
-(reference: graph.py:21-24).
+the view's name as an external input (reference: graph.py:21-24).  The
+position tie-break orders a view's owner before its consumers as long as each
+is a vertex of its own; a fused vertex stands at its earliest op, so the order
+also has an edge from the vertex that writes a view's owner to the view's
+readers.
 
 Implementation notes (behaviour-neutral): the topological order and the
 producer map of an immutable graph are computed once and cached, and the
@@ -22,7 +24,7 @@ position) instead of re-sorting a list after every pop.
 from __future__ import annotations
 
 import heapq
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from functools import cached_property
 
 from metellus_amd.orchestrator.ir import Op, Program, outs_of
@@ -51,6 +53,7 @@ class Graph:
     vertices: tuple[Vertex, ...]
     op_index: dict[int, int]
     program_outputs: frozenset[str]
+    owners: dict[str, str] = field(default_factory=dict)  # views that ops read -> their storage owners
 
     # -- construction --------------------------------------------------------
 
@@ -70,10 +73,11 @@ class Graph:
             vertices=tuple(verts),
             op_index={id(op): i for i, op in enumerate(program)},
             program_outputs=outs,
+            owners={t.name: t.buffer_key for op in program for t in op.inputs if t.buffer_key != t.name},
         )
 
     def _derive(self, vertices: tuple[Vertex, ...]) -> Graph:
-        return Graph(vertices=vertices, op_index=self.op_index, program_outputs=self.program_outputs)
+        return Graph(vertices=vertices, op_index=self.op_index, program_outputs=self.program_outputs, owners=self.owners)
 
     # -- cached structure ----------------------------------------------------
 
@@ -99,6 +103,8 @@ class Graph:
         indeg = [0] * n
         for pos, v in enumerate(self.vertices):
             preds = {writer[name] for name in v.inputs if name in writer}
+            owned = {self.owners.get(name) for name in v.inputs if name not in writer}
+            preds |= {writer[name] for name in owned if name in writer} - {pos}
             indeg[pos] = len(preds)
             for p in preds:
                 succ[p].add(pos)

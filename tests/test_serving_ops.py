@@ -378,3 +378,25 @@ def test_launch_rules_stay_within_what_the_kernels_take():
                 for eight in (False, True):
                     shape = int4_shape(rows, k, n, 32, eight, True)
                     assert 1 <= shape["waves"] <= 16 and shape["tiles"] in (1, 2, 4) and shape["together"] in (1, 2, 4)
+
+
+@pytest.mark.parametrize("view", ["transpose", "reshape"])
+@pytest.mark.parametrize("first", ["norm", "matmul", "reduction"])
+def test_a_chain_that_begins_before_a_view_of_another_kernels_output_runs_after_it(first, view):
+    ops = _ops(x=(64, 64), w=(64, 64))
+    ops.elementwise("exp", out="e", operands=("x",))
+    if first == "norm":
+        ops.rms_norm("x", out="h")
+    elif first == "matmul":
+        ops.matmul("x", "w", out="h")
+    else:
+        ops.reduction("max", out="h", x="x")
+    if first == "reduction":
+        ops.reshape("h", (64, 1), out="v")
+    elif view == "transpose":
+        ops.transpose("h", out="v")
+    else:
+        ops.reshape("h", (64, 64), out="v")
+    ops.elementwise("add", out="z", operands=("e", "v"), **({"y_broadcast": "col"} if first == "reduction" else {}))
+    groups = compile_program(ops)
+    assert [g.bindings[1] if "e" in g.outputs or "z" in g.outputs else "h" for g in groups] == ["h", "z"]
