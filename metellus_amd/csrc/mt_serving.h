@@ -655,7 +655,10 @@ struct mt_units {
     using N = typename mt_count<(ROOM * (GROUPS + 1ull) < (1ull << 32))>::type;
     static constexpr int LAST = ROWS < 64u ? (int)ROWS - 1 : 63;  // the lane whose sum is a scan's whole
     const int* lengths;
-    unsigned steps_, sum_;  // of this lane's sequence, and those up to it (64 sequences at most)
+    // The 64 sequences from from_, before_ units behind the first: the steps of this
+    // lane's, and the sum of those up to it.
+    unsigned steps_, sum_, from_;
+    N before_;
     unsigned workgroups, extra;
     N all;
 
@@ -685,22 +688,24 @@ struct mt_units {
             all += (N)ROWS * EXTRA * HEADS;
         }
         workgroups = all < most ? (unsigned)all : most;
+        from_ = 0u, before_ = 0u;
+        if (ROWS > 64u) scan(0u, steps_, sum_);
     }
-    // The sequence that unit u < all belongs to, the units before it and its steps.
-    MT_INLINE unsigned find(N u, N& at, unsigned& steps) const {
-        at = 0u;
-        for (unsigned b0 = 0;; b0 += 64u) {
-            unsigned mine = steps_, sum = sum_;
-            if (ROWS > 64u) scan(b0, mine, sum);
-            sum += extra * (mt_lane() + 1u);
-            const unsigned long long past = __ballot(at + (N)sum * HEADS > u);
-            if (past || b0 + 64u >= ROWS) {
+    // The sequence that unit u < all belongs to, the units before it and its steps; from
+    // call to call u grows.
+    MT_INLINE unsigned find(N u, N& at, unsigned& steps) {
+        for (;;) {
+            const unsigned sum = sum_ + extra * (mt_lane() + 1u);
+            const unsigned long long past = __ballot(before_ + (N)sum * HEADS > u);
+            if (past || from_ + 64u >= ROWS) {
                 const int who = __builtin_ctzll(past);
-                steps = (unsigned)__builtin_amdgcn_readlane((int)mine, who);
-                at += (N)((unsigned)__builtin_amdgcn_readlane((int)sum, who) - steps - extra) * HEADS;
-                return b0 + (unsigned)who;
+                steps = (unsigned)__builtin_amdgcn_readlane((int)steps_, who);
+                at = before_ + (N)((unsigned)__builtin_amdgcn_readlane((int)sum, who) - steps - extra) * HEADS;
+                return from_ + (unsigned)who;
             }
-            at += (N)(unsigned)__builtin_amdgcn_readlane((int)sum, LAST) * HEADS;
+            before_ += (N)(unsigned)__builtin_amdgcn_readlane((int)sum, LAST) * HEADS;
+            from_ += 64u;
+            scan(from_, steps_, sum_);
         }
     }
     MT_INLINE N first(unsigned w) const { return mt_uniform(all * w / workgroups); }
