@@ -185,14 +185,14 @@ def _assemble_cache_read(decision: DecisionView, op: CacheReadOp, function_name:
 # ---------------------------------------------------------------------------
 
 ATTENTION_WAVES = 8
-ATTENTION_WORKGROUPS = 256  # at most; the device cuts the work into as many equal ranges
+ATTENTION_WORKGROUPS = 256  # one to a compute unit; the device cuts the work into as many equal ranges
 
 
-def attention_workgroups(pairs: int, capacity: int, step: int, batch: int) -> int:
+def attention_workgroups(pairs: int, capacity: int, step: int, batch: int, most: int = ATTENTION_WORKGROUPS) -> int:
     """Workgroups of a launch: one for each unit of ``step`` positions of a sequence
-    (``pairs`` of them, times key heads) that there is room for, as many as fit on the
-    GPU at once, and a counter each in the workspace's head for all of a batch."""
-    return max(1, min(ATTENTION_WORKGROUPS, pairs * _ceil(capacity, step), (WS_HEAD_BYTES // 4 - 1) // batch))
+    (``pairs`` of them, times key heads) that there is room for, ``most`` at most, and a
+    counter each in the workspace's head for all of a batch."""
+    return max(1, min(most, pairs * _ceil(capacity, step), (WS_HEAD_BYTES // 4 - 1) // batch))
 
 
 def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_name: str | None, batch: int) -> KernelGroup:
@@ -212,9 +212,15 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
     heavy = heavy_with(held)
     parts = _ceil(share, held)
     pairs = rows * spec.kv_heads * parts
-    waves = 4 if heavy else ATTENTION_WAVES
+    waves, most = 4 if heavy else ATTENTION_WAVES, ATTENTION_WORKGROUPS
+    if spec.dtype != "float32" and not heavy and op.capacity <= 512:
+        # Short sequences in 8 bits: their ends are most of the time, and overlap where smaller
+        # workgroups share a compute unit (8 key heads of 128 in int8, four or two waves for
+        # eight: 1024 sequences of 256 keys 130, 110 and 175 us, 64 of 64 9.1, 8.2 and 13; 256
+        # of 512 55 and 62, 64 of 300 17.9 and 18.8; 64 of 1024 27 and 27; fp32 no faster).
+        waves, most = (2, 4 * ATTENTION_WORKGROUPS) if op.capacity <= 256 else (4, 2 * ATTENTION_WORKGROUPS)
     step = (16 if spec.dtype == "float32" else 32) * waves
-    groups = attention_workgroups(pairs, op.capacity, step, batch)
+    groups = attention_workgroups(pairs, op.capacity, step, batch, most)
     floats = _ceil(held * (spec.dim + 2), 4) * 4
     # q's operands in LDS: 16 bytes a lane for 16 dims of fp32 columns, or for 32 (16) of bf16 sets
     if spec.dtype == "float32":
