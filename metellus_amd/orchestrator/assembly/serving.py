@@ -282,6 +282,11 @@ def int4_shape(rows: int, k: int, n: int, group: int, eight: bool, zeros: bool) 
         # Sixteen waves where it is not (1 row, 11008 x 4096: 9.5 us, 8 waves 11.2).
         many = _ceil(n, 16) > INT4_WORKGROUPS
         tiles = 2 if rows > 4 and many else 1
+        # Four for fp32 where two are more than that and four are not, and their sums fit in
+        # registers (8 rows, 8192 x 11008, groups of 128 23 us, two tiles 30; 16 rows of
+        # groups of 64 45 and 59, of 32 71 and 73; 8 bits 25 and 25).
+        if tiles == 2 and 2 * INT4_WORKGROUPS < _ceil(n, 16) <= 4 * INT4_WORKGROUPS and not eight and sets * 128 // group < 16:
+            tiles = 4
         waves = 16 if not many and sets <= 2 else 8
         if eight:  # (1 row, 8192 x 11008: groups of 128 one block 17.3 us, two 15.3; of 32, 20.6 and 24.2)
             together = 1 if group == 32 else 2

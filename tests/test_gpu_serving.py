@@ -219,6 +219,9 @@ def test_matmul_int4(rows, k, n, group, eight, zeros):
     # two tiles of weight rows a wave, with an odd number of tiles and without
     (5, 416, 4099, 32, False, True), (16, 1056, 4128, 32, False, True), (9, 512, 8200, 128, False, False),
     (16, 704, 4100, 64, True, True), (6, 384, 5000, 128, True, False), (33, 288, 4097, 32, True, True),
+    # four tiles
+    (5, 416, 8205, 32, False, True), (16, 704, 16384, 64, False, True), (8, 1152, 11008, 128, False, False),
+    (12, 640, 9000, 128, False, True), (20, 288, 8193, 32, False, False),
     # sixteen waves, shares of k that differ by one, k shorter than the waves
     (1, 5024, 2000, 32, False, True), (2, 4416, 300, 64, False, False), (4, 2592, 4096, 32, False, True),
     (8, 3200, 500, 128, False, True), (16, 11008, 40, 64, True, False), (1, 2080, 33, 32, True, True),
