@@ -263,9 +263,10 @@ def int4_shape(rows: int, k: int, n: int, group: int, eight: bool, zeros: bool) 
     sets = 1 if eight else _ceil(held, 4)
     each = 4 if eight or held > 2 else held
     # Enough weight rows for a tile to most waves of the GPU: the waves share x's digits
-    # (4 rows, 4096 x 131072: 54 us, splitting k 80; 16 rows, 8192 x 28672: 57 and 74; one
-    # row 30 and 29).  Fewer rows: splitting k (16 rows, 4096 x 11008: 24 us).
-    shared = _ceil(n, 16) >= 1536
+    # (4 rows, 4096 x 131072: 54 us, splitting k 80; 8 rows, 4096 x 20480 18 and 24; 16400,
+    # the next tile after four a workgroup, 18 and 23; one row, 4096 x 20480 13.3 and 12.7,
+    # 24000 13.5 and 14.3).  Fewer rows: splitting k (8 rows, 4096 x 11008: 13.5, shared 18).
+    shared = _ceil(n, 16) > 4 * INT4_WORKGROUPS if rows > 4 else _ceil(n, 16) >= 5 * INT4_WORKGROUPS
     blocks = _ceil(k, 128)
     made = 1 if eight else 4 // each  # blocks of x made into digits at once
     tiles, waves, together = 1, 8, 4

@@ -214,6 +214,7 @@ def test_matmul_int4(rows, k, n, group, eight, zeros):
     (1, 1056, 24590, 32, False, True), (2, 1152, 24577, 64, False, False), (3, 640, 33000, 128, False, True),
     (16, 1632, 24600, 32, False, False), (16, 1664, 24576, 128, False, True), (7, 1024, 24579, 64, False, True),
     (20, 416, 24601, 32, False, True), (16, 1632, 24600, 32, True, True), (5, 7744, 24577, 64, True, False),
+    (6, 416, 16400, 32, False, True), (4, 416, 20479, 32, False, True), (16, 384, 16385, 128, True, False),
     # sixteen waves to a making of digits, k in phases and not
     (16, 1728, 65540, 64, False, True), (7, 384, 65536, 128, False, False), (11, 352, 70001, 32, False, False),
     # two tiles of weight rows a wave, with an odd number of tiles and without
