@@ -12,6 +12,8 @@ Tolerances follow from the kernels' roundings (u = 2^-24, half a step of fp32):
 
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 
@@ -529,6 +531,21 @@ def test_paged_attention_bad_pages_and_lengths(dtype, page_size):
     assert np.all(env[1] == 0) and np.all(env[2] == 0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_paged_attention_of_a_transposed_q(dtype):
+    plain = _attention(dtype, 8, 2, 64, 16, 40, [640, 3, 77, 0, 600], seed=31)
+    ops = Operations()
+    ops.kv_cache("cache", **{k: getattr(plain.build()[0].spec, k) for k in ("pages", "page_size", "kv_heads", "dim", "dtype")})
+    for name in ("cache", "pages", "lengths"):
+        if name != "cache":
+            ops.input(name, plain.uploads[name].shape, dtype="int32")
+        ops.from_numpy(plain.uploads[name], name)
+    _put(ops, "q_", np.ascontiguousarray(plain.uploads["q"].T))
+    ops.transpose("q_", out="q")
+    ops.paged_attention("q", cache="cache", pages="pages", lengths="lengths", out="o", heads=8)
+    np.testing.assert_array_equal(run(ops).env["o"], run(plain).env["o"])
+
+
 def test_paged_attention_values_that_are_not_finite():
     """Scores of -inf weigh nothing beside others and give NaN alone, as softmax does;
     an infinite value reaches its own dim."""
@@ -659,6 +676,53 @@ def test_a_resident_program_runs_again_and_again():
             runtime.run(env)
         for (runtime, env), o in zip(made, want):
             np.testing.assert_array_equal(env["o"].numpy(o.shape, np.float32), o)
+
+
+def test_attention_next_to_products_that_use_the_same_workspace():
+    """A product of few tiles (summed in parts), a split attention and the product of its
+    output: again and again, with the workspace's flags left zero by each."""
+    ops = _attention("int8", 8, 2, 64, 16, 256, [4096, 700], seed=40)
+    rng = np.random.default_rng(40)
+    _put(ops, "wv", rng.standard_normal((512, 64)).astype(np.float32))
+    _put(ops, "a", rng.standard_normal((64, 8192)).astype(np.float32))
+    _put(ops, "b", rng.standard_normal((8192, 64)).astype(np.float32))
+    ops.matmul("a", "b", out="c")
+    ops.matmul("o", "wv", out="p")
+    groups = compile_program(ops)
+    assert sum(g.kernel.workspace_bytes > 0 for g in groups) >= 2
+    first = run(ops).env
+    want = evaluate(ops)
+    _close(first["c"], want["c"], 1e-4 * np.sqrt(8192) * np.abs(want["c"]) + 8192 * U * (np.abs(ops.uploads["a"]) @ np.abs(ops.uploads["b"])))
+    for _ in range(3):
+        env = run(ops).env
+        for name in ("o", "c", "p"):
+            if name in first:
+                np.testing.assert_array_equal(env[name], first[name])
+    hip_backend.check_workspace()
+
+
+def test_two_threads_at_once():
+    """Each thread runs programs of its own over and over; they share the stream and the
+    workspace."""
+    programs = [[_attention("int8", 8, 2, 64, 16, 256, [4096, 700 + s], seed=s), _int4(5, 1056, 500, 32, False, True, s)] for s in (1, 2)]
+    want = [[run(ops).env for ops in each] for each in programs]
+    wrong = []
+
+    def work(each, env):
+        try:
+            for _ in range(10):
+                for ops, ref, name in zip(each, env, ("o", "y")):
+                    if not np.array_equal(run(ops).env[name], ref[name]):
+                        wrong.append(name)
+        except Exception as e:  # (an assertion in a thread would be lost)
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=pair) for pair in zip(programs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong
 
 
 def test_decoding_token_after_token():
