@@ -533,25 +533,28 @@ MT_INLINE void mt_cache_read(const unsigned char* cache, const int* slots, float
 //     it stands, and lane (n, g) loads rows 4 g + i's dims VV (16 c + n) .. + VV - 1
 //     of V.  No value changes lanes.
 //
-// KIND 0 (fp32): MFMAs 16x16x4 in fp32, tiles of 16 positions, a column a head, and
-// each value of V an operand by itself.
-// 8 bits: the values are exact in bf16, and q and p are three bf16 parts each (hi,
-// mid, lo: their 24 bits), in columns and rows 4 h + part of sets of 4 heads: MFMAs
-// 16x16x32, tiles of 32 positions.  The fp32 MFMAs take 64 values of the cache in 32
-// cycles, 4.9e12 a second on the GPU -- no more than HBM brings at one byte each;
-// these take 512 in 16.  Four rows of V are exchanged byte by byte in registers, so
-// that a dim's positions stand together.  (Weights below 2^-110 lose low parts.)
+// KIND 0 (fp32): MFMAs 16x16x4 in fp32, tiles of 16 positions, and each value of V an
+// operand by itself.
+// 8 bits: the values are exact in bf16, and q and p are three bf16 parts each (hi, mid,
+// lo: their 24 bits), an MFMA 16x16x32 for each in turn: tiles of 32 positions.  The fp32
+// MFMAs take 64 values of the cache in 32 cycles, 4.9e12 a second on the GPU -- no more
+// than HBM brings at one byte each; these take 512 in 48.  (The parts in columns of their
+// own, four heads to an MFMA, took as long for 4 heads, and every lane's softmax once more
+// for each further four: 8 heads 74 us for 58, 16 129 for 62.)  Four rows of V are
+// exchanged byte by byte in registers, so that a dim's positions stand together.  (Weights
+// below 2^-110 lose low parts.)
 //
 // A position's scales multiply its score and its weight.  A position that is
 // masked (behind the length, or in a page outside the cache) scores -inf and its
 // values are replaced by zeros, whatever its bytes hold.
 //
-// Bound: HBM, K and V once, up to 4 query heads of a key head in 8 bits and any number in
-// fp32 (32 sequences of 4096 keys, 8 key heads of 128: int8 with 1 to 4 query heads each
-// 55 us, e4m3 53 to 55, a copy's rate 50); with 8 the softmax and the splits of p, two
-// sets of columns in turn, take as long (74 and 66 us), with 16 130 and 118.  One
-// sequence of 131071 keys in e4m3 59 us, 4.7 TB/s; 2048 keys of 32 heads in fp32 15 us.
-// Beyond the stream a launch takes 5 us and a join over workgroups 4.
+// Bound: HBM, K and V once (32 sequences of 4080 keys, 8 key heads of 128, a copy's rate 50
+// us: int8 with 1 to 8 query heads each 55 to 58, 16 62; e4m3 54 to 57; fp32 of a quarter
+// of the keys 50 to 53).  Heads of 64 in 8 bits take as many vector instructions a position
+// as longer ones' halves and are bound by them (40 to 43 us for 26), and rows of 16
+// positions in two pages take more (pages of 20: 72 in int8).  One sequence of 131071 keys
+// in e4m3 59 us, 4.7 TB/s; 2048 keys of 32 heads in fp32 15 us.  Beyond the stream a launch
+// takes 5 us and a join over workgroups 4.
 // ---------------------------------------------------------------------------
 
 typedef short mt_i16x4 __attribute__((ext_vector_type(4)));
@@ -593,14 +596,10 @@ MT_INLINE mt_u32x2 mt_held4_bf16(unsigned w) {
     }
 }
 
-// Part `j` of x's three bf16 parts (8 bits each, together all 24), as a float whose
-// low half is 0; nothing for j = 3.
-MT_INLINE float mt_bf16_part(float x, unsigned j) {
-    const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFF0000u), r = x - hi;
-    const float mid = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
-    return j == 0u ? hi : j == 1u ? mid : j == 2u ? r - mid : 0.f;
-}
-// Two such parts in one word.
+// What the upper half of x, a bf16, leaves of it.  Three times that is all of x: 8 bits of
+// its 24 each, hi, mid and lo.
+MT_INLINE float mt_bf16_rest(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); }
+// The upper halves of two floats in one word.
 MT_INLINE unsigned mt_bf16_pair(float lo, float hi) {
     return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
@@ -720,7 +719,7 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     constexpr unsigned ITEM = C::ITEM, PARTS = (SHARE + HELD - 1u) / HELD;
     constexpr bool WIDE = KIND == 0;
     constexpr unsigned BLOCKS = WIDE ? 1u : 2u, TILE = 16u * BLOCKS;       // positions of a tile
-    constexpr unsigned SETS = WIDE ? 1u : (HELD + 3u) / 4u;                // MFMA column sets
+    constexpr unsigned SPLIT = WIDE ? 1u : 3u;                             // operands a value of q or p makes
     constexpr unsigned VK = WIDE ? 4u : D % 64u == 0u ? 16u : D % 32u == 0u ? 8u : 4u, NJ = D / (4u * VK);
     constexpr unsigned VV = WIDE || D <= 64u ? 4u : 8u, NV = (D + 16u * VV - 1u) / (16u * VV);
     constexpr unsigned KW = VK * ITEM / 4u, VW = VV * ITEM / 4u, FLOATS = (HELD * (D + 2u) + 3u) / 4u * 4u;
@@ -731,8 +730,8 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     // LDS: the operands of q, 16 bytes a lane each, of two pieces in turn; then the waves'
     // parts, [WAVES][HELD][D] sums and [WAVES][HELD] of m and of l.
     constexpr unsigned KO = WIDE ? 4u : VK < 8u ? VK : 8u, NO = VK / KO, OPS = NJ * NO;
-    mt_u32x4* q2 = reinterpret_cast<mt_u32x4*>(lds);  // [2][SETS][OPS][64]
-    float* sums = reinterpret_cast<float*>(lds + 2u * SETS * OPS * 1024u);
+    mt_u32x4* q2 = reinterpret_cast<mt_u32x4*>(lds);  // [2][SPLIT][OPS][64]
+    float* sums = reinterpret_cast<float*>(lds + 2u * SPLIT * OPS * 1024u);
     float* ms = sums + WAVES * HELD * D;
     float* ls = ms + WAVES * HELD;
     unsigned* flag = reinterpret_cast<unsigned*>(ls + WAVES * HELD);
@@ -844,22 +843,22 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         mt_st4(o + ((size_t)b_ * HK * SHARE + head_ * SHARE + part_ * HELD + h) * D + 4u * (at % (D / 4u)), r);
     };
 
-    // q, times the scale, as the MFMAs take it: dim d is element d % VK % KO of operand
-    // (d / (4 VK), d % VK / KO) in the lanes of g = d / VK % 4; fp32 in column h, or the
-    // parts of 8 (or 4) bf16 in columns 4 h + part of the set.
+    // q, times the scale, as the MFMAs take it: column h, dim d element d % VK % KO of operand
+    // (d / (4 VK), d % VK / KO) in the lanes of g = d / VK % 4; for 8 bits hi, mid and lo.
     const auto put_q = [&](const piece& p, mt_u32x4* qs) {
         const float by = (float)(scale * 1.4426950408889634);
         const float* qr = q + (size_t)p.b * QRS;
-        for (unsigned at = threadIdx.x; at < (WIDE ? 16u : 4u * SETS) * D; at += 64u * WAVES) {
+        for (unsigned at = threadIdx.x; at < 16u * D; at += 64u * WAVES) {
             const unsigned h = at / D, d = at % D, op = d / (4u * VK) * NO + d % VK / KO, e = d % KO, gd = d / VK % 4u;
             float v = 0.f;
             if (h < HELD && p.part * HELD + h < SHARE) v = qr[(size_t)((p.head * SHARE + p.part * HELD + h) * D + d) * QCS] * by;
+            mt_u32x4* to = qs + op * 64u + gd * 16u + h;
             if constexpr (WIDE) {
-                reinterpret_cast<float*>(qs + op * 64u + gd * 16u + h)[e] = v;
+                reinterpret_cast<float*>(to)[e] = v;
             } else {
-                unsigned short* to = reinterpret_cast<unsigned short*>(qs + (h / 4u * OPS + op) * 64u + gd * 16u + h % 4u * 4u);
 #pragma unroll
-                for (unsigned j = 0; j < 4u; ++j) to[8u * j + e] = (unsigned short)(__float_as_uint(mt_bf16_part(v, j)) >> 16);
+                for (unsigned j = 0; j < SPLIT; ++j, v = mt_bf16_rest(v))
+                    reinterpret_cast<unsigned short*>(to + j * (OPS * 64u))[e] = (unsigned short)(__float_as_uint(v) >> 16);
             }
         }
     };
@@ -885,18 +884,14 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 #pragma unroll
     for (unsigned bi = 0; bi < BLOCKS; ++bi)
         page_then[bi] = page_of(next, wave, bi), page_then_next[bi] = page_of(next, wave + WAVES, bi);
-    if (again) put_q(next, q2 + (turn ^ 1u) * (SETS * OPS * 64u));
-    const mt_u32x4* qs = q2 + turn * (SETS * OPS * 64u);
+    if (again) put_q(next, q2 + (turn ^ 1u) * (SPLIT * OPS * 64u));
+    const mt_u32x4* qs = q2 + turn * (SPLIT * OPS * 64u);
     __syncthreads();
 
-    mt_f32x4 acc[SETS][NV * VV];
-    float m[SETS], l[SETS];
+    mt_f32x4 acc[NV * VV];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (unsigned t = 0; t < SETS; ++t) {
-        m[t] = -INFINITY, l[t] = 0.f;
-#pragma unroll
-        for (unsigned i = 0; i < NV * VV; ++i) acc[t][i] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (unsigned i = 0; i < NV * VV; ++i) acc[i] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
     bool seen = false;
 #pragma unroll 1
     for (unsigned ti = wave;; ti += WAVES) {
@@ -905,55 +900,52 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
         for (unsigned bi = 0; bi < BLOCKS; ++bi) page_after[bi] = page_of(now, ti + 2u * WAVES, bi);
         const bool more = ti + WAVES < now.tiles;
         const unsigned start = more ? now.first : next.first, head = more ? now.head : next.head, tn = more ? ti + WAVES : wave;
-        mt_f32x4 s[SETS][BLOCKS];
+        mt_f32x4 s[BLOCKS];
+        if constexpr (WIDE) {
+            mt_f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (unsigned bi = 0; bi < BLOCKS; ++bi) {
-            if constexpr (WIDE) {
-                mt_f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+            for (unsigned jj = 0; jj < NJ; ++jj) {
+                const mt_f32x4 qv = __builtin_bit_cast(mt_f32x4, qs[jj * 64u + lane]);
 #pragma unroll
-                for (unsigned jj = 0; jj < NJ; ++jj) {
-                    const mt_f32x4 qv = __builtin_bit_cast(mt_f32x4, qs[jj * 64u + lane]);
+                for (unsigned e = 0; e < 4u; e += 2u) {
+                    s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[0][jj][e]), qv[e], s0, 0, 0, 0);
+                    s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[0][jj][e + 1u]), qv[e + 1u], s1, 0, 0, 0);
+                }
+            }
+            s[0] = s0 + s1;
+        } else {
+            // hi's products in one sum, mid's and lo's, 2^-8 of them, in another: each
+            // rounds to its own size.
+            mt_f32x4 sum[BLOCKS][2];
 #pragma unroll
-                    for (unsigned e = 0; e < 4u; e += 2u) {
-                        s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[bi][jj][e]), qv[e], s0, 0, 0, 0);
-                        s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kw[bi][jj][e + 1u]), qv[e + 1u], s1, 0, 0, 0);
+            for (unsigned bi = 0; bi < BLOCKS; ++bi) sum[bi][0] = sum[bi][1] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (unsigned op = 0; op < OPS; ++op) {
+                mt_u32x4 k8[BLOCKS];  // (the first two words where KO is 4)
+#pragma unroll
+                for (unsigned bi = 0; bi < BLOCKS; ++bi) {
+                    const unsigned* k = &kw[bi][op / NO][KO / 4u * (op % NO)];
+                    const mt_u32x2 lo = mt_held4_bf16<KIND>(k[0]), hi = KO == 8u ? mt_held4_bf16<KIND>(k[KO / 8u]) : lo;
+                    k8[bi] = mt_u32x4{lo.x, lo.y, hi.x, hi.y};
+                }
+#pragma unroll
+                for (unsigned j = 0; j < SPLIT; ++j) {
+                    const mt_u32x4 q8 = qs[(j * OPS + op) * 64u + lane];
+#pragma unroll
+                    for (unsigned bi = 0; bi < BLOCKS; ++bi) {
+                        mt_f32x4& to = sum[bi][j ? 1u : 0u];
+                        if constexpr (KO == 8u)
+                            to = mt_mfma16_bf16(k8[bi], q8, to);
+                        else
+                            to = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(mt_i16x4, mt_u32x2(k8[bi].xy)),
+                                                                           __builtin_bit_cast(mt_i16x4, mt_u32x2(q8.xy)), to, 0, 0, 0);
                     }
                 }
-                s[0][bi] = s0 + s1;
-            } else {
-#pragma unroll
-                for (unsigned t = 0; t < SETS; ++t) s[t][bi] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (unsigned jj = 0; jj < NJ; ++jj)
-#pragma unroll
-                    for (unsigned e = 0; e < NO; ++e) {
-                        if constexpr (KO == 8u) {
-                            const mt_u32x2 lo = mt_held4_bf16<KIND>(kw[bi][jj][2u * e]);
-                            const mt_u32x2 hi = mt_held4_bf16<KIND>(kw[bi][jj][2u * e + 1u]);
-                            const mt_u32x4 k8 = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-                            for (unsigned t = 0; t < SETS; ++t)
-                                s[t][bi] = mt_mfma16_bf16(k8, qs[(t * OPS + jj * NO + e) * 64u + lane], s[t][bi]);
-                        } else {
-                            const mt_u32x2 k4 = mt_held4_bf16<KIND>(kw[bi][jj][e]);
-#pragma unroll
-                            for (unsigned t = 0; t < SETS; ++t) {
-                                const mt_u32x2 o4 = qs[(t * OPS + jj * NO + e) * 64u + lane].xy;
-                                s[t][bi] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
-                                    __builtin_bit_cast(mt_i16x4, k4), __builtin_bit_cast(mt_i16x4, o4), s[t][bi], 0, 0, 0);
-                            }
-                        }
-                    }
-#pragma unroll
-                for (unsigned t = 0; t < SETS; ++t)
-#pragma unroll
-                    for (unsigned i = 0; i < 4u; ++i) {  // the parts of q together
-                        float v = s[t][bi][i];
-                        v += mt_xor_lanes<1u>(v);
-                        v += mt_xor_lanes<2u>(v);
-                        s[t][bi][i] = v * ks[bi][i];
-                    }
             }
+#pragma unroll
+            for (unsigned bi = 0; bi < BLOCKS; ++bi)
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i) s[bi][i] = (sum[bi][0][i] + sum[bi][1][i]) * ks[bi][i];
         }
         if (!more) {
 #pragma unroll
@@ -976,54 +968,41 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
             for (unsigned bi = 0; bi < BLOCKS; ++bi)
 #pragma unroll
                 for (unsigned i = 0; i < 4u; ++i)
-#pragma unroll
-                    for (unsigned t = 0; t < SETS; ++t)
-                        if (!ok[bi][i]) s[t][bi][i] = -INFINITY;
+                    if (!ok[bi][i]) s[bi][i] = -INFINITY;
         }
-        float p[SETS][BLOCKS][4];
+        float p[BLOCKS][4], top = -INFINITY;
 #pragma unroll
-        for (unsigned t = 0; t < SETS; ++t) {
-            float top = -INFINITY;
+        for (unsigned bi = 0; bi < BLOCKS; ++bi)
 #pragma unroll
-            for (unsigned bi = 0; bi < BLOCKS; ++bi)
+            for (unsigned i = 0; i < 4u; ++i) top = __builtin_fmaxf(top, s[bi][i]);
+        top = mt_fold_g(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+        if (__any(top > m)) {
+            const float grown = __builtin_fmaxf(m, top);
+            const float by = grown > m ? __builtin_amdgcn_exp2f(m - grown) : 1.f;
+            m = grown;
+            l *= by;
+            mt_f32x4 rows_by;
 #pragma unroll
-                for (unsigned i = 0; i < 4u; ++i) top = __builtin_fmaxf(top, s[t][bi][i]);
-            top = mt_fold_g(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
-            if (__any(top > m[t])) {
-                const float grown = __builtin_fmaxf(m[t], top);
-                const float by = grown > m[t] ? __builtin_amdgcn_exp2f(m[t] - grown) : 1.f;
-                m[t] = grown;
-                l[t] *= by;
-                if constexpr (WIDE) {
-                    mt_f32x4 rows_by;
+            for (unsigned i = 0; i < 4u; ++i) rows_by[i] = __shfl(by, (int)(4u * g + i), 64);
 #pragma unroll
-                    for (unsigned i = 0; i < 4u; ++i) rows_by[i] = __shfl(by, (int)(4u * g + i), 64);
+            for (unsigned i = 0; i < NV * VV; ++i) acc[i] = acc[i] * rows_by;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                    for (unsigned i = 0; i < NV * VV; ++i) acc[t][i] = acc[t][i] * rows_by;
-                } else {
-                    const float row_by = __shfl(by, (int)(4u * g), 64);
+        for (unsigned bi = 0; bi < BLOCKS; ++bi)
 #pragma unroll
-                    for (unsigned i = 0; i < NV * VV; ++i) acc[t][i] = acc[t][i] * row_by;
-                }
+            for (unsigned i = 0; i < 4u; ++i) {
+                const float e = __builtin_amdgcn_exp2f(s[bi][i] - base);
+                l += e;
+                p[bi][i] = WIDE ? e : e * vs[bi][i];
             }
-            const float base = m[t] == -INFINITY ? 0.f : m[t];
-#pragma unroll
-            for (unsigned bi = 0; bi < BLOCKS; ++bi)
-#pragma unroll
-                for (unsigned i = 0; i < 4u; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(s[t][bi][i] - base);
-                    l[t] += e;
-                    p[t][bi][i] = WIDE ? e : e * vs[bi][i];
-                }
-        }
         if (!whole) {
 #pragma unroll
             for (unsigned bi = 0; bi < BLOCKS; ++bi)
 #pragma unroll
                 for (unsigned i = 0; i < 4u; ++i) {
                     if (ok[bi][i]) continue;
-#pragma unroll
-                    for (unsigned t = 0; t < SETS; ++t) p[t][bi][i] = 0.f;
+                    p[bi][i] = 0.f;
 #pragma unroll
                     for (unsigned c = 0; c < NV; ++c)
 #pragma unroll
@@ -1037,20 +1016,19 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
                 for (unsigned c = 0; c < NV; ++c)
 #pragma unroll
                     for (unsigned e = 0; e < VV; ++e)
-                        acc[0][VV * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][0][i], __uint_as_float(vw[0][i][c][e]),
-                                                                                  acc[0][VV * c + e], 0, 0, 0);
+                        acc[VV * c + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[0][i], __uint_as_float(vw[0][i][c][e]),
+                                                                               acc[VV * c + e], 0, 0, 0);
         } else {
-            mt_u32x4 pb[SETS];
+            mt_u32x4 pb[SPLIT];
 #pragma unroll
-            for (unsigned t = 0; t < SETS; ++t)
+            for (unsigned j = 0; j < SPLIT; ++j) {
+                pb[j] = mt_u32x4{mt_bf16_pair(p[0][0], p[0][1]), mt_bf16_pair(p[0][2], p[0][3]),
+                                 mt_bf16_pair(p[BLOCKS - 1u][0], p[BLOCKS - 1u][1]), mt_bf16_pair(p[BLOCKS - 1u][2], p[BLOCKS - 1u][3])};
 #pragma unroll
-                for (unsigned bi = 0; bi < 2u; ++bi) {
-                    float f[4];
+                for (unsigned bi = 0; bi < BLOCKS; ++bi)
 #pragma unroll
-                    for (unsigned i = 0; i < 4u; ++i) f[i] = mt_bf16_part(p[t][bi % BLOCKS][i], n & 3u);
-                    pb[t][2u * bi] = mt_bf16_pair(f[0], f[1]);
-                    pb[t][2u * bi + 1u] = mt_bf16_pair(f[2], f[3]);
-                }
+                    for (unsigned i = 0; i < 4u; ++i) p[bi][i] = mt_bf16_rest(p[bi][i]);
+            }
 #pragma unroll
             for (unsigned c = 0; c < NV; ++c)
 #pragma unroll
@@ -1064,8 +1042,8 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
                         const mt_u32x2 v0 = mt_held4_bf16<KIND>(lo[u]), v1 = mt_held4_bf16<KIND>(hi[u]);
                         const mt_u32x4 v8 = {v0.x, v0.y, v1.x, v1.y};
 #pragma unroll
-                        for (unsigned t = 0; t < SETS; ++t)
-                            acc[t][VV * c + 4u * w + u] = mt_mfma16_bf16(pb[t], v8, acc[t][VV * c + 4u * w + u]);
+                        for (unsigned j = 0; j < SPLIT; ++j)
+                            acc[VV * c + 4u * w + u] = mt_mfma16_bf16(pb[j], v8, acc[VV * c + 4u * w + u]);
                     }
                 }
         }
@@ -1080,31 +1058,22 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
     // A part weighs 2^(m - the largest m); one whose scores are all -inf weighs nothing
     // and says in l whether it has positions: a softmax over such scores alone is 0 / 0,
     // one over no positions gives zeros.
-#pragma unroll
-    for (unsigned t = 0; t < SETS; ++t) {
-        l[t] = mt_fold_g(l[t], [](float x, float y) { return x + y; });
-        if (m[t] == -INFINITY) l[t] = seen ? 1.f : 0.f;
-        const unsigned h = WIDE ? n : 4u * t + (n >> 2);
-        if (g == 0u && h < HELD && (WIDE || (n & 3u) == 0u)) {
-            ms[wave * HELD + h] = m[t];
-            ls[wave * HELD + h] = l[t];
-        }
-#pragma unroll
-        for (unsigned c = 0; c < NV; ++c)
-#pragma unroll
-            for (unsigned e = 0; e < VV; ++e) {
-                const unsigned d = VV * (16u * c + n) + e;
-                if (D % (16u * VV) != 0u && d >= D) continue;
-                const mt_f32x4 a = acc[t][VV * c + e];
-                if constexpr (WIDE) {
-#pragma unroll
-                    for (unsigned i = 0; i < 4u; ++i)
-                        if (4u * g + i < HELD) sums[(wave * HELD + 4u * g + i) * D + d] = a[i];
-                } else {
-                    if (4u * t + g < HELD) sums[(wave * HELD + 4u * t + g) * D + d] = a[0] + a[1] + a[2];
-                }
-            }
+    l = mt_fold_g(l, [](float x, float y) { return x + y; });
+    if (m == -INFINITY) l = seen ? 1.f : 0.f;
+    if (g == 0u && n < HELD) {
+        ms[wave * HELD + n] = m;
+        ls[wave * HELD + n] = l;
     }
+#pragma unroll
+    for (unsigned c = 0; c < NV; ++c)
+#pragma unroll
+        for (unsigned e = 0; e < VV; ++e) {
+            const unsigned d = VV * (16u * c + n) + e;
+            if (D % (16u * VV) != 0u && d >= D) continue;
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i)
+                if (4u * g + i < HELD) sums[(wave * HELD + 4u * g + i) * D + d] = acc[VV * c + e][i];
+        }
     __syncthreads();
 
 #pragma unroll 1

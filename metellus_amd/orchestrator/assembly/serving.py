@@ -198,18 +198,10 @@ def attention_workgroups(pairs: int, capacity: int, step: int, batch: int, most:
 def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_name: str | None, batch: int) -> KernelGroup:
     spec, rows = op.spec, op.q.shape[0]
     share = op.heads // spec.kv_heads  # query heads of a key head
-    # Eight waves to a compute unit; four, with twice the registers each, where the sums
-    # of a wave's heads (or its tile of long fp32 rows) would not fit otherwise.
-    def heavy_with(held: int) -> bool:
-        sets = 1 if spec.dtype == "float32" else _ceil(held, 4)
-        return spec.dim > 128 or sets * spec.dim > (256 if spec.page_size % 16 == 0 else 128)
-
-    # At most 16 query heads at once, one fp32 MFMA's columns (four sets of bf16 ones); 8,
-    # and the keys read again for the others at the same time, where 16 long rows would not
-    # fit in registers or LDS, or where 8 leave eight waves (16 heads of 128 in int8: 130 us
-    # for 157, of 64 in pages of 20: 126 for 149; of 64 in pages of 16 16 do: 82 for 94).
-    held = min(share, 8 if spec.dim > 128 or (heavy_with(min(share, 16)) and not heavy_with(8)) else 16)
-    heavy = heavy_with(held)
+    # At most 16 query heads at once, an MFMA's columns; 8 of long fp32 rows.  Eight waves to
+    # a compute unit; four, with twice the registers each, for long rows.
+    heavy = spec.dim > 128
+    held = min(share, 8 if heavy and spec.dtype == "float32" else 16)
     parts = _ceil(share, held)
     pairs = rows * spec.kv_heads * parts
     waves, most = 4 if heavy else ATTENTION_WAVES, ATTENTION_WORKGROUPS
@@ -222,11 +214,11 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
     step = (16 if spec.dtype == "float32" else 32) * waves
     groups = attention_workgroups(pairs, op.capacity, step, batch, most)
     floats = _ceil(held * (spec.dim + 2), 4) * 4
-    # q's operands in LDS: 16 bytes a lane for 16 dims of fp32 columns, or for 32 (16) of bf16 sets
+    # q's operands in LDS: 16 bytes a lane for 16 dims of fp32, or for 32 (16) of three bf16 parts
     if spec.dtype == "float32":
         q_bytes = 1024 * (spec.dim // 16)
     else:
-        q_bytes = 1024 * _ceil(held, 4) * (spec.dim // (32 if spec.dim % 32 == 0 else 16))
+        q_bytes = 1024 * 3 * (spec.dim // (32 if spec.dim % 32 == 0 else 16))
     ws = WS_HEAD_BYTES + 4 * batch * groups * 2 * floats if groups > 1 else 0
     sig = _Signature()
     args = (sig.add("q", op.q), sig.add("cache", op.cache), sig.add("pages", op.pages), sig.add("lengths", op.lengths),

@@ -438,11 +438,15 @@ def _attention(dtype, heads, kv_heads, dim, page_size, width, lengths, seed=0, h
 
 def _attention_bound(ops: Operations) -> np.ndarray:
     """A score q . k * scale * log2(e): the factor rounds once, q times it once, the
-    products' fma chain dim times, the two halves' sum and a key's scale once more, so
-    (dim + 5) u of sum |q||k| scale, in both numerator and denominator: twice that in
+    products' fma chain dim times, the two halves' sum and a key's scale once more (8 bits:
+    hi's chain, mid's and lo's at 2^-8 of its size, their sum), so (dim + 5) u of sum
+    |q||k| scale, in both numerator and denominator: twice that in
     the exponent.  2^x of the device and the difference x - m add 2^-22 and u of the
     largest |score| log2(e).  Weights and sums are added in chains no longer than the
-    positions, with at most 3 more roundings for each joining step and a value's scale."""
+    positions, with at most 3 more roundings for each joining step and a value's scale.
+    (8 bits: a wave's sum rounds 3 times for each position of its own, for the parts of its
+    weight, and of n positions the first wave of at least two has 32 or (n + 32) / 2 at the
+    most, its weights' sum a few: under 2 (n + 16).)"""
     (op,) = ops.build()
     found = []
     get = lambda t: ops.uploads[t.buffer_key]  # noqa: E731
