@@ -497,6 +497,8 @@ MANY = [
     (36, 1, 256, 9, 30, [270]),
     (16, 1, 128, 5, 60, [300, 298, 7]),
     (33, 1, 128, 16, 20, [320, 1]),
+    # dims of which 32 is no divisor, with as many heads as are held at once and one more
+    (16, 1, 240, 16, 30, [480, 33]), (17, 1, 208, 7, 40, [280, 5]), (32, 2, 144, 16, 20, [300]), (5, 1, 176, 32, 9, [288, 100]),
 ]
 
 

@@ -400,3 +400,15 @@ def test_a_chain_that_begins_before_a_view_of_another_kernels_output_runs_after_
     ops.elementwise("add", out="z", operands=("e", "v"), **({"y_broadcast": "col"} if first == "reduction" else {}))
     groups = compile_program(ops)
     assert [g.bindings[1] if "e" in g.outputs or "z" in g.outputs else "h" for g in groups] == ["h", "z"]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "int8", "float8_e4m3"])
+def test_attention_of_every_dim_fits_in_lds(dtype):
+    for dim in range(16, 257, 16):
+        for share in (1, 3, 8, 16, 17):
+            for width in (1, 20, 1000):
+                ops = _ops(q=(2, share * dim), pages=((2, width), "int32"), lengths=((2,), "int32"))
+                ops.kv_cache("c", pages=9, page_size=16, kv_heads=1, dim=dim, dtype=dtype)
+                ops.paged_attention("q", cache="c", pages="pages", lengths="lengths", heads=share, out="o")
+                (g,) = compile_program(ops)
+                assert sum(a.shape[0] * 4 for f in g.kernel.fragments for a in f.tgmem_accesses) <= 163840
