@@ -1057,9 +1057,11 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 
     // A part weighs 2^(m - the largest m); one whose scores are all -inf weighs nothing
     // and says in l whether it has positions: a softmax over such scores alone is 0 / 0,
-    // one over no positions gives zeros.
+    // one over no positions gives zeros.  Maxima pass over scores that are NaN, sums do not:
+    // a part whose sum is NaN joins as one with a maximum, so that its NaN comes through.
     l = mt_fold_g(l, [](float x, float y) { return x + y; });
-    if (m == -INFINITY) l = seen ? 1.f : 0.f;
+    if (l != l) m = 0.f;
+    else if (m == -INFINITY) l = seen ? 1.f : 0.f;
     if (g == 0u && n < HELD) {
         ms[wave * HELD + n] = m;
         ls[wave * HELD + n] = l;

@@ -843,3 +843,72 @@ def test_a_cache_beyond_4_gib():
     for b in env.values():
         b.release()
     hip_backend.trim()
+
+
+# ---------------------------------------------------------------------------
+# keys that are NaN
+# ---------------------------------------------------------------------------
+
+
+def _with_nan_keys(ops: Operations, at) -> Operations:
+    """NaN in the key of head ``h`` at position ``p`` of sequence ``b``, for each (b, p, h) of ``at``."""
+    (op,) = ops.build()
+    spec, table = op.spec, ops.uploads["pages"]
+    k, v = (np.array(a) for a in spec.unpack(ops.uploads["cache"]))
+    for b, p, h in at:
+        k[table[b, p // spec.page_size] * spec.page_size + p % spec.page_size, h, 1] = np.nan
+    ops.from_numpy(spec.pack(k, v), "cache")
+    return ops
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page_size", [16, 12])
+def test_paged_attention_of_a_nan_key_alone_in_a_tile(dtype, page_size):
+    """The newest position, the only one of its tile, is NaN: so is the softmax, of its key
+    head alone.  Lengths of one more than any number of tiles of 16 and 32, and others."""
+    lengths = [1, 2, 17, 33, 49, 65, 97, 129, 161, 193, 257, 34, 40]
+    ops = _attention(dtype, 4, 2, 64, page_size, 24, lengths, seed=51)
+    _with_nan_keys(ops, [(b, n - 1, b % 2) for b, n in enumerate(lengths[:-2])] + [(11, 32, 0), (12, 5, 1)])
+    got, want = run(ops).env["o"], evaluate(ops)["o"]
+    with np.errstate(invalid="ignore"):
+        _close(got, want, _attention_bound(ops))
+    nan = np.isnan(got).reshape(len(lengths), 2, -1)
+    for b in range(len(lengths)):
+        bad = b % 2 if b < 11 else b - 11
+        assert np.all(nan[b, bad]) and not np.any(nan[b, 1 - bad])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_paged_attention_of_a_nan_key_alone_in_a_workgroups_part(dtype):
+    """Sequences split over workgroups, a last part of one position."""
+    for dim in (64, 256):
+        ops = _attention(dtype, 4, 2, dim, 16, 257, [4097], seed=52)
+        (g,) = compile_program(ops)
+        assert g.kernel.workspace_bytes > 0
+        _with_nan_keys(ops, [(0, 4096, 1)])
+        got, want = run(ops).env["o"], evaluate(ops)["o"]
+        with np.errstate(invalid="ignore"):
+            _close(got, want, _attention_bound(ops))
+        assert np.all(np.isnan(got.reshape(2, -1)[1])) and np.all(np.isfinite(got.reshape(2, -1)[0]))
+
+
+def test_paged_attention_of_a_nan_key_beside_scores_of_minus_infinity():
+    """A tile of one NaN score and others of -inf, next to tiles of finite scores and next
+    to tiles of -inf alone."""
+    ops = _attention("float32", 2, 1, 16, 16, 3, [48, 48, 48], seed=53)
+    (op,) = ops.build()
+    k, v = (np.array(a) for a in op.spec.unpack(ops.uploads["cache"]))
+    ops.uploads["q"][:] = np.abs(ops.uploads["q"])
+    for b in range(3):
+        at = ops.uploads["pages"][b][:, None] * 16 + np.arange(16)
+        k[at[1], 0, 0] = -np.inf
+        if b > 0:
+            k[at[1, 7], 0] = np.nan
+        if b > 1:
+            k[at[0], 0, 0] = k[at[2], 0, 0] = -np.inf
+    ops.from_numpy(op.spec.pack(k, v), "cache")
+    got, want = run(ops).env["o"], evaluate(ops)["o"]
+    assert np.all(np.isfinite(want[0])) and np.all(np.isnan(want[1:]))
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    ops.uploads["pages"][0, 1] = -1  # scores of -inf weigh what positions that are not there do
+    np.testing.assert_array_equal(got[0], run(ops).env["o"][0])
