@@ -111,8 +111,10 @@ def _primary_name(elem: ElementwiseOp) -> str | None:
 
 
 def _sole_consumer(graph: Graph, name: str) -> Vertex | None:
+    """The one reader of ``name``; None too where it reads a view of it, for a
+    kernel cannot read the buffer of a value that it makes itself."""
     readers = graph.consumers_of(name)
-    return readers[0] if len(readers) == 1 else None
+    return readers[0] if len(readers) == 1 and not graph.reads_view_of(readers[0], name) else None
 
 
 def _by_position(graph: Graph, ops) -> tuple[Op, ...]:
@@ -287,14 +289,16 @@ def try_multi_producer_chain_fuse(graph: Graph, blacklist: Blacklist) -> Graph |
             if ma.out.shape != mb.out.shape:
                 continue
             seeds = (ma.out.name, mb.out.name)
+            if any(c is pa or c is pb for name in seeds for c in graph.consumers_of(name)):
+                continue  # one matmul reads the other
             members: list[Vertex] = []
-            queue = [c for name in seeds for c in graph.consumers_of(name)]
+            queue = [c for name in seeds for c in graph.consumers_of(name) if name in c.inputs]
             while queue:
                 v = queue.pop()
                 if any(v is m for m in members) or v is pa or v is pb or not _is_elementwise_vertex(v):
                     continue
                 members.append(v)
-                queue.extend(c for name in v.outputs for c in graph.consumers_of(name))
+                queue.extend(c for name in v.outputs for c in graph.consumers_of(name) if name in c.inputs)
             if not members or (len(members) == 1 and len(members[0].ops) == 1):
                 continue
             chain = _by_position(graph, tuple(op for v in members for op in v.ops))
@@ -343,7 +347,7 @@ def try_prologue_absorb_multi(graph: Graph, blacklist: Blacklist) -> Graph | Non
         anchor_ids: list[int] = []
         for r in readers:
             anc = _anchor_of(r)
-            if anc is None or name not in _anchor_boundary_input_names(anc, r):
+            if anc is None or graph.reads_view_of(r, name) or name not in _anchor_boundary_input_names(anc, r):
                 break
             anchor_ids.append(id(anc))
         else:

@@ -9,11 +9,12 @@ contained op's program position, and ``check_dependencies`` verifies a
 rewritten graph against the original program.
 
 Views (transpose / reshape) are not graph nodes; a consumer of a view sees
-the view's name as an external input (reference: graph.py:21-24).  The
-position tie-break orders a view's owner before its consumers as long as each
-is a vertex of its own; a fused vertex stands at its earliest op, so the order
-also has an edge from the vertex that writes a view's owner to the view's
-readers.
+the view's name as an external input (reference: graph.py:21-24).  It reads
+the buffer of the view's owner all the same, so it counts as a reader of the
+owner: the owner's vertex exports it, ``consumers_of`` lists it, and the order
+has an edge to it (a fused vertex stands at its earliest op, so the position
+tie-break alone does not order the two).  No rewrite may put both into one
+vertex, whose kernel would read the buffer before it is written.
 
 Implementation notes (behaviour-neutral): the topological order and the
 producer map of an immutable graph are computed once and cached, and the
@@ -63,11 +64,12 @@ class Graph:
         (produced, never read).  A vertex exports its tensor iff something
         reads it or it is a program output."""
         read: set[str] = {t.name for op in program for t in op.inputs}
+        viewed: set[str] = {t.buffer_key for op in program for t in op.inputs}
         made: set[str] = {t.name for op in program for t in outs_of(op)}
         outs = frozenset(made - read) if program_outputs is None else frozenset(program_outputs)
         verts = []
         for op in program:
-            exported = tuple(t.name for t in outs_of(op) if t.name in read or t.name in outs)
+            exported = tuple(t.name for t in outs_of(op) if t.name in read or t.name in viewed or t.name in outs)
             verts.append(Vertex(ops=(op,), inputs=tuple(t.name for t in op.inputs), outputs=exported))
         return cls(
             vertices=tuple(verts),
@@ -137,9 +139,24 @@ class Graph:
     def producer_of(self, name: str) -> Vertex | None:
         return self._producers.get(name)
 
+    def _reads(self, vertex: Vertex) -> set[str]:
+        """What ``vertex`` reads: its inputs and the owners of the views among them."""
+        return set(vertex.inputs) | {self.owners[name] for name in vertex.inputs if name in self.owners}
+
+    @cached_property
+    def _consumers(self) -> dict[str, tuple[Vertex, ...]]:
+        found: dict[str, list[Vertex]] = {}
+        for v in self.topo_sort():
+            for name in self._reads(v):
+                found.setdefault(name, []).append(v)
+        return {name: tuple(vs) for name, vs in found.items()}
+
     def consumers_of(self, name: str) -> tuple[Vertex, ...]:
-        """Vertices reading ``name``, in topological order."""
-        return tuple(v for v in self.topo_sort() if name in v.inputs)
+        """Vertices reading ``name`` or a view of it, in topological order."""
+        return self._consumers.get(name, ())
+
+    def reads_view_of(self, vertex: Vertex, name: str) -> bool:
+        return any(self.owners.get(i) == name for i in vertex.inputs)
 
     def check_dependencies(self, original: Program) -> None:
         """Every producer->consumer edge of ``original`` must be honoured by
@@ -163,7 +180,7 @@ class Graph:
         made_by = {t.name: op for op in original for t in outs_of(op)}
         for op in original:
             for t in op.inputs:
-                prod = made_by.get(t.name)
+                prod = made_by.get(t.name) or made_by.get(t.buffer_key)
                 if prod is None:
                     continue
                 first_prod = min(where[id(prod)])
@@ -188,9 +205,10 @@ class Graph:
         """Collapse ``absorbed`` into one vertex holding ``ops`` (their union,
         in program order).  New inputs = absorbed inputs minus names made
         inside; new outputs = names made inside that a surviving vertex reads
-        or that are program outputs.  The new vertex takes the position of
-        the first absorbed vertex.  Raises if the collapse creates a cycle
-        (reference: graph.py:118-212)."""
+        (itself or a view of it) or that are program outputs.  The new vertex
+        takes the position of the first absorbed vertex.  Raises if the
+        collapse creates a cycle (reference: graph.py:118-212), or a vertex
+        that reads a view of what it makes."""
         if not absorbed:
             raise ValueError("replace: absorbed set is empty")
         present = {id(v) for v in self.vertices}
@@ -211,10 +229,13 @@ class Graph:
         read_outside: set[str] = set()
         for v in self.vertices:
             if id(v) not in taken:
-                read_outside.update(v.inputs)
+                read_outside.update(self._reads(v))
         read_inside: set[str] = set()
         for v in absorbed:
             read_inside.update(v.inputs)
+        for name in sorted(read_inside):
+            if self.owners.get(name) in made:
+                raise ValueError(f"replace: the collapsed vertex would read {name!r}, a view of {self.owners[name]!r}, which it makes")
         merged = Vertex(
             ops=tuple(ops),
             inputs=tuple(sorted(read_inside - made)),
@@ -270,6 +291,6 @@ class Graph:
         for name in vertex.outputs:
             if name in self.program_outputs:
                 raise ValueError(f"remove_vertex: output {name!r} is a program output; cannot remove")
-            if any(other is not vertex and name in other.inputs for other in self.vertices):
+            if any(other is not vertex and name in self._reads(other) for other in self.vertices):
                 raise ValueError(f"remove_vertex: output {name!r} still consumed by another vertex")
         return self._derive(tuple(v for v in self.vertices if v is not vertex))

@@ -1,8 +1,12 @@
 """Vertex graph substrate: construction, replace, topo order, flatten and the
 dependency check (assertions of the reference's tests/test_graph.py)."""
 
+import random
+
 import pytest
 
+from metellus_amd.api import compile_program
+from metellus_amd.orchestrator import fusion
 from orchestrator import Operations
 from orchestrator.graph import Graph, Vertex
 from orchestrator.ir import MatmulOp
@@ -201,3 +205,139 @@ def test_absorb_into_and_remove_vertex():
     g3.check_dependencies(prog)
     with pytest.raises(ValueError, match="empty"):
         g.absorb_into(m1, ())
+
+
+# -- views of values that a fused kernel would keep to itself ------------------
+
+
+def _wrong_views(program, vertices) -> list[str]:
+    """Views that some vertex reads although no vertex before it writes their owner."""
+    made = {op.out.name for op in program}
+    wrong, written = [], set()
+    for v in vertices:
+        for op in v.ops:
+            for t in op.inputs:
+                if t.buffer_key != t.name and t.buffer_key in made and t.buffer_key not in written:
+                    wrong.append(f"{t.name} of {t.buffer_key} in {op.out.name}")
+        written.update(v.outputs)
+    return wrong
+
+
+def _view_cases():
+    def norm_then_gram(ops):  # an elementwise value, its transpose and a sum with their product
+        ops.rms_norm("a", out="h")
+        ops.elementwise("exp", out="X", operands=("h",))
+        ops.transpose("X", out="Xt")
+        ops.matmul("Xt", "a", out="Y")
+        ops.elementwise("add", out="Z", operands=("X", "Y"))
+
+    def gram(ops):  # one product of a value and its transpose
+        ops.elementwise("exp", out="X", operands=("a",))
+        ops.transpose("X", out="Xt")
+        ops.matmul("X", "Xt", out="Y")
+
+    def chain(ops):  # an elementwise op of a value and its transpose
+        ops.elementwise("exp", out="X", operands=("a",))
+        ops.transpose("X", out="Xt")
+        ops.elementwise("add", out="Z", operands=("X", "Xt"))
+
+    def epilogue(ops):  # the same of a product
+        ops.matmul("a", "b", out="X")
+        ops.transpose("X", out="Xt")
+        ops.elementwise("add", out="Z", operands=("X", "Xt"))
+
+    def reduction(ops):  # a view's reduction beside a chain
+        ops.elementwise("exp", out="X", operands=("a",))
+        ops.elementwise("negate", out="Z", operands=("X",))
+        ops.transpose("X", out="Xt")
+        ops.reduction("sum", out="r", x="Xt")
+
+    def column(ops):  # a reduction's output as a column beside its epilogue
+        ops.reduction("sum", out="X", x="a")
+        ops.elementwise("recip", out="e", operands=("X",))
+        ops.reshape("X", (16, 1), out="Xc")
+        ops.elementwise("div", out="Z", operands=("b", "Xc"), y_broadcast="col")
+
+    def merge(ops):  # two products' sum, of which a view is read too
+        ops.matmul("a", "b", out="X")
+        ops.matmul("b", "a", out="W")
+        ops.elementwise("add", out="Z", operands=("X", "W"))
+        ops.transpose("X", out="Xt")
+        ops.matmul("Xt", "b", out="Y")
+
+    def merge_of_a_view(ops):  # ... where the second product reads a view of the first
+        ops.matmul("a", "b", out="X")
+        ops.transpose("X", out="Xt")
+        ops.matmul("Xt", "a", out="W")
+        ops.elementwise("exp", out="e", operands=("X",))
+        ops.elementwise("mul", out="Z", operands=("e", "W"))
+
+    def recomputed(ops):  # a prologue that two products share, and a third reads by a view
+        ops.elementwise("exp", out="X", operands=("a",))
+        ops.matmul("X", "b", out="Y")
+        ops.matmul("b", "X", out="W")
+        ops.reshape("X", (16, 16), out="Xs")
+        ops.matmul("Xs", "b", out="V")
+
+    return [norm_then_gram, gram, chain, epilogue, reduction, column, merge, merge_of_a_view, recomputed]
+
+
+@pytest.mark.parametrize("chains", [False, True])
+@pytest.mark.parametrize("case", _view_cases(), ids=lambda f: f.__name__)
+def test_the_owner_of_a_view_that_is_read_is_written_before(case, chains, monkeypatch):
+    monkeypatch.setattr(fusion, "MULTI_ANCHOR_MERGE_CHAINS", chains)
+    ops = Operations()
+    ops.input("a", shape=(16, 16))
+    ops.input("b", shape=(16, 16))
+    case(ops)
+    program = ops.build()
+    vertices = fusion.fuse(program)
+    assert _wrong_views(program, vertices) == []
+    g = Graph.from_program(program)
+    assert all("X" in v.outputs for v in g.vertices if v.ops[0].out.name == "X")
+    compile_program(ops)
+
+
+def test_a_vertex_may_not_read_a_view_of_what_it_makes():
+    ops = Operations()
+    ops.input("a", shape=(8, 8))
+    ops.elementwise("exp", out="X", operands=("a",))
+    ops.transpose("X", out="Xt")
+    ops.elementwise("add", out="Z", operands=("X", "Xt"))
+    g = Graph.from_program(ops.build())
+    (x, z) = g.vertices
+    assert g.consumers_of("X") == (z,) and g.reads_view_of(z, "X") and not g.reads_view_of(x, "X")
+    with pytest.raises(ValueError, match="a view of 'X', which it makes"):
+        g.replace(absorbed=(x, z), ops=(*x.ops, *z.ops))
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_programs_of_views(seed):
+    """Square matrices, so that every op fits every value: chains, products and row sums of
+    values, their transposes and reshapes, in any mixture."""
+    rng = random.Random(seed)
+    for _ in range(25):
+        ops = Operations()
+        names = ["a", "b"]
+        for n in names:
+            ops.input(n, shape=(8, 8))
+        for i in range(rng.randint(3, 9)):
+            kind, out = rng.choice(("exp", "add", "mul", "matmul", "view", "view", "reduce")), f"t{i}"
+            x, y = rng.choice(names), rng.choice(names)
+            if kind == "view":
+                ops.transpose(x, out=out)
+            elif kind == "exp":
+                ops.elementwise("exp", out=out, operands=(x,))
+            elif kind == "matmul":
+                ops.matmul(x, y, out=out)
+            elif kind == "reduce":
+                ops.reduction("max", out=out + "r", x=x)
+                ops.reshape(out + "r", (8, 1), out=out + "c")
+                ops.elementwise("subtract", out=out, operands=(y, out + "c"), y_broadcast="col")
+            else:
+                ops.elementwise(kind, out=out, operands=(x, y))
+            names.append(out)
+        program = ops.build()
+        vertices = fusion.fuse(program)
+        assert _wrong_views(program, vertices) == []
+        Graph.from_program(program).check_dependencies(program)
