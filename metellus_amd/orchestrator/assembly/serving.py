@@ -56,7 +56,7 @@ class _Signature:
         """The argument for ``t`` (``nullptr`` for a tensor that is not there)."""
         if t is None:
             return "nullptr"
-        self.buffers.append(f"{'' if out else 'const '}{_CTYPE[t.dtype]}* __restrict__ p_{role}")
+        self.buffers.append(f"{'' if out else 'const '}{_CTYPE[t.stored]}* __restrict__ p_{role}")
         self.bindings.append(t.buffer_key)
         return f"p_{role}"
 

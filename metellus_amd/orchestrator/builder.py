@@ -79,9 +79,10 @@ class Operations:
         dtype: str | None = None,
     ) -> Tensor:
         """Declare a caller-supplied tensor.  Redeclaring with the same shape
-        returns the existing tensor.  ``dtype`` (default: the program's) is one of
-        ``float32``, ``int32``, ``int8``, ``uint8``; the serving ops say which of
-        their operands take the others."""
+        returns the existing tensor.  ``dtype`` is what its elements are stored
+        as, one of ``float32`` (the default, whatever the program's label),
+        ``int32``, ``int8``, ``uint8``; the serving ops say which of their
+        operands take the others."""
         if dtype is not None and dtype not in ITEM_BYTES:
             raise ValueError(f"input: dtype must be one of {tuple(ITEM_BYTES)}; got {dtype!r}")
         return self._declare(name, shape, layout=layout, row_stride=row_stride, col_stride=col_stride, dtype=dtype)
@@ -92,7 +93,7 @@ class Operations:
         another type -- and storage owners (not views) are accepted
         (reference: builder.py:80-118)."""
         known = self._tensors.get(name)
-        want = known.dtype if known is not None and known.dtype in ITEM_BYTES else "float32"
+        want = known.stored if known is not None else "float32"
         if arr.dtype != np.dtype(want):
             raise ValueError(f"from_numpy: array dtype must be {want}; got {arr.dtype}")
         t = self._declare(name, tuple(arr.shape))
@@ -132,13 +133,14 @@ class Operations:
                     f"tensor {name!r} already declared with shape {known.shape}, "
                     f"cannot redeclare as {shape}"
                 )
-            if dtype is not None and known.dtype != dtype:
-                raise ValueError(f"tensor {name!r} already declared as {known.dtype}, cannot redeclare as {dtype}")
+            if dtype is not None and known.stored != dtype:
+                raise ValueError(f"tensor {name!r} already declared as {known.stored}, cannot redeclare as {dtype}")
             return known
         t = Tensor(
             name=name,
             shape=shape,
-            dtype=self._dtype if dtype is None else dtype,
+            dtype=self._label(dtype),
+            stored=dtype or "float32",
             layout=layout,
             row_stride=-1 if row_stride is None else row_stride,
             col_stride=-1 if col_stride is None else col_stride,
@@ -157,8 +159,8 @@ class Operations:
     def _lookup_float(self, name: str) -> Tensor:
         """An operand of the primitive ops, whose kernels read fp32."""
         t = self._lookup(name)
-        if t.dtype != "float32" and t.dtype in ITEM_BYTES:
-            raise ValueError(f"tensor {name!r} is {t.dtype}; this op takes fp32 tensors")
+        if t.stored != "float32":
+            raise ValueError(f"tensor {name!r} is {t.stored}; this op takes fp32 tensors")
         return t
 
     def _fresh(self, name: str, shape: tuple[int, ...], dtype: str | None = None) -> Tensor:
@@ -166,7 +168,11 @@ class Operations:
         validates, so a rejected op leaves no stray name."""
         if name in self._tensors:
             raise ValueError(f"output tensor {name!r} already defined; IR is SSA — pick a fresh name")
-        return Tensor(name=name, shape=tuple(shape), dtype=self._dtype if dtype is None else dtype)
+        return Tensor(name=name, shape=tuple(shape), dtype=self._label(dtype), stored=dtype or "float32")
+
+    def _label(self, dtype: str | None) -> str:
+        """fp32 tensors carry the program's label, whatever it is; others their type."""
+        return self._dtype if dtype in (None, "float32") else dtype
 
     def _emit(self, out: Tensor, op) -> Tensor:
         self._tensors[out.name] = out
@@ -380,7 +386,7 @@ class Operations:
         tk, tv, ts = self._lookup(k), self._lookup(v), self._lookup(slots)
         fresh = self._fresh(out, tc.shape, "uint8")
         op = CacheWriteOp(
-            written=Tensor(name=fresh.name, shape=tc.shape, dtype="uint8", buffer_key=tc.buffer_key),
+            written=Tensor(name=fresh.name, shape=tc.shape, dtype="uint8", stored="uint8", buffer_key=tc.buffer_key),
             cache=tc,
             spec=spec,
             k=tk,

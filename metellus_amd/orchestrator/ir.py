@@ -44,8 +44,7 @@ def _default_strides(shape: tuple[int, ...], layout: Layout) -> tuple[int, int]:
     raise ValueError(f"v0 supports 0D/1D/2D tensors only; got shape {shape}")
 
 
-# Bytes of an element.  Types that are not listed count as fp32, which is what
-# the four op kinds here compute in whatever the tensor's label.
+# Bytes of an element, by what a tensor's elements are stored as.
 ITEM_BYTES = {"float32": 4, "int32": 4, "int8": 1, "uint8": 1}
 
 
@@ -60,7 +59,9 @@ def _count(shape: tuple[int, ...]) -> int:
 class Tensor:
     """SSA value.  ``offset(row, col) = row*row_stride + col*col_stride``.
     ``row_stride``/``col_stride`` of -1 and ``buffer_key`` of "" are
-    sentinels filled in ``__post_init__`` (dense strides; own buffer)."""
+    sentinels filled in ``__post_init__`` (dense strides; own buffer).
+    ``dtype`` is a label, as in the reference; the elements are fp32 unless
+    ``stored`` says otherwise, which only the serving ops take."""
 
     name: str
     shape: tuple[int, ...]
@@ -69,8 +70,11 @@ class Tensor:
     row_stride: int = -1
     col_stride: int = -1
     buffer_key: str = ""
+    stored: str = "float32"
 
     def __post_init__(self) -> None:
+        if self.stored not in ITEM_BYTES:
+            raise ValueError(f"tensor elements are stored as one of {tuple(ITEM_BYTES)}; got {self.stored!r}")
         if any(d <= 0 for d in self.shape):
             raise ValueError(f"tensor dimensions must be positive; got shape {self.shape}")
         if self.row_stride == -1 or self.col_stride == -1:
@@ -84,7 +88,7 @@ class Tensor:
 
     @property
     def nbytes(self) -> int:
-        return ITEM_BYTES.get(self.dtype, 4) * _count(self.shape)
+        return ITEM_BYTES[self.stored] * _count(self.shape)
 
     @property
     def element_count(self) -> int:
@@ -123,6 +127,7 @@ class Tensor:
             row_stride=self.col_stride,
             col_stride=self.row_stride,
             buffer_key=self.buffer_key,
+            stored=self.stored,
         )
 
     def can_reshape_as_view(self, new_shape: tuple[int, ...]) -> bool:
@@ -155,6 +160,7 @@ class Tensor:
                 row_stride=self.row_stride,
                 col_stride=self.col_stride,
                 buffer_key=self.buffer_key,
+                stored=self.stored,
             )
         step = self.linear_step()
         assert step is not None
@@ -167,6 +173,7 @@ class Tensor:
             row_stride=rs,
             col_stride=cs,
             buffer_key=self.buffer_key,
+            stored=self.stored,
         )
 
 

@@ -27,14 +27,10 @@ import numpy as np
 
 from metellus_amd.orchestrator.builder import Operations
 from metellus_amd.orchestrator.dag import build_dag
-from metellus_amd.orchestrator.ir import ITEM_BYTES, outs_of
+from metellus_amd.orchestrator.ir import outs_of
 from metellus_amd.orchestrator.kernel_group import KernelGroup
 from metellus_amd.orchestrator.serving import CacheWriteOp
 from metellus_amd.runtime.program import Allocate, Dispatch, Download, Free, FromNumpy, Runtime
-
-
-def _host_dtype(t) -> np.dtype:
-    return np.dtype(t.dtype if t.dtype in ITEM_BYTES else np.float32)
 
 
 def schedule(
@@ -127,7 +123,7 @@ def schedule(
                     Download(
                         name=t.buffer_key,
                         shape=t.shape,
-                        dtype=_host_dtype(t),
+                        dtype=np.dtype(t.stored),
                         into=t.name,
                         row_stride=t.row_stride,
                         col_stride=t.col_stride,
@@ -135,7 +131,7 @@ def schedule(
                 )
             if k in names:
                 t = tensors[k]
-                steps.append(Download(name=k, shape=t.shape, dtype=_host_dtype(t), into=t.name))
+                steps.append(Download(name=k, shape=t.shape, dtype=np.dtype(t.stored), into=t.name))
             else:
                 steps.append(Free(name=k))
             retired.add(k)

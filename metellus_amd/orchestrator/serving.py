@@ -174,8 +174,8 @@ def quantize_rows(x: np.ndarray, dtype: str) -> tuple[np.ndarray, np.ndarray]:
 
 
 def _want(label: str, t: Tensor, dtype: str, shape: tuple[int, ...]) -> None:
-    if t.dtype != dtype:
-        raise ValueError(f"{label} must be {dtype}; got {t.dtype} ({t.name!r})")
+    if t.stored != dtype:
+        raise ValueError(f"{label} must be {dtype}; got {t.stored} ({t.name!r})")
     if t.shape != shape:
         raise ValueError(f"{label} must have shape {shape}; got {t.shape} ({t.name!r})")
 

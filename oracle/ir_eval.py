@@ -221,8 +221,7 @@ def evaluate(ops, inputs: dict | None = None) -> dict:
     storage: dict[str, np.ndarray] = {}
     src = ops.uploads if inputs is None else inputs
     for name, arr in src.items():
-        own = ops.tensors[name].dtype if name in ops.tensors else "float32"
-        storage[name] = np.ascontiguousarray(arr, dtype=own if own in ("int32", "int8", "uint8") else F32)
+        storage[name] = np.ascontiguousarray(arr, dtype=ops.tensors[name].stored if name in ops.tensors else F32)
     out: dict[str, np.ndarray] = {}
     for op in ops.build():
         if isinstance(op, ServingOp):

@@ -412,3 +412,32 @@ def test_attention_of_every_dim_fits_in_lds(dtype):
                 ops.paged_attention("q", cache="c", pages="pages", lengths="lengths", heads=share, out="o")
                 (g,) = compile_program(ops)
                 assert sum(a.shape[0] * 4 for f in g.kernel.fragments for a in f.tgmem_accesses) <= 163840
+
+
+@pytest.mark.parametrize("label", ["int8", "int32", "uint8", "float16", "anything"])
+def test_a_programs_dtype_is_a_label(label):
+    """Every op takes a program's tensors whatever its label says: they are fp32."""
+    ops = Operations(dtype=label)
+    for name in ("x", "y"):
+        assert ops.from_numpy(np.ones((4, 4), np.float32), name).dtype == label
+    ops.input("x", (4, 4), dtype="float32")
+    with pytest.raises(ValueError, match="already declared as float32"):
+        ops.input("x", (4, 4), dtype="int8" if label == "int8" else "int32")
+    ops.transpose("y", out="yt")
+    ops.matmul("x", "yt", out="m")
+    ops.elementwise("add", out="e", operands=("m", "yt"))
+    ops.reduction("sum", out="r", x="e")
+    ops.reshape("yt", (16,), out="f")  # a copy
+    ops.rms_norm("e", out="n")
+    ops.rms_norm("n", out="n8", scales="s")
+    ops.dequantize("n8", scales="s", out="d")
+    ops.elementwise("add", out="z", operands=("d", "x"))
+    assert all(t.dtype == label and t.nbytes == 4 * t.element_count for n, t in ops.tensors.items() if n != "n8")
+    assert ops.tensors["n8"].nbytes == 16
+    with pytest.raises(ValueError, match="x must be int8; got float32"):
+        ops.dequantize("x", scales="s", out="q")
+    with pytest.raises(ValueError, match="takes fp32 tensors"):
+        ops.elementwise("exp", out="q", operands=("n8",))
+    steps = schedule(ops, compile_program(ops)).fragments
+    assert {s.into: s.dtype for s in steps if isinstance(s, Download) and s.into in ("r", "z", "n8")} == {
+        "r": np.float32, "z": np.float32, "n8": np.int8}
