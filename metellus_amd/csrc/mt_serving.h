@@ -1162,10 +1162,16 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 // multiples of 2^-30 of a power of two above the largest, x = 2^(E-156) X, and
 // X = 2^24 d3 + 2^16 d2 + 2^8 d1 + d0 with digits of 8 bits.  The digits of 4
 // rows of x are the 16 rows of an MFMA 16x16x64; 16 weight rows are its columns.
-// What is lost is 2^-30 of the block's largest value per element; a block that
-// holds an infinity or a NaN counts as zeros there and is added in fp32, as the
-// formula says, at the end.  One or two rows of x (XR) make the digits of four or two
-// blocks at once instead.  x in 8 bits is 16 rows as it stands.
+// What is lost is under 2^-30 of that power of two per element.  Where four values in a
+// row, not all zero, lie below 2^-9 of it -- a few outliers stand far above the rest --
+// the rest could do with more, and the block goes without digits: it is added in fp32, as
+// is one that holds an infinity or a NaN.  So an element is off by at most 2^-21 of the
+// largest of its four, whatever the outliers' weights are.  Such a block costs about as
+// much again (one channel 1e4 times the others: 1 row, 11008 x 4096 7.3 -> 9.2 us; 4 rows,
+// 131072 x 4096 60 -> 72, in four blocks of the 32 112; all 32 blocks of one row 18); rows
+// without such blocks take what they took.  (A group's sum, up to 2^44, is times its scale
+// before x's exponent comes in: scales below 2^83.)  One or two rows of x (XR) make the
+// digits of four or two blocks at once instead.  x in 8 bits is 16 rows as it stands.
 //
 // With (n, g) = (lane % 16, lane / 16): lane (n, g) loads 16 bytes of weight row n, q of
 // k = 32 g .. + 31 of a block of 128, even ones in the low nibbles.  xor 0x88 turns q
@@ -1203,6 +1209,9 @@ MT_INLINE unsigned mt_max16(unsigned v) {
     step((unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
     return v;
 }
+
+// The larger of two; NaN where one is.
+MT_INLINE float mt_maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // a's upper half of the wave for b's lower half; a's odd rows of 16 for b's even ones.
 MT_INLINE void mt_swap32(unsigned& a, unsigned& b) {
@@ -1254,6 +1263,7 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
     constexpr unsigned BL = EIGHT ? 1u : 4u / XR;     // blocks of x made into digits at once
     constexpr unsigned DIGITS = 512u * XR * SETS;     // bytes of a block's digits: [SETS][4 XR rows][128]
     constexpr bool RAGGED = K % (128u * U) != 0u;
+    static_assert(SHARED || U / BL * SETS <= 16u, "a bit for each row of a chunk's blocks");
     static_assert(U % BL == 0u && (!SHARED || PB % U == 0u), "makings of digits are whole in a chunk, chunks in a phase");
     using OP = mt_operand<GB>;
     const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, wave = mt_wave();
@@ -1303,28 +1313,36 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
     // Row r's 16 bytes c of a block's digits stand at c ^ (r / 2 % 8): the 16 rows that a
     // quarter of a wave reads lie in different banks.
     const auto place = [](unsigned r, unsigned byte) { return 128u * r + (byte ^ (16u * (r / 2u % 8u))); };
-    // The digits of BL blocks to `to`, and E of this lane group's row and block (255: not finite).
+    // The digits of BL blocks to `to`, and E of this lane group's row and block (255: no
+    // digits, a block that is added in fp32).
     const auto make_digits = [&](const mt_u32x4 (&xv)[XV], unsigned char* to, int (&made)[SETS]) {
 #pragma unroll
         for (unsigned t = 0; t < SETS; ++t) {
-            unsigned top = 0u;  // the bits of |x| order as the values do, infinities and NaN last
+            float v[8], top[2];  // (NaN above all, as infinities are)
+#pragma unroll
+            for (unsigned j = 0; j < 8u; ++j) v[j] = __uint_as_float(xv[EIGHT ? 0u : 2u * t + j / 4u][j % 4u]);
+#pragma unroll
+            for (unsigned h = 0; h < 2u; ++h)
+                top[h] = mt_maximum(mt_maximum(mt_maximum(__builtin_fabsf(v[4u * h]), __builtin_fabsf(v[4u * h + 1u])),
+                                               __builtin_fabsf(v[4u * h + 2u])), __builtin_fabsf(v[4u * h + 3u]));
+            const int e = (int)((mt_max16(__float_as_uint(mt_maximum(top[0], top[1]))) >> 23) & 255u);
+            // Four values that are not all zero, all below 2^(E-135)?  The smallest top but 0 is
+            // the largest negated.  (Up to E = 8 a step is at most 2^-148.)
+            const unsigned a = 0u - __float_as_uint(top[0]), b = 0u - __float_as_uint(top[1]);
+            const int least = (e - 8) * 0x800000;
+            const bool wide = mt_max16(a > b ? a : b) > 0u - (unsigned)(least > 1 ? least : 1);
+            made[t] = wide ? 255 : e < 1 ? 1 : e;
             unsigned d[8];
 #pragma unroll
             for (unsigned j = 0; j < 8u; ++j) {
-                d[j] = xv[EIGHT ? 0u : 2u * t + j / 4u][j % 4u];
-                const unsigned a = d[j] & 0x7FFFFFFFu;
-                top = top > a ? top : a;
-            }
-            const int e = (int)(mt_max16(top) >> 23);
-            made[t] = e < 1 ? 1 : e;
-#pragma unroll
-            for (unsigned j = 0; j < 8u; ++j) {
-                const int whole = e == 255 ? 0 : (int)__builtin_ldexpf(__uint_as_float(d[j]), 156 - made[t]);
-                d[j] = ((unsigned)whole + 0x00808080u) ^ 0x00808080u;
+                const int whole = made[t] == 255 ? 0 : (int)__builtin_ldexpf(v[j], 156 - made[t]);
+                d[j] = (unsigned)whole + 0x00808080u;
             }
             unsigned ev[4], od[4];
             mt_bytes4(d[0], d[2], d[4], d[6], ev);
             mt_bytes4(d[1], d[3], d[5], d[7], od);
+#pragma unroll
+            for (unsigned i = 0; i < 3u; ++i) ev[i] ^= 0x80808080u, od[i] ^= 0x80808080u;
             unsigned char* block = to + (g / XR) * DIGITS + t * (512u * XR);
 #pragma unroll
             for (unsigned i = 0; i < 4u; ++i)
@@ -1332,10 +1350,11 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
         }
     };
 
-    bool special = false;
+    bool lacks = false;  // SHARED: whether a row has a block without digits in this phase
     int* es = reinterpret_cast<int*>(lds + (SHARED ? PB * DIGITS : 0u));  // SHARED: E, [PB][SETS][4]
     // SHARED: the digits of blocks p0 .. p0 + PB - 1.
     const auto make_phase = [&](unsigned p0) {
+        lacks = false;
         for (unsigned at = wave * BL; at < PB && p0 + at < NB; at += WAVES * BL) {
             mt_u32x4 xv[XV];
             load_x(p0 + at, xv);
@@ -1351,13 +1370,13 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
                 make_digits(xv, lds + at * DIGITS, made);
 #pragma unroll
                 for (unsigned t = 0; t < SETS; ++t) {
-                    special = special || made[t] == 255;
+                    lacks = lacks || made[t] == 255;
                     if (n == 0u) es[((at + g / XR) * SETS + t) * 4u + g % XR] = made[t];
                 }
             }
         }
         if constexpr (EIGHT) __syncthreads();
-        else special = __syncthreads_or(special);
+        else lacks = __syncthreads_or(lacks);
     };
 
     constexpr unsigned TILES = (N + 16u * R - 1u) / (16u * R);
@@ -1406,12 +1425,50 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
         for (unsigned r = 0; r < R; ++r)
 #pragma unroll
             for (unsigned a = 0; a < ACC; ++a) acc[r][a] = 0.f;
+        // The products of row m of x in block blk in fp32: a lane sums its 32 k of its weight
+        // rows (weights first, as a value of W is, so that nothing is larger on the way), the
+        // four pieces meet.
+        const auto add_plain = [&](unsigned blk, unsigned m) {
+            const float* xr = x + (size_t)(m0 + m) * XRS;
+            const unsigned k0 = blk * 128u + 32u * g;
+            float part[R];
+#pragma unroll
+            for (unsigned r = 0; r < R; ++r) part[r] = 0.f;
+            if (k0 < K) {
+                mt_f32x4 v[8];  // (all loads on the way together)
+                mt_u32x4 word[R];
+#pragma unroll
+                for (unsigned i = 0; i < 8u; ++i) v[i] = mt_row4<K, XCS>(xr, k0 + 4u * i);
+#pragma unroll
+                for (unsigned r = 0; r < R; ++r) word[r] = *reinterpret_cast<const mt_u32x4*>(wr[r] + (size_t)blk * 64u);
+#pragma unroll
+                for (unsigned r = 0; r < R; ++r) {
+                    const float by = scales[sr[r] + k0 / GROUP];
+                    float zero = 8.f;
+                    if constexpr (ZEROS) zero = zeros[sr[r] + k0 / GROUP];
+#pragma unroll
+                    for (unsigned i = 0; i < 32u; ++i)
+                        part[r] = __builtin_fmaf(v[i / 4u][i % 4u], ((float)((word[r][i / 8u] >> (4u * (i % 8u))) & 15u) - zero) * by, part[r]);
+                }
+            }
+#pragma unroll
+            for (unsigned r = 0; r < R; ++r) {
+                part[r] += mt_shfl_xor(part[r], 16);
+                part[r] += mt_shfl_xor(part[r], 32);
+#pragma unroll
+                for (unsigned t = 0; t < SETS; ++t)
+                    if (m / 4u == t && m % 4u == g) acc[r][t] += part[r];
+            }
+        };
         const mt_i32x4 zero4 = {0, 0, 0, 0};
         mt_u32x4 q[U][R], xv[XV];
         float s[R][GU], z[R][ZEROS ? GU : 1u];
         if (c0 < c1) {
+            // x first: its digits are made while the weights arrive (1 row, 11008 x 4096: 7.2 us,
+            // weights first 7.5).  Of more tiles weights first (8 rows, 8192 x 11008: 25 and 28).
+            if constexpr (!SHARED && R == 1u) load_x(c0 * U, xv);
             load_w(c0, q, s, z);
-            if constexpr (!SHARED) load_x(c0 * U, xv);
+            if constexpr (!SHARED && R != 1u) load_x(c0 * U, xv);
         }
 #pragma unroll 1
         for (unsigned phase = 0; phase < PHASES; ++phase) {
@@ -1428,6 +1485,9 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
             mt_u32x4 qn[U][R];
             float sn[R][GU], zn[R][ZEROS ? GU : 1u];
             if (c + 1u < c1) load_w(c + 1u, qn, sn, zn);
+            // Rows of the chunk's blocks that have no digits: bit 16 i + SETS b + t for E of set t
+            // and lane group i of making b.
+            unsigned long long plain = 0ull;
 #pragma unroll
             for (unsigned pu = 0; pu < U; pu += BL) {
                 mt_u32x4 xn[XV];
@@ -1439,7 +1499,8 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
                     if constexpr (!EIGHT) {
                         make_digits(xv, digits, made);
 #pragma unroll
-                        for (unsigned t = 0; t < SETS; ++t) special = special || made[t] == 255;
+                        for (unsigned t = 0; t < SETS; ++t)
+                            plain |= (__ballot(made[t] == 255) & 0x0001000100010001ull) << (pu / BL * SETS + t);
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                         __builtin_amdgcn_wave_barrier();
                     }
@@ -1538,6 +1599,20 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
                     for (unsigned i = 0; i < XV; ++i) xv[i] = xn[i];
                 }
             }
+            if constexpr (!EIGHT && !SHARED) {
+                if (__builtin_expect(plain != 0ull, 0)) {
+                    while (plain) {
+                        const unsigned bit = (unsigned)__builtin_ctzll(plain), i = bit / 16u, at = bit % 16u;
+                        plain &= plain - 1ull;
+                        add_plain(c * U + at / SETS * BL + i / XR, 4u * (at % SETS) + i % XR);
+                    }
+                    // What was on the way is loaded again: nothing of it is kept over these products.
+                    if (c + 1u < c1) {
+                        load_w(c + 1u, qn, sn, zn);
+                        load_x((c + 1u) * U, xv);
+                    }
+                }
+            }
 #pragma unroll
             for (unsigned r = 0; r < R; ++r) {
 #pragma unroll
@@ -1549,42 +1624,21 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
                 }
             }
         }
-        }
-        if constexpr (!EIGHT) {
-            if (SHARED ? special : __any(special)) {
-                // Rare: rows of x with infinities or NaN in a block.  Every lane sums its 32 k of
-                // its weight rows, the four pieces meet.
-#pragma unroll 1
-                for (unsigned blk = c0 * U; blk < c1 * U && blk < NB; ++blk)
-#pragma unroll 1
-                    for (unsigned m = 0; m < 4u * SETS && m0 + m < rows; ++m) {
-                        const float* xr = x + (size_t)(m0 + m) * XRS;
-                        bool bad = false;
-                        for (unsigned k = blk * 128u + lane; k < blk * 128u + 128u && k < K; k += 64u)
-                            bad = bad || !(__builtin_fabsf(xr[(size_t)k * XCS]) < INFINITY);
-                        if (!__any(bad)) continue;
-                        const unsigned k0 = blk * 128u + 32u * g;
-#pragma unroll
-                        for (unsigned r = 0; r < R; ++r) {
-                            float part = 0.f;
-                            if (k0 < K) {
-                                float zero = 8.f;
-                                if constexpr (ZEROS) zero = zeros[sr[r] + k0 / GROUP];
-#pragma unroll 1
-                                for (unsigned i = 0; i < 32u; ++i) {
-                                    const unsigned v = (wr[r][(size_t)blk * 64u + i / 2u] >> (4u * (i % 2u))) & 15u;
-                                    part += xr[(size_t)(k0 + i) * XCS] * ((float)v - zero);
-                                }
-                                part *= scales[sr[r] + k0 / GROUP];
-                            }
-                            part += mt_shfl_xor(part, 16);
-                            part += mt_shfl_xor(part, 32);
-#pragma unroll
-                            for (unsigned t = 0; t < SETS; ++t)
-                                if (m / 4u == t && m % 4u == g) acc[r][t] += part;
-                        }
+        if constexpr (SHARED && !EIGHT) {
+            if (__builtin_expect(lacks, 0)) {
+                constexpr unsigned MANY = 16u / SETS;  // blocks whose E the lanes look at together
+                for (unsigned b = phase * PB; b < NB && b < phase * PB + PB; b += MANY) {
+                    const unsigned blk = b + n / SETS;
+                    bool none = n < MANY * SETS && g < XR && blk < NB && blk < phase * PB + PB;
+                    if (none) none = es[((blk - phase * PB) * SETS + n % SETS) * 4u + g] == 255;
+                    for (unsigned long long plain = __ballot(none); plain; plain &= plain - 1ull) {
+                        const unsigned bit = (unsigned)__builtin_ctzll(plain);
+                        add_plain(b + bit % 16u / SETS, 4u * (bit % 16u % SETS) + bit / 16u);
                     }
+                }
+                if (cq < c1) load_w(cq, q, s, z);  // (as above)
             }
+        }
         }
         const auto put = [&](unsigned r, unsigned a, unsigned ln, float v) {
             const unsigned col = n0 + 16u * r + (ln & 15u), row = m0 + (EIGHT ? 4u * (ln >> 4) + a : 4u * a + (ln >> 4));

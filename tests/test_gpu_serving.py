@@ -912,3 +912,84 @@ def test_paged_attention_of_a_nan_key_beside_scores_of_minus_infinity():
     np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
     ops.uploads["pages"][0, 1] = -1  # scores of -inf weigh what positions that are not there do
     np.testing.assert_array_equal(got[0], run(ops).env["o"][0])
+
+
+# ---------------------------------------------------------------------------
+# 4-bit products of x with outliers
+# ---------------------------------------------------------------------------
+
+
+def _outlier_bound(ops: Operations, blocks) -> np.ndarray:
+    """As ``_int4_bound``, but a block of x in which a few values stand far above all
+    others (``blocks[m]`` names those of row m) is held to what products in fp32 are: a
+    weight rounds twice (q - z, times s), 32 terms of a lane's chain round once each, two
+    additions join the four lanes: 36 u of sum |x| |q - z| |s|, and no step of the largest."""
+    (op,) = ops.build()
+    x = np.abs(ops.uploads["x"].astype(np.float64))
+    s = ops.uploads["s"].astype(np.float64)
+    z = ops.uploads["z"].astype(np.float64) if op.zeros is not None else np.full(s.shape, 8.0)
+    raw, (rows, k), group = ops.uploads["w"], x.shape, op.group
+    q = np.empty((raw.shape[0], k))
+    q[:, 0::2], q[:, 1::2] = raw & 15, raw >> 4
+    own = np.abs(q - np.repeat(z, group, axis=1)) * np.abs(np.repeat(s, group, axis=1))
+    most = np.repeat((8 + np.abs(8 - z)) * np.abs(s), group, axis=1)
+    total, steps = np.zeros((rows, len(raw))), np.zeros((rows, len(raw)))
+    for m in range(rows):
+        for b in range(-(-k // 128)):
+            at = slice(128 * b, min(k, 128 * b + 128))
+            if b in blocks[m]:
+                total[m] += own[:, at] @ x[m, at] * (1 + 36 / (8 + k // group))
+            else:
+                total[m] += most[:, at] @ x[m, at]
+                steps[m] += x[m, at].max() * 2.0**-29 * (most[:, at].sum(axis=1) + 64 * np.abs(s[:, 128 * b // group : -(-at.stop // group)]).sum(axis=1))
+    return (8 + k // group + 8) * U * total + steps
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows, n, group, size", [
+    # splitting k (one, two and four tiles), sharing x's digits (one phase and several, 8 and 16 waves)
+    (1, 100, 32, 1e6), (1, 100, 64, 1e9), (2, 700, 32, 1e4), (3, 4100, 32, 3e5), (6, 4100, 64, 1e12), (16, 4100, 32, 1e6), (8, 9000, 32, 1e5),
+    (1, 24577, 32, 1e6), (2, 24577, 64, 1e7), (4, 24577, 32, 2e3), (6, 24577, 64, 1e6), (16, 16500, 32, 1e30), (9, 65540, 64, 1e6),
+])
+def test_matmul_int4_of_x_with_outliers(rows, n, group, size, zeros):
+    """Channels of x ``size`` times the others, whose weights are zero: the others' products
+    are as right as they are alone."""
+    k = 1696 if group == 32 else 1728
+    ops = _int4(rows, k, n, group, False, zeros, n + rows)
+    x, w = ops.uploads["x"], ops.uploads["w"]
+    channels = [(0, 5), (0, 130), (rows - 1, 700), (rows - 1, 701), (rows // 2, k - 1)]
+    blocks = [set() for _ in range(rows)]
+    if zeros:
+        z = ops.uploads["z"]
+        z[:] = np.round(z)
+    for m, at in channels:
+        x[m, at] = size * (1 + abs(x[m, at])) * (-1) ** at
+        blocks[m].add(at // 128)
+        q = z[:, at // group].astype(np.uint8) if zeros else np.full(n, 8, np.uint8)
+        w[:, at // 2] = (w[:, at // 2] & 0x0F) | (q << 4) if at % 2 else (w[:, at // 2] & 0xF0) | q
+    _close(run(ops).env["y"], evaluate(ops)["y"], _outlier_bound(ops, blocks))
+
+
+def test_matmul_int4_of_values_over_many_magnitudes():
+    """Values log-uniform over 2^-60 to 2^60, weights zero but for the smallest halves of
+    each block: what is left is held to its own size.  And subnormal values beside 1."""
+    rng = np.random.default_rng(60)
+    k, n = 512, 40
+    x = (2.0 ** rng.uniform(-60, 60, (3, k)) * rng.choice([-1, 1], (3, k))).astype(np.float32)
+    x[2] = (rng.integers(-2000, 2000, k) * 2.0**-149).astype(np.float32)
+    x[2, 7::128] = 1
+    ops = _int4(3, k, n, 128, False, False, 61)
+    ops.uploads["x"][:] = x
+    ops.uploads["s"][:] = 1.0
+    for m in range(3):
+        big = np.zeros(k, bool)
+        for b in range(0, k, 128):
+            a = np.abs(x[m, b : b + 128])
+            big[b : b + 128] = a > (np.median(a) if m < 2 else 0.5)
+        w = np.random.default_rng(m).integers(0, 16, (n, k)).astype(np.uint8)
+        w[:, big] = 8
+        ops.uploads["w"][:] = w[:, 0::2] | (w[:, 1::2] << 4)
+        got, want = run(ops).env["y"][m], evaluate(ops)["y"][m]
+        # every block is one of fp32 products: 36 u, and a wave's and the waves' sums
+        bound = (36 + k // 128 + 8) * U * (np.abs(w - 8.0) @ np.abs(x[m].astype(np.float64))) + 2.0**-149
+        _close(got, want, bound)
