@@ -1643,7 +1643,7 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
         const auto put = [&](unsigned r, unsigned a, unsigned ln, float v) {
             const unsigned col = n0 + 16u * r + (ln & 15u), row = m0 + (EIGHT ? 4u * (ln >> 4) + a : 4u * a + (ln >> 4));
             if (col < N && row < rows && (EIGHT || ln / 16u < XR))
-                y[(size_t)row * N + col] = EIGHT ? v * (xs[row] * 0.0625f) : v;
+                y[(size_t)row * N + col] = EIGHT ? (v * 0.0625f) * xs[row] : v;  // (a 16th of a subnormal scale loses bits)
         };
         if constexpr (SHARED) {
 #pragma unroll

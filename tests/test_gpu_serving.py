@@ -993,3 +993,15 @@ def test_matmul_int4_of_values_over_many_magnitudes():
         # every block is one of fp32 products: 36 u, and a wave's and the waves' sums
         bound = (36 + k // 128 + 8) * U * (np.abs(w - 8.0) @ np.abs(x[m].astype(np.float64))) + 2.0**-149
         _close(got, want, bound)
+
+
+def test_matmul_int4_of_subnormal_row_scales():
+    """x in 8 bits of rows so small that their scales are subnormal: y is their product
+    rounded, not one of a scale that lost bits."""
+    ops = _int4(5, 4096, 70, 64, True, False, 62)
+    ops.uploads["x"][:] = 127
+    ops.uploads["s"][:] = np.abs(ops.uploads["s"])
+    w = ops.uploads["w"]
+    w[:] = (w & 0x77) | 0x88  # q of 8 to 15
+    ops.uploads["xs"][:] = np.array([2.0**-149, 3 * 2.0**-149, 1000 * 2.0**-149, 1e-39, 0.01], np.float32)
+    _close(run(ops).env["y"], evaluate(ops)["y"], _int4_bound(ops) + 2.0**-149)
