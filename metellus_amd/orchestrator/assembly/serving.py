@@ -2,8 +2,11 @@
 ``csrc/mt_serving.h`` specialised for the op's sizes and strides.
 
 Bindings are the op's tensors in the order of the device function's
-parameters; the rows (or tokens) are a runtime dim.  How a kernel splits its
-work is chosen here, by sizes and types alone.
+parameters.  The rows (or tokens) of norms, cache ops and products are a runtime
+dim: a 4-bit product takes at most as many in a launch as it was cut for (the
+sets of rows are compiled in).  Attention has none: it is compiled for its number
+of sequences and the width of its table.  How a kernel splits its work is chosen
+here, by sizes and types alone.
 """
 
 from __future__ import annotations
@@ -231,7 +234,7 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
         lds_bytes=2 * q_bytes + 4 * waves * floats + 16,
         name="paged_attention",
     )
-    return _group(decision, sig, frag, function_name or f"paged_attention_{op.o.name}", {"M": rows},
+    return _group(decision, sig, frag, function_name or f"paged_attention_{op.o.name}", {},
                   (groups, 1, 1), 64 * waves, workspace_bytes=ws, workspace_batched=True,
                   workspace_waits=False)
 

@@ -453,3 +453,12 @@ def test_packing_scales_are_the_largest_over_the_peak_rounded_once(dtype, peak):
     for slot in range(spec.slots):
         _, scales = serving_eval._page_parts(spec, data, slot // 16)
         np.testing.assert_array_equal(scales[:, :, slot % 16], want[:, slot])
+
+
+def test_attention_has_no_runtime_rows():
+    """Its number of sequences is compiled in: no dim could name another."""
+    ops = _cache_ops()
+    ops.paged_attention("q", cache="cache", pages="pages", lengths="lengths", heads=4, out="o")
+    (g,) = compile_program(ops)
+    assert g.dims == () and g.kernel.dim_names == ()
+    assert hip_backend.compile_only(g.kernel.source) > 0
