@@ -1029,3 +1029,26 @@ def test_cache_scales_are_the_largest_over_the_peak_rounded_once(dtype):
     scales = np.stack([serving_eval._page_parts(spec, got, p)[1] for p in range(spec.pages)])
     np.testing.assert_array_equal(scales, want)
     _same_state(spec, got, evaluate(ops)["written"])
+
+
+def test_what_shares_the_workspace_is_right_as_well_as_repeatable():
+    """A split attention between a product summed in parts and the product of its output.
+    A product of k terms rounds at most k + 16 times on the way (its chain, 16 parts); the
+    attention's error goes through the second product."""
+    alone, ops = (_attention("int8", 8, 2, 64, 16, 256, [4096, 700], seed=40) for _ in range(2))
+    rng = np.random.default_rng(41)
+    _put(ops, "wv", rng.standard_normal((512, 64)).astype(np.float32))
+    _put(ops, "a", rng.standard_normal((64, 8192)).astype(np.float32))
+    _put(ops, "b", rng.standard_normal((8192, 64)).astype(np.float32))
+    ops.matmul("a", "b", out="c")
+    ops.matmul("o", "wv", out="p")
+    ops.elementwise("exp", out="e", operands=("o",))  # (o is read twice, so it stays a buffer)
+    assert sum(g.kernel.workspace_bytes > 0 for g in compile_program(ops)) >= 2
+    want, off, wv = evaluate(ops), _attention_bound(alone), np.abs(ops.uploads["wv"].astype(np.float64))
+    a, b = (np.abs(ops.uploads[n].astype(np.float64)) for n in "ab")
+    bounds = {"o": off, "c": (8192 + 16) * U * (a @ b), "p": off @ wv + (512 + 17) * U * (np.abs(want["o"]) @ wv)}
+    for _ in range(3):
+        env = run(ops).env
+        for name, bound in bounds.items():
+            _close(env[name], want[name], bound)
+    hip_backend.check_workspace()
