@@ -148,14 +148,14 @@ class KVCache:
 
 def quantize_rows(x: np.ndarray, dtype: str) -> tuple[np.ndarray, np.ndarray]:
     """Last-axis rows of fp32 in 8 bits (as bytes) and a fp32 scale each: the
-    largest magnitude over 127 (``int8``) or 448 (``float8_e4m3``), rounded once, the
+    largest magnitude times fp32's 1/127 (``int8``) or 1/448 (``float8_e4m3``), the
     values ``x / scale`` rounded to the nearest, ties to even.  A row of zeros has the
     scale 0; a row with a value that is not finite is zeros with the scale NaN."""
     x = np.asarray(x, dtype=np.float32)
     peak = _PEAK[dtype]
     top = np.abs(x).max(axis=-1)
     fine = np.isfinite(top)
-    scale = np.where(fine, np.where(fine, top, 0) / np.float32(peak), np.float32(np.nan)).astype(np.float32)
+    scale = np.where(fine, np.where(fine, top, 0) * (np.float32(1) / np.float32(peak)), np.float32(np.nan)).astype(np.float32)
     div = np.where(fine & (scale > 0), scale, 1).astype(np.float64)[..., None]
     v = np.where((fine & (scale > 0))[..., None], x, 0).astype(np.float64) / div  # 64 bits: borders fall as they should
     if dtype == "int8":

@@ -35,13 +35,14 @@ def nearest_e4m3(v: np.ndarray) -> np.ndarray:
 
 
 def quantize(row: np.ndarray, held: str):
-    """(bytes, scale) of one row: scale = max / 127 (int8) or / 448 (e4m3) rounded to float32."""
+    """(bytes, scale) of one row.  float32 rows: scale = max times float32's 1/127 or
+    1/448; float64 rows (a norm's): max / 127 rounded to float32."""
     row = np.asarray(row)
     if not np.all(np.isfinite(row)):
         return np.zeros(row.shape, np.uint8), F32(np.nan)
     peak = 127.0 if held == "int8" else 448.0
     top = np.abs(row).max()
-    scale = F32(F64(top) / peak)
+    scale = F32(top * (F32(1) / F32(peak))) if row.dtype == F32 else F32(top / peak)
     if scale == 0:
         return np.zeros(row.shape, np.uint8), scale
     v = row.astype(F64) / F64(scale)

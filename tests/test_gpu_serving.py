@@ -1007,30 +1007,6 @@ def test_matmul_int4_of_subnormal_row_scales():
     _close(run(ops).env["y"], evaluate(ops)["y"], _int4_bound(ops) + 2.0**-149)
 
 
-@pytest.mark.parametrize("dtype", ["int8", "float8_e4m3"])
-def test_cache_scales_are_the_largest_over_the_peak_rounded_once(dtype):
-    """2048 rows of N(0, 1), some of them very small or large, and the values beside them by
-    that scale."""
-    spec = KVCache(pages=16, page_size=64, kv_heads=2, dim=64, dtype=dtype)
-    rng = np.random.default_rng(71)
-    ops = Operations()
-    ops.kv_cache("cache", pages=16, page_size=64, kv_heads=2, dim=64, dtype=dtype)
-    ops.from_numpy(spec.empty(), "cache")
-    kv = rng.standard_normal((2, spec.slots, spec.row))
-    kv[:, :200] *= 2.0 ** rng.integers(-140, 120, (2, 200, 1))
-    for name, a in zip("kv", kv.astype(np.float32)):
-        _put(ops, name, a)
-    _put(ops, "slots", np.arange(spec.slots, dtype=np.int32))
-    ops.cache_write("cache", k="k", v="v", slots="slots", out="written")
-    got = run(ops).env["written"]
-    peak = 127.0 if dtype == "int8" else 448.0
-    top = np.abs(kv.astype(np.float32)).reshape(2, 16, 64, 2, 64).max(axis=-1).transpose(1, 0, 3, 2)
-    want = (top.astype(np.float64) / peak).astype(np.float32)
-    scales = np.stack([serving_eval._page_parts(spec, got, p)[1] for p in range(spec.pages)])
-    np.testing.assert_array_equal(scales, want)
-    _same_state(spec, got, evaluate(ops)["written"])
-
-
 def test_what_shares_the_workspace_is_right_as_well_as_repeatable():
     """A split attention between a product summed in parts and the product of its output.
     A product of k terms rounds at most k + 16 times on the way (its chain, 16 parts); the

@@ -443,18 +443,6 @@ def test_a_programs_dtype_is_a_label(label):
         "r": np.float32, "z": np.float32, "n8": np.int8}
 
 
-@pytest.mark.parametrize("dtype, peak", [("int8", 127.0), ("float8_e4m3", 448.0)])
-def test_packing_scales_are_the_largest_over_the_peak_rounded_once(dtype, peak):
-    spec = KVCache(pages=8, page_size=16, kv_heads=4, dim=32, dtype=dtype)
-    kv = np.random.default_rng(3).standard_normal((2, spec.slots, 4, 32)).astype(np.float32)
-    kv[0, :20] *= np.float32(1e-38)
-    data = spec.pack(kv[0], kv[1])
-    want = (np.abs(kv).max(axis=-1).astype(np.float64) / peak).astype(np.float32)
-    for slot in range(spec.slots):
-        _, scales = serving_eval._page_parts(spec, data, slot // 16)
-        np.testing.assert_array_equal(scales[:, :, slot % 16], want[:, slot])
-
-
 def test_attention_has_no_runtime_rows():
     """Its number of sequences is compiled in: no dim could name another."""
     ops = _cache_ops()
