@@ -339,8 +339,9 @@ MT_INLINE void mt_cache_put(unsigned char* cache, const mt_f32x4 (&v)[(D + 63u) 
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) top = __builtin_fmaxf(top, mt_shfl_xor(top, off));
         const bool fine = top < INFINITY;
-        // (the reciprocal's rounding moves a scale by an ulp at most; values are
-        // rounded against the scale that is stored)
+        // The largest times fp32's 1 / peak, as a division by a scalar is elsewhere on GPUs (torch's
+        // among them): two roundings, within 2^-23 of the quotient.  Caches that others
+        // wrote are then the same bytes.  Values are rounded against the scale that is stored.
         const float s = fine ? top * (1.0f / (KIND == 2 ? 448.0f : 127.0f)) : NAN;
         // Near the smallest scales the reciprocal overflows and steps times the
         // scale lose bits: there both sides of the quotient are taken 2^64 larger.

@@ -148,8 +148,8 @@ class KVCache:
 
 def quantize_rows(x: np.ndarray, dtype: str) -> tuple[np.ndarray, np.ndarray]:
     """Last-axis rows of fp32 in 8 bits (as bytes) and a fp32 scale each: the
-    largest magnitude times fp32's 1/127 (``int8``) or 1/448 (``float8_e4m3``), the
-    values ``x / scale`` rounded to the nearest, ties to even.  A row of zeros has the
+    largest magnitude times fp32's 1/127 (``int8``) or 1/448 (``float8_e4m3``), which is
+    within 2^-23 of the quotient, the values ``x / scale`` rounded to the nearest, ties to even.  A row of zeros has the
     scale 0; a row with a value that is not finite is zeros with the scale NaN."""
     x = np.asarray(x, dtype=np.float32)
     peak = _PEAK[dtype]

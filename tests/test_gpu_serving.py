@@ -1028,3 +1028,33 @@ def test_what_shares_the_workspace_is_right_as_well_as_repeatable():
         for name, bound in bounds.items():
             _close(env[name], want[name], bound)
     hip_backend.check_workspace()
+
+
+@pytest.mark.parametrize("dtype", ["int8", "float8_e4m3"])
+def test_cache_write_by_the_definition(dtype):
+    """2048 rows of N(0, 1), some of them very small or large, apart from the oracle: a scale is
+    the largest over the peak but for two roundings (2^-24 of it each, and half of the smallest
+    subnormal), a value the nearest multiple of it: half a step of x / scale off."""
+    spec = KVCache(pages=16, page_size=64, kv_heads=2, dim=64, dtype=dtype)
+    rng = np.random.default_rng(71)
+    ops = Operations()
+    ops.kv_cache("cache", pages=16, page_size=64, kv_heads=2, dim=64, dtype=dtype)
+    ops.from_numpy(spec.empty(), "cache")
+    kv = rng.standard_normal((2, spec.slots, spec.row))
+    kv[:, :200] *= 2.0 ** rng.integers(-140, 120, (2, 200, 1))
+    kv = kv.astype(np.float32)
+    for name, a in zip("kv", kv):
+        _put(ops, name, a)
+    _put(ops, "slots", np.arange(spec.slots, dtype=np.int32))
+    ops.cache_write("cache", k="k", v="v", slots="slots", out="written")
+    got = run(ops).env["written"]
+    peak = 127.0 if dtype == "int8" else 448.0
+    rows = kv.reshape(2, 16, 64, 2, 64).transpose(1, 0, 3, 2, 4).astype(np.float64)  # page, part, head, slot
+    parts = [serving_eval._page_parts(spec, got, p) for p in range(spec.pages)]
+    s, want = np.stack([p[1] for p in parts]).astype(np.float64), np.abs(rows).max(axis=-1) / peak
+    assert np.all(np.abs(s - want) <= want * 2.01 * 2.0**-24 + 2.0**-150)
+    raw = np.ascontiguousarray(np.stack([p[0] for p in parts]))
+    held = raw.view(np.int8).astype(np.float64) if dtype == "int8" else serving_eval.E4M3[raw]
+    v = np.clip(np.divide(rows, s[..., None], out=np.zeros_like(rows), where=s[..., None] > 0), -peak, peak)
+    half = 0.5 if dtype == "int8" else np.exp2(np.maximum(np.floor(np.log2(np.maximum(np.abs(v), 2.0**-6))), -6) - 4)
+    assert np.all(np.abs(held - v) <= half)

@@ -450,3 +450,23 @@ def test_attention_has_no_runtime_rows():
     (g,) = compile_program(ops)
     assert g.dims == () and g.kernel.dim_names == ()
     assert hip_backend.compile_only(g.kernel.source) > 0
+
+
+@pytest.mark.parametrize("dtype, peak", [("int8", 127.0), ("float8_e4m3", 448.0)])
+def test_packing_by_the_definition(dtype, peak):
+    """A scale is the largest over the peak but for two roundings (2^-24 of it each, and half of
+    the smallest subnormal); a value is the nearest multiple: half a step of x / scale off."""
+    spec = KVCache(pages=8, page_size=16, kv_heads=4, dim=32, dtype=dtype)
+    kv = np.random.default_rng(3).standard_normal((2, spec.slots, 4, 32)).astype(np.float32)
+    kv[0, :20] *= np.float32(1e-38)
+    data = spec.pack(kv[0], kv[1])
+    want = np.abs(kv).max(axis=-1).astype(np.float64) / peak
+    for slot in range(spec.slots):
+        values, scales = serving_eval._page_parts(spec, data, slot // 16)
+        s = scales[:, :, slot % 16].astype(np.float64)
+        assert np.all(np.abs(s - want[:, slot]) <= want[:, slot] * 2.01 * 2.0**-24 + 2.0**-150)
+        raw = np.ascontiguousarray(values[:, :, slot % 16])
+        held = raw.view(np.int8).astype(np.float64) if dtype == "int8" else serving_eval.E4M3[raw]
+        v = np.clip(kv[:, slot].astype(np.float64) / s[..., None], -peak, peak)
+        half = 0.5 if dtype == "int8" else np.exp2(np.maximum(np.floor(np.log2(np.maximum(np.abs(v), 2.0**-6))), -6) - 4)
+        assert np.all(np.abs(held - v) <= half)
