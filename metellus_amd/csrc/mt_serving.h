@@ -1465,11 +1465,13 @@ MT_INLINE void mt_matmul_int4(const float* x, const signed char* x8, const float
         mt_u32x4 q[U][R], xv[XV];
         float s[R][GU], z[R][ZEROS ? GU : 1u];
         if (c0 < c1) {
-            // x first: its digits are made while the weights arrive (1 row, 11008 x 4096: 7.2 us,
-            // weights first 7.5).  Of more tiles weights first (8 rows, 8192 x 11008: 25 and 28).
-            if constexpr (!SHARED && R == 1u) load_x(c0 * U, xv);
+            // x first where digits are made of it for one tile: while the weights arrive (1 row,
+            // 11008 x 4096: 7.2 us, weights first 7.5).  Of more tiles weights first (8 rows, 8192
+            // x 11008: 25 and 28), and for x in 8 bits, which is used with them.
+            constexpr bool AHEAD = !SHARED && !EIGHT && R == 1u;
+            if constexpr (AHEAD) load_x(c0 * U, xv);
             load_w(c0, q, s, z);
-            if constexpr (!SHARED && R != 1u) load_x(c0 * U, xv);
+            if constexpr (!SHARED && !AHEAD) load_x(c0 * U, xv);
         }
 #pragma unroll 1
         for (unsigned phase = 0; phase < PHASES; ++phase) {
