@@ -360,8 +360,9 @@ MT_INLINE void mt_cache_put(unsigned char* cache, const mt_f32x4 (&v)[(D + 63u) 
     }
 }
 
-// Bound: HBM, or the launch for few tokens.  8192 tokens of 8 heads of 128 in e4m3: 22.6
-// us, 3.7 TB/s, of which the look through the slots is about 4 us.
+// Bound: HBM, or the launch for few tokens.  8192 tokens of 8 heads of 128 in e4m3: 22.7
+// us, 3.7 TB/s (15.3 us at a copy's rate), of which the look through the slots is about 4 us;
+// in fp32 27 us, 5.0 TB/s.  The look grows with the square of the tokens: 32768 take 98 us.
 //
 // Token t's keys and values go to slot slots[t] (page slot / PS, row slot % PS);
 // a slot outside the cache is passed over, and of tokens that name the same
@@ -1168,9 +1169,9 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 // the rest could do with more, and the block goes without digits: it is added in fp32, as
 // is one that holds an infinity or a NaN.  So an element is off by at most 2^-21 of the
 // largest of its four, whatever the outliers' weights are.  Such a block costs about as
-// much again (one channel 1e4 times the others: 1 row, 11008 x 4096 7.3 -> 9.2 us; 4 rows,
-// 131072 x 4096 60 -> 72, in four blocks of the 32 112; all 32 blocks of one row 18); rows
-// without such blocks take what they took.  (A group's sum, up to 2^44, is times its scale
+// much again (one channel 1e4 times the others: 1 row, 11008 x 4096 8.2 -> 8.7 us; 4 rows,
+// 131072 x 4096 62 -> 75, in four blocks of the 32 112; all 32 blocks of one row 19); the
+// look for them costs others up to 4 % (8 rows, 11008 x 8192: 23.3 -> 24.3).  (A group's sum, up to 2^44, is times its scale
 // before x's exponent comes in: scales below 2^83.)  One or two rows of x (XR) make the
 // digits of four or two blocks at once instead.  x in 8 bits is 16 rows as it stands.
 //
@@ -1188,11 +1189,12 @@ MT_INLINE void mt_paged_attention(const float* q, const unsigned char* cache, co
 // weight rows and split k, each making the digits of its part as it goes, so that few
 // weight rows still keep many loads in flight.
 //
-// Bound: HBM, the weights once, for many weight rows (4 rows of x, 131072 x 4096: 54 us,
-// 5.3 TB/s).  For few a wave's share of k is a handful of blocks, and the waits for them
-// and the making of digits (about 12 vector instructions a value, in every workgroup)
-// count: 1 row, 11008 x 4096 7.5 us; 16 rows in 8 bits, 4096 x 11008 10.5; 5 rows, 4099 x
-// 5024 in groups of 32 15, of which vector instructions are 8.
+// Bound: HBM, the weights once, for many weight rows (n x k: 4 rows of x, 131072 x 4096:
+// 54 us, 5.3 TB/s).  For few a wave's share of k is a handful of blocks, and the waits for
+// them and the making of digits (about 12 vector instructions a value, in every workgroup)
+// count: 1 row, 11008 x 4096 7.3 us; 16 rows in 8 bits, 4096 x 11008 10.5; 5 rows, 4099 x
+// 5024 in groups of 32 15, of which vector instructions are 8; 11008 x 8192 in groups of 128
+// (48 MB, a copy's rate 8.7 us) 1 row 14, 8 rows 24, 16 rows 35, in 8 bits 15 and 22.
 // ---------------------------------------------------------------------------
 
 // The whole number that an MFMA's four digit rows stand for.

@@ -210,9 +210,10 @@ def _assemble_attention(decision: DecisionView, op: PagedAttentionOp, function_n
     waves, most = 4 if heavy else ATTENTION_WAVES, ATTENTION_WORKGROUPS
     if spec.dtype != "float32" and not heavy and op.capacity <= 512:
         # Short sequences in 8 bits: their ends are most of the time, and overlap where smaller
-        # workgroups share a compute unit (8 key heads of 128 in int8, four or two waves for
-        # eight: 1024 sequences of 256 keys 130, 110 and 175 us, 64 of 64 9.1, 8.2 and 13; 256
-        # of 512 55 and 62, 64 of 300 17.9 and 18.8; 64 of 1024 27 and 27; fp32 no faster).
+        # workgroups share a compute unit (8 key heads of 128 in int8, evenly ragged lengths, four
+        # or two waves for eight: 1024 sequences of up to 256 keys 130, 110 and 175 us, 64 of 64
+        # 9.1, 8.2 and 13; 256 of 512 55 and 62, 64 of 300 17.9 and 18.8; 64 of 1024 27 and 27;
+        # fp32 no faster).
         waves, most = (2, 4 * ATTENTION_WORKGROUPS) if op.capacity <= 256 else (4, 2 * ATTENTION_WORKGROUPS)
     step = (16 if spec.dtype == "float32" else 32) * waves
     groups = attention_workgroups(pairs, op.capacity, step, batch, most)
@@ -253,44 +254,48 @@ def int4_shape(rows: int, k: int, n: int, group: int, eight: bool, zeros: bool) 
     own) or waves that split k; ``waves`` of a workgroup, ``tiles`` of 16 weight rows
     that a wave takes together, blocks of 128 k that it loads ``together``; ``each`` row
     of x in a set of MFMA rows, ``sets`` of them; ``phase``, blocks of k whose digits
-    are in LDS at once."""
+    are in LDS at once.
+
+    Figures below: us a pass over three input sets in turn, sizes as weight rows x columns
+    (n x k), groups of 128 unless said."""
     held = min(rows, 16)
     sets = 1 if eight else _ceil(held, 4)
     each = 4 if eight or held > 2 else held
     # Enough weight rows for a tile to most waves of the GPU: the waves share x's digits
-    # (4 rows, 4096 x 131072: 54 us, splitting k 80; 8 rows, 4096 x 20480 18 and 24; 16400,
-    # the next tile after four a workgroup, 18 and 23; one row, 4096 x 20480 13.3 and 12.7,
-    # 24000 13.5 and 14.3).  Fewer rows: splitting k (8 rows, 4096 x 11008: 13.5, shared 18).
+    # (4 rows, 131072 x 4096: 62, splitting k 109; 8 rows, 20480 x 4096 18 and 26; 16400 x
+    # 4096, the next tile after four a workgroup, 18 and 24; one row, 24000 x 4096 13.5 and
+    # 13.6).  Fewer rows: splitting k (8 rows, 16384 x 4096: 15, shared 18; 11008 x 4096 14, 17).
     shared = _ceil(n, 16) > 4 * INT4_WORKGROUPS if rows > 4 else _ceil(n, 16) >= 5 * INT4_WORKGROUPS
     blocks = _ceil(k, 128)
     made = 1 if eight else 4 // each  # blocks of x made into digits at once
     tiles, waves, together = 1, 8, 4
     if shared:
         # Sixteen waves to a making of digits, each making some, where they still leave a
-        # workgroup to each compute unit (fp32, 131072 x 4096: 8 rows 71 us, eight waves 78;
-        # 16 rows 90 and 118; 4 rows 59 and 55; groups of 32 with zeros 65536 x 2048: 44, 41).
+        # workgroup to each compute unit (fp32, 131072 x 4096: 8 rows 80, eight waves 84; 16
+        # rows 102 and 118; 4 rows 69 and 61; 8 rows, groups of 32 with zeros, 65536 x 2048: 43, 43).
         if sets > 1 and group > 32 and _ceil(n, 16) >= 16 * INT4_WORKGROUPS:
             waves, together = 16, 2
     else:
         # Two tiles a wave halve the work on x, once one is more than a workgroup to each
-        # compute unit (5 rows, 5024 x 4099: 15 us, one tile 17; 16 rows 24 and 35; 8 bits,
-        # 16 rows, 11008 x 8192: 15 and 19; up to 4 rows one tile is as fast or faster).
-        # Sixteen waves where it is not (1 row, 11008 x 4096: 9.5 us, 8 waves 11.2).
+        # compute unit (4099 x 5024, groups of 32 with zeros: 5 rows 16, one tile 18; 16 rows 24
+        # and 35; 8 bits, 16 rows, 8192 x 11008: 16 and 19; fp32, 4 rows 18, the one tile taken 20).
+        # Sixteen waves where it is not (1 row, 4096 x 11008: 7.9, eight waves 8.9).
         many = _ceil(n, 16) > INT4_WORKGROUPS
         tiles = 2 if rows > 4 and many else 1
-        # Four for fp32 where two are more than that and four are not, and their sums fit in
-        # registers (8 rows, 8192 x 11008, groups of 128 23 us, two tiles 30; 16 rows of
-        # groups of 64 45 and 59, of 32 71 and 73; 8 bits 25 and 25).
+        # Four for fp32 where two are more than that and four are not (11008 x 8192: 8 rows 24,
+        # two tiles 30; 16 rows 35 and 47, of groups of 64 39 and 52; in 8 bits 19, the two taken
+        # 22), as long as a block's sums and scales stay few (of groups of 32 two, 61; four, a
+        # block at once, 47).
         if tiles == 2 and 2 * INT4_WORKGROUPS < _ceil(n, 16) <= 4 * INT4_WORKGROUPS and not eight and sets * 128 // group < 16:
             tiles = 4
         waves = 16 if not many and sets <= 2 else 8
-        if eight:  # (1 row, 8192 x 11008: groups of 128 one block 17.3 us, two 15.3; of 32, 20.6 and 24.2)
+        if eight:  # (1 row, 11008 x 8192: groups of 128 one block 17.4, two 15.3; of 32, 20.9 and 24.3)
             together = 1 if group == 32 else 2
-        elif rows <= 2:  # (2 rows, 8192 x 11008: two blocks 16.8 us, four 18.2)
+        elif rows <= 2:  # (2 rows, 11008 x 8192: two blocks 16.2, four 16.7)
             together = made
         else:
-            # As many as leave the waves' shares even (5 rows, 5024 x 4099, 40 blocks: one
-            # 17 us, four 29), and whose scales fit in registers.
+            # As many as leave the waves' shares even (5 rows, 4099 x 5024, 40 blocks: one 16,
+            # two 18, four 29), and whose scales fit in registers.
             share = {u: _ceil(_ceil(blocks, u), waves) * u for u in (1, 2, 4)
                      if u == 1 or u * tiles * max(1, sets // 2) * (1 + zeros) <= group // 16}
             together = max(u for u in share if share[u] <= 1.1 * min(share.values()))
