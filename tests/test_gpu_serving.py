@@ -1058,3 +1058,31 @@ def test_cache_write_by_the_definition(dtype):
     v = np.clip(np.divide(rows, s[..., None], out=np.zeros_like(rows), where=s[..., None] > 0), -peak, peak)
     half = 0.5 if dtype == "int8" else np.exp2(np.maximum(np.floor(np.log2(np.maximum(np.abs(v), 2.0**-6))), -6) - 4)
     assert np.all(np.abs(held - v) <= half)
+
+
+@pytest.mark.parametrize("n, zeros", [(70, True), (70, False), (16400, True)])
+def test_matmul_int4_with_outliers_of_a_transposed_x_of_more_rows_than_one_pass(n, zeros):
+    """20 rows, the outliers in the first and the second pass's rows; alone, again, and in a batch."""
+    rows, k, group = 20, 416, 32
+    programs, bounds = [], []
+    for seed in (81, 82):
+        ops = _int4(rows, k, n, group, False, zeros, seed, strides=True)
+        x, w = ops.uploads["x_"], ops.uploads["w"]  # (columns of x_ are rows of x)
+        blocks = [set() for _ in range(rows)]
+        if zeros:
+            ops.uploads["z"][:] = np.round(ops.uploads["z"])
+        for m, at in ((0, 7), (3, 131), (16, 260), (19, k - 2)):
+            x[at, m] = 1e6
+            blocks[m].add(at // 128)
+            q = ops.uploads["z"][:, at // group].astype(np.uint8) if zeros else np.full(n, 8, np.uint8)
+            w[:, at // 2] = (w[:, at // 2] & 0x0F) | (q << 4) if at % 2 else (w[:, at // 2] & 0xF0) | q
+        programs.append(ops)
+        ops._uploads["x"] = np.ascontiguousarray(x.T)  # (for the bound alone)
+        bounds.append(_outlier_bound(ops, blocks))
+        del ops._uploads["x"]
+    for ops, got, bound in zip(programs, run_batch(programs), bounds):
+        want = evaluate(ops)["y"]
+        first = run(ops).env["y"]
+        _close(first, want, bound)
+        np.testing.assert_array_equal(got.env["y"], first)
+        np.testing.assert_array_equal(run(ops).env["y"], first)
