@@ -246,7 +246,7 @@ class _Program:
                        rotary=Rotary(dim=case["dim"], part=case["part"], layout=case["layout"], **more))
             return {"q": "q_out", "k": "k_out"}
         if case["op"] == "adapters":
-            ops.adapters("x", base="base", a="a", b="b", ids="ids", scales="scales", down="down", out="y")
+            ops.adapters("x", base="base", a="a", b="b", ids="ids", scales="scales", out="y")
             return {"y": "y"}
         ops.sample("logits", uniforms="uniforms", out="tokens", logprobs="logprobs",
                    **{n: n for n in ("temperatures", "top_k", "top_p", "min_p") if n in inputs})
