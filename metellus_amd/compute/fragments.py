@@ -146,25 +146,31 @@ def lds_decl(name: str, shape: tuple[int, ...]) -> str:
     return f"__shared__ alignas(16) float {name}{dims};"
 
 
-@functools.lru_cache(maxsize=1)
-def device_header() -> str:
-    """The hand-written gfx950 device library prepended to every kernel, without
-    its comment lines and blank lines: the text is joined, encoded and looked up
-    in the code-object cache on every compile of a kernel."""
-    path = os.path.join(os.path.dirname(os.path.dirname(__file__)), "csrc", "mt_device.h")
+@functools.lru_cache(maxsize=None)
+def _header(name: str) -> str:
+    """A file of ``csrc`` without its comment lines and blank lines: the text is
+    joined, encoded and looked up in the code-object cache on every compile of a
+    kernel."""
+    path = os.path.join(os.path.dirname(os.path.dirname(__file__)), "csrc", name)
     with open(path, encoding="utf-8") as f:
         lines = (line.rstrip() for line in f)
         return "".join(f"{line}\n" for line in lines if line and not line.lstrip().startswith("//"))
 
 
-@functools.lru_cache(maxsize=1)
+def device_header() -> str:
+    """The hand-written gfx950 device library prepended to every kernel."""
+    return _header("mt_device.h")
+
+
 def serving_header() -> str:
     """The device code of the serving operators, for the helpers of their
     kernels (the others do not carry it)."""
-    path = os.path.join(os.path.dirname(os.path.dirname(__file__)), "csrc", "mt_serving.h")
-    with open(path, encoding="utf-8") as f:
-        lines = (line.rstrip() for line in f)
-        return "".join(f"{line}\n" for line in lines if line and not line.lstrip().startswith("//"))
+    return _header("mt_serving.h")
+
+
+def decoding_header() -> str:
+    """The device code of the decoding operators; it follows ``serving_header``."""
+    return _header("mt_decoding.h")
 
 
 _PARAM_RE = re.compile(r"^\s*(const\s+)?(\w[\w ]*?)\s*\*\s*__restrict__\s+(\w+)\s*$")

@@ -1,0 +1,564 @@
+// mt_decoding.h -- device code of the decoding operators (gfx950): what a decode
+// step does around its products and attention.  Follows mt_device.h and
+// mt_serving.h in the kernels of these operators only; a generated kernel is one
+// call of one function here.
+//
+//   * mt_page_tables    block tables, slots and positions of a step's tokens
+//   * mt_rotary         queries and keys turned by their positions
+//   * mt_adapter_down / mt_adapter_up
+//                       low-rank adapters of many requests beside a shared product
+//   * mt_sample         tokens from logits and given random numbers
+
+// ---------------------------------------------------------------------------
+// Block tables.  A sequence goes from `begin` positions to `end`: of its table's row it
+// has `have` entries and needs `need` more.  Every workgroup adds up all sequences
+// (8 bytes each), lane t the `each` sequences from t each on, and keeps the sums before
+// each lane in LDS; a token row, or a new entry, finds its lane there and its sequence
+// behind it.  So no workgroup waits for another, and the numbers do not depend on how
+// many there are.  A launch reads entries below `have` alone and writes those from there
+// on, so the table can be written in place.
+// ---------------------------------------------------------------------------
+
+// Sums of rows stop at 2^31 - 1, behind any row.
+MT_INLINE unsigned mt_add_rows(unsigned a, unsigned b) {
+    const unsigned sum = a + b;
+    return sum > 0x7FFFFFFFu ? 0x7FFFFFFFu : sum;
+}
+
+template <unsigned P>
+struct mt_growth {
+    unsigned begin, end, rows, have, need;
+    MT_INLINE mt_growth(int length, int count, unsigned room) {
+        begin = length < 0 ? 0u : (unsigned)length < room ? (unsigned)length : room;
+        rows = count < 0 ? 0u : (unsigned)count;
+        end = begin + (rows < room - begin ? rows : room - begin);
+        have = (begin + P - 1u) / P;
+        need = (end + P - 1u) / P - have;
+    }
+};
+
+// The last lane whose sum `before` is not above v.
+template <unsigned LANES>
+MT_INLINE unsigned mt_lane_of(const unsigned* before, unsigned v) {
+    unsigned lo = 0u, hi = LANES;
+#pragma unroll 1
+    while (hi - lo > 1u) {
+        const unsigned mid = (lo + hi) / 2u;
+        if (before[mid] <= v) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <unsigned P, unsigned LANES>
+MT_INLINE void mt_page_tables(int* pages, const int* free, const int* lengths, const int* counts, int* slots,
+                              int* positions, int* ends, int* used, unsigned rows, unsigned sequences, unsigned width,
+                              unsigned frees, unsigned* lds) {
+    constexpr unsigned WAVES = LANES / 64u;
+    unsigned *rows_before = lds, *need_before = lds + LANES + 1u, *sums = lds + 2u * (LANES + 1u);
+    const unsigned t = threadIdx.x, room = width * P, each = (sequences + LANES - 1u) / LANES;
+    const unsigned first = t * each < sequences ? t * each : sequences;
+    const unsigned last = first + each < sequences ? first + each : sequences;
+    unsigned made = 0u, need = 0u;
+    for (unsigned b = first; b < last; ++b) {
+        const mt_growth<P> s(lengths[b], counts[b], room);
+        made = mt_add_rows(made, s.rows);
+        need += s.need;
+        if (blockIdx.x == 0u) ends[b] = (int)s.end;
+    }
+    // sums up to this lane
+#pragma unroll
+    for (unsigned off = 1u; off < 64u; off *= 2u) {
+        const unsigned a = __shfl_up(made, off, 64), b = __shfl_up(need, off, 64);
+        if (mt_lane() >= off) made = mt_add_rows(made, a), need += b;
+    }
+    if (mt_lane() == 63u) sums[mt_wave()] = made, sums[WAVES + mt_wave()] = need;
+    __syncthreads();
+    for (unsigned w = 0; w < mt_wave(); ++w) made = mt_add_rows(made, sums[w]), need += sums[WAVES + w];
+    rows_before[t + 1u] = made, need_before[t + 1u] = need;
+    if (t == 0u) rows_before[0] = 0u, need_before[0] = 0u;
+    __syncthreads();
+
+    const unsigned all_rows = rows_before[LANES], all_need = need_before[LANES], stride = gridDim.x * LANES;
+    for (unsigned row = blockIdx.x * LANES + t; row < rows; row += stride) {
+        int slot = -1, position = -1;
+        if (row < all_rows) {
+            const unsigned lane = mt_lane_of<LANES>(rows_before, row);
+            unsigned b = lane * each, i = row - rows_before[lane], page = need_before[lane];
+            mt_growth<P> s(lengths[b], counts[b], room);
+            while (i >= s.rows) {
+                i -= s.rows, page += s.need, ++b;
+                s = mt_growth<P>(lengths[b], counts[b], room);
+            }
+            if (i < s.end - s.begin) {
+                const unsigned at = s.begin + i, entry = at / P;
+                position = (int)at;
+                page += entry - s.have;  // (where the entry is new)
+                const int number = entry < s.have ? pages[(size_t)b * width + entry] : page < frees ? free[page] : -1;
+                const long long found = (long long)number * P + at % P;
+                if (number >= 0 && found <= 0x7FFFFFFFll) slot = (int)found;
+            }
+        }
+        slots[row] = slot, positions[row] = position;
+    }
+    for (unsigned e = blockIdx.x * LANES + t; e < all_need; e += stride) {
+        const unsigned lane = mt_lane_of<LANES>(need_before, e);
+        unsigned b = lane * each, i = e - need_before[lane];
+        mt_growth<P> s(lengths[b], counts[b], room);
+        while (i >= s.need) {
+            i -= s.need, ++b;
+            s = mt_growth<P>(lengths[b], counts[b], room);
+        }
+        pages[(size_t)b * width + s.have + i] = e < frees ? free[e] : -1;
+    }
+    if (blockIdx.x == 0u && t == 0u) *used = (int)all_need;
+}
+
+// ---------------------------------------------------------------------------
+// Rotary positions: y1 = c x1 - s x2, y2 = c x2 + s x1 for the pairs of a head's first R
+// elements, (i, i + R / 2) or, NEAR, (2 i, 2 i + 1); the others are copied.
+//
+// c and s belong to a position and a pair, and all heads share them: a workgroup works
+// them out for its TOK rows once, in 64 bits, and keeps them in LDS in 32.  The angle is
+// counted in turns, position times a turn's share per position, as the exact sum of two
+// doubles, of which whole turns are taken away before anything is rounded to the size of
+// the rest: an angle is right to 2^-51 of a turn at any int32 position.
+// ---------------------------------------------------------------------------
+
+template <unsigned D, unsigned R, bool NEAR, unsigned V, unsigned XH, unsigned XRS, unsigned XCS, unsigned KH,
+          unsigned KRS, unsigned KCS, unsigned TOK>
+MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, const double (*turns)[2],
+                         double magnitude, float* y, float* k_out, unsigned rows, mt_f32x2* lds) {
+    constexpr unsigned HALF = R / 2u, LANES = 256u;
+    // What a lane takes at once: V pairs of elements R / 2 apart, V / 2 (one at the least) of
+    // neighbours, or V elements that stay.
+    constexpr unsigned PAIRS = NEAR ? (V == 1u ? 1u : V / 2u) : V, TURNED = HALF / PAIRS, ITEMS = TURNED + (D - R) / V;
+    const unsigned first = blockIdx.x * TOK;
+    for (unsigned i = threadIdx.x; i < TOK * HALF; i += LANES) {
+        const unsigned row = first + i / HALF, pair = i % HALF;
+        if (row < rows) {
+            const double at = (double)positions[row], turn = turns[pair][0];
+            const double whole = at * turn, rest = __builtin_fma(at, turn, -whole) + at * turns[pair][1];
+            double s, c;
+            sincospi(2.0 * ((whole - __builtin_rint(whole)) + rest), &s, &c);
+            lds[i] = mt_f32x2{(float)(c * magnitude), (float)(s * magnitude)};
+        }
+    }
+    __syncthreads();
+    for (unsigned at = threadIdx.x; at < TOK * (XH + KH) * ITEMS; at += LANES) {
+        const unsigned item = at % ITEMS, head = at / ITEMS % (XH + KH), t = at / (ITEMS * (XH + KH)), row = first + t;
+        if (row >= rows) break;  // (the rows of what follows are no smaller)
+        const bool key = KH != 0u && head >= XH;
+        const unsigned h = key ? head - XH : head;
+        const float* from = key ? k + (size_t)row * KRS : x + (size_t)row * XRS;
+        const size_t cs = key ? KCS : XCS;
+        float* to = key ? k_out + ((size_t)row * KH + h) * D : y + ((size_t)row * XH + h) * D;
+        const auto load = [&](unsigned e) {
+            mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (V == 4u) v = mt_ld4u(from + h * D + e);
+            else v[0] = from[(h * D + e) * cs];
+            return v;
+        };
+        const auto store = [&](unsigned e, mt_f32x4 v) {
+            if constexpr (V == 4u) __builtin_nontemporal_store(v, reinterpret_cast<mt_f32x4u*>(to + e));
+            else to[e] = v[0];
+        };
+        if (item >= TURNED) {
+            const unsigned e = R + (item - TURNED) * V;
+            store(e, load(e));
+            continue;
+        }
+        const mt_f32x2* cs_of = lds + t * HALF + item * PAIRS;
+        if constexpr (!NEAR) {
+            const unsigned e = item * V;
+            const mt_f32x4 one = load(e), two = load(HALF + e);
+            mt_f32x4 a = one, b = two;
+#pragma unroll
+            for (unsigned j = 0; j < V; ++j) {
+                const mt_f32x2 w = cs_of[j];
+                a[j] = __builtin_fmaf(one[j], w.x, -(two[j] * w.y));
+                b[j] = __builtin_fmaf(two[j], w.x, one[j] * w.y);
+            }
+            store(e, a);
+            store(HALF + e, b);
+        } else if constexpr (V == 4u) {
+            const mt_f32x4 v = load(4u * item);
+            const mt_f32x2 w0 = cs_of[0], w1 = cs_of[1];
+            store(4u * item, mt_f32x4{__builtin_fmaf(v[0], w0.x, -(v[1] * w0.y)), __builtin_fmaf(v[1], w0.x, v[0] * w0.y),
+                                      __builtin_fmaf(v[2], w1.x, -(v[3] * w1.y)), __builtin_fmaf(v[3], w1.x, v[2] * w1.y)});
+        } else {
+            const float one = load(2u * item)[0], two = load(2u * item + 1u)[0];
+            const mt_f32x2 w = cs_of[0];
+            store(2u * item, mt_f32x4{__builtin_fmaf(one, w.x, -(two * w.y)), 0.f, 0.f, 0.f});
+            store(2u * item + 1u, mt_f32x4{__builtin_fmaf(two, w.x, one * w.y), 0.f, 0.f, 0.f});
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Low-rank adapters: out[m] = base[m] + s[id] B[id] (A[id] x[m]), id = ids[m].
+//
+// Rows are taken 16 at a time, an MFMA's columns.  Of the 16, those with the same id are a
+// group, led by its first row: each group reads its adapter once and multiplies all 16
+// rows (MFMA columns do not mix), of which it stores its own.  So a batch whose rows
+// each have an adapter reads each of them once, and so does one whose rows share one.
+// fp32 MFMAs 16x16x4: with (n, g) = (lane % 16, lane / 16) a lane has 4 consecutive k of
+// row n of both operands, k = 4 g + i in the i-th of four MFMAs; the order of k is the
+// same for both, so the sum is the product's.  An element (row 4 g + i, column n) of the
+// result is lane (n, g)'s i-th: rows are ranks, or columns of the output, so a lane has
+// four neighbours of row m = n of `down` or `out`.
+// ---------------------------------------------------------------------------
+
+// Of the 16 rows from row0: bit m says whether row m is of the group that row j leads;
+// 0 where j leads none.  `id`: its adapter, -1 for rows without one.
+template <unsigned HELD>
+MT_INLINE unsigned mt_adapter_group(const int* ids, unsigned row0, unsigned rows, unsigned j, int& id) {
+    const unsigned n = mt_lane() & 15u;
+    int mine = -2;
+    if (row0 + n < rows) {
+        mine = ids[row0 + n];
+        if (mine < 0 || (unsigned)mine >= HELD) mine = -1;
+    }
+    id = __builtin_amdgcn_readlane(mine, (int)j);
+    const unsigned group = (unsigned)__ballot(mine == id) & 0xFFFFu;
+    return id != -2 && (unsigned)__builtin_ctz(group) == j ? group : 0u;
+}
+
+MT_INLINE mt_f32x4 mt_mfma16_f32(mt_f32x4 a, mt_f32x4 b, mt_f32x4 c) {
+#pragma unroll
+    for (unsigned i = 0; i < 4u; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+
+// A's part: blocks of RB x 16 ranks; the waves of the SPLITS workgroups of a group take
+// 64 columns of x in turn and add up in LDS; each split stores its part.
+template <unsigned K, unsigned R, unsigned RB, unsigned SPLITS, unsigned HELD, unsigned WAVES, unsigned XRS, unsigned XCS>
+MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, float* down, unsigned rows,
+                               mt_f32x4* lds) {
+    const unsigned row0 = blockIdx.x / 16u * 16u, split = blockIdx.y % SPLITS, r0 = blockIdx.y / SPLITS * RB * 16u;
+    const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4;
+    int id;
+    const unsigned group = mt_adapter_group<HELD>(ids, row0, rows, blockIdx.x % 16u, id);
+    if (group == 0u || id < 0) return;
+    const bool mine = (group >> n) & 1u;
+    const float* xr = x + (size_t)(row0 + n) * XRS;
+    const float* ar = a + ((size_t)(unsigned)id * R + r0 + n) * K;
+    mt_f32x4 acc[RB];
+#pragma unroll
+    for (unsigned b = 0; b < RB; ++b) acc[b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (unsigned k0 = 64u * (split * WAVES + mt_wave()); k0 < K; k0 += 64u * SPLITS * WAVES) {
+#pragma unroll
+        for (unsigned u = 0; u < 4u; ++u) {
+            const unsigned k = k0 + 16u * u + 4u * g;
+            mt_f32x4 xv = {0.f, 0.f, 0.f, 0.f}, av[RB];
+            if (mine && k < K) xv = mt_row4<K, XCS>(xr, k);
+#pragma unroll
+            for (unsigned b = 0; b < RB; ++b) {
+                av[b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                if (r0 + 16u * b + n < R && k < K) av[b] = mt_row4<K, 1u>(ar + (size_t)(16u * b) * K, k);
+            }
+#pragma unroll
+            for (unsigned b = 0; b < RB; ++b) acc[b] = mt_mfma16_f32(av[b], xv, acc[b]);
+        }
+    }
+#pragma unroll
+    for (unsigned b = 0; b < RB; ++b) lds[(mt_wave() * RB + b) * 64u + lane] = acc[b];
+    __syncthreads();
+    for (unsigned e = threadIdx.x; e < RB * 64u; e += WAVES * 64u) {
+        mt_f32x4 v = lds[e];
+        for (unsigned w = 1; w < WAVES; ++w) v = v + lds[w * RB * 64u + e];
+        const unsigned m = e & 15u, r = r0 + e / 64u * 16u + (e / 16u & 3u) * 4u;
+        if ((group >> m) & 1u) {
+            float* to = down + ((size_t)split * rows + row0 + m) * R;
+#pragma unroll
+            for (unsigned i = 0; i < 4u; ++i)
+                if (r + i < R) to[r + i] = v[i];
+        }
+    }
+}
+
+// B's part and the sum: a wave takes PER blocks of 16 columns of the output.
+template <unsigned N, unsigned R, unsigned SPLITS, unsigned HELD, unsigned WAVES, unsigned PER, unsigned YRS,
+          unsigned YCS>
+MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* b, const int* ids, const float* scales,
+                             float* out, unsigned rows) {
+    constexpr unsigned RC = (R + 15u) / 16u;
+    const unsigned row0 = blockIdx.x / 16u * 16u, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
+    int id;
+    const unsigned group = mt_adapter_group<HELD>(ids, row0, rows, blockIdx.x % 16u, id);
+    if (group == 0u) return;
+    const bool mine = (group >> n) & 1u;
+    const unsigned row = row0 + n;
+    mt_f32x4 t[RC];
+#pragma unroll
+    for (unsigned c = 0; c < RC; ++c) {
+        t[c] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+        const unsigned r = 16u * c + 4u * g;
+        if (mine && id >= 0 && r < R)
+            for (unsigned s = 0; s < SPLITS; ++s) t[c] = t[c] + mt_row4<R, 1u>(down + ((size_t)s * rows + row) * R, r);
+    }
+    const float scale = scales != nullptr && id >= 0 ? scales[id] : 1.f;
+    const unsigned n0 = (blockIdx.y * WAVES + mt_wave()) * PER * 16u;
+#pragma unroll 1
+    for (unsigned p = 0; p < PER; ++p) {
+        const unsigned from = n0 + 16u * p, col = from + 4u * g;
+        if (from >= N) break;
+        mt_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (id >= 0) {
+            const float* br = b + ((size_t)(unsigned)id * N + from + n) * R;
+#pragma unroll
+            for (unsigned c = 0; c < RC; ++c) {
+                mt_f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+                if (from + n < N && 16u * c + 4u * g < R) bv = mt_row4<R, 1u>(br, 16u * c + 4u * g);
+                acc = mt_mfma16_f32(bv, t[c], acc);
+            }
+        }
+        if (mine && col < N) {
+            mt_f32x4 v = mt_row4<N, YCS>(base + (size_t)row * YRS, col);
+            if (id >= 0) {
+#pragma unroll
+                for (unsigned i = 0; i < 4u; ++i) v[i] = __builtin_fmaf(scale, acc[i], v[i]);
+            }
+            mt_put_row4<N>(out + (size_t)row * N, col, v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Sampling.  w_i = exp((x_i - max) / T), worked out in 64 bits and held as a whole
+// number of 2^-SHIFT: sums of whole numbers are the same in any order, so every cut and
+// the token are too.  A weight is off by 2^-SHIFT-1 of the largest at most.
+//
+// A cut -- the k largest, or the largest that weigh p of all -- is where the amount (ones,
+// or weights) that lies above a key first reaches what is asked for: it is looked for a
+// byte of the key at a time, the amounts of the 256 values of a byte added up in LDS.
+// Among equals at the cut the first indexes stay.
+// ---------------------------------------------------------------------------
+
+typedef unsigned long long mt_u64;
+
+// A float's place in the order of floats; -0 is 0.
+MT_INLINE unsigned mt_order_key(float x) {
+    const unsigned b = __float_as_uint(x + 0.0f);
+    return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+MT_INLINE float mt_order_value(unsigned key) {
+    return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+template <typename OP>
+MT_INLINE mt_u64 mt_wave_fold(mt_u64 v, OP op) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = op(v, (mt_u64)__shfl_xor(v, off, 64));
+    return v;
+}
+
+// v (op) over the workgroup's waves; `lds` holds a word a wave.
+template <unsigned WAVES, typename OP>
+MT_INLINE mt_u64 mt_group_fold(mt_u64 v, mt_u64* lds, OP op) {
+    v = mt_wave_fold(v, op);
+    __syncthreads();
+    if (mt_lane() == 0u) lds[mt_wave()] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (unsigned w = 1; w < WAVES; ++w) v = op(v, lds[w]);
+    return v;
+}
+
+// The sum of v over the lanes before this one; `all`: over all of them.
+template <unsigned WAVES>
+MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
+    mt_u64 sum = v;
+#pragma unroll
+    for (unsigned off = 1u; off < 64u; off *= 2u) {
+        const mt_u64 other = __shfl_up(sum, off, 64);
+        if (mt_lane() >= off) sum += other;
+    }
+    __syncthreads();
+    if (mt_lane() == 63u) lds[mt_wave()] = sum;
+    __syncthreads();
+    mt_u64 before = 0;
+    all = 0;
+#pragma unroll
+    for (unsigned w = 0; w < WAVES; ++w) {
+        before += w < mt_wave() ? lds[w] : 0;
+        all += lds[w];
+    }
+    return before + sum - v;
+}
+
+// The weights of a row.
+template <unsigned SHIFT>
+struct mt_weights {
+    float top;
+    double by;  // the temperature
+    MT_INLINE double scaled(float x) const { return ((double)x - (double)top) / by; }
+    MT_INLINE double weight(float x) const {
+        if (x == top) return 1.0;
+        return x == -INFINITY || top == INFINITY ? 0.0 : exp(scaled(x));  // (whatever the temperature)
+    }
+    MT_INLINE mt_u64 held(float x) const { return (mt_u64)__builtin_rint(weight(x) * (double)(1ull << SHIFT)); }
+};
+
+// A cut of a row: what stays lies above `key`, or is one of its equals up to index `last`.
+struct mt_cut_at {
+    unsigned key, last;
+    MT_INLINE bool stays(unsigned k, unsigned i) const { return k > key || (k == key && i <= last); }
+};
+
+// each(f) calls f(index, x) for this lane's elements.  The cut where amount(index, x),
+// added up from the largest x on, first reaches `asked` (1 at the least, all of it at the
+// most); `above`: the amount above its key, `at`: of its equals.
+template <unsigned WAVES, typename EACH, typename AMOUNT>
+MT_INLINE unsigned mt_find_cut(EACH each, AMOUNT amount, mt_u64 asked, mt_u64& above, mt_u64& at, mt_u64* lds) {
+    mt_u64* bins = lds + 2u * WAVES;
+    unsigned key = 0u;
+    above = 0;
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        if (threadIdx.x < 256u) bins[threadIdx.x] = 0;
+        __syncthreads();
+        const unsigned known = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
+        each([&](unsigned i, float x) {
+            const unsigned k = mt_order_key(x);
+            if ((k & known) == key) {
+                const mt_u64 v = amount(i, x);
+                if (v != 0) atomicAdd(bins + ((k >> shift) & 255u), v);
+            }
+        });
+        __syncthreads();
+        // lane t: bin 255 - t, so that sums before it are of larger keys
+        mt_u64 all;
+        const mt_u64 mine = threadIdx.x < 256u ? bins[255u - threadIdx.x] : 0;
+        const mt_u64 before = above + mt_group_before<WAVES>(mine, lds, all);
+        if (threadIdx.x < 256u && before < asked && asked <= before + mine) {
+            lds[WAVES] = 255u - threadIdx.x;
+            lds[WAVES + 1u] = before;
+            lds[WAVES + 2u] = mine;
+        }
+        __syncthreads();
+        key |= (unsigned)lds[WAVES] << shift;
+        above = lds[WAVES + 1u], at = lds[WAVES + 2u];
+    }
+    return key;
+}
+
+template <unsigned V, unsigned SHIFT, unsigned WAVES, unsigned RS, unsigned CS>
+MT_INLINE void mt_sample(const float* logits, const float* uniforms, const float* temperatures, const int* top_k,
+                         const float* top_p, const float* min_p, int* tokens, float* logprobs, mt_u64* lds) {
+    constexpr unsigned LANES = 64u * WAVES, STEP = 4u * LANES;
+    const unsigned row = blockIdx.x, t = threadIdx.x;
+    const float* x = logits + (size_t)row * RS;
+    const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
+    const auto each = [&](auto f) {
+        for (unsigned c = 4u * t; c < V; c += STEP) {
+            const mt_f32x4 v = mt_row4<V, CS>(x, c);
+#pragma unroll
+            for (unsigned j = 0; j < 4u; ++j)
+                if (c + j < V) f(c + j, v[j]);
+        }
+    };
+    // The first of the largest, by key and index; nothing is above a NaN.
+    mt_u64 best = 0;
+    each([&](unsigned i, float v) {
+        const mt_u64 found = v == v ? ((mt_u64)mt_order_key(v) << 32) | (0xFFFFFFFFu - i) : ~0ull;
+        best = found > best ? found : best;
+    });
+    best = mt_group_fold<WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
+    const float top = mt_order_value((unsigned)(best >> 32));
+    const float temperature = temperatures != nullptr ? temperatures[row] : 1.f;
+    const bool none = best == ~0ull || top == -INFINITY;
+    if (none || !(temperature > 0.f)) {
+        if (t == 0u) {
+            tokens[row] = none ? -1 : (int)(0xFFFFFFFFu - (unsigned)best);
+            if (logprobs != nullptr) logprobs[row] = none ? NAN : 0.f;
+        }
+        return;
+    }
+    const mt_weights<SHIFT> weights{top, (double)temperature};
+
+    mt_cut_at cut{0u, 0xFFFFFFFFu};
+    // The index of the n-th of those equal to `key`, of which there are more.
+    const auto nth = [&](unsigned key, mt_u64 n) {
+        mt_u64 seen = 0;
+        for (unsigned c0 = 0; c0 < V; c0 += STEP) {
+            const unsigned c = c0 + 4u * t;
+            unsigned hits = 0u;
+            if (c < V) {
+                const mt_f32x4 v = mt_row4<V, CS>(x, c);
+#pragma unroll
+                for (unsigned j = 0; j < 4u; ++j)
+                    if (c + j < V && mt_order_key(v[j]) == key) hits |= 1u << j;
+            }
+            mt_u64 all, before = seen + mt_group_before<WAVES>(__builtin_popcount(hits), lds, all);
+#pragma unroll
+            for (unsigned j = 0; j < 4u; ++j)
+                if ((hits >> j) & 1u) {
+                    if (++before == n) lds[WAVES] = c + j;
+                }
+            seen += all;
+            if (seen >= n) break;  // (the same in all lanes)
+        }
+        __syncthreads();
+        const unsigned found = (unsigned)lds[WAVES];
+        __syncthreads();
+        return found;
+    };
+    const int k = top_k != nullptr ? top_k[row] : 0;
+    if (k > 0 && (unsigned)k < V) {
+        mt_u64 above, at;
+        cut.key = mt_find_cut<WAVES>(each, [](unsigned, float) { return (mt_u64)1; }, (mt_u64)k, above, at, lds);
+        if ((mt_u64)k - above < at) cut.last = nth(cut.key, (mt_u64)k - above);
+    }
+    const float p = top_p != nullptr ? top_p[row] : 1.f;
+    if (p < 1.f) {
+        const mt_cut_at by_k = cut;
+        const auto amount = [&](unsigned i, float v) { return by_k.stays(mt_order_key(v), i) ? weights.held(v) : (mt_u64)0; };
+        mt_u64 total = 0;
+        each([&](unsigned i, float v) { total += amount(i, v); });
+        total = mt_group_fold<WAVES>(total, lds, sum);
+        // the first of them stays whatever p is
+        mt_u64 asked = p > 0.f ? (mt_u64)__builtin_ceil((double)p * (double)total) : 1, above, at;
+        asked = asked < 1 ? 1 : asked < total ? asked : total;
+        cut.key = mt_find_cut<WAVES>(each, amount, asked, above, at, lds);
+        if (cut.key != by_k.key) cut.last = 0xFFFFFFFFu;
+        const mt_u64 one = weights.held(mt_order_value(cut.key)), n = (asked - above + one - 1) / one;
+        if (n < at / one) cut.last = nth(cut.key, n);
+    }
+    const float m = min_p != nullptr ? min_p[row] : 0.f;
+    const double least = m > 0.f ? (double)__builtin_fminf(m, 1.f) : 0.0;
+    const auto amount = [&](unsigned i, float v) {
+        return cut.stays(mt_order_key(v), i) && !(weights.weight(v) < least) ? weights.held(v) : (mt_u64)0;
+    };
+    mt_u64 total = 0;
+    each([&](unsigned i, float v) { total += amount(i, v); });
+    total = mt_group_fold<WAVES>(total, lds, sum);
+    const float u = uniforms[row];
+    mt_u64 target = u > 0.f ? (mt_u64)((double)__builtin_fminf(u, 1.f) * (double)total) : 0;
+    if (target >= total) target = total - 1;
+    mt_u64 seen = 0;
+    for (unsigned c0 = 0; c0 < V; c0 += STEP) {
+        const unsigned c = c0 + 4u * t;
+        mt_u64 w[4] = {0, 0, 0, 0};
+        mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (c < V) v = mt_row4<V, CS>(x, c);
+#pragma unroll
+        for (unsigned j = 0; j < 4u; ++j)
+            if (c + j < V) w[j] = amount(c + j, v[j]);
+        mt_u64 all, before = seen + mt_group_before<WAVES>(w[0] + w[1] + w[2] + w[3], lds, all);
+#pragma unroll
+        for (unsigned j = 0; j < 4u; ++j) {
+            if (before <= target && target < before + w[j]) {
+                tokens[row] = (int)(c + j);
+                if (logprobs != nullptr)
+                    logprobs[row] = (float)((v[j] == top ? 0.0 : weights.scaled(v[j])) -
+                                            log((double)total / (double)(1ull << SHIFT)));
+            }
+            before += w[j];
+        }
+        seen += all;
+        if (seen > target) break;  // (the same in all lanes)
+    }
+}

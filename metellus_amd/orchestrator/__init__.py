@@ -5,6 +5,14 @@ submodules (as in the reference, src/orchestrator/__init__.py)."""
 from metellus_amd.compute.elementwise.elementwise import BroadcastSpec
 from metellus_amd.orchestrator.builder import Operations
 from metellus_amd.orchestrator.dag import DAG, build_dag
+from metellus_amd.orchestrator.decoding import (
+    AdapterDownOp,
+    AdapterUpOp,
+    PageTablesOp,
+    Rotary,
+    RotaryOp,
+    SampleOp,
+)
 from metellus_amd.orchestrator.graph import Graph, Vertex
 from metellus_amd.orchestrator.ir import (
     ElementwiseOp,
@@ -29,6 +37,8 @@ from metellus_amd.orchestrator.serving import (
 )
 
 __all__ = [
+    "AdapterDownOp",
+    "AdapterUpOp",
     "BroadcastSpec",
     "CacheReadOp",
     "CacheWriteOp",
@@ -43,10 +53,14 @@ __all__ = [
     "Op",
     "OperandValue",
     "Operations",
+    "PageTablesOp",
     "PagedAttentionOp",
     "Program",
     "ReductionOp",
     "RmsNormOp",
+    "Rotary",
+    "RotaryOp",
+    "SampleOp",
     "Scalar",
     "ShapeOp",
     "Tensor",

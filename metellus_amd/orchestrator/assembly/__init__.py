@@ -5,6 +5,7 @@ strategy's template."""
 from __future__ import annotations
 
 from metellus_amd.orchestrator.assembly.decision import classify
+from metellus_amd.orchestrator.assembly.decoding import DECODING, assemble_decoding
 from metellus_amd.orchestrator.assembly.elementwise import assemble_elementwise
 from metellus_amd.orchestrator.assembly.matmul import assemble_matmul
 from metellus_amd.orchestrator.assembly.multi_anchor import assemble_multi_anchor
@@ -48,6 +49,8 @@ def assemble(vertex: Vertex, *, function_name: str | None = None, batch: int = 1
         return assemble_multi_anchor(decision, function_name, batch=batch)
     if s in SERVING:
         return assemble_serving(decision, function_name, batch=batch)
+    if s in DECODING:
+        return assemble_decoding(decision, function_name)
     raise ValueError(f"unknown strategy {s!r}")
 
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 from metellus_amd.compute.elementwise.elementwise import TERNARY_EXPRESSIONS
+from metellus_amd.orchestrator.decoding import AdapterDownOp, AdapterUpOp, PageTablesOp, RotaryOp, SampleOp
 from metellus_amd.orchestrator.graph import Vertex
 from metellus_amd.orchestrator.ir import ElementwiseOp, MatmulOp, Op, ReductionOp, Scalar, ShapeOp, Tensor
 from metellus_amd.orchestrator.kernel_group import FusionStrategy
@@ -28,6 +29,11 @@ _SERVING = {
     CacheWriteOp: FusionStrategy.CACHE_WRITE,
     CacheReadOp: FusionStrategy.CACHE_READ,
     PagedAttentionOp: FusionStrategy.PAGED_ATTENTION,
+    PageTablesOp: FusionStrategy.PAGE_TABLES,
+    RotaryOp: FusionStrategy.ROTARY,
+    AdapterDownOp: FusionStrategy.ADAPTER_DOWN,
+    AdapterUpOp: FusionStrategy.ADAPTER_UP,
+    SampleOp: FusionStrategy.SAMPLE,
 }
 
 

@@ -1,0 +1,203 @@
+"""Decoding strategies: one kernel per op, a call of a device function of
+``csrc/mt_decoding.h`` specialised for the op's sizes and strides, as the serving
+strategies are.  How a kernel splits its work is chosen here, by sizes and types
+alone.
+"""
+
+from __future__ import annotations
+
+from metellus_amd.compute.fragments import decoding_header
+from metellus_amd.compute.serving import ServingFragment
+from metellus_amd.orchestrator.assembly.decision import DecisionView
+from metellus_amd.orchestrator.assembly.serving import _ceil, _group, _Signature
+from metellus_amd.orchestrator.decoding import AdapterDownOp, AdapterUpOp, PageTablesOp, Rotary, RotaryOp, SampleOp
+from metellus_amd.orchestrator.ir import Tensor
+from metellus_amd.orchestrator.kernel_group import FusionStrategy, KernelGroup
+
+DECODING = frozenset(
+    {
+        FusionStrategy.PAGE_TABLES,
+        FusionStrategy.ROTARY,
+        FusionStrategy.ADAPTER_DOWN,
+        FusionStrategy.ADAPTER_UP,
+        FusionStrategy.SAMPLE,
+    }
+)
+
+
+def _strides(t: Tensor | None) -> tuple[int, int]:
+    return (t.row_stride, t.col_stride) if t is not None else (0, 0)
+
+
+# ---------------------------------------------------------------------------
+# block tables
+# ---------------------------------------------------------------------------
+
+
+def page_table_lanes(sequences: int) -> int:
+    """Lanes that add up the sequences: one each while they fit in a workgroup."""
+    return 256 if sequences <= 256 else 1024
+
+
+def _assemble_page_tables(decision: DecisionView, op: PageTablesOp, function_name: str | None) -> KernelGroup:
+    (sequences, width), tokens = op.pages.shape, op.slots.shape[0]
+    lanes = page_table_lanes(sequences)
+    sig = _Signature()
+    args = (
+        sig.add("pages", op.pages, out=True),
+        sig.add("free", op.free),
+        sig.add("lengths", op.lengths),
+        sig.add("counts", op.counts),
+        sig.add("slots", op.slots, out=True),
+        sig.add("positions", op.positions, out=True),
+        sig.add("ends", op.ends, out=True),
+        sig.add("used", op.used, out=True),
+        "M", "S", "W", "F", "(unsigned*)mt_lds",
+    )
+    frag = ServingFragment(
+        "mt_page_tables",
+        (int(op.page_size), lanes),
+        args,
+        lds_bytes=4 * (2 * (lanes + 1) + 2 * (lanes // 64)),
+        name="page_tables",
+    )
+    dims = {"M": tokens, "S": sequences, "W": width, "F": op.free.shape[0]}
+    return _group(decision, sig, frag, function_name or f"page_tables_{op.written.name}", dims,
+                  (min(256, _ceil(tokens, lanes)), 1, 1), lanes, headers=(decoding_header(),))
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+
+def rotary_vector(spec: Rotary, *tensors: Tensor | None) -> int:
+    """Elements that a lane takes at once: four where pairs and what is left of a head
+    divide by it and elements are neighbours."""
+    dense = all(t is None or t.col_stride == 1 for t in tensors)
+    quads = spec.part % (8 if spec.layout == "half" else 4) == 0 and spec.dim % 4 == 0
+    return 4 if dense and quads else 1
+
+
+def _turns(spec: Rotary) -> str:
+    rows = ", ".join(f"{{{a.hex()}, {b.hex()}}}" for a, b in spec.turns)
+    return f"static __device__ const double mt_turns[{spec.part // 2}][2] = {{{rows}}};"
+
+
+def _assemble_rotary(decision: DecisionView, op: RotaryOp, function_name: str | None) -> KernelGroup:
+    spec, rows = op.spec, op.x.shape[0]
+    heads = op.x.shape[1] // spec.dim
+    kv_heads = op.k.shape[1] // spec.dim if op.k is not None else 0
+    together = 4 if rows >= 1024 else 1
+    sig = _Signature()
+    args = (
+        sig.add("x", op.x),
+        sig.add("k", op.k),
+        sig.add("positions", op.positions),
+        "mt_turns",
+        repr(float(spec.magnitude)),
+        sig.add("y", op.y, out=True),
+        sig.add("k_out", op.k_out, out=True),
+        "M",
+        "(mt_f32x2*)mt_lds",
+    )
+    frag = ServingFragment(
+        "mt_rotary",
+        (spec.dim, spec.part, spec.layout == "interleaved", rotary_vector(spec, op.x, op.k), heads, *_strides(op.x),
+         kv_heads, *_strides(op.k), together),
+        args,
+        lds_bytes=together * spec.part // 2 * 8,
+        name="rotary",
+    )
+    return _group(decision, sig, frag, function_name or f"rotary_{op.y.name}", {"M": rows}, (_ceil(rows, together), 1, 1), 256,
+                  headers=(decoding_header(), _turns(spec)))
+
+
+# ---------------------------------------------------------------------------
+# adapters
+# ---------------------------------------------------------------------------
+
+ADAPTER_DOWN_WAVES = 8
+ADAPTER_DOWN_BLOCKS = 4  # of 16 ranks, that a wave multiplies x by at once
+ADAPTER_UP_WAVES, ADAPTER_UP_PER = 4, 4
+
+
+def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_name: str | None) -> KernelGroup:
+    rows, inner = op.x.shape
+    blocks = min(ADAPTER_DOWN_BLOCKS, _ceil(op.rank, 16))
+    sig = _Signature()
+    args = (sig.add("x", op.x), sig.add("a", op.a), sig.add("ids", op.ids), sig.add("down", op.down, out=True), "M",
+            "(mt_f32x4*)mt_lds")
+    frag = ServingFragment(
+        "mt_adapter_down",
+        (inner, op.rank, blocks, op.splits, op.held, ADAPTER_DOWN_WAVES, *_strides(op.x)),
+        args,
+        lds_bytes=ADAPTER_DOWN_WAVES * blocks * 1024,
+        name="adapter_down",
+    )
+    grid = (16 * _ceil(rows, 16), op.splits * _ceil(op.rank, 16 * blocks), 1)
+    return _group(decision, sig, frag, function_name or f"adapter_down_{op.name}", {"M": rows}, grid, 64 * ADAPTER_DOWN_WAVES,
+                  headers=(decoding_header(),))
+
+
+def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name: str | None) -> KernelGroup:
+    rows, cols = op.base.shape
+    sig = _Signature()
+    args = (sig.add("base", op.base), sig.add("down", op.down), sig.add("b", op.b), sig.add("ids", op.ids),
+            sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M")
+    frag = ServingFragment(
+        "mt_adapter_up",
+        (cols, op.rank, op.splits, op.held, ADAPTER_UP_WAVES, ADAPTER_UP_PER, *_strides(op.base)),
+        args,
+        name="adapter_up",
+    )
+    grid = (16 * _ceil(rows, 16), _ceil(cols, 16 * ADAPTER_UP_WAVES * ADAPTER_UP_PER), 1)
+    return _group(decision, sig, frag, function_name or f"adapter_up_{op.y.name}", {"M": rows}, grid, 64 * ADAPTER_UP_WAVES,
+                  headers=(decoding_header(),))
+
+
+# ---------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------
+
+SAMPLE_WAVES = 16
+
+
+def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | None) -> KernelGroup:
+    rows, cols = op.logits.shape
+    sig = _Signature()
+    args = (
+        sig.add("logits", op.logits),
+        sig.add("uniforms", op.uniforms),
+        sig.add("temperatures", op.temperatures),
+        sig.add("top_k", op.top_k),
+        sig.add("top_p", op.top_p),
+        sig.add("min_p", op.min_p),
+        sig.add("tokens", op.tokens, out=True),
+        sig.add("logprobs", op.logprobs, out=True),
+        "(mt_u64*)mt_lds",
+    )
+    frag = ServingFragment(
+        "mt_sample",
+        # (weights of 2^-shift, so that a row of ones adds up in 63 bits)
+        (cols, 62 - (cols - 1).bit_length(), SAMPLE_WAVES, *_strides(op.logits)),
+        args,
+        lds_bytes=8 * (2 * SAMPLE_WAVES + 256),
+        name="sample",
+    )
+    return _group(decision, sig, frag, function_name or f"sample_{op.tokens.name}", {}, (rows, 1, 1), 64 * SAMPLE_WAVES,
+                  headers=(decoding_header(),))
+
+
+_ASSEMBLE = {
+    PageTablesOp: _assemble_page_tables,
+    RotaryOp: _assemble_rotary,
+    AdapterDownOp: _assemble_adapter_down,
+    AdapterUpOp: _assemble_adapter_up,
+    SampleOp: _assemble_sample,
+}
+
+
+def assemble_decoding(decision: DecisionView, function_name: str | None) -> KernelGroup:
+    op = decision.serving_op
+    return _ASSEMBLE[type(op)](decision, op, function_name)

@@ -65,14 +65,14 @@ class _Signature:
 
 
 def _group(decision: DecisionView, sig: _Signature, fragment: ServingFragment, function_name: str, dims: dict[str, int],
-           grid: tuple[int, int, int], lanes: int, **context) -> KernelGroup:
+           grid: tuple[int, int, int], lanes: int, headers: tuple[str, ...] = (), **context) -> KernelGroup:
     ctx = CodegenContext(
         function_name=function_name,
         buffers=tuple(sig.buffers),
         dims=tuple(dims),
         tg_x=lanes,
         tg_y=1,
-        helpers=(serving_header(),),
+        helpers=(serving_header(), *headers),
         **context,
     )
     return KernelGroup(

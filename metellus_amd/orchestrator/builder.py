@@ -5,7 +5,8 @@ src/orchestrator/builder.py:50-342): ``input``, ``from_numpy``, ``matmul``,
 ``elementwise``, ``transpose``, ``reshape``, ``reduction``, ``build``,
 ``tensors``, ``uploads``; beyond it the serving ops (``rms_norm``,
 ``dequantize``, ``matmul_int4``, ``kv_cache``, ``cache_write``, ``cache_read``,
-``paged_attention``) and inputs of their types.  Validation is delegated to the op dataclasses;
+``paged_attention``), the decoding ops (``page_tables``, ``rotary``, ``adapters``,
+``sample``) and inputs of their types.  Validation is delegated to the op dataclasses;
 the builder resolves names, keeps SSA freshness and records host payloads.
 
     ops = Operations()
@@ -20,6 +21,16 @@ from __future__ import annotations
 import numpy as np
 
 from metellus_amd.compute.elementwise.elementwise import BroadcastSpec
+from metellus_amd.orchestrator.decoding import (
+    ADAPTER_RANK_MAX,
+    AdapterDownOp,
+    AdapterUpOp,
+    PageTablesOp,
+    Rotary,
+    RotaryOp,
+    SampleOp,
+    adapter_splits,
+)
 from metellus_amd.orchestrator.ir import (
     ITEM_BYTES,
     ElementwiseOp,
@@ -66,6 +77,8 @@ class Operations:
         self._caches: dict[str, KVCache] = {}
         self._written: dict[str, str] = {}  # a cache's older state -> the state after the write
         self._cache_readers: dict[str, list[Tensor]] = {}
+        self._tables: dict[str, str] = {}  # a block table's older state -> the state after it
+        self._scratch: set[str] = set()  # what one kernel of an operator leaves for the next
 
     # -- registry ------------------------------------------------------------
 
@@ -154,6 +167,12 @@ class Operations:
             raise ValueError(
                 f"tensor {name!r} is not declared — call ops.input(...) first or use an op that produces it"
             )
+        if name in self._tables:
+            raise ValueError(
+                f"block table {name!r} has been written since; its buffer now holds {self._tables[name]!r} — read that"
+            )
+        if name in self._scratch:
+            raise ValueError(f"tensor {name!r} is an operator's own; no op reads it")
         return t
 
     def _lookup_float(self, name: str) -> Tensor:
@@ -442,6 +461,167 @@ class Operations:
         self._cache_readers.setdefault(cache, []).append(op.out)
         return op.o
 
+    # -- decoding ops (no counterpart in the reference) -------------------------
+
+    def page_tables(
+        self,
+        pages: str,
+        free: str,
+        lengths: str,
+        counts: str,
+        page_size: int,
+        tokens: int,
+        out: str,
+        slots: str,
+        positions: str,
+        ends: str,
+        used: str,
+    ) -> Tensor:
+        """Make room for a step's tokens: sequence b goes on from ``lengths[b]`` by
+        ``counts[b]`` positions, and the pages that it lacks are taken from ``free`` in
+        turn.  In place: ``out`` is the table after it, on the buffer of ``pages``, which
+        may not be read any more; entries that no new page goes to are left as they were.
+        Further outputs, int32 all: ``slots`` and ``positions`` of ``tokens`` rows (each
+        sequence's after the other's; -1 behind the last, which ``cache_write`` passes
+        over), the lengths after the step in ``ends``, and in ``used`` how many pages were
+        needed (more than ``free`` has: the rest of the entries is -1, and their tokens
+        have no slots).  A sequence grows to the end of its table and no further."""
+        tp, tf, tl, tc = self._lookup(pages), self._lookup(free), self._lookup(lengths), self._lookup(counts)
+        if isinstance(tokens, bool) or not isinstance(tokens, (int, np.integer)) or not 0 < tokens < 2**31:
+            raise ValueError(f"page_tables tokens must be a positive int32; got {tokens!r}")
+        states = {pages, *self._tables}
+        views = sorted(n for n, t in self._tensors.items() if t.buffer_key == tp.buffer_key and n not in states)
+        if views or (tp.buffer_key != pages and pages not in self._tables.values()):
+            raise ValueError(f"page_tables writes {pages!r} in place: it can be no view and have none; got {views or [tp.buffer_key]}")
+        fresh = self._fresh(out, tp.shape, "int32")
+        op = PageTablesOp(
+            written=Tensor(name=fresh.name, shape=tp.shape, dtype="int32", stored="int32", buffer_key=tp.buffer_key),
+            slots=self._fresh(slots, (int(tokens),), "int32"),
+            positions=self._fresh(positions, (int(tokens),), "int32"),
+            ends=self._fresh(ends, tl.shape, "int32"),
+            used=self._fresh(used, (1,), "int32"),
+            pages=tp,
+            free=tf,
+            lengths=tl,
+            counts=tc,
+            page_size=page_size,
+            after=(
+                *self._owners(tf, tl, tc),
+                *(o.out for o in self._ops if any(t.name == pages for t in o.inputs)),  # who read the older state
+            ),
+        )
+        self._emit_all(op)
+        self._tables[pages] = out
+        return op.written
+
+    def rotary(
+        self, x: str, positions: str, out: str, rotary: Rotary, k: str | None = None, k_out: str | None = None
+    ) -> Tensor:
+        """``out`` is ``x`` with the heads of row t turned to ``positions[t]`` (int32, any),
+        as ``rotary`` says; ``k_out`` is ``k`` turned alike, in the same launch."""
+        if not isinstance(rotary, Rotary):
+            raise ValueError(f"rotary must be a Rotary; got {rotary!r}")
+        tx, tp, tk = self._lookup(x), self._lookup(positions), self._optional(k)
+        if (k is None) != (k_out is None):
+            raise ValueError("rotary: k and k_out go together")
+        op = RotaryOp(
+            y=self._fresh(out, tx.shape, "float32"),
+            x=tx,
+            positions=tp,
+            spec=rotary,
+            k=tk,
+            k_out=None if tk is None else self._fresh(k_out, tk.shape, "float32"),
+            after=self._owners(tx, tp, tk),
+        )
+        self._emit_all(op)
+        return op.y
+
+    def adapters(
+        self, x: str, base: str, a: str, b: str, ids: str, out: str, scales: str | None = None
+    ) -> Tensor:
+        """``out`` = ``base`` + scales[i] * B_i (A_i x) by rows, i = ``ids`` of the row
+        (int32): low-rank adapters, each row's own, beside a product that all share
+        (``base``).  ``a`` (adapters * rank, columns of x) and ``b`` (adapters * columns of
+        base, rank) hold every adapter's A and B, one after the other; ``scales`` are 1
+        unless given.  A row whose id is none of theirs (-1) is its row of ``base``."""
+        tx, ty, ta, tb = self._lookup(x), self._lookup_float(base), self._lookup(a), self._lookup(b)
+        ti, ts = self._lookup(ids), self._optional(scales)
+        for label, t in (("x", tx), ("base", ty), ("a", ta), ("b", tb)):
+            if len(t.shape) != 2:
+                raise ValueError(f"adapters {label} must be 2D; got shape {t.shape} ({t.name!r})")
+        cols, rank = ty.shape[1], tb.shape[1]
+        if rank > ADAPTER_RANK_MAX:
+            raise ValueError(f"adapters: ranks up to {ADAPTER_RANK_MAX}; {b!r} has {rank}")
+        if tb.shape[0] % cols or ta.shape[0] != tb.shape[0] // cols * rank:
+            raise ValueError(
+                f"adapters a must have shape (adapters * rank, {tx.shape[1]}) and b (adapters * {cols}, rank); "
+                f"got {ta.shape} and {tb.shape}"
+            )
+        if tx.shape[0] != ty.shape[0]:
+            raise ValueError(f"adapters x and base must have as many rows; got {tx.shape} and {ty.shape}")
+        splits = adapter_splits(*tx.shape)
+        down = AdapterDownOp(
+            down=self._fresh(f"{out}.down", (splits * tx.shape[0], rank), "float32"),
+            x=tx,
+            a=ta,
+            ids=ti,
+            rank=rank,
+            splits=splits,
+            name=out,
+            after=self._owners(tx, ta, ti),
+        )
+        up = AdapterUpOp(
+            y=self._fresh(out, ty.shape, "float32"),
+            base=ty,
+            down=down.down,
+            b=tb,
+            ids=ti,
+            rank=rank,
+            splits=splits,
+            scales=ts,
+            after=self._owners(ty, tb, ti, ts),
+        )
+        self._emit_all(down)
+        self._emit_all(up)
+        self._scratch.add(down.down.name)
+        return up.y
+
+    def sample(
+        self,
+        logits: str,
+        uniforms: str,
+        out: str,
+        temperatures: str | None = None,
+        top_k: str | None = None,
+        top_p: str | None = None,
+        min_p: str | None = None,
+        logprobs: str | None = None,
+    ) -> Tensor:
+        """``out`` (int32) is a token for each row of ``logits``, drawn by the row's number
+        in ``uniforms``, 0 <= u < 1 (others count as the nearer end).  With w_i =
+        exp((x_i - max) / temperature): the ``top_k`` largest logits (int32; none or below
+        1: all; the lower index first among equals), of those the fewest of the largest
+        that weigh ``top_p`` of them (1 and above: all), of those the ones with
+        w_i >= ``min_p``; then the first index up to which more than u of the weight that
+        is left has come by.  All four are a number for each row.  A temperature of 0 (or
+        below, or NaN) takes the largest, 1 where not given.  ``logprobs``: the logarithm
+        of the probability that the token was drawn with.  Logits of +inf share
+        all the weight.  A row of -inf alone, or with a NaN, gives -1, its logprob NaN."""
+        tl, tu = self._lookup(logits), self._lookup(uniforms)
+        given = {n: self._optional(v) for n, v in
+                 (("temperatures", temperatures), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p))}
+        rows = tl.shape[:1] if tl.shape else (1,)
+        op = SampleOp(
+            tokens=self._fresh(out, rows, "int32"),
+            logits=tl,
+            uniforms=tu,
+            logprobs=None if logprobs is None else self._fresh(logprobs, rows, "float32"),
+            after=self._owners(tl, tu, *given.values()),
+            **given,
+        )
+        self._emit_all(op)
+        return op.tokens
+
     # -- results -------------------------------------------------------------
 
     def build(self) -> Program:
@@ -454,3 +634,8 @@ class Operations:
     @property
     def uploads(self) -> dict[str, np.ndarray]:
         return dict(self._uploads)
+
+    @property
+    def scratch(self) -> frozenset[str]:
+        """Tensors that one kernel of an operator leaves for the next: no outputs."""
+        return frozenset(self._scratch)

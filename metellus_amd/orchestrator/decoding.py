@@ -1,0 +1,336 @@
+"""The decoding ops: what a decode step does around its products and attention.
+
+No counterpart in the reference.  Serving ops like those of
+``orchestrator.serving`` (whole operators, a kernel each, tensors of other types
+than fp32):
+
+* ``PageTablesOp``  block tables, slots and positions of a step's tokens, in place
+* ``RotaryOp``      queries and keys turned by their positions
+* ``AdapterDownOp``, ``AdapterUpOp``
+                    low-rank adapters of many requests, added to a shared product
+* ``SampleOp``      tokens from logits and given random numbers
+
+``Rotary`` describes a rotation: which elements of a head are pairs, and their
+angles.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from decimal import Decimal, localcontext
+
+import numpy as np
+
+from metellus_amd.orchestrator.ir import Tensor
+from metellus_amd.orchestrator.serving import HEAD_DIM_MAX, _INT32_MAX, ServingOp, _dense, _rows, _want
+
+ROTARY_LAYOUTS = ("half", "interleaved")
+POSITIONS_MAX = _INT32_MAX - 1024  # of a table's row (its positions and a step's rows are int32)
+ADAPTER_RANK_MAX = 256
+VOCABULARY_MAX = 2**24
+
+# pi to 64 digits: 2 pi has to outlast a double's 53 bits twice
+_PI = Decimal("3.141592653589793238462643383279502884197169399375105820974944592")
+
+
+@dataclass(frozen=True)
+class Rotary:
+    """The rotation of heads of ``dim``: the first ``part`` of its elements (all
+    unless given) are pairs, (i, i + part / 2) in the ``half`` layout and
+    (2 i, 2 i + 1) in the ``interleaved`` one; pair i turns by position times
+    frequency i, base^(-2 i / part), and is then ``magnitude`` times as long.
+
+    ``factor`` slows the frequencies down for contexts longer than a model was
+    trained for: all of them alike, or, with the trained length ``original``, by
+    parts: a pair that turns t = original * frequency / (2 pi) times within it keeps
+    its frequency for t >= ``high``, has it divided by ``factor`` for t <= ``low``,
+    and in between a mix, linear in t.  ``frequencies`` are taken as they are
+    instead, for schedules other than these."""
+
+    dim: int
+    part: int | None = None
+    base: float = 10000.0
+    layout: str = "half"
+    factor: float = 1.0
+    original: int | None = None
+    low: float = 1.0
+    high: float = 32.0
+    magnitude: float = 1.0
+    frequencies: tuple[float, ...] | None = None
+
+    def __post_init__(self) -> None:
+        if self.part is None:
+            object.__setattr__(self, "part", self.dim)
+        for name in ("dim", "part"):
+            v = getattr(self, name)
+            if isinstance(v, bool) or not isinstance(v, (int, np.integer)) or v <= 0:
+                raise ValueError(f"rotary: {name} must be a positive int; got {v!r}")
+            object.__setattr__(self, name, int(v))
+        if self.dim > HEAD_DIM_MAX:
+            raise ValueError(f"rotary: dim must be at most {HEAD_DIM_MAX}; got {self.dim}")
+        if self.part % 2 or self.part > self.dim:
+            raise ValueError(f"rotary: part must be even and at most dim = {self.dim}; got {self.part}")
+        if self.layout not in ROTARY_LAYOUTS:
+            raise ValueError(f"rotary: layout must be one of {ROTARY_LAYOUTS}; got {self.layout!r}")
+        if not 1.0 <= self.base < math.inf:
+            raise ValueError(f"rotary: base must be finite and at least 1; got {self.base}")
+        if not 0.0 < self.factor < math.inf:
+            raise ValueError(f"rotary: factor must be finite and above 0; got {self.factor}")
+        if self.original is not None:
+            if isinstance(self.original, bool) or not isinstance(self.original, (int, np.integer)) or self.original <= 0:
+                raise ValueError(f"rotary: original must be a positive int; got {self.original!r}")
+            if not 0.0 <= self.low < self.high < math.inf:
+                raise ValueError(f"rotary: low and high must be finite, 0 <= low < high; got {self.low} and {self.high}")
+        if not 0.0 < self.magnitude <= 2.0**60:
+            raise ValueError(f"rotary: magnitude must be above 0 and at most 2^60; got {self.magnitude}")
+        if self.frequencies is not None:
+            given = tuple(float(f) for f in self.frequencies)
+            if len(given) != self.part // 2:
+                raise ValueError(f"rotary: {self.part // 2} pairs need as many frequencies; got {len(given)}")
+            object.__setattr__(self, "frequencies", given)
+        if not all(abs(f) <= 2.0**20 for f in self.angles):
+            raise ValueError("rotary: frequencies must be finite and within 2^20")
+
+    @property
+    def angles(self) -> tuple[float, ...]:
+        """Radians that each pair turns for a step of position."""
+        if self.frequencies is not None:
+            return self.frequencies
+        plain = [self.base ** (-2 * i / self.part) for i in range(self.part // 2)]
+        if self.original is None:
+            return tuple(f / self.factor for f in plain)
+        made = []
+        for f in plain:
+            kept = (self.original * f / (2 * math.pi) - self.low) / (self.high - self.low)
+            kept = min(1.0, max(0.0, kept))
+            made.append((1 - kept) * f / self.factor + kept * f)
+        return tuple(made)
+
+    @property
+    def turns(self) -> tuple[tuple[float, float], ...]:
+        """``angles`` in whole turns, each as the sum of two doubles."""
+        found = []
+        with localcontext() as ctx:
+            ctx.prec = 60
+            for f in self.angles:
+                t = Decimal(f) / (2 * _PI)
+                head = float(t)
+                found.append((head, float(t - Decimal(head))))
+        return tuple(found)
+
+
+def adapter_splits(rows: int, inner: int) -> int:
+    """Shares of x's columns that workgroups take apart, where rows alone are too few
+    workgroups to fill the GPU: at least 256 columns each."""
+    return max(1, min(-(-inner // 256), 512 // rows))
+
+
+# ---------------------------------------------------------------------------
+# ops
+# ---------------------------------------------------------------------------
+
+
+def _list(label: str, t: Tensor, dtype: str, n: int | None = None) -> int:
+    """A dense 1-D tensor of ``dtype``; its length."""
+    if len(t.shape) != 1:
+        raise ValueError(f"{label} must be 1D; got shape {t.shape} ({t.name!r})")
+    _want(label, t, dtype, t.shape if n is None else (n,))
+    _dense(label, t)
+    return t.shape[0]
+
+
+@dataclass(frozen=True)
+class PageTablesOp(ServingOp):
+    """With L = lengths clamped to the table's room, C = max(counts, 0) and E = L + C
+    clamped to it (``ends``): sequence b has the first ceil(L / page_size) entries of
+    its row of ``pages``, and gets those up to ceil(E / page_size) from ``free``, whose
+    numbers go to the sequences in turn, -1 behind its end.  ``used`` is how many were
+    needed.  Token rows are packed, C of each sequence after the other: the i-th of
+    sequence b has position L + i and that position's slot; -1 for both beyond the
+    room and behind the last sequence, and for a slot whose page is below 0."""
+
+    written: Tensor
+    slots: Tensor
+    positions: Tensor
+    ends: Tensor
+    used: Tensor
+    pages: Tensor
+    free: Tensor
+    lengths: Tensor
+    counts: Tensor
+    page_size: int
+    after: tuple[Tensor, ...] = ()
+
+    def __post_init__(self) -> None:
+        if len(self.pages.shape) != 2:
+            raise ValueError(f"page_tables pages must be 2D; got shape {self.pages.shape} ({self.pages.name!r})")
+        _want("page_tables pages", self.pages, "int32", self.pages.shape)
+        _dense("page_tables pages", self.pages)
+        rows, width = self.pages.shape
+        if isinstance(self.page_size, bool) or not isinstance(self.page_size, (int, np.integer)) or self.page_size <= 0:
+            raise ValueError(f"page_tables page_size must be a positive int; got {self.page_size!r}")
+        if width * self.page_size > POSITIONS_MAX or rows * width > _INT32_MAX:
+            raise ValueError(f"page_tables: {rows} rows of {width} pages of {self.page_size}; positions and entries are int32")
+        _list("page_tables free", self.free, "int32")
+        _list("page_tables lengths", self.lengths, "int32", rows)
+        _list("page_tables counts", self.counts, "int32", rows)
+
+    @property
+    def overwrites(self) -> Tensor:
+        return self.pages
+
+    @property
+    def outs(self) -> tuple[Tensor, ...]:
+        return (self.written, self.slots, self.positions, self.ends, self.used)
+
+    @property
+    def reads(self) -> tuple[Tensor, ...]:
+        return (self.pages, self.free, self.lengths, self.counts)
+
+
+@dataclass(frozen=True)
+class RotaryOp(ServingOp):
+    """Row t of ``x`` (and of ``k``) by ``positions[t]``, every head alike."""
+
+    y: Tensor
+    x: Tensor
+    positions: Tensor
+    spec: Rotary
+    k: Tensor | None = None
+    k_out: Tensor | None = None
+    after: tuple[Tensor, ...] = ()
+
+    def __post_init__(self) -> None:
+        rows = 0
+        for label, t in (("rotary x", self.x), ("rotary k", self.k)):
+            if t is None:
+                continue
+            n, cols = _rows(label, t, "float32")
+            if cols % self.spec.dim:
+                raise ValueError(f"{label} must have whole heads of {self.spec.dim}; got shape {t.shape} ({t.name!r})")
+            if rows and n != rows:
+                raise ValueError(f"{label} must have {rows} rows; got shape {t.shape} ({t.name!r})")
+            rows = n
+        _list("rotary positions", self.positions, "int32", rows)
+        if (self.k is None) != (self.k_out is None):
+            raise ValueError("rotary: k and k_out go together")
+
+    @property
+    def outs(self) -> tuple[Tensor, ...]:
+        return tuple(t for t in (self.y, self.k_out) if t is not None)
+
+    @property
+    def reads(self) -> tuple[Tensor, ...]:
+        return tuple(t for t in (self.x, self.k, self.positions) if t is not None)
+
+
+
+@dataclass(frozen=True)
+class AdapterDownOp(ServingOp):
+    """Part s of ``down`` (``splits`` parts of x's rows): x[m] . A[ids[m]] over the
+    s-th share of the columns; rows whose id is no adapter's are not written."""
+
+    down: Tensor
+    x: Tensor
+    a: Tensor
+    ids: Tensor
+    rank: int
+    splits: int
+    name: str  # of the operator's output
+    after: tuple[Tensor, ...] = ()
+
+    def __post_init__(self) -> None:
+        rows, inner = _rows("adapters x", self.x, "float32")
+        if len(self.a.shape) != 2 or self.a.shape[1] != inner or self.a.shape[0] % self.rank:
+            raise ValueError(f"adapters a must have shape (adapters * {self.rank}, {inner}); got {self.a.shape} ({self.a.name!r})")
+        _want("adapters a", self.a, "float32", self.a.shape)
+        _dense("adapters a", self.a)
+        _list("adapters ids", self.ids, "int32", rows)
+
+    @property
+    def held(self) -> int:
+        return self.a.shape[0] // self.rank
+
+    @property
+    def outs(self) -> tuple[Tensor, ...]:
+        return (self.down,)
+
+    @property
+    def reads(self) -> tuple[Tensor, ...]:
+        return (self.x, self.a, self.ids)
+
+
+@dataclass(frozen=True)
+class AdapterUpOp(ServingOp):
+    """y[m] = base[m] + scales[ids[m]] * B[ids[m]] (the parts of down[m] added)."""
+
+    y: Tensor
+    base: Tensor
+    down: Tensor
+    b: Tensor
+    ids: Tensor
+    rank: int
+    splits: int
+    scales: Tensor | None = None
+    after: tuple[Tensor, ...] = ()
+
+    def __post_init__(self) -> None:
+        rows, cols = _rows("adapters base", self.base, "float32")
+        held = self.b.shape[0] // cols
+        _want("adapters b", self.b, "float32", (held * cols, self.rank))
+        _dense("adapters b", self.b)
+        _list("adapters ids", self.ids, "int32", rows)
+        if self.scales is not None:
+            _list("adapters scales", self.scales, "float32", held)
+
+    @property
+    def held(self) -> int:
+        return self.b.shape[0] // self.base.shape[1]
+
+    @property
+    def outs(self) -> tuple[Tensor, ...]:
+        return (self.y,)
+
+    @property
+    def reads(self) -> tuple[Tensor, ...]:
+        return tuple(t for t in (self.base, self.down, self.b, self.ids, self.scales) if t is not None)
+
+
+@dataclass(frozen=True)
+class SampleOp(ServingOp):
+    """For a row x with temperature T: w_i = exp((x_i - max x) / T).  In the order of
+    x descending, the lower index first among equals: the first ``top_k`` stay; of
+    those, the ones before which there is less than ``top_p`` of their weight; of
+    those, the ones of weight ``min_p`` at least.  The token is the first index, in
+    index order, up to which more than u times the weight that stayed has come by."""
+
+    tokens: Tensor
+    logits: Tensor
+    uniforms: Tensor
+    logprobs: Tensor | None = None
+    temperatures: Tensor | None = None
+    top_k: Tensor | None = None
+    top_p: Tensor | None = None
+    min_p: Tensor | None = None
+    after: tuple[Tensor, ...] = ()
+
+    def __post_init__(self) -> None:
+        rows, cols = _rows("sample logits", self.logits, "float32")
+        if cols > VOCABULARY_MAX:
+            raise ValueError(f"sample logits: at most {VOCABULARY_MAX} columns; got shape {self.logits.shape}")
+        for label, t, dtype in (("uniforms", self.uniforms, "float32"), ("temperatures", self.temperatures, "float32"),
+                                ("top_k", self.top_k, "int32"), ("top_p", self.top_p, "float32"),
+                                ("min_p", self.min_p, "float32")):
+            if t is not None:
+                _list(f"sample {label}", t, dtype, rows)
+
+    @property
+    def outs(self) -> tuple[Tensor, ...]:
+        return tuple(t for t in (self.tokens, self.logprobs) if t is not None)
+
+    @property
+    def reads(self) -> tuple[Tensor, ...]:
+        return tuple(
+            t for t in (self.logits, self.uniforms, self.temperatures, self.top_k, self.top_p, self.min_p) if t is not None
+        )

@@ -35,6 +35,12 @@ class FusionStrategy(str, Enum):
     CACHE_WRITE = "cache_write"
     CACHE_READ = "cache_read"
     PAGED_ATTENTION = "paged_attention"
+    # the decoding ops (orchestrator.decoding)
+    PAGE_TABLES = "page_tables"
+    ROTARY = "rotary"
+    ADAPTER_DOWN = "adapter_down"
+    ADAPTER_UP = "adapter_up"
+    SAMPLE = "sample"
 
     def __str__(self) -> str:
         return self.value

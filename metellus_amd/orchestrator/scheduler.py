@@ -15,7 +15,8 @@ Plan, in order:
    buffer's life) -- or freed.
 
 Fused intermediates never get a buffer, so they are never downloaded.  A
-state of a kv cache that a later write overwrote is gone too.
+state of a kv cache or block table that a later write overwrote is gone too, and
+what one kernel of an operator leaves for the next is no output.
 Frees are stream-ordered in the native shim, so they need no host sync.
 """
 
@@ -29,7 +30,7 @@ from metellus_amd.orchestrator.builder import Operations
 from metellus_amd.orchestrator.dag import build_dag
 from metellus_amd.orchestrator.ir import outs_of
 from metellus_amd.orchestrator.kernel_group import KernelGroup
-from metellus_amd.orchestrator.serving import CacheWriteOp
+from metellus_amd.orchestrator.serving import ServingOp
 from metellus_amd.runtime.program import Allocate, Dispatch, Download, Free, FromNumpy, Runtime
 
 
@@ -48,10 +49,13 @@ def schedule(
     dag = build_dag(program)
     tensors = ops.tensors
     uploads = ops.uploads
+    scratch = ops.scratch
 
-    # (a cache is written in place: its buffer is the input's)
-    made = [t for op in program for t in outs_of(op) if not isinstance(op, CacheWriteOp)]
-    overwritten = {op.cache.name for op in program if isinstance(op, CacheWriteOp)}
+    # (what is written in place, a cache or a block table, is the input's buffer)
+    in_place = [op.overwrites for op in program if isinstance(op, ServingOp) and op.overwrites is not None]
+    overwritten = {t.name for t in in_place}
+    kept = {t.buffer_key for t in in_place}
+    made = [t for op in program for t in outs_of(op) if t.buffer_key not in kept]
     produced = {t.buffer_key for t in made}
     required = {tensors[n].buffer_key for n in dag.inputs} - produced
     provided = set(uploads)
@@ -76,13 +80,13 @@ def schedule(
             raise ValueError(f"schedule: unknown output names {unknown}")
         gone = sorted(n for n in wanted if n in overwritten and n not in uploads)
         if gone:
-            raise ValueError(f"schedule: outputs {gone} are states of a kv cache that a later write overwrites")
-        absent = sorted(n for n in wanted if n in uploads or tensors[n].buffer_key not in live_keys)
+            raise ValueError(f"schedule: outputs {gone} are states of a kv cache or block table that a later write overwrites")
+        absent = sorted(n for n in wanted if n in uploads or n in scratch or tensors[n].buffer_key not in live_keys)
         if absent:
             raise ValueError(f"schedule: outputs {absent} are program inputs or not materialised by any kernel")
     names_by_key: dict[str, list[str]] = {}
     for name, t in tensors.items():
-        if name in overwritten:
+        if name in overwritten or name in scratch:
             continue
         if name not in uploads and t.buffer_key in live_keys and (wanted is None or name in wanted):
             names_by_key.setdefault(t.buffer_key, []).append(name)

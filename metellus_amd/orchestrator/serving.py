@@ -214,6 +214,12 @@ class ServingOp:
         raise NotImplementedError
 
     @property
+    def overwrites(self) -> Tensor | None:
+        """The older name of a buffer that the op writes in place (its new one is among
+        ``outs``)."""
+        return None
+
+    @property
     def inputs(self) -> tuple[Tensor, ...]:
         known = {t.name for t in self.reads}
         return (*self.reads, *(t for t in self.after if t.name not in known))
@@ -344,6 +350,10 @@ class CacheWriteOp(ServingOp):
         _want("cache_write v", self.v, "float32", (rows, self.spec.row))
         _want("cache_write slots", self.slots, "int32", (rows,))
         _dense("cache_write slots", self.slots)
+
+    @property
+    def overwrites(self) -> Tensor:
+        return self.cache
 
     @property
     def outs(self) -> tuple[Tensor, ...]:

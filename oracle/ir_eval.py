@@ -24,7 +24,8 @@ the program is fused:
   (reference: src/compute/reduction/reduction.py:172-193);
 * matmul accumulated in float64 (the reference for a tolerance check);
 * ``ShapeOp`` -- a strided gather (reference: src/compute/copy/copy.py:25-54);
-* the serving ops -- ``oracle/serving_eval.py``, in float64.
+* the serving ops -- ``oracle/serving_eval.py``, in float64, and the decoding ops --
+  ``oracle/decoding_eval.py``.
 
 ``ordered_row_reduce`` additionally replays the exact combine order of the
 gfx950 reduction kernel (lane chunks, four vector accumulators, wave64

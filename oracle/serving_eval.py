@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import numpy as np
 
+from oracle.decoding_eval import evaluate_decoding
+
 F32, F64 = np.float32, np.float64
 
 
@@ -167,5 +169,6 @@ def evaluate_serving(op, get) -> dict:
     if kind == "DequantizeOp":
         with np.errstate(invalid="ignore"):
             return {op.y.name: get(op.x).astype(F64) * get(op.scales).astype(F64)[:, None]}
-    return {"RmsNormOp": _norm, "Int4MatmulOp": _int4, "CacheWriteOp": _write, "CacheReadOp": _read,
-            "PagedAttentionOp": _attention}[kind](op, get)
+    known = {"RmsNormOp": _norm, "Int4MatmulOp": _int4, "CacheWriteOp": _write, "CacheReadOp": _read,
+             "PagedAttentionOp": _attention}
+    return known[kind](op, get) if kind in known else evaluate_decoding(op, get)

@@ -1,0 +1,348 @@
+"""The decoding ops without a GPU: what the builder and the scheduler accept and refuse,
+the order around a table written in place, a rotation's frequencies, the oracle on cases
+worked out by hand, and that every kernel variant compiles for gfx950."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from metellus_amd.api import compile_program
+from metellus_amd.orchestrator import Operations, Rotary
+from metellus_amd.orchestrator.decoding import adapter_splits
+from metellus_amd.orchestrator.fusion import fuse
+from metellus_amd.orchestrator.scheduler import schedule
+from metellus_amd.runtime import hip_backend
+from metellus_amd.runtime.program import Dispatch, Download, Free
+from oracle import decoding_eval
+from oracle.ir_eval import evaluate
+
+
+def _ops(**inputs) -> Operations:
+    """Inputs by name: a shape, or (shape, dtype)."""
+    ops = Operations()
+    for name, what in inputs.items():
+        if isinstance(what[0], tuple):
+            ops.input(name, what[0], dtype=what[1])
+        else:
+            ops.input(name, what)
+    return ops
+
+
+PAGES = dict(pages=((4, 6), "int32"), free=((9,), "int32"), lengths=((4,), "int32"), counts=((4,), "int32"))
+PAGE_CALL = dict(pages="pages", free="free", lengths="lengths", counts="counts", page_size=8, tokens=10, out="table",
+                 slots="slots", positions="positions", ends="ends", used="used")
+ROTARY = dict(q=(3, 64), k=(3, 32), at=((3,), "int32"))
+ADAPTERS = dict(x=(5, 12), y=(5, 20), a=(3 * 4, 12), b=(3 * 20, 4), ids=((5,), "int32"), s=(3,))
+ADAPTER_CALL = dict(x="x", base="y", a="a", b="b", ids="ids", out="z")
+SAMPLE = dict(x=(3, 50), u=(3,), k=((3,), "int32"), p=(3,))
+
+
+# -- refusals -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("inputs, call, match", [
+    (dict(pages=((24,), "int32")), {}, "must be 2D"),
+    (dict(pages=(4, 6)), {}, "must be int32"),
+    (dict(free=((3, 3), "int32")), {}, "free must be 1D"),
+    (dict(free=(9,)), {}, "free must be int32"),
+    (dict(lengths=((5,), "int32")), {}, "lengths must have shape"),
+    (dict(counts=((3,), "int32")), {}, "counts must have shape"),
+    ({}, dict(page_size=0), "page_size must be a positive int"),
+    ({}, dict(page_size=True), "page_size must be a positive int"),
+    ({}, dict(page_size=2**29), "positions and entries are int32"),
+    ({}, dict(tokens=0), "tokens must be a positive int32"),
+    ({}, dict(tokens=2**31), "tokens must be a positive int32"),
+    ({}, dict(slots="table"), "output names must differ"),
+    ({}, dict(ends="free"), "already defined"),
+    ({}, dict(pages="nothing"), "is not declared"),
+])
+def test_page_tables_refusals(inputs, call, match):
+    ops = _ops(**{**PAGES, **inputs})
+    with pytest.raises(ValueError, match=match):
+        ops.page_tables(**{**PAGE_CALL, **call})
+    assert not ops.build() and "table" not in ops.tensors and "slots" not in ops.tensors
+
+
+def test_a_written_table_has_one_name():
+    ops = _ops(**PAGES, q=(4, 32))
+    ops.kv_cache("cache", pages=20, page_size=8, kv_heads=1, dim=32)
+    ops.page_tables(**PAGE_CALL)
+    for call in (
+        lambda: ops.paged_attention("q", cache="cache", pages="pages", lengths="ends", heads=1, out="o"),
+        lambda: ops.transpose("pages", out="t"),
+        lambda: ops.reshape("pages", (24,), out="t"),
+        lambda: ops.page_tables(**{**PAGE_CALL, **{n: n + "2" for n in ("out", "slots", "positions", "ends", "used")}}),
+    ):
+        with pytest.raises(ValueError, match="its buffer now holds 'table' — read that"):
+            call()
+    ops.paged_attention("q", cache="cache", pages="table", lengths="ends", heads=1, out="o")
+    more = {**PAGE_CALL, "pages": "table", "lengths": "ends", **{n: n + "2" for n in ("out", "slots", "positions", "ends", "used")}}
+    assert ops.page_tables(**more).buffer_key == "pages"  # a step after the step
+
+
+def test_a_table_with_views_is_not_written():
+    ops = _ops(**PAGES)
+    ops.reshape("pages", (24,), out="flat")
+    with pytest.raises(ValueError, match="can be no view and have none"):
+        ops.page_tables(**PAGE_CALL)
+    ops = _ops(**PAGES)
+    ops.input("wide", (6, 4), dtype="int32")
+    ops.reshape("wide", (4, 6), out="view")
+    with pytest.raises(ValueError, match="can be no view and have none"):
+        ops.page_tables(**{**PAGE_CALL, "pages": "view"})
+
+
+@pytest.mark.parametrize("inputs, call, match", [
+    (dict(q=(3, 60)), {}, "whole heads of 32"),
+    (dict(k=(4, 32)), {}, "k must have 3 rows"),
+    (dict(at=((4,), "int32")), {}, "positions must have shape"),
+    (dict(at=(3,)), {}, "positions must be int32"),
+    (dict(q=(96,)), {}, "must be 2D"),
+    ({}, dict(k_out=None), "go together"),
+    ({}, dict(rotary=128), "must be a Rotary"),
+    ({}, dict(out="k"), "already defined"),
+    ({}, dict(k_out="q1"), "output names must differ"),
+])
+def test_rotary_refusals(inputs, call, match):
+    ops = _ops(**{**ROTARY, **inputs})
+    with pytest.raises(ValueError, match=match):
+        ops.rotary(**{**dict(x="q", positions="at", out="q1", rotary=Rotary(dim=32), k="k", k_out="k1"), **call})
+    assert not ops.build()
+
+
+@pytest.mark.parametrize("wrong, match", [
+    (dict(dim=0), "dim must be a positive int"),
+    (dict(dim=258), "at most 256"),
+    (dict(dim=64, part=33), "part must be even"),
+    (dict(dim=64, part=66), "part must be even and at most"),
+    (dict(dim=63), "part must be even"),
+    (dict(dim=64, layout="both"), "layout must be one of"),
+    (dict(dim=64, base=0.5), "base must be"),
+    (dict(dim=64, base=math.inf), "base must be"),
+    (dict(dim=64, factor=0.0), "factor must be"),
+    (dict(dim=64, factor=math.nan), "factor must be"),
+    (dict(dim=64, original=0), "original must be"),
+    (dict(dim=64, original=4096, low=4.0, high=4.0), "low < high"),
+    (dict(dim=64, magnitude=math.nan), "magnitude must be"),
+    (dict(dim=64, frequencies=(1.0,)), "need as many frequencies"),
+    (dict(dim=2, frequencies=(math.nan,)), "finite and within"),
+])
+def test_rotation_refusals(wrong, match):
+    with pytest.raises(ValueError, match=match):
+        Rotary(**wrong)
+
+
+@pytest.mark.parametrize("inputs, call, match", [
+    (dict(a=(3 * 4, 13)), {}, "must have shape"),
+    (dict(a=(3 * 4 + 1, 12)), {}, "must have shape"),
+    (dict(a=(4 * 4, 12)), {}, "must have shape"),
+    (dict(b=(3 * 20 + 1, 4)), {}, "must have shape"),
+    (dict(b=(60 * 4,)), {}, "b must be 2D"),
+    (dict(y=(4, 20)), {}, "as many rows"),
+    (dict(ids=((4,), "int32")), {}, "ids must have shape"),
+    (dict(ids=(5,)), {}, "ids must be int32"),
+    (dict(x=((5, 12), "int8")), {}, "x must be float32"),
+    (dict(a=((12, 12), "int8")), {}, "a must be float32"),
+    (dict(a=(3 * 257, 12), b=(60, 257)), {}, "ranks up to 256"),
+    (dict(s=(4,)), dict(scales="s"), "scales must have shape"),
+    ({}, dict(out="x"), "already defined"),
+    ({}, dict(a="at"), "a must be dense"),
+])
+def test_adapters_refusals(inputs, call, match):
+    ops = _ops(**{**ADAPTERS, "turned": (12, 12), **inputs})
+    ops.transpose("turned", out="at")
+    with pytest.raises(ValueError, match=match):
+        ops.adapters(**{**ADAPTER_CALL, **call})
+    assert not ops.build() and not ops.scratch and "z.down" not in ops.tensors
+
+
+@pytest.mark.parametrize("inputs, call, match", [
+    (dict(x=(50,)), {}, "must be 2D"),
+    (dict(x=((3, 50), "int8")), {}, "logits must be float32"),
+    (dict(x=(3, 2**24 + 1)), {}, "columns"),
+    (dict(u=(4,)), {}, "uniforms must have shape"),
+    ({}, dict(top_k="p"), "top_k must be int32"),
+    ({}, dict(top_p="k"), "top_p must be float32"),
+    (dict(p=(2,)), dict(min_p="p"), "min_p must have shape"),
+    (dict(p=(3, 1)), dict(temperatures="p"), "temperatures must be 1D"),
+    ({}, dict(out="u"), "already defined"),
+    ({}, dict(logprobs="t"), "output names must differ"),
+])
+def test_sample_refusals(inputs, call, match):
+    ops = _ops(**{**SAMPLE, **inputs})
+    with pytest.raises(ValueError, match=match):
+        ops.sample(**{**dict(logits="x", uniforms="u", out="t"), **call})
+    assert not ops.build()
+
+
+# -- programs ----------------------------------------------------------------------
+
+
+def test_who_read_the_older_table_comes_first():
+    """Attention over the table as it was is before the op that writes it, whatever else it
+    waits for."""
+    ops = _ops(**PAGES, x=(4, 8), w=(8, 32))
+    ops.kv_cache("cache", pages=20, page_size=8, kv_heads=1, dim=32)
+    ops.matmul("x", "w", out="q")
+    ops.paged_attention("q", cache="cache", pages="pages", lengths="lengths", heads=1, out="o")
+    ops.page_tables(**PAGE_CALL)
+    ops.paged_attention("q", cache="cache", pages="table", lengths="ends", heads=1, out="o2")
+    kinds = [v.ops[0].out.name for v in fuse(ops.build())]
+    assert kinds.index("o") < kinds.index("table") < kinds.index("o2")
+
+
+def test_scheduling_a_table():
+    """The new state is downloaded from the input's buffer; the old one is no output."""
+    ops = _ops(**PAGES)
+    for name, (shape, _) in PAGES.items():
+        ops.from_numpy(np.zeros(shape, np.int32), name)
+    ops.page_tables(**PAGE_CALL)
+    groups = compile_program(ops)
+    steps = schedule(ops, groups).fragments
+    assert {s.into for s in steps if isinstance(s, Download)} == {"table", "slots", "positions", "ends", "used"}
+    some = schedule(ops, groups, outputs=["slots"]).fragments
+    assert [s.into for s in some if isinstance(s, Download)] == ["slots"]
+    with pytest.raises(ValueError, match="program inputs"):
+        schedule(ops, groups, outputs=["pages"])
+
+
+def test_scheduling_adapters():
+    """What lies between the two products is no output, and nothing reads it."""
+    ops = _ops(**ADAPTERS)
+    ops.adapters(**ADAPTER_CALL, scales="s")
+    for name, shape in ADAPTERS.items():
+        shape, dtype = shape if isinstance(shape[0], tuple) else (shape, "float32")
+        ops.from_numpy(np.zeros(shape, dtype), name)
+    groups = compile_program(ops)
+    steps = schedule(ops, groups).fragments
+    assert [s.into for s in steps if isinstance(s, Download)] == ["z"]
+    assert "z.down" in [s.name for s in steps if isinstance(s, Free)]
+    assert len([s for s in steps if isinstance(s, Dispatch)]) == 2
+    with pytest.raises(ValueError, match="not materialised"):
+        schedule(ops, groups, outputs=["z.down"])
+    with pytest.raises(ValueError, match="operator's own"):
+        ops.reduction("sum", out="r", x="z.down")
+
+
+def test_shares_of_columns():
+    assert adapter_splits(1, 4096) == 16 and adapter_splits(1, 100) == 1
+    assert adapter_splits(32, 4096) == 16 and adapter_splits(4096, 4096) == 1
+    for rows in (1, 3, 50, 700):
+        for inner in (1, 255, 257, 5003, 16384):
+            assert 1 <= adapter_splits(rows, inner) <= -(-inner // 256)
+
+
+# -- a rotation's frequencies --------------------------------------------------------
+
+
+@pytest.mark.parametrize("spec", [
+    Rotary(dim=128), Rotary(dim=64, factor=4.0), Rotary(dim=128, base=500000.0, factor=8.0, original=8192, low=1.0, high=4.0),
+    Rotary(dim=96, part=40, factor=32.0, original=4096), Rotary(dim=4, frequencies=(0.5, -3.0)),
+])
+def test_frequencies(spec):
+    """As the definition says (two ways of the mix: 2^-50 of a value), and in turns: the
+    two doubles together are the frequency over 2 pi to 2^-100."""
+    np.testing.assert_allclose(spec.angles, decoding_eval.rotary_frequencies(spec), rtol=2.0**-50)
+    two_pi = 2 * 31415926535897932384626433832795028841971693993751
+    for f, (head, tail) in zip(spec.angles, spec.turns):
+        n, d = float(f).as_integer_ratio()
+        (hn, hd), (tn, td) = head.as_integer_ratio(), tail.as_integer_ratio()
+        # (head + tail) * 2 pi - f, in units of 10^-49 / (hd td d)
+        off = abs((hn * td + tn * hd) * two_pi * d - n * 10**49 * hd * td)
+        assert off * 2**100 <= abs(n) * 10**49 * hd * td
+        assert abs(tail) <= abs(head) * 2.0**-53
+
+
+# -- the oracle ----------------------------------------------------------------------
+
+
+def test_oracle_of_a_table():
+    ops = _ops(pages=((3, 3), "int32"), free=((4,), "int32"), lengths=((3,), "int32"), counts=((3,), "int32"))
+    for name, v in (("pages", [[7, -1, -1], [-1, -1, -1], [1, 2, 3]]), ("free", [9, 8, 6, 5]), ("lengths", [3, 0, 11]), ("counts", [2, 5, 3])):
+        ops.from_numpy(np.array(v, np.int32), name)
+    ops.page_tables(**{**PAGE_CALL, "page_size": 4, "tokens": 12})
+    ref = evaluate(ops)
+    np.testing.assert_array_equal(ref["table"], [[7, 9, -1], [8, 6, -1], [1, 2, 3]])
+    np.testing.assert_array_equal(ref["positions"], [3, 4, 0, 1, 2, 3, 4, 11, -1, -1, -1, -1])
+    np.testing.assert_array_equal(ref["slots"], [31, 36, 32, 33, 34, 35, 24, 15, -1, -1, -1, -1])
+    np.testing.assert_array_equal(ref["ends"], [5, 5, 12])
+    assert ref["used"] == [3]
+
+
+def test_oracle_of_a_rotation():
+    """A quarter turn takes (1, 0) to (0, 1); the whole rotation is a complex product."""
+    ops = _ops(q=(2, 4), at=((2,), "int32"))
+    ops.from_numpy(np.array([[1, 2, 0, 5], [1, 2, 0, 5]], np.float32), "q")
+    ops.from_numpy(np.array([1, 3], np.int32), "at")
+    ops.rotary("q", positions="at", out="y", rotary=Rotary(dim=4, frequencies=(math.pi / 2, 0.0)))
+    np.testing.assert_allclose(evaluate(ops)["y"], [[0, 2, 1, 5], [0, 2, -1, 5]], atol=1e-15)
+
+
+def test_oracle_of_adapters():
+    ops = _ops(**ADAPTERS)
+    rng = np.random.default_rng(0)
+    made = {n: rng.standard_normal(ADAPTERS[n]).astype(np.float32) for n in ("x", "y", "a", "b", "s")}
+    made["ids"] = np.array([2, -1, 0, 3, 2], np.int32)
+    for n, v in made.items():
+        ops.from_numpy(v, n)
+    ops.adapters(**ADAPTER_CALL, scales="s")
+    got = evaluate(ops)["z"]
+    for m, i in enumerate(made["ids"]):
+        want = made["y"][m].astype(np.float64)
+        if 0 <= i < 3:
+            want = want + made["s"][i] * (made["b"][20 * i : 20 * i + 20].astype(np.float64) @ (made["a"][4 * i : 4 * i + 4].astype(np.float64) @ made["x"][m]))
+        np.testing.assert_allclose(got[m], want, rtol=1e-6, atol=1e-6)  # (down is rounded to fp32 in between)
+
+
+def test_oracle_of_a_draw():
+    x = np.log(np.array([1, 4, 2, 4, 5], np.float32))
+    draw = decoding_eval.sample_row
+    assert [draw(x, u)[0] for u in (0.0, 0.05, 0.07, 0.31, 0.35, 0.43, 0.44, 0.68, 0.7, 0.99)] == [0, 0, 1, 1, 2, 2, 3, 3, 4, 4]
+    assert draw(x, 0.0, top_k=2)[0] == 1 and draw(x, 0.99, top_k=2)[0] == 4  # 5, and the first of the 4s
+    assert draw(x, 0.3, top_p=0.5)[0] == 1 and draw(x, 0.5, top_p=0.5)[0] == 4  # 5 of 16 is less than 8: the first 4 too
+    assert draw(x, 0.0, min_p=0.5)[0] == 1 and draw(x, 0.3, min_p=0.9)[0] == 4
+    assert draw(x, 0.9, temperature=0.0) == (4, 0.0)
+    assert draw(x, 1.0)[0] == 4 and draw(x, 0.2)[1] == pytest.approx(math.log(4 / 16))
+    assert draw(np.array([-np.inf, np.nan]), 0.5)[0] == -1 and draw(np.array([-np.inf] * 2), 0.5)[0] == -1
+
+
+# -- kernels compile --------------------------------------------------------------------
+
+
+def _compile(ops: Operations) -> None:
+    for g in compile_program(ops):
+        hip_backend.compile_only(g.kernel.source)
+        hip_backend.compile_only(g.kernel.batched().source)
+
+
+@pytest.mark.parametrize("sequences", [4, 300])
+def test_page_tables_compile(sequences):
+    ops = _ops(pages=((sequences, 6), "int32"), free=((9,), "int32"), lengths=((sequences,), "int32"), counts=((sequences,), "int32"))
+    ops.page_tables(**PAGE_CALL)
+    _compile(ops)
+
+
+@pytest.mark.parametrize("spec", [Rotary(dim=32), Rotary(dim=32, layout="interleaved"), Rotary(dim=16, part=6),
+                                  Rotary(dim=16, part=6, layout="interleaved")])
+def test_rotary_compiles(spec):
+    ops = _ops(**ROTARY)
+    ops.rotary("q", positions="at", out="q1", rotary=spec, k="k", k_out="k1")
+    _compile(ops)
+
+
+@pytest.mark.parametrize("rank", [3, 16, 100])
+def test_adapters_compile(rank):
+    ops = _ops(**{**ADAPTERS, "a": (3 * rank, 12), "b": (60, rank)})
+    ops.adapters(**ADAPTER_CALL, scales="s" if rank == 16 else None)
+    _compile(ops)
+
+
+@pytest.mark.parametrize("asked", [{}, dict(top_k="k"), dict(top_k="k", top_p="p", min_p="p", temperatures="p", logprobs="lp")])
+@pytest.mark.parametrize("cols", [50, 40000])
+def test_sample_compiles(asked, cols):
+    ops = _ops(**{**SAMPLE, "x": (3, cols)})
+    ops.sample("x", uniforms="u", out="t", **asked)
+    _compile(ops)

@@ -1,0 +1,527 @@
+"""The decoding ops on the GPU against the oracle in float64 (``oracle.decoding_eval``).
+
+Tolerances follow from the kernels' roundings (u = 2^-24, half a step of fp32):
+
+* page_tables: exact.
+* rotary: see ``_rotary_bound``.
+* adapters: see ``_adapter_bound``.
+* sample: tokens exact; a logprob is rounded once, and the sum of n weights held in
+  2^-s is off by n 2^-s of a sum that is 1 at the least (s = 62 - log2 n).
+"""
+
+from __future__ import annotations
+
+import threading
+
+import numpy as np
+import pytest
+
+from metellus_amd.api import compile_program, run, run_batch
+from metellus_amd.orchestrator import KVCache, Operations, Rotary
+from metellus_amd.orchestrator.assembly.decoding import ADAPTER_DOWN_WAVES
+from metellus_amd.orchestrator.decoding import AdapterDownOp, AdapterUpOp
+from metellus_amd.runtime import Buffer, Dispatch, Runtime
+from oracle import decoding_eval
+from oracle.ir_eval import evaluate
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+
+
+def _put(ops: Operations, name: str, a: np.ndarray) -> None:
+    ops.input(name, a.shape, dtype=str(a.dtype))
+    ops.from_numpy(a, name)
+
+
+def _close(got, want, bound):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+    flat = np.isfinite(want)
+    np.testing.assert_array_equal(got[~flat & ~np.isnan(want)], want[~flat & ~np.isnan(want)])
+    bound = np.broadcast_to(bound, want.shape)
+    off = np.abs(got - want)[flat]
+    assert np.all(off <= bound[flat]), f"off by {np.max(off / np.maximum(bound[flat], 1e-300)):.3g} times the bound"
+
+
+# ---------------------------------------------------------------------------
+# block tables
+# ---------------------------------------------------------------------------
+
+PAGE_OUTPUTS = ("slots", "positions", "ends", "used", "table")
+
+
+def _page_ops(table, free, lengths, counts, page_size, tokens):
+    ops = Operations()
+    for name, v in (("pages", table), ("free", free), ("lengths", lengths), ("counts", counts)):
+        _put(ops, name, np.asarray(v, np.int32))
+    ops.page_tables("pages", free="free", lengths="lengths", counts="counts", page_size=page_size, tokens=tokens, out="table",
+                    slots="slots", positions="positions", ends="ends", used="used")
+    return ops
+
+
+def _page_check(ops):
+    env, ref = run(ops).env, evaluate(ops)
+    for name in PAGE_OUTPUTS:
+        np.testing.assert_array_equal(env[name], ref[name], err_msg=name)
+        assert env[name].dtype == np.int32
+
+
+@pytest.mark.parametrize("sequences, width, page_size, most, tokens", [
+    (1, 1, 1, 1, 1), (1, 4, 16, 1, 3), (3, 7, 5, 4, 9), (64, 9, 16, 1, 64), (65, 3, 20, 30, 500), (255, 4, 8, 2, 300),
+    (256, 4, 8, 2, 256), (257, 4, 8, 2, 250), (1023, 6, 3, 9, 4000), (1025, 6, 16, 3, 1000), (5000, 3, 7, 2, 9000),
+    (2, 9000, 16, 30000, 70000),
+])
+def test_page_tables(sequences, width, page_size, most, tokens):
+    rng = np.random.default_rng(sequences * 1009 + tokens)
+    lengths = rng.integers(0, width * page_size + 1, sequences)
+    counts = rng.integers(0, most + 1, sequences)
+    table = np.full((sequences, width), -1)
+    used = -(-lengths // page_size)
+    numbers = rng.permutation(2 * sequences * width).astype(np.int32)
+    live = np.arange(width)[None] < used[:, None]
+    table[live] = numbers[: live.sum()]
+    _page_check(_page_ops(table, numbers[live.sum() :], lengths, counts, page_size, tokens))
+
+
+def test_page_tables_of_lengths_out_of_range():
+    """Lengths and counts below 0, beyond the table, and as large as they get; numbers below 0
+    and pages whose slots are past int32."""
+    big = 2**31 - 1
+    lengths = [-5, big, 30, 31, 32, 0, -(2**31), 7, 16]
+    counts = [3, 2, 5, 1, 1, -4, 1, big, big]
+    table = np.tile(np.arange(4, dtype=np.int32), (9, 1)) + 10 * np.arange(9, dtype=np.int32)[:, None]
+    table[2, 3], table[7, 0] = -9, 2**29
+    _page_check(_page_ops(table, [100, 101, -7, 2**28, 103, 104, 105, 106], lengths, counts, 8, 60))
+
+
+def test_page_tables_out_of_pages():
+    """More pages needed than there are: the rest of the entries is -1, and their tokens
+    have no slots."""
+    lengths, counts = [0, 16, 3], [40, 1, 60]
+    ops = _page_ops(np.full((3, 8), 77), [5, 6, 7], lengths, counts, 16, 128)
+    _page_check(ops)
+    env = run(ops).env
+    assert env["used"][0] == 3 + 1 + 3
+    np.testing.assert_array_equal(env["table"][1], [77, -1, 77, 77, 77, 77, 77, 77])  # others as they were
+
+
+def test_page_tables_of_few_rows():
+    """Sequences whose tokens the rows do not hold still grow."""
+    _page_check(_page_ops(np.zeros((5, 6), np.int32), np.arange(20, 40), [0, 3, 8, 9, 2], [6, 0, 9, 4, 5], 4, 8))
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+
+def _rotary_bound(spec, x, positions):
+    """y1 = c x1 - s x2: c and s are rounded once (u of themselves), s x2 once more (u),
+    and the sum once; so |c x1| u + 2 |s x2| u + |y1| u, 1 % more for what is u^2 and for
+    the 64 bits before, and the smallest step for products that have few bits.  y2 alike."""
+    angles = decoding_eval.rotary_angles(spec, positions)
+    heads = np.abs(x.astype(np.float64)).reshape(x.shape[0], -1, spec.dim)
+    bound = np.zeros(heads.shape)
+    for j, (a, b) in enumerate(decoding_eval.rotary_pairs(spec)):
+        c, s = np.abs(np.cos(angles[:, j, None])) * spec.magnitude, np.abs(np.sin(angles[:, j, None])) * spec.magnitude
+        for one, two in ((a, b), (b, a)):
+            bound[:, :, one] = 1.01 * U * (2 * heads[:, :, one] * c + 3 * heads[:, :, two] * s) + 2.0**-148
+    return bound.reshape(x.shape)
+
+
+def _rotary_check(ops, spec, **names):
+    env, ref = run(ops).env, evaluate(ops)
+    at = ops.uploads["at"]
+    for name, out in names.items():
+        x = ops.uploads[name] if name in ops.uploads else ops.uploads[name + "_"].T
+        _close(env[out], ref[out], _rotary_bound(spec, x, at))
+
+
+SPECS = [
+    Rotary(dim=128), Rotary(dim=64, layout="interleaved"), Rotary(dim=96, part=40, layout="interleaved", factor=4.0),
+    Rotary(dim=80, part=20), Rotary(dim=10, part=6, layout="interleaved"), Rotary(dim=3, part=2),
+    Rotary(dim=256, base=500000.0, factor=8.0, original=8192, low=1.0, high=4.0),
+    Rotary(dim=128, part=64, factor=16.0, original=4096, magnitude=1.2772588722239782),
+    Rotary(dim=8, frequencies=(1.0, -0.5, 0.0, 1048576.0)),
+]
+
+
+@pytest.mark.parametrize("spec", SPECS)
+@pytest.mark.parametrize("rows", [1, 3, 17, 1025])
+def test_rotary(spec, rows):
+    rng = np.random.default_rng(rows + spec.dim)
+    ops = Operations()
+    _put(ops, "q", rng.standard_normal((rows, 3 * spec.dim)).astype(np.float32))
+    _put(ops, "k", rng.standard_normal((rows, 2 * spec.dim)).astype(np.float32))
+    _put(ops, "at", rng.integers(0, 200000, rows).astype(np.int32))
+    ops.rotary("q", positions="at", out="q1", rotary=spec, k="k", k_out="k1")
+    _rotary_check(ops, spec, q="q1", k="k1")
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_far_positions(layout):
+    """The farthest positions of int32, below 0 too; k alone has no turn of its own."""
+    spec = Rotary(dim=32, layout=layout)
+    at = np.array([0, 1, -1, 2**31 - 1, -(2**31), 2**24 + 1, 1000003], np.int32)
+    rng = np.random.default_rng(2)
+    ops = Operations()
+    _put(ops, "q", rng.standard_normal((7, 64)).astype(np.float32))
+    _put(ops, "at", at)
+    ops.rotary("q", positions="at", out="q1", rotary=spec)
+    _rotary_check(ops, spec, q="q1")
+
+
+@pytest.mark.parametrize("spec", [SPECS[0], SPECS[2], SPECS[4]])
+def test_rotary_of_strided_rows(spec):
+    """q a transposed view, k rows with gaps; infinities and NaN stay with their pairs."""
+    rng = np.random.default_rng(5)
+    d = spec.dim
+    ops = Operations()
+    q = rng.standard_normal((2 * d, 5)).astype(np.float32)
+    q[d, 2], q[d + 1, 3] = np.inf, np.nan
+    _put(ops, "q_", q)
+    ops.transpose("q_", out="q")
+    ops.input("k", (5, d), row_stride=d, col_stride=1)
+    ops.from_numpy(rng.standard_normal((5, d)).astype(np.float32), "k")
+    _put(ops, "at", np.arange(5, dtype=np.int32))
+    ops.rotary("q", positions="at", out="q1", rotary=spec, k="k", k_out="k1")
+    _rotary_check(ops, spec, q="q1", k="k1")
+
+
+def test_rotary_keeps_what_is_not_turned():
+    """Elements behind ``part`` are the same bits, and so is a head at position 0."""
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal((4, 192)).astype(np.float32)
+    ops = Operations()
+    _put(ops, "q", x)
+    _put(ops, "at", np.array([0, 5, 6, 0], np.int32))
+    ops.rotary("q", positions="at", out="y", rotary=Rotary(dim=96, part=64))
+    y = run(ops).env["y"]
+    np.testing.assert_array_equal(y.reshape(4, 2, 96)[:, :, 64:], x.reshape(4, 2, 96)[:, :, 64:])
+    np.testing.assert_array_equal(y[[0, 3]], x[[0, 3]])
+
+
+# ---------------------------------------------------------------------------
+# adapters
+# ---------------------------------------------------------------------------
+
+
+def _adapter_bound(ops):
+    """``down`` is a wave's fp32 sum over its blocks of 64 columns (each term at most two
+    roundings, its product's and the sum's), then sums over waves and splits; ``up`` a sum
+    over the rank, rounded up to 16, of what is off by that; scaled and added to base with
+    one rounding.  u of the magnitudes for each."""
+    down, up = [next(o for o in ops.build() if isinstance(o, kind)) for kind in (AdapterDownOp, AdapterUpOp)]
+    value = {n: a.astype(np.float64) for n, a in ops.uploads.items()}
+    x = value["x"] if "x" in value else value["x_"].T
+    base = evaluate(ops)["y"]
+    inner, rank, n = x.shape[1], down.rank, up.y.shape[1]
+    terms = 2 * 64 * -(-inner // (64 * down.splits * ADAPTER_DOWN_WAVES)) + ADAPTER_DOWN_WAVES + down.splits
+    bound = np.abs(base) * U
+    for m, i in enumerate(ops.uploads["ids"]):
+        if 0 <= i < down.held:
+            t = np.abs(value["a"][i * rank : (i + 1) * rank]) @ np.abs(x[m])
+            each = np.abs(value["b"][i * n : (i + 1) * n]) @ t
+            scale = abs(value["s"][i]) if up.scales is not None else 1.0
+            bound[m] += 1.01 * U * (terms + 2 * (rank + 15)) * each * scale
+    return bound + 2.0**-149
+
+
+def _adapters(rows, inner, cols, rank, held, ids, scales=True, seed=1, strides=False):
+    rng = np.random.default_rng(seed)
+    ops = Operations()
+    x, base = rng.standard_normal((rows, inner)).astype(np.float32), rng.standard_normal((rows, cols)).astype(np.float32)
+    if strides:
+        for name, v in (("x", x), ("base", base)):
+            _put(ops, name + "_", np.ascontiguousarray(v.T))
+            ops.transpose(name + "_", out=name)
+    else:
+        _put(ops, "x", x)
+        _put(ops, "base", base)
+    _put(ops, "a", rng.standard_normal((held * rank, inner)).astype(np.float32))
+    _put(ops, "b", rng.standard_normal((held * cols, rank)).astype(np.float32))
+    _put(ops, "ids", np.asarray(ids, np.int32))
+    if scales:
+        _put(ops, "s", rng.uniform(-2, 2, held).astype(np.float32))
+    ops.adapters("x", base="base", a="a", b="b", ids="ids", scales="s" if scales else None, out="y")
+    return ops
+
+
+def _adapter_check(ops):
+    env, ref = run(ops).env, evaluate(ops)
+    _close(env["y"], ref["y"], _adapter_bound(ops))
+    assert set(env) & set(ops.scratch) == set()
+    return env["y"]
+
+
+@pytest.mark.parametrize("rows, inner, cols, rank, held", [
+    (1, 1, 1, 1, 1), (1, 64, 16, 4, 2), (1, 4096, 300, 16, 3), (2, 100, 17, 8, 5), (7, 333, 129, 23, 4), (16, 512, 256, 16, 16),
+    (17, 1000, 1003, 64, 3), (33, 257, 65, 5, 40), (100, 640, 1024, 65, 7), (3, 129, 260, 256, 2), (600, 96, 48, 12, 9),
+])
+@pytest.mark.parametrize("scales", [False, True])
+def test_adapters(rows, inner, cols, rank, held, scales):
+    rng = np.random.default_rng(rows + inner)
+    ids = rng.integers(-1, held, rows)
+    _adapter_check(_adapters(rows, inner, cols, rank, held, ids, scales, seed=rows * 31 + rank))
+
+
+@pytest.mark.parametrize("ids", [
+    [0] * 40, list(range(40)), [i // 7 for i in range(40)], [-1] * 40, [-1, 3] * 20, [39 - i for i in range(40)],
+    [2**31 - 1, -(2**31), 40, 39, 0] * 8,
+])
+def test_adapters_by_group(ids):
+    """Rows that share one, that have one each, in runs, in turn; ids that are no adapter's."""
+    ops = _adapters(40, 300, 70, 8, 40, ids)
+    y = _adapter_check(ops)
+    none = [m for m, i in enumerate(ids) if not 0 <= i < 40]
+    np.testing.assert_array_equal(y[none], ops.uploads["base"][none])
+
+
+def test_adapters_of_strided_rows():
+    _adapter_check(_adapters(19, 130, 70, 6, 3, [i % 4 - 1 for i in range(19)], strides=True))
+
+
+def test_adapters_rows_do_not_mix():
+    """Infinities and NaN of a row, and of an adapter, stay with the rows that have them."""
+    ops = _adapters(18, 200, 40, 9, 4, [0, 1, 2, 3, -1, 0] * 3, scales=False)
+    ops.uploads["x"][1, 7], ops.uploads["x"][3, 100] = np.inf, np.nan
+    ops.uploads["a"][2 * 9 + 1, 5] = np.nan
+    clean = _adapters(18, 200, 40, 9, 4, [0, 1, 2, 3, -1, 0] * 3, scales=False)
+    got, want = run(ops).env["y"], run(clean).env["y"]
+    for m in range(18):
+        if m in (1, 3) or m % 6 == 2:
+            assert not np.any(np.isfinite(got[m]))
+        else:
+            np.testing.assert_array_equal(got[m], want[m])
+
+
+# ---------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------
+
+
+def _sample_ops(x, u, **asked):
+    ops = Operations()
+    _put(ops, "x", np.asarray(x, np.float32))
+    _put(ops, "u", np.asarray(u, np.float32))
+    rows = ops.uploads["x"].shape[0]
+    for name, v in asked.items():
+        _put(ops, name, np.broadcast_to(np.asarray(v, np.int32 if name == "top_k" else np.float32), (rows,)).copy())
+    ops.sample("x", uniforms="u", out="t", logprobs="lp", **{n: n for n in asked})
+    return ops
+
+
+def _sample_check(ops):
+    env, ref = run(ops).env, evaluate(ops)
+    np.testing.assert_array_equal(env["t"], ref["t"])
+    n = ops.tensors["x"].shape[1]
+    _close(env["lp"], ref["lp"], 1.01 * U * np.abs(ref["lp"]) + n * 2.0 ** ((n - 1).bit_length() - 62) + 2.0**-149)
+    return env["t"]
+
+
+FILTERS = [
+    {}, {"temperatures": 0.7}, {"top_k": 1}, {"top_k": 40, "temperatures": 1.3}, {"top_p": 0.9}, {"min_p": 0.05},
+    {"top_k": 50, "top_p": 0.8, "min_p": 0.02, "temperatures": 0.6}, {"top_p": 0.999, "temperatures": 2.0},
+    {"top_k": 1000, "top_p": 0.95}, {"temperatures": 0.0}, {"temperatures": 0.01, "top_k": 7}, {"temperatures": 1e30, "top_p": 0.5},
+]
+
+
+@pytest.mark.parametrize("rows, cols", [(1, 1), (2, 2), (5, 63), (7, 1000), (3, 4096), (4, 4097), (3, 8191), (2, 32003), (2, 131072)])
+@pytest.mark.parametrize("asked", FILTERS)
+def test_sample(rows, cols, asked):
+    rng = np.random.default_rng(rows * 7 + cols)
+    x = 2 * rng.standard_normal((rows, cols)).astype(np.float32)
+    x[:, rng.integers(0, cols, 5)] += 6
+    _sample_check(_sample_ops(x, rng.random(rows), **asked))
+
+
+def test_sample_rows_ask_for_different_things():
+    rng = np.random.default_rng(3)
+    rows = 64
+    _sample_check(_sample_ops(
+        3 * rng.standard_normal((rows, 5003)), rng.random(rows), temperatures=rng.choice([0.0, 0.5, 1.0, -1.0, np.nan, 3.0], rows),
+        top_k=rng.choice([0, 1, 5, 100, 5003, 10**6, -3], rows), top_p=rng.choice([0.0, 0.3, 0.9, 1.0, 2.0, -1.0, np.nan], rows),
+        min_p=rng.choice([0.0, 0.1, 1.0, 5.0, -1.0, np.nan], rows)))
+
+
+@pytest.mark.parametrize("cols", [8, 1000, 20000])
+def test_sample_equal_logits(cols):
+    """Ties: every index of a row of equals, cut by k and by p in the middle of them."""
+    u = (np.arange(16) + 0.5) / 16
+    x = np.zeros((16, cols), np.float32)
+    x[:, ::2] = -0.0  # (no other value than 0)
+    assert len(set(_sample_check(_sample_ops(x, u)).tolist())) == min(16, cols)
+    for asked in ({"top_k": cols // 4}, {"top_p": 0.5}, {"top_k": cols // 2, "top_p": 0.5}, {"min_p": 1.0}):
+        t = _sample_check(_sample_ops(x, u, **asked))
+        assert t.max() < cols // (4 if "top_k" in asked else 2) or "min_p" in asked
+    x[:, 5:] = -1.0
+    x[:, cols - 1] = 2.0
+    for asked in ({"top_k": 3}, {"top_k": 7, "top_p": 0.75}, {"top_p": 0.9, "temperatures": 0.25}, {"top_k": cols - 1}):
+        _sample_check(_sample_ops(x, u, **asked))
+
+
+@pytest.mark.parametrize("cols", [30, 9000])
+def test_sample_uniforms_at_their_ends(cols):
+    """u of 0, next to 1, and outside: the first and the last that stayed."""
+    rng = np.random.default_rng(8)
+    u = np.array([0.0, 1 - 2.0**-24, 1.0, 7.0, -1.0, np.nan, np.inf, -np.inf, 1e-45], np.float32)
+    x = np.tile(rng.standard_normal(cols).astype(np.float32), (9, 1))
+    x[:, 0] = x[:, -1] = -np.inf
+    for asked in ({}, {"top_k": 9}, {"top_p": 0.4}, {"min_p": 0.3}):
+        t = _sample_check(_sample_ops(x, u, **asked))
+        assert t[0] == t[4] == t[5] == t[7] > 0 and t[2] == t[3] == t[6] < cols - 1
+
+
+@pytest.mark.parametrize("cols", [5, 700, 12345])
+def test_sample_masked_rows(cols):
+    """Rows of -inf, of the type's lowest value, with infinities and NaN, one that is left."""
+    low = np.finfo(np.float32).min
+    x = np.zeros((9, cols), np.float32)
+    x[0] = -np.inf
+    x[1] = low
+    x[2, 3] = np.nan
+    x[3], x[3, 4] = -np.inf, -3.0
+    x[4, 1] = x[4, 3] = np.inf
+    x[5], x[5, 2] = -np.inf, low
+    x[6, 0] = -np.nan
+    x[7], x[7, 1], x[7, 2] = low, 3e38, np.inf
+    x[8] = 1e-45
+    u = np.full(9, 0.6)
+    for asked in ({}, {"top_k": 2}, {"top_p": 0.7}, {"min_p": 0.5}, {"temperatures": 0.0}, {"top_k": 4, "top_p": 0.5},
+                  {"temperatures": np.inf}, {"temperatures": 1e-45}):
+        t = _sample_check(_sample_ops(x, u, **asked))
+        assert t[0] == t[2] == t[6] == -1 and t[3] == 4 and t[5] == 2
+
+
+def test_sample_of_strided_logits():
+    rng = np.random.default_rng(9)
+    ops = Operations()
+    _put(ops, "x_", rng.standard_normal((301, 4)).astype(np.float32))
+    ops.transpose("x_", out="x")
+    _put(ops, "u", rng.random(4).astype(np.float32))
+    _put(ops, "k", np.array([3, 0, 50, 1], np.int32))
+    ops.sample("x", uniforms="u", out="t", top_k="k")
+    np.testing.assert_array_equal(run(ops).env["t"], evaluate(ops)["t"])
+
+
+def test_sample_draws_what_it_says():
+    """Over an even grid of numbers, each token comes as often as its probability says (a
+    token's share of the grid is off by one point at the most)."""
+    x = np.array([1.0, 0.0, 2.0, -1.0, 0.5], np.float32)
+    n = 4000
+    t = _sample_check(_sample_ops(np.tile(x, (n, 1)), (np.arange(n) + 0.5) / n, temperatures=0.8))
+    p = np.exp(x.astype(np.float64) / np.float32(0.8))
+    assert np.all(np.abs(np.bincount(t, minlength=5) - n * p / p.sum()) <= 1)
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+
+HEADS, KV_HEADS, DIM, COLS = 4, 2, 32, 100
+
+
+def _step(seed, sequences=5):
+    """A decode step: slots and positions, adapters beside a shared product, rotation, the
+    cache written, attention over it, logits and tokens."""
+    rng = np.random.default_rng(seed)
+    ops = Operations()
+    spec = KVCache(pages=40, page_size=8, kv_heads=KV_HEADS, dim=DIM)
+    lengths = rng.integers(0, 30, sequences).astype(np.int32)
+    lengths[0], lengths[1] = 0, 16
+    table = np.full((sequences, 5), -1, np.int32)
+    order = rng.permutation(40).astype(np.int32)
+    at = 0
+    for b, n in enumerate(-(-lengths // 8)):
+        table[b, :n] = order[at : at + n]
+        at += n
+    counts = np.ones(sequences, np.int32)
+    counts[-1] = 0
+    for name, v in (("pages", table), ("free", order[at:]), ("lengths", lengths), ("counts", counts)):
+        _put(ops, name, v)
+    kv = rng.standard_normal((2, spec.slots, KV_HEADS, DIM)).astype(np.float32)
+    ops.kv_cache("cache", pages=40, page_size=8, kv_heads=KV_HEADS, dim=DIM)
+    ops.from_numpy(spec.pack(kv[0], kv[1]), "cache")
+    for name, shape in (("x", (sequences, 64)), ("wq", (64, HEADS * DIM)), ("k", (sequences, KV_HEADS * DIM)),
+                        ("v", (sequences, KV_HEADS * DIM)), ("a", (3 * 4, 64)), ("b", (3 * HEADS * DIM, 4)),
+                        ("wo", (HEADS * DIM, COLS))):
+        _put(ops, name, (rng.standard_normal(shape) / 8).astype(np.float32))
+    _put(ops, "ids", rng.integers(-1, 3, sequences).astype(np.int32))
+    _put(ops, "u", rng.random(sequences).astype(np.float32))
+    _put(ops, "topk", np.full(sequences, 5, np.int32))
+    ops.page_tables("pages", free="free", lengths="lengths", counts="counts", page_size=8, tokens=sequences, out="table",
+                    slots="slots", positions="at", ends="ends", used="used")
+    ops.matmul("x", "wq", out="q0")
+    ops.adapters("x", base="q0", a="a", b="b", ids="ids", out="q1")
+    ops.rotary("q1", positions="at", out="q", rotary=Rotary(dim=DIM), k="k", k_out="kr")
+    ops.cache_write("cache", k="kr", v="v", slots="slots", out="cache1")
+    ops.paged_attention("q", cache="cache1", pages="table", lengths="ends", heads=HEADS, out="o")
+    ops.matmul("o", "wo", out="logits")
+    ops.sample("logits", uniforms="u", out="tokens", top_k="topk")
+    return ops
+
+
+NAMES = ["table", "slots", "at", "ends", "used", "q1", "q", "kr", "o", "logits", "tokens"]
+
+
+def test_a_decode_step():
+    """Each op's result from what it was given on the GPU, so that no rounding before it
+    decides a cut: whole numbers exactly, the rest by the fp32 bars of their sizes (a few
+    dozen terms around 1: 2^-14 of the largest)."""
+    ops = _step(1)
+    env, ref = run(ops, outputs=NAMES).env, evaluate(ops)
+    for name in ("table", "slots", "at", "ends", "used"):
+        np.testing.assert_array_equal(env[name], ref[name], err_msg=name)
+    for name in ("q1", "q", "kr", "o", "logits"):
+        assert np.abs(env[name] - ref[name]).max() <= 2.0**-14 * np.abs(ref[name]).max(), name
+    u, k = ops.uploads["u"], ops.uploads["topk"]
+    want = [decoding_eval.sample_row(env["logits"][b], u[b], top_k=k[b])[0] for b in range(5)]
+    np.testing.assert_array_equal(env["tokens"], want)
+
+
+def test_a_batch_of_decode_steps():
+    programs = [_step(s) for s in range(1, 5)]
+    for ops, got in zip(programs, run_batch(programs, outputs=NAMES)):
+        alone = run(ops, outputs=NAMES).env
+        for name in NAMES:
+            np.testing.assert_array_equal(got.env[name], alone[name], err_msg=name)
+
+
+def test_a_loop_of_steps_keeps_its_buffers():
+    """The program compiled once and run again and again over one dict of buffers, as a
+    serving loop does; every run gives what the first gave."""
+    ops = _step(2)
+    groups = compile_program(ops)
+    env = {}
+    for name, v in ops.uploads.items():
+        env[name] = Buffer.from_numpy(v)
+    for t in ops.tensors.values():
+        if t.buffer_key not in env:
+            env[t.buffer_key] = Buffer(t.nbytes)
+    runtime = Runtime(tuple(Dispatch(g.kernel, g.bindings, g.dims, g.grid, g.threads) for g in groups))
+    want = run(ops, outputs=NAMES).env
+    for _ in range(3):
+        runtime.run(env)
+        for name in NAMES:
+            t = ops.tensors[name]
+            np.testing.assert_array_equal(env[t.buffer_key].numpy(t.shape, np.dtype(t.stored)), want[name], err_msg=name)
+
+
+def test_steps_of_two_threads():
+    programs = [_step(7), _step(8)]
+    want = [run(p, outputs=NAMES).env for p in programs]
+    got: list = [None, None]
+
+    def work(i):
+        for _ in range(4):
+            got[i] = run(programs[i], outputs=NAMES).env
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        for name in NAMES:
+            np.testing.assert_array_equal(a[name], b[name], err_msg=name)
