@@ -198,10 +198,12 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // ---------------------------------------------------------------------------
 // Low-rank adapters: out[m] = base[m] + s[id] B[id] (A[id] x[m]), id = ids[m].
 //
-// Rows are taken 16 at a time, an MFMA's columns.  Of the 16, those with the same id are a
-// group, led by its first row: each group reads its adapter once and multiplies all 16
-// rows (MFMA columns do not mix), of which it stores its own.  So a batch whose rows
-// each have an adapter reads each of them once, and so does one whose rows share one.
+// Rows are taken in tiles of 16 MB.  Of a tile's, those with the same id are a group, led
+// by its first row: a group reads its adapter once and multiplies all of the 16-row blocks
+// that have rows of it (an MFMA's columns do not mix), of which it stores its own.  So a
+// batch whose rows each have an adapter reads each of them once, and so does one whose rows
+// share one.  LOOP: a workgroup does all groups of a tile, otherwise a workgroup does the
+// one that its row leads, if it does.
 // fp32 MFMAs 16x16x4: with (n, g) = (lane % 16, lane / 16) a lane has 4 consecutive k of
 // row n of both operands, k = 4 g + i in the i-th of four MFMAs; the order of k is the
 // same for both, so the sum is the product's.  An element (row 4 g + i, column n) of the
@@ -209,20 +211,29 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // four neighbours of row m = n of `down` or `out`.
 // ---------------------------------------------------------------------------
 
-// Of the 16 rows from row0: bit m says whether row m is of the group that row j leads;
-// 0 where j leads none.  `id`: its adapter, -1 for rows without one.
-template <unsigned HELD>
-MT_INLINE unsigned mt_adapter_group(const int* ids, unsigned row0, unsigned rows, unsigned j, int& id) {
-    const unsigned n = mt_lane() & 15u;
-    int mine = -2;
-    if (row0 + n < rows) {
-        mine = ids[row0 + n];
-        if (mine < 0 || (unsigned)mine >= HELD) mine = -1;
+// Tiles and the rows that lead their groups.  Workgroups in turn go to the GPU's eight
+// parts in turn, so tiles, not leaders, are next to each other: few of a tile's rows lead.
+template <unsigned MB, unsigned HELD>
+struct mt_adapter_rows {
+    static constexpr unsigned TILE = 16u * MB;
+    unsigned row0, mine;  // the tile's first row, the id of this lane's (-1: none, -2: no row)
+    MT_INLINE mt_adapter_rows(const int* ids, unsigned tile, unsigned rows) : row0(tile * TILE) {
+        const unsigned row = row0 + mt_lane() % TILE;
+        int found = -2;
+        if (row < rows) {
+            found = ids[row];
+            if (found < 0 || (unsigned)found >= HELD) found = -1;
+        }
+        mine = (unsigned)found;
     }
-    id = __builtin_amdgcn_readlane(mine, (int)j);
-    const unsigned group = (unsigned)__ballot(mine == id) & 0xFFFFu;
-    return id != -2 && (unsigned)__builtin_ctz(group) == j ? group : 0u;
-}
+    // Of the tile's rows: bit m says whether row m is of the group that row j leads; 0 where
+    // j leads none.
+    MT_INLINE unsigned long long group(unsigned j, int& id) const {
+        id = __builtin_amdgcn_readlane((int)mine, (int)j);
+        const unsigned long long all = __ballot((int)mine == id) & (TILE == 64u ? ~0ull : (1ull << TILE) - 1ull);
+        return id != -2 && (unsigned)__builtin_ctzll(all) == j ? all : 0ull;
+    }
+};
 
 MT_INLINE mt_f32x4 mt_mfma16_f32(mt_f32x4 a, mt_f32x4 b, mt_f32x4 c) {
 #pragma unroll
@@ -230,97 +241,190 @@ MT_INLINE mt_f32x4 mt_mfma16_f32(mt_f32x4 a, mt_f32x4 b, mt_f32x4 c) {
     return c;
 }
 
+// The tile of a workgroup.  LOOP: the GPU's eight parts, which take workgroups in turn, have
+// neighbouring tiles each, whose rows are likely to share adapters; there are eight times
+// a whole number of workgroups then, and the last may have no tile.
+template <bool LOOP>
+MT_INLINE unsigned mt_adapter_tile(unsigned tiles) {
+    return LOOP ? blockIdx.x % 8u * (gridDim.x / 8u) + blockIdx.x / 8u : blockIdx.x % tiles;
+}
+
 // A's part: blocks of RB x 16 ranks; the waves of the SPLITS workgroups of a group take
-// 64 columns of x in turn and add up in LDS; each split stores its part.
-template <unsigned K, unsigned R, unsigned RB, unsigned SPLITS, unsigned HELD, unsigned WAVES, unsigned XRS, unsigned XCS>
+// 64 columns of x in turn and add up in LDS; each split stores its part.  Loads of 16
+// columns go out as the registers of those 64 before are free, so MFMAs and memory go on
+// together.
+template <unsigned K, unsigned R, unsigned RB, unsigned MB, bool LOOP, unsigned SPLITS, unsigned HELD, unsigned WAVES,
+          unsigned XRS, unsigned XCS>
 MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, float* down, unsigned rows,
                                mt_f32x4* lds) {
-    const unsigned row0 = blockIdx.x / 16u * 16u, split = blockIdx.y % SPLITS, r0 = blockIdx.y / SPLITS * RB * 16u;
-    const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4;
-    int id;
-    const unsigned group = mt_adapter_group<HELD>(ids, row0, rows, blockIdx.x % 16u, id);
-    if (group == 0u || id < 0) return;
-    const bool mine = (group >> n) & 1u;
-    const float* xr = x + (size_t)(row0 + n) * XRS;
-    const float* ar = a + ((size_t)(unsigned)id * R + r0 + n) * K;
-    mt_f32x4 acc[RB];
+    constexpr unsigned TILE = 16u * MB;
+    const unsigned tiles = (rows + TILE - 1u) / TILE, split = blockIdx.y % SPLITS, r0 = blockIdx.y / SPLITS * RB * 16u;
+    const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, at = mt_adapter_tile<LOOP>(tiles);
+    if (at >= tiles) return;
+    const mt_adapter_rows<MB, HELD> tile(ids, at, rows);
+#pragma unroll 1
+    for (unsigned j = LOOP ? 0u : blockIdx.x / tiles; j < TILE; ++j) {
+        int id;
+        const unsigned long long group = tile.group(j, id);
+        if (group != 0ull && id >= 0) {
+            const float* ar = a + ((size_t)(unsigned)id * R + r0 + n) * K;
+            mt_f32x4 acc[MB][RB], xv[4][MB], av[4][RB];
 #pragma unroll
-    for (unsigned b = 0; b < RB; ++b) acc[b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-    for (unsigned k0 = 64u * (split * WAVES + mt_wave()); k0 < K; k0 += 64u * SPLITS * WAVES) {
+            for (unsigned m = 0; m < MB; ++m)
 #pragma unroll
-        for (unsigned u = 0; u < 4u; ++u) {
-            const unsigned k = k0 + 16u * u + 4u * g;
-            mt_f32x4 xv = {0.f, 0.f, 0.f, 0.f}, av[RB];
-            if (mine && k < K) xv = mt_row4<K, XCS>(xr, k);
+                for (unsigned b = 0; b < RB; ++b) acc[m][b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+            const auto load = [&](unsigned k0, unsigned u) {
+                const unsigned k = k0 + 16u * u + 4u * g;
 #pragma unroll
-            for (unsigned b = 0; b < RB; ++b) {
-                av[b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-                if (r0 + 16u * b + n < R && k < K) av[b] = mt_row4<K, 1u>(ar + (size_t)(16u * b) * K, k);
+                for (unsigned m = 0; m < MB; ++m) {
+                    xv[u][m] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (((group >> (16u * m + n)) & 1ull) && (K % 64u == 0u || k < K))
+                        xv[u][m] = mt_row4<K, XCS>(x + (size_t)(tile.row0 + 16u * m + n) * XRS, k);
+                }
+#pragma unroll
+                for (unsigned b = 0; b < RB; ++b) {
+                    av[u][b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                    if ((R % 16u == 0u && RB * 16u >= R || r0 + 16u * b + n < R) && (K % 64u == 0u || k < K))
+                        av[u][b] = mt_row4<K, 1u>(ar + (size_t)(16u * b) * K, k);
+                }
+            };
+            unsigned k0 = 64u * (split * WAVES + mt_wave());
+            if (k0 < K) {
+#pragma unroll
+                for (unsigned u = 0; u < 4u; ++u) load(k0, u);
             }
+            for (; k0 < K; k0 += 64u * SPLITS * WAVES) {
+                const unsigned next = k0 + 64u * SPLITS * WAVES;
 #pragma unroll
-            for (unsigned b = 0; b < RB; ++b) acc[b] = mt_mfma16_f32(av[b], xv, acc[b]);
+                for (unsigned u = 0; u < 4u; ++u) {
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (unsigned m = 0; m < MB; ++m)
+                        if (MB == 1u || ((group >> (16u * m)) & 0xFFFFull))
+#pragma unroll
+                            for (unsigned b = 0; b < RB; ++b) acc[m][b] = mt_mfma16_f32(av[u][b], xv[u][m], acc[m][b]);
+                    if (next < K) load(next, u);
+                }
+            }
+            if (LOOP) __syncthreads();  // (the group before has been added up)
+#pragma unroll
+            for (unsigned m = 0; m < MB; ++m)
+#pragma unroll
+                for (unsigned b = 0; b < RB; ++b) lds[((mt_wave() * MB + m) * RB + b) * 64u + lane] = acc[m][b];
+            __syncthreads();
+            for (unsigned e = threadIdx.x; e < MB * RB * 64u; e += WAVES * 64u) {
+                mt_f32x4 v = lds[e];
+#pragma unroll
+                for (unsigned w = 1; w < WAVES; ++w) v = v + lds[w * MB * RB * 64u + e];
+                const unsigned m = e / (64u * RB) * 16u + e % 16u, r = r0 + e / 64u % RB * 16u + e / 16u % 4u * 4u;
+                if ((group >> m) & 1ull) {
+                    float* to = down + ((size_t)split * rows + tile.row0 + m) * R;
+                    if (R % 4u == 0u) {
+                        if (r < R) mt_st4(to + r, v);
+                    } else {
+#pragma unroll
+                        for (unsigned i = 0; i < 4u; ++i)
+                            if (r + i < R) to[r + i] = v[i];
+                    }
+                }
+            }
         }
-    }
-#pragma unroll
-    for (unsigned b = 0; b < RB; ++b) lds[(mt_wave() * RB + b) * 64u + lane] = acc[b];
-    __syncthreads();
-    for (unsigned e = threadIdx.x; e < RB * 64u; e += WAVES * 64u) {
-        mt_f32x4 v = lds[e];
-        for (unsigned w = 1; w < WAVES; ++w) v = v + lds[w * RB * 64u + e];
-        const unsigned m = e & 15u, r = r0 + e / 64u * 16u + (e / 16u & 3u) * 4u;
-        if ((group >> m) & 1u) {
-            float* to = down + ((size_t)split * rows + row0 + m) * R;
-#pragma unroll
-            for (unsigned i = 0; i < 4u; ++i)
-                if (r + i < R) to[r + i] = v[i];
-        }
+        if (!LOOP) break;
     }
 }
 
-// B's part and the sum: a wave takes PER blocks of 16 columns of the output.
-template <unsigned N, unsigned R, unsigned SPLITS, unsigned HELD, unsigned WAVES, unsigned PER, unsigned YRS,
-          unsigned YCS>
+// B's part and the sum: a wave takes PER blocks of 16 columns of the output, and loads
+// AHEAD of them, of B and of base, before it needs them.  Tiles of several blocks of rows
+// have `down`'s parts added up in LDS, once for all waves.
+template <unsigned N, unsigned R, unsigned MB, bool LOOP, unsigned SPLITS, unsigned HELD, unsigned WAVES, unsigned PER,
+          unsigned AHEAD, unsigned YRS, unsigned YCS>
 MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* b, const int* ids, const float* scales,
-                             float* out, unsigned rows) {
-    constexpr unsigned RC = (R + 15u) / 16u;
-    const unsigned row0 = blockIdx.x / 16u * 16u, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
-    int id;
-    const unsigned group = mt_adapter_group<HELD>(ids, row0, rows, blockIdx.x % 16u, id);
-    if (group == 0u) return;
-    const bool mine = (group >> n) & 1u;
-    const unsigned row = row0 + n;
-    mt_f32x4 t[RC];
-#pragma unroll
-    for (unsigned c = 0; c < RC; ++c) {
-        t[c] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-        const unsigned r = 16u * c + 4u * g;
-        if (mine && id >= 0 && r < R)
-            for (unsigned s = 0; s < SPLITS; ++s) t[c] = t[c] + mt_row4<R, 1u>(down + ((size_t)s * rows + row) * R, r);
-    }
-    const float scale = scales != nullptr && id >= 0 ? scales[id] : 1.f;
-    const unsigned n0 = (blockIdx.y * WAVES + mt_wave()) * PER * 16u;
+                             float* out, unsigned rows, float* lds) {
+    constexpr unsigned RC = (R + 15u) / 16u, TILE = 16u * MB, PITCH = 16u * RC + 4u;
+    static_assert(PER % AHEAD == 0u, "blocks in whole sets");
+    const unsigned tiles = (rows + TILE - 1u) / TILE, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
+    const unsigned n0 = (blockIdx.y * WAVES + mt_wave()) * PER * 16u, at = mt_adapter_tile<LOOP>(tiles);
+    if (at >= tiles) return;
+    const mt_adapter_rows<MB, HELD> tile(ids, at, rows);
 #pragma unroll 1
-    for (unsigned p = 0; p < PER; ++p) {
-        const unsigned from = n0 + 16u * p, col = from + 4u * g;
-        if (from >= N) break;
-        mt_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        if (id >= 0) {
-            const float* br = b + ((size_t)(unsigned)id * N + from + n) * R;
+    for (unsigned j = LOOP ? 0u : blockIdx.x / tiles; j < TILE; ++j) {
+        int id;
+        const unsigned long long group = tile.group(j, id);
+        if (group != 0ull) {
+            mt_f32x4 bv[AHEAD][RC], v[AHEAD][MB], t[MB][RC];
+            const auto load = [&](unsigned from, unsigned p) {
+                const float* br = b + ((size_t)(unsigned)(id < 0 ? 0 : id) * N + from + n) * R;
 #pragma unroll
-            for (unsigned c = 0; c < RC; ++c) {
-                mt_f32x4 bv = {0.f, 0.f, 0.f, 0.f};
-                if (from + n < N && 16u * c + 4u * g < R) bv = mt_row4<R, 1u>(br, 16u * c + 4u * g);
-                acc = mt_mfma16_f32(bv, t[c], acc);
+                for (unsigned c = 0; c < RC; ++c) {
+                    bv[p][c] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (id >= 0 && (N % 16u == 0u || from + n < N) && (R % 16u == 0u || 16u * c + 4u * g < R))
+                        bv[p][c] = mt_row4<R, 1u>(br, 16u * c + 4u * g);
+                }
+                const unsigned col = from + 4u * g;
+#pragma unroll
+                for (unsigned m = 0; m < MB; ++m) {
+                    v[p][m] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                    if (((group >> (16u * m + n)) & 1ull) && (N % 16u == 0u || col < N))
+                        v[p][m] = mt_row4<N, YCS>(base + (size_t)(tile.row0 + 16u * m + n) * YRS, col);
+                }
+            };
+#pragma unroll
+            for (unsigned p = 0; p < AHEAD; ++p)
+                if (n0 + 16u * p < N) load(n0 + 16u * p, p);
+            // the sums of down's parts; nothing for rows of other groups
+            const auto parts = [&](unsigned m, unsigned r) {
+                mt_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+                if (((group >> m) & 1ull) && id >= 0 && r < R) {
+#pragma unroll
+                    for (unsigned s = 0; s < SPLITS; ++s)
+                        sum = sum + mt_row4<R, 1u>(down + ((size_t)s * rows + tile.row0 + m) * R, r);
+                }
+                return sum;
+            };
+            if constexpr (MB > 1u) {
+                if (LOOP) __syncthreads();  // (the group before has been multiplied)
+                for (unsigned e = threadIdx.x; e < TILE * RC * 4u; e += WAVES * 64u) {
+                    const unsigned m = e / (RC * 4u), r = e % (RC * 4u) * 4u;
+                    *reinterpret_cast<mt_f32x4*>(lds + m * PITCH + r) = parts(m, r);
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (unsigned m = 0; m < MB; ++m)
+#pragma unroll
+                for (unsigned c = 0; c < RC; ++c) {
+                    if constexpr (MB > 1u) {
+                        t[m][c] = *reinterpret_cast<const mt_f32x4*>(lds + (16u * m + n) * PITCH + 16u * c + 4u * g);
+                    } else {
+                        t[m][c] = parts(n, 16u * c + 4u * g);
+                    }
+                }
+            const float scale = scales != nullptr && id >= 0 ? scales[id] : 1.f;
+#pragma unroll 1
+            for (unsigned p0 = 0; p0 < PER; p0 += AHEAD) {
+#pragma unroll
+                for (unsigned p = 0; p < AHEAD; ++p) {
+                    const unsigned from = n0 + 16u * (p0 + p), col = from + 4u * g;
+                    if (from >= N) break;
+#pragma unroll
+                    for (unsigned m = 0; m < MB; ++m) {
+                        if (MB > 1u && !((group >> (16u * m)) & 0xFFFFull)) continue;
+                        if (id >= 0) {
+                            mt_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (unsigned c = 0; c < RC; ++c) acc = mt_mfma16_f32(bv[p][c], t[m][c], acc);
+#pragma unroll
+                            for (unsigned i = 0; i < 4u; ++i) v[p][m][i] = __builtin_fmaf(scale, acc[i], v[p][m][i]);
+                        }
+                        if (((group >> (16u * m + n)) & 1ull) && (N % 16u == 0u || col < N))
+                            mt_put_row4<N>(out + (size_t)(tile.row0 + 16u * m + n) * N, col, v[p][m]);
+                    }
+                    if (p0 + p + AHEAD < PER && from + 16u * AHEAD < N) load(from + 16u * AHEAD, p);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
         }
-        if (mine && col < N) {
-            mt_f32x4 v = mt_row4<N, YCS>(base + (size_t)row * YRS, col);
-            if (id >= 0) {
-#pragma unroll
-                for (unsigned i = 0; i < 4u; ++i) v[i] = __builtin_fmaf(scale, acc[i], v[i]);
-            }
-            mt_put_row4<N>(out + (size_t)row * N, col, v);
-        }
+        if (!LOOP) break;
     }
 }
 

@@ -10,7 +10,16 @@ from metellus_amd.compute.fragments import decoding_header
 from metellus_amd.compute.serving import ServingFragment
 from metellus_amd.orchestrator.assembly.decision import DecisionView
 from metellus_amd.orchestrator.assembly.serving import _ceil, _group, _Signature
-from metellus_amd.orchestrator.decoding import AdapterDownOp, AdapterUpOp, PageTablesOp, Rotary, RotaryOp, SampleOp
+from metellus_amd.orchestrator.decoding import (
+    ADAPTER_DOWN_WAVES,
+    ADAPTER_MANY_ROWS,
+    AdapterDownOp,
+    AdapterUpOp,
+    PageTablesOp,
+    Rotary,
+    RotaryOp,
+    SampleOp,
+)
 from metellus_amd.orchestrator.ir import Tensor
 from metellus_amd.orchestrator.kernel_group import FusionStrategy, KernelGroup
 
@@ -117,42 +126,66 @@ def _assemble_rotary(decision: DecisionView, op: RotaryOp, function_name: str | 
 # adapters
 # ---------------------------------------------------------------------------
 
-ADAPTER_DOWN_WAVES = 8
-ADAPTER_DOWN_BLOCKS = 4  # of 16 ranks, that a wave multiplies x by at once
-ADAPTER_UP_WAVES, ADAPTER_UP_PER = 4, 4
+ADAPTER_BLOCKS = 4  # of 16 ranks, that a wave multiplies x by at once
+
+
+def adapter_tile(rows: int, rank: int) -> tuple[int, bool]:
+    """Blocks of 16 rows in a tile (one where the rank leaves no registers for more), and
+    whether a workgroup does all groups of its tile."""
+    many = rows >= ADAPTER_MANY_ROWS
+    return (4 if many and rank <= 64 else 1), many
+
+
+def _adapter_workgroups(rows: int, tile: int, loop: bool) -> int:
+    tiles = _ceil(rows, 16 * tile)
+    return 8 * _ceil(tiles, 8) if loop else 16 * tile * tiles
 
 
 def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_name: str | None) -> KernelGroup:
     rows, inner = op.x.shape
-    blocks = min(ADAPTER_DOWN_BLOCKS, _ceil(op.rank, 16))
+    blocks = min(ADAPTER_BLOCKS, _ceil(op.rank, 16))
+    tile, loop = adapter_tile(rows, op.rank)
+    waves = ADAPTER_DOWN_WAVES[loop]
     sig = _Signature()
     args = (sig.add("x", op.x), sig.add("a", op.a), sig.add("ids", op.ids), sig.add("down", op.down, out=True), "M",
             "(mt_f32x4*)mt_lds")
     frag = ServingFragment(
         "mt_adapter_down",
-        (inner, op.rank, blocks, op.splits, op.held, ADAPTER_DOWN_WAVES, *_strides(op.x)),
+        (inner, op.rank, blocks, tile, loop, op.splits, op.held, waves, *_strides(op.x)),
         args,
-        lds_bytes=ADAPTER_DOWN_WAVES * blocks * 1024,
+        lds_bytes=waves * tile * blocks * 1024,
         name="adapter_down",
     )
-    grid = (16 * _ceil(rows, 16), op.splits * _ceil(op.rank, 16 * blocks), 1)
-    return _group(decision, sig, frag, function_name or f"adapter_down_{op.name}", {"M": rows}, grid, 64 * ADAPTER_DOWN_WAVES,
+    grid = (_adapter_workgroups(rows, tile, loop), op.splits * _ceil(op.rank, 16 * blocks), 1)
+    return _group(decision, sig, frag, function_name or f"adapter_down_{op.name}", {"M": rows}, grid, 64 * waves,
                   headers=(decoding_header(),))
+
+
+def adapter_up_shape(rows: int, rank: int) -> tuple[int, int, int]:
+    """Waves of a workgroup, the blocks of 16 columns that each takes, and those it loads
+    ahead."""
+    tile, _ = adapter_tile(rows, rank)
+    if tile > 1:
+        return 8, 8, 2
+    return 4, 4, 4 if rank <= 32 else 2 if rank <= 64 else 1
 
 
 def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name: str | None) -> KernelGroup:
     rows, cols = op.base.shape
+    tile, loop = adapter_tile(rows, op.rank)
+    waves, per, ahead = adapter_up_shape(rows, op.rank)
     sig = _Signature()
     args = (sig.add("base", op.base), sig.add("down", op.down), sig.add("b", op.b), sig.add("ids", op.ids),
-            sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M")
+            sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M", "(float*)mt_lds" if tile > 1 else "nullptr")
     frag = ServingFragment(
         "mt_adapter_up",
-        (cols, op.rank, op.splits, op.held, ADAPTER_UP_WAVES, ADAPTER_UP_PER, *_strides(op.base)),
+        (cols, op.rank, tile, loop, op.splits, op.held, waves, per, ahead, *_strides(op.base)),
         args,
+        lds_bytes=64 * tile * (16 * _ceil(op.rank, 16) + 4) if tile > 1 else 0,
         name="adapter_up",
     )
-    grid = (16 * _ceil(rows, 16), _ceil(cols, 16 * ADAPTER_UP_WAVES * ADAPTER_UP_PER), 1)
-    return _group(decision, sig, frag, function_name or f"adapter_up_{op.y.name}", {"M": rows}, grid, 64 * ADAPTER_UP_WAVES,
+    grid = (_adapter_workgroups(rows, tile, loop), _ceil(cols, 16 * waves * per), 1)
+    return _group(decision, sig, frag, function_name or f"adapter_up_{op.y.name}", {"M": rows}, grid, 64 * waves,
                   headers=(decoding_header(),))
 
 

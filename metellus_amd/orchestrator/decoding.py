@@ -120,10 +120,16 @@ class Rotary:
         return tuple(found)
 
 
+ADAPTER_MANY_ROWS = 1024  # from here on tiles of 64 rows, a workgroup for all groups of each
+ADAPTER_DOWN_WAVES = (4, 8)  # a workgroup's for fewer rows, and for so many
+
+
 def adapter_splits(rows: int, inner: int) -> int:
     """Shares of x's columns that workgroups take apart, where rows alone are too few
-    workgroups to fill the GPU: at least 256 columns each."""
-    return max(1, min(-(-inner // 256), 512 // rows))
+    workgroups to fill the GPU: at least as many columns as its waves take at once."""
+    many = rows >= ADAPTER_MANY_ROWS
+    wanted = -(-256 // -(-rows // 64)) if many else 512 // rows
+    return max(1, min(-(-inner // (64 * ADAPTER_DOWN_WAVES[many])), wanted))
 
 
 # ---------------------------------------------------------------------------

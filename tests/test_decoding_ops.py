@@ -229,8 +229,9 @@ def test_scheduling_adapters():
 
 def test_shares_of_columns():
     assert adapter_splits(1, 4096) == 16 and adapter_splits(1, 100) == 1
-    assert adapter_splits(32, 4096) == 16 and adapter_splits(4096, 4096) == 1
-    for rows in (1, 3, 50, 700):
+    assert adapter_splits(32, 4096) == 16 and adapter_splits(4096, 4096) == 4 and adapter_splits(600, 4096) == 1
+    assert adapter_splits(16384, 4096) == 1
+    for rows in (1, 3, 50, 700, 1024, 5000):
         for inner in (1, 255, 257, 5003, 16384):
             assert 1 <= adapter_splits(rows, inner) <= -(-inner // 256)
 
@@ -333,9 +334,10 @@ def test_rotary_compiles(spec):
     _compile(ops)
 
 
+@pytest.mark.parametrize("rows", [5, 2000])
 @pytest.mark.parametrize("rank", [3, 16, 100])
-def test_adapters_compile(rank):
-    ops = _ops(**{**ADAPTERS, "a": (3 * rank, 12), "b": (60, rank)})
+def test_adapters_compile(rank, rows):
+    ops = _ops(**{**ADAPTERS, "x": (rows, 12), "y": (rows, 20), "ids": ((rows,), "int32"), "a": (3 * rank, 12), "b": (60, rank)})
     ops.adapters(**ADAPTER_CALL, scales="s" if rank == 16 else None)
     _compile(ops)
 

@@ -18,8 +18,7 @@ import pytest
 
 from metellus_amd.api import compile_program, run, run_batch
 from metellus_amd.orchestrator import KVCache, Operations, Rotary
-from metellus_amd.orchestrator.assembly.decoding import ADAPTER_DOWN_WAVES
-from metellus_amd.orchestrator.decoding import AdapterDownOp, AdapterUpOp
+from metellus_amd.orchestrator.decoding import ADAPTER_DOWN_WAVES, ADAPTER_MANY_ROWS, AdapterDownOp, AdapterUpOp
 from metellus_amd.runtime import Buffer, Dispatch, Runtime
 from oracle import decoding_eval
 from oracle.ir_eval import evaluate
@@ -217,7 +216,8 @@ def _adapter_bound(ops):
     x = value["x"] if "x" in value else value["x_"].T
     base = evaluate(ops)["y"]
     inner, rank, n = x.shape[1], down.rank, up.y.shape[1]
-    terms = 2 * 64 * -(-inner // (64 * down.splits * ADAPTER_DOWN_WAVES)) + ADAPTER_DOWN_WAVES + down.splits
+    waves = ADAPTER_DOWN_WAVES[x.shape[0] >= ADAPTER_MANY_ROWS]
+    terms = 2 * 64 * -(-inner // (64 * down.splits * waves)) + waves + down.splits
     bound = np.abs(base) * U
     for m, i in enumerate(ops.uploads["ids"]):
         if 0 <= i < down.held:
@@ -258,6 +258,7 @@ def _adapter_check(ops):
 @pytest.mark.parametrize("rows, inner, cols, rank, held", [
     (1, 1, 1, 1, 1), (1, 64, 16, 4, 2), (1, 4096, 300, 16, 3), (2, 100, 17, 8, 5), (7, 333, 129, 23, 4), (16, 512, 256, 16, 16),
     (17, 1000, 1003, 64, 3), (33, 257, 65, 5, 40), (100, 640, 1024, 65, 7), (3, 129, 260, 256, 2), (600, 96, 48, 12, 9),
+    (1024, 1500, 100, 16, 5), (1100, 70, 33, 64, 3), (1061, 600, 70, 70, 200),
 ])
 @pytest.mark.parametrize("scales", [False, True])
 def test_adapters(rows, inner, cols, rank, held, scales):
