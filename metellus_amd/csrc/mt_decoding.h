@@ -502,7 +502,18 @@ struct mt_weights {
         if (x == top) return 1.0;
         return x == -INFINITY || top == INFINITY ? 0.0 : exp(scaled(x));  // (whatever the temperature)
     }
-    MT_INLINE mt_u64 held(float x) const { return (mt_u64)__builtin_rint(weight(x) * (double)(1ull << SHIFT)); }
+    MT_INLINE static mt_u64 whole(double w) { return (mt_u64)__builtin_rint(w * (double)(1ull << SHIFT)); }
+    MT_INLINE mt_u64 held(float x) const { return whole(weight(x)); }
+    // 0 for a weight below `least`.
+    MT_INLINE mt_u64 kept(float x, double least) const {
+        const double w = weight(x);
+        return w < least ? 0 : whole(w);
+    }
+    MT_INLINE void answer(unsigned row, unsigned i, float x, mt_u64 total, int* tokens, float* logprobs) const {
+        tokens[row] = (int)i;
+        if (logprobs != nullptr)
+            logprobs[row] = (float)((x == top ? 0.0 : scaled(x)) - log((double)total / (double)(1ull << SHIFT)));
+    }
 };
 
 // A cut of a row: what stays lies above `key`, or is one of its equals up to index `last`.
@@ -549,14 +560,67 @@ MT_INLINE unsigned mt_find_cut(EACH each, AMOUNT amount, mt_u64 asked, mt_u64& a
     return key;
 }
 
-template <unsigned V, unsigned SHIFT, unsigned WAVES, unsigned RS, unsigned CS>
-MT_INLINE void mt_sample(const float* logits, const float* uniforms, const float* temperatures, const int* top_k,
-                         const float* top_p, const float* min_p, int* tokens, float* logprobs, mt_u64* lds) {
+// A row's numbers.
+struct mt_asked {
+    float temperature, p, u;
+    double least;
+    int k;
+    MT_INLINE mt_asked(unsigned row, const float* uniforms, const float* temperatures, const int* top_k, const float* top_p,
+                       const float* min_p) {
+        temperature = temperatures != nullptr ? temperatures[row] : 1.f;
+        k = top_k != nullptr ? top_k[row] : 0;
+        p = top_p != nullptr ? top_p[row] : 1.f;
+        u = uniforms[row];
+        const float m = min_p != nullptr ? min_p[row] : 0.f;
+        least = m > 0.f ? (double)__builtin_fminf(m, 1.f) : 0.0;
+    }
+    // The weight before which the largest stay, of `total`: the first always does.
+    MT_INLINE mt_u64 weight_asked(mt_u64 total) const {
+        const mt_u64 asked = p > 0.f ? (mt_u64)__builtin_ceil((double)p * (double)total) : 1;
+        return asked < 1 ? 1 : asked < total ? asked : total;
+    }
+    // The weight before the token, of `total`.
+    MT_INLINE mt_u64 target(mt_u64 total) const {
+        const mt_u64 found = u > 0.f ? (mt_u64)((double)__builtin_fminf(u, 1.f) * (double)total) : 0;
+        return found < total ? found : total - 1;
+    }
+};
+
+// Where a cut falls among equals: of those equal to cut.key, which weigh or count `one` each
+// and `at` together, those stay that it takes to reach what is asked for; nth(key, n) is the
+// index of the n-th.
+template <typename NTH>
+MT_INLINE void mt_cut_equals(mt_cut_at& cut, mt_u64 asked, mt_u64 above, mt_u64 at, mt_u64 one, NTH nth) {
+    const mt_u64 n = (asked - above + one - 1) / one;
+    if (n < at / one) cut.last = nth(cut.key, n);
+}
+
+// The first of a row's largest, by key and index: larger is better, and nothing is above a NaN.
+MT_INLINE mt_u64 mt_best(unsigned i, float v) {
+    return v == v ? ((mt_u64)mt_order_key(v) << 32) | (0xFFFFFFFFu - i) : ~0ull;
+}
+
+// The answer for a row that has no choice; false for one that has.
+MT_INLINE bool mt_sample_plain(mt_u64 best, float temperature, unsigned row, bool writes, int* tokens, float* logprobs) {
+    const bool none = best == ~0ull || mt_order_value((unsigned)(best >> 32)) == -INFINITY;
+    if (!none && temperature > 0.f) return false;
+    if (writes) {
+        tokens[row] = none ? -1 : (int)(0xFFFFFFFFu - (unsigned)best);
+        if (logprobs != nullptr) logprobs[row] = none ? NAN : 0.f;
+    }
+    return true;
+}
+
+// One workgroup draws from a whole row, in as many passes over it as it takes: for rows
+// that the two kernels below do not have in pieces small enough.
+template <unsigned V, unsigned SHIFT, unsigned WAVES, unsigned CS>
+MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_weights<SHIFT>& weights, unsigned row,
+                               int* tokens, float* logprobs, mt_u64* lds) {
     constexpr unsigned LANES = 64u * WAVES, STEP = 4u * LANES;
-    const unsigned row = blockIdx.x, t = threadIdx.x;
-    const float* x = logits + (size_t)row * RS;
+    const unsigned t = threadIdx.x;
     const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
     const auto each = [&](auto f) {
+#pragma unroll 1
         for (unsigned c = 4u * t; c < V; c += STEP) {
             const mt_f32x4 v = mt_row4<V, CS>(x, c);
 #pragma unroll
@@ -564,29 +628,10 @@ MT_INLINE void mt_sample(const float* logits, const float* uniforms, const float
                 if (c + j < V) f(c + j, v[j]);
         }
     };
-    // The first of the largest, by key and index; nothing is above a NaN.
-    mt_u64 best = 0;
-    each([&](unsigned i, float v) {
-        const mt_u64 found = v == v ? ((mt_u64)mt_order_key(v) << 32) | (0xFFFFFFFFu - i) : ~0ull;
-        best = found > best ? found : best;
-    });
-    best = mt_group_fold<WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
-    const float top = mt_order_value((unsigned)(best >> 32));
-    const float temperature = temperatures != nullptr ? temperatures[row] : 1.f;
-    const bool none = best == ~0ull || top == -INFINITY;
-    if (none || !(temperature > 0.f)) {
-        if (t == 0u) {
-            tokens[row] = none ? -1 : (int)(0xFFFFFFFFu - (unsigned)best);
-            if (logprobs != nullptr) logprobs[row] = none ? NAN : 0.f;
-        }
-        return;
-    }
-    const mt_weights<SHIFT> weights{top, (double)temperature};
-
-    mt_cut_at cut{0u, 0xFFFFFFFFu};
     // The index of the n-th of those equal to `key`, of which there are more.
     const auto nth = [&](unsigned key, mt_u64 n) {
         mt_u64 seen = 0;
+#pragma unroll 1
         for (unsigned c0 = 0; c0 < V; c0 += STEP) {
             const unsigned c = c0 + 4u * t;
             unsigned hits = 0u;
@@ -610,39 +655,30 @@ MT_INLINE void mt_sample(const float* logits, const float* uniforms, const float
         __syncthreads();
         return found;
     };
-    const int k = top_k != nullptr ? top_k[row] : 0;
-    if (k > 0 && (unsigned)k < V) {
-        mt_u64 above, at;
-        cut.key = mt_find_cut<WAVES>(each, [](unsigned, float) { return (mt_u64)1; }, (mt_u64)k, above, at, lds);
-        if ((mt_u64)k - above < at) cut.last = nth(cut.key, (mt_u64)k - above);
+    mt_cut_at cut{0u, 0xFFFFFFFFu};
+    mt_u64 above, at;
+    if (asked.k > 0 && (unsigned)asked.k < V) {
+        cut.key = mt_find_cut<WAVES>(each, [](unsigned, float) { return (mt_u64)1; }, (mt_u64)asked.k, above, at, lds);
+        mt_cut_equals(cut, (mt_u64)asked.k, above, at, 1, nth);
     }
-    const float p = top_p != nullptr ? top_p[row] : 1.f;
-    if (p < 1.f) {
+    if (asked.p < 1.f) {
         const mt_cut_at by_k = cut;
         const auto amount = [&](unsigned i, float v) { return by_k.stays(mt_order_key(v), i) ? weights.held(v) : (mt_u64)0; };
         mt_u64 total = 0;
         each([&](unsigned i, float v) { total += amount(i, v); });
         total = mt_group_fold<WAVES>(total, lds, sum);
-        // the first of them stays whatever p is
-        mt_u64 asked = p > 0.f ? (mt_u64)__builtin_ceil((double)p * (double)total) : 1, above, at;
-        asked = asked < 1 ? 1 : asked < total ? asked : total;
-        cut.key = mt_find_cut<WAVES>(each, amount, asked, above, at, lds);
+        const mt_u64 wanted = asked.weight_asked(total);
+        cut.key = mt_find_cut<WAVES>(each, amount, wanted, above, at, lds);
         if (cut.key != by_k.key) cut.last = 0xFFFFFFFFu;
-        const mt_u64 one = weights.held(mt_order_value(cut.key)), n = (asked - above + one - 1) / one;
-        if (n < at / one) cut.last = nth(cut.key, n);
+        mt_cut_equals(cut, wanted, above, at, weights.held(mt_order_value(cut.key)), nth);
     }
-    const float m = min_p != nullptr ? min_p[row] : 0.f;
-    const double least = m > 0.f ? (double)__builtin_fminf(m, 1.f) : 0.0;
-    const auto amount = [&](unsigned i, float v) {
-        return cut.stays(mt_order_key(v), i) && !(weights.weight(v) < least) ? weights.held(v) : (mt_u64)0;
-    };
+    const auto amount = [&](unsigned i, float v) { return cut.stays(mt_order_key(v), i) ? weights.kept(v, asked.least) : (mt_u64)0; };
     mt_u64 total = 0;
     each([&](unsigned i, float v) { total += amount(i, v); });
     total = mt_group_fold<WAVES>(total, lds, sum);
-    const float u = uniforms[row];
-    mt_u64 target = u > 0.f ? (mt_u64)((double)__builtin_fminf(u, 1.f) * (double)total) : 0;
-    if (target >= total) target = total - 1;
+    const mt_u64 target = asked.target(total);
     mt_u64 seen = 0;
+#pragma unroll 1
     for (unsigned c0 = 0; c0 < V; c0 += STEP) {
         const unsigned c = c0 + 4u * t;
         mt_u64 w[4] = {0, 0, 0, 0};
@@ -654,15 +690,352 @@ MT_INLINE void mt_sample(const float* logits, const float* uniforms, const float
         mt_u64 all, before = seen + mt_group_before<WAVES>(w[0] + w[1] + w[2] + w[3], lds, all);
 #pragma unroll
         for (unsigned j = 0; j < 4u; ++j) {
-            if (before <= target && target < before + w[j]) {
-                tokens[row] = (int)(c + j);
-                if (logprobs != nullptr)
-                    logprobs[row] = (float)((v[j] == top ? 0.0 : weights.scaled(v[j])) -
-                                            log((double)total / (double)(1ull << SHIFT)));
-            }
+            if (before <= target && target < before + w[j]) weights.answer(row, c + j, v[j], total, tokens, logprobs);
             before += w[j];
         }
         seen += all;
         if (seen > target) break;  // (the same in all lanes)
     }
+}
+
+// ---------------------------------------------------------------------------
+// Two kernels draw from rows of which S chunks are in as many workgroups, PER neighbours to
+// a lane.
+//
+// The first finds a chunk's largest and, for rows that k or p cut, counts its logits by how
+// far below it they are: 512 bins of a sixteenth of the temperature, on a grid that all
+// chunks share (bin f of x is floor(16 x / T)), each with its number of logits and about
+// what they weigh.  What lies further below, 31.9 temperatures and more, weighs less than
+// 2^-45 of the largest, and is 0 as it is held.
+// The second adds the chunks' bins up, in every workgroup for itself, and so knows in which
+// bin the cut is.  What lies above it stays, and is only added up; what lies in it -- or,
+// where k and p both cut, everything from k's bin on, for p's cut depends on where k's is --
+// is listed, in the order of the indexes.  The last of a row's workgroups to arrive finds
+// the cut in the list, adds what stays to the sums of the chunks, and looks through the
+// chunk that the random number falls into.
+// All of it counts with the same whole numbers as one workgroup alone, and what the bins
+// say about weights, in 32 bits, is checked; rows that do not fit -- a list beyond LIST, a
+// bin that p's cut is next to, logits so large that a bin is none of theirs -- are drawn
+// from by one workgroup.
+// ---------------------------------------------------------------------------
+
+constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 8192u;
+constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
+
+// The bin of x on the grid of a temperature.
+struct mt_grid {
+    float by;
+    MT_INLINE explicit mt_grid(float temperature) : by(16.0f / temperature) {}
+    MT_INLINE float bin(float x) const { return __builtin_floorf(x * by); }
+};
+
+// This lane's PER logits of a chunk; -inf behind the row's end.
+template <unsigned V, unsigned PER, unsigned CS>
+MT_INLINE void mt_sample_load(const float* x, unsigned i0, float (&v)[PER]) {
+#pragma unroll
+    for (unsigned q = 0; q < PER; q += 4u) {
+        mt_f32x4 four = {0.f, 0.f, 0.f, 0.f};
+        if (i0 + q < V) four = mt_row4<V, CS>(x, i0 + q);
+#pragma unroll
+        for (unsigned j = 0; j < 4u; ++j) v[q + j] = i0 + q + j < V ? four[j] : -INFINITY;
+    }
+}
+
+// What the kernels leave in memory: the largest of each chunk; its bins; the sums of its
+// weights; the listed logits; a row's arrivals.
+template <unsigned S, unsigned ROOM>
+struct mt_sample_parts {
+    mt_u64* best;        // [row][S]
+    mt_u64* bins;        // [row][S][MT_SAMPLE_BINS]
+    mt_u64* sums;        // [row][S][4]: all, above the cut, above it and kept, listed
+    mt_u64* list;        // [row][S][ROOM]: key and index
+    unsigned* arrivals;  // [row]
+};
+
+template <unsigned V, unsigned PER, unsigned S, unsigned WAVES, unsigned RS, unsigned CS, bool CUT>
+MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, const int* top_k, const float* top_p,
+                              mt_u64* best_out, mt_u64* bins_out, unsigned* arrivals, mt_u64* lds) {
+    constexpr unsigned LANES = 64u * WAVES;
+    const unsigned row = blockIdx.x / S, chunk = blockIdx.x % S, t = threadIdx.x, i0 = (chunk * LANES + t) * PER;
+    if (chunk == 0u && t == 0u) arrivals[row] = 0u;
+    float v[PER];
+    mt_sample_load<V, PER, CS>(logits + (size_t)row * RS, i0, v);
+    mt_u64* bins = lds + WAVES;
+    if (CUT)
+        for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins[b] = 0;
+    mt_u64 best = 0;
+#pragma unroll
+    for (unsigned e = 0; e < PER; ++e)
+        if (i0 + e < V) {
+            const mt_u64 found = mt_best(i0 + e, v[e]);
+            best = found > best ? found : best;
+        }
+    best = mt_group_fold<WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
+    if (t == 0u) best_out[(size_t)row * S + chunk] = best;
+    if constexpr (CUT) {
+        const float temperature = temperatures != nullptr ? temperatures[row] : 1.f;
+        const bool by_p = top_p != nullptr && top_p[row] < 1.f, by_k = top_k != nullptr && top_k[row] > 0;
+        if (!(temperature > 0.f) || !(by_p || by_k)) return;
+        const mt_grid grid(temperature);
+        const float first = grid.bin(mt_order_value((unsigned)(best >> 32)));
+#pragma unroll
+        for (unsigned e = 0; e < PER; ++e) {
+            const float f = grid.bin(v[e]), below = first - f;
+            if (i0 + e < V && below >= 0.f && below < (float)MT_SAMPLE_BINS) {
+                mt_u64 word = 1ull << MT_SAMPLE_COUNT_AT;
+                if (by_p) word += (mt_u64)(__builtin_amdgcn_exp2f((v[e] * grid.by - f) * (1.44269504f / 16.f)) * 1048576.f);
+                atomicAdd(bins + (unsigned)below, word);
+            }
+        }
+        __syncthreads();
+        for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins_out[((size_t)row * S + chunk) * MT_SAMPLE_BINS + b] = bins[b];
+    }
+}
+
+template <unsigned V, unsigned PER, unsigned S, unsigned SHIFT, unsigned WAVES, unsigned RS, unsigned CS, bool CUT>
+MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const float* temperatures, const int* top_k,
+                              const float* top_p, const float* min_p, const mt_u64* best_in, const mt_u64* bins_in,
+                              unsigned* arrivals, mt_u64* sums, mt_u64* list, int* tokens, float* logprobs, mt_u64* lds) {
+    constexpr unsigned LANES = 64u * WAVES, ROOM = PER * LANES < MT_SAMPLE_LIST ? PER * LANES : MT_SAMPLE_LIST;
+    constexpr unsigned DEEP = MT_SAMPLE_LIST / LANES;
+    const unsigned row = blockIdx.x / S, chunk = blockIdx.x % S, t = threadIdx.x, i0 = (chunk * LANES + t) * PER;
+    const float* x = logits + (size_t)row * RS;
+    const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
+    const mt_asked asked(row, uniforms, temperatures, top_k, top_p, min_p);
+    float v[PER];
+    mt_sample_load<V, PER, CS>(x, i0, v);
+    mt_u64 best = 0;
+    for (unsigned c = mt_lane(); c < S; c += 64u) {
+        const mt_u64 found = best_in[(size_t)row * S + c];
+        best = found > best ? found : best;
+    }
+    best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
+    if (mt_sample_plain(best, asked.temperature, row, chunk == 0u && t == 0u, tokens, logprobs)) return;
+    const mt_weights<SHIFT> weights{mt_order_value((unsigned)(best >> 32)), (double)asked.temperature};
+    const mt_grid grid(asked.temperature);
+    const float first = grid.bin(weights.top);
+
+    // From which bin on logits are listed, and up to which: those above the first stay, those
+    // below the last go.
+    bool by_k = asked.k > 0 && (unsigned)asked.k < V, by_p = asked.p < 1.f, whole = false;
+    unsigned from = MT_SAMPLE_BINS, upto = MT_SAMPLE_BINS;  // (none listed, all stay)
+    mt_u64 above_k = 0;                                     // logits above `from`
+    if constexpr (CUT) {
+        if (by_k || by_p) {
+            // lane t: bin t of the row, the sums up to it
+            constexpr unsigned EACH = LANES / MT_SAMPLE_BINS;
+            static_assert(EACH >= 1u && LANES % MT_SAMPLE_BINS == 0u, "a lane to a bin at the least");
+            mt_u64 number = 0, mass = 0;
+            const unsigned bin = t % MT_SAMPLE_BINS;
+            for (unsigned c = t / MT_SAMPLE_BINS; c < S; c += EACH) {
+                const float shift = first - grid.bin(mt_order_value((unsigned)(best_in[(size_t)row * S + c] >> 32)));
+                if (shift >= 0.f && shift <= (float)bin) {
+                    const mt_u64 word = bins_in[((size_t)row * S + c) * MT_SAMPLE_BINS + (bin - (unsigned)shift)];
+                    number += word >> MT_SAMPLE_COUNT_AT, mass += word & ((1ull << MT_SAMPLE_COUNT_AT) - 1ull);
+                }
+            }
+            if constexpr (EACH > 1u) {
+                mt_u64* other = lds + 2u * WAVES;
+                for (unsigned h = 1; h < EACH; ++h) {
+                    __syncthreads();
+                    if (t / MT_SAMPLE_BINS == h) other[2u * bin] = number, other[2u * bin + 1u] = mass;
+                    __syncthreads();
+                    if (t < MT_SAMPLE_BINS) number += other[2u * bin], mass += other[2u * bin + 1u];
+                }
+                if (t >= MT_SAMPLE_BINS) number = 0, mass = 0;
+            }
+            // weights of the bin in 2^-20 of the first bin's edge, as a whole number of 2^-40
+            mass = (mt_u64)((double)mass * exp(-0.0625 * (double)bin) * 1048576.0);
+            mt_u64 all_number, all_mass;
+            const mt_u64 n0 = mt_group_before<WAVES>(number, lds, all_number), m0 = mt_group_before<WAVES>(mass, lds, all_mass);
+            if (t == 0u) lds[WAVES] = MT_SAMPLE_BINS, lds[WAVES + 1u] = MT_SAMPLE_BINS, lds[WAVES + 2u] = 0, lds[WAVES + 3u] = 0;
+            __syncthreads();
+            const mt_u64 k = (mt_u64)asked.k;
+            if (by_k && n0 < k && k <= n0 + number) lds[WAVES] = bin, lds[WAVES + 2u] = n0, lds[WAVES + 3u] = n0 + number;
+            if (by_p) {
+                const mt_u64 wanted = asked.weight_asked(all_mass);
+                if (m0 < wanted && wanted <= m0 + mass) lds[WAVES + 1u] = bin, lds[WAVES + 4u] = number;
+            }
+            __syncthreads();
+            const unsigned k_bin = (unsigned)lds[WAVES], p_bin = (unsigned)lds[WAVES + 1u];
+            mt_u64 listed = 0;
+            if (k_bin == MT_SAMPLE_BINS) by_k = false;  // (what weighs anything stays)
+            if (by_k) {
+                from = by_p ? 0u : k_bin, upto = k_bin;
+                above_k = by_p ? 0 : lds[WAVES + 2u];
+                listed = lds[WAVES + 3u] - above_k;
+            } else if (by_p) {
+                from = upto = p_bin;
+                listed = lds[WAVES + 4u];
+                whole = p_bin == MT_SAMPLE_BINS;
+            }
+            whole = whole || listed > MT_SAMPLE_LIST || !(__builtin_fabsf(first) < 1048576.f);
+            __syncthreads();
+        }
+    }
+    if (whole && chunk != 0u) return;  // (the same in all workgroups of the row)
+    const bool cuts = from < MT_SAMPLE_BINS;
+    if (!whole) {
+        mt_u64 all = 0, above = 0, kept = 0;
+        unsigned marks = 0u;  // which of this lane's are listed
+#pragma unroll
+        for (unsigned e = 0; e < PER; ++e) {
+            if (i0 + e >= V) continue;
+            bool stays = true;
+            if (CUT && cuts) {
+                const float below = first - grid.bin(v[e]);
+                stays = below < (float)from;
+                if (!stays && below <= (float)upto) marks |= 1u << e;
+            }
+            if (stays || (by_p && !by_k)) {
+                const double w = weights.weight(v[e]);
+                const mt_u64 h = weights.whole(w);
+                all += h;
+                if (stays) above += h, kept += w < asked.least ? 0 : h;
+            }
+        }
+        mt_u64* mine = sums + ((size_t)row * S + chunk) * 4u;
+        const auto put = [](mt_u64* to, mt_u64 value) { __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        const auto get = [](const mt_u64* from_) {
+            return __hip_atomic_load(const_cast<mt_u64*>(from_), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        mt_u64 listed = 0;
+        if (CUT && cuts) {
+            mt_u64 at = mt_group_before<WAVES>(__builtin_popcount(marks), lds, listed);
+#pragma unroll
+            for (unsigned e = 0; e < PER; ++e)
+                if ((marks >> e) & 1u) {
+                    if (at < ROOM) put(list + ((size_t)row * S + chunk) * ROOM + at, ((mt_u64)mt_order_key(v[e]) << 32) | (i0 + e));
+                    ++at;
+                }
+        }
+        if (CUT && by_p && !by_k) all = mt_group_fold<WAVES>(all, lds, sum), above = mt_group_fold<WAVES>(above, lds, sum);
+        kept = mt_group_fold<WAVES>(kept, lds, sum);
+        if (t == 0u) put(mine, all), put(mine + 1, above), put(mine + 2, kept), put(mine + 3, listed);
+        if constexpr (S > 1u) {
+            __builtin_amdgcn_s_waitcnt(0);  // every lane's stores have reached memory
+            __syncthreads();
+            if (t == 0u) lds[0] = __hip_atomic_fetch_add(arrivals + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (lds[0] + 1u != S) return;
+        } else {
+            __builtin_amdgcn_s_waitcnt(0);
+        }
+        __syncthreads();
+
+        // The last workgroup of the row.  In LDS: what stays of each chunk, and where each
+        // chunk's part of the list begins.
+        mt_u64 *chunk_kept = lds + 2u * WAVES + 256u, *begins = chunk_kept + S;
+        mt_u64 row_all = 0, row_above = 0;
+        unsigned n = 0u;
+        for (unsigned c = 0; c < S; c += 64u) {  // (each wave for itself)
+            const bool live = c + mt_lane() < S;
+            const mt_u64* at = sums + ((size_t)row * S + c + mt_lane()) * 4u;
+            const mt_u64 part = live ? get(at + 3) : 0;
+            if (CUT && by_p && !by_k) {
+                row_all += mt_wave_fold(live ? get(at) : 0, sum);
+                row_above += mt_wave_fold(live ? get(at + 1) : 0, sum);
+            }
+            mt_u64 before = part;
+#pragma unroll
+            for (unsigned off = 1u; off < 64u; off *= 2u) {
+                const mt_u64 other = __shfl_up(before, off, 64);
+                if (mt_lane() >= off) before += other;
+            }
+            if (live && t < 64u) begins[c + mt_lane()] = n + before - part, chunk_kept[c + mt_lane()] = get(at + 2);
+            n += (unsigned)__shfl(before, 63, 64);
+        }
+        __syncthreads();
+        mt_cut_at cut{0u, 0xFFFFFFFFu};
+        if (CUT && cuts) {
+            // lane t: entries DEEP t .. of the list
+            mt_u64 entry[DEEP];
+            unsigned of = 0u;  // the chunk of an entry
+            const unsigned l0 = t * DEEP;
+            for (unsigned c = 1; c < S; ++c) of += begins[c] <= l0 ? 1u : 0u;
+            const auto chunk_of = [&](unsigned l, unsigned from_) {
+                while (from_ + 1u < S && begins[from_ + 1u] <= l) ++from_;
+                return from_;
+            };
+            unsigned c = of;
+#pragma unroll
+            for (unsigned d = 0; d < DEEP; ++d) {
+                entry[d] = 0;
+                if (l0 + d < n) {
+                    c = chunk_of(l0 + d, c);
+                    entry[d] = get(list + ((size_t)row * S + c) * ROOM + (l0 + d - begins[c]));
+                }
+            }
+            const auto each = [&](auto f) {
+#pragma unroll
+                for (unsigned d = 0; d < DEEP; ++d)
+                    if (l0 + d < n) f((unsigned)entry[d], mt_order_value((unsigned)(entry[d] >> 32)));
+            };
+            const auto nth = [&](unsigned key, mt_u64 number) {
+                unsigned hits = 0u;
+                each([&](unsigned, float y) { hits += mt_order_key(y) == key ? 1u : 0u; });
+                mt_u64 every, before = mt_group_before<WAVES>(hits, lds, every);
+                each([&](unsigned i, float y) {
+                    if (mt_order_key(y) == key && ++before == number) lds[WAVES] = i;
+                });
+                __syncthreads();
+                const unsigned found = (unsigned)lds[WAVES];
+                __syncthreads();
+                return found;
+            };
+            mt_u64 over, at;
+            if (by_k) {
+                const mt_u64 wanted = (mt_u64)asked.k - above_k;
+                cut.key = mt_find_cut<WAVES>(each, [](unsigned, float) { return (mt_u64)1; }, wanted, over, at, lds);
+                mt_cut_equals(cut, wanted, over, at, 1, nth);
+            }
+            if (by_p) {
+                const mt_cut_at by = cut;
+                const auto amount = [&](unsigned i, float y) { return by.stays(mt_order_key(y), i) ? weights.held(y) : (mt_u64)0; };
+                mt_u64 total = 0;
+                each([&](unsigned i, float y) { total += amount(i, y); });
+                total = mt_group_fold<WAVES>(total, lds, sum);
+                const mt_u64 wanted = asked.weight_asked(by_k ? total : row_all);
+                if (!by_k && !(row_above < wanted && wanted <= row_above + total)) {  // (next to a bin's edge)
+                    whole = true;
+                } else {
+                    cut.key = mt_find_cut<WAVES>(each, amount, wanted - row_above, over, at, lds);
+                    if (cut.key != by.key) cut.last = 0xFFFFFFFFu;
+                    mt_cut_equals(cut, wanted - row_above, over, at, weights.held(mt_order_value(cut.key)), nth);
+                }
+            }
+            each([&](unsigned i, float y) {
+                if (cut.stays(mt_order_key(y), i)) {
+                    const mt_u64 h = weights.kept(y, asked.least);
+                    if (h != 0) atomicAdd(chunk_kept + i / (PER * LANES), h);
+                }
+            });
+            __syncthreads();
+        }
+        if (!whole) {
+            // The chunk that the random number falls into, and the token in it.
+            mt_u64 total = 0;
+            for (unsigned c = 0; c < S; ++c) total += chunk_kept[c];
+            const mt_u64 target = asked.target(total);
+            mt_u64 before = 0;
+            unsigned in = 0u;
+            while (in + 1u < S && before + chunk_kept[in] <= target) before += chunk_kept[in], ++in;
+            const unsigned k0 = (in * LANES + t) * PER;
+            mt_sample_load<V, PER, CS>(x, k0, v);
+            mt_u64 w[PER], lane_all = 0, every;
+#pragma unroll
+            for (unsigned e = 0; e < PER; ++e) {
+                w[e] = k0 + e < V && cut.stays(mt_order_key(v[e]), k0 + e) ? weights.kept(v[e], asked.least) : 0;
+                lane_all += w[e];
+            }
+            before += mt_group_before<WAVES>(lane_all, lds, every);
+#pragma unroll
+            for (unsigned e = 0; e < PER; ++e) {
+                if (before <= target && target < before + w[e]) weights.answer(row, k0 + e, v[e], total, tokens, logprobs);
+                before += w[e];
+            }
+            return;
+        }
+    }
+    mt_sample_whole<V, SHIFT, WAVES, CS>(x, asked, weights, row, tokens, logprobs, lds);
 }

@@ -12,6 +12,7 @@ from metellus_amd.orchestrator.decoding import (
     Rotary,
     RotaryOp,
     SampleOp,
+    SampleScanOp,
 )
 from metellus_amd.orchestrator.graph import Graph, Vertex
 from metellus_amd.orchestrator.ir import (
@@ -61,6 +62,7 @@ __all__ = [
     "Rotary",
     "RotaryOp",
     "SampleOp",
+    "SampleScanOp",
     "Scalar",
     "ShapeOp",
     "Tensor",

@@ -8,7 +8,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 from metellus_amd.compute.elementwise.elementwise import TERNARY_EXPRESSIONS
-from metellus_amd.orchestrator.decoding import AdapterDownOp, AdapterUpOp, PageTablesOp, RotaryOp, SampleOp
+from metellus_amd.orchestrator.decoding import AdapterDownOp, AdapterUpOp, PageTablesOp, RotaryOp, SampleOp, SampleScanOp
 from metellus_amd.orchestrator.graph import Vertex
 from metellus_amd.orchestrator.ir import ElementwiseOp, MatmulOp, Op, ReductionOp, Scalar, ShapeOp, Tensor
 from metellus_amd.orchestrator.kernel_group import FusionStrategy
@@ -33,6 +33,7 @@ _SERVING = {
     RotaryOp: FusionStrategy.ROTARY,
     AdapterDownOp: FusionStrategy.ADAPTER_DOWN,
     AdapterUpOp: FusionStrategy.ADAPTER_UP,
+    SampleScanOp: FusionStrategy.SAMPLE_SCAN,
     SampleOp: FusionStrategy.SAMPLE,
 }
 

@@ -13,12 +13,16 @@ from metellus_amd.orchestrator.assembly.serving import _ceil, _group, _Signature
 from metellus_amd.orchestrator.decoding import (
     ADAPTER_DOWN_WAVES,
     ADAPTER_MANY_ROWS,
+    SAMPLE_BINS,
+    SAMPLE_LANES,
     AdapterDownOp,
     AdapterUpOp,
     PageTablesOp,
     Rotary,
     RotaryOp,
     SampleOp,
+    SampleScanOp,
+    sample_chunks,
 )
 from metellus_amd.orchestrator.ir import Tensor
 from metellus_amd.orchestrator.kernel_group import FusionStrategy, KernelGroup
@@ -29,6 +33,7 @@ DECODING = frozenset(
         FusionStrategy.ROTARY,
         FusionStrategy.ADAPTER_DOWN,
         FusionStrategy.ADAPTER_UP,
+        FusionStrategy.SAMPLE_SCAN,
         FusionStrategy.SAMPLE,
     }
 )
@@ -193,11 +198,45 @@ def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name:
 # sampling
 # ---------------------------------------------------------------------------
 
-SAMPLE_WAVES = 16
+SAMPLE_WAVES = SAMPLE_LANES // 64
+
+
+def _words(sig: _Signature, role: str, t: Tensor | None, *, out: bool = False) -> str:
+    """A buffer of 64-bit words."""
+    arg = sig.add(role, t, out=out)
+    return arg if t is None else f"({'' if out else 'const '}mt_u64*){arg}"
+
+
+def _assemble_sample_scan(decision: DecisionView, op: SampleScanOp, function_name: str | None) -> KernelGroup:
+    rows, cols = op.logits.shape
+    per, chunks = sample_chunks(rows, cols)
+    cuts = op.bins is not None
+    sig = _Signature()
+    args = (
+        sig.add("logits", op.logits),
+        sig.add("temperatures", op.temperatures),
+        sig.add("top_k", op.top_k),
+        sig.add("top_p", op.top_p),
+        _words(sig, "best", op.best, out=True),
+        _words(sig, "bins", op.bins, out=True),
+        f"(unsigned*){sig.add('arrivals', op.arrivals, out=True)}",
+        "(mt_u64*)mt_lds",
+    )
+    frag = ServingFragment(
+        "mt_sample_scan",
+        (cols, per, chunks, SAMPLE_WAVES, *_strides(op.logits), cuts),
+        args,
+        lds_bytes=8 * (SAMPLE_WAVES + (SAMPLE_BINS if cuts else 0)),
+        name="sample_scan",
+    )
+    return _group(decision, sig, frag, function_name or f"sample_scan_{op.name}", {}, (rows * chunks, 1, 1), SAMPLE_LANES,
+                  headers=(decoding_header(),))
 
 
 def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | None) -> KernelGroup:
     rows, cols = op.logits.shape
+    per, chunks = sample_chunks(rows, cols)
+    cuts = op.bins is not None
     sig = _Signature()
     args = (
         sig.add("logits", op.logits),
@@ -206,19 +245,25 @@ def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | 
         sig.add("top_k", op.top_k),
         sig.add("top_p", op.top_p),
         sig.add("min_p", op.min_p),
+        _words(sig, "best", op.best),
+        _words(sig, "bins", op.bins),
+        f"(unsigned*){sig.add('arrivals', op.arrivals, out=True)}",
+        _words(sig, "sums", op.sums, out=True),
+        _words(sig, "list", op.listed, out=True),
         sig.add("tokens", op.tokens, out=True),
         sig.add("logprobs", op.logprobs, out=True),
         "(mt_u64*)mt_lds",
     )
+    # A row of ones adds up in 63 bits, and what lies below the bins weighs nothing.
+    shift = min(44, 62 - (cols - 1).bit_length())
     frag = ServingFragment(
-        "mt_sample",
-        # (weights of 2^-shift, so that a row of ones adds up in 63 bits)
-        (cols, 62 - (cols - 1).bit_length(), SAMPLE_WAVES, *_strides(op.logits)),
+        "mt_sample_pick",
+        (cols, per, chunks, shift, SAMPLE_WAVES, *_strides(op.logits), cuts),
         args,
-        lds_bytes=8 * (2 * SAMPLE_WAVES + 256),
+        lds_bytes=8 * (2 * SAMPLE_WAVES + max(2 * SAMPLE_BINS, 256 + 2 * chunks)),
         name="sample",
     )
-    return _group(decision, sig, frag, function_name or f"sample_{op.tokens.name}", {}, (rows, 1, 1), 64 * SAMPLE_WAVES,
+    return _group(decision, sig, frag, function_name or f"sample_{op.tokens.name}", {}, (rows * chunks, 1, 1), SAMPLE_LANES,
                   headers=(decoding_header(),))
 
 
@@ -227,6 +272,7 @@ _ASSEMBLE = {
     RotaryOp: _assemble_rotary,
     AdapterDownOp: _assemble_adapter_down,
     AdapterUpOp: _assemble_adapter_up,
+    SampleScanOp: _assemble_sample_scan,
     SampleOp: _assemble_sample,
 }
 

@@ -23,13 +23,17 @@ import numpy as np
 from metellus_amd.compute.elementwise.elementwise import BroadcastSpec
 from metellus_amd.orchestrator.decoding import (
     ADAPTER_RANK_MAX,
+    SAMPLE_BINS,
     AdapterDownOp,
     AdapterUpOp,
     PageTablesOp,
     Rotary,
     RotaryOp,
     SampleOp,
+    SampleScanOp,
     adapter_splits,
+    sample_chunks,
+    sample_room,
 )
 from metellus_amd.orchestrator.ir import (
     ITEM_BYTES,
@@ -610,17 +614,44 @@ class Operations:
         tl, tu = self._lookup(logits), self._lookup(uniforms)
         given = {n: self._optional(v) for n, v in
                  (("temperatures", temperatures), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p))}
-        rows = tl.shape[:1] if tl.shape else (1,)
-        op = SampleOp(
-            tokens=self._fresh(out, rows, "int32"),
+        if len(tl.shape) != 2:
+            raise ValueError(f"sample logits must be 2D; got shape {tl.shape} ({tl.name!r})")
+        rows, cols = tl.shape
+        per, chunks = sample_chunks(rows, cols)
+        cuts = top_k is not None or top_p is not None
+
+        def made(part: str, width: int) -> Tensor:
+            return self._fresh(f"{out}.{part}", (rows * chunks, width), "int32")
+
+        scan = SampleScanOp(
+            best=made("best", 2),
+            arrivals=self._fresh(f"{out}.arrivals", (rows,), "int32"),
+            logits=tl,
+            name=out,
+            bins=made("bins", 2 * SAMPLE_BINS) if cuts else None,
+            **{n: t if cuts else None for n, t in given.items() if n != "min_p"},
+            after=self._owners(tl, *given.values()),
+        )
+        pick = SampleOp(
+            tokens=self._fresh(out, (rows,), "int32"),
             logits=tl,
             uniforms=tu,
-            logprobs=None if logprobs is None else self._fresh(logprobs, rows, "float32"),
+            best=scan.best,
+            arrivals=scan.arrivals,
+            bins=scan.bins,
+            sums=made("sums", 8),
+            listed=made("list", 2 * sample_room(per)) if cuts else None,
+            logprobs=None if logprobs is None else self._fresh(logprobs, (rows,), "float32"),
             after=self._owners(tl, tu, *given.values()),
             **given,
         )
-        self._emit_all(op)
-        return op.tokens
+        names = [t.name for t in (*scan.outs, *pick.outs)]
+        if len(set(names)) < len(names):
+            raise ValueError(f"output names must differ; got {names}")
+        self._emit_all(scan)
+        self._emit_all(pick)
+        self._scratch.update(t.name for t in (*scan.outs, pick.sums, pick.listed) if t is not None)
+        return pick.tokens
 
     # -- results -------------------------------------------------------------
 

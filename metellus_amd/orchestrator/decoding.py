@@ -8,7 +8,8 @@ than fp32):
 * ``RotaryOp``      queries and keys turned by their positions
 * ``AdapterDownOp``, ``AdapterUpOp``
                     low-rank adapters of many requests, added to a shared product
-* ``SampleOp``      tokens from logits and given random numbers
+* ``SampleScanOp``, ``SampleOp``
+                    tokens from logits and given random numbers
 
 ``Rotary`` describes a rotation: which elements of a head are pairs, and their
 angles.
@@ -28,7 +29,9 @@ from metellus_amd.orchestrator.serving import HEAD_DIM_MAX, _INT32_MAX, ServingO
 ROTARY_LAYOUTS = ("half", "interleaved")
 POSITIONS_MAX = _INT32_MAX - 1024  # of a table's row (its positions and a step's rows are int32)
 ADAPTER_RANK_MAX = 256
-VOCABULARY_MAX = 2**24
+VOCABULARY_MAX = 2**20
+SAMPLE_LANES = 1024
+SAMPLE_BINS, SAMPLE_LIST = 512, 8192  # of a row's chunk; logits that a row has listed at most
 
 # pi to 64 digits: 2 pi has to outlast a double's 53 bits twice
 _PI = Decimal("3.141592653589793238462643383279502884197169399375105820974944592")
@@ -303,6 +306,53 @@ class AdapterUpOp(ServingOp):
         return tuple(t for t in (self.base, self.down, self.b, self.ids, self.scales) if t is not None)
 
 
+def sample_chunks(rows: int, cols: int) -> tuple[int, int]:
+    """Neighbouring logits that a lane of SAMPLE_LANES takes, and the chunks of a row that
+    this makes: at most 64, and more of them where rows are few."""
+    per = 4
+    while per < 16 and (rows * -(-cols // (per * SAMPLE_LANES)) > 512 or cols > 64 * per * SAMPLE_LANES):
+        per *= 2
+    return per, -(-cols // (per * SAMPLE_LANES))
+
+
+def sample_room(per: int) -> int:
+    """Listed logits that a chunk has room for."""
+    return min(per * SAMPLE_LANES, SAMPLE_LIST)
+
+
+@dataclass(frozen=True)
+class SampleScanOp(ServingOp):
+    """The largest logit of each chunk (int64s, as two int32), and its bins for rows that
+    ``top_k`` or ``top_p`` cut; the rows' arrivals are cleared."""
+
+    best: Tensor
+    arrivals: Tensor
+    logits: Tensor
+    name: str  # of the operator's output
+    bins: Tensor | None = None
+    temperatures: Tensor | None = None
+    top_k: Tensor | None = None
+    top_p: Tensor | None = None
+    after: tuple[Tensor, ...] = ()
+
+    def __post_init__(self) -> None:
+        rows, cols = _rows("sample logits", self.logits, "float32")
+        if cols > VOCABULARY_MAX:
+            raise ValueError(f"sample logits: at most {VOCABULARY_MAX} columns; got shape {self.logits.shape}")
+        for label, t, dtype in (("temperatures", self.temperatures, "float32"), ("top_k", self.top_k, "int32"),
+                                ("top_p", self.top_p, "float32")):
+            if t is not None:
+                _list(f"sample {label}", t, dtype, rows)
+
+    @property
+    def outs(self) -> tuple[Tensor, ...]:
+        return tuple(t for t in (self.best, self.arrivals, self.bins) if t is not None)
+
+    @property
+    def reads(self) -> tuple[Tensor, ...]:
+        return tuple(t for t in (self.logits, self.temperatures, self.top_k, self.top_p) if t is not None)
+
+
 @dataclass(frozen=True)
 class SampleOp(ServingOp):
     """For a row x with temperature T: w_i = exp((x_i - max x) / T).  In the order of
@@ -314,6 +364,11 @@ class SampleOp(ServingOp):
     tokens: Tensor
     logits: Tensor
     uniforms: Tensor
+    best: Tensor
+    arrivals: Tensor
+    sums: Tensor
+    bins: Tensor | None = None
+    listed: Tensor | None = None
     logprobs: Tensor | None = None
     temperatures: Tensor | None = None
     top_k: Tensor | None = None
@@ -322,9 +377,7 @@ class SampleOp(ServingOp):
     after: tuple[Tensor, ...] = ()
 
     def __post_init__(self) -> None:
-        rows, cols = _rows("sample logits", self.logits, "float32")
-        if cols > VOCABULARY_MAX:
-            raise ValueError(f"sample logits: at most {VOCABULARY_MAX} columns; got shape {self.logits.shape}")
+        rows, _ = _rows("sample logits", self.logits, "float32")
         for label, t, dtype in (("uniforms", self.uniforms, "float32"), ("temperatures", self.temperatures, "float32"),
                                 ("top_k", self.top_k, "int32"), ("top_p", self.top_p, "float32"),
                                 ("min_p", self.min_p, "float32")):
@@ -333,10 +386,13 @@ class SampleOp(ServingOp):
 
     @property
     def outs(self) -> tuple[Tensor, ...]:
-        return tuple(t for t in (self.tokens, self.logprobs) if t is not None)
+        return tuple(t for t in (self.tokens, self.logprobs, self.sums, self.listed) if t is not None)
 
     @property
     def reads(self) -> tuple[Tensor, ...]:
         return tuple(
-            t for t in (self.logits, self.uniforms, self.temperatures, self.top_k, self.top_p, self.min_p) if t is not None
+            t
+            for t in (self.logits, self.uniforms, self.temperatures, self.top_k, self.top_p, self.min_p, self.best, self.bins,
+                      self.arrivals)
+            if t is not None
         )

@@ -40,6 +40,7 @@ class FusionStrategy(str, Enum):
     ROTARY = "rotary"
     ADAPTER_DOWN = "adapter_down"
     ADAPTER_UP = "adapter_up"
+    SAMPLE_SCAN = "sample_scan"
     SAMPLE = "sample"
 
     def __str__(self) -> str:

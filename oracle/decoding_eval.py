@@ -143,6 +143,10 @@ def sample_row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     return int(at), float(scaled[at] - np.log(upto[-1]))
 
 
+def _sample_scan(op, get):
+    return {t.name: np.zeros(t.shape, np.int32) for t in op.outs}  # the kernels' own
+
+
 def _sample(op, get):
     x = get(op.logits)
     asked = {}
@@ -151,7 +155,8 @@ def _sample(op, get):
         if t is not None:
             asked[name.rstrip("s") if name == "temperatures" else name] = get(t)
     found = [sample_row(x[r], get(op.uniforms)[r], **{n: v[r] for n, v in asked.items()}) for r in range(x.shape[0])]
-    made = {op.tokens.name: np.array([f[0] for f in found], np.int32)}
+    made = {t.name: np.zeros(t.shape, np.int32) for t in (op.sums, op.listed) if t is not None}  # the kernels' own
+    made[op.tokens.name] = np.array([f[0] for f in found], np.int32)
     if op.logprobs is not None:
         made[op.logprobs.name] = np.array([f[1] for f in found])
     return made
@@ -160,4 +165,4 @@ def _sample(op, get):
 def evaluate_decoding(op, get) -> dict:
     """``{output name: array}`` of one op; ``get(tensor)`` reads an input."""
     return {"PageTablesOp": _page_tables, "RotaryOp": _rotary, "AdapterDownOp": _adapter_down,
-            "AdapterUpOp": _adapter_up, "SampleOp": _sample}[type(op).__name__](op, get)
+            "AdapterUpOp": _adapter_up, "SampleScanOp": _sample_scan, "SampleOp": _sample}[type(op).__name__](op, get)

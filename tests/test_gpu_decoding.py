@@ -6,7 +6,7 @@ Tolerances follow from the kernels' roundings (u = 2^-24, half a step of fp32):
 * rotary: see ``_rotary_bound``.
 * adapters: see ``_adapter_bound``.
 * sample: tokens exact; a logprob is rounded once, and the sum of n weights held in
-  2^-s is off by n 2^-s of a sum that is 1 at the least (s = 62 - log2 n).
+  2^-s is off by n 2^-s of a sum that is 1 at the least (s = 62 - log2 n, 44 at the most).
 """
 
 from __future__ import annotations
@@ -317,7 +317,7 @@ def _sample_check(ops):
     env, ref = run(ops).env, evaluate(ops)
     np.testing.assert_array_equal(env["t"], ref["t"])
     n = ops.tensors["x"].shape[1]
-    _close(env["lp"], ref["lp"], 1.01 * U * np.abs(ref["lp"]) + n * 2.0 ** ((n - 1).bit_length() - 62) + 2.0**-149)
+    _close(env["lp"], ref["lp"], 1.01 * U * np.abs(ref["lp"]) + n * 2.0 ** -min(44, 62 - (n - 1).bit_length()) + 2.0**-149)
     return env["t"]
 
 
@@ -393,6 +393,29 @@ def test_sample_masked_rows(cols):
                   {"temperatures": np.inf}, {"temperatures": 1e-45}):
         t = _sample_check(_sample_ops(x, u, **asked))
         assert t[0] == t[2] == t[6] == -1 and t[3] == 4 and t[5] == 2
+
+
+@pytest.mark.parametrize("cols", [300, 30000])
+def test_sample_cut_between_weights(cols):
+    """p next to where a third of the logits, all equal, weigh as much as the rest: 32 bits
+    do not see on which side it is, 64 do."""
+    p = np.float32(0.5) + np.arange(-8, 9).astype(np.float32) * np.float32(2.0**-24)
+    x = np.full((17, cols), -np.log(2.0), np.float32)
+    x[:, : cols // 3] = 0.0
+    t = _sample_check(_sample_ops(x, np.full(17, 1 - 2.0**-24), top_p=p))
+    assert (t < cols // 3).any() and (t >= cols // 3).any()
+
+
+@pytest.mark.parametrize("rows, cols", [(1, 40000), (3, 70001), (2, 262144)])
+@pytest.mark.parametrize("scale", [0.1, 1.0, 30.0, 1e6])
+def test_sample_spreads_of_logits(rows, cols, scale):
+    """From rows that are next to even -- more in a bin than are listed -- to ones in which a
+    few logits have all the weight, or are past the bins' grid."""
+    rng = np.random.default_rng(cols)
+    x = scale * rng.standard_normal((rows, cols))
+    for asked in ({}, {"top_p": 0.6}, {"top_k": 30}, {"top_k": 20000}, {"top_k": 20000, "top_p": 0.3}, {"min_p": 0.4},
+                  {"top_k": 300, "top_p": 0.7, "min_p": 0.01}):
+        _sample_check(_sample_ops(x, rng.random(rows), **asked))
 
 
 def test_sample_of_strided_logits():
