@@ -741,16 +741,71 @@ MT_INLINE void mt_sample_load(const float* x, unsigned i0, float (&v)[PER]) {
     }
 }
 
-// What the kernels leave in memory: the largest of each chunk; its bins; the sums of its
-// weights; the listed logits; a row's arrivals.
-template <unsigned S, unsigned ROOM>
-struct mt_sample_parts {
-    mt_u64* best;        // [row][S]
-    mt_u64* bins;        // [row][S][MT_SAMPLE_BINS]
-    mt_u64* sums;        // [row][S][4]: all, above the cut, above it and kept, listed
-    mt_u64* list;        // [row][S][ROOM]: key and index
-    unsigned* arrivals;  // [row]
-};
+constexpr unsigned MT_SAMPLE_CLOSE = 256u;  // logits that are compared one by one
+
+// The cut of a list of n logits: an entry is a key and, below it, the index upside down, so
+// that larger is earlier; `amount`s, of which `asked` is at most the sum.  Up to 64 are
+// compared one by one; of more, those that fall into the cut's part of 1024 even parts of
+// the list's range of keys.  False where these are too many.
+template <unsigned WAVES, unsigned DEEP>
+MT_INLINE bool mt_list_cut(const mt_u64 (&entry)[DEEP], const mt_u64 (&amount)[DEEP], unsigned n, mt_u64 asked,
+                           mt_cut_at& cut, mt_u64* lds) {
+    constexpr unsigned LANES = 64u * WAVES;
+    mt_u64 *bins = lds + 2u * WAVES, *close = bins + LANES, *close_amount = close + MT_SAMPLE_CLOSE;
+    const unsigned t = threadIdx.x;
+    mt_u64 over = 0;
+    unsigned m = n;
+    if (n <= 64u) {
+        __syncthreads();
+        if (t < n) close[t] = entry[0], close_amount[t] = amount[0];
+    } else {
+        // the largest key, and the least upside down
+        mt_u64 span = 0;
+        const auto both = [](mt_u64 a, mt_u64 b) {
+            const mt_u64 low = 0xFFFFFFFFull, high = (a > b ? a : b) & ~low, x = a & low, y = b & low;
+            return high | (x > y ? x : y);
+        };
+#pragma unroll
+        for (unsigned d = 0; d < DEEP; ++d)
+            if (amount[d] != 0) span = both(span, (entry[d] & ~0xFFFFFFFFull) | (0xFFFFFFFFull - (entry[d] >> 32)));
+        span = mt_group_fold<WAVES>(span, lds, both);
+        const unsigned top = (unsigned)(span >> 32), range = top - (0xFFFFFFFFu - (unsigned)span);
+        const unsigned shift = range >= LANES ? 32u - __builtin_clz(range / LANES) : 0u;
+        bins[t] = 0;
+        if (t == 0u) lds[WAVES] = 0, lds[WAVES + 1u] = 0, lds[WAVES + 2u] = 0;
+        __syncthreads();
+#pragma unroll
+        for (unsigned d = 0; d < DEEP; ++d)
+            if (amount[d] != 0) atomicAdd(bins + ((top - (unsigned)(entry[d] >> 32)) >> shift), amount[d]);
+        __syncthreads();
+        mt_u64 all;
+        const mt_u64 mine = bins[t], before = mt_group_before<WAVES>(mine, lds, all);
+        if (before < asked && asked <= before + mine) lds[WAVES] = t, lds[WAVES + 1u] = before;
+        __syncthreads();
+        const unsigned bin = (unsigned)lds[WAVES];
+        over = lds[WAVES + 1u];
+#pragma unroll
+        for (unsigned d = 0; d < DEEP; ++d)
+            if (amount[d] != 0 && (top - (unsigned)(entry[d] >> 32)) >> shift == bin) {
+                const unsigned at = (unsigned)atomicAdd(lds + WAVES + 2u, 1ull);
+                if (at < MT_SAMPLE_CLOSE) close[at] = entry[d], close_amount[at] = amount[d];
+            }
+        __syncthreads();
+        m = (unsigned)lds[WAVES + 2u];
+        if (m > MT_SAMPLE_CLOSE) return false;  // (the same in all lanes)
+    }
+    __syncthreads();
+    if (t < m) {
+        const mt_u64 own = close[t], weighs = close_amount[t];
+        mt_u64 before = over;
+#pragma unroll 4
+        for (unsigned j = 0; j < m; ++j) before += close[j] > own ? close_amount[j] : 0;
+        if (before < asked && asked <= before + weighs) lds[WAVES + 3u] = own;
+    }
+    __syncthreads();
+    cut.key = (unsigned)(lds[WAVES + 3u] >> 32), cut.last = 0xFFFFFFFFu - (unsigned)lds[WAVES + 3u];
+    return true;
+}
 
 template <unsigned V, unsigned PER, unsigned S, unsigned WAVES, unsigned RS, unsigned CS, bool CUT>
 MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, const int* top_k, const float* top_p,
@@ -905,7 +960,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
 #pragma unroll
             for (unsigned e = 0; e < PER; ++e)
                 if ((marks >> e) & 1u) {
-                    if (at < ROOM) put(list + ((size_t)row * S + chunk) * ROOM + at, ((mt_u64)mt_order_key(v[e]) << 32) | (i0 + e));
+                    if (at < ROOM) put(list + ((size_t)row * S + chunk) * ROOM + at, mt_best(i0 + e, v[e]));
                     ++at;
                 }
         }
@@ -925,7 +980,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
 
         // The last workgroup of the row.  In LDS: what stays of each chunk, and where each
         // chunk's part of the list begins.
-        mt_u64 *chunk_kept = lds + 2u * WAVES + 256u, *begins = chunk_kept + S;
+        mt_u64 *chunk_kept = lds + 2u * WAVES + LANES + 2u * MT_SAMPLE_CLOSE, *begins = chunk_kept + S;
         mt_u64 row_all = 0, row_above = 0;
         unsigned n = 0u;
         for (unsigned c = 0; c < S; c += 64u) {  // (each wave for itself)
@@ -948,68 +1003,48 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
         __syncthreads();
         mt_cut_at cut{0u, 0xFFFFFFFFu};
         if (CUT && cuts) {
-            // lane t: entries DEEP t .. of the list
-            mt_u64 entry[DEEP];
-            unsigned of = 0u;  // the chunk of an entry
-            const unsigned l0 = t * DEEP;
-            for (unsigned c = 1; c < S; ++c) of += begins[c] <= l0 ? 1u : 0u;
-            const auto chunk_of = [&](unsigned l, unsigned from_) {
-                while (from_ + 1u < S && begins[from_ + 1u] <= l) ++from_;
-                return from_;
-            };
-            unsigned c = of;
+            // lane t: entries t, t + LANES .. of the list, and what they count or weigh
+            mt_u64 entry[DEEP], amount[DEEP];
 #pragma unroll
             for (unsigned d = 0; d < DEEP; ++d) {
-                entry[d] = 0;
-                if (l0 + d < n) {
-                    c = chunk_of(l0 + d, c);
-                    entry[d] = get(list + ((size_t)row * S + c) * ROOM + (l0 + d - begins[c]));
+                const unsigned l = t + d * LANES;
+                entry[d] = 0, amount[d] = 0;
+                if (l < n) {
+                    unsigned lo = 0u, hi = S;
+                    while (hi - lo > 1u) {
+                        const unsigned mid = (lo + hi) / 2u;
+                        if (begins[mid] <= l) lo = mid;
+                        else hi = mid;
+                    }
+                    entry[d] = get(list + ((size_t)row * S + lo) * ROOM + (l - (unsigned)begins[lo]));
+                    amount[d] = 1;
                 }
             }
-            const auto each = [&](auto f) {
+            const auto stays = [&](mt_u64 one) { return cut.stays((unsigned)(one >> 32), 0xFFFFFFFFu - (unsigned)one); };
+            if (by_k) whole = !mt_list_cut<WAVES>(entry, amount, n, (mt_u64)asked.k - above_k, cut, lds);
+            mt_u64 total = 0;
+            unsigned light = 0u;  // those below min_p
 #pragma unroll
-                for (unsigned d = 0; d < DEEP; ++d)
-                    if (l0 + d < n) f((unsigned)entry[d], mt_order_value((unsigned)(entry[d] >> 32)));
-            };
-            const auto nth = [&](unsigned key, mt_u64 number) {
-                unsigned hits = 0u;
-                each([&](unsigned, float y) { hits += mt_order_key(y) == key ? 1u : 0u; });
-                mt_u64 every, before = mt_group_before<WAVES>(hits, lds, every);
-                each([&](unsigned i, float y) {
-                    if (mt_order_key(y) == key && ++before == number) lds[WAVES] = i;
-                });
-                __syncthreads();
-                const unsigned found = (unsigned)lds[WAVES];
-                __syncthreads();
-                return found;
-            };
-            mt_u64 over, at;
-            if (by_k) {
-                const mt_u64 wanted = (mt_u64)asked.k - above_k;
-                cut.key = mt_find_cut<WAVES>(each, [](unsigned, float) { return (mt_u64)1; }, wanted, over, at, lds);
-                mt_cut_equals(cut, wanted, over, at, 1, nth);
+            for (unsigned d = 0; d < DEEP; ++d) {
+                if (amount[d] != 0) {
+                    const double w = weights.weight(mt_order_value((unsigned)(entry[d] >> 32)));
+                    amount[d] = stays(entry[d]) ? weights.whole(w) : 0;
+                    total += amount[d];
+                    if (w < asked.least) light |= 1u << d;
+                }
             }
-            if (by_p) {
-                const mt_cut_at by = cut;
-                const auto amount = [&](unsigned i, float y) { return by.stays(mt_order_key(y), i) ? weights.held(y) : (mt_u64)0; };
-                mt_u64 total = 0;
-                each([&](unsigned i, float y) { total += amount(i, y); });
+            if (by_p && !whole) {
                 total = mt_group_fold<WAVES>(total, lds, sum);
                 const mt_u64 wanted = asked.weight_asked(by_k ? total : row_all);
-                if (!by_k && !(row_above < wanted && wanted <= row_above + total)) {  // (next to a bin's edge)
-                    whole = true;
-                } else {
-                    cut.key = mt_find_cut<WAVES>(each, amount, wanted - row_above, over, at, lds);
-                    if (cut.key != by.key) cut.last = 0xFFFFFFFFu;
-                    mt_cut_equals(cut, wanted - row_above, over, at, weights.held(mt_order_value(cut.key)), nth);
-                }
+                if (by_k || (row_above < wanted && wanted <= row_above + total))
+                    whole = !mt_list_cut<WAVES>(entry, amount, n, wanted - row_above, cut, lds);
+                else
+                    whole = true;  // (next to a bin's edge)
             }
-            each([&](unsigned i, float y) {
-                if (cut.stays(mt_order_key(y), i)) {
-                    const mt_u64 h = weights.kept(y, asked.least);
-                    if (h != 0) atomicAdd(chunk_kept + i / (PER * LANES), h);
-                }
-            });
+#pragma unroll
+            for (unsigned d = 0; d < DEEP; ++d)
+                if (amount[d] != 0 && !((light >> d) & 1u) && stays(entry[d]))
+                    atomicAdd(chunk_kept + (0xFFFFFFFFu - (unsigned)entry[d]) / (PER * LANES), amount[d]);
             __syncthreads();
         }
         if (!whole) {

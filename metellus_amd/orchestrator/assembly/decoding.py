@@ -14,6 +14,7 @@ from metellus_amd.orchestrator.decoding import (
     ADAPTER_DOWN_WAVES,
     ADAPTER_MANY_ROWS,
     SAMPLE_BINS,
+    SAMPLE_CLOSE,
     SAMPLE_LANES,
     AdapterDownOp,
     AdapterUpOp,
@@ -260,7 +261,7 @@ def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | 
         "mt_sample_pick",
         (cols, per, chunks, shift, SAMPLE_WAVES, *_strides(op.logits), cuts),
         args,
-        lds_bytes=8 * (2 * SAMPLE_WAVES + max(2 * SAMPLE_BINS, 256 + 2 * chunks)),
+        lds_bytes=8 * (2 * SAMPLE_WAVES + SAMPLE_LANES + 2 * SAMPLE_CLOSE + 2 * chunks),
         name="sample",
     )
     return _group(decision, sig, frag, function_name or f"sample_{op.tokens.name}", {}, (rows * chunks, 1, 1), SAMPLE_LANES,

@@ -32,6 +32,7 @@ ADAPTER_RANK_MAX = 256
 VOCABULARY_MAX = 2**20
 SAMPLE_LANES = 1024
 SAMPLE_BINS, SAMPLE_LIST = 512, 8192  # of a row's chunk; logits that a row has listed at most
+SAMPLE_CLOSE = 256  # of those, that are compared one by one
 
 # pi to 64 digits: 2 pi has to outlast a double's 53 bits twice
 _PI = Decimal("3.141592653589793238462643383279502884197169399375105820974944592")
