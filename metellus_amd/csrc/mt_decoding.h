@@ -492,15 +492,37 @@ MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
     return before + sum - v;
 }
 
+// e^z for z <= 0, right to about 2^-51 of itself; 0 below -700.  z = n log 2 + r, and the
+// series of e^r: for |r| up to log(2) / 2 its 14th term is under 2^-57.
+MT_INLINE double mt_exp_below(double z) {
+    const double n = __builtin_rint(z * 0x1.71547652b82fep+0);  // 1 / log 2
+    const double r = __builtin_fma(n, -0x1.abc9e3b39803fp-56, __builtin_fma(n, -0x1.62e42fefa39efp-1, z));  // (log 2 in two parts)
+    double e = 1.0 / 6227020800.0;
+    e = __builtin_fma(e, r, 1.0 / 479001600.0);
+    e = __builtin_fma(e, r, 1.0 / 39916800.0);
+    e = __builtin_fma(e, r, 1.0 / 3628800.0);
+    e = __builtin_fma(e, r, 1.0 / 362880.0);
+    e = __builtin_fma(e, r, 1.0 / 40320.0);
+    e = __builtin_fma(e, r, 1.0 / 5040.0);
+    e = __builtin_fma(e, r, 1.0 / 720.0);
+    e = __builtin_fma(e, r, 1.0 / 120.0);
+    e = __builtin_fma(e, r, 1.0 / 24.0);
+    e = __builtin_fma(e, r, 1.0 / 6.0);
+    e = __builtin_fma(e, r, 0.5);
+    e = __builtin_fma(e, r, 1.0);
+    e = __builtin_fma(e, r, 1.0);
+    return z < -700.0 ? 0.0 : __builtin_ldexp(e, (int)n);
+}
+
 // The weights of a row.
 template <unsigned SHIFT>
 struct mt_weights {
     float top;
-    double by;  // the temperature
-    MT_INLINE double scaled(float x) const { return ((double)x - (double)top) / by; }
+    double by;  // one over the temperature
+    MT_INLINE double scaled(float x) const { return ((double)x - (double)top) * by; }
     MT_INLINE double weight(float x) const {
         if (x == top) return 1.0;
-        return x == -INFINITY || top == INFINITY ? 0.0 : exp(scaled(x));  // (whatever the temperature)
+        return x == -INFINITY || top == INFINITY ? 0.0 : mt_exp_below(scaled(x));  // (whatever the temperature)
     }
     MT_INLINE static mt_u64 whole(double w) { return (mt_u64)__builtin_rint(w * (double)(1ull << SHIFT)); }
     MT_INLINE mt_u64 held(float x) const { return whole(weight(x)); }
@@ -509,10 +531,10 @@ struct mt_weights {
         const double w = weight(x);
         return w < least ? 0 : whole(w);
     }
-    MT_INLINE void answer(unsigned row, unsigned i, float x, mt_u64 total, int* tokens, float* logprobs) const {
+    MT_INLINE static double log_of(mt_u64 total) { return log((double)total * (1.0 / (double)(1ull << SHIFT))); }
+    MT_INLINE void answer(unsigned row, unsigned i, float x, double log_total, int* tokens, float* logprobs) const {
         tokens[row] = (int)i;
-        if (logprobs != nullptr)
-            logprobs[row] = (float)((x == top ? 0.0 : scaled(x)) - log((double)total / (double)(1ull << SHIFT)));
+        if (logprobs != nullptr) logprobs[row] = (float)((x == top ? 0.0 : scaled(x)) - log_total);
     }
 };
 
@@ -621,11 +643,18 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
     const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
     const auto each = [&](auto f) {
 #pragma unroll 1
-        for (unsigned c = 4u * t; c < V; c += STEP) {
-            const mt_f32x4 v = mt_row4<V, CS>(x, c);
+        for (unsigned c0 = 4u * t; c0 < V; c0 += 4u * STEP) {
+            mt_f32x4 v[4];
 #pragma unroll
-            for (unsigned j = 0; j < 4u; ++j)
-                if (c + j < V) f(c + j, v[j]);
+            for (unsigned q = 0; q < 4u; ++q) {
+                v[q] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                if (c0 + q * STEP < V) v[q] = mt_row4<V, CS>(x, c0 + q * STEP);
+            }
+#pragma unroll
+            for (unsigned q = 0; q < 4u; ++q)
+#pragma unroll
+                for (unsigned j = 0; j < 4u; ++j)
+                    if (c0 + q * STEP + j < V) f(c0 + q * STEP + j, v[q][j]);
         }
     };
     // The index of the n-th of those equal to `key`, of which there are more.
@@ -677,6 +706,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
     each([&](unsigned i, float v) { total += amount(i, v); });
     total = mt_group_fold<WAVES>(total, lds, sum);
     const mt_u64 target = asked.target(total);
+    const double log_total = weights.log_of(total);
     mt_u64 seen = 0;
 #pragma unroll 1
     for (unsigned c0 = 0; c0 < V; c0 += STEP) {
@@ -690,7 +720,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
         mt_u64 all, before = seen + mt_group_before<WAVES>(w[0] + w[1] + w[2] + w[3], lds, all);
 #pragma unroll
         for (unsigned j = 0; j < 4u; ++j) {
-            if (before <= target && target < before + w[j]) weights.answer(row, c + j, v[j], total, tokens, logprobs);
+            if (before <= target && target < before + w[j]) weights.answer(row, c + j, v[j], log_total, tokens, logprobs);
             before += w[j];
         }
         seen += all;
@@ -699,8 +729,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 }
 
 // ---------------------------------------------------------------------------
-// Two kernels draw from rows of which S chunks are in as many workgroups, PER neighbours to
-// a lane.
+// Two kernels draw from rows of which S chunks are in as many workgroups.
 //
 // The first finds a chunk's largest and, for rows that k or p cut, counts its logits by how
 // far below it they are: 512 bins of a sixteenth of the temperature, on a grid that all
@@ -710,16 +739,22 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // The second adds the chunks' bins up, in every workgroup for itself, and so knows in which
 // bin the cut is.  What lies above it stays, and is only added up; what lies in it -- or,
 // where k and p both cut, everything from k's bin on, for p's cut depends on where k's is --
-// is listed, in the order of the indexes.  The last of a row's workgroups to arrive finds
-// the cut in the list, adds what stays to the sums of the chunks, and looks through the
-// chunk that the random number falls into.
+// is listed, in any order.  The last of a row's workgroups to arrive finds the cut in the
+// list, adds what stays to the sums of the chunks, and looks through the chunk that the
+// random number falls into.
 // All of it counts with the same whole numbers as one workgroup alone, and what the bins
-// say about weights, in 32 bits, is checked; rows that do not fit -- a list beyond LIST, a
-// bin that p's cut is next to, logits so large that a bin is none of theirs -- are drawn
-// from by one workgroup.
+// say about weights, in 32 bits, is checked; rows that do not fit -- a list beyond LIST,
+// hundreds of logits that are next to equal at the cut, a cut by p next to a bin's edge,
+// logits so large that the grid has no bin for them -- are drawn from by one workgroup.
+//
+// Workgroups are of four waves: the steps from the bins to the token follow each other, all
+// waves take them, and with more of them a compute unit takes turns.
 // ---------------------------------------------------------------------------
 
+constexpr unsigned MT_SAMPLE_WAVES = 4u, MT_SAMPLE_LANES = 256u;
 constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 8192u;
+constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
+constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
 constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
 
 // The bin of x on the grid of a temperature.
@@ -729,144 +764,178 @@ struct mt_grid {
     MT_INLINE float bin(float x) const { return __builtin_floorf(x * by); }
 };
 
-// This lane's PER logits of a chunk; -inf behind the row's end.
-template <unsigned V, unsigned PER, unsigned CS>
-MT_INLINE void mt_sample_load(const float* x, unsigned i0, float (&v)[PER]) {
-#pragma unroll
-    for (unsigned q = 0; q < PER; q += 4u) {
-        mt_f32x4 four = {0.f, 0.f, 0.f, 0.f};
-        if (i0 + q < V) four = mt_row4<V, CS>(x, i0 + q);
-#pragma unroll
-        for (unsigned j = 0; j < 4u; ++j) v[q + j] = i0 + q + j < V ? four[j] : -INFINITY;
+// Calls f(index, x) for this lane's logits of the chunk from i0 on, 16 of them loaded at a
+// time; those of short chunks stay in registers for the next call.
+template <unsigned V, unsigned CHUNK, unsigned CS>
+struct mt_sample_chunk {
+    static constexpr unsigned QUADS = CHUNK / (4u * MT_SAMPLE_LANES);
+    static constexpr bool KEEP = QUADS <= 16u;
+    mt_f32x4 kept[KEEP ? QUADS : 4u];
+    const float* x;
+    unsigned i0;
+    MT_INLINE unsigned index(unsigned q) const { return i0 + 4u * (threadIdx.x + MT_SAMPLE_LANES * q); }
+    MT_INLINE mt_f32x4 load(unsigned q) const {
+        mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (index(q) < V) v = mt_row4<V, CS>(x, index(q));
+        return v;
     }
-}
-
-constexpr unsigned MT_SAMPLE_CLOSE = 256u;  // logits that are compared one by one
-
-// The cut of a list of n logits: an entry is a key and, below it, the index upside down, so
-// that larger is earlier; `amount`s, of which `asked` is at most the sum.  Up to 64 are
-// compared one by one; of more, those that fall into the cut's part of 1024 even parts of
-// the list's range of keys.  False where these are too many.
-template <unsigned WAVES, unsigned DEEP>
-MT_INLINE bool mt_list_cut(const mt_u64 (&entry)[DEEP], const mt_u64 (&amount)[DEEP], unsigned n, mt_u64 asked,
-                           mt_cut_at& cut, mt_u64* lds) {
-    constexpr unsigned LANES = 64u * WAVES;
-    mt_u64 *bins = lds + 2u * WAVES, *close = bins + LANES, *close_amount = close + MT_SAMPLE_CLOSE;
-    const unsigned t = threadIdx.x;
-    mt_u64 over = 0;
-    unsigned m = n;
-    if (n <= 64u) {
-        __syncthreads();
-        if (t < n) close[t] = entry[0], close_amount[t] = amount[0];
-    } else {
-        // the largest key, and the least upside down
-        mt_u64 span = 0;
-        const auto both = [](mt_u64 a, mt_u64 b) {
-            const mt_u64 low = 0xFFFFFFFFull, high = (a > b ? a : b) & ~low, x = a & low, y = b & low;
-            return high | (x > y ? x : y);
-        };
+    MT_INLINE mt_sample_chunk(const float* x_, unsigned i0_) : x(x_), i0(i0_) {
+        if constexpr (KEEP) {
 #pragma unroll
-        for (unsigned d = 0; d < DEEP; ++d)
-            if (amount[d] != 0) span = both(span, (entry[d] & ~0xFFFFFFFFull) | (0xFFFFFFFFull - (entry[d] >> 32)));
-        span = mt_group_fold<WAVES>(span, lds, both);
-        const unsigned top = (unsigned)(span >> 32), range = top - (0xFFFFFFFFu - (unsigned)span);
-        const unsigned shift = range >= LANES ? 32u - __builtin_clz(range / LANES) : 0u;
-        bins[t] = 0;
-        if (t == 0u) lds[WAVES] = 0, lds[WAVES + 1u] = 0, lds[WAVES + 2u] = 0;
-        __syncthreads();
+            for (unsigned q = 0; q < QUADS; ++q) kept[q] = load(q);
+        }
+    }
+    template <typename F>
+    MT_INLINE void each(F f) {
+        if constexpr (KEEP) {
 #pragma unroll
-        for (unsigned d = 0; d < DEEP; ++d)
-            if (amount[d] != 0) atomicAdd(bins + ((top - (unsigned)(entry[d] >> 32)) >> shift), amount[d]);
-        __syncthreads();
-        mt_u64 all;
-        const mt_u64 mine = bins[t], before = mt_group_before<WAVES>(mine, lds, all);
-        if (before < asked && asked <= before + mine) lds[WAVES] = t, lds[WAVES + 1u] = before;
-        __syncthreads();
-        const unsigned bin = (unsigned)lds[WAVES];
-        over = lds[WAVES + 1u];
+            for (unsigned q = 0; q < QUADS; ++q)
 #pragma unroll
-        for (unsigned d = 0; d < DEEP; ++d)
-            if (amount[d] != 0 && (top - (unsigned)(entry[d] >> 32)) >> shift == bin) {
-                const unsigned at = (unsigned)atomicAdd(lds + WAVES + 2u, 1ull);
-                if (at < MT_SAMPLE_CLOSE) close[at] = entry[d], close_amount[at] = amount[d];
+                for (unsigned j = 0; j < 4u; ++j)
+                    if (index(q) + j < V) f(index(q) + j, kept[q][j]);
+        } else {
+#pragma unroll 1
+            for (unsigned q0 = 0; q0 < QUADS; q0 += 4u) {
+#pragma unroll
+                for (unsigned q = 0; q < 4u; ++q) kept[q] = load(q0 + q);
+#pragma unroll
+                for (unsigned q = 0; q < 4u; ++q)
+#pragma unroll
+                    for (unsigned j = 0; j < 4u; ++j)
+                        if (index(q0 + q) + j < V) f(index(q0 + q) + j, kept[q][j]);
             }
-        __syncthreads();
-        m = (unsigned)lds[WAVES + 2u];
-        if (m > MT_SAMPLE_CLOSE) return false;  // (the same in all lanes)
+        }
     }
-    __syncthreads();
-    if (t < m) {
-        const mt_u64 own = close[t], weighs = close_amount[t];
-        mt_u64 before = over;
-#pragma unroll 4
-        for (unsigned j = 0; j < m; ++j) before += close[j] > own ? close_amount[j] : 0;
-        if (before < asked && asked <= before + weighs) lds[WAVES + 3u] = own;
-    }
-    __syncthreads();
-    cut.key = (unsigned)(lds[WAVES + 3u] >> 32), cut.last = 0xFFFFFFFFu - (unsigned)lds[WAVES + 3u];
-    return true;
-}
+};
 
-template <unsigned V, unsigned PER, unsigned S, unsigned WAVES, unsigned RS, unsigned CS, bool CUT>
+// best: [row][S]; bins: [row][S][MT_SAMPLE_BINS]; counts: [row][2], the row's arrivals and the
+// length of its list.
+template <unsigned V, unsigned CHUNK, unsigned S, unsigned RS, unsigned CS, bool CUT>
 MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, const int* top_k, const float* top_p,
-                              mt_u64* best_out, mt_u64* bins_out, unsigned* arrivals, mt_u64* lds) {
-    constexpr unsigned LANES = 64u * WAVES;
-    const unsigned row = blockIdx.x / S, chunk = blockIdx.x % S, t = threadIdx.x, i0 = (chunk * LANES + t) * PER;
-    if (chunk == 0u && t == 0u) arrivals[row] = 0u;
-    float v[PER];
-    mt_sample_load<V, PER, CS>(logits + (size_t)row * RS, i0, v);
+                              mt_u64* best_out, mt_u64* bins_out, unsigned* counts, mt_u64* lds) {
+    constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES;
+    const unsigned row = blockIdx.x / S, part = blockIdx.x % S, t = threadIdx.x;
+    if (part == 0u && t < 2u) counts[2u * row + t] = 0u;
+    mt_sample_chunk<V, CHUNK, CS> chunk(logits + (size_t)row * RS, part * CHUNK);
     mt_u64* bins = lds + WAVES;
     if (CUT)
         for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins[b] = 0;
     mt_u64 best = 0;
-#pragma unroll
-    for (unsigned e = 0; e < PER; ++e)
-        if (i0 + e < V) {
-            const mt_u64 found = mt_best(i0 + e, v[e]);
-            best = found > best ? found : best;
-        }
+    chunk.each([&](unsigned i, float x) {
+        const mt_u64 found = mt_best(i, x);
+        best = found > best ? found : best;
+    });
     best = mt_group_fold<WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
-    if (t == 0u) best_out[(size_t)row * S + chunk] = best;
+    if (t == 0u) best_out[(size_t)row * S + part] = best;
     if constexpr (CUT) {
         const float temperature = temperatures != nullptr ? temperatures[row] : 1.f;
         const bool by_p = top_p != nullptr && top_p[row] < 1.f, by_k = top_k != nullptr && top_k[row] > 0;
         if (!(temperature > 0.f) || !(by_p || by_k)) return;
         const mt_grid grid(temperature);
         const float first = grid.bin(mt_order_value((unsigned)(best >> 32)));
-#pragma unroll
-        for (unsigned e = 0; e < PER; ++e) {
-            const float f = grid.bin(v[e]), below = first - f;
-            if (i0 + e < V && below >= 0.f && below < (float)MT_SAMPLE_BINS) {
+        chunk.each([&](unsigned, float x) {
+            const float f = grid.bin(x), below = first - f;
+            if (below >= 0.f && below < (float)MT_SAMPLE_BINS) {
                 mt_u64 word = 1ull << MT_SAMPLE_COUNT_AT;
-                if (by_p) word += (mt_u64)(__builtin_amdgcn_exp2f((v[e] * grid.by - f) * (1.44269504f / 16.f)) * 1048576.f);
+                if (by_p) word += (unsigned)(__builtin_amdgcn_exp2f((x * grid.by - f) * (1.44269504f / 16.f)) * 1048576.f);
                 atomicAdd(bins + (unsigned)below, word);
             }
-        }
+        });
         __syncthreads();
-        for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins_out[((size_t)row * S + chunk) * MT_SAMPLE_BINS + b] = bins[b];
+        for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins_out[((size_t)row * S + part) * MT_SAMPLE_BINS + b] = bins[b];
     }
 }
 
-template <unsigned V, unsigned PER, unsigned S, unsigned SHIFT, unsigned WAVES, unsigned RS, unsigned CS, bool CUT>
+// The cut of a list: an entry is a key and, below it, the index upside down, so that larger
+// is earlier.  Where amount(entry), added up from the largest on, first reaches `asked`.  Up
+// to 64 are compared one by one; of more, those in the cut's part of the list's range, whose
+// parts place(entry) numbers from the largest on.  False where these are too many, or the
+// amounts less than asked.  `lds`: results, MT_SAMPLE_PARTS and two times MT_SAMPLE_CLOSE words.
+template <typename AMOUNT, typename PLACE>
+MT_INLINE bool mt_list_cut(const mt_u64* list, unsigned n, AMOUNT amount, PLACE place, mt_u64 asked, mt_cut_at& cut,
+                           mt_u64* lds) {
+    constexpr unsigned WAVES = MT_SAMPLE_WAVES, LANES = MT_SAMPLE_LANES, EACH = MT_SAMPLE_PARTS / LANES;
+    mt_u64 *found = lds + WAVES, *parts = found + 4u, *close = parts + MT_SAMPLE_PARTS, *weighs = close + MT_SAMPLE_CLOSE;
+    const unsigned t = threadIdx.x;
+    mt_u64 over = 0;
+    unsigned m = n;
+    __syncthreads();
+    if (t < 4u) found[t] = 0;
+    if (n <= 64u) {
+        if (t < n) close[t] = list[t], weighs[t] = amount(list[t]);
+    } else {
+        for (unsigned b = t; b < MT_SAMPLE_PARTS; b += LANES) parts[b] = 0;
+        __syncthreads();
+        for (unsigned l = t; l < n; l += LANES) {
+            const mt_u64 w = amount(list[l]);
+            if (w != 0) atomicAdd(parts + place(list[l]), w);
+        }
+        __syncthreads();
+        mt_u64 mine[EACH], sum = 0, all;
+#pragma unroll
+        for (unsigned b = 0; b < EACH; ++b) mine[b] = parts[t * EACH + b], sum += mine[b];
+        mt_u64 before = mt_group_before<WAVES>(sum, lds, all);
+        if (all < asked) return false;  // (the same in all lanes)
+#pragma unroll
+        for (unsigned b = 0; b < EACH; ++b) {
+            if (before < asked && asked <= before + mine[b]) found[0] = t * EACH + b, found[1] = before;
+            before += mine[b];
+        }
+        __syncthreads();
+        const unsigned at = (unsigned)found[0];
+        over = found[1];
+        for (unsigned l = t; l < n; l += LANES)
+            if (place(list[l]) == at) {
+                const unsigned to = (unsigned)atomicAdd(found + 2, 1ull);
+                if (to < MT_SAMPLE_CLOSE) close[to] = list[l], weighs[to] = amount(list[l]);
+            }
+        __syncthreads();
+        m = (unsigned)found[2];
+        if (m > MT_SAMPLE_CLOSE) return false;
+    }
+    __syncthreads();
+    if (t < m) {
+        const mt_u64 own = close[t], weight = weighs[t];
+        mt_u64 before = over;
+#pragma unroll 4
+        for (unsigned j = 0; j < m; ++j) before += close[j] > own ? weighs[j] : 0;
+        if (before < asked && asked <= before + weight) found[3] = own;
+    }
+    __syncthreads();
+    cut.key = (unsigned)(found[3] >> 32), cut.last = 0xFFFFFFFFu - (unsigned)found[3];
+    return found[3] != 0;
+}
+
+// sums: [row][S][3], all weights, those above the cut, and those of them that min_p leaves;
+// list: [row][MT_SAMPLE_LIST].
+template <unsigned V, unsigned CHUNK, unsigned S, unsigned SHIFT, unsigned RS, unsigned CS, bool CUT>
 MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const float* temperatures, const int* top_k,
                               const float* top_p, const float* min_p, const mt_u64* best_in, const mt_u64* bins_in,
-                              unsigned* arrivals, mt_u64* sums, mt_u64* list, int* tokens, float* logprobs, mt_u64* lds) {
-    constexpr unsigned LANES = 64u * WAVES, ROOM = PER * LANES < MT_SAMPLE_LIST ? PER * LANES : MT_SAMPLE_LIST;
-    constexpr unsigned DEEP = MT_SAMPLE_LIST / LANES;
-    const unsigned row = blockIdx.x / S, chunk = blockIdx.x % S, t = threadIdx.x, i0 = (chunk * LANES + t) * PER;
+                              unsigned* counts, mt_u64* sums, mt_u64* list, int* tokens, float* logprobs, mt_u64* lds) {
+    constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES, EACH = MT_SAMPLE_BINS / LANES;
+    constexpr unsigned SPAN = CHUNK / LANES;  // neighbours of a chunk that a lane adds up
+    const unsigned row = blockIdx.x / S, part = blockIdx.x % S, t = threadIdx.x;
     const float* x = logits + (size_t)row * RS;
     const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
+    const auto put = [](mt_u64* to, mt_u64 value) { __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const auto get = [](const mt_u64* from) {
+        return __hip_atomic_load(const_cast<mt_u64*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    // LDS: the folds' words and some results, a word for each chunk and four more; for cuts,
+    // mt_list_cut's, and the list
+    mt_u64 *chunk_kept = lds + WAVES + 4u, *words = chunk_kept + S, *cut_lds = words + 4u;
+    mt_u64* held = cut_lds + WAVES + 4u + MT_SAMPLE_PARTS + 2u * MT_SAMPLE_CLOSE;
     const mt_asked asked(row, uniforms, temperatures, top_k, top_p, min_p);
-    float v[PER];
-    mt_sample_load<V, PER, CS>(x, i0, v);
+    mt_sample_chunk<V, CHUNK, CS> chunk(x, part * CHUNK);
     mt_u64 best = 0;
     for (unsigned c = mt_lane(); c < S; c += 64u) {
-        const mt_u64 found = best_in[(size_t)row * S + c];
-        best = found > best ? found : best;
+        const mt_u64 one = best_in[(size_t)row * S + c];
+        best = one > best ? one : best;
+        if (CUT && t < 64u) chunk_kept[c] = one;
     }
     best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
-    if (mt_sample_plain(best, asked.temperature, row, chunk == 0u && t == 0u, tokens, logprobs)) return;
-    const mt_weights<SHIFT> weights{mt_order_value((unsigned)(best >> 32)), (double)asked.temperature};
+    if (mt_sample_plain(best, asked.temperature, row, part == 0u && t == 0u, tokens, logprobs)) return;
+    const mt_weights<SHIFT> weights{mt_order_value((unsigned)(best >> 32)), 1.0 / (double)asked.temperature};
     const mt_grid grid(asked.temperature);
     const float first = grid.bin(weights.top);
 
@@ -875,199 +944,202 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     bool by_k = asked.k > 0 && (unsigned)asked.k < V, by_p = asked.p < 1.f, whole = false;
     unsigned from = MT_SAMPLE_BINS, upto = MT_SAMPLE_BINS;  // (none listed, all stay)
     mt_u64 above_k = 0;                                     // logits above `from`
+    if (t < 4u) words[t] = 0;
+    __syncthreads();
     if constexpr (CUT) {
         if (by_k || by_p) {
-            // lane t: bin t of the row, the sums up to it
-            constexpr unsigned EACH = LANES / MT_SAMPLE_BINS;
-            static_assert(EACH >= 1u && LANES % MT_SAMPLE_BINS == 0u, "a lane to a bin at the least");
-            mt_u64 number = 0, mass = 0;
-            const unsigned bin = t % MT_SAMPLE_BINS;
-            for (unsigned c = t / MT_SAMPLE_BINS; c < S; c += EACH) {
-                const float shift = first - grid.bin(mt_order_value((unsigned)(best_in[(size_t)row * S + c] >> 32)));
-                if (shift >= 0.f && shift <= (float)bin) {
-                    const mt_u64 word = bins_in[((size_t)row * S + c) * MT_SAMPLE_BINS + (bin - (unsigned)shift)];
-                    number += word >> MT_SAMPLE_COUNT_AT, mass += word & ((1ull << MT_SAMPLE_COUNT_AT) - 1ull);
+            // this lane's bins, EACH neighbours: their logits and weights, and those before them
+            mt_u64 number[EACH], mass[EACH], numbers = 0, masses = 0;
+#pragma unroll
+            for (unsigned b = 0; b < EACH; ++b) number[b] = mass[b] = 0;
+#pragma unroll 8
+            for (unsigned c = 0; c < S; ++c) {  // (loads that do not wait for each other)
+                const float shift = first - grid.bin(mt_order_value((unsigned)(chunk_kept[c] >> 32)));
+                const int by = shift >= 0.f && shift < (float)MT_SAMPLE_BINS ? (int)shift : (int)MT_SAMPLE_BINS;
+#pragma unroll
+                for (unsigned b = 0; b < EACH; ++b) {
+                    const int at = (int)(t * EACH + b) - by;
+                    const mt_u64 word = bins_in[((size_t)row * S + c) * MT_SAMPLE_BINS + (at < 0 ? 0 : at)];
+                    number[b] += at < 0 ? 0 : word >> MT_SAMPLE_COUNT_AT;
+                    mass[b] += at < 0 ? 0 : word & ((1ull << MT_SAMPLE_COUNT_AT) - 1ull);
                 }
             }
-            if constexpr (EACH > 1u) {
-                mt_u64* other = lds + 2u * WAVES;
-                for (unsigned h = 1; h < EACH; ++h) {
-                    __syncthreads();
-                    if (t / MT_SAMPLE_BINS == h) other[2u * bin] = number, other[2u * bin + 1u] = mass;
-                    __syncthreads();
-                    if (t < MT_SAMPLE_BINS) number += other[2u * bin], mass += other[2u * bin + 1u];
-                }
-                if (t >= MT_SAMPLE_BINS) number = 0, mass = 0;
+#pragma unroll
+            for (unsigned b = 0; b < EACH; ++b) {
+                numbers += number[b];
+                // in 2^-40 of the first bin's lower edge
+                mass[b] = (mt_u64)((double)mass[b] * mt_exp_below(-0.0625 * (double)(t * EACH + b)) * 1048576.0);
+                masses += mass[b];
             }
-            // weights of the bin in 2^-20 of the first bin's edge, as a whole number of 2^-40
-            mass = (mt_u64)((double)mass * exp(-0.0625 * (double)bin) * 1048576.0);
-            mt_u64 all_number, all_mass;
-            const mt_u64 n0 = mt_group_before<WAVES>(number, lds, all_number), m0 = mt_group_before<WAVES>(mass, lds, all_mass);
-            if (t == 0u) lds[WAVES] = MT_SAMPLE_BINS, lds[WAVES + 1u] = MT_SAMPLE_BINS, lds[WAVES + 2u] = 0, lds[WAVES + 3u] = 0;
-            __syncthreads();
-            const mt_u64 k = (mt_u64)asked.k;
-            if (by_k && n0 < k && k <= n0 + number) lds[WAVES] = bin, lds[WAVES + 2u] = n0, lds[WAVES + 3u] = n0 + number;
-            if (by_p) {
-                const mt_u64 wanted = asked.weight_asked(all_mass);
-                if (m0 < wanted && wanted <= m0 + mass) lds[WAVES + 1u] = bin, lds[WAVES + 4u] = number;
-            }
-            __syncthreads();
-            const unsigned k_bin = (unsigned)lds[WAVES], p_bin = (unsigned)lds[WAVES + 1u];
-            mt_u64 listed = 0;
-            if (k_bin == MT_SAMPLE_BINS) by_k = false;  // (what weighs anything stays)
+            mt_u64 *found = lds + WAVES, all;
+            if (t == 0u) found[0] = found[1] = MT_SAMPLE_BINS;
             if (by_k) {
-                from = by_p ? 0u : k_bin, upto = k_bin;
-                above_k = by_p ? 0 : lds[WAVES + 2u];
-                listed = lds[WAVES + 3u] - above_k;
-            } else if (by_p) {
-                from = upto = p_bin;
-                listed = lds[WAVES + 4u];
-                whole = p_bin == MT_SAMPLE_BINS;
+                mt_u64 before = mt_group_before<WAVES>(numbers, lds, all);
+                const mt_u64 k = (mt_u64)asked.k;
+#pragma unroll
+                for (unsigned b = 0; b < EACH; ++b) {
+                    if (before < k && k <= before + number[b]) found[0] = t * EACH + b, found[2] = before, found[3] = number[b];
+                    before += number[b];
+                }
+                __syncthreads();
+                upto = (unsigned)found[0];
+                by_k = upto != MT_SAMPLE_BINS;  // (else what weighs anything stays)
+                if (by_k) {
+                    from = by_p ? 0u : upto, above_k = by_p ? 0 : found[2];
+                    whole = (by_p ? found[2] + found[3] : found[3]) > MT_SAMPLE_LIST;
+                }
             }
-            whole = whole || listed > MT_SAMPLE_LIST || !(__builtin_fabsf(first) < 1048576.f);
+            if (by_p && !by_k) {
+                __syncthreads();
+                mt_u64 before = mt_group_before<WAVES>(masses, lds, all);
+                const mt_u64 wanted = asked.weight_asked(all);
+#pragma unroll
+                for (unsigned b = 0; b < EACH; ++b) {
+                    if (before < wanted && wanted <= before + mass[b]) found[1] = t * EACH + b, found[3] = number[b];
+                    before += mass[b];
+                }
+                __syncthreads();
+                from = upto = (unsigned)found[1];
+                whole = from == MT_SAMPLE_BINS || found[3] > MT_SAMPLE_LIST;
+            }
+            whole = whole || !(__builtin_fabsf(first) < 1048576.f);
             __syncthreads();
         }
     }
-    if (whole && chunk != 0u) return;  // (the same in all workgroups of the row)
+    if (whole && part != 0u) return;  // (the same in all workgroups of the row)
     const bool cuts = from < MT_SAMPLE_BINS;
     if (!whole) {
         mt_u64 all = 0, above = 0, kept = 0;
-        unsigned marks = 0u;  // which of this lane's are listed
-#pragma unroll
-        for (unsigned e = 0; e < PER; ++e) {
-            if (i0 + e >= V) continue;
+        const bool weigh_all = by_p && !by_k;
+        chunk.each([&](unsigned i, float v) {
             bool stays = true;
             if (CUT && cuts) {
-                const float below = first - grid.bin(v[e]);
+                const float below = first - grid.bin(v);
                 stays = below < (float)from;
-                if (!stays && below <= (float)upto) marks |= 1u << e;
+                if (!stays && below <= (float)upto) {
+                    const unsigned to = (unsigned)atomicAdd(words + 3, 1ull);
+                    if (to < MT_SAMPLE_LIST) held[to] = mt_best(i, v);
+                }
             }
-            if (stays || (by_p && !by_k)) {
-                const double w = weights.weight(v[e]);
+            if (stays || weigh_all) {
+                const double w = weights.weight(v);
                 const mt_u64 h = weights.whole(w);
                 all += h;
                 if (stays) above += h, kept += w < asked.least ? 0 : h;
             }
-        }
-        mt_u64* mine = sums + ((size_t)row * S + chunk) * 4u;
-        const auto put = [](mt_u64* to, mt_u64 value) { __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-        const auto get = [](const mt_u64* from_) {
-            return __hip_atomic_load(const_cast<mt_u64*>(from_), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        };
-        mt_u64 listed = 0;
-        if (CUT && cuts) {
-            mt_u64 at = mt_group_before<WAVES>(__builtin_popcount(marks), lds, listed);
-#pragma unroll
-            for (unsigned e = 0; e < PER; ++e)
-                if ((marks >> e) & 1u) {
-                    if (at < ROOM) put(list + ((size_t)row * S + chunk) * ROOM + at, mt_best(i0 + e, v[e]));
-                    ++at;
-                }
-        }
-        if (CUT && by_p && !by_k) all = mt_group_fold<WAVES>(all, lds, sum), above = mt_group_fold<WAVES>(above, lds, sum);
-        kept = mt_group_fold<WAVES>(kept, lds, sum);
-        if (t == 0u) put(mine, all), put(mine + 1, above), put(mine + 2, kept), put(mine + 3, listed);
-        if constexpr (S > 1u) {
-            __builtin_amdgcn_s_waitcnt(0);  // every lane's stores have reached memory
-            __syncthreads();
-            if (t == 0u) lds[0] = __hip_atomic_fetch_add(arrivals + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
-            if (lds[0] + 1u != S) return;
-        } else {
-            __builtin_amdgcn_s_waitcnt(0);
+        });
+        if (from != 0u || weigh_all) {  // (else nothing stays before the list is looked at)
+            all = mt_wave_fold(all, sum), above = mt_wave_fold(above, sum), kept = mt_wave_fold(kept, sum);
+            if (mt_lane() == 0u) atomicAdd(words, all), atomicAdd(words + 1, above), atomicAdd(words + 2, kept);
         }
         __syncthreads();
-
-        // The last workgroup of the row.  In LDS: what stays of each chunk, and where each
-        // chunk's part of the list begins.
-        mt_u64 *chunk_kept = lds + 2u * WAVES + LANES + 2u * MT_SAMPLE_CLOSE, *begins = chunk_kept + S;
-        mt_u64 row_all = 0, row_above = 0;
-        unsigned n = 0u;
-        for (unsigned c = 0; c < S; c += 64u) {  // (each wave for itself)
-            const bool live = c + mt_lane() < S;
-            const mt_u64* at = sums + ((size_t)row * S + c + mt_lane()) * 4u;
-            const mt_u64 part = live ? get(at + 3) : 0;
-            if (CUT && by_p && !by_k) {
-                row_all += mt_wave_fold(live ? get(at) : 0, sum);
-                row_above += mt_wave_fold(live ? get(at + 1) : 0, sum);
+        unsigned n = (unsigned)words[3];  // (at most LIST, as the bins said)
+        n = n < MT_SAMPLE_LIST ? n : MT_SAMPLE_LIST;
+        mt_u64 row_all = words[0], row_above = words[1];
+        if constexpr (S > 1u) {
+            mt_u64* mine = sums + ((size_t)row * S + part) * 3u;
+            if (t < 3u) put(mine + t, words[t]);
+            if (CUT && n != 0u) {
+                __syncthreads();
+                if (t == 0u) words[3] = __hip_atomic_fetch_add(counts + 2u * row + 1u, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+                for (unsigned l = t; l < n; l += LANES)
+                    if ((unsigned)words[3] + l < MT_SAMPLE_LIST) put(list + (size_t)row * MT_SAMPLE_LIST + (unsigned)words[3] + l, held[l]);
             }
-            mt_u64 before = part;
-#pragma unroll
-            for (unsigned off = 1u; off < 64u; off *= 2u) {
-                const mt_u64 other = __shfl_up(before, off, 64);
-                if (mt_lane() >= off) before += other;
+            __builtin_amdgcn_s_waitcnt(0);  // every lane's stores have reached memory
+            __syncthreads();
+            if (t == 0u) words[3] = __hip_atomic_fetch_add(counts + 2u * row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (words[3] + 1u != S) return;
+            // the last workgroup of the row: what stays of each chunk, and the list
+            mt_u64 one_all = 0, one_above = 0;
+            for (unsigned c = mt_lane(); c < S; c += 64u) {
+                const mt_u64* of = sums + ((size_t)row * S + c) * 3u;
+                if (CUT && weigh_all) one_all += get(of), one_above += get(of + 1);
+                if (t < 64u) chunk_kept[c] = get(of + 2);
             }
-            if (live && t < 64u) begins[c + mt_lane()] = n + before - part, chunk_kept[c + mt_lane()] = get(at + 2);
-            n += (unsigned)__shfl(before, 63, 64);
+            if (CUT && cuts) {
+                n = __hip_atomic_load(counts + 2u * row + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                n = n < MT_SAMPLE_LIST ? n : MT_SAMPLE_LIST;
+                for (unsigned l = t; l < n; l += LANES) held[l] = get(list + (size_t)row * MT_SAMPLE_LIST + l);
+                if (weigh_all) row_all = mt_wave_fold(one_all, sum), row_above = mt_wave_fold(one_above, sum);
+            }
+        } else {
+            if (t == 0u) chunk_kept[0] = words[2];
         }
         __syncthreads();
         mt_cut_at cut{0u, 0xFFFFFFFFu};
         if (CUT && cuts) {
-            // lane t: entries t, t + LANES .. of the list, and what they count or weigh
-            mt_u64 entry[DEEP], amount[DEEP];
-#pragma unroll
-            for (unsigned d = 0; d < DEEP; ++d) {
-                const unsigned l = t + d * LANES;
-                entry[d] = 0, amount[d] = 0;
-                if (l < n) {
-                    unsigned lo = 0u, hi = S;
-                    while (hi - lo > 1u) {
-                        const unsigned mid = (lo + hi) / 2u;
-                        if (begins[mid] <= l) lo = mid;
-                        else hi = mid;
-                    }
-                    entry[d] = get(list + ((size_t)row * S + lo) * ROOM + (l - (unsigned)begins[lo]));
-                    amount[d] = 1;
-                }
-            }
+            const auto value = [](mt_u64 one) { return mt_order_value((unsigned)(one >> 32)); };
             const auto stays = [&](mt_u64 one) { return cut.stays((unsigned)(one >> 32), 0xFFFFFFFFu - (unsigned)one); };
-            if (by_k) whole = !mt_list_cut<WAVES>(entry, amount, n, (mt_u64)asked.k - above_k, cut, lds);
-            mt_u64 total = 0;
-            unsigned light = 0u;  // those below min_p
-#pragma unroll
-            for (unsigned d = 0; d < DEEP; ++d) {
-                if (amount[d] != 0) {
-                    const double w = weights.weight(mt_order_value((unsigned)(entry[d] >> 32)));
-                    amount[d] = stays(entry[d]) ? weights.whole(w) : 0;
-                    total += amount[d];
-                    if (w < asked.least) light |= 1u << d;
-                }
-            }
+            // the part of bins `from` .. `upto` that a logit is in
+            const float scale = (float)MT_SAMPLE_PARTS / (float)(upto - from + 1u), edge = first - (float)from + 1.f;
+            const auto place = [&](mt_u64 one) {
+                const float at = (edge - value(one) * grid.by) * scale;
+                return at < 0.f ? 0u : at < (float)MT_SAMPLE_PARTS ? (unsigned)at : MT_SAMPLE_PARTS - 1u;
+            };
+            if (by_k)
+                whole = !mt_list_cut(held, n, [](mt_u64) { return (mt_u64)1; }, place, (mt_u64)asked.k - above_k, cut, cut_lds);
             if (by_p && !whole) {
-                total = mt_group_fold<WAVES>(total, lds, sum);
-                const mt_u64 wanted = asked.weight_asked(by_k ? total : row_all);
-                if (by_k || (row_above < wanted && wanted <= row_above + total))
-                    whole = !mt_list_cut<WAVES>(entry, amount, n, wanted - row_above, cut, lds);
-                else
-                    whole = true;  // (next to a bin's edge)
+                if (by_k) {
+                    mt_u64 total = 0;
+                    for (unsigned l = t; l < n; l += LANES) total += stays(held[l]) ? weights.held(value(held[l])) : 0;
+                    row_all = mt_group_fold<WAVES>(total, lds, sum), row_above = 0;
+                }
+                const mt_u64 wanted = asked.weight_asked(row_all);
+                const mt_cut_at by = cut;
+                whole = wanted <= row_above ||
+                        !mt_list_cut(held, n, [&](mt_u64 one) {
+                            return by.stays((unsigned)(one >> 32), 0xFFFFFFFFu - (unsigned)one) ? weights.held(value(one)) : (mt_u64)0;
+                        }, place, wanted - row_above, cut, cut_lds);
             }
-#pragma unroll
-            for (unsigned d = 0; d < DEEP; ++d)
-                if (amount[d] != 0 && !((light >> d) & 1u) && stays(entry[d]))
-                    atomicAdd(chunk_kept + (0xFFFFFFFFu - (unsigned)entry[d]) / (PER * LANES), amount[d]);
+            for (unsigned l = t; l < n; l += LANES)
+                if (stays(held[l])) {
+                    const mt_u64 h = weights.kept(value(held[l]), asked.least);
+                    if (h != 0) atomicAdd(chunk_kept + (0xFFFFFFFFu - (unsigned)held[l]) / CHUNK, h);
+                }
             __syncthreads();
         }
         if (!whole) {
-            // The chunk that the random number falls into, and the token in it.
-            mt_u64 total = 0;
+            // The chunk that the random number falls into, the lane's neighbours in it, the token.
+            mt_u64 total = 0, before = 0, every;
             for (unsigned c = 0; c < S; ++c) total += chunk_kept[c];
             const mt_u64 target = asked.target(total);
-            mt_u64 before = 0;
             unsigned in = 0u;
             while (in + 1u < S && before + chunk_kept[in] <= target) before += chunk_kept[in], ++in;
-            const unsigned k0 = (in * LANES + t) * PER;
-            mt_sample_load<V, PER, CS>(x, k0, v);
-            mt_u64 w[PER], lane_all = 0, every;
+            const auto amount = [&](unsigned i, float v) {
+                return i < V && cut.stays(mt_order_key(v), i) ? weights.kept(v, asked.least) : (mt_u64)0;
+            };
+            const unsigned l0 = in * CHUNK + t * SPAN;
+            mt_u64 lane_all = 0;
+#pragma unroll 4
+            for (unsigned e = 0; e < SPAN; e += 4u) {
+                if (l0 + e >= V) break;
+                const mt_f32x4 v = mt_row4<V, CS>(x, l0 + e);
 #pragma unroll
-            for (unsigned e = 0; e < PER; ++e) {
-                w[e] = k0 + e < V && cut.stays(mt_order_key(v[e]), k0 + e) ? weights.kept(v[e], asked.least) : 0;
-                lane_all += w[e];
+                for (unsigned j = 0; j < 4u; ++j) lane_all += amount(l0 + e + j, v[j]);
             }
             before += mt_group_before<WAVES>(lane_all, lds, every);
+            if (before <= target && target < before + lane_all) words[0] = l0, words[1] = before;
+            __syncthreads();
+            if (t >= 64u) return;
+            before = words[1];
+            const double log_total = weights.log_of(total);
+#pragma unroll 1
+            for (unsigned e = 0; e < SPAN; e += 64u) {
+                const unsigned i = (unsigned)words[0] + e + t;
+                const float v = e + t < SPAN && i < V ? x[(size_t)i * CS] : -INFINITY;
+                const mt_u64 w = e + t < SPAN ? amount(i, v) : 0;
+                mt_u64 upto_here = w;
 #pragma unroll
-            for (unsigned e = 0; e < PER; ++e) {
-                if (before <= target && target < before + w[e]) weights.answer(row, k0 + e, v[e], total, tokens, logprobs);
-                before += w[e];
+                for (unsigned off = 1u; off < 64u; off *= 2u) {
+                    const mt_u64 other = __shfl_up(upto_here, off, 64);
+                    if (t >= off) upto_here += other;
+                }
+                if (before + upto_here - w <= target && target < before + upto_here)
+                    weights.answer(row, i, v, log_total, tokens, logprobs);
+                before += (mt_u64)__shfl(upto_here, 63, 64);
+                if (before > target) break;
             }
             return;
         }

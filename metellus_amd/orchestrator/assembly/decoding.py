@@ -14,8 +14,7 @@ from metellus_amd.orchestrator.decoding import (
     ADAPTER_DOWN_WAVES,
     ADAPTER_MANY_ROWS,
     SAMPLE_BINS,
-    SAMPLE_CLOSE,
-    SAMPLE_LANES,
+    SAMPLE_LIST,
     AdapterDownOp,
     AdapterUpOp,
     PageTablesOp,
@@ -199,7 +198,8 @@ def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name:
 # sampling
 # ---------------------------------------------------------------------------
 
-SAMPLE_WAVES = SAMPLE_LANES // 64
+SAMPLE_WAVES = 4
+SAMPLE_CUT_WORDS = SAMPLE_WAVES + 4 + 1024 + 2 * 256  # of LDS, that finding a cut in a list takes
 
 
 def _words(sig: _Signature, role: str, t: Tensor | None, *, out: bool = False) -> str:
@@ -210,7 +210,7 @@ def _words(sig: _Signature, role: str, t: Tensor | None, *, out: bool = False) -
 
 def _assemble_sample_scan(decision: DecisionView, op: SampleScanOp, function_name: str | None) -> KernelGroup:
     rows, cols = op.logits.shape
-    per, chunks = sample_chunks(rows, cols)
+    chunk, chunks = sample_chunks(rows, cols)
     cuts = op.bins is not None
     sig = _Signature()
     args = (
@@ -220,23 +220,23 @@ def _assemble_sample_scan(decision: DecisionView, op: SampleScanOp, function_nam
         sig.add("top_p", op.top_p),
         _words(sig, "best", op.best, out=True),
         _words(sig, "bins", op.bins, out=True),
-        f"(unsigned*){sig.add('arrivals', op.arrivals, out=True)}",
+        f"(unsigned*){sig.add('counts', op.counts, out=True)}",
         "(mt_u64*)mt_lds",
     )
     frag = ServingFragment(
         "mt_sample_scan",
-        (cols, per, chunks, SAMPLE_WAVES, *_strides(op.logits), cuts),
+        (cols, chunk, chunks, *_strides(op.logits), cuts),
         args,
         lds_bytes=8 * (SAMPLE_WAVES + (SAMPLE_BINS if cuts else 0)),
         name="sample_scan",
     )
-    return _group(decision, sig, frag, function_name or f"sample_scan_{op.name}", {}, (rows * chunks, 1, 1), SAMPLE_LANES,
+    return _group(decision, sig, frag, function_name or f"sample_scan_{op.name}", {}, (rows * chunks, 1, 1), 64 * SAMPLE_WAVES,
                   headers=(decoding_header(),))
 
 
 def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | None) -> KernelGroup:
     rows, cols = op.logits.shape
-    per, chunks = sample_chunks(rows, cols)
+    chunk, chunks = sample_chunks(rows, cols)
     cuts = op.bins is not None
     sig = _Signature()
     args = (
@@ -248,7 +248,7 @@ def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | 
         sig.add("min_p", op.min_p),
         _words(sig, "best", op.best),
         _words(sig, "bins", op.bins),
-        f"(unsigned*){sig.add('arrivals', op.arrivals, out=True)}",
+        f"(unsigned*){sig.add('counts', op.counts, out=True)}",
         _words(sig, "sums", op.sums, out=True),
         _words(sig, "list", op.listed, out=True),
         sig.add("tokens", op.tokens, out=True),
@@ -259,12 +259,13 @@ def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | 
     shift = min(44, 62 - (cols - 1).bit_length())
     frag = ServingFragment(
         "mt_sample_pick",
-        (cols, per, chunks, shift, SAMPLE_WAVES, *_strides(op.logits), cuts),
+        (cols, chunk, chunks, shift, *_strides(op.logits), cuts),
         args,
-        lds_bytes=8 * (2 * SAMPLE_WAVES + SAMPLE_LANES + 2 * SAMPLE_CLOSE + 2 * chunks),
+        # (one workgroup for a whole row takes two words a wave and 256)
+        lds_bytes=8 * max(SAMPLE_WAVES + 8 + chunks + (SAMPLE_CUT_WORDS + SAMPLE_LIST if cuts else 0), 2 * SAMPLE_WAVES + 256),
         name="sample",
     )
-    return _group(decision, sig, frag, function_name or f"sample_{op.tokens.name}", {}, (rows * chunks, 1, 1), SAMPLE_LANES,
+    return _group(decision, sig, frag, function_name or f"sample_{op.tokens.name}", {}, (rows * chunks, 1, 1), 64 * SAMPLE_WAVES,
                   headers=(decoding_header(),))
 
 

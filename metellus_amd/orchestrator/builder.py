@@ -24,6 +24,7 @@ from metellus_amd.compute.elementwise.elementwise import BroadcastSpec
 from metellus_amd.orchestrator.decoding import (
     ADAPTER_RANK_MAX,
     SAMPLE_BINS,
+    SAMPLE_LIST,
     AdapterDownOp,
     AdapterUpOp,
     PageTablesOp,
@@ -33,7 +34,6 @@ from metellus_amd.orchestrator.decoding import (
     SampleScanOp,
     adapter_splits,
     sample_chunks,
-    sample_room,
 )
 from metellus_amd.orchestrator.ir import (
     ITEM_BYTES,
@@ -617,18 +617,18 @@ class Operations:
         if len(tl.shape) != 2:
             raise ValueError(f"sample logits must be 2D; got shape {tl.shape} ({tl.name!r})")
         rows, cols = tl.shape
-        per, chunks = sample_chunks(rows, cols)
+        _, chunks = sample_chunks(rows, cols)
         cuts = top_k is not None or top_p is not None
 
-        def made(part: str, width: int) -> Tensor:
-            return self._fresh(f"{out}.{part}", (rows * chunks, width), "int32")
+        def made(part: str, rows: int, words: int) -> Tensor:
+            return self._fresh(f"{out}.{part}", (rows, 2 * words), "int32")
 
         scan = SampleScanOp(
-            best=made("best", 2),
-            arrivals=self._fresh(f"{out}.arrivals", (rows,), "int32"),
+            best=made("best", rows * chunks, 1),
+            counts=made("counts", rows, 1),
             logits=tl,
             name=out,
-            bins=made("bins", 2 * SAMPLE_BINS) if cuts else None,
+            bins=made("bins", rows * chunks, SAMPLE_BINS) if cuts else None,
             **{n: t if cuts else None for n, t in given.items() if n != "min_p"},
             after=self._owners(tl, *given.values()),
         )
@@ -637,10 +637,10 @@ class Operations:
             logits=tl,
             uniforms=tu,
             best=scan.best,
-            arrivals=scan.arrivals,
+            counts=scan.counts,
             bins=scan.bins,
-            sums=made("sums", 8),
-            listed=made("list", 2 * sample_room(per)) if cuts else None,
+            sums=made("sums", rows * chunks, 3),
+            listed=made("list", rows, SAMPLE_LIST) if cuts else None,
             logprobs=None if logprobs is None else self._fresh(logprobs, (rows,), "float32"),
             after=self._owners(tl, tu, *given.values()),
             **given,

@@ -30,9 +30,8 @@ ROTARY_LAYOUTS = ("half", "interleaved")
 POSITIONS_MAX = _INT32_MAX - 1024  # of a table's row (its positions and a step's rows are int32)
 ADAPTER_RANK_MAX = 256
 VOCABULARY_MAX = 2**20
-SAMPLE_LANES = 1024
-SAMPLE_BINS, SAMPLE_LIST = 512, 8192  # of a row's chunk; logits that a row has listed at most
-SAMPLE_CLOSE = 256  # of those, that are compared one by one
+SAMPLE_CHUNK = 4096  # logits, and the smallest share of a workgroup
+SAMPLE_BINS, SAMPLE_LIST = 512, 8192  # of a chunk; logits that a row has listed at most
 
 # pi to 64 digits: 2 pi has to outlast a double's 53 bits twice
 _PI = Decimal("3.141592653589793238462643383279502884197169399375105820974944592")
@@ -308,26 +307,21 @@ class AdapterUpOp(ServingOp):
 
 
 def sample_chunks(rows: int, cols: int) -> tuple[int, int]:
-    """Neighbouring logits that a lane of SAMPLE_LANES takes, and the chunks of a row that
-    this makes: at most 64, and more of them where rows are few."""
-    per = 4
-    while per < 16 and (rows * -(-cols // (per * SAMPLE_LANES)) > 512 or cols > 64 * per * SAMPLE_LANES):
-        per *= 2
-    return per, -(-cols // (per * SAMPLE_LANES))
-
-
-def sample_room(per: int) -> int:
-    """Listed logits that a chunk has room for."""
-    return min(per * SAMPLE_LANES, SAMPLE_LIST)
+    """Logits of a chunk, and the chunks of a row: as many as make 512 workgroups of all
+    rows, but at most 16, for each workgroup adds all of a row's bins up."""
+    chunk = SAMPLE_CHUNK
+    while cols > chunk and (rows * -(-cols // chunk) > 512 or cols > 16 * chunk):
+        chunk *= 2
+    return chunk, -(-cols // chunk)
 
 
 @dataclass(frozen=True)
 class SampleScanOp(ServingOp):
     """The largest logit of each chunk (int64s, as two int32), and its bins for rows that
-    ``top_k`` or ``top_p`` cut; the rows' arrivals are cleared."""
+    ``top_k`` or ``top_p`` cut; the rows' counts of arrivals and listed logits are cleared."""
 
     best: Tensor
-    arrivals: Tensor
+    counts: Tensor
     logits: Tensor
     name: str  # of the operator's output
     bins: Tensor | None = None
@@ -347,7 +341,7 @@ class SampleScanOp(ServingOp):
 
     @property
     def outs(self) -> tuple[Tensor, ...]:
-        return tuple(t for t in (self.best, self.arrivals, self.bins) if t is not None)
+        return tuple(t for t in (self.best, self.counts, self.bins) if t is not None)
 
     @property
     def reads(self) -> tuple[Tensor, ...]:
@@ -366,7 +360,7 @@ class SampleOp(ServingOp):
     logits: Tensor
     uniforms: Tensor
     best: Tensor
-    arrivals: Tensor
+    counts: Tensor
     sums: Tensor
     bins: Tensor | None = None
     listed: Tensor | None = None
@@ -394,6 +388,6 @@ class SampleOp(ServingOp):
         return tuple(
             t
             for t in (self.logits, self.uniforms, self.temperatures, self.top_k, self.top_p, self.min_p, self.best, self.bins,
-                      self.arrivals)
+                      self.counts)
             if t is not None
         )
