@@ -755,6 +755,7 @@ constexpr unsigned MT_SAMPLE_WAVES = 4u, MT_SAMPLE_LANES = 256u;
 constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 8192u;
 constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
 constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
+constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... by one wave, all of a list
 constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
 
 // The bin of x on the grid of a temperature.
@@ -906,6 +907,69 @@ MT_INLINE bool mt_list_cut(const mt_u64* list, unsigned n, AMOUNT amount, PLACE 
     return found[3] != 0;
 }
 
+// A cut by k, one by p if asked, and the token, by one wave, of a list of at most two entries
+// a lane that has everything that may stay: entries are ranked by comparing each with all, the weights
+// before a rank or an index found by adding up those that compare so.  `lds`: 128 words.
+template <unsigned SHIFT>
+MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& asked, const mt_weights<SHIFT>& weights,
+                               unsigned row, int* tokens, float* logprobs, mt_u64* lds) {
+    const unsigned t = mt_lane();
+    const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
+    mt_u64 one[2], weight[2], before[2] = {0, 0};
+    unsigned rank[2] = {0u, 0u};
+    double w[2];
+#pragma unroll
+    for (unsigned d = 0; d < 2u; ++d) {
+        one[d] = t + 64u * d < n ? list[t + 64u * d] : 0;
+        w[d] = weights.weight(mt_order_value((unsigned)(one[d] >> 32)));
+    }
+#pragma unroll 4
+    for (unsigned j = 0; j < n; ++j) {
+        const mt_u64 other = list[j];
+        rank[0] += other > one[0] ? 1u : 0u, rank[1] += other > one[1] ? 1u : 0u;
+    }
+    mt_u64 total = 0;
+#pragma unroll
+    for (unsigned d = 0; d < 2u; ++d) {
+        weight[d] = one[d] != 0 && rank[d] < (unsigned)asked.k ? weights.whole(w[d]) : 0;
+        lds[t + 64u * d] = weight[d];
+        total += weight[d];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (asked.p < 1.f) {
+        const mt_u64 wanted = asked.weight_asked(mt_wave_fold(total, sum));
+#pragma unroll 4
+        for (unsigned j = 0; j < n; ++j) {
+            const mt_u64 other = list[j], more = lds[j];
+            before[0] += other > one[0] ? more : 0, before[1] += other > one[1] ? more : 0;
+        }
+        weight[0] = before[0] < wanted ? weight[0] : 0, weight[1] = before[1] < wanted ? weight[1] : 0;
+    }
+    total = 0;
+#pragma unroll
+    for (unsigned d = 0; d < 2u; ++d) {
+        if (w[d] < asked.least) weight[d] = 0;
+        total += weight[d];
+        before[d] = 0;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (all have read the weights)
+    lds[t] = weight[0], lds[t + 64u] = weight[1];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    total = mt_wave_fold(total, sum);
+    const mt_u64 target = asked.target(total);
+    const double log_total = weights.log_of(total);
+#pragma unroll 4
+    for (unsigned j = 0; j < n; ++j) {
+        const mt_u64 more = lds[j];
+        const unsigned other = (unsigned)list[j];  // (upside down: larger is an earlier index)
+        before[0] += other > (unsigned)one[0] ? more : 0, before[1] += other > (unsigned)one[1] ? more : 0;
+    }
+#pragma unroll
+    for (unsigned d = 0; d < 2u; ++d)
+        if (before[d] <= target && target < before[d] + weight[d])
+            weights.answer(row, 0xFFFFFFFFu - (unsigned)one[d], mt_order_value((unsigned)(one[d] >> 32)), log_total, tokens, logprobs);
+}
+
 // sums: [row][S][3], all weights, those above the cut, and those of them that min_p leaves;
 // list: [row][MT_SAMPLE_LIST].
 template <unsigned V, unsigned CHUNK, unsigned S, unsigned SHIFT, unsigned RS, unsigned CS, bool CUT>
@@ -952,7 +1016,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             mt_u64 number[EACH], mass[EACH], numbers = 0, masses = 0;
 #pragma unroll
             for (unsigned b = 0; b < EACH; ++b) number[b] = mass[b] = 0;
-#pragma unroll 8
+#pragma unroll
             for (unsigned c = 0; c < S; ++c) {  // (loads that do not wait for each other)
                 const float shift = first - grid.bin(mt_order_value((unsigned)(chunk_kept[c] >> 32)));
                 const int by = shift >= 0.f && shift < (float)MT_SAMPLE_BINS ? (int)shift : (int)MT_SAMPLE_BINS;
@@ -985,8 +1049,10 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
                 upto = (unsigned)found[0];
                 by_k = upto != MT_SAMPLE_BINS;  // (else what weighs anything stays)
                 if (by_k) {
-                    from = by_p ? 0u : upto, above_k = by_p ? 0 : found[2];
-                    whole = (by_p ? found[2] + found[3] : found[3]) > MT_SAMPLE_LIST;
+                    // (of few, all are listed: nothing else stays then)
+                    const bool every = by_p || found[2] + found[3] <= MT_SAMPLE_SHORT;
+                    from = every ? 0u : upto, above_k = every ? 0 : found[2];
+                    whole = found[2] + found[3] - above_k > MT_SAMPLE_LIST;
                 }
             }
             if (by_p && !by_k) {
@@ -1068,6 +1134,10 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             if (t == 0u) chunk_kept[0] = words[2];
         }
         __syncthreads();
+        if (CUT && by_k && from == 0u && n <= MT_SAMPLE_SHORT) {
+            if (t < 64u) mt_sample_short<SHIFT>(held, n, asked, weights, row, tokens, logprobs, cut_lds);
+            return;
+        }
         mt_cut_at cut{0u, 0xFFFFFFFFu};
         if (CUT && cuts) {
             const auto value = [](mt_u64 one) { return mt_order_value((unsigned)(one >> 32)); };
