@@ -457,6 +457,29 @@ MT_INLINE mt_u64 mt_wave_fold(mt_u64 v, OP op) {
     return v;
 }
 
+// The sum of v over this lane and those before it, by adding from one lane, two, four and
+// eight before in rows of 16, then from the ends of the rows before.
+template <int FROM, int ROWS>
+MT_INLINE mt_u64 mt_add_from(mt_u64 v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, FROM, ROWS, 15, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), FROM, ROWS, 15, false);
+    return v + (((mt_u64)hi << 32) | lo);
+}
+MT_INLINE mt_u64 mt_wave_upto(mt_u64 v) {
+    v = mt_add_from<0x111, 15>(v);  // row_shr:1
+    v = mt_add_from<0x112, 15>(v);
+    v = mt_add_from<0x114, 15>(v);
+    v = mt_add_from<0x118, 15>(v);
+    v = mt_add_from<0x142, 10>(v);  // row_bcast:15 into rows 1 and 3
+    return mt_add_from<0x143, 12>(v);  // row_bcast:31 into rows 2 and 3
+}
+// The last lane's word.
+MT_INLINE mt_u64 mt_wave_last(mt_u64 v) {
+    return ((mt_u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), 63) << 32) |
+           (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, 63);
+}
+MT_INLINE mt_u64 mt_wave_sum(mt_u64 v) { return mt_wave_last(mt_wave_upto(v)); }
+
 // v (op) over the workgroup's waves; `lds` holds a word a wave.
 template <unsigned WAVES, typename OP>
 MT_INLINE mt_u64 mt_group_fold(mt_u64 v, mt_u64* lds, OP op) {
@@ -470,15 +493,23 @@ MT_INLINE mt_u64 mt_group_fold(mt_u64 v, mt_u64* lds, OP op) {
     return v;
 }
 
+// The sum of v over the workgroup.
+template <unsigned WAVES>
+MT_INLINE mt_u64 mt_group_sum(mt_u64 v, mt_u64* lds) {
+    v = mt_wave_sum(v);
+    __syncthreads();
+    if (mt_lane() == 0u) lds[mt_wave()] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (unsigned w = 0; w < WAVES; ++w) v += lds[w];
+    return v;
+}
+
 // The sum of v over the lanes before this one; `all`: over all of them.
 template <unsigned WAVES>
 MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
-    mt_u64 sum = v;
-#pragma unroll
-    for (unsigned off = 1u; off < 64u; off *= 2u) {
-        const mt_u64 other = __shfl_up(sum, off, 64);
-        if (mt_lane() >= off) sum += other;
-    }
+    const mt_u64 sum = mt_wave_upto(v);
     __syncthreads();
     if (mt_lane() == 63u) lds[mt_wave()] = sum;
     __syncthreads();
@@ -492,13 +523,12 @@ MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
     return before + sum - v;
 }
 
-// e^z for z <= 0, right to about 2^-51 of itself; 0 below -700.  z = n log 2 + r, and the
-// series of e^r: for |r| up to log(2) / 2 its 14th term is under 2^-57.
+// e^z for z <= 0, right to about 2^-50 of itself; 0 below -700, and for a NaN.  z = n log 2 +
+// r, and the series of e^r: for |r| up to log(2) / 2 its 13th term is under 2^-51.
 MT_INLINE double mt_exp_below(double z) {
     const double n = __builtin_rint(z * 0x1.71547652b82fep+0);  // 1 / log 2
     const double r = __builtin_fma(n, -0x1.abc9e3b39803fp-56, __builtin_fma(n, -0x1.62e42fefa39efp-1, z));  // (log 2 in two parts)
-    double e = 1.0 / 6227020800.0;
-    e = __builtin_fma(e, r, 1.0 / 479001600.0);
+    double e = 1.0 / 479001600.0;
     e = __builtin_fma(e, r, 1.0 / 39916800.0);
     e = __builtin_fma(e, r, 1.0 / 3628800.0);
     e = __builtin_fma(e, r, 1.0 / 362880.0);
@@ -511,7 +541,10 @@ MT_INLINE double mt_exp_below(double z) {
     e = __builtin_fma(e, r, 0.5);
     e = __builtin_fma(e, r, 1.0);
     e = __builtin_fma(e, r, 1.0);
-    return z < -700.0 ? 0.0 : __builtin_ldexp(e, (int)n);
+    const bool some = z >= -700.0;
+    // (e is 0.7 to 1.5: its exponent takes n as it is)
+    const mt_u64 bits = __builtin_bit_cast(mt_u64, e) + ((mt_u64)(unsigned)(some ? (int)n : 0) << 52);
+    return some ? __builtin_bit_cast(double, bits) : 0.0;
 }
 
 // The weights of a row.
@@ -519,12 +552,15 @@ template <unsigned SHIFT>
 struct mt_weights {
     float top;
     double by;  // one over the temperature
-    MT_INLINE double scaled(float x) const { return ((double)x - (double)top) * by; }
-    MT_INLINE double weight(float x) const {
-        if (x == top) return 1.0;
-        return x == -INFINITY || top == INFINITY ? 0.0 : mt_exp_below(scaled(x));  // (whatever the temperature)
+    MT_INLINE double scaled(float x) const { return x == top ? 0.0 : ((double)x - (double)top) * by; }
+    // (an x that is -inf weighs nothing, and beside a top of +inf so do all others, whatever
+    // the temperature: what they are scaled to is -inf or no number)
+    MT_INLINE double weight(float x) const { return mt_exp_below(scaled(x)); }
+    // The nearest whole number of 2^-SHIFT: in the last bits of a sum with 1.5 2^52.
+    MT_INLINE static mt_u64 whole(double w) {
+        const double sum = __builtin_fma(w, (double)(1ull << SHIFT), 0x1.8p52);
+        return __builtin_bit_cast(mt_u64, sum) - __builtin_bit_cast(mt_u64, 0x1.8p52);
     }
-    MT_INLINE static mt_u64 whole(double w) { return (mt_u64)__builtin_rint(w * (double)(1ull << SHIFT)); }
     MT_INLINE mt_u64 held(float x) const { return whole(weight(x)); }
     // 0 for a weight below `least`.
     MT_INLINE mt_u64 kept(float x, double least) const {
@@ -534,7 +570,7 @@ struct mt_weights {
     MT_INLINE static double log_of(mt_u64 total) { return log((double)total * (1.0 / (double)(1ull << SHIFT))); }
     MT_INLINE void answer(unsigned row, unsigned i, float x, double log_total, int* tokens, float* logprobs) const {
         tokens[row] = (int)i;
-        if (logprobs != nullptr) logprobs[row] = (float)((x == top ? 0.0 : scaled(x)) - log_total);
+        if (logprobs != nullptr) logprobs[row] = (float)(scaled(x) - log_total);
     }
 };
 
@@ -640,7 +676,6 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
                                int* tokens, float* logprobs, mt_u64* lds) {
     constexpr unsigned LANES = 64u * WAVES, STEP = 4u * LANES;
     const unsigned t = threadIdx.x;
-    const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
     const auto each = [&](auto f) {
 #pragma unroll 1
         for (unsigned c0 = 4u * t; c0 < V; c0 += 4u * STEP) {
@@ -695,7 +730,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
         const auto amount = [&](unsigned i, float v) { return by_k.stays(mt_order_key(v), i) ? weights.held(v) : (mt_u64)0; };
         mt_u64 total = 0;
         each([&](unsigned i, float v) { total += amount(i, v); });
-        total = mt_group_fold<WAVES>(total, lds, sum);
+        total = mt_group_sum<WAVES>(total, lds);
         const mt_u64 wanted = asked.weight_asked(total);
         cut.key = mt_find_cut<WAVES>(each, amount, wanted, above, at, lds);
         if (cut.key != by_k.key) cut.last = 0xFFFFFFFFu;
@@ -704,7 +739,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
     const auto amount = [&](unsigned i, float v) { return cut.stays(mt_order_key(v), i) ? weights.kept(v, asked.least) : (mt_u64)0; };
     mt_u64 total = 0;
     each([&](unsigned i, float v) { total += amount(i, v); });
-    total = mt_group_fold<WAVES>(total, lds, sum);
+    total = mt_group_sum<WAVES>(total, lds);
     const mt_u64 target = asked.target(total);
     const double log_total = weights.log_of(total);
     mt_u64 seen = 0;
@@ -752,7 +787,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // ---------------------------------------------------------------------------
 
 constexpr unsigned MT_SAMPLE_WAVES = 4u, MT_SAMPLE_LANES = 256u;
-constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 8192u;
+constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 7168u;
 constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
 constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
 constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... by one wave, all of a list
@@ -765,49 +800,37 @@ struct mt_grid {
     MT_INLINE float bin(float x) const { return __builtin_floorf(x * by); }
 };
 
-// Calls f(index, x) for this lane's logits of the chunk from i0 on, 16 of them loaded at a
-// time; those of short chunks stay in registers for the next call.
-template <unsigned V, unsigned CHUNK, unsigned CS>
-struct mt_sample_chunk {
-    static constexpr unsigned QUADS = CHUNK / (4u * MT_SAMPLE_LANES);
-    static constexpr bool KEEP = QUADS <= 16u;
-    mt_f32x4 kept[KEEP ? QUADS : 4u];
-    const float* x;
-    unsigned i0;
-    MT_INLINE unsigned index(unsigned q) const { return i0 + 4u * (threadIdx.x + MT_SAMPLE_LANES * q); }
-    MT_INLINE mt_f32x4 load(unsigned q) const {
-        mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (index(q) < V) v = mt_row4<V, CS>(x, index(q));
+// Calls f(q, i, v) for this lane's quads of the chunk from i0 on, of which the q-th of all
+// lanes are 1024 neighbours: i is the first one's index, v the four, -inf behind the row's
+// end.  Four quads are loaded while the four before are looked at.
+template <unsigned V, unsigned CHUNK, unsigned CS, typename F>
+MT_INLINE void mt_sample_each(const float* x, unsigned i0, F f) {
+    constexpr unsigned QUADS = CHUNK / (4u * MT_SAMPLE_LANES);
+    static_assert(QUADS % 4u == 0u, "quads four at a time");
+    const auto index = [&](unsigned q) { return i0 + 4u * (threadIdx.x + MT_SAMPLE_LANES * q); };
+    const auto load = [&](unsigned q) {
+        mt_f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const unsigned i = index(q);
+        if (q < QUADS && i < V) {
+            v = mt_row4<V, CS>(x, i);
+#pragma unroll
+            for (unsigned j = 1; j < 4u; ++j)
+                if (V % 4u != 0u && i + j >= V) v[j] = -INFINITY;
+        }
         return v;
-    }
-    MT_INLINE mt_sample_chunk(const float* x_, unsigned i0_) : x(x_), i0(i0_) {
-        if constexpr (KEEP) {
+    };
+    mt_f32x4 next[4];
 #pragma unroll
-            for (unsigned q = 0; q < QUADS; ++q) kept[q] = load(q);
-        }
-    }
-    template <typename F>
-    MT_INLINE void each(F f) {
-        if constexpr (KEEP) {
-#pragma unroll
-            for (unsigned q = 0; q < QUADS; ++q)
-#pragma unroll
-                for (unsigned j = 0; j < 4u; ++j)
-                    if (index(q) + j < V) f(index(q) + j, kept[q][j]);
-        } else {
+    for (unsigned q = 0; q < 4u; ++q) next[q] = load(q);
 #pragma unroll 1
-            for (unsigned q0 = 0; q0 < QUADS; q0 += 4u) {
+    for (unsigned q0 = 0; q0 < QUADS; q0 += 4u) {
+        mt_f32x4 now[4];
 #pragma unroll
-                for (unsigned q = 0; q < 4u; ++q) kept[q] = load(q0 + q);
+        for (unsigned q = 0; q < 4u; ++q) now[q] = next[q], next[q] = load(q0 + 4u + q);
 #pragma unroll
-                for (unsigned q = 0; q < 4u; ++q)
-#pragma unroll
-                    for (unsigned j = 0; j < 4u; ++j)
-                        if (index(q0 + q) + j < V) f(index(q0 + q) + j, kept[q][j]);
-            }
-        }
+        for (unsigned q = 0; q < 4u; ++q) f(q0 + q, index(q0 + q), now[q]);
     }
-};
+}
 
 // best: [row][S]; bins: [row][S][MT_SAMPLE_BINS]; counts: [row][2], the row's arrivals and the
 // length of its list.
@@ -817,14 +840,17 @@ MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, co
     constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES;
     const unsigned row = blockIdx.x / S, part = blockIdx.x % S, t = threadIdx.x;
     if (part == 0u && t < 2u) counts[2u * row + t] = 0u;
-    mt_sample_chunk<V, CHUNK, CS> chunk(logits + (size_t)row * RS, part * CHUNK);
+    const float* x = logits + (size_t)row * RS;
     mt_u64* bins = lds + WAVES;
     if (CUT)
         for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins[b] = 0;
     mt_u64 best = 0;
-    chunk.each([&](unsigned i, float x) {
-        const mt_u64 found = mt_best(i, x);
-        best = found > best ? found : best;
+    mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned, unsigned i, mt_f32x4 v) {
+#pragma unroll
+        for (unsigned j = 0; j < 4u; ++j) {
+            const mt_u64 found = i + j < V ? mt_best(i + j, v[j]) : 0;
+            best = found > best ? found : best;
+        }
     });
     best = mt_group_fold<WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
     if (t == 0u) best_out[(size_t)row * S + part] = best;
@@ -834,12 +860,15 @@ MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, co
         if (!(temperature > 0.f) || !(by_p || by_k)) return;
         const mt_grid grid(temperature);
         const float first = grid.bin(mt_order_value((unsigned)(best >> 32)));
-        chunk.each([&](unsigned, float x) {
-            const float f = grid.bin(x), below = first - f;
-            if (below >= 0.f && below < (float)MT_SAMPLE_BINS) {
-                mt_u64 word = 1ull << MT_SAMPLE_COUNT_AT;
-                if (by_p) word += (unsigned)(__builtin_amdgcn_exp2f((x * grid.by - f) * (1.44269504f / 16.f)) * 1048576.f);
-                atomicAdd(bins + (unsigned)below, word);
+        mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned, unsigned, mt_f32x4 v) {
+#pragma unroll
+            for (unsigned j = 0; j < 4u; ++j) {
+                const float f = grid.bin(v[j]), below = first - f;
+                if (below >= 0.f && below < (float)MT_SAMPLE_BINS) {
+                    mt_u64 word = 1ull << MT_SAMPLE_COUNT_AT;
+                    if (by_p) word += (unsigned)(__builtin_amdgcn_exp2f((v[j] * grid.by - f) * (1.44269504f / 16.f)) * 1048576.f);
+                    atomicAdd(bins + (unsigned)below, word);
+                }
             }
         });
         __syncthreads();
@@ -914,7 +943,6 @@ template <unsigned SHIFT>
 MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& asked, const mt_weights<SHIFT>& weights,
                                unsigned row, int* tokens, float* logprobs, mt_u64* lds) {
     const unsigned t = mt_lane();
-    const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
     mt_u64 one[2], weight[2], before[2] = {0, 0};
     unsigned rank[2] = {0u, 0u};
     double w[2];
@@ -937,7 +965,7 @@ MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& a
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (asked.p < 1.f) {
-        const mt_u64 wanted = asked.weight_asked(mt_wave_fold(total, sum));
+        const mt_u64 wanted = asked.weight_asked(mt_wave_sum(total));
 #pragma unroll 4
         for (unsigned j = 0; j < n; ++j) {
             const mt_u64 other = list[j], more = lds[j];
@@ -955,7 +983,7 @@ MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& a
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (all have read the weights)
     lds[t] = weight[0], lds[t + 64u] = weight[1];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    total = mt_wave_fold(total, sum);
+    total = mt_wave_sum(total);
     const mt_u64 target = asked.target(total);
     const double log_total = weights.log_of(total);
 #pragma unroll 4
@@ -970,32 +998,30 @@ MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& a
             weights.answer(row, 0xFFFFFFFFu - (unsigned)one[d], mt_order_value((unsigned)(one[d] >> 32)), log_total, tokens, logprobs);
 }
 
-// sums: [row][S][3], all weights, those above the cut, and those of them that min_p leaves;
-// list: [row][MT_SAMPLE_LIST].
+// sums: [row][S][2], all weights and those above the cut, behind them for each row, the
+// weights that stay of each segment of 256; list: [row][MT_SAMPLE_LIST].
 template <unsigned V, unsigned CHUNK, unsigned S, unsigned SHIFT, unsigned RS, unsigned CS, bool CUT>
 MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const float* temperatures, const int* top_k,
                               const float* top_p, const float* min_p, const mt_u64* best_in, const mt_u64* bins_in,
                               unsigned* counts, mt_u64* sums, mt_u64* list, int* tokens, float* logprobs, mt_u64* lds) {
     constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES, EACH = MT_SAMPLE_BINS / LANES;
-    constexpr unsigned SPAN = CHUNK / LANES;  // neighbours of a chunk that a lane adds up
+    constexpr unsigned SEGMENTS = CHUNK / 256u, ROW = 2u * S + S * SEGMENTS;  // a chunk's, and the words of a row's sums
     const unsigned row = blockIdx.x / S, part = blockIdx.x % S, t = threadIdx.x;
     const float* x = logits + (size_t)row * RS;
-    const auto sum = [](mt_u64 a, mt_u64 b) { return a + b; };
     const auto put = [](mt_u64* to, mt_u64 value) { __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     const auto get = [](const mt_u64* from) {
         return __hip_atomic_load(const_cast<mt_u64*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
-    // LDS: the folds' words and some results, a word for each chunk and four more; for cuts,
+    // LDS: the folds' words and some results, four more, what stays of each segment; for cuts,
     // mt_list_cut's, and the list
-    mt_u64 *chunk_kept = lds + WAVES + 4u, *words = chunk_kept + S, *cut_lds = words + 4u;
+    mt_u64 *words = lds + WAVES + 4u, *kept = words + 4u, *cut_lds = kept + S * SEGMENTS;
     mt_u64* held = cut_lds + WAVES + 4u + MT_SAMPLE_PARTS + 2u * MT_SAMPLE_CLOSE;
     const mt_asked asked(row, uniforms, temperatures, top_k, top_p, min_p);
-    mt_sample_chunk<V, CHUNK, CS> chunk(x, part * CHUNK);
     mt_u64 best = 0;
     for (unsigned c = mt_lane(); c < S; c += 64u) {
         const mt_u64 one = best_in[(size_t)row * S + c];
         best = one > best ? one : best;
-        if (CUT && t < 64u) chunk_kept[c] = one;
+        if (CUT && t < 64u) kept[c] = one;
     }
     best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
     if (mt_sample_plain(best, asked.temperature, row, part == 0u && t == 0u, tokens, logprobs)) return;
@@ -1018,7 +1044,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             for (unsigned b = 0; b < EACH; ++b) number[b] = mass[b] = 0;
 #pragma unroll
             for (unsigned c = 0; c < S; ++c) {  // (loads that do not wait for each other)
-                const float shift = first - grid.bin(mt_order_value((unsigned)(chunk_kept[c] >> 32)));
+                const float shift = first - grid.bin(mt_order_value((unsigned)(kept[c] >> 32)));
                 const int by = shift >= 0.f && shift < (float)MT_SAMPLE_BINS ? (int)shift : (int)MT_SAMPLE_BINS;
 #pragma unroll
                 for (unsigned b = 0; b < EACH; ++b) {
@@ -1075,36 +1101,49 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     if (whole && part != 0u) return;  // (the same in all workgroups of the row)
     const bool cuts = from < MT_SAMPLE_BINS;
     if (!whole) {
-        mt_u64 all = 0, above = 0, kept = 0;
+        mt_u64 all = 0, above = 0;
         const bool weigh_all = by_p && !by_k;
-        chunk.each([&](unsigned i, float v) {
-            bool stays = true;
-            if (CUT && cuts) {
-                const float below = first - grid.bin(v);
-                stays = below < (float)from;
-                if (!stays && below <= (float)upto) {
-                    const unsigned to = (unsigned)atomicAdd(words + 3, 1ull);
-                    if (to < MT_SAMPLE_LIST) held[to] = mt_best(i, v);
+        mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned q, unsigned i, mt_f32x4 v) {
+            const float most = __builtin_fmaxf(__builtin_fmaxf(v[0], v[1]), __builtin_fmaxf(v[2], v[3]));
+            const float nearest = CUT ? first - grid.bin(most) : 0.f;
+            mt_u64 stay = 0;
+            if (!CUT || !cuts || weigh_all || nearest < (float)from) {
+#pragma unroll
+                for (unsigned j = 0; j < 4u; ++j) {
+                    const double w = weights.weight(v[j]);
+                    const mt_u64 h = weights.whole(w);
+                    all += h;
+                    if (!CUT || !cuts || first - grid.bin(v[j]) < (float)from) above += h, stay += w < asked.least ? 0 : h;
                 }
             }
-            if (stays || weigh_all) {
-                const double w = weights.weight(v);
-                const mt_u64 h = weights.whole(w);
-                all += h;
-                if (stays) above += h, kept += w < asked.least ? 0 : h;
+            if (CUT && cuts && nearest <= (float)upto) {
+#pragma unroll
+                for (unsigned j = 0; j < 4u; ++j) {
+                    const float below = first - grid.bin(v[j]);
+                    if (below >= (float)from && below <= (float)upto) {
+                        const unsigned to = (unsigned)atomicAdd(words + 3, 1ull);
+                        if (to < MT_SAMPLE_LIST) held[to] = mt_best(i + j, v[j]);
+                    }
+                }
+            }
+            if (from != 0u) {  // (else nothing stays before the list is looked at)
+                stay = mt_wave_upto(stay);
+                if (mt_lane() == 63u) kept[q * WAVES + mt_wave()] = stay;
             }
         });
-        if (from != 0u || weigh_all) {  // (else nothing stays before the list is looked at)
-            all = mt_wave_fold(all, sum), above = mt_wave_fold(above, sum), kept = mt_wave_fold(kept, sum);
-            if (mt_lane() == 0u) atomicAdd(words, all), atomicAdd(words + 1, above), atomicAdd(words + 2, kept);
+        if (weigh_all) {
+            all = mt_wave_sum(all), above = mt_wave_sum(above);
+            if (mt_lane() == 0u) atomicAdd(words, all), atomicAdd(words + 1, above);
         }
         __syncthreads();
         unsigned n = (unsigned)words[3];  // (at most LIST, as the bins said)
         n = n < MT_SAMPLE_LIST ? n : MT_SAMPLE_LIST;
         mt_u64 row_all = words[0], row_above = words[1];
         if constexpr (S > 1u) {
-            mt_u64* mine = sums + ((size_t)row * S + part) * 3u;
-            if (t < 3u) put(mine + t, words[t]);
+            mt_u64 *of = sums + (size_t)row * ROW, *segments = of + 2u * S;
+            if (weigh_all && t < 2u) put(of + 2u * part + t, words[t]);
+            if (from != 0u)
+                for (unsigned c = t; c < SEGMENTS; c += LANES) put(segments + part * SEGMENTS + c, kept[c]);
             if (CUT && n != 0u) {
                 __syncthreads();
                 if (t == 0u) words[3] = __hip_atomic_fetch_add(counts + 2u * row + 1u, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1117,21 +1156,20 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             if (t == 0u) words[3] = __hip_atomic_fetch_add(counts + 2u * row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (words[3] + 1u != S) return;
-            // the last workgroup of the row: what stays of each chunk, and the list
-            mt_u64 one_all = 0, one_above = 0;
-            for (unsigned c = mt_lane(); c < S; c += 64u) {
-                const mt_u64* of = sums + ((size_t)row * S + c) * 3u;
-                if (CUT && weigh_all) one_all += get(of), one_above += get(of + 1);
-                if (t < 64u) chunk_kept[c] = get(of + 2);
-            }
+            // the last workgroup of the row: what stays of each segment, and the list
+            for (unsigned c = t; c < S * SEGMENTS; c += LANES) kept[c] = from != 0u ? get(segments + c) : 0;
             if (CUT && cuts) {
                 n = __hip_atomic_load(counts + 2u * row + 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 n = n < MT_SAMPLE_LIST ? n : MT_SAMPLE_LIST;
                 for (unsigned l = t; l < n; l += LANES) held[l] = get(list + (size_t)row * MT_SAMPLE_LIST + l);
-                if (weigh_all) row_all = mt_wave_fold(one_all, sum), row_above = mt_wave_fold(one_above, sum);
+                if (weigh_all) {
+                    mt_u64 one_all = 0, one_above = 0;
+                    for (unsigned c = mt_lane(); c < S; c += 64u) one_all += get(of + 2u * c), one_above += get(of + 2u * c + 1u);
+                    row_all = mt_wave_sum(one_all), row_above = mt_wave_sum(one_above);
+                }
             }
-        } else {
-            if (t == 0u) chunk_kept[0] = words[2];
+        } else if (from == 0u) {
+            for (unsigned c = t; c < SEGMENTS; c += LANES) kept[c] = 0;
         }
         __syncthreads();
         if (CUT && by_k && from == 0u && n <= MT_SAMPLE_SHORT) {
@@ -1154,7 +1192,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
                 if (by_k) {
                     mt_u64 total = 0;
                     for (unsigned l = t; l < n; l += LANES) total += stays(held[l]) ? weights.held(value(held[l])) : 0;
-                    row_all = mt_group_fold<WAVES>(total, lds, sum), row_above = 0;
+                    row_all = mt_group_sum<WAVES>(total, lds), row_above = 0;
                 }
                 const mt_u64 wanted = asked.weight_asked(row_all);
                 const mt_cut_at by = cut;
@@ -1166,50 +1204,39 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             for (unsigned l = t; l < n; l += LANES)
                 if (stays(held[l])) {
                     const mt_u64 h = weights.kept(value(held[l]), asked.least);
-                    if (h != 0) atomicAdd(chunk_kept + (0xFFFFFFFFu - (unsigned)held[l]) / CHUNK, h);
+                    if (h != 0) atomicAdd(kept + (0xFFFFFFFFu - (unsigned)held[l]) / 256u, h);
                 }
             __syncthreads();
         }
         if (!whole) {
-            // The chunk that the random number falls into, the lane's neighbours in it, the token.
-            mt_u64 total = 0, before = 0, every;
-            for (unsigned c = 0; c < S; ++c) total += chunk_kept[c];
+            // The segment that the random number falls into, and the token in it.
+            constexpr unsigned PER = (S * SEGMENTS + LANES - 1u) / LANES;
+            mt_u64 mine = 0, total;
+            for (unsigned c = t * PER; c < (t + 1u) * PER && c < S * SEGMENTS; ++c) mine += kept[c];
+            mt_u64 before = mt_group_before<WAVES>(mine, lds, total);
             const mt_u64 target = asked.target(total);
-            unsigned in = 0u;
-            while (in + 1u < S && before + chunk_kept[in] <= target) before += chunk_kept[in], ++in;
-            const auto amount = [&](unsigned i, float v) {
-                return i < V && cut.stays(mt_order_key(v), i) ? weights.kept(v, asked.least) : (mt_u64)0;
-            };
-            const unsigned l0 = in * CHUNK + t * SPAN;
-            mt_u64 lane_all = 0;
-#pragma unroll 4
-            for (unsigned e = 0; e < SPAN; e += 4u) {
-                if (l0 + e >= V) break;
-                const mt_f32x4 v = mt_row4<V, CS>(x, l0 + e);
-#pragma unroll
-                for (unsigned j = 0; j < 4u; ++j) lane_all += amount(l0 + e + j, v[j]);
+            if (before <= target && target < before + mine) {
+                unsigned c = t * PER;
+                while (before + kept[c] <= target) before += kept[c++];
+                words[0] = c, words[1] = before;
             }
-            before += mt_group_before<WAVES>(lane_all, lds, every);
-            if (before <= target && target < before + lane_all) words[0] = l0, words[1] = before;
             __syncthreads();
             if (t >= 64u) return;
+            const unsigned i = (unsigned)words[0] * 256u + 4u * t;
             before = words[1];
-            const double log_total = weights.log_of(total);
-#pragma unroll 1
-            for (unsigned e = 0; e < SPAN; e += 64u) {
-                const unsigned i = (unsigned)words[0] + e + t;
-                const float v = e + t < SPAN && i < V ? x[(size_t)i * CS] : -INFINITY;
-                const mt_u64 w = e + t < SPAN ? amount(i, v) : 0;
-                mt_u64 upto_here = w;
+            mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if (i < V) v = mt_row4<V, CS>(x, i);
+            double log_total = weights.log_of(total);
+            asm volatile("" : "+v"(log_total));  // (here, while the load is on its way)
+            mt_u64 w[4];
 #pragma unroll
-                for (unsigned off = 1u; off < 64u; off *= 2u) {
-                    const mt_u64 other = __shfl_up(upto_here, off, 64);
-                    if (t >= off) upto_here += other;
-                }
-                if (before + upto_here - w <= target && target < before + upto_here)
-                    weights.answer(row, i, v, log_total, tokens, logprobs);
-                before += (mt_u64)__shfl(upto_here, 63, 64);
-                if (before > target) break;
+            for (unsigned j = 0; j < 4u; ++j)
+                w[j] = i + j < V && cut.stays(mt_order_key(v[j]), i + j) ? weights.kept(v[j], asked.least) : 0;
+            before += mt_wave_upto(w[0] + w[1] + w[2] + w[3]) - (w[0] + w[1] + w[2] + w[3]);
+#pragma unroll
+            for (unsigned j = 0; j < 4u; ++j) {
+                if (before <= target && target < before + w[j]) weights.answer(row, i + j, v[j], log_total, tokens, logprobs);
+                before += w[j];
             }
             return;
         }

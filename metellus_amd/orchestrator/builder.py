@@ -617,7 +617,7 @@ class Operations:
         if len(tl.shape) != 2:
             raise ValueError(f"sample logits must be 2D; got shape {tl.shape} ({tl.name!r})")
         rows, cols = tl.shape
-        _, chunks = sample_chunks(rows, cols)
+        chunk, chunks = sample_chunks(rows, cols)
         cuts = top_k is not None or top_p is not None
 
         def made(part: str, rows: int, words: int) -> Tensor:
@@ -639,7 +639,7 @@ class Operations:
             best=scan.best,
             counts=scan.counts,
             bins=scan.bins,
-            sums=made("sums", rows * chunks, 3),
+            sums=made("sums", rows, (2 + chunk // 256) * chunks),
             listed=made("list", rows, SAMPLE_LIST) if cuts else None,
             logprobs=None if logprobs is None else self._fresh(logprobs, (rows,), "float32"),
             after=self._owners(tl, tu, *given.values()),

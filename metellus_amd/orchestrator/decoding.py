@@ -31,7 +31,7 @@ POSITIONS_MAX = _INT32_MAX - 1024  # of a table's row (its positions and a step'
 ADAPTER_RANK_MAX = 256
 VOCABULARY_MAX = 2**20
 SAMPLE_CHUNK = 4096  # logits, and the smallest share of a workgroup
-SAMPLE_BINS, SAMPLE_LIST = 512, 8192  # of a chunk; logits that a row has listed at most
+SAMPLE_BINS, SAMPLE_LIST = 512, 7168  # of a chunk; logits that a row has listed at most
 
 # pi to 64 digits: 2 pi has to outlast a double's 53 bits twice
 _PI = Decimal("3.141592653589793238462643383279502884197169399375105820974944592")
