@@ -790,7 +790,7 @@ constexpr unsigned MT_SAMPLE_WAVES = 4u, MT_SAMPLE_LANES = 256u;
 constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 7168u;
 constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
 constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
-constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... by one wave, all of a list
+constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... all of a list, for both cuts and the token
 constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
 
 // The bin of x on the grid of a temperature.
@@ -936,66 +936,47 @@ MT_INLINE bool mt_list_cut(const mt_u64* list, unsigned n, AMOUNT amount, PLACE 
     return found[3] != 0;
 }
 
-// A cut by k, one by p if asked, and the token, by one wave, of a list of at most two entries
-// a lane that has everything that may stay: entries are ranked by comparing each with all, the weights
-// before a rank or an index found by adding up those that compare so.  `lds`: 128 words.
+// A cut by k, one by p if asked, and the token, of a list of up to 128 that has everything
+// that may stay: each entry is compared with all, half of them by one lane and half by
+// another, and the weights of those that are larger, or have an earlier index, added up.
+// `lds`: WAVES words, and twice 128.
 template <unsigned SHIFT>
 MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& asked, const mt_weights<SHIFT>& weights,
                                unsigned row, int* tokens, float* logprobs, mt_u64* lds) {
-    const unsigned t = mt_lane();
-    mt_u64 one[2], weight[2], before[2] = {0, 0};
-    unsigned rank[2] = {0u, 0u};
-    double w[2];
-#pragma unroll
-    for (unsigned d = 0; d < 2u; ++d) {
-        one[d] = t + 64u * d < n ? list[t + 64u * d] : 0;
-        w[d] = weights.weight(mt_order_value((unsigned)(one[d] >> 32)));
-    }
+    constexpr unsigned WAVES = MT_SAMPLE_WAVES, MOST = MT_SAMPLE_SHORT;
+    static_assert(MT_SAMPLE_LANES == 2u * MOST, "two lanes to an entry");
+    const unsigned l = threadIdx.x % MOST, half = threadIdx.x / MOST;
+    const unsigned begin = half ? n / 2u : 0u, end = half ? n : n / 2u;
+    mt_u64 *other = lds + WAVES, *amount = other + MOST;
+    const mt_u64 one = l < n ? list[l] : 0;
+    const double w = weights.weight(mt_order_value((unsigned)(one >> 32)));
+    // the sum over the entries j of which more(j) tells, in the lanes of the first half
+    const auto before = [&](auto more) {
+        mt_u64 sum = 0;
 #pragma unroll 4
-    for (unsigned j = 0; j < n; ++j) {
-        const mt_u64 other = list[j];
-        rank[0] += other > one[0] ? 1u : 0u, rank[1] += other > one[1] ? 1u : 0u;
-    }
-    mt_u64 total = 0;
-#pragma unroll
-    for (unsigned d = 0; d < 2u; ++d) {
-        weight[d] = one[d] != 0 && rank[d] < (unsigned)asked.k ? weights.whole(w[d]) : 0;
-        lds[t + 64u * d] = weight[d];
-        total += weight[d];
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (unsigned j = begin; j < end; ++j) sum += more(j);
+        __syncthreads();
+        if (half) other[l] = sum;
+        __syncthreads();
+        return half ? 0 : sum + other[l];
+    };
+    const mt_u64 rank = before([&](unsigned j) { return (mt_u64)(list[j] > one ? 1 : 0); });
+    mt_u64 weight = !half && one != 0 && rank < (mt_u64)asked.k ? weights.whole(w) : 0;
     if (asked.p < 1.f) {
-        const mt_u64 wanted = asked.weight_asked(mt_wave_sum(total));
-#pragma unroll 4
-        for (unsigned j = 0; j < n; ++j) {
-            const mt_u64 other = list[j], more = lds[j];
-            before[0] += other > one[0] ? more : 0, before[1] += other > one[1] ? more : 0;
-        }
-        weight[0] = before[0] < wanted ? weight[0] : 0, weight[1] = before[1] < wanted ? weight[1] : 0;
+        if (!half) amount[l] = weight;
+        const mt_u64 wanted = asked.weight_asked(mt_group_sum<WAVES>(weight, lds));
+        const mt_u64 larger = before([&](unsigned j) { return list[j] > one ? amount[j] : 0; });
+        if (!(larger < wanted)) weight = 0;
     }
-    total = 0;
-#pragma unroll
-    for (unsigned d = 0; d < 2u; ++d) {
-        if (w[d] < asked.least) weight[d] = 0;
-        total += weight[d];
-        before[d] = 0;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (all have read the weights)
-    lds[t] = weight[0], lds[t + 64u] = weight[1];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    total = mt_wave_sum(total);
-    const mt_u64 target = asked.target(total);
+    if (w < asked.least) weight = 0;
+    __syncthreads();
+    if (!half) amount[l] = weight;
+    const mt_u64 total = mt_group_sum<WAVES>(weight, lds), target = asked.target(total);
     const double log_total = weights.log_of(total);
-#pragma unroll 4
-    for (unsigned j = 0; j < n; ++j) {
-        const mt_u64 more = lds[j];
-        const unsigned other = (unsigned)list[j];  // (upside down: larger is an earlier index)
-        before[0] += other > (unsigned)one[0] ? more : 0, before[1] += other > (unsigned)one[1] ? more : 0;
-    }
-#pragma unroll
-    for (unsigned d = 0; d < 2u; ++d)
-        if (before[d] <= target && target < before[d] + weight[d])
-            weights.answer(row, 0xFFFFFFFFu - (unsigned)one[d], mt_order_value((unsigned)(one[d] >> 32)), log_total, tokens, logprobs);
+    // (the index is upside down: larger is earlier)
+    const mt_u64 earlier = before([&](unsigned j) { return (unsigned)list[j] > (unsigned)one ? amount[j] : 0; });
+    if (earlier <= target && target < earlier + weight)
+        weights.answer(row, 0xFFFFFFFFu - (unsigned)one, mt_order_value((unsigned)(one >> 32)), log_total, tokens, logprobs);
 }
 
 // sums: [row][S][2], all weights and those above the cut, behind them for each row, the
@@ -1173,7 +1154,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
         }
         __syncthreads();
         if (CUT && by_k && from == 0u && n <= MT_SAMPLE_SHORT) {
-            if (t < 64u) mt_sample_short<SHIFT>(held, n, asked, weights, row, tokens, logprobs, cut_lds);
+            mt_sample_short<SHIFT>(held, n, asked, weights, row, tokens, logprobs, cut_lds);
             return;
         }
         mt_cut_at cut{0u, 0xFFFFFFFFu};
