@@ -211,8 +211,7 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // four neighbours of row m = n of `down` or `out`.
 // ---------------------------------------------------------------------------
 
-// Tiles and the rows that lead their groups.  Workgroups in turn go to the GPU's eight
-// parts in turn, so tiles, not leaders, are next to each other: few of a tile's rows lead.
+// The rows of a tile, and the groups that they lead.
 template <unsigned MB, unsigned HELD>
 struct mt_adapter_rows {
     static constexpr unsigned TILE = 16u * MB;
@@ -241,69 +240,128 @@ MT_INLINE mt_f32x4 mt_mfma16_f32(mt_f32x4 a, mt_f32x4 b, mt_f32x4 c) {
     return c;
 }
 
-// The tile of a workgroup.  LOOP: the GPU's eight parts, which take workgroups in turn, have
-// neighbouring tiles each, whose rows are likely to share adapters; there are eight times
-// a whole number of workgroups then, and the last may have no tile.
+// A workgroup's tile and its share of the columns (blockIdx.x; blockIdx.y is the row of the
+// tile that may lead, so that those of first rows, which all do, go first).  LOOP: the GPU's
+// eight parts, which take workgroups in turn, have neighbouring tiles each, whose rows are
+// likely to share adapters; there are eight times a whole number of tiles then, and the
+// last may not be there.
 template <bool LOOP>
-MT_INLINE unsigned mt_adapter_tile(unsigned tiles) {
-    return LOOP ? blockIdx.x % 8u * (gridDim.x / 8u) + blockIdx.x / 8u : blockIdx.x % tiles;
+struct mt_adapter_place {
+    unsigned tile, share;
+    MT_INLINE explicit mt_adapter_place(unsigned tiles) {
+        const unsigned around = LOOP ? (tiles + 7u) / 8u * 8u : tiles, at = blockIdx.x % around;
+        tile = LOOP ? at % 8u * (around / 8u) + at / 8u : at;
+        share = blockIdx.x / around;
+    }
+};
+
+// Elements c .. c + 3 of a row of COLS elements CS apart, 0 behind its end, without a branch.
+// (MFMAs take all lanes' registers, whichever lanes are at them: lanes that may part on their
+// way through a loop of MFMAs, at a condition of their own that the compiler knows from the
+// round before, must not.)
+template <unsigned COLS, unsigned CS>
+MT_INLINE mt_f32x4 mt_quad(const float* row, unsigned c) {
+    mt_f32x4 v;
+    if constexpr (CS == 1u && COLS >= 4u) {
+        const unsigned at = c < COLS - 4u ? c : COLS - 4u, by = c - at;
+        const mt_f32x4 w = mt_ld4u(row + at);
+        if constexpr (COLS % 4u == 0u) {
+#pragma unroll
+            for (unsigned j = 0; j < 4u; ++j) v[j] = by == 0u ? w[j] : 0.f;
+        } else {
+            v[0] = by == 0u ? w[0] : by == 1u ? w[1] : by == 2u ? w[2] : by == 3u ? w[3] : 0.f;
+            v[1] = by == 0u ? w[1] : by == 1u ? w[2] : by == 2u ? w[3] : 0.f;
+            v[2] = by == 0u ? w[2] : by == 1u ? w[3] : 0.f;
+            v[3] = by == 0u ? w[3] : 0.f;
+        }
+    } else {
+#pragma unroll
+        for (unsigned j = 0; j < 4u; ++j) {
+            const float one = row[(size_t)(c + j < COLS ? c + j : COLS - 1u) * CS];
+            v[j] = c + j < COLS ? one : 0.f;
+        }
+    }
+    return v;
+}
+// All four in the row.
+template <unsigned CS>
+MT_INLINE mt_f32x4 mt_quad_in(const float* row, unsigned c) {
+    if constexpr (CS == 1u) return mt_ld4u(row + c);
+    return mt_f32x4{row[(size_t)c * CS], row[(size_t)(c + 1u) * CS], row[(size_t)(c + 2u) * CS], row[(size_t)(c + 3u) * CS]};
 }
 
 // A's part: blocks of RB x 16 ranks; the waves of the SPLITS workgroups of a group take
 // 64 columns of x in turn and add up in LDS; each split stores its part.  Loads of 16
 // columns go out as the registers of those 64 before are free, so MFMAs and memory go on
-// together.
+// together.  Lanes of rows of other groups load the leader's, which are loaded anyway.
 template <unsigned K, unsigned R, unsigned RB, unsigned MB, bool LOOP, unsigned SPLITS, unsigned HELD, unsigned WAVES,
           unsigned XRS, unsigned XCS>
 MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, float* down, unsigned rows,
                                mt_f32x4* lds) {
-    constexpr unsigned TILE = 16u * MB;
-    const unsigned tiles = (rows + TILE - 1u) / TILE, split = blockIdx.y % SPLITS, r0 = blockIdx.y / SPLITS * RB * 16u;
-    const unsigned lane = mt_lane(), n = lane & 15u, g = lane >> 4, at = mt_adapter_tile<LOOP>(tiles);
-    if (at >= tiles) return;
-    const mt_adapter_rows<MB, HELD> tile(ids, at, rows);
+    constexpr unsigned TILE = 16u * MB, STEP = 64u * SPLITS * WAVES, WHOLE = K / 64u * 64u;
+    const unsigned tiles = (rows + TILE - 1u) / TILE, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
+    const mt_adapter_place<LOOP> at(tiles);
+    const unsigned split = at.share % SPLITS, r0 = at.share / SPLITS * RB * 16u;
+    if (at.tile >= tiles) return;
+    const mt_adapter_rows<MB, HELD> tile(ids, at.tile, rows);
 #pragma unroll 1
-    for (unsigned j = LOOP ? 0u : blockIdx.x / tiles; j < TILE; ++j) {
+    for (unsigned j = blockIdx.y; j < TILE; ++j) {
         int id;
         const unsigned long long group = tile.group(j, id);
         if (group != 0ull && id >= 0) {
-            const float* ar = a + ((size_t)(unsigned)id * R + r0 + n) * K;
+            const float *xr[MB], *ar[RB];
             mt_f32x4 acc[MB][RB], xv[4][MB], av[4][RB];
 #pragma unroll
-            for (unsigned m = 0; m < MB; ++m)
+            for (unsigned m = 0; m < MB; ++m) {
+                const unsigned row = (group >> (16u * m + n)) & 1ull ? 16u * m + n : j;
+                xr[m] = x + (size_t)(tile.row0 + row) * XRS;
 #pragma unroll
                 for (unsigned b = 0; b < RB; ++b) acc[m][b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (unsigned b = 0; b < RB; ++b) {
+                const unsigned r = r0 + 16u * b + n;
+                ar[b] = a + ((size_t)(unsigned)id * R + (r < R ? r : R - 1u)) * K;
+            }
             const auto load = [&](unsigned k0, unsigned u) {
                 const unsigned k = k0 + 16u * u + 4u * g;
 #pragma unroll
-                for (unsigned m = 0; m < MB; ++m) {
-                    xv[u][m] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (((group >> (16u * m + n)) & 1ull) && (K % 64u == 0u || k < K))
-                        xv[u][m] = mt_row4<K, XCS>(x + (size_t)(tile.row0 + 16u * m + n) * XRS, k);
-                }
+                for (unsigned m = 0; m < MB; ++m) xv[u][m] = mt_quad_in<XCS>(xr[m], k);
 #pragma unroll
-                for (unsigned b = 0; b < RB; ++b) {
-                    av[u][b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-                    if ((R % 16u == 0u && RB * 16u >= R || r0 + 16u * b + n < R) && (K % 64u == 0u || k < K))
-                        av[u][b] = mt_row4<K, 1u>(ar + (size_t)(16u * b) * K, k);
-                }
+                for (unsigned b = 0; b < RB; ++b) av[u][b] = mt_quad_in<1u>(ar[b], k);
+            };
+            const auto multiply = [&](unsigned u) {
+#pragma unroll
+                for (unsigned m = 0; m < MB; ++m)
+                    if (MB == 1u || ((group >> (16u * m)) & 0xFFFFull))  // (a block with rows of the group)
+#pragma unroll
+                        for (unsigned b = 0; b < RB; ++b) acc[m][b] = mt_mfma16_f32(av[u][b], xv[u][m], acc[m][b]);
             };
             unsigned k0 = 64u * (split * WAVES + mt_wave());
-            if (k0 < K) {
+            if (k0 < WHOLE) {
 #pragma unroll
                 for (unsigned u = 0; u < 4u; ++u) load(k0, u);
+#pragma unroll 1
+                for (; k0 + STEP < WHOLE; k0 += STEP) {
+#pragma unroll
+                    for (unsigned u = 0; u < 4u; ++u) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        multiply(u);
+                        load(k0 + STEP, u);
+                    }
+                }
+#pragma unroll
+                for (unsigned u = 0; u < 4u; ++u) multiply(u);
             }
-            for (; k0 < K; k0 += 64u * SPLITS * WAVES) {
-                const unsigned next = k0 + 64u * SPLITS * WAVES;
+            if (WHOLE != K && WHOLE / 64u % (SPLITS * WAVES) == split * WAVES + mt_wave()) {  // the last columns
 #pragma unroll
                 for (unsigned u = 0; u < 4u; ++u) {
-                    __builtin_amdgcn_sched_barrier(0);
+                    const unsigned k = WHOLE + 16u * u + 4u * g;
 #pragma unroll
-                    for (unsigned m = 0; m < MB; ++m)
-                        if (MB == 1u || ((group >> (16u * m)) & 0xFFFFull))
+                    for (unsigned m = 0; m < MB; ++m) xv[u][m] = mt_quad<K, XCS>(xr[m], k);
 #pragma unroll
-                            for (unsigned b = 0; b < RB; ++b) acc[m][b] = mt_mfma16_f32(av[u][b], xv[u][m], acc[m][b]);
-                    if (next < K) load(next, u);
+                    for (unsigned b = 0; b < RB; ++b) av[u][b] = mt_quad<K, 1u>(ar[b], k);
+                    multiply(u);
                 }
             }
             if (LOOP) __syncthreads();  // (the group before has been added up)
@@ -343,29 +401,35 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
     constexpr unsigned RC = (R + 15u) / 16u, TILE = 16u * MB, PITCH = 16u * RC + 4u;
     static_assert(PER % AHEAD == 0u, "blocks in whole sets");
     const unsigned tiles = (rows + TILE - 1u) / TILE, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
-    const unsigned n0 = (blockIdx.y * WAVES + mt_wave()) * PER * 16u, at = mt_adapter_tile<LOOP>(tiles);
-    if (at >= tiles) return;
-    const mt_adapter_rows<MB, HELD> tile(ids, at, rows);
+    const mt_adapter_place<LOOP> at(tiles);
+    const unsigned n0 = (at.share * WAVES + mt_wave()) * PER * 16u;
+    if (at.tile >= tiles) return;
+    const mt_adapter_rows<MB, HELD> tile(ids, at.tile, rows);
 #pragma unroll 1
-    for (unsigned j = LOOP ? 0u : blockIdx.x / tiles; j < TILE; ++j) {
+    for (unsigned j = blockIdx.y; j < TILE; ++j) {
         int id;
         const unsigned long long group = tile.group(j, id);
         if (group != 0ull) {
+            const float* yr[MB];
             mt_f32x4 bv[AHEAD][RC], v[AHEAD][MB], t[MB][RC];
-            const auto load = [&](unsigned from, unsigned p) {
-                const float* br = b + ((size_t)(unsigned)(id < 0 ? 0 : id) * N + from + n) * R;
 #pragma unroll
-                for (unsigned c = 0; c < RC; ++c) {
-                    bv[p][c] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (id >= 0 && (N % 16u == 0u || from + n < N) && (R % 16u == 0u || 16u * c + 4u * g < R))
-                        bv[p][c] = mt_row4<R, 1u>(br, 16u * c + 4u * g);
-                }
+            for (unsigned m = 0; m < MB; ++m) {
+                const unsigned row = (group >> (16u * m + n)) & 1ull ? 16u * m + n : j;
+                yr[m] = base + (size_t)(tile.row0 + row) * YRS;
+            }
+            // (n0, and so the block, is the same in all lanes of a wave)
+            const auto load = [&](unsigned from, unsigned p) {
                 const unsigned col = from + 4u * g;
+                if (id >= 0) {
+                    const float* br = b + ((size_t)(unsigned)id * N + (from + n < N ? from + n : N - 1u)) * R;
+#pragma unroll
+                    for (unsigned c = 0; c < RC; ++c)
+                        bv[p][c] = 16u * c + 16u <= R ? mt_quad_in<1u>(br, 16u * c + 4u * g) : mt_quad<R, 1u>(br, 16u * c + 4u * g);
+                }
 #pragma unroll
                 for (unsigned m = 0; m < MB; ++m) {
-                    v[p][m] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
-                    if (((group >> (16u * m + n)) & 1ull) && (N % 16u == 0u || col < N))
-                        v[p][m] = mt_row4<N, YCS>(base + (size_t)(tile.row0 + 16u * m + n) * YRS, col);
+                    if (from + 16u <= N) v[p][m] = mt_quad_in<YCS>(yr[m], col);
+                    else v[p][m] = mt_quad<N, YCS>(yr[m], col);
                 }
             };
 #pragma unroll
@@ -401,11 +465,10 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
                 }
             const float scale = scales != nullptr && id >= 0 ? scales[id] : 1.f;
 #pragma unroll 1
-            for (unsigned p0 = 0; p0 < PER; p0 += AHEAD) {
+            for (unsigned p0 = 0; p0 < PER && n0 + 16u * p0 < N; p0 += AHEAD) {
 #pragma unroll
                 for (unsigned p = 0; p < AHEAD; ++p) {
                     const unsigned from = n0 + 16u * (p0 + p), col = from + 4u * g;
-                    if (from >= N) break;
 #pragma unroll
                     for (unsigned m = 0; m < MB; ++m) {
                         if (MB > 1u && !((group >> (16u * m)) & 0xFFFFull)) continue;
@@ -416,8 +479,9 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
 #pragma unroll
                             for (unsigned i = 0; i < 4u; ++i) v[p][m][i] = __builtin_fmaf(scale, acc[i], v[p][m][i]);
                         }
-                        if (((group >> (16u * m + n)) & 1ull) && (N % 16u == 0u || col < N))
-                            mt_put_row4<N>(out + (size_t)(tile.row0 + 16u * m + n) * N, col, v[p][m]);
+                        unsigned stores = ((group >> (16u * m + n)) & 1ull) && col < N;
+                        asm volatile("" : "+v"(stores));  // (known to no other round)
+                        if (stores) mt_put_row4<N>(out + (size_t)(tile.row0 + 16u * m + n) * N, col, v[p][m]);
                     }
                     if (p0 + p + AHEAD < PER && from + 16u * AHEAD < N) load(from + 16u * AHEAD, p);
                     __builtin_amdgcn_sched_barrier(0);

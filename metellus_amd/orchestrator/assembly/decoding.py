@@ -141,9 +141,9 @@ def adapter_tile(rows: int, rank: int) -> tuple[int, bool]:
     return (4 if many and rank <= 64 else 1), many
 
 
-def _adapter_workgroups(rows: int, tile: int, loop: bool) -> int:
+def _adapter_grid(rows: int, tile: int, loop: bool, shares: int) -> tuple[int, int, int]:
     tiles = _ceil(rows, 16 * tile)
-    return 8 * _ceil(tiles, 8) if loop else 16 * tile * tiles
+    return (8 * _ceil(tiles, 8) * shares, 1, 1) if loop else (tiles * shares, 16 * tile, 1)
 
 
 def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_name: str | None) -> KernelGroup:
@@ -161,7 +161,7 @@ def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_n
         lds_bytes=waves * tile * blocks * 1024,
         name="adapter_down",
     )
-    grid = (_adapter_workgroups(rows, tile, loop), op.splits * _ceil(op.rank, 16 * blocks), 1)
+    grid = _adapter_grid(rows, tile, loop, op.splits * _ceil(op.rank, 16 * blocks))
     return _group(decision, sig, frag, function_name or f"adapter_down_{op.name}", {"M": rows}, grid, 64 * waves,
                   headers=(decoding_header(),))
 
@@ -189,7 +189,7 @@ def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name:
         lds_bytes=64 * tile * (16 * _ceil(op.rank, 16) + 4) if tile > 1 else 0,
         name="adapter_up",
     )
-    grid = (_adapter_workgroups(rows, tile, loop), _ceil(cols, 16 * waves * per), 1)
+    grid = _adapter_grid(rows, tile, loop, _ceil(cols, 16 * waves * per))
     return _group(decision, sig, frag, function_name or f"adapter_up_{op.y.name}", {"M": rows}, grid, 64 * waves,
                   headers=(decoding_header(),))
 

@@ -129,10 +129,12 @@ ADAPTER_DOWN_WAVES = (4, 8)  # a workgroup's for fewer rows, and for so many
 
 def adapter_splits(rows: int, inner: int) -> int:
     """Shares of x's columns that workgroups take apart, where rows alone are too few
-    workgroups to fill the GPU: at least as many columns as its waves take at once."""
-    many = rows >= ADAPTER_MANY_ROWS
-    wanted = -(-256 // -(-rows // 64)) if many else 512 // rows
-    return max(1, min(-(-inner // (64 * ADAPTER_DOWN_WAVES[many])), wanted))
+    workgroups to fill the GPU: of 512 columns at least, and not so many that adding them
+    up takes longer (us: 1 row of 4096 columns, rank 16, whole 17, in 4 9.4, 8 9.6; 32 rows 30,
+    13.4, 12.3, in 16 12.8; 77 of 5003, rank 23, 37, 21, 18, 20; 8 of 11008, rank 64, in 8
+    23, 12 20, 20 32)."""
+    wanted = -(-256 // -(-rows // 64)) if rows >= ADAPTER_MANY_ROWS else min(12, 2048 // rows)
+    return max(1, min(-(-inner // 512), wanted))
 
 
 # ---------------------------------------------------------------------------

@@ -228,12 +228,12 @@ def test_scheduling_adapters():
 
 
 def test_shares_of_columns():
-    assert adapter_splits(1, 4096) == 16 and adapter_splits(1, 100) == 1
-    assert adapter_splits(32, 4096) == 16 and adapter_splits(4096, 4096) == 4 and adapter_splits(600, 4096) == 1
+    assert adapter_splits(1, 4096) == 8 and adapter_splits(1, 100) == 1 and adapter_splits(8, 11008) == 12
+    assert adapter_splits(32, 4096) == 8 and adapter_splits(4096, 4096) == 4 and adapter_splits(600, 4096) == 3
     assert adapter_splits(16384, 4096) == 1
     for rows in (1, 3, 50, 700, 1024, 5000):
-        for inner in (1, 255, 257, 5003, 16384):
-            assert 1 <= adapter_splits(rows, inner) <= -(-inner // 256)
+        for inner in (1, 511, 513, 5003, 16384):
+            assert 1 <= adapter_splits(rows, inner) <= -(-inner // 512)
 
 
 # -- a rotation's frequencies --------------------------------------------------------

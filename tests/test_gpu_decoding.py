@@ -259,6 +259,7 @@ def _adapter_check(ops):
     (1, 1, 1, 1, 1), (1, 64, 16, 4, 2), (1, 4096, 300, 16, 3), (2, 100, 17, 8, 5), (7, 333, 129, 23, 4), (16, 512, 256, 16, 16),
     (17, 1000, 1003, 64, 3), (33, 257, 65, 5, 40), (100, 640, 1024, 65, 7), (3, 129, 260, 256, 2), (600, 96, 48, 12, 9),
     (1024, 1500, 100, 16, 5), (1100, 70, 33, 64, 3), (1061, 600, 70, 70, 200),
+    (5, 11008, 50, 20, 3), (40, 7003, 90, 33, 3), (1100, 6001, 500, 33, 2), (2050, 2048, 64, 100, 4), (3, 3, 3, 2, 2),
 ])
 @pytest.mark.parametrize("scales", [False, True])
 def test_adapters(rows, inner, cols, rank, held, scales):
