@@ -846,15 +846,16 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // hundreds of logits that are next to equal at the cut, a cut by p next to a bin's edge,
 // logits so large that the grid has no bin for them -- are drawn from by one workgroup.
 //
-// Workgroups are of four waves: the steps from the bins to the token follow each other, all
-// waves take them, and with more of them a compute unit takes turns.
+// The list takes half a compute unit's LDS, so there are two workgroups on each, of eight
+// waves (us, 64 rows of 131072 cut by p: eight waves, 512 workgroups 43, 1024 55, four waves
+// 64; one row 18, 17, 20; 64 rows cut by k 25, 39, 35).
 // ---------------------------------------------------------------------------
 
-constexpr unsigned MT_SAMPLE_WAVES = 4u, MT_SAMPLE_LANES = 256u;
+constexpr unsigned MT_SAMPLE_WAVES = 8u, MT_SAMPLE_LANES = 512u;
 constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 7168u;
 constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
 constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
-constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... all of a list, for both cuts and the token
+constexpr unsigned MT_SAMPLE_SHORT = 256u;   // ... all of a list, for both cuts and the token
 constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
 
 // The bin of x on the grid of a temperature.
@@ -870,7 +871,8 @@ struct mt_grid {
 template <unsigned V, unsigned CHUNK, unsigned CS, typename F>
 MT_INLINE void mt_sample_each(const float* x, unsigned i0, F f) {
     constexpr unsigned QUADS = CHUNK / (4u * MT_SAMPLE_LANES);
-    static_assert(QUADS % 4u == 0u, "quads four at a time");
+    constexpr unsigned DEEP = QUADS < 4u ? QUADS : 4u;
+    static_assert(QUADS % DEEP == 0u, "whole sets of quads");
     const auto index = [&](unsigned q) { return i0 + 4u * (threadIdx.x + MT_SAMPLE_LANES * q); };
     const auto load = [&](unsigned q) {
         mt_f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -883,16 +885,16 @@ MT_INLINE void mt_sample_each(const float* x, unsigned i0, F f) {
         }
         return v;
     };
-    mt_f32x4 next[4];
+    mt_f32x4 next[DEEP];
 #pragma unroll
-    for (unsigned q = 0; q < 4u; ++q) next[q] = load(q);
+    for (unsigned q = 0; q < DEEP; ++q) next[q] = load(q);
 #pragma unroll 1
-    for (unsigned q0 = 0; q0 < QUADS; q0 += 4u) {
-        mt_f32x4 now[4];
+    for (unsigned q0 = 0; q0 < QUADS; q0 += DEEP) {
+        mt_f32x4 now[DEEP];
 #pragma unroll
-        for (unsigned q = 0; q < 4u; ++q) now[q] = next[q], next[q] = load(q0 + 4u + q);
+        for (unsigned q = 0; q < DEEP; ++q) now[q] = next[q], next[q] = load(q0 + DEEP + q);
 #pragma unroll
-        for (unsigned q = 0; q < 4u; ++q) f(q0 + q, index(q0 + q), now[q]);
+        for (unsigned q = 0; q < DEEP; ++q) f(q0 + q, index(q0 + q), now[q]);
     }
 }
 
@@ -1000,10 +1002,10 @@ MT_INLINE bool mt_list_cut(const mt_u64* list, unsigned n, AMOUNT amount, PLACE 
     return found[3] != 0;
 }
 
-// A cut by k, one by p if asked, and the token, of a list of up to 128 that has everything
+// A cut by k, one by p if asked, and the token, of a list of up to 256 that has everything
 // that may stay: each entry is compared with all, half of them by one lane and half by
 // another, and the weights of those that are larger, or have an earlier index, added up.
-// `lds`: WAVES words, and twice 128.
+// `lds`: WAVES words, and twice 256.
 template <unsigned SHIFT>
 MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& asked, const mt_weights<SHIFT>& weights,
                                unsigned row, int* tokens, float* logprobs, mt_u64* lds) {

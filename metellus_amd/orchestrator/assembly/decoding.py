@@ -198,7 +198,7 @@ def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name:
 # sampling
 # ---------------------------------------------------------------------------
 
-SAMPLE_WAVES = 4
+SAMPLE_WAVES = 8
 SAMPLE_CUT_WORDS = SAMPLE_WAVES + 4 + 1024 + 2 * 256  # of LDS, that finding a cut in a list takes
 
 

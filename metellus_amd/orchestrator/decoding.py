@@ -309,10 +309,10 @@ class AdapterUpOp(ServingOp):
 
 
 def sample_chunks(rows: int, cols: int) -> tuple[int, int]:
-    """Logits of a chunk, and the chunks of a row: as many as make 1024 workgroups of all
+    """Logits of a chunk, and the chunks of a row: as many as make 512 workgroups of all
     rows, but at most 16, for each workgroup adds all of a row's bins up."""
     chunk = SAMPLE_CHUNK
-    while cols > chunk and (rows * -(-cols // chunk) > 1024 or cols > 16 * chunk):
+    while cols > chunk and (rows * -(-cols // chunk) > 512 or cols > 16 * chunk):
         chunk *= 2
     return chunk, -(-cols // chunk)
 
