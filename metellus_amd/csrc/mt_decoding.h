@@ -299,6 +299,9 @@ template <unsigned K, unsigned R, unsigned RB, unsigned MB, bool LOOP, unsigned 
 MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, float* down, unsigned rows,
                                mt_f32x4* lds) {
     constexpr unsigned TILE = 16u * MB, STEP = 64u * SPLITS * WAVES, WHOLE = K / 64u * 64u;
+    // Sums that an MFMA does not wait for the one before with, added at the end: few tiles are
+    // too few MFMAs to wait in turn (and shorter sums round less).
+    constexpr unsigned SUMS = MB == 1u ? 4u : 1u;
     const unsigned tiles = (rows + TILE - 1u) / TILE, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
     const mt_adapter_place<LOOP> at(tiles);
     const unsigned split = at.share % SPLITS, r0 = at.share / SPLITS * RB * 16u;
@@ -310,13 +313,15 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
         const unsigned long long group = tile.group(j, id);
         if (group != 0ull && id >= 0) {
             const float *xr[MB], *ar[RB];
-            mt_f32x4 acc[MB][RB], xv[4][MB], av[4][RB];
+            mt_f32x4 acc[SUMS][MB][RB], xv[4][MB], av[4][RB];
 #pragma unroll
             for (unsigned m = 0; m < MB; ++m) {
                 const unsigned row = (group >> (16u * m + n)) & 1ull ? 16u * m + n : j;
                 xr[m] = x + (size_t)(tile.row0 + row) * XRS;
 #pragma unroll
-                for (unsigned b = 0; b < RB; ++b) acc[m][b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
+                for (unsigned b = 0; b < RB; ++b)
+#pragma unroll
+                    for (unsigned q = 0; q < SUMS; ++q) acc[q][m][b] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
             }
 #pragma unroll
             for (unsigned b = 0; b < RB; ++b) {
@@ -335,7 +340,11 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
                 for (unsigned m = 0; m < MB; ++m)
                     if (MB == 1u || ((group >> (16u * m)) & 0xFFFFull))  // (a block with rows of the group)
 #pragma unroll
-                        for (unsigned b = 0; b < RB; ++b) acc[m][b] = mt_mfma16_f32(av[u][b], xv[u][m], acc[m][b]);
+                        for (unsigned b = 0; b < RB; ++b)
+#pragma unroll
+                            for (unsigned i = 0; i < 4u; ++i)
+                                acc[i % SUMS][m][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[u][b][i], xv[u][m][i],
+                                                                                           acc[i % SUMS][m][b], 0, 0, 0);
             };
             unsigned k0 = 64u * (split * WAVES + mt_wave());
             if (k0 < WHOLE) {
@@ -368,7 +377,12 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
 #pragma unroll
             for (unsigned m = 0; m < MB; ++m)
 #pragma unroll
-                for (unsigned b = 0; b < RB; ++b) lds[((mt_wave() * MB + m) * RB + b) * 64u + lane] = acc[m][b];
+                for (unsigned b = 0; b < RB; ++b) {
+                    mt_f32x4 v = acc[0][m][b];
+#pragma unroll
+                    for (unsigned q = 1; q < SUMS; ++q) v = v + acc[q][m][b];
+                    lds[((mt_wave() * MB + m) * RB + b) * 64u + lane] = v;
+                }
             __syncthreads();
             for (unsigned e = threadIdx.x; e < MB * RB * 64u; e += WAVES * 64u) {
                 mt_f32x4 v = lds[e];
