@@ -869,7 +869,7 @@ constexpr unsigned MT_SAMPLE_WAVES = 8u, MT_SAMPLE_LANES = 512u;
 constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 7168u;
 constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
 constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
-constexpr unsigned MT_SAMPLE_SHORT = 256u;   // ... all of a list, for both cuts and the token
+constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... all of a list, for both cuts and the token
 constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
 
 // The bin of x on the grid of a temperature.
@@ -1007,8 +1007,11 @@ MT_INLINE bool mt_list_cut(const mt_u64* list, unsigned n, AMOUNT amount, PLACE 
     if (t < m) {
         const mt_u64 own = close[t], weight = weighs[t];
         mt_u64 before = over;
-#pragma unroll 4
-        for (unsigned j = 0; j < m; ++j) before += close[j] > own ? weighs[j] : 0;
+#pragma unroll 8
+        for (unsigned j = 0; j < m; ++j) {
+            const mt_u64 other = close[j], more = weighs[j];  // (both loaded whatever the first is)
+            before += other > own ? more : 0;
+        }
         if (before < asked && asked <= before + weight) found[3] = own;
     }
     __syncthreads();
@@ -1016,45 +1019,47 @@ MT_INLINE bool mt_list_cut(const mt_u64* list, unsigned n, AMOUNT amount, PLACE 
     return found[3] != 0;
 }
 
-// A cut by k, one by p if asked, and the token, of a list of up to 256 that has everything
-// that may stay: each entry is compared with all, half of them by one lane and half by
-// another, and the weights of those that are larger, or have an earlier index, added up.
-// `lds`: WAVES words, and twice 256.
+// A cut by k, one by p if asked, and the token, of a list of up to 128 that has everything
+// that may stay: each entry is compared with all, a share of them by each of the lanes that
+// have it, and the weights of those that are larger, or have an earlier index, are added up.
+// `lds`: WAVES words, and twice 128.
 template <unsigned SHIFT>
 MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& asked, const mt_weights<SHIFT>& weights,
                                unsigned row, int* tokens, float* logprobs, mt_u64* lds) {
-    constexpr unsigned WAVES = MT_SAMPLE_WAVES, MOST = MT_SAMPLE_SHORT;
-    static_assert(MT_SAMPLE_LANES == 2u * MOST, "two lanes to an entry");
-    const unsigned l = threadIdx.x % MOST, half = threadIdx.x / MOST;
-    const unsigned begin = half ? n / 2u : 0u, end = half ? n : n / 2u;
-    mt_u64 *other = lds + WAVES, *amount = other + MOST;
+    constexpr unsigned WAVES = MT_SAMPLE_WAVES, LANES = MT_SAMPLE_LANES, MOST = MT_SAMPLE_SHORT;
+    const unsigned width = n <= 64u ? 64u : MOST, shares = LANES / width;
+    const unsigned t = threadIdx.x, l = t % width, share = t / width;
+    const unsigned begin = n * share / shares, end = n * (share + 1u) / shares;
+    mt_u64 *sums = lds + WAVES, *amount = sums + MOST;
     const mt_u64 one = l < n ? list[l] : 0;
     const double w = weights.weight(mt_order_value((unsigned)(one >> 32)));
-    // the sum over the entries j of which more(j) tells, in the lanes of the first half
+    // the sum of what more(entry, its amount) says of each entry
     const auto before = [&](auto more) {
+        __syncthreads();
+        if (t < MOST) sums[t] = 0;
+        __syncthreads();
         mt_u64 sum = 0;
-#pragma unroll 4
-        for (unsigned j = begin; j < end; ++j) sum += more(j);
+#pragma unroll 8
+        for (unsigned j = begin; j < end; ++j) sum += more(list[j], amount[j]);
+        atomicAdd(sums + l, sum);
         __syncthreads();
-        if (half) other[l] = sum;
-        __syncthreads();
-        return half ? 0 : sum + other[l];
+        return sums[l];
     };
-    const mt_u64 rank = before([&](unsigned j) { return (mt_u64)(list[j] > one ? 1 : 0); });
-    mt_u64 weight = !half && one != 0 && rank < (mt_u64)asked.k ? weights.whole(w) : 0;
+    const mt_u64 rank = before([&](mt_u64 other, mt_u64) { return (mt_u64)(other > one ? 1 : 0); });
+    mt_u64 weight = share == 0u && one != 0 && rank < (mt_u64)asked.k ? weights.whole(w) : 0;
     if (asked.p < 1.f) {
-        if (!half) amount[l] = weight;
+        if (share == 0u) amount[l] = weight;
         const mt_u64 wanted = asked.weight_asked(mt_group_sum<WAVES>(weight, lds));
-        const mt_u64 larger = before([&](unsigned j) { return list[j] > one ? amount[j] : 0; });
+        const mt_u64 larger = before([&](mt_u64 other, mt_u64 more) { return other > one ? more : 0; });
         if (!(larger < wanted)) weight = 0;
     }
     if (w < asked.least) weight = 0;
     __syncthreads();
-    if (!half) amount[l] = weight;
+    if (share == 0u) amount[l] = weight;
     const mt_u64 total = mt_group_sum<WAVES>(weight, lds), target = asked.target(total);
     const double log_total = weights.log_of(total);
     // (the index is upside down: larger is earlier)
-    const mt_u64 earlier = before([&](unsigned j) { return (unsigned)list[j] > (unsigned)one ? amount[j] : 0; });
+    const mt_u64 earlier = before([&](mt_u64 other, mt_u64 more) { return (unsigned)other > (unsigned)one ? more : 0; });
     if (earlier <= target && target < earlier + weight)
         weights.answer(row, 0xFFFFFFFFu - (unsigned)one, mt_order_value((unsigned)(one >> 32)), log_total, tokens, logprobs);
 }
