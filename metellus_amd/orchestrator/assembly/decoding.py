@@ -150,7 +150,7 @@ def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_n
     rows, inner = op.x.shape
     blocks = min(ADAPTER_BLOCKS, _ceil(op.rank, 16))
     tile, loop = adapter_tile(rows, op.rank)
-    waves = ADAPTER_DOWN_WAVES[loop]
+    waves = ADAPTER_DOWN_WAVES
     sig = _Signature()
     args = (sig.add("x", op.x), sig.add("a", op.a), sig.add("ids", op.ids), sig.add("down", op.down, out=True), "M",
             "(mt_f32x4*)mt_lds")
@@ -171,7 +171,7 @@ def adapter_up_shape(rows: int, rank: int) -> tuple[int, int, int]:
     ahead."""
     tile, _ = adapter_tile(rows, rank)
     if tile > 1:
-        return 8, 8, 2
+        return 4, 8, 2
     return 4, 4, 4 if rank <= 32 else 2 if rank <= 64 else 1
 
 

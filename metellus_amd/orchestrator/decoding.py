@@ -124,7 +124,7 @@ class Rotary:
 
 
 ADAPTER_MANY_ROWS = 1024  # from here on tiles of 64 rows, a workgroup for all groups of each
-ADAPTER_DOWN_WAVES = (4, 8)  # a workgroup's for fewer rows, and for so many
+ADAPTER_DOWN_WAVES = 4  # a workgroup's
 
 
 def adapter_splits(rows: int, inner: int) -> int:
