@@ -845,10 +845,10 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // Two kernels draw from rows of which S chunks are in as many workgroups.
 //
 // The first finds a chunk's largest and, for rows that k or p cut, counts its logits by how
-// far below it they are: 512 bins of a sixteenth of the temperature, on a grid that all
-// chunks share (bin f of x is floor(16 x / T)), each with its number of logits and about
-// what they weigh.  What lies further below, 31.9 temperatures and more, weighs less than
-// 2^-45 of the largest, and is 0 as it is held.
+// far below it they are: 512 bins of a sixteenth of the temperature, or more and finer ones
+// of long rows, on a grid that all chunks share (bin f of x is floor(16 x / T)), each with its
+// number of logits and about what they weigh.  What lies further below, 31.9 temperatures
+// and more, weighs less than 2^-45 of the largest, and is 0 as it is held.
 // The second adds the chunks' bins up, in every workgroup for itself, and so knows in which
 // bin the cut is.  What lies above it stays, and is only added up; what lies in it -- or,
 // where k and p both cut, everything from k's bin on, for p's cut depends on where k's is --
@@ -856,9 +856,9 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // list, adds what stays to the sums of the chunks, and looks through the chunk that the
 // random number falls into.
 // All of it counts with the same whole numbers as one workgroup alone, and what the bins
-// say about weights, in 32 bits, is checked; rows that do not fit -- a list beyond LIST,
-// hundreds of logits that are next to equal at the cut, a cut by p next to a bin's edge,
-// logits so large that the grid has no bin for them -- are drawn from by one workgroup.
+// say about weights, in 32 bits, is checked; rows that do not fit -- a list beyond LIST, a
+// cut by p next to a bin's edge, logits so large that the grid has no bin for them -- are
+// drawn from by one workgroup.
 //
 // The list takes half a compute unit's LDS, so there are two workgroups on each, of eight
 // waves (us, 64 rows of 131072 cut by p: eight waves, 512 workgroups 43, 1024 55, four waves
@@ -866,16 +866,17 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // ---------------------------------------------------------------------------
 
 constexpr unsigned MT_SAMPLE_WAVES = 8u, MT_SAMPLE_LANES = 512u;
-constexpr unsigned MT_SAMPLE_BINS = 512u, MT_SAMPLE_LIST = 7168u;
+constexpr unsigned MT_SAMPLE_LIST = 7168u;
 constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
 constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
 constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... all of a list, for both cuts and the token
 constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
 
-// The bin of x on the grid of a temperature.
+// The bin of x on the grid of a temperature, a thirty-second of the bins to each.
+template <unsigned BINS>
 struct mt_grid {
     float by;
-    MT_INLINE explicit mt_grid(float temperature) : by(16.0f / temperature) {}
+    MT_INLINE explicit mt_grid(float temperature) : by((float)(BINS / 32u) / temperature) {}
     MT_INLINE float bin(float x) const { return __builtin_floorf(x * by); }
 };
 
@@ -912,9 +913,9 @@ MT_INLINE void mt_sample_each(const float* x, unsigned i0, F f) {
     }
 }
 
-// best: [row][S]; bins: [row][S][MT_SAMPLE_BINS]; counts: [row][2], the row's arrivals and the
+// best: [row][S]; bins: [row][S][BINS]; counts: [row][2], the row's arrivals and the
 // length of its list.
-template <unsigned V, unsigned CHUNK, unsigned S, unsigned RS, unsigned CS, bool CUT>
+template <unsigned V, unsigned CHUNK, unsigned S, unsigned BINS, unsigned RS, unsigned CS, bool CUT>
 MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, const int* top_k, const float* top_p,
                               mt_u64* best_out, mt_u64* bins_out, unsigned* counts, mt_u64* lds) {
     constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES;
@@ -923,7 +924,7 @@ MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, co
     const float* x = logits + (size_t)row * RS;
     mt_u64* bins = lds + WAVES;
     if (CUT)
-        for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins[b] = 0;
+        for (unsigned b = t; b < BINS; b += LANES) bins[b] = 0;
     mt_u64 best = 0;
     mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned, unsigned i, mt_f32x4 v) {
 #pragma unroll
@@ -938,70 +939,87 @@ MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, co
         const float temperature = temperatures != nullptr ? temperatures[row] : 1.f;
         const bool by_p = top_p != nullptr && top_p[row] < 1.f, by_k = top_k != nullptr && top_k[row] > 0;
         if (!(temperature > 0.f) || !(by_p || by_k)) return;
-        const mt_grid grid(temperature);
+        const mt_grid<BINS> grid(temperature);
         const float first = grid.bin(mt_order_value((unsigned)(best >> 32)));
         mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned, unsigned, mt_f32x4 v) {
 #pragma unroll
             for (unsigned j = 0; j < 4u; ++j) {
                 const float f = grid.bin(v[j]), below = first - f;
-                if (below >= 0.f && below < (float)MT_SAMPLE_BINS) {
+                if (below >= 0.f && below < (float)BINS) {
                     mt_u64 word = 1ull << MT_SAMPLE_COUNT_AT;
-                    if (by_p) word += (unsigned)(__builtin_amdgcn_exp2f((v[j] * grid.by - f) * (1.44269504f / 16.f)) * 1048576.f);
+                    if (by_p) word += (unsigned)(__builtin_amdgcn_exp2f((v[j] * grid.by - f) * (1.44269504f * 32.f / (float)BINS)) * 1048576.f);
                     atomicAdd(bins + (unsigned)below, word);
                 }
             }
         });
         __syncthreads();
-        for (unsigned b = t; b < MT_SAMPLE_BINS; b += LANES) bins_out[((size_t)row * S + part) * MT_SAMPLE_BINS + b] = bins[b];
+        for (unsigned b = t; b < BINS; b += LANES) bins_out[((size_t)row * S + part) * BINS + b] = bins[b];
     }
 }
 
 // The cut of a list: an entry is a key and, below it, the index upside down, so that larger
-// is earlier.  Where amount(entry), added up from the largest on, first reaches `asked`.  Up
-// to 64 are compared one by one; of more, those in the cut's part of the list's range, whose
-// parts place(entry) numbers from the largest on.  False where these are too many, or the
-// amounts less than asked.  `lds`: results, MT_SAMPLE_PARTS and two times MT_SAMPLE_CLOSE words.
+// is earlier, and no two are the same.  Where amount(entry), added up from the largest on,
+// first reaches `asked`: up to 64 are compared one by one; of more, those in the cut's part of
+// the list's range, whose parts place(entry) numbers from the largest on -- and while they
+// are more than MT_SAMPLE_CLOSE, as with equal logits, those in the cut's part of the range
+// from the least to the largest of them, ten bits of which that takes off.  False where the
+// amounts are less than asked.  `lds`: results, MT_SAMPLE_PARTS and two times
+// MT_SAMPLE_CLOSE words.
 template <typename AMOUNT, typename PLACE>
 MT_INLINE bool mt_list_cut(const mt_u64* list, unsigned n, AMOUNT amount, PLACE place, mt_u64 asked, mt_cut_at& cut,
                            mt_u64* lds) {
     constexpr unsigned WAVES = MT_SAMPLE_WAVES, LANES = MT_SAMPLE_LANES, EACH = MT_SAMPLE_PARTS / LANES;
-    mt_u64 *found = lds + WAVES, *parts = found + 4u, *close = parts + MT_SAMPLE_PARTS, *weighs = close + MT_SAMPLE_CLOSE;
+    mt_u64 *found = lds + WAVES, *parts = found + 8u, *close = parts + MT_SAMPLE_PARTS, *weighs = close + MT_SAMPLE_CLOSE;
     const unsigned t = threadIdx.x;
-    mt_u64 over = 0;
+    mt_u64 over = 0, least = 0, most = ~0ull;
     unsigned m = n;
     __syncthreads();
-    if (t < 4u) found[t] = 0;
+    if (t < 8u) found[t] = 0;
     if (n <= 64u) {
         if (t < n) close[t] = list[t], weighs[t] = amount(list[t]);
     } else {
-        for (unsigned b = t; b < MT_SAMPLE_PARTS; b += LANES) parts[b] = 0;
-        __syncthreads();
-        for (unsigned l = t; l < n; l += LANES) {
-            const mt_u64 w = amount(list[l]);
-            if (w != 0) atomicAdd(parts + place(list[l]), w);
-        }
-        __syncthreads();
-        mt_u64 mine[EACH], sum = 0, all;
-#pragma unroll
-        for (unsigned b = 0; b < EACH; ++b) mine[b] = parts[t * EACH + b], sum += mine[b];
-        mt_u64 before = mt_group_before<WAVES>(sum, lds, all);
-        if (all < asked) return false;  // (the same in all lanes)
-#pragma unroll
-        for (unsigned b = 0; b < EACH; ++b) {
-            if (before < asked && asked <= before + mine[b]) found[0] = t * EACH + b, found[1] = before;
-            before += mine[b];
-        }
-        __syncthreads();
-        const unsigned at = (unsigned)found[0];
-        over = found[1];
-        for (unsigned l = t; l < n; l += LANES)
-            if (place(list[l]) == at) {
-                const unsigned to = (unsigned)atomicAdd(found + 2, 1ull);
-                if (to < MT_SAMPLE_CLOSE) close[to] = list[l], weighs[to] = amount(list[l]);
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+            const unsigned bits = 64u - (unsigned)__builtin_clzll((most - least) | 1ull), shift = bits > 10u ? bits - 10u : 0u;
+            const auto part = [&](mt_u64 e) { return again ? (unsigned)((most - e) >> shift) : place(e); };
+            for (unsigned b = t; b < MT_SAMPLE_PARTS; b += LANES) parts[b] = 0;
+            if (t < 8u) found[t] = t == 4u ? ~0ull : 0;
+            __syncthreads();
+            for (unsigned l = t; l < n; l += LANES) {
+                const mt_u64 e = list[l];
+                if (e >= least && e <= most) {
+                    const mt_u64 w = amount(e);
+                    if (w != 0) atomicAdd(parts + part(e), w);
+                }
             }
-        __syncthreads();
-        m = (unsigned)found[2];
-        if (m > MT_SAMPLE_CLOSE) return false;
+            __syncthreads();
+            mt_u64 mine[EACH], sum = 0, all;
+#pragma unroll
+            for (unsigned b = 0; b < EACH; ++b) mine[b] = parts[t * EACH + b], sum += mine[b];
+            mt_u64 before = over + mt_group_before<WAVES>(sum, lds, all);
+            if (over + all < asked) return false;  // (the same in all lanes)
+#pragma unroll
+            for (unsigned b = 0; b < EACH; ++b) {
+                if (before < asked && asked <= before + mine[b]) found[0] = t * EACH + b, found[1] = before;
+                before += mine[b];
+            }
+            __syncthreads();
+            const unsigned at = (unsigned)found[0];
+            over = found[1];
+            for (unsigned l = t; l < n; l += LANES) {
+                const mt_u64 e = list[l];
+                if (e >= least && e <= most && part(e) == at) {
+                    const unsigned to = (unsigned)atomicAdd(found + 2, 1ull);
+                    if (to < MT_SAMPLE_CLOSE) close[to] = e, weighs[to] = amount(e);
+                    atomicMin(found + 4, e);
+                    atomicMax(found + 5, e);
+                }
+            }
+            __syncthreads();
+            m = (unsigned)found[2], least = found[4], most = found[5];
+            if (m <= MT_SAMPLE_CLOSE) break;  // (at the latest with a part for each)
+            __syncthreads();
+        }
     }
     __syncthreads();
     if (t < m) {
@@ -1066,11 +1084,11 @@ MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& a
 
 // sums: [row][S][2], all weights and those above the cut, behind them for each row, the
 // weights that stay of each segment of 256; list: [row][MT_SAMPLE_LIST].
-template <unsigned V, unsigned CHUNK, unsigned S, unsigned SHIFT, unsigned RS, unsigned CS, bool CUT>
+template <unsigned V, unsigned CHUNK, unsigned S, unsigned BINS, unsigned SHIFT, unsigned RS, unsigned CS, bool CUT>
 MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const float* temperatures, const int* top_k,
                               const float* top_p, const float* min_p, const mt_u64* best_in, const mt_u64* bins_in,
                               unsigned* counts, mt_u64* sums, mt_u64* list, int* tokens, float* logprobs, mt_u64* lds) {
-    constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES, EACH = MT_SAMPLE_BINS / LANES;
+    constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES, EACH = BINS / LANES;
     constexpr unsigned SEGMENTS = CHUNK / 256u, ROW = 2u * S + S * SEGMENTS;  // a chunk's, and the words of a row's sums
     const unsigned row = blockIdx.x / S, part = blockIdx.x % S, t = threadIdx.x;
     const float* x = logits + (size_t)row * RS;
@@ -1081,7 +1099,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     // LDS: the folds' words and some results, four more, what stays of each segment; for cuts,
     // mt_list_cut's, and the list
     mt_u64 *words = lds + WAVES + 4u, *kept = words + 4u, *cut_lds = kept + S * SEGMENTS;
-    mt_u64* held = cut_lds + WAVES + 4u + MT_SAMPLE_PARTS + 2u * MT_SAMPLE_CLOSE;
+    mt_u64* held = cut_lds + WAVES + 8u + MT_SAMPLE_PARTS + 2u * MT_SAMPLE_CLOSE;
     const mt_asked asked(row, uniforms, temperatures, top_k, top_p, min_p);
     mt_u64 best = 0;
     for (unsigned c = mt_lane(); c < S; c += 64u) {
@@ -1092,13 +1110,13 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
     if (mt_sample_plain(best, asked.temperature, row, part == 0u && t == 0u, tokens, logprobs)) return;
     const mt_weights<SHIFT> weights{mt_order_value((unsigned)(best >> 32)), 1.0 / (double)asked.temperature};
-    const mt_grid grid(asked.temperature);
+    const mt_grid<BINS> grid(asked.temperature);
     const float first = grid.bin(weights.top);
 
     // From which bin on logits are listed, and up to which: those above the first stay, those
     // below the last go.
     bool by_k = asked.k > 0 && (unsigned)asked.k < V, by_p = asked.p < 1.f, whole = false;
-    unsigned from = MT_SAMPLE_BINS, upto = MT_SAMPLE_BINS;  // (none listed, all stay)
+    unsigned from = BINS, upto = BINS;  // (none listed, all stay)
     mt_u64 above_k = 0;                                     // logits above `from`
     if (t < 4u) words[t] = 0;
     __syncthreads();
@@ -1111,11 +1129,11 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
 #pragma unroll
             for (unsigned c = 0; c < S; ++c) {  // (loads that do not wait for each other)
                 const float shift = first - grid.bin(mt_order_value((unsigned)(kept[c] >> 32)));
-                const int by = shift >= 0.f && shift < (float)MT_SAMPLE_BINS ? (int)shift : (int)MT_SAMPLE_BINS;
+                const int by = shift >= 0.f && shift < (float)BINS ? (int)shift : (int)BINS;
 #pragma unroll
                 for (unsigned b = 0; b < EACH; ++b) {
                     const int at = (int)(t * EACH + b) - by;
-                    const mt_u64 word = bins_in[((size_t)row * S + c) * MT_SAMPLE_BINS + (at < 0 ? 0 : at)];
+                    const mt_u64 word = bins_in[((size_t)row * S + c) * BINS + (at < 0 ? 0 : at)];
                     number[b] += at < 0 ? 0 : word >> MT_SAMPLE_COUNT_AT;
                     mass[b] += at < 0 ? 0 : word & ((1ull << MT_SAMPLE_COUNT_AT) - 1ull);
                 }
@@ -1124,11 +1142,11 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             for (unsigned b = 0; b < EACH; ++b) {
                 numbers += number[b];
                 // in 2^-40 of the first bin's lower edge
-                mass[b] = (mt_u64)((double)mass[b] * mt_exp_below(-0.0625 * (double)(t * EACH + b)) * 1048576.0);
+                mass[b] = (mt_u64)((double)mass[b] * mt_exp_below(-32.0 / (double)BINS * (double)(t * EACH + b)) * 1048576.0);
                 masses += mass[b];
             }
             mt_u64 *found = lds + WAVES, all;
-            if (t == 0u) found[0] = found[1] = MT_SAMPLE_BINS;
+            if (t == 0u) found[0] = found[1] = BINS;
             if (by_k) {
                 mt_u64 before = mt_group_before<WAVES>(numbers, lds, all);
                 const mt_u64 k = (mt_u64)asked.k;
@@ -1139,7 +1157,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
                 }
                 __syncthreads();
                 upto = (unsigned)found[0];
-                by_k = upto != MT_SAMPLE_BINS;  // (else what weighs anything stays)
+                by_k = upto != BINS;  // (else what weighs anything stays)
                 if (by_k) {
                     // (of few, all are listed: nothing else stays then)
                     const bool every = by_p || found[2] + found[3] <= MT_SAMPLE_SHORT;
@@ -1158,14 +1176,14 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
                 }
                 __syncthreads();
                 from = upto = (unsigned)found[1];
-                whole = from == MT_SAMPLE_BINS || found[3] > MT_SAMPLE_LIST;
+                whole = from == BINS || found[3] > MT_SAMPLE_LIST;
             }
             whole = whole || !(__builtin_fabsf(first) < 1048576.f);
             __syncthreads();
         }
     }
     if (whole && part != 0u) return;  // (the same in all workgroups of the row)
-    const bool cuts = from < MT_SAMPLE_BINS;
+    const bool cuts = from < BINS;
     if (!whole) {
         mt_u64 all = 0, above = 0;
         const bool weigh_all = by_p && !by_k;

@@ -13,7 +13,6 @@ from metellus_amd.orchestrator.assembly.serving import _ceil, _group, _Signature
 from metellus_amd.orchestrator.decoding import (
     ADAPTER_DOWN_WAVES,
     ADAPTER_MANY_ROWS,
-    SAMPLE_BINS,
     SAMPLE_LIST,
     AdapterDownOp,
     AdapterUpOp,
@@ -22,6 +21,7 @@ from metellus_amd.orchestrator.decoding import (
     RotaryOp,
     SampleOp,
     SampleScanOp,
+    sample_bins,
     sample_chunks,
 )
 from metellus_amd.orchestrator.ir import Tensor
@@ -199,7 +199,7 @@ def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name:
 # ---------------------------------------------------------------------------
 
 SAMPLE_WAVES = 8
-SAMPLE_CUT_WORDS = SAMPLE_WAVES + 4 + 1024 + 2 * 256  # of LDS, that finding a cut in a list takes
+SAMPLE_CUT_WORDS = SAMPLE_WAVES + 8 + 1024 + 2 * 256  # of LDS, that finding a cut in a list takes
 
 
 def _words(sig: _Signature, role: str, t: Tensor | None, *, out: bool = False) -> str:
@@ -225,9 +225,9 @@ def _assemble_sample_scan(decision: DecisionView, op: SampleScanOp, function_nam
     )
     frag = ServingFragment(
         "mt_sample_scan",
-        (cols, chunk, chunks, *_strides(op.logits), cuts),
+        (cols, chunk, chunks, sample_bins(cols), *_strides(op.logits), cuts),
         args,
-        lds_bytes=8 * (SAMPLE_WAVES + (SAMPLE_BINS if cuts else 0)),
+        lds_bytes=8 * (SAMPLE_WAVES + (sample_bins(cols) if cuts else 0)),
         name="sample_scan",
     )
     return _group(decision, sig, frag, function_name or f"sample_scan_{op.name}", {}, (rows * chunks, 1, 1), 64 * SAMPLE_WAVES,
@@ -259,7 +259,7 @@ def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | 
     shift = min(44, 62 - (cols - 1).bit_length())
     frag = ServingFragment(
         "mt_sample_pick",
-        (cols, chunk, chunks, shift, *_strides(op.logits), cuts),
+        (cols, chunk, chunks, sample_bins(cols), shift, *_strides(op.logits), cuts),
         args,
         # (one workgroup for a whole row takes two words a wave and 256)
         lds_bytes=8 * max(SAMPLE_WAVES + 8 + chunk * chunks // 256 + (SAMPLE_CUT_WORDS + SAMPLE_LIST if cuts else 0), 2 * SAMPLE_WAVES + 256),

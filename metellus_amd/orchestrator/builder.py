@@ -23,7 +23,6 @@ import numpy as np
 from metellus_amd.compute.elementwise.elementwise import BroadcastSpec
 from metellus_amd.orchestrator.decoding import (
     ADAPTER_RANK_MAX,
-    SAMPLE_BINS,
     SAMPLE_LIST,
     AdapterDownOp,
     AdapterUpOp,
@@ -33,6 +32,7 @@ from metellus_amd.orchestrator.decoding import (
     SampleOp,
     SampleScanOp,
     adapter_splits,
+    sample_bins,
     sample_chunks,
 )
 from metellus_amd.orchestrator.ir import (
@@ -628,7 +628,7 @@ class Operations:
             counts=made("counts", rows, 1),
             logits=tl,
             name=out,
-            bins=made("bins", rows * chunks, SAMPLE_BINS) if cuts else None,
+            bins=made("bins", rows * chunks, sample_bins(cols)) if cuts else None,
             **{n: t if cuts else None for n, t in given.items() if n != "min_p"},
             after=self._owners(tl, *given.values()),
         )

@@ -31,7 +31,8 @@ POSITIONS_MAX = _INT32_MAX - 1024  # of a table's row (its positions and a step'
 ADAPTER_RANK_MAX = 256
 VOCABULARY_MAX = 2**20
 SAMPLE_CHUNK = 4096  # logits, and the smallest share of a workgroup
-SAMPLE_BINS, SAMPLE_LIST = 512, 7168  # of a chunk; logits that a row has listed at most
+SAMPLE_BINS_FINE = 131072  # columns up to which there are 512 bins
+SAMPLE_LIST = 7168  # logits that a row has listed at most
 
 # pi to 64 digits: 2 pi has to outlast a double's 53 bits twice
 _PI = Decimal("3.141592653589793238462643383279502884197169399375105820974944592")
@@ -315,6 +316,13 @@ def sample_chunks(rows: int, cols: int) -> tuple[int, int]:
     while cols > chunk and (rows * -(-cols // chunk) > 512 or cols > 16 * chunk):
         chunk *= 2
     return chunk, -(-cols // chunk)
+
+
+def sample_bins(cols: int) -> int:
+    """Bins of 32 temperatures: the finer, the shorter the lists of what is in one, and the
+    longer adding them up takes (us of the second kernel with 512 and 1024: 64 rows of 131072
+    cut by k 20, 26, by p 44, 44; one row 11, 16 and 16, 20)."""
+    return 512 if cols <= SAMPLE_BINS_FINE else 1024 if cols <= 2 * SAMPLE_BINS_FINE else 2048
 
 
 @dataclass(frozen=True)

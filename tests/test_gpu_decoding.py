@@ -159,10 +159,9 @@ def test_rotary(spec, rows):
     _rotary_check(ops, spec, q="q1", k="k1")
 
 
-@pytest.mark.parametrize("layout", ["half", "interleaved"])
-def test_rotary_far_positions(layout):
-    """The farthest positions of int32, below 0 too; k alone has no turn of its own."""
-    spec = Rotary(dim=32, layout=layout)
+@pytest.mark.parametrize("spec", [Rotary(dim=32), Rotary(dim=32, layout="interleaved"), Rotary(dim=64, frequencies=(2.0**20, -0.3) * 16)])
+def test_rotary_far_positions(spec):
+    """The farthest positions of int32, below 0 too, and the largest frequencies; q alone."""
     at = np.array([0, 1, -1, 2**31 - 1, -(2**31), 2**24 + 1, 1000003], np.int32)
     rng = np.random.default_rng(2)
     ops = Operations()
@@ -418,6 +417,25 @@ def test_sample_spreads_of_logits(rows, cols, scale):
     for asked in ({}, {"top_p": 0.6}, {"top_k": 30}, {"top_k": 20000}, {"top_k": 20000, "top_p": 0.3}, {"min_p": 0.4},
                   {"top_k": 300, "top_p": 0.7, "min_p": 0.01}):
         _sample_check(_sample_ops(x, rng.random(rows), **asked))
+
+
+@pytest.mark.parametrize("rows, cols", [(3, 600), (2, 50000), (1, 300000)])
+def test_sample_logits_of_few_bits(rows, cols):
+    """Logits of eight bits, as of a product in bfloat16: hundreds are equal at every cut."""
+    rng = np.random.default_rng(cols)
+    x = rng.standard_normal((rows, cols)).astype(np.float32)
+    x = (x.view(np.uint32) & 0xFFFF0000).view(np.float32)
+    for asked in ({}, {"top_p": 0.6}, {"top_k": 300}, {"top_k": 2000, "top_p": 0.5}, {"top_k": 150, "top_p": 0.7},
+                  {"top_k": 37, "top_p": 0.01, "temperatures": 0.3}, {"top_p": 0.97, "min_p": 0.02, "temperatures": 1.7}):
+        _sample_check(_sample_ops(x, rng.random(rows), **asked))
+
+
+@pytest.mark.parametrize("rows, cols", [(520, 9000), (1, 1048576), (700, 70), (65, 33000)])
+def test_sample_many_rows_and_columns(rows, cols):
+    rng = np.random.default_rng(rows)
+    x = 2 * rng.standard_normal((rows, cols)).astype(np.float32)
+    _sample_check(_sample_ops(x, rng.random(rows), top_k=rng.choice([0, 40, 3000], rows), top_p=rng.choice([0.5, 0.95, 1.0], rows),
+                              temperatures=rng.choice([0.0, 0.5, 1.0], rows)))
 
 
 def test_sample_of_strided_logits():
