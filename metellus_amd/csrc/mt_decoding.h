@@ -405,100 +405,107 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
     }
 }
 
-// B's part and the sum: a wave takes PER blocks of 16 columns of the output, and loads
-// AHEAD of them, of B and of base, before it needs them.  Tiles of several blocks of rows
-// have `down`'s parts added up in LDS, once for all waves.
+// B's part and the sum: the waves of a workgroup take BL blocks of 16 columns of the output
+// in turn, PER times.  `down`'s parts are added up in LDS, once for all waves.  A block of 16
+// rows goes through LDS on its way out, where rows become what lanes next to each other have:
+// base is read and the output written 64 BL bytes of a row at a time, and by the four waves
+// 256 BL (4096 rows of 4096, rank 64: 64 bytes of a row at a time 58 us).
 template <unsigned N, unsigned R, unsigned MB, bool LOOP, unsigned SPLITS, unsigned HELD, unsigned WAVES, unsigned PER,
-          unsigned AHEAD, unsigned YRS, unsigned YCS>
+          unsigned BL, unsigned YRS, unsigned YCS>
 MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* b, const int* ids, const float* scales,
                              float* out, unsigned rows, float* lds) {
-    constexpr unsigned RC = (R + 15u) / 16u, TILE = 16u * MB, PITCH = 16u * RC + 4u;
-    static_assert(PER % AHEAD == 0u, "blocks in whole sets");
+    constexpr unsigned RC = (R + 15u) / 16u, TILE = 16u * MB, PITCH = 16u * RC + 4u, WIDE = 16u * BL, OUT_PITCH = WIDE + 4u;
+    constexpr unsigned ALONG = 4u * BL, ABREAST = 64u / ALONG;  // lanes along a row, and rows at a time
     const unsigned tiles = (rows + TILE - 1u) / TILE, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
     const mt_adapter_place<LOOP> at(tiles);
-    const unsigned n0 = (at.share * WAVES + mt_wave()) * PER * 16u;
     if (at.tile >= tiles) return;
     const mt_adapter_rows<MB, HELD> tile(ids, at.tile, rows);
+    float* turn = lds + TILE * PITCH + mt_wave() * 16u * OUT_PITCH;  // this wave's block of rows
 #pragma unroll 1
     for (unsigned j = blockIdx.y; j < TILE; ++j) {
         int id;
         const unsigned long long group = tile.group(j, id);
         if (group != 0ull) {
-            const float* yr[MB];
-            mt_f32x4 bv[AHEAD][RC], v[AHEAD][MB], t[MB][RC];
+            mt_f32x4 bv[BL][RC], v[BL];
+            const auto columns = [&](unsigned p) { return ((at.share * PER + p) * WAVES + mt_wave()) * WIDE; };
+            const auto load = [&](unsigned from) {
+                if (id < 0) return;
 #pragma unroll
-            for (unsigned m = 0; m < MB; ++m) {
-                const unsigned row = (group >> (16u * m + n)) & 1ull ? 16u * m + n : j;
-                yr[m] = base + (size_t)(tile.row0 + row) * YRS;
-            }
-            // (n0, and so the block, is the same in all lanes of a wave)
-            const auto load = [&](unsigned from, unsigned p) {
-                const unsigned col = from + 4u * g;
-                if (id >= 0) {
-                    const float* br = b + ((size_t)(unsigned)id * N + (from + n < N ? from + n : N - 1u)) * R;
+                for (unsigned q = 0; q < BL; ++q) {
+                    const unsigned col = from + 16u * q + n;
+                    const float* br = b + ((size_t)(unsigned)id * N + (col < N ? col : N - 1u)) * R;
 #pragma unroll
                     for (unsigned c = 0; c < RC; ++c)
-                        bv[p][c] = 16u * c + 16u <= R ? mt_quad_in<1u>(br, 16u * c + 4u * g) : mt_quad<R, 1u>(br, 16u * c + 4u * g);
-                }
-#pragma unroll
-                for (unsigned m = 0; m < MB; ++m) {
-                    if (from + 16u <= N) v[p][m] = mt_quad_in<YCS>(yr[m], col);
-                    else v[p][m] = mt_quad<N, YCS>(yr[m], col);
+                        bv[q][c] = 16u * c + 16u <= R ? mt_quad_in<1u>(br, 16u * c + 4u * g) : mt_quad<R, 1u>(br, 16u * c + 4u * g);
                 }
             };
+            // base's part of block m, as it goes out (rows of other groups: the leader's)
+            const auto load_base = [&](unsigned from, unsigned m) {
+                const unsigned col = from + 4u * (lane % ALONG);
 #pragma unroll
-            for (unsigned p = 0; p < AHEAD; ++p)
-                if (n0 + 16u * p < N) load(n0 + 16u * p, p);
+                for (unsigned q = 0; q < BL; ++q) {
+                    const unsigned row = 16u * m + q * ABREAST + lane / ALONG;
+                    const float* yr = base + (size_t)(tile.row0 + ((group >> row) & 1ull ? row : j)) * YRS;
+                    if (from + WIDE <= N) v[q] = mt_quad_in<YCS>(yr, col);
+                    else v[q] = mt_quad<N, YCS>(yr, col);
+                }
+            };
+            if (columns(0u) < N) load(columns(0u));
             // the sums of down's parts; nothing for rows of other groups
-            const auto parts = [&](unsigned m, unsigned r) {
+            if (LOOP) __syncthreads();  // (the group before has been multiplied)
+            for (unsigned e = threadIdx.x; e < TILE * RC * 4u; e += WAVES * 64u) {
+                const unsigned m = e / (RC * 4u), r = e % (RC * 4u) * 4u;
                 mt_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
                 if (((group >> m) & 1ull) && id >= 0 && r < R) {
 #pragma unroll
                     for (unsigned s = 0; s < SPLITS; ++s)
                         sum = sum + mt_row4<R, 1u>(down + ((size_t)s * rows + tile.row0 + m) * R, r);
                 }
-                return sum;
-            };
-            if constexpr (MB > 1u) {
-                if (LOOP) __syncthreads();  // (the group before has been multiplied)
-                for (unsigned e = threadIdx.x; e < TILE * RC * 4u; e += WAVES * 64u) {
-                    const unsigned m = e / (RC * 4u), r = e % (RC * 4u) * 4u;
-                    *reinterpret_cast<mt_f32x4*>(lds + m * PITCH + r) = parts(m, r);
-                }
-                __syncthreads();
+                *reinterpret_cast<mt_f32x4*>(lds + m * PITCH + r) = sum;
             }
-#pragma unroll
-            for (unsigned m = 0; m < MB; ++m)
-#pragma unroll
-                for (unsigned c = 0; c < RC; ++c) {
-                    if constexpr (MB > 1u) {
-                        t[m][c] = *reinterpret_cast<const mt_f32x4*>(lds + (16u * m + n) * PITCH + 16u * c + 4u * g);
-                    } else {
-                        t[m][c] = parts(n, 16u * c + 4u * g);
-                    }
-                }
             const float scale = scales != nullptr && id >= 0 ? scales[id] : 1.f;
+            __syncthreads();
 #pragma unroll 1
-            for (unsigned p0 = 0; p0 < PER && n0 + 16u * p0 < N; p0 += AHEAD) {
+            for (unsigned p = 0; p < PER && columns(p) < N; ++p) {
+                const unsigned from = columns(p);
+                if (p != 0u) load(from);
+#pragma unroll 1
+                for (unsigned m = 0; m < MB; ++m) {
+                    if (!((group >> (16u * m)) & 0xFFFFull)) continue;
+                    load_base(from, m);
+                    if (id >= 0) {
+                        mt_f32x4 acc[BL];
 #pragma unroll
-                for (unsigned p = 0; p < AHEAD; ++p) {
-                    const unsigned from = n0 + 16u * (p0 + p), col = from + 4u * g;
+                        for (unsigned q = 0; q < BL; ++q) acc[q] = mt_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (unsigned m = 0; m < MB; ++m) {
-                        if (MB > 1u && !((group >> (16u * m)) & 0xFFFFull)) continue;
-                        if (id >= 0) {
-                            mt_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                        for (unsigned c = 0; c < RC; ++c) {
+                            const mt_f32x4 t = *reinterpret_cast<const mt_f32x4*>(lds + (16u * m + n) * PITCH + 16u * c + 4u * g);
 #pragma unroll
-                            for (unsigned c = 0; c < RC; ++c) acc = mt_mfma16_f32(bv[p][c], t[m][c], acc);
+                            for (unsigned i = 0; i < 4u; ++i)
 #pragma unroll
-                            for (unsigned i = 0; i < 4u; ++i) v[p][m][i] = __builtin_fmaf(scale, acc[i], v[p][m][i]);
+                                for (unsigned q = 0; q < BL; ++q)
+                                    acc[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[q][c][i], t[i], acc[q], 0, 0, 0);
                         }
-                        unsigned stores = ((group >> (16u * m + n)) & 1ull) && col < N;
-                        asm volatile("" : "+v"(stores));  // (known to no other round)
-                        if (stores) mt_put_row4<N>(out + (size_t)(tile.row0 + 16u * m + n) * N, col, v[p][m]);
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the block before has been read)
+#pragma unroll
+                        for (unsigned q = 0; q < BL; ++q)
+                            *reinterpret_cast<mt_f32x4*>(turn + n * OUT_PITCH + 16u * q + 4u * g) = acc[q];
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                        for (unsigned q = 0; q < BL; ++q) {
+                            const mt_f32x4 sum = *reinterpret_cast<const mt_f32x4*>(
+                                turn + (q * ABREAST + lane / ALONG) * OUT_PITCH + 4u * (lane % ALONG));
+#pragma unroll
+                            for (unsigned i = 0; i < 4u; ++i) v[q][i] = __builtin_fmaf(scale, sum[i], v[q][i]);
+                        }
                     }
-                    if (p0 + p + AHEAD < PER && from + 16u * AHEAD < N) load(from + 16u * AHEAD, p);
-                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (unsigned q = 0; q < BL; ++q) {
+                        const unsigned row = 16u * m + q * ABREAST + lane / ALONG, col = from + 4u * (lane % ALONG);
+                        unsigned stores = ((group >> row) & 1ull) && col < N;
+                        asm volatile("" : "+v"(stores));  // (known to no other round)
+                        if (stores) mt_put_row4<N>(out + (size_t)(tile.row0 + row) * N, col, v[q]);
+                    }
                 }
             }
         }

@@ -167,29 +167,26 @@ def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_n
 
 
 def adapter_up_shape(rows: int, rank: int) -> tuple[int, int, int]:
-    """Waves of a workgroup, the blocks of 16 columns that each takes, and those it loads
-    ahead."""
-    tile, _ = adapter_tile(rows, rank)
-    if tile > 1:
-        return 4, 8, 2
-    return 4, 4, 4 if rank <= 32 else 2 if rank <= 64 else 1
+    """Waves of a workgroup, how often each takes a set of columns, and the blocks of 16 in a
+    set: as many as leave registers for their part of B."""
+    return 4, 2 if rows >= ADAPTER_MANY_ROWS else 1, 4 if rank <= 64 else 2 if rank <= 128 else 1
 
 
 def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name: str | None) -> KernelGroup:
     rows, cols = op.base.shape
     tile, loop = adapter_tile(rows, op.rank)
-    waves, per, ahead = adapter_up_shape(rows, op.rank)
+    waves, per, blocks = adapter_up_shape(rows, op.rank)
     sig = _Signature()
     args = (sig.add("base", op.base), sig.add("down", op.down), sig.add("b", op.b), sig.add("ids", op.ids),
-            sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M", "(float*)mt_lds" if tile > 1 else "nullptr")
+            sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M", "(float*)mt_lds")
     frag = ServingFragment(
         "mt_adapter_up",
-        (cols, op.rank, tile, loop, op.splits, op.held, waves, per, ahead, *_strides(op.base)),
+        (cols, op.rank, tile, loop, op.splits, op.held, waves, per, blocks, *_strides(op.base)),
         args,
-        lds_bytes=64 * tile * (16 * _ceil(op.rank, 16) + 4) if tile > 1 else 0,
+        lds_bytes=64 * (tile * (16 * _ceil(op.rank, 16) + 4) + waves * (16 * blocks + 4)),
         name="adapter_up",
     )
-    grid = _adapter_grid(rows, tile, loop, _ceil(cols, 16 * waves * per))
+    grid = _adapter_grid(rows, tile, loop, _ceil(cols, 16 * waves * per * blocks))
     return _group(decision, sig, frag, function_name or f"adapter_up_{op.y.name}", {"M": rows}, grid, 64 * waves,
                   headers=(decoding_header(),))
 
