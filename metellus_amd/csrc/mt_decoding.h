@@ -849,7 +849,8 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 }
 
 // ---------------------------------------------------------------------------
-// Two kernels draw from rows of which S chunks are in as many workgroups.
+// Two kernels draw from rows of which S chunks are in as many workgroups; of one chunk, the
+// second alone, which does the first's part for itself.
 //
 // The first finds a chunk's largest and, for rows that k or p cut, counts its logits by how
 // far below it they are: 512 bins of a sixteenth of the temperature, or more and finer ones
@@ -877,7 +878,7 @@ constexpr unsigned MT_SAMPLE_LIST = 7168u;
 constexpr unsigned MT_SAMPLE_PARTS = 1024u;  // of a list's range, where its cut is looked for
 constexpr unsigned MT_SAMPLE_CLOSE = 256u;   // logits that are compared one by one
 constexpr unsigned MT_SAMPLE_SHORT = 128u;   // ... all of a list, for both cuts and the token
-constexpr unsigned MT_SAMPLE_COUNT_AT = 48u;  // a bin's word: its logits from this bit on, 2^20 of their weights below
+constexpr unsigned MT_SAMPLE_COUNT_AT = 43u;  // a bin's word: up to 2^20 logits from this bit on, 2^20 of their weights below
 
 // The bin of x on the grid of a temperature, a thirty-second of the bins to each.
 template <unsigned BINS>
@@ -920,45 +921,57 @@ MT_INLINE void mt_sample_each(const float* x, unsigned i0, F f) {
     }
 }
 
-// best: [row][S]; bins: [row][S][BINS]; counts: [row][2], the row's arrivals and the
-// length of its list.
-template <unsigned V, unsigned CHUNK, unsigned S, unsigned BINS, unsigned RS, unsigned CS, bool CUT>
-MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, const int* top_k, const float* top_p,
-                              mt_u64* best_out, mt_u64* bins_out, unsigned* counts, mt_u64* lds) {
-    constexpr unsigned LANES = MT_SAMPLE_LANES, WAVES = MT_SAMPLE_WAVES;
-    const unsigned row = blockIdx.x / S, part = blockIdx.x % S, t = threadIdx.x;
-    if (part == 0u && t < 2u) counts[2u * row + t] = 0u;
-    const float* x = logits + (size_t)row * RS;
-    mt_u64* bins = lds + WAVES;
-    if (CUT)
-        for (unsigned b = t; b < BINS; b += LANES) bins[b] = 0;
+// The first of a chunk's largest, in all lanes.
+template <unsigned V, unsigned CHUNK, unsigned CS>
+MT_INLINE mt_u64 mt_sample_best(const float* x, unsigned i0, mt_u64* lds) {
     mt_u64 best = 0;
-    mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned, unsigned i, mt_f32x4 v) {
+    mt_sample_each<V, CHUNK, CS>(x, i0, [&](unsigned, unsigned i, mt_f32x4 v) {
 #pragma unroll
         for (unsigned j = 0; j < 4u; ++j) {
             const mt_u64 found = i + j < V ? mt_best(i + j, v[j]) : 0;
             best = found > best ? found : best;
         }
     });
-    best = mt_group_fold<WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
+    return mt_group_fold<MT_SAMPLE_WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
+}
+
+// A chunk's logits, and about what they weigh where asked, added to the bins in LDS, which are 0;
+// `first`: the bin of its largest.
+template <unsigned V, unsigned CHUNK, unsigned CS, unsigned BINS>
+MT_INLINE void mt_sample_count(const float* x, unsigned i0, const mt_grid<BINS>& grid, float first, bool weigh, mt_u64* bins) {
+    mt_sample_each<V, CHUNK, CS>(x, i0, [&](unsigned, unsigned, mt_f32x4 v) {
+#pragma unroll
+        for (unsigned j = 0; j < 4u; ++j) {
+            const float f = grid.bin(v[j]), below = first - f;
+            if (below >= 0.f && below < (float)BINS) {
+                mt_u64 word = 1ull << MT_SAMPLE_COUNT_AT;
+                if (weigh) word += (unsigned)(__builtin_amdgcn_exp2f((v[j] * grid.by - f) * (1.44269504f * 32.f / (float)BINS)) * 1048576.f);
+                atomicAdd(bins + (unsigned)below, word);
+            }
+        }
+    });
+}
+
+// best: [row][S]; bins: [row][S][BINS]; counts: [row][2], the row's arrivals and the length of
+// its list.
+template <unsigned V, unsigned CHUNK, unsigned S, unsigned BINS, unsigned RS, unsigned CS, bool CUT>
+MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, const int* top_k, const float* top_p,
+                              mt_u64* best_out, mt_u64* bins_out, unsigned* counts, mt_u64* lds) {
+    constexpr unsigned LANES = MT_SAMPLE_LANES;
+    const unsigned row = blockIdx.x / S, part = blockIdx.x % S, t = threadIdx.x;
+    if (part == 0u && t < 2u) counts[2u * row + t] = 0u;
+    const float* x = logits + (size_t)row * RS;
+    mt_u64* bins = lds + MT_SAMPLE_WAVES;
+    if (CUT)
+        for (unsigned b = t; b < BINS; b += LANES) bins[b] = 0;
+    const mt_u64 best = mt_sample_best<V, CHUNK, CS>(x, part * CHUNK, lds);
     if (t == 0u) best_out[(size_t)row * S + part] = best;
     if constexpr (CUT) {
         const float temperature = temperatures != nullptr ? temperatures[row] : 1.f;
         const bool by_p = top_p != nullptr && top_p[row] < 1.f, by_k = top_k != nullptr && top_k[row] > 0;
         if (!(temperature > 0.f) || !(by_p || by_k)) return;
         const mt_grid<BINS> grid(temperature);
-        const float first = grid.bin(mt_order_value((unsigned)(best >> 32)));
-        mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned, unsigned, mt_f32x4 v) {
-#pragma unroll
-            for (unsigned j = 0; j < 4u; ++j) {
-                const float f = grid.bin(v[j]), below = first - f;
-                if (below >= 0.f && below < (float)BINS) {
-                    mt_u64 word = 1ull << MT_SAMPLE_COUNT_AT;
-                    if (by_p) word += (unsigned)(__builtin_amdgcn_exp2f((v[j] * grid.by - f) * (1.44269504f * 32.f / (float)BINS)) * 1048576.f);
-                    atomicAdd(bins + (unsigned)below, word);
-                }
-            }
-        });
+        mt_sample_count<V, CHUNK, CS>(x, part * CHUNK, grid, grid.bin(mt_order_value((unsigned)(best >> 32))), by_p, bins);
         __syncthreads();
         for (unsigned b = t; b < BINS; b += LANES) bins_out[((size_t)row * S + part) * BINS + b] = bins[b];
     }
@@ -1109,12 +1122,16 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     mt_u64* held = cut_lds + WAVES + 8u + MT_SAMPLE_PARTS + 2u * MT_SAMPLE_CLOSE;
     const mt_asked asked(row, uniforms, temperatures, top_k, top_p, min_p);
     mt_u64 best = 0;
-    for (unsigned c = mt_lane(); c < S; c += 64u) {
-        const mt_u64 one = best_in[(size_t)row * S + c];
-        best = one > best ? one : best;
-        if (CUT && t < 64u) kept[c] = one;
+    if constexpr (S == 1u) {
+        best = mt_sample_best<V, CHUNK, CS>(x, 0u, lds);
+    } else {
+        for (unsigned c = mt_lane(); c < S; c += 64u) {
+            const mt_u64 one = best_in[(size_t)row * S + c];
+            best = one > best ? one : best;
+            if (CUT && t < 64u) kept[c] = one;
+        }
+        best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
     }
-    best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
     if (mt_sample_plain(best, asked.temperature, row, part == 0u && t == 0u, tokens, logprobs)) return;
     const mt_weights<SHIFT> weights{mt_order_value((unsigned)(best >> 32)), 1.0 / (double)asked.temperature};
     const mt_grid<BINS> grid(asked.temperature);
@@ -1133,6 +1150,19 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             mt_u64 number[EACH], mass[EACH], numbers = 0, masses = 0;
 #pragma unroll
             for (unsigned b = 0; b < EACH; ++b) number[b] = mass[b] = 0;
+            if constexpr (S == 1u) {
+                mt_u64* bins = held;  // (the list comes later)
+                for (unsigned b = t; b < BINS; b += LANES) bins[b] = 0;
+                __syncthreads();
+                mt_sample_count<V, CHUNK, CS>(x, 0u, grid, first, by_p, bins);
+                __syncthreads();
+#pragma unroll
+                for (unsigned b = 0; b < EACH; ++b) {
+                    const mt_u64 word = bins[t * EACH + b];
+                    number[b] = word >> MT_SAMPLE_COUNT_AT, mass[b] = word & ((1ull << MT_SAMPLE_COUNT_AT) - 1ull);
+                }
+                __syncthreads();
+            } else
 #pragma unroll
             for (unsigned c = 0; c < S; ++c) {  // (loads that do not wait for each other)
                 const float shift = first - grid.bin(mt_order_value((unsigned)(kept[c] >> 32)));

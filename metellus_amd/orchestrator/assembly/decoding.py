@@ -234,7 +234,7 @@ def _assemble_sample_scan(decision: DecisionView, op: SampleScanOp, function_nam
 def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | None) -> KernelGroup:
     rows, cols = op.logits.shape
     chunk, chunks = sample_chunks(rows, cols)
-    cuts = op.bins is not None
+    cuts = op.top_k is not None or op.top_p is not None
     sig = _Signature()
     args = (
         sig.add("logits", op.logits),
@@ -245,7 +245,7 @@ def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | 
         sig.add("min_p", op.min_p),
         _words(sig, "best", op.best),
         _words(sig, "bins", op.bins),
-        f"(unsigned*){sig.add('counts', op.counts, out=True)}",
+        "nullptr" if op.counts is None else f"(unsigned*){sig.add('counts', op.counts, out=True)}",
         _words(sig, "sums", op.sums, out=True),
         _words(sig, "list", op.listed, out=True),
         sig.add("tokens", op.tokens, out=True),

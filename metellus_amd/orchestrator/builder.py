@@ -618,39 +618,42 @@ class Operations:
             raise ValueError(f"sample logits must be 2D; got shape {tl.shape} ({tl.name!r})")
         rows, cols = tl.shape
         chunk, chunks = sample_chunks(rows, cols)
-        cuts = top_k is not None or top_p is not None
+        apart, cuts = chunks > 1, top_k is not None or top_p is not None
 
-        def made(part: str, rows: int, words: int) -> Tensor:
-            return self._fresh(f"{out}.{part}", (rows, 2 * words), "int32")
+        def made(part: str, rows: int, words: int, wanted: bool = True) -> Tensor | None:
+            return self._fresh(f"{out}.{part}", (rows, 2 * words), "int32") if wanted else None
 
-        scan = SampleScanOp(
-            best=made("best", rows * chunks, 1),
-            counts=made("counts", rows, 1),
-            logits=tl,
-            name=out,
-            bins=made("bins", rows * chunks, sample_bins(cols)) if cuts else None,
-            **{n: t if cuts else None for n, t in given.items() if n != "min_p"},
-            after=self._owners(tl, *given.values()),
-        )
         pick = SampleOp(
             tokens=self._fresh(out, (rows,), "int32"),
             logits=tl,
             uniforms=tu,
-            best=scan.best,
-            counts=scan.counts,
-            bins=scan.bins,
-            sums=made("sums", rows, (2 + chunk // 256) * chunks),
-            listed=made("list", rows, SAMPLE_LIST) if cuts else None,
+            best=made("best", rows * chunks, 1, apart),
+            counts=made("counts", rows, 1, apart),
+            bins=made("bins", rows * chunks, sample_bins(cols), apart and cuts),
+            sums=made("sums", rows, (2 + chunk // 256) * chunks, apart),
+            listed=made("list", rows, SAMPLE_LIST, apart and cuts),
             logprobs=None if logprobs is None else self._fresh(logprobs, (rows,), "float32"),
             after=self._owners(tl, tu, *given.values()),
             **given,
         )
-        names = [t.name for t in (*scan.outs, *pick.outs)]
+        if apart:
+            scan = SampleScanOp(
+                best=pick.best,
+                counts=pick.counts,
+                logits=tl,
+                name=out,
+                bins=pick.bins,
+                **{n: t if cuts else None for n, t in given.items() if n != "min_p"},
+                after=self._owners(tl, *given.values()),
+            )
+        names = [t.name for t in pick.outs]
         if len(set(names)) < len(names):
             raise ValueError(f"output names must differ; got {names}")
-        self._emit_all(scan)
+        if apart:
+            self._emit_all(scan)
         self._emit_all(pick)
-        self._scratch.update(t.name for t in (*scan.outs, pick.sums, pick.listed) if t is not None)
+        own = (pick.best, pick.counts, pick.bins, pick.sums, pick.listed)
+        self._scratch.update(t.name for t in own if t is not None)
         return pick.tokens
 
     # -- results -------------------------------------------------------------

@@ -341,9 +341,7 @@ class SampleScanOp(ServingOp):
     after: tuple[Tensor, ...] = ()
 
     def __post_init__(self) -> None:
-        rows, cols = _rows("sample logits", self.logits, "float32")
-        if cols > VOCABULARY_MAX:
-            raise ValueError(f"sample logits: at most {VOCABULARY_MAX} columns; got shape {self.logits.shape}")
+        rows, _ = _rows("sample logits", self.logits, "float32")
         for label, t, dtype in (("temperatures", self.temperatures, "float32"), ("top_k", self.top_k, "int32"),
                                 ("top_p", self.top_p, "float32")):
             if t is not None:
@@ -369,9 +367,10 @@ class SampleOp(ServingOp):
     tokens: Tensor
     logits: Tensor
     uniforms: Tensor
-    best: Tensor
-    counts: Tensor
-    sums: Tensor
+    # what rows of several chunks have between the kernels and between workgroups
+    best: Tensor | None = None
+    counts: Tensor | None = None
+    sums: Tensor | None = None
     bins: Tensor | None = None
     listed: Tensor | None = None
     logprobs: Tensor | None = None
@@ -382,7 +381,9 @@ class SampleOp(ServingOp):
     after: tuple[Tensor, ...] = ()
 
     def __post_init__(self) -> None:
-        rows, _ = _rows("sample logits", self.logits, "float32")
+        rows, cols = _rows("sample logits", self.logits, "float32")
+        if cols > VOCABULARY_MAX:
+            raise ValueError(f"sample logits: at most {VOCABULARY_MAX} columns; got shape {self.logits.shape}")
         for label, t, dtype in (("uniforms", self.uniforms, "float32"), ("temperatures", self.temperatures, "float32"),
                                 ("top_k", self.top_k, "int32"), ("top_p", self.top_p, "float32"),
                                 ("min_p", self.min_p, "float32")):

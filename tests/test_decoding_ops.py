@@ -11,7 +11,7 @@ import pytest
 
 from metellus_amd.api import compile_program
 from metellus_amd.orchestrator import Operations, Rotary
-from metellus_amd.orchestrator.decoding import adapter_splits
+from metellus_amd.orchestrator.decoding import adapter_splits, sample_chunks
 from metellus_amd.orchestrator.fusion import fuse
 from metellus_amd.orchestrator.scheduler import schedule
 from metellus_amd.runtime import hip_backend
@@ -234,6 +234,27 @@ def test_shares_of_columns():
     for rows in (1, 3, 50, 700, 1024, 5000):
         for inner in (1, 511, 513, 5003, 16384):
             assert 1 <= adapter_splits(rows, inner) <= -(-inner // 512)
+
+
+def test_scheduling_a_draw():
+    """Rows of several chunks take two kernels, whose own tensors are no outputs; short ones one."""
+    for cols, kernels in ((50, 1), (40000, 2)):
+        ops = _ops(**{**SAMPLE, "x": (3, cols)})
+        ops.sample("x", uniforms="u", out="t", top_k="k", top_p="p", logprobs="lp")
+        for name in SAMPLE:
+            t = ops.tensors[name]
+            ops.from_numpy(np.zeros(t.shape, t.stored), name)
+        steps = schedule(ops, compile_program(ops)).fragments
+        assert len([s for s in steps if isinstance(s, Dispatch)]) == kernels
+        assert sorted(s.into for s in steps if isinstance(s, Download)) == ["lp", "t"]
+
+
+def test_chunks_of_a_row():
+    assert sample_chunks(1, 131072) == (8192, 16) and sample_chunks(64, 131072) == (16384, 8) and sample_chunks(1, 70) == (4096, 1)
+    for rows in (1, 7, 300, 5000):
+        for cols in (1, 4096, 4097, 100003, 2**20):
+            chunk, chunks = sample_chunks(rows, cols)
+            assert chunks * chunk >= cols > (chunks - 1) * chunk and chunks <= 16 and (chunks == 1 or rows * chunks <= 512)
 
 
 # -- a rotation's frequencies --------------------------------------------------------

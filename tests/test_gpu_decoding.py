@@ -280,8 +280,9 @@ def test_adapters_by_group(ids):
     np.testing.assert_array_equal(y[none], ops.uploads["base"][none])
 
 
-def test_adapters_of_strided_rows():
-    _adapter_check(_adapters(19, 130, 70, 6, 3, [i % 4 - 1 for i in range(19)], strides=True))
+@pytest.mark.parametrize("rows", [19, 1030])
+def test_adapters_of_strided_rows(rows):
+    _adapter_check(_adapters(rows, 130, 70, 6, 3, [i % 4 - 1 for i in range(rows)], strides=True))
 
 
 def test_adapters_rows_do_not_mix():
@@ -438,10 +439,21 @@ def test_sample_many_rows_and_columns(rows, cols):
                               temperatures=rng.choice([0.0, 0.5, 1.0], rows)))
 
 
-def test_sample_of_strided_logits():
+def test_sample_a_bin_of_many():
+    """Rows of one chunk, all of whose logits are in one bin: more than 16 bits count."""
+    rows, cols = 260, 131072
+    u = (np.arange(rows) + 0.5) / rows
+    ops = _sample_ops(np.zeros((rows, cols), np.float32), u, top_k=70000)
+    assert len(ops.build()) == 1
+    t = run(ops).env["t"]
+    np.testing.assert_array_equal(t, np.floor(u.astype(np.float32).astype(np.float64) * 70000).astype(np.int32))
+
+
+@pytest.mark.parametrize("cols", [301, 30001])
+def test_sample_of_strided_logits(cols):
     rng = np.random.default_rng(9)
     ops = Operations()
-    _put(ops, "x_", rng.standard_normal((301, 4)).astype(np.float32))
+    _put(ops, "x_", rng.standard_normal((cols, 4)).astype(np.float32))
     ops.transpose("x_", out="x")
     _put(ops, "u", rng.random(4).astype(np.float32))
     _put(ops, "k", np.array([3, 0, 50, 1], np.int32))
