@@ -632,15 +632,41 @@ MT_INLINE double mt_exp_below(double z) {
     return some ? __builtin_bit_cast(double, bits) : 0.0;
 }
 
+// 2^(l / 64) for the lanes l of a wave, for mt_weights.
+constexpr unsigned MT_POWERS = 64u;
+MT_INLINE double mt_power(unsigned l) { return 2.0 * mt_exp_below(0x1.62e42fefa39efp-7 * ((double)l - 64.0)); }
+
 // The weights of a row.
 template <unsigned SHIFT>
 struct mt_weights {
     float top;
-    double by;  // one over the temperature
-    MT_INLINE double scaled(float x) const { return x == top ? 0.0 : ((double)x - (double)top) * by; }
+    double from;           // as `top`, and for +inf a number that +inf is above
+    double by;             // one over the temperature
+    const double* powers;  // 2^(l / 64), in LDS
+    MT_INLINE mt_weights(float largest, float temperature, const double* lds)
+        : top(largest), from(largest == INFINITY ? 1e308 : (double)largest), by(__builtin_fmax(1.0 / (double)temperature, 1e-300)),
+          powers(lds) {}
     // (an x that is -inf weighs nothing, and beside a top of +inf so do all others, whatever
-    // the temperature: what they are scaled to is -inf or no number)
-    MT_INLINE double weight(float x) const { return mt_exp_below(scaled(x)); }
+    // the temperature)
+    MT_INLINE double scaled(float x) const { return __builtin_fmin(((double)x - from) * by, 0.0); }
+    // e^z, z being x scaled, right to about 2^-50 of itself; nothing is a multiple of 2^-44
+    // below e^-708.  z = n log(2) / 64 + r, and the series of e^r: for |r| up to log(2) / 128
+    // its sixth term is under 2^-54.  (n is in the last bits of a sum with 1.5 2^52.  A series
+    // alone, of twelve products in turn, took 60 % longer.)
+    MT_INLINE double weight(float x) const {
+        const double z = __builtin_fmax(scaled(x), -708.0);
+        const double sum = __builtin_fma(z, 0x1.71547652b82fep+6, 0x1.8p52), n = sum - 0x1.8p52;
+        const unsigned whole_n = (unsigned)__builtin_bit_cast(mt_u64, sum);
+        const double power = powers[whole_n % MT_POWERS];
+        const double r = __builtin_fma(n, -0x1.abc9e3b39803fp-62, __builtin_fma(n, -0x1.62e42fefa39efp-7, z));  // (log 2 in two parts)
+        double e = __builtin_fma(1.0 / 120.0, r, 1.0 / 24.0);
+        e = __builtin_fma(e, r, 1.0 / 6.0);
+        e = __builtin_fma(e, r, 0.5);
+        e = __builtin_fma(e, r, 1.0);
+        e = __builtin_fma(e, r, 1.0) * power;
+        // (e is 0.99 to 2: its exponent takes the rest of n as it is)
+        return __builtin_bit_cast(double, __builtin_bit_cast(mt_u64, e) + ((mt_u64)((whole_n & ~(MT_POWERS - 1u)) << 14) << 32));
+    }
     // The nearest whole number of 2^-SHIFT: in the last bits of a sum with 1.5 2^52.
     MT_INLINE static mt_u64 whole(double w) {
         const double sum = __builtin_fma(w, (double)(1ull << SHIFT), 0x1.8p52);
@@ -888,26 +914,29 @@ struct mt_grid {
     MT_INLINE float bin(float x) const { return __builtin_floorf(x * by); }
 };
 
+// Four logits from i on, -inf behind the row's end.
+template <unsigned V, unsigned CS>
+MT_INLINE mt_f32x4 mt_sample_quad(const float* x, unsigned i) {
+    mt_f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (i < V) {
+        v = mt_row4<V, CS>(x, i);
+#pragma unroll
+        for (unsigned j = 1; j < 4u; ++j)
+            if (V % 4u != 0u && i + j >= V) v[j] = -INFINITY;
+    }
+    return v;
+}
+
 // Calls f(q, i, v) for this lane's quads of the chunk from i0 on, of which the q-th of all
-// lanes are 1024 neighbours: i is the first one's index, v the four, -inf behind the row's
-// end.  Four quads are loaded while the four before are looked at.
+// lanes are 2048 neighbours: i is the first one's index, v the four.  Four quads are loaded
+// while the four before are looked at.
 template <unsigned V, unsigned CHUNK, unsigned CS, typename F>
 MT_INLINE void mt_sample_each(const float* x, unsigned i0, F f) {
     constexpr unsigned QUADS = CHUNK / (4u * MT_SAMPLE_LANES);
     constexpr unsigned DEEP = QUADS < 4u ? QUADS : 4u;
     static_assert(QUADS % DEEP == 0u, "whole sets of quads");
     const auto index = [&](unsigned q) { return i0 + 4u * (threadIdx.x + MT_SAMPLE_LANES * q); };
-    const auto load = [&](unsigned q) {
-        mt_f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const unsigned i = index(q);
-        if (q < QUADS && i < V) {
-            v = mt_row4<V, CS>(x, i);
-#pragma unroll
-            for (unsigned j = 1; j < 4u; ++j)
-                if (V % 4u != 0u && i + j >= V) v[j] = -INFINITY;
-        }
-        return v;
-    };
+    const auto load = [&](unsigned q) { return mt_sample_quad<V, CS>(x, q < QUADS ? index(q) : V); };
     mt_f32x4 next[DEEP];
 #pragma unroll
     for (unsigned q = 0; q < DEEP; ++q) next[q] = load(q);
@@ -921,11 +950,43 @@ MT_INLINE void mt_sample_each(const float* x, unsigned i0, F f) {
     }
 }
 
-// The first of a chunk's largest, in all lanes.
+// mt_sample_each as an object, called as often as its logits are looked at; the second has
+// what a lane looks at in registers where that is eight quads or less, and loads them once.
 template <unsigned V, unsigned CHUNK, unsigned CS>
-MT_INLINE mt_u64 mt_sample_best(const float* x, unsigned i0, mt_u64* lds) {
+struct mt_sample_again {
+    const float* x;
+    unsigned i0;
+    template <typename F>
+    MT_INLINE void operator()(F f) const { mt_sample_each<V, CHUNK, CS>(x, i0, f); }
+};
+template <unsigned V, unsigned CHUNK, unsigned CS>
+struct mt_sample_kept {
+    static constexpr unsigned QUADS = CHUNK / (4u * MT_SAMPLE_LANES);
+    static constexpr bool KEEPS = QUADS <= 8u;
+    const float* x;
+    unsigned i0;
+    mt_f32x4 held[KEEPS ? QUADS : 1u];
+    MT_INLINE mt_sample_kept(const float* row, unsigned from) : x(row), i0(from) {
+        if constexpr (KEEPS)
+#pragma unroll
+            for (unsigned q = 0; q < QUADS; ++q) held[q] = mt_sample_quad<V, CS>(x, index(q));
+    }
+    MT_INLINE unsigned index(unsigned q) const { return i0 + 4u * (threadIdx.x + MT_SAMPLE_LANES * q); }
+    template <typename F>
+    MT_INLINE void operator()(F f) const {
+        if constexpr (KEEPS) {
+#pragma unroll
+            for (unsigned q = 0; q < QUADS; ++q) f(q, index(q), held[q]);
+        } else
+            mt_sample_each<V, CHUNK, CS>(x, i0, f);
+    }
+};
+
+// The first of a chunk's largest, in all lanes.
+template <unsigned V, typename EACH>
+MT_INLINE mt_u64 mt_sample_best(EACH each, mt_u64* lds) {
     mt_u64 best = 0;
-    mt_sample_each<V, CHUNK, CS>(x, i0, [&](unsigned, unsigned i, mt_f32x4 v) {
+    each([&](unsigned, unsigned i, mt_f32x4 v) {
 #pragma unroll
         for (unsigned j = 0; j < 4u; ++j) {
             const mt_u64 found = i + j < V ? mt_best(i + j, v[j]) : 0;
@@ -937,9 +998,9 @@ MT_INLINE mt_u64 mt_sample_best(const float* x, unsigned i0, mt_u64* lds) {
 
 // A chunk's logits, and about what they weigh where asked, added to the bins in LDS, which are 0;
 // `first`: the bin of its largest.
-template <unsigned V, unsigned CHUNK, unsigned CS, unsigned BINS>
-MT_INLINE void mt_sample_count(const float* x, unsigned i0, const mt_grid<BINS>& grid, float first, bool weigh, mt_u64* bins) {
-    mt_sample_each<V, CHUNK, CS>(x, i0, [&](unsigned, unsigned, mt_f32x4 v) {
+template <unsigned BINS, typename EACH>
+MT_INLINE void mt_sample_count(EACH each, const mt_grid<BINS>& grid, float first, bool weigh, mt_u64* bins) {
+    each([&](unsigned, unsigned, mt_f32x4 v) {
 #pragma unroll
         for (unsigned j = 0; j < 4u; ++j) {
             const float f = grid.bin(v[j]), below = first - f;
@@ -964,14 +1025,15 @@ MT_INLINE void mt_sample_scan(const float* logits, const float* temperatures, co
     mt_u64* bins = lds + MT_SAMPLE_WAVES;
     if (CUT)
         for (unsigned b = t; b < BINS; b += LANES) bins[b] = 0;
-    const mt_u64 best = mt_sample_best<V, CHUNK, CS>(x, part * CHUNK, lds);
+    const mt_sample_kept<V, CHUNK, CS> each(x, part * CHUNK);
+    const mt_u64 best = mt_sample_best<V>(each, lds);
     if (t == 0u) best_out[(size_t)row * S + part] = best;
     if constexpr (CUT) {
         const float temperature = temperatures != nullptr ? temperatures[row] : 1.f;
         const bool by_p = top_p != nullptr && top_p[row] < 1.f, by_k = top_k != nullptr && top_k[row] > 0;
         if (!(temperature > 0.f) || !(by_p || by_k)) return;
         const mt_grid<BINS> grid(temperature);
-        mt_sample_count<V, CHUNK, CS>(x, part * CHUNK, grid, grid.bin(mt_order_value((unsigned)(best >> 32))), by_p, bins);
+        mt_sample_count(each, grid, grid.bin(mt_order_value((unsigned)(best >> 32))), by_p, bins);
         __syncthreads();
         for (unsigned b = t; b < BINS; b += LANES) bins_out[((size_t)row * S + part) * BINS + b] = bins[b];
     }
@@ -1116,14 +1178,17 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     const auto get = [](const mt_u64* from) {
         return __hip_atomic_load(const_cast<mt_u64*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     };
-    // LDS: the folds' words and some results, four more, what stays of each segment; for cuts,
+    // LDS: powers, the folds' words and some results, four more, what stays of each segment; for cuts,
     // mt_list_cut's, and the list
+    const double* powers = reinterpret_cast<const double*>(lds);
+    if (t < MT_POWERS) lds[t] = __builtin_bit_cast(mt_u64, mt_power(t));  // (read behind the next barrier)
+    lds += MT_POWERS;
     mt_u64 *words = lds + WAVES + 4u, *kept = words + 4u, *cut_lds = kept + S * SEGMENTS;
     mt_u64* held = cut_lds + WAVES + 8u + MT_SAMPLE_PARTS + 2u * MT_SAMPLE_CLOSE;
     const mt_asked asked(row, uniforms, temperatures, top_k, top_p, min_p);
     mt_u64 best = 0;
     if constexpr (S == 1u) {
-        best = mt_sample_best<V, CHUNK, CS>(x, 0u, lds);
+        best = mt_sample_best<V>(mt_sample_again<V, CHUNK, CS>{x, 0u}, lds);
     } else {
         for (unsigned c = mt_lane(); c < S; c += 64u) {
             const mt_u64 one = best_in[(size_t)row * S + c];
@@ -1133,7 +1198,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
         best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
     }
     if (mt_sample_plain(best, asked.temperature, row, part == 0u && t == 0u, tokens, logprobs)) return;
-    const mt_weights<SHIFT> weights{mt_order_value((unsigned)(best >> 32)), 1.0 / (double)asked.temperature};
+    const mt_weights<SHIFT> weights(mt_order_value((unsigned)(best >> 32)), asked.temperature, powers);
     const mt_grid<BINS> grid(asked.temperature);
     const float first = grid.bin(weights.top);
 
@@ -1154,7 +1219,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
                 mt_u64* bins = held;  // (the list comes later)
                 for (unsigned b = t; b < BINS; b += LANES) bins[b] = 0;
                 __syncthreads();
-                mt_sample_count<V, CHUNK, CS>(x, 0u, grid, first, by_p, bins);
+                mt_sample_count(mt_sample_again<V, CHUNK, CS>{x, 0u}, grid, first, by_p, bins);
                 __syncthreads();
 #pragma unroll
                 for (unsigned b = 0; b < EACH; ++b) {
@@ -1224,32 +1289,49 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     if (!whole) {
         mt_u64 all = 0, above = 0;
         const bool weigh_all = by_p && !by_k;
+        // what is above this stays as far as the bins say, and of what is above that all is weighed
+        const float whole_from = cuts ? (float)from : INFINITY, weighed = weigh_all ? INFINITY : whole_from;
+        for (unsigned c = t; c < SEGMENTS; c += LANES) kept[c] = 0;
+        __syncthreads();
         mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned q, unsigned i, mt_f32x4 v) {
-            const float most = __builtin_fmaxf(__builtin_fmaxf(v[0], v[1]), __builtin_fmaxf(v[2], v[3]));
-            const float nearest = CUT ? first - grid.bin(most) : 0.f;
+            float below[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (CUT)
+#pragma unroll
+                for (unsigned j = 0; j < 4u; ++j) below[j] = first - grid.bin(v[j]);
+            const float nearest = __builtin_fminf(__builtin_fminf(below[0], below[1]), __builtin_fminf(below[2], below[3]));
             mt_u64 stay = 0;
-            if (!CUT || !cuts || weigh_all || nearest < (float)from) {
+            if (!CUT || __ballot(!(nearest >= weighed)) != 0) {
 #pragma unroll
                 for (unsigned j = 0; j < 4u; ++j) {
                     const double w = weights.weight(v[j]);
                     const mt_u64 h = weights.whole(w);
-                    all += h;
-                    if (!CUT || !cuts || first - grid.bin(v[j]) < (float)from) above += h, stay += w < asked.least ? 0 : h;
+                    const bool in = !CUT || !(below[j] >= whole_from);
+                    all += h, above += in ? h : 0, stay += in && w >= asked.least ? h : 0;
                 }
             }
-            if (CUT && cuts && nearest <= (float)upto) {
+            if (CUT && cuts && __ballot(nearest <= (float)upto) != 0) {
+                // one place in the list for all of the wave's, then each its own
+                mt_u64 listed[4];
+                unsigned number = 0u, to = 0u;
 #pragma unroll
                 for (unsigned j = 0; j < 4u; ++j) {
-                    const float below = first - grid.bin(v[j]);
-                    if (below >= (float)from && below <= (float)upto) {
-                        const unsigned to = (unsigned)atomicAdd(words + 3, 1ull);
-                        if (to < MT_SAMPLE_LIST) held[to] = mt_best(i + j, v[j]);
-                    }
+                    listed[j] = __ballot(below[j] >= (float)from && below[j] <= (float)upto);
+                    number += (unsigned)__builtin_popcountll(listed[j]);
+                }
+                if (mt_lane() == 0u && number != 0u) to = atomicAdd((unsigned*)(words + 3), number);
+                to = (unsigned)__builtin_amdgcn_readfirstlane((int)to);
+#pragma unroll
+                for (unsigned j = 0; j < 4u; ++j) {
+                    const unsigned own = __builtin_amdgcn_mbcnt_hi((unsigned)(listed[j] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)listed[j], to));
+                    if (below[j] >= (float)from && below[j] <= (float)upto && own < MT_SAMPLE_LIST) held[own] = mt_best(i + j, v[j]);
+                    to += (unsigned)__builtin_popcountll(listed[j]);
                 }
             }
             if (from != 0u) {  // (else nothing stays before the list is looked at)
-                stay = mt_wave_upto(stay);
-                if (mt_lane() == 63u) kept[q * WAVES + mt_wave()] = stay;
+                stay = mt_add_from<0x112, 15>(mt_add_from<0x111, 15>(stay));  // over four lanes
+                unsigned to = q * WAVES + mt_wave();
+                asm volatile("" : "+v"(to));  // (else lanes are added up one after another before the atomic)
+                if ((mt_lane() & 3u) == 3u) atomicAdd(kept + to, stay);
             }
         });
         if (weigh_all) {
@@ -1289,8 +1371,6 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
                     row_all = mt_wave_sum(one_all), row_above = mt_wave_sum(one_above);
                 }
             }
-        } else if (from == 0u) {
-            for (unsigned c = t; c < SEGMENTS; c += LANES) kept[c] = 0;
         }
         __syncthreads();
         if (CUT && by_k && from == 0u && n <= MT_SAMPLE_SHORT) {

@@ -258,8 +258,8 @@ def _assemble_sample(decision: DecisionView, op: SampleOp, function_name: str | 
         "mt_sample_pick",
         (cols, chunk, chunks, sample_bins(cols), shift, *_strides(op.logits), cuts),
         args,
-        # (one workgroup for a whole row takes two words a wave and 256)
-        lds_bytes=8 * max(SAMPLE_WAVES + 8 + chunk * chunks // 256 + (SAMPLE_CUT_WORDS + SAMPLE_LIST if cuts else 0), 2 * SAMPLE_WAVES + 256),
+        # (64 powers; one workgroup for a whole row takes two words a wave and 256)
+        lds_bytes=8 * (64 + max(SAMPLE_WAVES + 8 + chunk * chunks // 256 + (SAMPLE_CUT_WORDS + SAMPLE_LIST if cuts else 0), 2 * SAMPLE_WAVES + 256)),
         name="sample",
     )
     return _group(decision, sig, frag, function_name or f"sample_{op.tokens.name}", {}, (rows * chunks, 1, 1), 64 * SAMPLE_WAVES,
