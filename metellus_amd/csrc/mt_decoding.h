@@ -290,6 +290,9 @@ MT_INLINE mt_f32x4 mt_quad_in(const float* row, unsigned c) {
     return mt_f32x4{row[(size_t)c * CS], row[(size_t)(c + 1u) * CS], row[(size_t)(c + 2u) * CS], row[(size_t)(c + 3u) * CS]};
 }
 
+// A row of `down`, in whole quads.
+MT_INLINE constexpr unsigned mt_quads(unsigned ranks) { return (ranks + 3u) / 4u * 4u; }
+
 // A's part: blocks of RB x 16 ranks; the waves of the SPLITS workgroups of a group take
 // 64 columns of x in turn and add up in LDS; each split stores its part.  Loads of 16
 // columns go out as the registers of those 64 before are free, so MFMAs and memory go on
@@ -390,14 +393,10 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
                 for (unsigned w = 1; w < WAVES; ++w) v = v + lds[w * MB * RB * 64u + e];
                 const unsigned m = e / (64u * RB) * 16u + e % 16u, r = r0 + e / 64u % RB * 16u + e / 16u % 4u * 4u;
                 if ((group >> m) & 1ull) {
-                    float* to = down + ((size_t)split * rows + tile.row0 + m) * R;
-                    if (R % 4u == 0u) {
-                        if (r < R) mt_st4(to + r, v);
-                    } else {
+                    // (nothing behind R: the last of A's rows stood in for those)
 #pragma unroll
-                        for (unsigned i = 0; i < 4u; ++i)
-                            if (r + i < R) to[r + i] = v[i];
-                    }
+                    for (unsigned i = 1; i < 4u; ++i) v[i] = r + i < R ? v[i] : 0.f;
+                    if (r < R) mt_st4(down + ((size_t)split * rows + tile.row0 + m) * mt_quads(R) + r, v);
                 }
             }
         }
@@ -459,7 +458,7 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
                 if (((group >> m) & 1ull) && id >= 0 && r < R) {
 #pragma unroll
                     for (unsigned s = 0; s < SPLITS; ++s)
-                        sum = sum + mt_row4<R, 1u>(down + ((size_t)s * rows + tile.row0 + m) * R, r);
+                        sum = sum + mt_ld4(down + ((size_t)s * rows + tile.row0 + m) * mt_quads(R) + r);
                 }
                 *reinterpret_cast<mt_f32x4*>(lds + m * PITCH + r) = sum;
             }

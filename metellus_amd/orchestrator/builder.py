@@ -565,7 +565,7 @@ class Operations:
             raise ValueError(f"adapters x and base must have as many rows; got {tx.shape} and {ty.shape}")
         splits = adapter_splits(*tx.shape)
         down = AdapterDownOp(
-            down=self._fresh(f"{out}.down", (splits * tx.shape[0], rank), "float32"),
+            down=self._fresh(f"{out}.down", (splits * tx.shape[0], -(-rank // 4) * 4), "float32"),
             x=tx,
             a=ta,
             ids=ti,

@@ -241,7 +241,8 @@ class RotaryOp(ServingOp):
 @dataclass(frozen=True)
 class AdapterDownOp(ServingOp):
     """Part s of ``down`` (``splits`` parts of x's rows): x[m] . A[ids[m]] over the
-    s-th share of the columns; rows whose id is no adapter's are not written."""
+    s-th share of the columns, ranks in whole fours; rows whose id is no adapter's are not
+    written."""
 
     down: Tensor
     x: Tensor

@@ -100,14 +100,14 @@ def _adapter_down(op, get):
     for m, i in enumerate(get(op.ids)):
         if 0 <= i < op.held:
             with np.errstate(all="ignore"):
-                down[m] = a[i * op.rank : (i + 1) * op.rank] @ x[m]  # (the first part has it all)
+                down[m, : op.rank] = a[i * op.rank : (i + 1) * op.rank] @ x[m]  # (the first part has it all)
     return {op.down.name: down}
 
 
 def _adapter_up(op, get):
     y, b = get(op.base).astype(F64), np.ascontiguousarray(get(op.b)).astype(F64)
     n = y.shape[1]
-    down = get(op.down).astype(F64).reshape(op.splits, -1, op.rank).sum(axis=0)
+    down = get(op.down).astype(F64).reshape(op.splits, -1, op.down.shape[1]).sum(axis=0)[:, : op.rank]
     for m, i in enumerate(get(op.ids)):
         if 0 <= i < op.held:
             with np.errstate(all="ignore"):
