@@ -262,6 +262,7 @@ struct mt_adapter_place {
 template <unsigned COLS, unsigned CS>
 MT_INLINE mt_f32x4 mt_quad(const float* row, unsigned c) {
     mt_f32x4 v;
+    asm volatile("" : "+v"(c));  // (known to no other round)
     if constexpr (CS == 1u && COLS >= 4u) {
         const unsigned at = c < COLS - 4u ? c : COLS - 4u, by = c - at;
         const mt_f32x4 w = mt_ld4u(row + at);
