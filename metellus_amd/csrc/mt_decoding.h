@@ -10,6 +10,85 @@
 //   * mt_sample         tokens from logits and given random numbers
 
 // ---------------------------------------------------------------------------
+// Sums over lanes.
+// ---------------------------------------------------------------------------
+
+typedef unsigned long long mt_u64;
+
+template <typename OP>
+MT_INLINE mt_u64 mt_wave_fold(mt_u64 v, OP op) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = op(v, (mt_u64)__shfl_xor(v, off, 64));
+    return v;
+}
+
+// The sum of v over this lane and those before it, by adding from one lane, two, four and
+// eight before in rows of 16, then from the ends of the rows before.
+template <int FROM, int ROWS>
+MT_INLINE mt_u64 mt_add_from(mt_u64 v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, FROM, ROWS, 15, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), FROM, ROWS, 15, false);
+    return v + (((mt_u64)hi << 32) | lo);
+}
+MT_INLINE mt_u64 mt_wave_upto(mt_u64 v) {
+    v = mt_add_from<0x111, 15>(v);  // row_shr:1
+    v = mt_add_from<0x112, 15>(v);
+    v = mt_add_from<0x114, 15>(v);
+    v = mt_add_from<0x118, 15>(v);
+    v = mt_add_from<0x142, 10>(v);  // row_bcast:15 into rows 1 and 3
+    return mt_add_from<0x143, 12>(v);  // row_bcast:31 into rows 2 and 3
+}
+// The last lane's word.
+MT_INLINE mt_u64 mt_wave_last(mt_u64 v) {
+    return ((mt_u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), 63) << 32) |
+           (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, 63);
+}
+MT_INLINE mt_u64 mt_wave_sum(mt_u64 v) { return mt_wave_last(mt_wave_upto(v)); }
+
+// v (op) over the workgroup's waves; `lds` holds a word a wave.
+template <unsigned WAVES, typename OP>
+MT_INLINE mt_u64 mt_group_fold(mt_u64 v, mt_u64* lds, OP op) {
+    v = mt_wave_fold(v, op);
+    __syncthreads();
+    if (mt_lane() == 0u) lds[mt_wave()] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (unsigned w = 1; w < WAVES; ++w) v = op(v, lds[w]);
+    return v;
+}
+
+// The sum of v over the workgroup.
+template <unsigned WAVES>
+MT_INLINE mt_u64 mt_group_sum(mt_u64 v, mt_u64* lds) {
+    v = mt_wave_sum(v);
+    __syncthreads();
+    if (mt_lane() == 0u) lds[mt_wave()] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (unsigned w = 0; w < WAVES; ++w) v += lds[w];
+    return v;
+}
+
+// The sum of v over the lanes before this one; `all`: over all of them.
+template <unsigned WAVES>
+MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
+    const mt_u64 sum = mt_wave_upto(v);
+    __syncthreads();
+    if (mt_lane() == 63u) lds[mt_wave()] = sum;
+    __syncthreads();
+    mt_u64 before = 0;
+    all = 0;
+#pragma unroll
+    for (unsigned w = 0; w < WAVES; ++w) {
+        before += w < mt_wave() ? lds[w] : 0;
+        all += lds[w];
+    }
+    return before + sum - v;
+}
+
+// ---------------------------------------------------------------------------
 // Block tables.  A sequence goes from `begin` positions to `end`: of its table's row it
 // has `have` entries and needs `need` more.  Every workgroup adds up all sequences
 // (8 bytes each), lane t the `each` sequences from t each on, and keeps the sums before
@@ -211,20 +290,100 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // four neighbours of row m = n of `down` or `out`.
 // ---------------------------------------------------------------------------
 
+// Rows are put in order before they are cut into tiles, MT_ADAPTER_ORDERED at a time: by id
+// (by a part of it: rows in one part stay as they are), and rows of an id in their own order,
+// so that all workgroups find the same.  Where ids change less than twice a tile they stay as
+// they are.  Each workgroup counts all of the rows' ids for itself and keeps the rows of its
+// tile: rows[m], m < TILE, or nothing behind the last.  (us, rank 64 of 4096 x 4096, in
+// the order they come in and in this: ids drawn from 64 150 rows 56, 46; 600 rows 163, 78; 2048
+// rows 632, 72; ids of 8 prompts 150 rows 21.5, 22.5; 600 rows 45.5, 48.6; 4096 rows 72, 75.)
+// `lds`: WAVES words of sums, WAVES times BINS numbers, and a byte a row.
+constexpr unsigned MT_ADAPTER_BINS = 256u, MT_ADAPTER_ORDERED = 4096u;
+constexpr unsigned MT_ADAPTER_ROWS = 64u;  // words of LDS, in front of all others, for a tile's rows
+template <unsigned TILE, unsigned WAVES>
+MT_INLINE void mt_adapter_order(const int* ids, unsigned tile, unsigned all_rows, unsigned* rows, mt_u64* lds) {
+    constexpr unsigned LANES = 64u * WAVES, BINS = MT_ADAPTER_BINS;
+    static_assert(LANES == BINS, "a lane for each bin");
+    unsigned* counts = reinterpret_cast<unsigned*>(lds + WAVES);
+    unsigned char* keys = reinterpret_cast<unsigned char*>(counts + WAVES * BINS);
+    const unsigned from = tile * TILE / MT_ADAPTER_ORDERED * MT_ADAPTER_ORDERED, begin = tile * TILE - from;
+    const unsigned n = all_rows - from < MT_ADAPTER_ORDERED ? all_rows - from : MT_ADAPTER_ORDERED;
+    const unsigned t = threadIdx.x, wave = mt_wave();
+    constexpr unsigned EACH = MT_ADAPTER_ORDERED / LANES;
+    unsigned id[EACH], last[EACH], changes = 0u;  // (all loaded before the first is looked at)
+#pragma unroll
+    for (unsigned e = 0; e < EACH; ++e) {
+        id[e] = last[e] = 0u;
+        if (e * LANES < n) {
+            const unsigned i = e * LANES + t < n ? e * LANES + t : n - 1u;
+            id[e] = (unsigned)ids[from + i], last[e] = (unsigned)ids[from + (i != 0u ? i - 1u : 0u)];
+        }
+    }
+#pragma unroll
+    for (unsigned e = 0; e < EACH; ++e)
+        if (e * LANES + t < n) {
+            changes += id[e] != last[e] ? 1u : 0u;
+            keys[e * LANES + t] = (unsigned char)(id[e] % BINS);
+        }
+    for (unsigned c = t; c < WAVES * BINS; c += LANES) counts[c] = 0u;
+    mt_u64 all;
+    mt_group_before<WAVES>(changes, lds, all);
+    if (all < 2u * ((n + TILE - 1u) / TILE)) {  // (the same in all workgroups)
+        if (t < TILE) rows[t] = from + begin + t;
+        __syncthreads();
+        return;
+    }
+    // wave w counts the w-th share of the rows, and goes through it in order
+    const unsigned share = (n + LANES - 1u) / LANES * 64u, first = wave * share, end = first + share < n ? first + share : n;
+    for (unsigned i = first + mt_lane(); i < end; i += 64u) atomicAdd(counts + wave * BINS + keys[i], 1u);
+    __syncthreads();
+    unsigned number = 0u;
+#pragma unroll
+    for (unsigned w = 0; w < WAVES; ++w) number += counts[w * BINS + t];
+    unsigned place = (unsigned)mt_group_before<WAVES>(number, lds, all);
+#pragma unroll
+    for (unsigned w = 0; w < WAVES; ++w) {
+        const unsigned own = counts[w * BINS + t];
+        counts[w * BINS + t] = place;
+        place += own;
+    }
+    __syncthreads();
+    for (unsigned i0 = first; i0 < end; i0 += 64u) {
+        const unsigned i = i0 + mt_lane();
+        const unsigned key = i < end ? keys[i] : 0u;
+        mt_u64 alike = __ballot(i < end);
+#pragma unroll
+        for (unsigned bit = 1u; bit < BINS; bit *= 2u) {
+            const mt_u64 has = __ballot((key & bit) != 0u);
+            alike &= (key & bit) != 0u ? has : ~has;
+        }
+        const unsigned before = __builtin_amdgcn_mbcnt_hi((unsigned)(alike >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)alike, 0u));
+        const unsigned base = counts[wave * BINS + key];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (i < end) {
+            if (before == 0u) counts[wave * BINS + key] = base + (unsigned)__builtin_popcountll(alike);
+            if (base + before - begin < TILE) rows[base + before - begin] = from + i;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+}
+
 // The rows of a tile, and the groups that they lead.
-template <unsigned MB, unsigned HELD>
+template <unsigned MB, unsigned HELD, bool ORDER>
 struct mt_adapter_rows {
     static constexpr unsigned TILE = 16u * MB;
-    unsigned row0, mine;  // the tile's first row, the id of this lane's (-1: none, -2: no row)
-    MT_INLINE mt_adapter_rows(const int* ids, unsigned tile, unsigned rows) : row0(tile * TILE) {
-        const unsigned row = row0 + mt_lane() % TILE;
-        int found = -2;
-        if (row < rows) {
-            found = ids[row];
-            if (found < 0 || (unsigned)found >= HELD) found = -1;
+    unsigned row0, mine;       // the tile's first row, the id of this lane's (-1: none, -2: no row)
+    const unsigned* in_order;  // the rows, in LDS
+    MT_INLINE mt_adapter_rows(unsigned tile, const unsigned* lds) : row0(tile * TILE), mine(0xFFFFFFFEu), in_order(lds) {}
+    MT_INLINE void of(const int* ids, unsigned rows) {
+        if (row0 + mt_lane() % TILE < rows) {
+            const int found = ids[row(mt_lane() % TILE)];
+            mine = found < 0 || (unsigned)found >= HELD ? 0xFFFFFFFFu : (unsigned)found;
         }
-        mine = (unsigned)found;
     }
+    // The m-th row.
+    MT_INLINE unsigned row(unsigned m) const { return ORDER ? in_order[m] : row0 + m; }
     // Of the tile's rows: bit m says whether row m is of the group that row j leads; 0 where
     // j leads none.
     MT_INLINE unsigned long long group(unsigned j, int& id) const {
@@ -298,9 +457,9 @@ MT_INLINE constexpr unsigned mt_quads(unsigned ranks) { return (ranks + 3u) / 4u
 // 64 columns of x in turn and add up in LDS; each split stores its part.  Loads of 16
 // columns go out as the registers of those 64 before are free, so MFMAs and memory go on
 // together.  Lanes of rows of other groups load the leader's, which are loaded anyway.
-template <unsigned K, unsigned R, unsigned RB, unsigned MB, bool LOOP, unsigned SPLITS, unsigned HELD, unsigned WAVES,
-          unsigned XRS, unsigned XCS>
-MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, float* down, unsigned rows,
+template <unsigned K, unsigned R, unsigned RB, unsigned MB, bool LOOP, bool ORDER, unsigned SPLITS, unsigned HELD,
+          unsigned WAVES, unsigned XRS, unsigned XCS>
+MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, float* down, int* order, unsigned rows,
                                mt_f32x4* lds) {
     constexpr unsigned TILE = 16u * MB, STEP = 64u * SPLITS * WAVES, WHOLE = K / 64u * 64u;
     // Sums that an MFMA does not wait for the one before with, added at the end: few tiles are
@@ -310,7 +469,17 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
     const mt_adapter_place<LOOP> at(tiles);
     const unsigned split = at.share % SPLITS, r0 = at.share / SPLITS * RB * 16u;
     if (at.tile >= tiles) return;
-    const mt_adapter_rows<MB, HELD> tile(ids, at.tile, rows);
+    unsigned* in_order = reinterpret_cast<unsigned*>(lds);
+    if constexpr (ORDER) {
+        lds += MT_ADAPTER_ROWS / 4u;
+        mt_adapter_order<TILE, WAVES>(ids, at.tile, rows, in_order, reinterpret_cast<mt_u64*>(lds));
+    }
+    mt_adapter_rows<MB, HELD, ORDER> tile(at.tile, in_order);
+    tile.of(ids, rows);
+    if (ORDER && at.share == 0u && blockIdx.y == 0u && threadIdx.x < TILE && tile.row0 + lane < rows) {  // for the second kernel
+        order[2u * (size_t)(tile.row0 + lane)] = (int)in_order[lane];
+        order[2u * (size_t)(tile.row0 + lane) + 1u] = (int)tile.mine;
+    }
 #pragma unroll 1
     for (unsigned j = blockIdx.y; j < TILE; ++j) {
         int id;
@@ -321,7 +490,7 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
 #pragma unroll
             for (unsigned m = 0; m < MB; ++m) {
                 const unsigned row = (group >> (16u * m + n)) & 1ull ? 16u * m + n : j;
-                xr[m] = x + (size_t)(tile.row0 + row) * XRS;
+                xr[m] = x + (size_t)tile.row(row) * XRS;
 #pragma unroll
                 for (unsigned b = 0; b < RB; ++b)
 #pragma unroll
@@ -397,7 +566,7 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
                     // (nothing behind R: the last of A's rows stood in for those)
 #pragma unroll
                     for (unsigned i = 1; i < 4u; ++i) v[i] = r + i < R ? v[i] : 0.f;
-                    if (r < R) mt_st4(down + ((size_t)split * rows + tile.row0 + m) * mt_quads(R) + r, v);
+                    if (r < R) mt_st4(down + ((size_t)split * rows + tile.row(m)) * mt_quads(R) + r, v);
                 }
             }
         }
@@ -410,16 +579,28 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
 // rows goes through LDS on its way out, where rows become what lanes next to each other have:
 // base is read and the output written 64 BL bytes of a row at a time, and by the four waves
 // 256 BL (4096 rows of 4096, rank 64: 64 bytes of a row at a time 58 us).
-template <unsigned N, unsigned R, unsigned MB, bool LOOP, unsigned SPLITS, unsigned HELD, unsigned WAVES, unsigned PER,
-          unsigned BL, unsigned YRS, unsigned YCS>
-MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* b, const int* ids, const float* scales,
-                             float* out, unsigned rows, float* lds) {
+template <unsigned N, unsigned R, unsigned MB, bool LOOP, bool ORDER, unsigned SPLITS, unsigned HELD, unsigned WAVES,
+          unsigned PER, unsigned BL, unsigned YRS, unsigned YCS>
+MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* b, const int* ids, const int* order,
+                             const float* scales, float* out, unsigned rows, float* lds) {
     constexpr unsigned RC = (R + 15u) / 16u, TILE = 16u * MB, PITCH = 16u * RC + 4u, WIDE = 16u * BL, OUT_PITCH = WIDE + 4u;
     constexpr unsigned ALONG = 4u * BL, ABREAST = 64u / ALONG;  // lanes along a row, and rows at a time
     const unsigned tiles = (rows + TILE - 1u) / TILE, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
     const mt_adapter_place<LOOP> at(tiles);
     if (at.tile >= tiles) return;
-    const mt_adapter_rows<MB, HELD> tile(ids, at.tile, rows);
+    unsigned* in_order = reinterpret_cast<unsigned*>(lds);
+    mt_adapter_rows<MB, HELD, ORDER> tile(at.tile, in_order);
+    if constexpr (ORDER) {
+        lds += MT_ADAPTER_ROWS;
+        const unsigned m = lane % TILE;
+        if (tile.row0 + m < rows) {
+            const int* one = order + 2u * (size_t)(tile.row0 + m);
+            tile.mine = (unsigned)one[1];
+            if (threadIdx.x < TILE) in_order[m] = (unsigned)one[0];
+        }
+        __syncthreads();
+    } else
+        tile.of(ids, rows);
     float* turn = lds + TILE * PITCH + mt_wave() * 16u * OUT_PITCH;  // this wave's block of rows
 #pragma unroll 1
     for (unsigned j = blockIdx.y; j < TILE; ++j) {
@@ -445,7 +626,7 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
 #pragma unroll
                 for (unsigned q = 0; q < BL; ++q) {
                     const unsigned row = 16u * m + q * ABREAST + lane / ALONG;
-                    const float* yr = base + (size_t)(tile.row0 + ((group >> row) & 1ull ? row : j)) * YRS;
+                    const float* yr = base + (size_t)tile.row((group >> row) & 1ull ? row : j) * YRS;
                     if (from + WIDE <= N) v[q] = mt_quad_in<YCS>(yr, col);
                     else v[q] = mt_quad<N, YCS, LOOP>(yr, col);
                 }
@@ -459,7 +640,7 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
                 if (((group >> m) & 1ull) && id >= 0 && r < R) {
 #pragma unroll
                     for (unsigned s = 0; s < SPLITS; ++s)
-                        sum = sum + mt_ld4(down + ((size_t)s * rows + tile.row0 + m) * mt_quads(R) + r);
+                        sum = sum + mt_ld4(down + ((size_t)s * rows + tile.row(m)) * mt_quads(R) + r);
                 }
                 *reinterpret_cast<mt_f32x4*>(lds + m * PITCH + r) = sum;
             }
@@ -504,7 +685,7 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
                         const unsigned row = 16u * m + q * ABREAST + lane / ALONG, col = from + 4u * (lane % ALONG);
                         unsigned stores = ((group >> row) & 1ull) && col < N;
                         asm volatile("" : "+v"(stores));  // (known to no other round)
-                        if (stores) mt_put_row4<N>(out + (size_t)(tile.row0 + row) * N, col, v[q]);
+                        if (stores) mt_put_row4<N>(out + (size_t)tile.row(row) * N, col, v[q]);
                     }
                 }
             }
@@ -524,8 +705,6 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
 // Among equals at the cut the first indexes stay.
 // ---------------------------------------------------------------------------
 
-typedef unsigned long long mt_u64;
-
 // A float's place in the order of floats; -0 is 0.
 MT_INLINE unsigned mt_order_key(float x) {
     const unsigned b = __float_as_uint(x + 0.0f);
@@ -533,79 +712,6 @@ MT_INLINE unsigned mt_order_key(float x) {
 }
 MT_INLINE float mt_order_value(unsigned key) {
     return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xFFFFFFFFu));
-}
-
-template <typename OP>
-MT_INLINE mt_u64 mt_wave_fold(mt_u64 v, OP op) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = op(v, (mt_u64)__shfl_xor(v, off, 64));
-    return v;
-}
-
-// The sum of v over this lane and those before it, by adding from one lane, two, four and
-// eight before in rows of 16, then from the ends of the rows before.
-template <int FROM, int ROWS>
-MT_INLINE mt_u64 mt_add_from(mt_u64 v) {
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, FROM, ROWS, 15, false);
-    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), FROM, ROWS, 15, false);
-    return v + (((mt_u64)hi << 32) | lo);
-}
-MT_INLINE mt_u64 mt_wave_upto(mt_u64 v) {
-    v = mt_add_from<0x111, 15>(v);  // row_shr:1
-    v = mt_add_from<0x112, 15>(v);
-    v = mt_add_from<0x114, 15>(v);
-    v = mt_add_from<0x118, 15>(v);
-    v = mt_add_from<0x142, 10>(v);  // row_bcast:15 into rows 1 and 3
-    return mt_add_from<0x143, 12>(v);  // row_bcast:31 into rows 2 and 3
-}
-// The last lane's word.
-MT_INLINE mt_u64 mt_wave_last(mt_u64 v) {
-    return ((mt_u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), 63) << 32) |
-           (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, 63);
-}
-MT_INLINE mt_u64 mt_wave_sum(mt_u64 v) { return mt_wave_last(mt_wave_upto(v)); }
-
-// v (op) over the workgroup's waves; `lds` holds a word a wave.
-template <unsigned WAVES, typename OP>
-MT_INLINE mt_u64 mt_group_fold(mt_u64 v, mt_u64* lds, OP op) {
-    v = mt_wave_fold(v, op);
-    __syncthreads();
-    if (mt_lane() == 0u) lds[mt_wave()] = v;
-    __syncthreads();
-    v = lds[0];
-#pragma unroll
-    for (unsigned w = 1; w < WAVES; ++w) v = op(v, lds[w]);
-    return v;
-}
-
-// The sum of v over the workgroup.
-template <unsigned WAVES>
-MT_INLINE mt_u64 mt_group_sum(mt_u64 v, mt_u64* lds) {
-    v = mt_wave_sum(v);
-    __syncthreads();
-    if (mt_lane() == 0u) lds[mt_wave()] = v;
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (unsigned w = 0; w < WAVES; ++w) v += lds[w];
-    return v;
-}
-
-// The sum of v over the lanes before this one; `all`: over all of them.
-template <unsigned WAVES>
-MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
-    const mt_u64 sum = mt_wave_upto(v);
-    __syncthreads();
-    if (mt_lane() == 63u) lds[mt_wave()] = sum;
-    __syncthreads();
-    mt_u64 before = 0;
-    all = 0;
-#pragma unroll
-    for (unsigned w = 0; w < WAVES; ++w) {
-        before += w < mt_wave() ? lds[w] : 0;
-        all += lds[w];
-    }
-    return before + sum - v;
 }
 
 // e^z for z <= 0, right to about 2^-50 of itself; 0 below -700, and for a NaN.  z = n log 2 +

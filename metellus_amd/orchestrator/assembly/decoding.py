@@ -151,14 +151,17 @@ def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_n
     blocks = min(ADAPTER_BLOCKS, _ceil(op.rank, 16))
     tile, loop = adapter_tile(rows, op.rank)
     waves = ADAPTER_DOWN_WAVES
+    order, lds_bytes = op.order is not None, waves * tile * blocks * 1024
+    if order:  # sums, numbers of 256 bins a wave, a byte for each of 4096 rows; a tile's rows
+        lds_bytes = 4 * 64 + max(lds_bytes, waves * (8 + 4 * 256) + 4096)
     sig = _Signature()
-    args = (sig.add("x", op.x), sig.add("a", op.a), sig.add("ids", op.ids), sig.add("down", op.down, out=True), "M",
-            "(mt_f32x4*)mt_lds")
+    args = (sig.add("x", op.x), sig.add("a", op.a), sig.add("ids", op.ids), sig.add("down", op.down, out=True),
+            sig.add("order", op.order, out=True), "M", "(mt_f32x4*)mt_lds")
     frag = ServingFragment(
         "mt_adapter_down",
-        (inner, op.rank, blocks, tile, loop, op.splits, op.held, waves, *_strides(op.x)),
+        (inner, op.rank, blocks, tile, loop, order, op.splits, op.held, waves, *_strides(op.x)),
         args,
-        lds_bytes=waves * tile * blocks * 1024,
+        lds_bytes=lds_bytes,
         name="adapter_down",
     )
     grid = _adapter_grid(rows, tile, loop, op.splits * _ceil(op.rank, 16 * blocks))
@@ -176,14 +179,17 @@ def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name:
     rows, cols = op.base.shape
     tile, loop = adapter_tile(rows, op.rank)
     waves, per, blocks = adapter_up_shape(rows, op.rank)
+    lds_bytes = 64 * (tile * (16 * _ceil(op.rank, 16) + 4) + waves * (16 * blocks + 4))
+    order = op.order is not None
+    lds_bytes += 4 * 64 if order else 0
     sig = _Signature()
     args = (sig.add("base", op.base), sig.add("down", op.down), sig.add("b", op.b), sig.add("ids", op.ids),
-            sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M", "(float*)mt_lds")
+            sig.add("order", op.order), sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M", "(float*)mt_lds")
     frag = ServingFragment(
         "mt_adapter_up",
-        (cols, op.rank, tile, loop, op.splits, op.held, waves, per, blocks, *_strides(op.base)),
+        (cols, op.rank, tile, loop, order, op.splits, op.held, waves, per, blocks, *_strides(op.base)),
         args,
-        lds_bytes=64 * (tile * (16 * _ceil(op.rank, 16) + 4) + waves * (16 * blocks + 4)),
+        lds_bytes=lds_bytes,
         name="adapter_up",
     )
     grid = _adapter_grid(rows, tile, loop, _ceil(cols, 16 * waves * per * blocks))

@@ -22,6 +22,7 @@ import numpy as np
 
 from metellus_amd.compute.elementwise.elementwise import BroadcastSpec
 from metellus_amd.orchestrator.decoding import (
+    ADAPTER_ORDER_ROWS,
     ADAPTER_RANK_MAX,
     SAMPLE_LIST,
     AdapterDownOp,
@@ -572,6 +573,7 @@ class Operations:
             rank=rank,
             splits=splits,
             name=out,
+            order=self._fresh(f"{out}.order", (tx.shape[0], 2), "int32") if tx.shape[0] >= ADAPTER_ORDER_ROWS else None,
             after=self._owners(tx, ta, ti),
         )
         up = AdapterUpOp(
@@ -583,11 +585,12 @@ class Operations:
             rank=rank,
             splits=splits,
             scales=ts,
+            order=down.order,
             after=self._owners(ty, tb, ti, ts),
         )
         self._emit_all(down)
         self._emit_all(up)
-        self._scratch.add(down.down.name)
+        self._scratch.update(t.name for t in down.outs)
         return up.y
 
     def sample(

@@ -126,6 +126,7 @@ class Rotary:
 
 ADAPTER_MANY_ROWS = 1024  # from here on tiles of 64 rows, a workgroup for all groups of each
 ADAPTER_DOWN_WAVES = 4  # a workgroup's
+ADAPTER_ORDER_ROWS = 128  # from here on rows of many adapters are put in order first
 
 
 def adapter_splits(rows: int, inner: int) -> int:
@@ -134,7 +135,7 @@ def adapter_splits(rows: int, inner: int) -> int:
     up takes longer (us: 1 row of 4096 columns, rank 16, whole 17, in 4 9.4, 8 9.6; 32 rows 30,
     13.4, 12.3, in 16 12.8; 77 of 5003, rank 23, 37, 21, 18, 20; 8 of 11008, rank 64, in 8
     23, 12 20, 20 32)."""
-    wanted = -(-256 // -(-rows // 64)) if rows >= ADAPTER_MANY_ROWS else min(12, 2048 // rows)
+    wanted = 256 // -(-rows // 64) if rows >= ADAPTER_MANY_ROWS else min(12, 2048 // rows)
     return max(1, min(-(-inner // 512), wanted))
 
 
@@ -251,6 +252,7 @@ class AdapterDownOp(ServingOp):
     rank: int
     splits: int
     name: str  # of the operator's output
+    order: Tensor | None = None  # the rows and their ids as they are taken in turn
     after: tuple[Tensor, ...] = ()
 
     def __post_init__(self) -> None:
@@ -267,7 +269,7 @@ class AdapterDownOp(ServingOp):
 
     @property
     def outs(self) -> tuple[Tensor, ...]:
-        return (self.down,)
+        return (self.down,) if self.order is None else (self.down, self.order)
 
     @property
     def reads(self) -> tuple[Tensor, ...]:
@@ -286,6 +288,7 @@ class AdapterUpOp(ServingOp):
     rank: int
     splits: int
     scales: Tensor | None = None
+    order: Tensor | None = None
     after: tuple[Tensor, ...] = ()
 
     def __post_init__(self) -> None:
@@ -307,7 +310,7 @@ class AdapterUpOp(ServingOp):
 
     @property
     def reads(self) -> tuple[Tensor, ...]:
-        return tuple(t for t in (self.base, self.down, self.b, self.ids, self.scales) if t is not None)
+        return tuple(t for t in (self.base, self.down, self.b, self.ids, self.scales, self.order) if t is not None)
 
 
 def sample_chunks(rows: int, cols: int) -> tuple[int, int]:

@@ -101,7 +101,11 @@ def _adapter_down(op, get):
         if 0 <= i < op.held:
             with np.errstate(all="ignore"):
                 down[m, : op.rank] = a[i * op.rank : (i + 1) * op.rank] @ x[m]  # (the first part has it all)
-    return {op.down.name: down}
+    found = {op.down.name: down}
+    if op.order is not None:  # (in which order rows are taken is the kernel's choice)
+        ids = np.asarray(get(op.ids))
+        found[op.order.name] = np.stack([np.arange(len(ids)), np.where((ids < 0) | (ids >= op.held), -1, ids)], axis=1).astype(np.int32)
+    return found
 
 
 def _adapter_up(op, get):

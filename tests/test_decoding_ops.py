@@ -11,7 +11,7 @@ import pytest
 
 from metellus_amd.api import compile_program
 from metellus_amd.orchestrator import Operations, Rotary
-from metellus_amd.orchestrator.decoding import adapter_splits, sample_chunks
+from metellus_amd.orchestrator.decoding import ADAPTER_ORDER_ROWS, adapter_splits, sample_chunks
 from metellus_amd.orchestrator.fusion import fuse
 from metellus_amd.orchestrator.scheduler import schedule
 from metellus_amd.runtime import hip_backend
@@ -225,6 +225,18 @@ def test_scheduling_adapters():
         schedule(ops, groups, outputs=["z.down"])
     with pytest.raises(ValueError, match="operator's own"):
         ops.reduction("sum", out="r", x="z.down")
+
+
+def test_scheduling_adapters_of_many_rows():
+    """The rows in the order that they are taken in are no output either; fewer rows have none."""
+    for rows, own in ((ADAPTER_ORDER_ROWS, {"z.down", "z.order"}), (ADAPTER_ORDER_ROWS - 1, {"z.down"})):
+        ops = _ops(x=(rows, 8), y=(rows, 20), a=(12, 8), b=(60, 4), s=(3,), ids=((rows,), "int32"))
+        for t in list(ops.tensors.values()):
+            ops.from_numpy(np.zeros(t.shape, t.stored), t.name)
+        ops.adapters(**ADAPTER_CALL, scales="s")
+        steps = schedule(ops, compile_program(ops)).fragments
+        assert ops.scratch == own and [s.into for s in steps if isinstance(s, Download)] == ["z"]
+        assert set(evaluate(ops)) == own | {"z"}
 
 
 def test_shares_of_columns():

@@ -285,6 +285,23 @@ def test_adapters_of_strided_rows(rows):
     _adapter_check(_adapters(rows, 130, 70, 6, 3, [i % 4 - 1 for i in range(rows)], strides=True))
 
 
+@pytest.mark.parametrize("rows, rank, held", [(128, 5, 3), (130, 16, 300), (700, 8, 1), (1025, 7, 64), (4099, 4, 600), (8300, 6, 40)])
+@pytest.mark.parametrize("kind", ["random", "turns", "runs", "few"])
+def test_adapters_by_any_order_of_rows(rows, rank, held, kind):
+    """Rows of many adapters, also more than are put in order at once: against the formula,
+    and another order of the same rows gives the same bits."""
+    rng = np.random.default_rng(rows)
+    ids = {"random": rng.integers(-1, held + 1, rows), "turns": np.arange(rows) % held, "runs": np.arange(rows) // 33 % held,
+           "few": np.where(rng.random(rows) < 0.01, held - 1, -1)}[kind]
+    ops = _adapters(rows, 70, 37, rank, held, ids)
+    y = _adapter_check(ops)
+    other = rng.permutation(rows)
+    again = _adapters(rows, 70, 37, rank, held, ids[other])
+    for name in ("x", "base"):
+        again.uploads[name][:] = ops.uploads[name][other]
+    np.testing.assert_array_equal(run(again).env["y"], y[other])
+
+
 def test_adapters_rows_do_not_mix():
     """Infinities and NaN of a row, and of an adapter, stay with the rows that have them."""
     ops = _adapters(18, 200, 40, 9, 4, [0, 1, 2, 3, -1, 0] * 3, scales=False)
