@@ -281,7 +281,7 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // by its first row: a group reads its adapter once and multiplies all of the 16-row blocks
 // that have rows of it (an MFMA's columns do not mix), of which it stores its own.  So a
 // batch whose rows each have an adapter reads each of them once, and so does one whose rows
-// share one.  LOOP: a workgroup does all groups of a tile, otherwise a workgroup does the
+// share one.  TURNS workgroups take a tile's groups in turn, or with none a workgroup does the
 // one that its row leads, if it does.
 // fp32 MFMAs 16x16x4: with (n, g) = (lane % 16, lane / 16) a lane has 4 consecutive k of
 // row n of both operands, k = 4 g + i in the i-th of four MFMAs; the order of k is the
@@ -400,7 +400,7 @@ MT_INLINE mt_f32x4 mt_mfma16_f32(mt_f32x4 a, mt_f32x4 b, mt_f32x4 c) {
 }
 
 // A workgroup's tile and its share of the columns (blockIdx.x; blockIdx.y is the row of the
-// tile that may lead, so that those of first rows, which all do, go first).  LOOP: the GPU's
+// tile that may lead, so that those of first rows, which all do, go first).  With turns the GPU's
 // eight parts, which take workgroups in turn, have neighbouring tiles each, whose rows are
 // likely to share adapters; there are eight times a whole number of tiles then, and the
 // last may not be there.
@@ -457,10 +457,11 @@ MT_INLINE constexpr unsigned mt_quads(unsigned ranks) { return (ranks + 3u) / 4u
 // 64 columns of x in turn and add up in LDS; each split stores its part.  Loads of 16
 // columns go out as the registers of those 64 before are free, so MFMAs and memory go on
 // together.  Lanes of rows of other groups load the leader's, which are loaded anyway.
-template <unsigned K, unsigned R, unsigned RB, unsigned MB, bool LOOP, bool ORDER, unsigned SPLITS, unsigned HELD,
+template <unsigned K, unsigned R, unsigned RB, unsigned MB, unsigned TURNS, bool ORDER, unsigned SPLITS, unsigned HELD,
           unsigned WAVES, unsigned XRS, unsigned XCS>
 MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, float* down, int* order, unsigned rows,
                                mt_f32x4* lds) {
+    constexpr bool LOOP = TURNS != 0u;
     constexpr unsigned TILE = 16u * MB, STEP = 64u * SPLITS * WAVES, WHOLE = K / 64u * 64u;
     // Sums that an MFMA does not wait for the one before with, added at the end: few tiles are
     // too few MFMAs to wait in turn (and shorter sums round less).
@@ -481,10 +482,10 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
         order[2u * (size_t)(tile.row0 + lane) + 1u] = (int)tile.mine;
     }
 #pragma unroll 1
-    for (unsigned j = blockIdx.y; j < TILE; ++j) {
+    for (unsigned j = LOOP ? 0u : blockIdx.y, taken = 0u; j < TILE; ++j) {
         int id;
         const unsigned long long group = tile.group(j, id);
-        if (group != 0ull && id >= 0) {
+        if (group != 0ull && (TURNS <= 1u || taken++ % TURNS == blockIdx.y) && id >= 0) {
             const float *xr[MB], *ar[RB];
             mt_f32x4 acc[SUMS][MB][RB], xv[4][MB], av[4][RB];
 #pragma unroll
@@ -579,10 +580,11 @@ MT_INLINE void mt_adapter_down(const float* x, const float* a, const int* ids, f
 // rows goes through LDS on its way out, where rows become what lanes next to each other have:
 // base is read and the output written 64 BL bytes of a row at a time, and by the four waves
 // 256 BL (4096 rows of 4096, rank 64: 64 bytes of a row at a time 58 us).
-template <unsigned N, unsigned R, unsigned MB, bool LOOP, bool ORDER, unsigned SPLITS, unsigned HELD, unsigned WAVES,
+template <unsigned N, unsigned R, unsigned MB, unsigned TURNS, bool ORDER, unsigned SPLITS, unsigned HELD, unsigned WAVES,
           unsigned PER, unsigned BL, unsigned YRS, unsigned YCS>
 MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* b, const int* ids, const int* order,
                              const float* scales, float* out, unsigned rows, float* lds) {
+    constexpr bool LOOP = TURNS != 0u;
     constexpr unsigned RC = (R + 15u) / 16u, TILE = 16u * MB, PITCH = 16u * RC + 4u, WIDE = 16u * BL, OUT_PITCH = WIDE + 4u;
     constexpr unsigned ALONG = 4u * BL, ABREAST = 64u / ALONG;  // lanes along a row, and rows at a time
     const unsigned tiles = (rows + TILE - 1u) / TILE, lane = mt_lane(), n = lane & 15u, g = lane >> 4;
@@ -603,10 +605,10 @@ MT_INLINE void mt_adapter_up(const float* base, const float* down, const float* 
         tile.of(ids, rows);
     float* turn = lds + TILE * PITCH + mt_wave() * 16u * OUT_PITCH;  // this wave's block of rows
 #pragma unroll 1
-    for (unsigned j = blockIdx.y; j < TILE; ++j) {
+    for (unsigned j = LOOP ? 0u : blockIdx.y, taken = 0u; j < TILE; ++j) {
         int id;
         const unsigned long long group = tile.group(j, id);
-        if (group != 0ull) {
+        if (group != 0ull && (TURNS <= 1u || taken++ % TURNS == blockIdx.y)) {
             mt_f32x4 bv[BL][RC], v[BL];
             const auto columns = [&](unsigned p) { return ((at.share * PER + p) * WAVES + mt_wave()) * WIDE; };
             const auto load = [&](unsigned from) {

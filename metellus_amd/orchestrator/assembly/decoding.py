@@ -12,7 +12,6 @@ from metellus_amd.orchestrator.assembly.decision import DecisionView
 from metellus_amd.orchestrator.assembly.serving import _ceil, _group, _Signature
 from metellus_amd.orchestrator.decoding import (
     ADAPTER_DOWN_WAVES,
-    ADAPTER_MANY_ROWS,
     SAMPLE_LIST,
     AdapterDownOp,
     AdapterUpOp,
@@ -131,25 +130,34 @@ def _assemble_rotary(decision: DecisionView, op: RotaryOp, function_name: str | 
 # adapters
 # ---------------------------------------------------------------------------
 
+ADAPTER_TURNS = 256, 2  # rows, from which on as many workgroups take a tile's groups in turn
 ADAPTER_BLOCKS = 4  # of 16 ranks, that a wave multiplies x by at once
 
 
-def adapter_tile(rows: int, rank: int) -> tuple[int, bool]:
-    """Blocks of 16 rows in a tile (one where the rank leaves no registers for more), and
-    whether a workgroup does all groups of its tile."""
-    many = rows >= ADAPTER_MANY_ROWS
-    return (4 if many and rank <= 64 else 1), many
+def adapter_tile(rank: int, many: bool) -> int:
+    """Blocks of 16 rows in a tile: one where the rank leaves no registers for more."""
+    return 4 if many and rank <= 64 else 1
 
 
-def _adapter_grid(rows: int, tile: int, loop: bool, shares: int) -> tuple[int, int, int]:
+def adapter_turns(rows: int, many: bool) -> int:
+    """Workgroups that take a tile's groups in turn; 0: one for each row that may lead one, which
+    has nothing to do where it does not.  (us, 0, 1, 2, 4 and 8, ids drawn from 64, rank 64 of
+    4096 x 4096: 150 rows 48, 100, 68, 72, 69; 300 59, 72, 61, 62, 69; 600 74, 70, 63, 66, 71;
+    1000 102, 78, 72, 75, 86; 8 prompts: 600 43, 38, 39, 40, 43; 2000 of 1024 x 1024 39, 39, 28,
+    29, 34.)"""
+    least, turns = ADAPTER_TURNS
+    return 1 if many else turns if rows >= least else 0
+
+
+def _adapter_grid(rows: int, tile: int, turns: int, shares: int) -> tuple[int, int, int]:
     tiles = _ceil(rows, 16 * tile)
-    return (8 * _ceil(tiles, 8) * shares, 1, 1) if loop else (tiles * shares, 16 * tile, 1)
+    return (8 * _ceil(tiles, 8) * shares, turns, 1) if turns else (tiles * shares, 16 * tile, 1)
 
 
 def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_name: str | None) -> KernelGroup:
     rows, inner = op.x.shape
     blocks = min(ADAPTER_BLOCKS, _ceil(op.rank, 16))
-    tile, loop = adapter_tile(rows, op.rank)
+    tile, turns = adapter_tile(op.rank, op.many), adapter_turns(rows, op.many)
     waves = ADAPTER_DOWN_WAVES
     order, lds_bytes = op.order is not None, waves * tile * blocks * 1024
     if order:  # sums, numbers of 256 bins a wave, a byte for each of 4096 rows; a tile's rows
@@ -159,26 +167,26 @@ def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_n
             sig.add("order", op.order, out=True), "M", "(mt_f32x4*)mt_lds")
     frag = ServingFragment(
         "mt_adapter_down",
-        (inner, op.rank, blocks, tile, loop, order, op.splits, op.held, waves, *_strides(op.x)),
+        (inner, op.rank, blocks, tile, turns, order, op.splits, op.held, waves, *_strides(op.x)),
         args,
         lds_bytes=lds_bytes,
         name="adapter_down",
     )
-    grid = _adapter_grid(rows, tile, loop, op.splits * _ceil(op.rank, 16 * blocks))
+    grid = _adapter_grid(rows, tile, turns, op.splits * _ceil(op.rank, 16 * blocks))
     return _group(decision, sig, frag, function_name or f"adapter_down_{op.name}", {"M": rows}, grid, 64 * waves,
                   headers=(decoding_header(),))
 
 
-def adapter_up_shape(rows: int, rank: int) -> tuple[int, int, int]:
+def adapter_up_shape(rank: int, many: bool) -> tuple[int, int, int]:
     """Waves of a workgroup, how often each takes a set of columns, and the blocks of 16 in a
     set: as many as leave registers for their part of B."""
-    return 4, 2 if rows >= ADAPTER_MANY_ROWS else 1, 4 if rank <= 64 else 2 if rank <= 128 else 1
+    return 4, 2 if many else 1, 4 if rank <= 64 else 2 if rank <= 128 else 1
 
 
 def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name: str | None) -> KernelGroup:
     rows, cols = op.base.shape
-    tile, loop = adapter_tile(rows, op.rank)
-    waves, per, blocks = adapter_up_shape(rows, op.rank)
+    tile, turns = adapter_tile(op.rank, op.many), adapter_turns(rows, op.many)
+    waves, per, blocks = adapter_up_shape(op.rank, op.many)
     lds_bytes = 64 * (tile * (16 * _ceil(op.rank, 16) + 4) + waves * (16 * blocks + 4))
     order = op.order is not None
     lds_bytes += 4 * 64 if order else 0
@@ -187,12 +195,12 @@ def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name:
             sig.add("order", op.order), sig.add("scales", op.scales), sig.add("out", op.y, out=True), "M", "(float*)mt_lds")
     frag = ServingFragment(
         "mt_adapter_up",
-        (cols, op.rank, tile, loop, order, op.splits, op.held, waves, per, blocks, *_strides(op.base)),
+        (cols, op.rank, tile, turns, order, op.splits, op.held, waves, per, blocks, *_strides(op.base)),
         args,
         lds_bytes=lds_bytes,
         name="adapter_up",
     )
-    grid = _adapter_grid(rows, tile, loop, _ceil(cols, 16 * waves * per * blocks))
+    grid = _adapter_grid(rows, tile, turns, _ceil(cols, 16 * waves * per * blocks))
     return _group(decision, sig, frag, function_name or f"adapter_up_{op.y.name}", {"M": rows}, grid, 64 * waves,
                   headers=(decoding_header(),))
 

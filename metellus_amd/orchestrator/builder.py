@@ -32,6 +32,7 @@ from metellus_amd.orchestrator.decoding import (
     RotaryOp,
     SampleOp,
     SampleScanOp,
+    adapter_many,
     adapter_splits,
     sample_bins,
     sample_chunks,
@@ -564,7 +565,8 @@ class Operations:
             )
         if tx.shape[0] != ty.shape[0]:
             raise ValueError(f"adapters x and base must have as many rows; got {tx.shape} and {ty.shape}")
-        splits = adapter_splits(*tx.shape)
+        many = adapter_many(*tx.shape, cols, rank)
+        splits = adapter_splits(*tx.shape, many)
         down = AdapterDownOp(
             down=self._fresh(f"{out}.down", (splits * tx.shape[0], -(-rank // 4) * 4), "float32"),
             x=tx,
@@ -572,6 +574,7 @@ class Operations:
             ids=ti,
             rank=rank,
             splits=splits,
+            many=many,
             name=out,
             order=self._fresh(f"{out}.order", (tx.shape[0], 2), "int32") if tx.shape[0] >= ADAPTER_ORDER_ROWS else None,
             after=self._owners(tx, ta, ti),
@@ -584,6 +587,7 @@ class Operations:
             ids=ti,
             rank=rank,
             splits=splits,
+            many=many,
             scales=ts,
             order=down.order,
             after=self._owners(ty, tb, ti, ts),

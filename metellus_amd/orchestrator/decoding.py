@@ -124,18 +124,27 @@ class Rotary:
         return tuple(found)
 
 
-ADAPTER_MANY_ROWS = 1024  # from here on tiles of 64 rows, a workgroup for all groups of each
 ADAPTER_DOWN_WAVES = 4  # a workgroup's
 ADAPTER_ORDER_ROWS = 128  # from here on rows of many adapters are put in order first
 
 
-def adapter_splits(rows: int, inner: int) -> int:
+def adapter_many(rows: int, inner: int, cols: int, rank: int) -> bool:
+    """Whether tiles have 64 rows, for which adapters are read less often, or 16, of which there
+    are more workgroups.  (us, 64 and 16, ids of 8 prompts, and drawn from 64: rank 64, 1100 rows
+    of 4096 x 4096 58 and 64, 110 and 86; 1500 58 and 73, 96 and 96; 2048 52 and 78, 73 and 89; 4096
+    of 1024 x 1024 45 and 33, 52 and 41; 12000 of 256 x 256 41 and 37, 56 and 58; rank 16, 4096 of
+    4096 x 4096 57 and 57, 64 and 67; 1500 36 and 34, 50 and 39.)"""
+    return rows * min(inner, cols) * min(rank, 64) >= 5 << 26
+
+
+def adapter_splits(rows: int, inner: int, many: bool) -> int:
     """Shares of x's columns that workgroups take apart, where rows alone are too few
     workgroups to fill the GPU: of 512 columns at least, and not so many that adding them
     up takes longer (us: 1 row of 4096 columns, rank 16, whole 17, in 4 9.4, 8 9.6; 32 rows 30,
     13.4, 12.3, in 16 12.8; 77 of 5003, rank 23, 37, 21, 18, 20; 8 of 11008, rank 64, in 8
-    23, 12 20, 20 32)."""
-    wanted = 256 // -(-rows // 64) if rows >= ADAPTER_MANY_ROWS else min(12, 2048 // rows)
+    23, 12 20, 20 32; 600 of 4096, rank 64, in 3 49, 5 43, 6 43), or that some come after
+    others (3000 rows of 4096 columns, rank 64: in 6 98, in 5 87)."""
+    wanted = 256 // -(-rows // 64) if many else min(12, 3000 // rows)
     return max(1, min(-(-inner // 512), wanted))
 
 
@@ -251,6 +260,7 @@ class AdapterDownOp(ServingOp):
     ids: Tensor
     rank: int
     splits: int
+    many: bool
     name: str  # of the operator's output
     order: Tensor | None = None  # the rows and their ids as they are taken in turn
     after: tuple[Tensor, ...] = ()
@@ -287,6 +297,7 @@ class AdapterUpOp(ServingOp):
     ids: Tensor
     rank: int
     splits: int
+    many: bool
     scales: Tensor | None = None
     order: Tensor | None = None
     after: tuple[Tensor, ...] = ()

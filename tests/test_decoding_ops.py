@@ -4,6 +4,7 @@ worked out by hand, and that every kernel variant compiles for gfx950."""
 
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
@@ -11,7 +12,7 @@ import pytest
 
 from metellus_amd.api import compile_program
 from metellus_amd.orchestrator import Operations, Rotary
-from metellus_amd.orchestrator.decoding import ADAPTER_ORDER_ROWS, adapter_splits, sample_chunks
+from metellus_amd.orchestrator.decoding import ADAPTER_ORDER_ROWS, adapter_many, adapter_splits, sample_chunks
 from metellus_amd.orchestrator.fusion import fuse
 from metellus_amd.orchestrator.scheduler import schedule
 from metellus_amd.runtime import hip_backend
@@ -240,12 +241,15 @@ def test_scheduling_adapters_of_many_rows():
 
 
 def test_shares_of_columns():
-    assert adapter_splits(1, 4096) == 8 and adapter_splits(1, 100) == 1 and adapter_splits(8, 11008) == 12
-    assert adapter_splits(32, 4096) == 8 and adapter_splits(4096, 4096) == 4 and adapter_splits(600, 4096) == 3
-    assert adapter_splits(16384, 4096) == 1
-    for rows in (1, 3, 50, 700, 1024, 5000):
+    few, many = [functools.partial(adapter_splits, many=m) for m in (False, True)]
+    assert few(1, 4096) == 8 and few(1, 100) == 1 and few(8, 11008) == 12 and few(32, 4096) == 8 and few(600, 4096) == 5
+    assert many(4096, 4096) == 4 and many(3000, 4096) == 5 and many(16384, 4096) == 1
+    for rows in (1, 3, 50, 700, 1024, 5000, 20000):
         for inner in (1, 511, 513, 5003, 16384):
-            assert 1 <= adapter_splits(rows, inner) <= -(-inner // 512)
+            for shares in (few, many):
+                assert 1 <= shares(rows, inner) <= -(-inner // 512)
+    assert adapter_many(2048, 4096, 4096, 64) and not adapter_many(2048, 4096, 2048, 64) and not adapter_many(2048, 1024, 4096, 64)
+    assert not adapter_many(2048, 4096, 4096, 16) and not adapter_many(4096, 1024, 1024, 256)
 
 
 def test_scheduling_a_draw():

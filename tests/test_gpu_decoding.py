@@ -280,9 +280,22 @@ def test_adapters_by_group(ids):
     np.testing.assert_array_equal(y[none], ops.uploads["base"][none])
 
 
-@pytest.mark.parametrize("rows", [19, 1030])
-def test_adapters_of_strided_rows(rows):
-    _adapter_check(_adapters(rows, 130, 70, 6, 3, [i % 4 - 1 for i in range(rows)], strides=True))
+@pytest.mark.parametrize("rows, inner, cols, rank, held", [
+    (2100, 2501, 2500, 64, 3), (4100, 2560, 2499, 33, 8), (2100, 2500, 2503, 100, 40), (80000, 70, 67, 64, 9), (82000, 66, 71, 256, 5),
+    (2048, 2600, 2561, 64, 900),
+])
+def test_adapters_of_many_rows(rows, inner, cols, rank, held):
+    """Tiles whose groups one workgroup does all: of 64 rows, and of 16 for ranks above 64."""
+    rng = np.random.default_rng(rows + inner)
+    runs = np.sort(rng.integers(-1, held, rows // 2))
+    ops = _adapters(rows, inner, cols, rank, held, np.concatenate([runs, rng.integers(-1, held, rows - len(runs))]))
+    assert next(o for o in ops.build() if isinstance(o, AdapterUpOp)).many
+    _adapter_check(ops)
+
+
+@pytest.mark.parametrize("rows, rank", [(19, 6), (140, 6), (1030, 6), (80000, 64)])
+def test_adapters_of_strided_rows(rows, rank):
+    _adapter_check(_adapters(rows, 130, 70, rank, 3, [i % 4 - 1 for i in range(rows)], strides=True))
 
 
 @pytest.mark.parametrize("rows, rank, held", [(128, 5, 3), (130, 16, 300), (700, 8, 1), (1025, 7, 64), (4099, 4, 600), (8300, 6, 40)])
