@@ -7,7 +7,8 @@
 //   * mt_rotary         queries and keys turned by their positions
 //   * mt_adapter_down / mt_adapter_up
 //                       low-rank adapters of many requests beside a shared product
-//   * mt_sample         tokens from logits and given random numbers
+//   * mt_sample_scan / mt_sample_pick
+//                       tokens from logits and given random numbers
 
 // ---------------------------------------------------------------------------
 // Sums over lanes.
@@ -96,6 +97,9 @@ MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
 // behind it.  So no workgroup waits for another, and the numbers do not depend on how
 // many there are.  A launch reads entries below `have` alone and writes those from there
 // on, so the table can be written in place.
+// Bound by the latency of a launch and of loads in turn -- lengths, then a row's own -- of a few
+// KB (32 sequences, a token each: kernel 3.2 us, call 4.9; 1021 sequences and 16384 tokens,
+// 64 bytes of them written to a lane: 6.2 and 6.0).
 // ---------------------------------------------------------------------------
 
 // Sums of rows stop at 2^31 - 1, behind any row.
@@ -202,6 +206,9 @@ MT_INLINE void mt_page_tables(int* pages, const int* free, const int* lengths, c
 // counted in turns, position times a turn's share per position, as the exact sum of two
 // doubles, of which whole turns are taken away before anything is rounded to the size of
 // the rest: an angle is right to 2^-51 of a turn at any int32 position.
+// Bound by memory: every element is read and written once (8192 rows of 40 heads of 128 63 us,
+// 5.3 TB/s, a copy's rate; four rows to a workgroup, whose angles the other rows' loads hide: one
+// row 74), or by the launch (a row 4.7 us, of which the kernel 2.2).
 // ---------------------------------------------------------------------------
 
 template <unsigned D, unsigned R, bool NEAR, unsigned V, unsigned XH, unsigned XRS, unsigned XCS, unsigned KH,
@@ -288,6 +295,11 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // same for both, so the sum is the product's.  An element (row 4 g + i, column n) of the
 // result is lane (n, g)'s i-th: rows are ranks, or columns of the output, so a lane has
 // four neighbours of row m = n of `down` or `out`.
+// Bound by two launches and the latency of loads in turn for few rows (us: 1 row of 4096 x
+// 4096, rank 16, kernels 3.8 and 3.5, call 8.5; 32 rows of 4096 x 11008, an adapter each, 4.4 and
+// 8.0, of which 64 MB of adapters could take 5; 77 of 5003 x 4099, rank 23, 6.9 and 7.6); for
+// prompts by MFMAs, half of their rate in the first kernel, and by base and out in the second
+// (4096 rows of 4096 x 4096, rank 64: 32 and 42).
 // ---------------------------------------------------------------------------
 
 // Rows are put in order before they are cut into tiles, MT_ADAPTER_ORDERED at a time: by id
@@ -1005,6 +1017,10 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // The list takes half a compute unit's LDS, so there are two workgroups on each, of eight
 // waves (us, 64 rows of 131072 cut by p: eight waves, 512 workgroups 43, 1024 55, four waves
 // 64; one row 18, 17, 20; 64 rows cut by k 25, 39, 35).
+// Bound by vector instructions where rows are weighed in whole (64 rows of 131072, us: the scan 10,
+// with bins 15, of 6.5 to read them; the second kernel 16 with no cut, 20 by k, 36 by p, of
+// which the pass over the logits takes 8, 2 and 16, and the last workgroup's list, from its
+// arrival on, 3, 7 and 13), by two launches and that list for few rows (one of 131072 5.5 and 12).
 // ---------------------------------------------------------------------------
 
 constexpr unsigned MT_SAMPLE_WAVES = 8u, MT_SAMPLE_LANES = 512u;
