@@ -99,7 +99,7 @@ MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
 // on, so the table can be written in place.
 // Bound by the latency of a launch and of loads in turn -- lengths, then a row's own -- of a few
 // KB (32 sequences, a token each: kernel 3.2 us, call 4.9; 1021 sequences and 16384 tokens,
-// 64 bytes of them written to a lane: 6.2 and 6.0).
+// 6 and 5.9).
 // ---------------------------------------------------------------------------
 
 // Sums of rows stop at 2^31 - 1, behind any row.
@@ -206,9 +206,8 @@ MT_INLINE void mt_page_tables(int* pages, const int* free, const int* lengths, c
 // counted in turns, position times a turn's share per position, as the exact sum of two
 // doubles, of which whole turns are taken away before anything is rounded to the size of
 // the rest: an angle is right to 2^-51 of a turn at any int32 position.
-// Bound by memory: every element is read and written once (8192 rows of 40 heads of 128 63 us,
-// 5.3 TB/s, a copy's rate; four rows to a workgroup, whose angles the other rows' loads hide: one
-// row 74), or by the launch (a row 4.7 us, of which the kernel 2.2).
+// Bound by memory: every element is read and written once (8192 rows of 40 heads of 128 58 us,
+// 5.8 TB/s, where a copy of 1 GiB has 5.1), or by the launch (a row 4.7 us, of which the kernel 2.2).
 // ---------------------------------------------------------------------------
 
 template <unsigned D, unsigned R, bool NEAR, unsigned V, unsigned XH, unsigned XRS, unsigned XCS, unsigned KH,

@@ -48,8 +48,9 @@ def _strides(t: Tensor | None) -> tuple[int, int]:
 
 
 def page_table_lanes(sequences: int) -> int:
-    """Lanes that add up the sequences: one each while they fit in a workgroup."""
-    return 256 if sequences <= 256 else 1024
+    """Lanes that add up the sequences.  (us, 256, 512 and 1024: 32 sequences 5.4, 5.4, 5.9; 1021
+    with 16384 tokens 6.2, 5.9, 6.8; 2048 6.7, 5.9, 6.0.)"""
+    return 256 if sequences <= 256 else 512
 
 
 def _assemble_page_tables(decision: DecisionView, op: PageTablesOp, function_name: str | None) -> KernelGroup:
@@ -92,6 +93,13 @@ def rotary_vector(spec: Rotary, *tensors: Tensor | None) -> int:
     return 4 if dense and quads else 1
 
 
+def rotary_rows(rows: int, elements: int) -> int:
+    """Rows of a workgroup, by what a row has: as many as make 2048, up to 4.  (us, 1, 2 and 4 rows,
+    16384 of 2 heads of 64 7.2, 5.7, 5.4; of 16 24.3, 21.0, 21.3; 8192 of 40 heads of 128 58, 61,
+    64; 512 of them 5.8, 6.0, 6.5.)"""
+    return max(1, min(4, 2048 // elements)) if rows >= 1024 else 1
+
+
 def _turns(spec: Rotary) -> str:
     rows = ", ".join(f"{{{a.hex()}, {b.hex()}}}" for a, b in spec.turns)
     return f"static __device__ const double mt_turns[{spec.part // 2}][2] = {{{rows}}};"
@@ -101,7 +109,7 @@ def _assemble_rotary(decision: DecisionView, op: RotaryOp, function_name: str | 
     spec, rows = op.spec, op.x.shape[0]
     heads = op.x.shape[1] // spec.dim
     kv_heads = op.k.shape[1] // spec.dim if op.k is not None else 0
-    together = 4 if rows >= 1024 else 1
+    together = rotary_rows(rows, (heads + kv_heads) * spec.dim)
     sig = _Signature()
     args = (
         sig.add("x", op.x),
@@ -179,8 +187,10 @@ def _assemble_adapter_down(decision: DecisionView, op: AdapterDownOp, function_n
 
 def adapter_up_shape(rank: int, many: bool) -> tuple[int, int, int]:
     """Waves of a workgroup, how often each takes a set of columns, and the blocks of 16 in a
-    set: as many as leave registers for their part of B."""
-    return 4, 2 if many else 1, 4 if rank <= 64 else 2 if rank <= 128 else 1
+    set.  (us, 1, 2 and 4 blocks: 77 rows, rank 23, 12.8, 12.9, 14.3; 32 rows of 11008 12.6, 11.5,
+    11.7; 600 of 4096, rank 64, 62, 61, 63; 4096 86, 73, 74, and 80 with 2 taken once; 16 rows, rank
+    128, 16.9 and 17.6.)"""
+    return 4, 2 if many else 1, 2 if rank <= 64 else 1
 
 
 def _assemble_adapter_up(decision: DecisionView, op: AdapterUpOp, function_name: str | None) -> KernelGroup:
