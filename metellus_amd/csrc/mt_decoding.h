@@ -99,7 +99,7 @@ MT_INLINE mt_u64 mt_group_before(mt_u64 v, mt_u64* lds, mt_u64& all) {
 // on, so the table can be written in place.
 // Bound by the latency of a launch and of loads in turn -- lengths, then a row's own -- of a few
 // KB (32 sequences, a token each: kernel 3.2 us, call 4.9; 1021 sequences and 16384 tokens,
-// 6 and 5.9).
+// 5.5 and 5.4).
 // ---------------------------------------------------------------------------
 
 // Sums of rows stop at 2^31 - 1, behind any row.
@@ -295,8 +295,8 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // result is lane (n, g)'s i-th: rows are ranks, or columns of the output, so a lane has
 // four neighbours of row m = n of `down` or `out`.
 // Bound by two launches and the latency of loads in turn for few rows (us: 1 row of 4096 x
-// 4096, rank 16, kernels 3.8 and 3.5, call 8.5; 32 rows of 4096 x 11008, an adapter each, 4.4 and
-// 8.0, of which 64 MB of adapters could take 5; 77 of 5003 x 4099, rank 23, 6.9 and 7.6); for
+// 4096, rank 16, kernels 3.9 and 3.3, call 8.1; 32 rows of 4096 x 11008, an adapter each, 4.2 and
+// 7.7, of which 29 MB take 5.7; 77 of 5003 x 4099, rank 23, 7.0 and 6.4); for
 // prompts by MFMAs, half of their rate in the first kernel, and by base and out in the second
 // (4096 rows of 4096 x 4096, rank 64: 32 and 42).
 // ---------------------------------------------------------------------------
