@@ -69,7 +69,7 @@ def _page_check(ops):
 
 @pytest.mark.parametrize("sequences, width, page_size, most, tokens", [
     (1, 1, 1, 1, 1), (1, 4, 16, 1, 3), (3, 7, 5, 4, 9), (64, 9, 16, 1, 64), (65, 3, 20, 30, 500), (255, 4, 8, 2, 300),
-    (256, 4, 8, 2, 256), (257, 4, 8, 2, 250), (1023, 6, 3, 9, 4000), (1025, 6, 16, 3, 1000), (5000, 3, 7, 2, 9000),
+    (256, 4, 8, 2, 256), (257, 4, 8, 2, 250), (512, 5, 16, 2, 600), (513, 5, 16, 2, 600), (1023, 6, 3, 9, 4000), (1025, 6, 16, 3, 1000), (5000, 3, 7, 2, 9000),
     (2, 9000, 16, 30000, 70000),
 ])
 def test_page_tables(sequences, width, page_size, most, tokens):
@@ -143,7 +143,7 @@ SPECS = [
     Rotary(dim=80, part=20), Rotary(dim=10, part=6, layout="interleaved"), Rotary(dim=3, part=2),
     Rotary(dim=256, base=500000.0, factor=8.0, original=8192, low=1.0, high=4.0),
     Rotary(dim=128, part=64, factor=16.0, original=4096, magnitude=1.2772588722239782),
-    Rotary(dim=8, frequencies=(1.0, -0.5, 0.0, 1048576.0)),
+    Rotary(dim=8, frequencies=(1.0, -0.5, 0.0, 1048576.0)), Rotary(dim=160, part=96),
 ]
 
 
@@ -611,3 +611,43 @@ def test_steps_of_two_threads():
     for a, b in zip(got, want):
         for name in NAMES:
             np.testing.assert_array_equal(a[name], b[name], err_msg=name)
+
+
+def test_one_tensor_for_several_arguments():
+    rng = np.random.default_rng(77)
+    ops = Operations()
+    spec = Rotary(dim=16)
+    _put(ops, "x", rng.standard_normal((6, 32)).astype(np.float32))
+    _put(ops, "n", np.array([3, 0, 5, 1, 2, 4], np.int32))
+    ops.rotary("x", positions="n", out="y", rotary=spec, k="x", k_out="z")
+    _put(ops, "ab", rng.standard_normal((64, 32)).astype(np.float32))
+    ops.adapters("x", base="x", a="ab", b="ab", ids="n", out="w")
+    _put(ops, "u", rng.random(6).astype(np.float32))
+    ops.sample("x", uniforms="u", temperatures="u", top_k="n", top_p="u", min_p="u", out="t")
+    _put(ops, "table", np.full((6, 9), -1, np.int32))
+    ops.page_tables("table", free="n", lengths="n", counts="n", page_size=4, tokens=20, out="table1", slots="s", positions="p",
+                    ends="e", used="used")
+    env, ref = run(ops).env, evaluate(ops)
+    bound = _rotary_bound(spec, ops.uploads["x"], ops.uploads["n"])
+    _close(env["y"], ref["y"], bound)
+    _close(env["z"], ref["z"], bound)
+    held = np.abs(ops.uploads["ab"].astype(np.float64)).reshape(2, 32, 32)  # two adapters' A, and their B
+    each = np.zeros((6, 32))
+    for m, i in enumerate(ops.uploads["n"]):
+        if i < 2:
+            each[m] = held[i] @ (held[i] @ np.abs(ops.uploads["x"][m].astype(np.float64)))
+    # (_adapter_bound's terms: one block of 64 columns, the waves, one share; rank 32)
+    _close(env["w"], ref["w"], np.abs(ref["w"]) * U + 1.01 * U * (2 * 64 + ADAPTER_DOWN_WAVES + 1 + 2 * (32 + 15)) * each + 2.0**-149)
+    for name in ("t", "table1", "s", "p", "e", "used"):
+        np.testing.assert_array_equal(env[name], ref[name], err_msg=name)
+
+
+@pytest.mark.parametrize("rows, cols", [(3, 50), (3, 40000)])
+def test_run_again_with_other_inputs(rows, cols):
+    """Nothing is kept from a call for the next: a program run over and over, other logits,
+    numbers and ids each time, scratch as the run before left it."""
+    rng = np.random.default_rng(cols)
+    for _ in range(3):
+        x = (3 * rng.standard_normal((rows, cols))).astype(np.float32)
+        ops = _sample_ops(x, rng.random(rows), top_k=rng.integers(0, 60, rows), top_p=rng.uniform(0.2, 1.1, rows))
+        _sample_check(ops)
