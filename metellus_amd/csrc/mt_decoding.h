@@ -16,20 +16,22 @@
 
 typedef unsigned long long mt_u64;
 
-template <typename OP>
-MT_INLINE mt_u64 mt_wave_fold(mt_u64 v, OP op) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = op(v, (mt_u64)__shfl_xor(v, off, 64));
-    return v;
-}
-
 // The sum of v over this lane and those before it, by adding from one lane, two, four and
 // eight before in rows of 16, then from the ends of the rows before.
 template <int FROM, int ROWS>
-MT_INLINE mt_u64 mt_add_from(mt_u64 v) {
+MT_INLINE mt_u64 mt_from(mt_u64 v) {  // (0 where there is no such lane)
     const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, FROM, ROWS, 15, false);
     const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), FROM, ROWS, 15, false);
-    return v + (((mt_u64)hi << 32) | lo);
+    return ((mt_u64)hi << 32) | lo;
+}
+template <int FROM, int ROWS>
+MT_INLINE mt_u64 mt_add_from(mt_u64 v) {
+    return v + mt_from<FROM, ROWS>(v);
+}
+template <int FROM, int ROWS>
+MT_INLINE mt_u64 mt_most_from(mt_u64 v) {
+    const mt_u64 other = mt_from<FROM, ROWS>(v);
+    return other > v ? other : v;
 }
 MT_INLINE mt_u64 mt_wave_upto(mt_u64 v) {
     v = mt_add_from<0x111, 15>(v);  // row_shr:1
@@ -46,16 +48,21 @@ MT_INLINE mt_u64 mt_wave_last(mt_u64 v) {
 }
 MT_INLINE mt_u64 mt_wave_sum(mt_u64 v) { return mt_wave_last(mt_wave_upto(v)); }
 
-// v (op) over the workgroup's waves; `lds` holds a word a wave.
-template <unsigned WAVES, typename OP>
-MT_INLINE mt_u64 mt_group_fold(mt_u64 v, mt_u64* lds, OP op) {
-    v = mt_wave_fold(v, op);
+// The largest of a wave's, and of a workgroup's.
+MT_INLINE mt_u64 mt_wave_most(mt_u64 v) {
+    v = mt_most_from<0x112, 15>(mt_most_from<0x111, 15>(v));
+    v = mt_most_from<0x118, 15>(mt_most_from<0x114, 15>(v));
+    return mt_wave_last(mt_most_from<0x143, 12>(mt_most_from<0x142, 10>(v)));
+}
+template <unsigned WAVES>
+MT_INLINE mt_u64 mt_group_most(mt_u64 v, mt_u64* lds) {
+    v = mt_wave_most(v);
     __syncthreads();
     if (mt_lane() == 0u) lds[mt_wave()] = v;
     __syncthreads();
     v = lds[0];
 #pragma unroll
-    for (unsigned w = 1; w < WAVES; ++w) v = op(v, lds[w]);
+    for (unsigned w = 1; w < WAVES; ++w) v = lds[w] > v ? lds[w] : v;
     return v;
 }
 
@@ -403,12 +410,6 @@ struct mt_adapter_rows {
         return id != -2 && (unsigned)__builtin_ctzll(all) == j ? all : 0ull;
     }
 };
-
-MT_INLINE mt_f32x4 mt_mfma16_f32(mt_f32x4 a, mt_f32x4 b, mt_f32x4 c) {
-#pragma unroll
-    for (unsigned i = 0; i < 4u; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-}
 
 // A workgroup's tile and its share of the columns (blockIdx.x; blockIdx.y is the row of the
 // tile that may lead, so that those of first rows, which all do, go first).  With turns the GPU's
@@ -1116,7 +1117,7 @@ MT_INLINE mt_u64 mt_sample_best(EACH each, mt_u64* lds) {
             best = found > best ? found : best;
         }
     });
-    return mt_group_fold<MT_SAMPLE_WAVES>(best, lds, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
+    return mt_group_most<MT_SAMPLE_WAVES>(best, lds);
 }
 
 // A chunk's logits, and about what they weigh where asked, added to the bins in LDS, which are 0;
@@ -1318,7 +1319,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
             best = one > best ? one : best;
             if (CUT && t < 64u) kept[c] = one;
         }
-        best = mt_wave_fold(best, [](mt_u64 a, mt_u64 b) { return a > b ? a : b; });
+        best = mt_wave_most(best);
     }
     if (mt_sample_plain(best, asked.temperature, row, part == 0u && t == 0u, tokens, logprobs)) return;
     const mt_weights<SHIFT> weights(mt_order_value((unsigned)(best >> 32)), asked.temperature, powers);
