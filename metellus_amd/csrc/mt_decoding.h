@@ -302,10 +302,10 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // result is lane (n, g)'s i-th: rows are ranks, or columns of the output, so a lane has
 // four neighbours of row m = n of `down` or `out`.
 // Bound by two launches and the latency of loads in turn for few rows (us: 1 row of 4096 x
-// 4096, rank 16, kernels 3.9 and 3.3, call 8.1; 32 rows of 4096 x 11008, an adapter each, 4.2 and
-// 7.7, of which 29 MB take 5.7; 77 of 5003 x 4099, rank 23, 7.0 and 6.4); for
+// 4096, rank 16, kernels 3.8 and 3.1, call 8.4; 32 rows of 4096 x 11008, an adapter each, 4.4 and
+// 8.0, of which 29 MB take 5.7; 77 of 5003 x 4099, rank 23, 7.1 and 6.5); for
 // prompts by MFMAs, half of their rate in the first kernel, and by base and out in the second
-// (4096 rows of 4096 x 4096, rank 64: 32 and 42).
+// (4096 rows of 4096 x 4096, rank 64: 32 and 43).
 // ---------------------------------------------------------------------------
 
 // Rows are put in order before they are cut into tiles, MT_ADAPTER_ORDERED at a time: by id
@@ -1020,7 +1020,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // Bound by vector instructions where rows are weighed in whole (64 rows of 131072, us: the scan 10,
 // with bins 15, of 6.5 to read them; the second kernel 16 with no cut, 20 by k, 36 by p, of
 // which the pass over the logits takes 8, 2 and 16, and the last workgroup's list, from its
-// arrival on, 3, 7 and 13), by two launches and that list for few rows (one of 131072 5.5 and 12).
+// arrival on, 3, 7 and 13), by two launches and that list for few rows (one of 131072 5.3 and 12).
 // ---------------------------------------------------------------------------
 
 constexpr unsigned MT_SAMPLE_WAVES = 8u, MT_SAMPLE_LANES = 512u;
