@@ -793,10 +793,10 @@ struct mt_weights {
         return __builtin_bit_cast(mt_u64, sum) - __builtin_bit_cast(mt_u64, 0x1.8p52);
     }
     MT_INLINE mt_u64 held(float x) const { return whole(weight(x)); }
-    // 0 for a weight below `least`.
+    // 0 for a weight below e^least, told by its logarithm: weights that differ by less than
+    // they are rounded by still do.
     MT_INLINE mt_u64 kept(float x, double least) const {
-        const double w = weight(x);
-        return w < least ? 0 : whole(w);
+        return scaled(x) < least ? 0 : whole(weight(x));
     }
     MT_INLINE static double log_of(mt_u64 total) { return log((double)total * (1.0 / (double)(1ull << SHIFT))); }
     MT_INLINE void answer(unsigned row, unsigned i, float x, double log_total, int* tokens, float* logprobs) const {
@@ -852,7 +852,7 @@ MT_INLINE unsigned mt_find_cut(EACH each, AMOUNT amount, mt_u64 asked, mt_u64& a
 // A row's numbers.
 struct mt_asked {
     float temperature, p, u;
-    double least;
+    double least;  // a weight's logarithm
     int k;
     MT_INLINE mt_asked(unsigned row, const float* uniforms, const float* temperatures, const int* top_k, const float* top_p,
                        const float* min_p) {
@@ -861,7 +861,8 @@ struct mt_asked {
         p = top_p != nullptr ? top_p[row] : 1.f;
         u = uniforms[row];
         const float m = min_p != nullptr ? min_p[row] : 0.f;
-        least = m > 0.f ? (double)__builtin_fminf(m, 1.f) : 0.0;
+        least = m > 0.f ? log((double)__builtin_fminf(m, 1.f)) : -INFINITY;
+        if (temperature == INFINITY) least = __builtin_fmin(least, -1e-200);  // (what is finite is scaled to less than that)
     }
     // The weight before which the largest stay, of `total`: the first always does.
     MT_INLINE mt_u64 weight_asked(mt_u64 total) const {
@@ -1277,7 +1278,7 @@ MT_INLINE void mt_sample_short(const mt_u64* list, unsigned n, const mt_asked& a
         const mt_u64 larger = before([&](mt_u64 other, mt_u64 more) { return other > one ? more : 0; });
         if (!(larger < wanted)) weight = 0;
     }
-    if (w < asked.least) weight = 0;
+    if (weights.scaled(mt_order_value((unsigned)(one >> 32))) < asked.least) weight = 0;
     __syncthreads();
     if (share == 0u) amount[l] = weight;
     const mt_u64 total = mt_group_sum<WAVES>(weight, lds), target = asked.target(total);
@@ -1430,7 +1431,7 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
                     const double w = weights.weight(v[j]);
                     const mt_u64 h = weights.whole(w);
                     const bool in = !CUT || !(below[j] >= whole_from);
-                    all += h, above += in ? h : 0, stay += in && w >= asked.least ? h : 0;
+                    all += h, above += in ? h : 0, stay += in && weights.scaled(v[j]) >= asked.least ? h : 0;
                 }
             }
             if (CUT && cuts && __ballot(nearest <= (float)upto) != 0) {

@@ -139,7 +139,7 @@ def sample_row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         before = upto - weight[order]
         order = order[: max(1, int((before < np.longdouble(top_p) * upto[-1]).sum()))]
     if min_p > 0:
-        order = order[weight[order] >= min(1.0, float(min_p))]
+        order = order[scaled[order] >= math.log(min(1.0, float(min_p)))]  # (of weights, not of what they are rounded to)
     order = np.sort(order)
     upto = np.cumsum(weight[order])
     behind = np.nonzero(upto > (np.longdouble(u) if u > 0 else 0) * upto[-1])[0]

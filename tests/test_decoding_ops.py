@@ -343,6 +343,9 @@ def test_oracle_of_a_draw():
     assert draw(x, 0.3, top_p=0.5)[0] == 1 and draw(x, 0.5, top_p=0.5)[0] == 4  # 5 of 16 is less than 8: the first 4 too
     assert draw(x, 0.0, min_p=0.5)[0] == 1 and draw(x, 0.3, min_p=0.9)[0] == 4
     assert draw(x, 0.9, temperature=0.0) == (4, 0.0)
+    close = np.array([-1e-20, 0, 0, -1e-25], np.float32)  # all of weight 1 as numbers of 64 bits
+    assert draw(close, 0.9, min_p=1.0) == (2, pytest.approx(math.log(1 / 2))) and draw(close, 0.9)[0] == 3
+    assert draw(close, 0.9, min_p=1.0, temperature=math.inf)[0] == 3
     assert draw(x, 1.0)[0] == 4 and draw(x, 0.2)[1] == pytest.approx(math.log(4 / 16))
     assert draw(np.array([-np.inf, np.nan]), 0.5)[0] == -1 and draw(np.array([-np.inf] * 2), 0.5)[0] == -1
 

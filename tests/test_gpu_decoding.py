@@ -642,6 +642,22 @@ def test_one_tensor_for_several_arguments():
         np.testing.assert_array_equal(env[name], ref[name], err_msg=name)
 
 
+@pytest.mark.parametrize("rows, cols", [(4, 50), (4, 300), (2, 40000)])
+def test_sample_weights_just_below_the_largest(rows, cols):
+    """min_p = 1 keeps the largest and its equals, however close the others come; all that are
+    finite at an infinite temperature."""
+    x = np.full((rows, cols), -1e-20, np.float32)
+    x[:, [1, cols - 2]] = 0.0
+    x[:, 3] = -1e-25
+    x[:, 4] = -np.inf
+    for asked in ({"min_p": 1.0}, {"min_p": 1.0, "top_k": 100}, {"min_p": 1.0, "top_p": 0.9, "temperatures": 1e30},
+                  {"min_p": 0.5, "temperatures": np.inf}, {"min_p": 1.0, "temperatures": np.inf}):
+        ops = _sample_ops(x, (np.arange(rows) + 0.5) / rows, **asked)
+        t = _sample_check(ops)
+        if asked.get("temperatures") != np.inf:
+            assert set(t) == {1, cols - 2}
+
+
 @pytest.mark.parametrize("rows, cols", [(3, 50), (3, 40000)])
 def test_run_again_with_other_inputs(rows, cols):
     """Nothing is kept from a call for the next: a program run over and over, other logits,
