@@ -1414,8 +1414,10 @@ MT_INLINE void mt_sample_pick(const float* logits, const float* uniforms, const 
     if (!whole) {
         mt_u64 all = 0, above = 0;
         const bool weigh_all = by_p && !by_k;
-        // what is above this stays as far as the bins say, and of what is above that all is weighed
-        const float whole_from = cuts ? (float)from : INFINITY, weighed = weigh_all ? INFINITY : whole_from;
+        // Logits of bins before `whole_from` stay as far as the bins say, those of bins before `weighed`
+        // are weighed.  (NaN where nothing cuts, which no bin is at or behind, not the infinite and NaN
+        // ones of logits off the grid either: all are weighed, the largest too, and a row's total is never 0.)
+        const float whole_from = cuts ? (float)from : NAN, weighed = weigh_all ? INFINITY : whole_from;
         for (unsigned c = t; c < SEGMENTS; c += LANES) kept[c] = 0;
         __syncthreads();
         mt_sample_each<V, CHUNK, CS>(x, part * CHUNK, [&](unsigned q, unsigned i, mt_f32x4 v) {

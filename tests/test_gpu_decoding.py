@@ -667,3 +667,76 @@ def test_run_again_with_other_inputs(rows, cols):
         x = (3 * rng.standard_normal((rows, cols))).astype(np.float32)
         ops = _sample_ops(x, rng.random(rows), top_k=rng.integers(0, 60, rows), top_p=rng.uniform(0.2, 1.1, rows))
         _sample_check(ops)
+
+
+class _Kept:
+    """A program compiled once, and its buffers, which start full of 0xF9 bytes: what no
+    kernel writes is no token (-101058055), and no scratch is clear."""
+
+    def __init__(self, ops):
+        groups = compile_program(ops)
+        self.ops, self.env = ops, {name: Buffer.from_numpy(v) for name, v in ops.uploads.items()}
+        for t in ops.tensors.values():
+            if t.buffer_key not in self.env:
+                self.env[t.buffer_key] = Buffer(t.nbytes)
+                self.env[t.buffer_key].fill(0xF9)
+        self.runtime = Runtime(tuple(Dispatch(g.kernel, g.bindings, g.dims, g.grid, g.threads) for g in groups))
+
+    def run(self, **inputs):
+        """With other inputs, where given; all that the program has made."""
+        for name, v in inputs.items():
+            self.ops.uploads[name][...] = v
+            self.env[name].write(self.ops.uploads[name])
+        self.runtime.run(self.env)
+        return {n: self.env[t.buffer_key].numpy(t.shape, np.dtype(t.stored)) for n, t in self.ops.tensors.items()}
+
+
+def _sample_compare(ops, env):
+    ref = evaluate(ops)
+    np.testing.assert_array_equal(env["t"], ref["t"])
+    n = ops.tensors["x"].shape[1]
+    _close(env["lp"], ref["lp"], 1.01 * U * np.abs(ref["lp"]) + n * 2.0 ** -min(44, 62 - (n - 1).bit_length()) + 2.0**-149)
+
+
+OFF = {"top_k": (0, -3, 10**6), "top_p": (1.0, 2.0, np.nan)}  # what cuts nothing
+
+
+@pytest.mark.parametrize("cols", [5, 700, 12345, 40000])
+@pytest.mark.parametrize("temperature", [1.0, 1e-36, 1e-37, 1e-38, 1e-45, 3e38, np.inf])
+def test_sample_rows_off_the_grid_that_nothing_cuts(cols, temperature):
+    """Rows that k and p leave whole in programs that have k or p: with infinities one in four
+    neighbours and four, and logits that fp32 does not hold divided by the temperature."""
+    rng = np.random.default_rng(cols)
+    low, x = np.finfo(np.float32).min, rng.standard_normal((9, cols)).astype(np.float32)
+    x[0, 3] = np.inf
+    x[1, 1] = x[1, cols - 1] = np.inf
+    x[2, :4] = np.inf
+    x[3], x[3, 2] = low, 30.0
+    x[4], x[4, 4] = -np.inf, np.inf
+    x[5], x[5, 0] = -30.0, low
+    x[6] = np.inf
+    x[7, 2], x[7, 4] = 3e38, -np.inf
+    for name, values in OFF.items():
+        for off in values:
+            ops = _sample_ops(x, rng.random(9), temperatures=temperature, **{name: off})
+            _sample_compare(ops, _Kept(ops).run())
+
+
+@pytest.mark.parametrize("cols", [700, 12345, 40000])
+def test_sample_rows_cut_and_whole_with_infinities(cols):
+    """The same rows beside each other cut by k, by p, by both and by neither, at ordinary and
+    at tiny temperatures."""
+    rng = np.random.default_rng(cols + 1)
+    low, rows = np.finfo(np.float32).min, 256
+    x = 3 * rng.standard_normal((rows, cols)).astype(np.float32)
+    x[0::8, 3] = np.inf
+    x[1::8, 1] = x[1::8, cols - 1] = np.inf
+    x[2::8, 8:12] = np.inf
+    x[3::8] = -np.inf
+    x[3::8, 6] = 1.0
+    x[4::8, 9:] = low
+    x[5::8], x[5::8, 7] = low, np.inf
+    ops = _sample_ops(
+        x, rng.random(rows), temperatures=rng.choice([1.0, 0.7, 1e-36, 1e-38, 1e-45, 0.0, np.inf], rows),
+        top_k=rng.choice([0, 2, 50, 10**6], rows), top_p=rng.choice([1.0, 0.7, np.nan], rows), min_p=rng.choice([0.0, 0.5], rows))
+    _sample_compare(ops, _Kept(ops).run())
