@@ -653,7 +653,7 @@ class Operations:
                 **{n: t if cuts else None for n, t in given.items() if n != "min_p"},
                 after=self._owners(tl, *given.values()),
             )
-        names = [t.name for t in pick.outs]
+        names = [t.name for t in (*(scan.outs if apart else ()), *pick.outs)]
         if len(set(names)) < len(names):
             raise ValueError(f"output names must differ; got {names}")
         if apart:

@@ -388,3 +388,19 @@ def test_sample_compiles(asked, cols):
     ops = _ops(**{**SAMPLE, "x": (3, cols)})
     ops.sample("x", uniforms="u", out="t", **asked)
     _compile(ops)
+
+
+# -- calls at the border of what is allowed -----------------------------------------------
+
+
+@pytest.mark.parametrize("taken", ["t", "t.best", "t.counts", "t.bins", "t.sums", "t.list"])
+def test_sample_names_differ_from_its_own_tensors(taken):
+    """Also from those of the first of the two kernels that rows of several chunks take; a
+    refused call leaves no name behind."""
+    ops = _ops(**{**SAMPLE, "x": (3, 40000)})
+    before = set(ops.tensors)
+    with pytest.raises(ValueError, match="output names must differ"):
+        ops.sample("x", uniforms="u", out="t", top_k="k", logprobs=taken)
+    assert not ops.build() and not ops.scratch and set(ops.tensors) == before
+    ops.sample("x", uniforms="u", out="t", top_k="k", logprobs="lp")
+    assert len(compile_program(ops)) == 2
