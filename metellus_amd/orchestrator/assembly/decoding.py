@@ -70,7 +70,7 @@ def _assemble_page_tables(decision: DecisionView, op: PageTablesOp, function_nam
     )
     frag = ServingFragment(
         "mt_page_tables",
-        (int(op.page_size), lanes),
+        (op.page_size, lanes),
         args,
         lds_bytes=4 * (2 * (lanes + 1) + 2 * (lanes // 64)),
         name="page_tables",

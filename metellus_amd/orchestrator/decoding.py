@@ -192,6 +192,7 @@ class PageTablesOp(ServingOp):
         rows, width = self.pages.shape
         if isinstance(self.page_size, bool) or not isinstance(self.page_size, (int, np.integer)) or self.page_size <= 0:
             raise ValueError(f"page_tables page_size must be a positive int; got {self.page_size!r}")
+        object.__setattr__(self, "page_size", int(self.page_size))  # (numpy's products wrap)
         if width * self.page_size > POSITIONS_MAX or rows * width > _INT32_MAX:
             raise ValueError(f"page_tables: {rows} rows of {width} pages of {self.page_size}; positions and entries are int32")
         _list("page_tables free", self.free, "int32")

@@ -404,3 +404,16 @@ def test_sample_names_differ_from_its_own_tensors(taken):
     assert not ops.build() and not ops.scratch and set(ops.tensors) == before
     ops.sample("x", uniforms="u", out="t", top_k="k", logprobs="lp")
     assert len(compile_program(ops)) == 2
+
+
+@pytest.mark.parametrize("page_size", [np.int32(2**29), np.int64(2**29), np.uint32(2**29), np.int32(2**30)])
+def test_page_sizes_of_numpy_are_checked_as_others(page_size):
+    """A table's positions are counted in Python's whole numbers, which do not wrap."""
+    ops = _ops(**PAGES)
+    with pytest.raises(ValueError, match="positions and entries are int32"):
+        ops.page_tables(**{**PAGE_CALL, "page_size": page_size})
+    wide = _ops(**{**PAGES, "pages": ((4, 9000), "int32")})
+    for i, small in enumerate((np.int8(16), np.uint8(16), np.int16(16))):
+        call = {**PAGE_CALL, "page_size": small, **{n: f"{n}{i}" for n in ("out", "slots", "positions", "ends", "used")}}
+        wide.page_tables(**{**call, "pages": "pages" if i == 0 else f"out{i - 1}"})
+    assert [type(op.page_size) for op in wide.build()] == [int] * 3
