@@ -116,7 +116,7 @@ def _assemble_rotary(decision: DecisionView, op: RotaryOp, function_name: str | 
         sig.add("k", op.k),
         sig.add("positions", op.positions),
         "mt_turns",
-        repr(float(spec.magnitude)),
+        repr(spec.magnitude),
         sig.add("y", op.y, out=True),
         sig.add("k_out", op.k_out, out=True),
         "M",

@@ -71,6 +71,14 @@ class Rotary:
             if isinstance(v, bool) or not isinstance(v, (int, np.integer)) or v <= 0:
                 raise ValueError(f"rotary: {name} must be a positive int; got {v!r}")
             object.__setattr__(self, name, int(v))
+        for name in ("base", "factor", "low", "high", "magnitude"):
+            v = getattr(self, name)
+            try:
+                if isinstance(v, (str, bytes)):
+                    raise TypeError
+                object.__setattr__(self, name, float(v))  # (in 64 bits, whatever numpy's type is)
+            except (TypeError, ValueError, OverflowError):
+                raise ValueError(f"rotary: {name} must be a number of 64 bits; got {v!r}") from None
         if self.dim > HEAD_DIM_MAX:
             raise ValueError(f"rotary: dim must be at most {HEAD_DIM_MAX}; got {self.dim}")
         if self.part % 2 or self.part > self.dim:
@@ -84,6 +92,7 @@ class Rotary:
         if self.original is not None:
             if isinstance(self.original, bool) or not isinstance(self.original, (int, np.integer)) or self.original <= 0:
                 raise ValueError(f"rotary: original must be a positive int; got {self.original!r}")
+            object.__setattr__(self, "original", int(self.original))
             if not 0.0 <= self.low < self.high < math.inf:
                 raise ValueError(f"rotary: low and high must be finite, 0 <= low < high; got {self.low} and {self.high}")
         if not 0.0 < self.magnitude <= 2.0**60:

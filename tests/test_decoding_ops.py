@@ -417,3 +417,28 @@ def test_page_sizes_of_numpy_are_checked_as_others(page_size):
         call = {**PAGE_CALL, "page_size": small, **{n: f"{n}{i}" for n in ("out", "slots", "positions", "ends", "used")}}
         wide.page_tables(**{**call, "pages": "pages" if i == 0 else f"out{i - 1}"})
     assert [type(op.page_size) for op in wide.build()] == [int] * 3
+
+
+def test_rotations_by_numbers_of_numpy():
+    """Numbers of numpy's types count as the Python numbers that they are equal to: the same
+    spec, with the same turns, in the same kernel."""
+    f32 = np.float32
+    spec = Rotary(dim=np.int64(64), base=f32(500000), factor=f32(8), original=np.int32(8192), low=f32(1), high=f32(4),
+                  magnitude=f32(1.25))
+    plain = Rotary(dim=64, base=500000.0, factor=8.0, original=8192, low=1.0, high=4.0, magnitude=1.25)
+    assert spec == plain and spec.turns == plain.turns and all(type(f) is float for f in spec.angles)
+    assert Rotary(dim=64, base=f32(10000), factor=f32(4)).turns == Rotary(dim=64, factor=4.0).turns
+    ops = _ops(**{**ROTARY, "k": (3, 64)})
+    ops.rotary("q", positions="at", out="q1", rotary=spec, k="k", k_out="k1")
+    (one,) = compile_program(ops)
+    ops = _ops(**{**ROTARY, "k": (3, 64)})
+    ops.rotary("q", positions="at", out="q1", rotary=plain, k="k", k_out="k1")
+    (two,) = compile_program(ops)
+    assert one.kernel.source == two.kernel.source
+
+
+@pytest.mark.parametrize("name", ["base", "factor", "low", "high", "magnitude"])
+@pytest.mark.parametrize("value", ["1", None, 1j, 10**400, [2.0]])
+def test_rotations_by_what_is_no_number(name, value):
+    with pytest.raises(ValueError, match=f"rotary: {name} must be"):
+        Rotary(dim=64, original=4096, **{name: value})
