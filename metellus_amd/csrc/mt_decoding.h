@@ -141,10 +141,11 @@ MT_INLINE unsigned mt_lane_of(const unsigned* before, unsigned v) {
 }
 
 template <unsigned P, unsigned LANES>
-MT_INLINE void mt_page_tables(int* pages, const int* free, const int* lengths, const int* counts, int* slots,
-                              int* positions, int* ends, int* used, unsigned rows, unsigned sequences, unsigned width,
-                              unsigned frees, unsigned* lds) {
+MT_INLINE void mt_page_tables(int* pages, const int* free, const int* taken, const int* lengths, const int* counts,
+                              int* slots, int* positions, int* ends, int* used, unsigned rows, unsigned sequences,
+                              unsigned width, unsigned frees, unsigned* lds) {
     constexpr unsigned WAVES = LANES / 64u;
+    const unsigned gone = taken != nullptr && *taken > 0 ? (unsigned)*taken : 0u;  // (and the needed: below 2^32)
     unsigned *rows_before = lds, *need_before = lds + LANES + 1u, *sums = lds + 2u * (LANES + 1u);
     const unsigned t = threadIdx.x, room = width * P, each = (sequences + LANES - 1u) / LANES;
     const unsigned first = t * each < sequences ? t * each : sequences;
@@ -183,7 +184,7 @@ MT_INLINE void mt_page_tables(int* pages, const int* free, const int* lengths, c
             if (i < s.end - s.begin) {
                 const unsigned at = s.begin + i, entry = at / P;
                 position = (int)at;
-                page += entry - s.have;  // (where the entry is new)
+                page += gone + entry - s.have;  // (where the entry is new)
                 const int number = entry < s.have ? pages[(size_t)b * width + entry] : page < frees ? free[page] : -1;
                 const long long found = (long long)number * P + at % P;
                 if (number >= 0 && found <= 0x7FFFFFFFll) slot = (int)found;
@@ -199,9 +200,9 @@ MT_INLINE void mt_page_tables(int* pages, const int* free, const int* lengths, c
             i -= s.need, ++b;
             s = mt_growth<P>(lengths[b], counts[b], room);
         }
-        pages[(size_t)b * width + s.have + i] = e < frees ? free[e] : -1;
+        pages[(size_t)b * width + s.have + i] = gone + e < frees ? free[gone + e] : -1;
     }
-    if (blockIdx.x == 0u && t == 0u) *used = (int)all_need;
+    if (blockIdx.x == 0u && t == 0u) *used = (int)mt_add_rows(gone, all_need);
 }
 
 // ---------------------------------------------------------------------------

@@ -60,6 +60,7 @@ def _assemble_page_tables(decision: DecisionView, op: PageTablesOp, function_nam
     args = (
         sig.add("pages", op.pages, out=True),
         sig.add("free", op.free),
+        sig.add("taken", op.taken),
         sig.add("lengths", op.lengths),
         sig.add("counts", op.counts),
         sig.add("slots", op.slots, out=True),

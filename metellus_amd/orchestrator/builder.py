@@ -84,6 +84,7 @@ class Operations:
         self._written: dict[str, str] = {}  # a cache's older state -> the state after the write
         self._cache_readers: dict[str, list[Tensor]] = {}
         self._tables: dict[str, str] = {}  # a block table's older state -> the state after it
+        self._used: dict[tuple[str, str], str] = {}  # (table, free)'s buffers -> how many of free are gone
         self._scratch: set[str] = set()  # what one kernel of an operator leaves for the next
 
     # -- registry ------------------------------------------------------------
@@ -482,6 +483,7 @@ class Operations:
         positions: str,
         ends: str,
         used: str,
+        taken: str | None = None,
     ) -> Tensor:
         """Make room for a step's tokens: sequence b goes on from ``lengths[b]`` by
         ``counts[b]`` positions, and the pages that it lacks are taken from ``free`` in
@@ -489,10 +491,16 @@ class Operations:
         may not be read any more; entries that no new page goes to are left as they were.
         Further outputs, int32 all: ``slots`` and ``positions`` of ``tokens`` rows (each
         sequence's after the other's; -1 behind the last, which ``cache_write`` passes
-        over), the lengths after the step in ``ends``, and in ``used`` how many pages were
-        needed (more than ``free`` has: the rest of the entries is -1, and their tokens
-        have no slots).  A sequence grows to the end of its table and no further."""
+        over), the lengths after the step in ``ends``, and in ``used`` how many of ``free`` are
+        gone after it (more than it has: the rest of the entries is -1, and their tokens
+        have no slots).  A sequence grows to the end of its table and no further.
+
+        ``taken`` (int32, one number) is how many of ``free`` are gone before the step, so the
+        ``used`` of the step before; without it none are, but in a program that has made
+        room in this table from this ``free`` before, what is gone since.  A ``free`` that
+        begins with pages that an earlier step gave out gives them out again."""
         tp, tf, tl, tc = self._lookup(pages), self._lookup(free), self._lookup(lengths), self._lookup(counts)
+        tt = self._optional(taken if taken is not None else self._used.get((tp.buffer_key, tf.buffer_key)))
         if isinstance(tokens, bool) or not isinstance(tokens, (int, np.integer)) or not 0 < tokens < 2**31:
             raise ValueError(f"page_tables tokens must be a positive int32; got {tokens!r}")
         states = {pages, *self._tables}
@@ -511,13 +519,15 @@ class Operations:
             lengths=tl,
             counts=tc,
             page_size=page_size,
+            taken=tt,
             after=(
-                *self._owners(tf, tl, tc),
+                *self._owners(tf, tl, tc, tt),
                 *(o.out for o in self._ops if any(t.name == pages for t in o.inputs)),  # who read the older state
             ),
         )
         self._emit_all(op)
         self._tables[pages] = out
+        self._used[tp.buffer_key, tf.buffer_key] = used
         return op.written
 
     def rotary(

@@ -176,8 +176,9 @@ class PageTablesOp(ServingOp):
     """With L = lengths clamped to the table's room, C = max(counts, 0) and E = L + C
     clamped to it (``ends``): sequence b has the first ceil(L / page_size) entries of
     its row of ``pages``, and gets those up to ceil(E / page_size) from ``free``, whose
-    numbers go to the sequences in turn, -1 behind its end.  ``used`` is how many were
-    needed.  Token rows are packed, C of each sequence after the other: the i-th of
+    numbers go to the sequences in turn from the ``taken``-th on (the first, where not
+    given or below 0), -1 behind its end.  ``used`` is ``taken`` and how many were needed,
+    2^31 - 1 at the most.  Token rows are packed, C of each sequence after the other: the i-th of
     sequence b has position L + i and that position's slot; -1 for both beyond the
     room and behind the last sequence, and for a slot whose page is below 0."""
 
@@ -191,6 +192,7 @@ class PageTablesOp(ServingOp):
     lengths: Tensor
     counts: Tensor
     page_size: int
+    taken: Tensor | None = None
     after: tuple[Tensor, ...] = ()
 
     def __post_init__(self) -> None:
@@ -207,6 +209,8 @@ class PageTablesOp(ServingOp):
         _list("page_tables free", self.free, "int32")
         _list("page_tables lengths", self.lengths, "int32", rows)
         _list("page_tables counts", self.counts, "int32", rows)
+        if self.taken is not None:
+            _list("page_tables taken", self.taken, "int32", 1)
 
     @property
     def overwrites(self) -> Tensor:
@@ -218,7 +222,7 @@ class PageTablesOp(ServingOp):
 
     @property
     def reads(self) -> tuple[Tensor, ...]:
-        return (self.pages, self.free, self.lengths, self.counts)
+        return tuple(t for t in (self.pages, self.free, self.lengths, self.counts, self.taken) if t is not None)
 
 
 @dataclass(frozen=True)

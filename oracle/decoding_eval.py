@@ -16,7 +16,8 @@ F64 = np.float64
 def _page_tables(op, get):
     p, table, free = op.page_size, np.array(get(op.pages)), list(get(op.free))
     width, rows = table.shape[1], op.slots.shape[0]
-    slots, positions, ends, used = [], [], [], 0
+    slots, positions, ends = [], [], []
+    used = 0 if op.taken is None else max(0, int(get(op.taken)[0]))
     for b, (length, count) in enumerate(zip(get(op.lengths).tolist(), get(op.counts).tolist())):
         begin = min(max(length, 0), width * p)
         have = -(-begin // p)
@@ -32,7 +33,7 @@ def _page_tables(op, get):
             slots.append(slot if page >= 0 and slot < 2**31 else -1)
         ends.append(end)
     pad = [-1] * (rows - len(slots))
-    made = {op.slots: slots + pad, op.positions: positions + pad, op.ends: ends, op.used: [used]}
+    made = {op.slots: slots + pad, op.positions: positions + pad, op.ends: ends, op.used: [min(used, 2**31 - 1)]}
     return {op.written.name: table, **{t.name: np.array(v, np.int32) for t, v in made.items()}}
 
 

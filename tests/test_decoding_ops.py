@@ -442,3 +442,58 @@ def test_rotations_by_numbers_of_numpy():
 def test_rotations_by_what_is_no_number(name, value):
     with pytest.raises(ValueError, match=f"rotary: {name} must be"):
         Rotary(dim=64, original=4096, **{name: value})
+
+
+def _more(i: int, **call) -> dict:
+    """The i-th step on the same table."""
+    before = "table" if i == 2 else f"out{i - 1}"
+    return {**PAGE_CALL, "pages": before, "lengths": "ends" if i == 2 else f"ends{i - 1}",
+            **{n: f"{n}{i}" for n in ("out", "slots", "positions", "ends", "used")}, **call}
+
+
+def test_steps_of_a_table_take_other_pages():
+    """A program that makes room in a table again goes on in ``free`` where it was; another
+    list begins at its first, and so does another table."""
+    ops = _ops(**PAGES, others=((9,), "int32"), pages2=((4, 6), "int32"), gone=((1,), "int32"))
+    ops.page_tables(**PAGE_CALL)
+    ops.page_tables(**_more(2))
+    ops.page_tables(**_more(3, free="others"))
+    ops.page_tables(**_more(4))
+    ops.page_tables(**_more(5, taken="gone"))
+    ops.page_tables(**{**_more(6), "pages": "pages2"})
+    assert [o.taken and o.taken.name for o in ops.build()] == [None, "used", None, "used2", "gone", None]
+
+
+def test_oracle_of_steps_of_a_table():
+    ops = _ops(pages=((2, 4), "int32"), free=((5,), "int32"), lengths=((2,), "int32"), counts=((2,), "int32"))
+    for name, v in (("pages", np.full((2, 4), -1)), ("free", [9, 8, 6, 5, 4]), ("lengths", [0, 0]), ("counts", [3, 2])):
+        ops.from_numpy(np.array(v, np.int32), name)
+    ops.page_tables(**{**PAGE_CALL, "page_size": 2, "tokens": 5})
+    ops.page_tables(**_more(2, page_size=2, tokens=5))
+    ref = evaluate(ops)
+    np.testing.assert_array_equal(ref["table"], [[9, 8, -1, -1], [6, -1, -1, -1]])
+    np.testing.assert_array_equal(ref["out2"], [[9, 8, 5, -1], [6, 4, -1, -1]])
+    np.testing.assert_array_equal(ref["slots2"], [17, 10, 11, 8, 9])
+    assert ref["used"] == [3] and ref["used2"] == [5]
+
+
+@pytest.mark.parametrize("inputs, call, match", [
+    (dict(gone=((2,), "int32")), {}, "taken must have shape"),
+    (dict(gone=(1,)), {}, "taken must be int32"),
+    (dict(gone=((1, 1), "int32")), {}, "taken must be 1D"),
+    ({}, dict(taken="nothing"), "is not declared"),
+])
+def test_page_tables_refusals_of_taken(inputs, call, match):
+    ops = _ops(**{**PAGES, "gone": ((1,), "int32"), **inputs})
+    with pytest.raises(ValueError, match=match):
+        ops.page_tables(**{**PAGE_CALL, "taken": "gone", **call})
+    assert not ops.build() and "table" not in ops.tensors
+
+
+def test_page_tables_of_taken_compile():
+    ops = _ops(**PAGES, gone=((1,), "int32"))
+    ops.page_tables(**PAGE_CALL, taken="gone")
+    ops.page_tables(**_more(2))
+    _compile(ops)
+    kinds = [v.ops[0].out.name for v in fuse(ops.build())]
+    assert kinds == ["table", "out2"]

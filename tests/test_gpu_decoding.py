@@ -740,3 +740,78 @@ def test_sample_rows_cut_and_whole_with_infinities(cols):
         x, rng.random(rows), temperatures=rng.choice([1.0, 0.7, 1e-36, 1e-38, 1e-45, 0.0, np.inf], rows),
         top_k=rng.choice([0, 2, 50, 10**6], rows), top_p=rng.choice([1.0, 0.7, np.nan], rows), min_p=rng.choice([0.0, 0.5], rows))
     _sample_compare(ops, _Kept(ops).run())
+
+
+def _grow(ops, i, pages, lengths, free="free", **call):
+    ops.page_tables(pages, free=free, lengths=lengths, counts=f"counts{i}", page_size=call.pop("page_size"), tokens=call.pop("tokens"),
+                    out=f"table{i}", slots=f"slots{i}", positions=f"positions{i}", ends=f"ends{i}", used=f"used{i}", **call)
+
+
+@pytest.mark.parametrize("sequences, width, page_size, tokens", [(1, 40, 1, 9), (5, 9, 4, 30), (300, 12, 16, 700), (1030, 8, 3, 4000)])
+def test_a_table_grows_by_several_steps(sequences, width, page_size, tokens):
+    """Three steps in a program, from one list: each goes on where the one before ended, so
+    every page has one owner."""
+    rng = np.random.default_rng(sequences)
+    ops = Operations()
+    _put(ops, "table0", np.full((sequences, width), -1, np.int32))
+    _put(ops, "free", rng.permutation(sequences * width).astype(np.int32))
+    _put(ops, "ends0", np.zeros(sequences, np.int32))
+    for i in (1, 2, 3):
+        _put(ops, f"counts{i}", rng.integers(0, width * page_size // 4 + 2, sequences).astype(np.int32))
+        _grow(ops, i, f"table{i - 1}", f"ends{i - 1}", page_size=page_size, tokens=tokens)
+    names = [f"{n}{i}" for i in (1, 2, 3) for n in ("slots", "positions", "ends", "used")] + ["table3"]
+    env, ref = run(ops, outputs=names).env, evaluate(ops)
+    for name in names:
+        np.testing.assert_array_equal(env[name], ref[name], err_msg=name)
+    held = env["table3"][env["table3"] >= 0]
+    assert len(held) == len(set(held.tolist())) == env["used3"][0]
+
+
+@pytest.mark.parametrize("taken", [0, 3, 7, 8, 100, 2**31 - 1, -1, -(2**31)])
+def test_page_tables_behind_what_is_taken(taken):
+    """From the middle of the list, its end and behind it; numbers below 0 are 0."""
+    ops = Operations()
+    _put(ops, "table0", np.full((3, 5), -1, np.int32))
+    _put(ops, "free", np.arange(10, 18, dtype=np.int32))
+    for name, v in (("ends0", [0, 4, 9]), ("counts1", [9, 1, 6]), ("gone", [taken])):
+        _put(ops, name, np.array(v, np.int32))
+    _grow(ops, 1, "table0", "ends0", page_size=4, tokens=20, taken="gone")
+    env, ref = run(ops).env, evaluate(ops)
+    for name in ("table1", "slots1", "positions1", "ends1", "used1"):
+        np.testing.assert_array_equal(env[name], ref[name], err_msg=name)
+
+
+def test_a_loop_of_steps_that_grow():
+    """A program run again and again over its buffers, each step's lengths and what is gone of
+    the list from the step before: a table that fills up page by page, and attention over it
+    that reads what each step wrote."""
+    rng = np.random.default_rng(21)
+    sequences, page_size, width, heads, dim = 6, 4, 5, 2, 32
+    spec = KVCache(pages=sequences * width, page_size=page_size, kv_heads=heads, dim=dim)
+    ops = Operations()
+    _put(ops, "table0", np.full((sequences, width), -1, np.int32))
+    _put(ops, "free", rng.permutation(sequences * width).astype(np.int32))
+    _put(ops, "ends0", np.zeros(sequences, np.int32))
+    _put(ops, "gone", np.zeros(1, np.int32))
+    _put(ops, "counts1", np.ones(sequences, np.int32))
+    for name in ("q", "k", "v"):
+        _put(ops, name, np.zeros((sequences, heads * dim), np.float32))
+    ops.kv_cache("cache", pages=spec.pages, page_size=page_size, kv_heads=heads, dim=dim)
+    ops.from_numpy(spec.empty(), "cache")
+    _grow(ops, 1, "table0", "ends0", page_size=page_size, tokens=sequences, taken="gone")
+    ops.cache_write("cache", k="k", v="v", slots="slots1", out="cache1")
+    ops.paged_attention("q", cache="cache1", pages="table1", lengths="ends1", heads=heads, out="o")
+    kept, more = _Kept(ops), {}
+    for step in range(width * page_size + 2):
+        data = {n: rng.standard_normal((sequences, heads * dim)).astype(np.float32) for n in ("q", "k", "v")}
+        counts = (np.arange(sequences) % 3 <= step % 3).astype(np.int32)  # (not all go on in each)
+        got = kept.run(**data, counts1=counts, **more)
+        ref = evaluate(ops)
+        for name in ("table1", "slots1", "positions1", "ends1", "used1"):
+            np.testing.assert_array_equal(got[name], ref[name], err_msg=f"{name}, step {step}")
+        # (attention's sum of up to 20 products of terms around 1: 2^-14 of the largest)
+        assert np.abs(got["o"] - ref["o"]).max() <= 2.0**-14 * max(1.0, np.abs(ref["o"]).max())
+        ops.uploads["table0"][...], ops.uploads["cache"][...] = got["table1"], got["cache1"]  # (the oracle's next state)
+        more = {"ends0": got["ends1"], "gone": got["used1"]}
+    held = got["table1"][got["table1"] >= 0]
+    assert len(held) == len(set(held.tolist())) == got["used1"][0] and (got["ends1"] == width * page_size).any()
