@@ -815,3 +815,68 @@ def test_a_loop_of_steps_that_grow():
         more = {"ends0": got["ends1"], "gone": got["used1"]}
     held = got["table1"][got["table1"] >= 0]
     assert len(held) == len(set(held.tolist())) == got["used1"][0] and (got["ends1"] == width * page_size).any()
+
+
+def _sample_inputs(rng, rows, cols):
+    """Logits and what rows ask of them: cut or whole, greedy, masked, and drawn from by one
+    workgroup (a bin of more logits than are listed)."""
+    x = (3 * rng.standard_normal((rows, cols))).astype(np.float32)
+    kind = rng.integers(0, 7, rows)
+    x[kind == 0] = rng.standard_normal((int((kind == 0).sum()), cols)) / 100  # (one bin of all)
+    x[kind == 1, rng.integers(0, cols)] = np.nan
+    x[kind == 2] = -np.inf
+    x[kind == 2, rng.integers(0, cols)] = 5
+    x[kind == 3, rng.integers(0, cols)] = np.inf
+    return {
+        "x": x, "u": rng.random(rows), "temperatures": rng.choice([0.0, 0.7, 1.0, 1.5, 1e-38], rows),
+        "top_k": np.where(kind == 0, cols // 3, rng.choice([0, 1, 30, 400, 10**6], rows)),
+        "top_p": rng.choice([0.3, 0.9, 0.99, 1.0, np.nan], rows), "min_p": rng.choice([0.0, 0.05], rows),
+    }
+
+
+@pytest.mark.parametrize("rows, cols", [(24, 300), (24, 40000), (3, 131072), (24, 9001)])
+def test_sample_again_in_its_buffers(rows, cols):
+    """Nothing is kept from a call for the next: one program over one set of buffers, other
+    logits and numbers in each run, so that rows change between the paths, over scratch as
+    the run before left it.  Answers are cleared to what is no token before each run."""
+    rng = np.random.default_rng(rows * cols)
+    first = _sample_inputs(rng, rows, cols)
+    kept = _Kept(_sample_ops(first.pop("x"), first.pop("u"), **first))
+    for _ in range(6):
+        for name in ("t", "lp"):
+            kept.env[name].fill(0xF9)
+        _sample_compare(kept.ops, kept.run(**_sample_inputs(rng, rows, cols)))
+
+
+@pytest.mark.parametrize("rows, inner, cols, rank, held", [
+    (9, 300, 70, 8, 4), (128, 300, 70, 8, 4), (200, 257, 65, 16, 90), (700, 130, 37, 5, 300), (4200, 70, 37, 4, 50),
+    (2048, 2600, 2561, 64, 40),
+])
+def test_adapters_again_in_their_buffers(rows, inner, cols, rank, held):
+    """The same for adapters: other rows, ids in another order -- in runs, at random, of few,
+    none, all alike -- and other weights each time."""
+    rng = np.random.default_rng(rows + rank)
+    kept = _Kept(_adapters(rows, inner, cols, rank, held, rng.integers(-1, held, rows)))
+    kinds = (np.arange(rows) * held // rows, rng.integers(-1, held + 1, rows), np.where(rng.random(rows) < 0.03, held - 1, -1),
+             np.full(rows, -1), np.full(rows, held // 2), np.arange(rows)[::-1] % held)
+    for ids in kinds:
+        kept.env["y"].fill(0xF9)
+        env = kept.run(x=rng.standard_normal((rows, inner)), base=rng.standard_normal((rows, cols)), ids=ids,
+                       a=rng.standard_normal((held * rank, inner)), s=rng.uniform(-2, 2, held))
+        _close(env["y"], evaluate(kept.ops)["y"], _adapter_bound(kept.ops))
+
+
+def test_rotary_again_in_its_buffers():
+    rng = np.random.default_rng(31)
+    spec = Rotary(dim=64, part=48, layout="interleaved")
+    ops = Operations()
+    _put(ops, "q", np.zeros((70, 192), np.float32))
+    _put(ops, "k", np.zeros((70, 64), np.float32))
+    _put(ops, "at", np.zeros(70, np.int32))
+    ops.rotary("q", positions="at", out="q1", rotary=spec, k="k", k_out="k1")
+    kept = _Kept(ops)
+    for far in (100, 2**20, 2**31 - 1):
+        env = kept.run(q=rng.standard_normal((70, 192)), k=rng.standard_normal((70, 64)), at=rng.integers(-far, far, 70))
+        ref = evaluate(ops)
+        for name, out in (("q", "q1"), ("k", "k1")):
+            _close(env[out], ref[out], _rotary_bound(spec, ops.uploads[name], ops.uploads["at"]))
