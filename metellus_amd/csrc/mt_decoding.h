@@ -1017,12 +1017,15 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // drawn from by one workgroup.
 //
 // The list takes half a compute unit's LDS, so there are two workgroups on each, of eight
-// waves (us, 64 rows of 131072 cut by p: eight waves, 512 workgroups 43, 1024 55, four waves
-// 64; one row 18, 17, 20; 64 rows cut by k 25, 39, 35).
-// Bound by vector instructions where rows are weighed in whole (64 rows of 131072, us: the scan 10,
-// with bins 15, of 6.5 to read them; the second kernel 16 with no cut, 20 by k, 36 by p, of
+// waves (us a call, eight waves in 512, 256 and 1024 workgroups, four in 512 and 1024: 64 rows of
+// 131072 cut by p 45, 50, 59, 55, 67; cut by k 30, 33, 42, 34, 43; filters mixed 41, 48, 42, 51,
+// 45; not cut 22, 22, 22, 23, 22; one row 17.5, 17.6, 17.6, 19.2, 19.0).
+// Many rows are bound by what each does in turn, and a batch by its rows that p alone cuts, which
+// take longest while the others' compute units are done (64 rows of 131072, us: the scan 9.6, with
+// bins 11.6, of 6.5 to read them; the second kernel 15 with no cut, 19 by k, 36 by p, of
 // which the pass over the logits takes 8, 2 and 16, and the last workgroup's list, from its
-// arrival on, 3, 7 and 13), by two launches and that list for few rows (one of 131072 5.3 and 12).
+// arrival on, 3, 7 and 13; vector instructions are 5 of the 30 of mixed filters).  Few rows are
+// bound by two launches and that list (one of 131072 5.3 and 12).
 // ---------------------------------------------------------------------------
 
 constexpr unsigned MT_SAMPLE_WAVES = 8u, MT_SAMPLE_LANES = 512u;

@@ -558,8 +558,9 @@ class Operations:
         """``out`` = ``base`` + scales[i] * B_i (A_i x) by rows, i = ``ids`` of the row
         (int32): low-rank adapters, each row's own, beside a product that all share
         (``base``).  ``a`` (adapters * rank, columns of x) and ``b`` (adapters * columns of
-        base, rank) hold every adapter's A and B, one after the other; ``scales`` are 1
-        unless given.  A row whose id is none of theirs (-1) is its row of ``base``."""
+        base, rank) hold every adapter's A and B, one after the other (all of one rank: a
+        smaller one has zeros behind its own, which are read and multiplied as others are);
+        ``scales`` are 1 unless given.  A row whose id is none of theirs (-1) is its row of ``base``."""
         tx, ty, ta, tb = self._lookup(x), self._lookup_float(base), self._lookup(a), self._lookup(b)
         ti, ts = self._lookup(ids), self._optional(scales)
         for label, t in (("x", tx), ("base", ty), ("a", ta), ("b", tb)):
@@ -627,7 +628,9 @@ class Operations:
         is left has come by.  All four are a number for each row.  A temperature of 0 (or
         below, or NaN) takes the largest, 1 where not given.  ``logprobs``: the logarithm
         of the probability that the token was drawn with.  Logits of +inf share
-        all the weight.  A row of -inf alone, or with a NaN, gives -1, its logprob NaN."""
+        all the weight.  A row of -inf alone, or with a NaN, gives -1, its logprob NaN.
+        Weights are held to 2^-44 of the largest (2^-42 for the longest rows): what weighs
+        less than half of that weighs nothing, at the ends of u too."""
         tl, tu = self._lookup(logits), self._lookup(uniforms)
         given = {n: self._optional(v) for n, v in
                  (("temperatures", temperatures), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p))}

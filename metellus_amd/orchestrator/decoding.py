@@ -152,7 +152,9 @@ def adapter_splits(rows: int, inner: int, many: bool) -> int:
     up takes longer (us: 1 row of 4096 columns, rank 16, whole 17, in 4 9.4, 8 9.6; 32 rows 30,
     13.4, 12.3, in 16 12.8; 77 of 5003, rank 23, 37, 21, 18, 20; 8 of 11008, rank 64, in 8
     23, 12 20, 20 32; 600 of 4096, rank 64, in 3 49, 5 43, 6 43), or that some come after
-    others (3000 rows of 4096 columns, rank 64: in 6 98, in 5 87)."""
+    others (3000 rows of 4096 columns, rank 64: in 6 98, in 5 87).  Two workgroups of large tiles
+    fit a compute unit, and take longer than one (4096 rows of 4096 columns, rank 64, in 4 and
+    in 8: this kernel 32 and 41, the second, with twice the parts, 39 and 49)."""
     wanted = 256 // -(-rows // 64) if many else min(12, 3000 // rows)
     return max(1, min(-(-inner // 512), wanted))
 
@@ -349,8 +351,9 @@ def sample_chunks(rows: int, cols: int) -> tuple[int, int]:
 
 def sample_bins(cols: int) -> int:
     """Bins of 32 temperatures: the finer, the shorter the lists of what is in one, and the
-    longer adding them up takes (us of the second kernel with 512 and 1024: 64 rows of 131072
-    cut by k 20, 26, by p 44, 44; one row 11, 16 and 16, 20)."""
+    longer adding them up takes (us a call with 512 and 1024: 64 rows of 131072 cut by k 30.4 and
+    32.4, by p 45.1 and 44.3, filters mixed 40.6 and 40.0; one row by k 15.6 and 17.0, by p 20.0
+    and 20.7)."""
     return 512 if cols <= SAMPLE_BINS_FINE else 1024 if cols <= 2 * SAMPLE_BINS_FINE else 2048
 
 
