@@ -880,3 +880,58 @@ def test_rotary_again_in_its_buffers():
         ref = evaluate(ops)
         for name, out in (("q", "q1"), ("k", "k1")):
             _close(env[out], ref[out], _rotary_bound(spec, ops.uploads[name], ops.uploads["at"]))
+
+
+@pytest.mark.parametrize("rows, cols", [(513, 12345), (600, 4097), (300, 66000)])
+def test_sample_long_rows_of_one_chunk(rows, cols):
+    """So many rows that one workgroup has each: one kernel, without scratch."""
+    rng = np.random.default_rng(rows)
+    first = _sample_inputs(rng, rows, cols)
+    kept = _Kept(_sample_ops(first.pop("x"), first.pop("u"), **first))
+    assert len(kept.ops.build()) == 1
+    _sample_compare(kept.ops, kept.run())
+
+
+def _grown(seed, pages, sequences=5, width=6, page_size=4, heads=2, dim=16):
+    """Two steps of prompts in a program, from a list of ``pages``; attention behind each."""
+    rng = np.random.default_rng(seed)
+    ops = Operations()
+    spec = KVCache(pages=sequences * width, page_size=page_size, kv_heads=heads, dim=dim)
+    _put(ops, "table0", np.full((sequences, width), -1, np.int32))
+    _put(ops, "free", rng.permutation(spec.pages)[:pages].astype(np.int32))
+    _put(ops, "ends0", np.zeros(sequences, np.int32))
+    ops.kv_cache("cache0", pages=spec.pages, page_size=page_size, kv_heads=heads, dim=dim)
+    ops.from_numpy(spec.empty(), "cache0")
+    _put(ops, "q", rng.standard_normal((sequences, heads * dim)).astype(np.float32))
+    for i in (1, 2):
+        _put(ops, f"counts{i}", rng.integers(0, 11, sequences).astype(np.int32))
+        for name in ("k", "v"):
+            _put(ops, f"{name}{i}", rng.standard_normal((55, heads * dim)).astype(np.float32))
+        _grow(ops, i, f"table{i - 1}", f"ends{i - 1}", page_size=page_size, tokens=55)
+        ops.cache_write(f"cache{i - 1}", k=f"k{i}", v=f"v{i}", slots=f"slots{i}", out=f"cache{i}")
+        ops.paged_attention("q", cache=f"cache{i}", pages=f"table{i}", lengths=f"ends{i}", heads=heads, out=f"o{i}")
+    return ops
+
+
+GROWN = [f"{n}{i}" for i in (1, 2) for n in ("slots", "positions", "ends", "used", "o")] + ["table2"]
+
+
+@pytest.mark.parametrize("pages", [30, 7, 1])
+def test_two_steps_with_attention(pages):
+    """With pages enough, and with too few: what has no page is a hole, then and later."""
+    ops = _grown(pages, pages)
+    env, ref = run(ops, outputs=GROWN).env, evaluate(ops)
+    for name in GROWN:
+        if name.startswith("o"):  # (sums of up to 20 products of terms around 1: 2^-14 of the largest)
+            assert np.abs(env[name] - ref[name]).max() <= 2.0**-14 * max(1.0, np.abs(ref[name]).max()), name
+        else:
+            np.testing.assert_array_equal(env[name], ref[name], err_msg=name)
+    assert (env["used2"][0] > pages) == (pages < 30)
+
+
+def test_a_batch_of_two_steps():
+    programs = [_grown(s, 14) for s in range(3)]
+    for ops, got in zip(programs, run_batch(programs, outputs=GROWN)):
+        alone = run(ops, outputs=GROWN).env
+        for name in GROWN:
+            np.testing.assert_array_equal(got.env[name], alone[name], err_msg=name)
