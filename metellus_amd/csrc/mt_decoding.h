@@ -1024,7 +1024,7 @@ MT_INLINE void mt_sample_whole(const float* x, const mt_asked& asked, const mt_w
 // take longest while the others' compute units are done (64 rows of 131072, us: the scan 9.6, with
 // bins 11.6, of 6.5 to read them; the second kernel 15 with no cut, 19 by k, 36 by p, of
 // which the pass over the logits takes 8, 2 and 16, and the last workgroup's list, from its
-// arrival on, 3, 7 and 13; vector instructions are 5 of the 30 of mixed filters).  Few rows are
+// arrival on, 3, 7 and 13; vector instructions are 6 of the 30 of mixed filters).  Few rows are
 // bound by two launches and that list (one of 131072 5.3 and 12).
 // ---------------------------------------------------------------------------
 
