@@ -314,8 +314,8 @@ MT_INLINE void mt_rotary(const float* x, const float* k, const int* positions, c
 // so that all workgroups find the same.  Where ids change less than twice a tile they stay as
 // they are.  Each workgroup counts all of the rows' ids for itself and keeps the rows of its
 // tile: rows[m], m < TILE, or nothing behind the last.  (us, rank 64 of 4096 x 4096, in
-// the order they come in and in this: ids drawn from 64 150 rows 56, 46; 600 rows 163, 78; 2048
-// rows 632, 72; ids of 8 prompts 150 rows 21.5, 22.5; 600 rows 45.5, 48.6; 4096 rows 72, 75.)
+// the order they come in and in this: of 64 adapters in turn, shuffled, 150 rows 54, 45; 600 rows
+// 211, 60; 2048 rows 560, 72; of 8 prompts 150 rows 20.7, 23.2; 600 rows 36.3, 37.7; 4096 rows 72, 74.)
 // `lds`: WAVES words of sums, WAVES times BINS numbers, and a byte a row.
 constexpr unsigned MT_ADAPTER_BINS = 256u, MT_ADAPTER_ORDERED = 4096u;
 constexpr unsigned MT_ADAPTER_ROWS = 64u;  // words of LDS, in front of all others, for a tile's rows
